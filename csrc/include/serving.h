@@ -1,0 +1,83 @@
+// Parameters and launch entry points of the serving operators: the mixture-of-
+// experts layer for a few tokens (csrc/kernels/moe_few.cu) and the dense
+// product with an epilogue (csrc/kernels/linear.cu).  The torch bindings in
+// csrc/kernels/serving_bindings.cpp check the tensors and fill these.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "types.h"
+
+namespace raiccl {
+
+constexpr int kFewTokens = 64;     // tokens of one call at most: an expert's tokens are the bits of one 64-bit word
+constexpr int kFewExperts = 255;   // experts at most (the routing key's byte for the expert)
+constexpr int kFewTopK = 8;
+
+// Routing of T tokens.  Element strides; mask_stride 0 for one mask of all tokens.
+struct FewRouteParams {
+  const void* x;          // [T, D]
+  long long x_stride;
+  const void* w;          // [E, D]
+  long long w_stride;
+  const float* bias;      // [E] or nullptr
+  const uint8_t* mask;    // [T, E] or [E], nonzero: never chosen; or nullptr
+  long long mask_stride;
+  int T, D, E, k;
+  int gate_mode;          // 0 ones, 1 softmax over the chosen, 2 softmax over all that are not blocked
+  int bf16;               // element type of x and w
+  int vec;                // rows of x and w are 16-byte aligned multiples of 16 bytes
+  int* ids;               // [T, k], -1 where no expert was left
+  float* gates;           // [T, k], 0 there
+};
+
+// The experts' MLPs and the weighted sum of the routed tokens.
+struct FewExpertParams {
+  const void* x;          // [T, D]
+  long long x_stride;
+  const void* w1;         // [E, N1, D], N1 = F, or 2F (gate rows, then up rows) for SwiGLU
+  long long w1_estride, w1_stride;
+  const void* w2;         // [E, O, F]
+  long long w2_estride, w2_stride;
+  const float* b1;        // [E, N1] or nullptr
+  const float* b2;        // [E, O] or nullptr
+  const void* residual;   // [T, O] or nullptr
+  long long res_stride;
+  void* out;              // [T, O]
+  long long out_stride;
+  const int* ids;         // [T, k]
+  const float* gates;     // [T, k]
+  float* h;               // [T k, F] scratch
+  float* y;               // [T k, O] scratch
+  int T, D, E, k, F, O;
+  int act;
+  int bf16, out_bf16, res_bf16;
+};
+
+void launch_few_route(const FewRouteParams& p, cudaStream_t s);
+void launch_few_experts(const FewExpertParams& p, cudaStream_t s);
+
+// out = act(x w^T + bias) + residual; SwiGLU: w holds F gate rows, then F up
+// rows, and N = F is the width of out.
+struct LinearParams {
+  const void* x;          // [M, K]
+  long long x_stride;
+  const void* w;          // [N, K] (SwiGLU: [2N, K])
+  long long w_stride;
+  const float* bias;      // [N] (SwiGLU: [2N]) or nullptr
+  const void* residual;   // [M, N] or nullptr
+  long long res_stride;
+  void* out;              // [M, N]
+  long long out_stride;
+  long long M;
+  int N, K;
+  int act;
+  int bf16, out_bf16, res_bf16;
+};
+
+void launch_linear(const LinearParams& p, cudaStream_t s);
+
+}  // namespace raiccl

@@ -1,0 +1,257 @@
+// A whole mixture-of-experts layer for a few tokens (1 to 64): one decode step
+// of a served model.  The progressive layer handles thousands of tokens per
+// call, chunk by chunk; here every cost but reading the chosen experts'
+// weights once is overhead.
+//
+//   l[t, e] = x[t] . Wr[e] + br[e]           blocked experts: -inf
+//   ids[t]  = the k largest (larger value, then smaller expert; NaN last)
+//   g[t]    = 1, softmax over the chosen, or softmax over all
+//   out[t]  = sum_j g[t, j] (W2[e] act(W1[e] x[t] + b1[e]) + b2[e]) + residual[t],  e = ids[t, j]
+#include <cooperative_groups.h>
+
+#include <stdexcept>
+
+#include "serving.h"
+#include "serving_device.cuh"
+#include "sm100_ptx.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace raiccl {
+
+// ---------------------------------------------------------------------------
+// Routing: one cluster per token, its CTAs and their warps share the experts.
+// ---------------------------------------------------------------------------
+constexpr int kRouteThreads = 256;
+constexpr int kRouteWarps = kRouteThreads / 32;
+
+// Sort key, larger = preferred: 0 for no candidate (blocked, or a logit of
+// -inf), then NaN, then numbers by value (an order-preserving map of the float
+// bits, -0 taken as +0); among equals the smaller expert.
+__device__ __forceinline__ unsigned long long few_key(float v, int e) {
+  if (v == -INFINITY) return 0ull;
+  if (v != v) return (1ull << 40) | (unsigned long long)(255 - e);
+  const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
+  const uint32_t u = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return (2ull << 40) | ((unsigned long long)u << 8) | (unsigned long long)(255 - e);
+}
+
+// x . w of one row pair by one warp, in 32 bits: each lane sums its vectors'
+// partial sums, a butterfly adds the lanes.
+template <typename T>
+__device__ __forceinline__ float route_dot(const T* x, const T* w, int D, int vec) {
+  const int lane = threadIdx.x & 31;
+  float acc = 0.f;
+  if (vec) {
+    constexpr int V = 16 / sizeof(T);
+    const int n = D / V;
+#pragma unroll 8
+    for (int i = lane; i < n; i += 32) {
+      const uint4 xr = __ldg((const uint4*)x + i);
+      const uint4 wr = __ldg((const uint4*)w + i);
+      float s = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) s = fmaf(as_float(((const T*)&xr)[v]), as_float(((const T*)&wr)[v]), s);
+      acc += s;
+    }
+  } else {
+#pragma unroll 8
+    for (int i = lane; i < D; i += 32) acc = fmaf(as_float(x[i]), as_float(w[i]), acc);
+  }
+  return warp_sum(acc);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams p) {
+  __shared__ float logits[kFewExperts + 1];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int t = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* x = (const T*)p.x + (long long)t * p.x_stride;
+  float* lead = cluster.map_shared_rank(logits, 0);
+  for (int e = warp * ranks + rank; e < p.E; e += kRouteWarps * ranks) {
+    float v = route_dot(x, (const T*)p.w + (long long)e * p.w_stride, p.D, p.vec);
+    if (lane == 0) {
+      if (p.bias) v += p.bias[e];
+      if (p.mask && p.mask[(long long)t * p.mask_stride + e]) v = -INFINITY;
+      lead[e] = v;
+    }
+  }
+  cluster.sync();
+  if (rank != 0 || warp != 0) return;
+  // k rounds of a warp-wide maximum; lane l holds experts l, l + 32, ...
+  constexpr int PER = (kFewExperts + 32) / 32;
+  unsigned long long key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = i * 32 + lane;
+    key[i] = e < p.E ? few_key(logits[e], e) : 0ull;
+  }
+  int chosen = -1;      // lane j: choice j
+  float top = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < p.k; ++j) {
+    unsigned long long best = 0ull;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) best = key[i] > best ? key[i] : best;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+      best = other > best ? other : best;
+    }
+    if (best == 0ull) break;  // the same on every lane
+    const int e = 255 - (int)(best & 255ull);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (key[i] == best) key[i] = 0ull;
+    if (lane == j) { chosen = e; top = logits[e]; }
+  }
+  float gate = chosen < 0 ? 0.f : 1.f;
+  if (p.gate_mode != 0) {
+    const float peak = __shfl_sync(0xffffffffu, top, 0);  // the largest number, or NaN if there is none
+    float part = 0.f;
+    if (p.gate_mode == 1) {
+      part = chosen < 0 ? 0.f : expf(top - peak);
+    } else {
+      for (int e = lane; e < p.E; e += 32) part += logits[e] == -INFINITY ? 0.f : expf(logits[e] - peak);
+    }
+    const float total = warp_sum(part);
+    if (chosen >= 0) gate = expf(top - peak) / total;
+  }
+  if (lane < p.k) {
+    p.ids[(long long)t * p.k + lane] = chosen;
+    p.gates[(long long)t * p.k + lane] = gate;
+  }
+}
+
+void launch_few_route(const FewRouteParams& p, cudaStream_t s) {
+  // enough CTAs that each warp has one or two experts
+  const int want = (p.E + 2 * kRouteWarps - 1) / (2 * kRouteWarps);
+  const int ranks = want > 4 ? 8 : want > 2 ? 4 : want;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ranks, p.T);
+  cfg.blockDim = dim3(kRouteThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (p.bf16) cudaLaunchKernelEx(&cfg, few_route_kernel<__nv_bfloat16>, p);
+  else cudaLaunchKernelEx(&cfg, few_route_kernel<float>, p);
+}
+
+// ---------------------------------------------------------------------------
+// Experts: one warp per weight row and expert; a row is read once for up to
+// eight of the expert's tokens at a time.
+// ---------------------------------------------------------------------------
+constexpr int kRowThreads = 256;
+constexpr int kRowTokens = 8;
+
+// The expert's (token, choice) pairs t k + j in token order -> list; returns their number.
+__device__ __forceinline__ int few_pairs(const int* ids, int T, int k, int e, int* list) {
+  __shared__ unsigned long long mask;
+  if (threadIdx.x == 0) mask = 0ull;
+  __syncthreads();
+  for (int i = threadIdx.x; i < T * k; i += blockDim.x)
+    if (ids[i] == e) atomicOr(&mask, 1ull << (i / k));
+  __syncthreads();
+  const unsigned long long m = mask;
+  for (int i = threadIdx.x; i < T * k; i += blockDim.x)
+    if (ids[i] == e) list[__popcll(m & ((1ull << (i / k)) - 1ull))] = i;
+  __syncthreads();
+  return __popcll(m);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams p) {
+  __shared__ int list[kFewTokens];
+  const int e = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = few_pairs(p.ids, p.T, p.k, e, list);
+  const int f = blockIdx.x * (kRowThreads / 32) + warp;
+  if (n == 0 || f >= p.F) return;
+  const bool glu = p.act == (int)Act::kSwiGLU;
+  const T* wg = (const T*)p.w1 + (long long)e * p.w1_estride + (long long)f * p.w1_stride;
+  const T* wu = wg + (long long)p.F * p.w1_stride;
+  for (int i0 = 0; i0 < n; i0 += kRowTokens) {
+    float g[kRowTokens] = {}, u[kRowTokens] = {};
+    const T* x[kRowTokens];
+    for (int i = 0; i < kRowTokens; ++i)
+      x[i] = (const T*)p.x + (long long)(list[min(i0 + i, n - 1)] / p.k) * p.x_stride;
+    for (int d = lane; d < p.D; d += 32) {
+      const float a = as_float(wg[d]), b = glu ? as_float(wu[d]) : 0.f;
+#pragma unroll
+      for (int i = 0; i < kRowTokens; ++i) {
+        const float v = as_float(x[i][d]);
+        g[i] = fmaf(a, v, g[i]);
+        if (glu) u[i] = fmaf(b, v, u[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRowTokens; ++i) {
+      g[i] = warp_sum(g[i]);
+      u[i] = warp_sum(u[i]);
+      if (lane == 0 && i0 + i < n) {
+        const float* b1 = p.b1 ? p.b1 + (long long)e * (glu ? 2 : 1) * p.F : nullptr;
+        const float z = g[i] + (b1 ? b1[f] : 0.f);
+        p.h[(long long)list[i0 + i] * p.F + f] =
+            glu ? serving_swiglu(z, u[i] + (b1 ? b1[p.F + f] : 0.f)) : serving_act(z, p.act);
+      }
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams p) {
+  __shared__ int list[kFewTokens];
+  const int e = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = few_pairs(p.ids, p.T, p.k, e, list);
+  const int o = blockIdx.x * (kRowThreads / 32) + warp;
+  if (n == 0 || o >= p.O) return;
+  const T* w = (const T*)p.w2 + (long long)e * p.w2_estride + (long long)o * p.w2_stride;
+  for (int i0 = 0; i0 < n; i0 += kRowTokens) {
+    float acc[kRowTokens] = {};
+    const float* h[kRowTokens];
+    for (int i = 0; i < kRowTokens; ++i) h[i] = p.h + (long long)list[min(i0 + i, n - 1)] * p.F;
+    for (int f = lane; f < p.F; f += 32) {
+      const float a = as_float(w[f]);
+#pragma unroll
+      for (int i = 0; i < kRowTokens; ++i) acc[i] = fmaf(a, h[i][f], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRowTokens; ++i) {
+      acc[i] = warp_sum(acc[i]);
+      if (lane == 0 && i0 + i < n)
+        p.y[(long long)list[i0 + i] * p.O + o] = acc[i] + (p.b2 ? p.b2[(long long)e * p.O + o] : 0.f);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kRowThreads) few_join_kernel(FewExpertParams p) {
+  const long long i = (long long)blockIdx.x * kRowThreads + threadIdx.x;
+  if (i >= (long long)p.T * p.O) return;
+  const int t = (int)(i / p.O), o = (int)(i % p.O);
+  float acc = 0.f;
+  for (int j = 0; j < p.k; ++j)
+    if (p.ids[t * p.k + j] >= 0) acc = fmaf(p.gates[t * p.k + j], p.y[(long long)(t * p.k + j) * p.O + o], acc);
+  if (p.residual) acc += load_elem(p.residual, (long long)t * p.res_stride + o, p.res_bf16);
+  store_elem(p.out, (long long)t * p.out_stride + o, acc, p.out_bf16);
+}
+
+template <typename T>
+static void launch_rows(const FewExpertParams& p, cudaStream_t s) {
+  constexpr int W = kRowThreads / 32;
+  few_hidden_kernel<T><<<dim3((p.F + W - 1) / W, p.E), kRowThreads, 0, s>>>(p);
+  few_output_kernel<T><<<dim3((p.O + W - 1) / W, p.E), kRowThreads, 0, s>>>(p);
+  few_join_kernel<<<(unsigned)(((long long)p.T * p.O + kRowThreads - 1) / kRowThreads), kRowThreads, 0, s>>>(p);
+}
+
+void launch_few_experts(const FewExpertParams& p, cudaStream_t s) {
+  if (p.bf16) launch_rows<__nv_bfloat16>(p, s);
+  else launch_rows<float>(p, s);
+}
+
+}  // namespace raiccl

@@ -1,0 +1,44 @@
+"""Dense product with bias, activation and residual in its epilogue (csrc/kernels/linear.cu).
+
+The projections next to the experts (a shared expert, an attention output):
+``grouped_gemm`` multiplies row segments by per-expert weights and needs its
+segments on the device; ``linear`` is one weight for all rows, any sizes, from
+one decode row to a prefill batch.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ._native import kernels
+from .grouped_gemm import ACT_IDS
+
+
+def linear(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None = None,
+    *,
+    act: str = "none",
+    residual: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """act(x @ weight.T + bias) + residual.
+
+    x [M, K], weight [N, K]: both bf16 or both fp32, rows contiguous, any row
+    stride.  ``act="swiglu"``: weight holds N/2 gate rows, then N/2 up rows,
+    and the result, silu(gate) * up, is [M, N/2].  bias: fp32 [N].  residual:
+    fp32 or bf16 of the result's shape; ``out`` may be the same tensor.
+
+    Sums are kept in fp32 and rounded once, to out_dtype (default: x's type;
+    fp32 inputs give fp32).  fp32 inputs are multiplied to fp32 accuracy, not
+    to tf32's.  Enqueues on the current stream without synchronising and can
+    be captured in a CUDA graph.  There is no backward.
+    """
+    if act not in ACT_IDS:
+        raise ValueError(f"linear: act must be one of {sorted(ACT_IDS)}")
+    return kernels().linear(x, weight, bias, ACT_IDS[act], residual, out, out_dtype)
+
+
+__all__ = ["linear"]

@@ -1,0 +1,269 @@
+"""moe_few_tokens(): the mixture-of-experts layer for a few tokens, against 64 bits."""
+
+import pytest
+import torch
+
+from serving_reference import HALF, PARTS, U, check_close, check_norm, linear64, moe64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, FP32 = torch.bfloat16, torch.float32
+INF = float("inf")
+
+
+def _moe(*a, **k):
+    from revealaiccl_b200.ops.moe_few import moe_few_tokens
+    return moe_few_tokens(*a, **k)
+
+
+def _make(T, D, E, F, O, act, dtype, seed=0, bias=False):
+    g = torch.Generator(DEV).manual_seed(seed)
+
+    def n(*shape, s=1.0):
+        return torch.randn(*shape, generator=g, device=DEV) * s
+
+    n1 = 2 * F if act == "swiglu" else F
+    a = dict(x=n(T, D).to(dtype), router_w=n(E, D, s=D ** -0.5).to(dtype), w1=n(E, n1, D, s=D ** -0.5).to(dtype),
+             w2=n(E, O, F, s=F ** -0.5).to(dtype))
+    if bias:
+        a.update(router_b=n(E, s=0.1), b1=n(E, n1, s=0.1), b2=n(E, O, s=0.1))
+    return a
+
+
+def _check(a, k, act, gate_mode, norm=True, **kw):
+    out, ids, gates = _moe(**a, top_k=k, act=act, gate_mode=gate_mode, **kw)
+    kw = {n: v for n, v in kw.items() if n != "out"}
+    want, bound, rid, rg, grel, gap = moe64(**a, top_k=k, act=act, gate_mode=gate_mode, **kw)
+    # The choices are the reference's where no two logits lie closer than their errors: a logit of order one is summed
+    # by 32 lanes in D / 32 steps each and five additions, errors of 2^-24 and random sign; four times that, for two logits.
+    assert gap > 4 * U * ((a["x"].shape[1] / 32) ** 0.5 + 8), "two logits too close to tell"
+    assert ids.dtype == torch.int32 and torch.equal(ids.cpu(), rid)
+    check_close(gates.cpu(), rg, grel * rg.abs() + U * rg.abs() + 2.0 ** -126)  # fp32 has no normal number below 2^-126
+    check_close(out, want, bound)
+    dt, odt = a["x"].dtype, out.dtype
+    if norm and want.numel() >= 64 and not want.isnan().any():
+        hidden = HALF[dt] if dt == BF16 else 2 * PARTS
+        check_norm(out, want, 2 * (HALF[odt] + hidden + U * (a["x"].shape[1] ** 0.5 + a["w2"].shape[2] ** 0.5 + 16)) + grel)
+    return out, ids, gates
+
+
+SIZES = [  # T, D, E, k, F, O
+    (1, 1, 1, 1, 1, 1), (1, 64, 4, 1, 16, 16), (1, 2048, 4, 1, 32, 16), (2, 256, 64, 6, 176, 256), (3, 100, 5, 2, 77, 33),
+    (4, 128, 8, 8, 128, 128), (7, 512, 16, 4, 200, 512), (8, 1024, 8, 2, 1792, 1024), (13, 264, 60, 4, 40, 136),
+    (16, 384, 255, 8, 24, 384), (17, 520, 24, 3, 344, 72), (31, 65, 9, 3, 129, 250), (33, 256, 64, 6, 704, 256),
+    (37, 512, 4, 2, 3000, 130), (48, 200, 128, 5, 56, 200), (63, 320, 3, 3, 320, 640), (64, 256, 8, 2, 1024, 256),
+    (64, 128, 1, 1, 5000, 128), (64, 192, 32, 8, 96, 1000),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T,D,E,k,F,O", SIZES)
+def test_sizes(T, D, E, k, F, O, dtype):
+    act = ("swiglu", "relu", "gelu", "silu", "swiglu")[(T + D + F) % 5]
+    mode = ("topk_softmax", "softmax", "none")[(T + E) % 3]
+    _check(_make(T, D, E, F, O, act, dtype, seed=T + D, bias=(T + k) % 2 == 0), k, act, mode)
+
+
+@pytest.mark.parametrize("act", ["swiglu", "relu", "gelu", "silu", "none"])
+@pytest.mark.parametrize("mode", ["topk_softmax", "softmax", "none"])
+@pytest.mark.parametrize("dtype,out_dtype,res_dtype", [(BF16, BF16, BF16), (BF16, FP32, BF16), (BF16, BF16, FP32), (FP32, FP32, FP32),
+                                                       (FP32, FP32, BF16)])
+def test_acts_gates_types(act, mode, dtype, out_dtype, res_dtype):
+    a = _make(9, 256, 12, 160, 192, act, dtype, seed=3, bias=True)
+    r = torch.randn(9, 192, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(res_dtype)
+    out, _, _ = _check(a, 3, act, mode, residual=r, out_dtype=out_dtype)
+    assert out.dtype == out_dtype
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T", [1, 6, 64])
+def test_every_token_on_one_expert(T, dtype):
+    a = _make(T, 256, 16, 512, 256, "swiglu", dtype, bias=True)
+    a["router_b"][11] += 100.0
+    _, ids, _ = _check(a, 1, "swiglu", "softmax")
+    assert (ids == 11).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+def test_masks(dtype):
+    """Blocked experts, tokens with fewer free experts than choices, tokens with none; what is blocked is not read."""
+    T, E = 12, 8
+    a = _make(T, 256, E, 96, 128, "swiglu", dtype, bias=True)
+    g = torch.Generator(DEV).manual_seed(5)
+    mask = torch.rand(T, E, generator=g, device=DEV) < 0.4
+    mask[0] = True            # none left
+    mask[1] = True
+    mask[1, 3] = False        # one left
+    mask[:, 6] = True         # blocked for every token: may hold anything
+    for name in ("w1", "w2", "b1", "b2"):
+        a[name][6] = float("nan")
+    a["router_w"][6] = float("nan")
+    r = torch.randn(T, 128, generator=g, device=DEV).to(dtype)
+    clean = {n: v.clone() for n, v in a.items()}
+    for name, v in clean.items():
+        if name != "x":
+            v[6] = 0
+    out, ids, gates = _moe(**a, top_k=3, act="swiglu", gate_mode="topk_softmax", block_mask=mask, residual=r)
+    want, wid, wgates = _check(clean, 3, "swiglu", "topk_softmax", block_mask=mask, residual=r)
+    assert torch.equal(out, want) and torch.equal(ids, wid) and torch.equal(gates, wgates)
+    assert (ids[0] == -1).all() and (gates[0] == 0).all() and torch.equal(out[0], r[0])
+    assert ids[1].tolist() == [3, -1, -1] and gates[1].tolist() == [1, 0, 0]
+    out, ids, _ = _moe(**clean, top_k=3, act="swiglu", gate_mode="softmax", block_mask=mask.to(torch.uint8))
+    assert (out[0] == 0).all()
+    # one mask for all tokens, all blocked
+    out, ids, _ = _moe(**clean, top_k=2, act="swiglu", gate_mode="none", block_mask=torch.ones(E, device=DEV, dtype=torch.bool))
+    assert (out == 0).all() and (ids == -1).all()
+
+
+@pytest.mark.parametrize("mode", ["topk_softmax", "softmax", "none"])
+def test_bias_as_mask(mode):
+    """A bias of -inf blocks; the type's lowest value is a number like any other and comes last."""
+    a = _make(5, 128, 6, 64, 64, "silu", BF16, bias=True)
+    a["router_b"][2] = -INF
+    a["router_b"][4] = torch.finfo(FP32).min
+    _, ids, gates = _check(a, 6, "silu", mode)
+    assert (ids[:, 5] == -1).all() and (ids[:, 4] == 4).all() and (gates[:, 5] == 0).all()
+    a["router_b"][:] = -INF
+    out, ids, gates = _moe(**a, top_k=2, act="silu", gate_mode=mode)
+    assert (ids == -1).all() and (gates == 0).all() and (out == 0).all()
+
+
+def test_ties_go_to_the_lower_expert():
+    a = _make(10, 256, 32, 32, 32, "relu", BF16)
+    a["router_w"][:] = a["router_w"][:1]
+    _, ids, _ = _moe(**a, top_k=8, act="relu", gate_mode="softmax")
+    assert (ids.cpu() == torch.arange(8, dtype=torch.int32)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+def test_special_values_stay_where_they_are(dtype):
+    """A NaN or infinite token, and weights of experts that nobody chose, leave the other tokens alone."""
+    a = _make(6, 128, 16, 80, 96, "swiglu", dtype)
+    base, ids, _ = _moe(**a, top_k=2, act="swiglu", gate_mode="topk_softmax")
+    unused = [e for e in range(16) if not (ids == e).any()]
+    b = {n: v.clone() for n, v in a.items()}
+    for e in unused:
+        b["w1"][e], b["w2"][e] = float("nan"), INF
+    out, _, _ = _moe(**b, top_k=2, act="swiglu", gate_mode="topk_softmax")
+    assert unused and torch.equal(out, base)
+    a["x"][2, 7] = float("nan")
+    a["x"][4, 9] = INF
+    out, ids, _ = _moe(**a, top_k=2, act="swiglu", gate_mode="topk_softmax")
+    assert out[2].isnan().all() and ids[2].tolist() == [0, 1]
+    keep = [0, 1, 3, 5]
+    assert torch.equal(out[keep], base[keep])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("offset,pad", [(0, 8), (1, 0), (8, 24)])
+def test_strides(dtype, offset, pad):
+    """Every tensor as a window of a wider buffer, every other expert of a larger bank; what lies around out stays."""
+    T, D, E, F, O = 5, 128, 6, 80, 72
+    g = torch.Generator(DEV).manual_seed(2)
+
+    def window(*shape, s):
+        wide = (torch.randn(*shape[:-1], shape[-1] + offset + pad, generator=g, device=DEV) * s).to(dtype)
+        return wide[..., offset:offset + shape[-1]]
+
+    a = dict(x=window(T, D, s=1.0), router_w=window(E, D, s=D ** -0.5), w1=window(2 * E, 2 * F, D, s=D ** -0.5)[::2],
+             w2=window(2 * E, O, F, s=F ** -0.5)[1::2])
+    ob = torch.full((T + 2, O + offset + pad), 7.0, device=DEV, dtype=dtype)
+    r = window(T, O, s=1.0)
+    mask = torch.zeros(T, E + 3, device=DEV, dtype=torch.bool)[:, 1:E + 1]
+    _check(a, 2, "swiglu", "topk_softmax", residual=r, block_mask=mask, out=ob[1:T + 1, offset:offset + O])
+    ob[1:T + 1, offset:offset + O] = 7.0
+    assert torch.equal(ob, torch.full_like(ob, 7.0))
+
+
+def test_empty_batch_and_in_place():
+    a = _make(4, 64, 4, 32, 64, "swiglu", BF16)
+    e = dict(a, x=a["x"][:0])
+    out, ids, gates = _moe(**e, top_k=2)
+    assert out.shape == (0, 64) and ids.shape == (0, 2) and gates.shape == (0, 2)
+    r = torch.randn(4, 64, device=DEV).bfloat16()
+    want, _, _ = _moe(**a, top_k=2, residual=r)
+    got, _, _ = _moe(**a, top_k=2, residual=r, out=r)
+    assert got.data_ptr() == r.data_ptr() and torch.equal(got, want)
+
+
+def test_far_experts():
+    """Element offsets past 32 bits in the experts' weights: the last of 60 experts of a bank of 4.3 G elements."""
+    D, F, E = 4096, 5888, 60
+    bank = torch.zeros(E, 2 * F + F, D, device=DEV, dtype=BF16)
+    w1, w2 = bank[:, :2 * F], bank.view(E, -1)[:, 2 * F * D:].view(E, D, F)
+    g = torch.Generator(DEV).manual_seed(0)
+    x = torch.randn(2, D, generator=g, device=DEV).bfloat16()
+    for e in (0, E - 1):
+        w1[e].normal_(0, D ** -0.5, generator=g)
+        w2[e].normal_(0, F ** -0.5, generator=g)
+    bias = torch.zeros(E, device=DEV)
+    bias[[0, E - 1]] = 100.0
+    rw = (torch.randn(E, D, generator=g, device=DEV) * D ** -0.5).bfloat16()
+    out, ids, gates = _moe(x, rw, w1, w2, top_k=2, router_b=bias)
+    assert (ids.sort(dim=1).values.cpu() == torch.tensor([0, E - 1])).all()
+    pick = torch.tensor([0, E - 1], device=DEV)
+    want, bound, _, _, _, _ = moe64(x, rw[pick], w1[pick], w2[pick], top_k=2, act="swiglu", gate_mode="topk_softmax",
+                                    router_b=bias[pick])
+    check_close(out, want, bound)
+
+
+def test_repeats_and_streams():
+    """The same bits every time, on side streams too and while another call runs."""
+    sets = [_make(T, 512, E, F, 512, "swiglu", BF16, seed=T) for T, E, F in ((1, 64, 352), (30, 16, 512), (64, 8, 1000))]
+    want = [_moe(**a, top_k=2) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(20):
+        for a, s in zip(sets, streams):
+            with torch.cuda.stream(s):
+                got.append(_moe(**a, top_k=2))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert all(torch.equal(u, v) for u, v in zip(g, want[i % len(want)]))
+
+
+def test_a_block_of_a_served_model():
+    """Attention output projection, experts and a shared expert as one decode step, eager and as two captured graphs
+    replayed in turn, with new inputs each time."""
+    from revealaiccl_b200.ops.linear import linear
+    T, D, E, F, S = 11, 256, 16, 96, 160
+    a = _make(T, D, E, F, D, "swiglu", BF16, seed=8)
+    g = torch.Generator(DEV).manual_seed(9)
+    attn = torch.randn(T, D, generator=g, device=DEV).bfloat16()
+    wo = (torch.randn(D, D, generator=g, device=DEV) * D ** -0.5).bfloat16()
+    su = (torch.randn(2 * S, D, generator=g, device=DEV) * D ** -0.5).bfloat16()
+    sd = (torch.randn(D, S, generator=g, device=DEV) * S ** -0.5).bfloat16()
+    x = a.pop("x")
+
+    def step():
+        h = linear(attn, wo, residual=x)
+        y, ids, gates = _moe(h, **a, top_k=4, residual=h)
+        return h, linear(linear(h, su, act="swiglu"), sd, residual=y, out=y), ids, gates
+
+    def check(result):
+        h, y, ids, gates = result
+        want, bound = linear64(attn, wo, residual=x)
+        check_close(h, want, bound)
+        want, bound, rid, rg, _, gap = moe64(h, **a, top_k=4, act="swiglu", gate_mode="topk_softmax", residual=h)
+        assert gap > 1e-6 and torch.equal(ids.cpu(), rid)
+        u = linear(h, su, act="swiglu")
+        s, sb = linear64(u, sd)
+        # the routed sum was rounded once before the shared expert's product was added
+        check_close(y, want + s, bound + sb + HALF[BF16] * (want + s).abs() + HALF[BF16] * bound)
+
+    check(step())
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            result = step()
+        graphs.append((graph, result))
+    for i in range(4):
+        attn.normal_(generator=g), x.normal_(generator=g)
+        want = [t.clone() for t in step()]
+        graph, result = graphs[i % 2]
+        graph.replay()
+        assert all(torch.equal(u, v) for u, v in zip(result, want))
+        check(result)

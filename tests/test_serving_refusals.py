@@ -1,0 +1,101 @@
+"""What linear() and moe_few_tokens() refuse: shapes, types and strides are checked before the device, so no GPU is needed."""
+
+import pytest
+import torch
+
+from revealaiccl_b200.ops import _native
+
+if not _native.has_kernels():  # pragma: no cover
+    pytest.skip("kernel library not built", allow_module_level=True)
+
+BF16 = torch.bfloat16
+
+
+def _linear(**kw):
+    from revealaiccl_b200.ops.linear import linear
+    a = dict(x=torch.zeros(3, 16, dtype=BF16), weight=torch.zeros(8, 16, dtype=BF16))
+    a.update(kw)
+    return linear(a.pop("x"), a.pop("weight"), a.pop("bias", None), **a)
+
+
+def _moe(**kw):
+    from revealaiccl_b200.ops.moe_few import moe_few_tokens
+    a = dict(x=torch.zeros(3, 16, dtype=BF16), router_w=torch.zeros(4, 16, dtype=BF16), w1=torch.zeros(4, 24, 16, dtype=BF16),
+             w2=torch.zeros(4, 10, 12, dtype=BF16), top_k=2)
+    a.update(kw)
+    return moe_few_tokens(**a)
+
+
+X = torch.zeros(3, 16, dtype=BF16)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(), "CUDA device"),
+    (dict(act="tanh"), "act must be one of"),
+    (dict(x=torch.zeros(16, dtype=BF16)), r"x is \[M, K\]"),
+    (dict(weight=torch.zeros(8, 15, dtype=BF16)), "15 columns"),
+    (dict(weight=torch.zeros(7, 16, dtype=BF16), act="swiglu"), "as many up rows"),
+    (dict(weight=torch.zeros(8, 16)), "both be bf16 or both be fp32"),
+    (dict(x=X.half(), weight=torch.zeros(8, 16).half()), "both be bf16 or both be fp32"),
+    (dict(x=torch.zeros(16, 3, dtype=BF16).t()), "contiguous rows"),
+    (dict(bias=torch.zeros(8, dtype=BF16)), "bias must be a contiguous fp32"),
+    (dict(bias=torch.zeros(7)), "bias must be a contiguous fp32"),
+    (dict(residual=torch.zeros(3, 7)), "shape of the output"),
+    (dict(residual=torch.zeros(8, 3).t()), "residual must be fp32 or bf16 with contiguous rows"),
+    (dict(out=torch.zeros(2, 8, dtype=BF16)), "out must have shape"),
+    (dict(out=torch.zeros(3, 8), out_dtype=BF16), "another type"),
+    (dict(out=torch.zeros(8, dtype=BF16).expand(3, 8)), "do not overlap"),
+    (dict(out_dtype=torch.float16), "the output is fp32"),
+    (dict(x=X.float(), weight=torch.zeros(8, 16), out_dtype=BF16), "the output is fp32"),
+])
+def test_linear_refuses(kw, words):
+    with pytest.raises(ValueError, match=words):
+        _linear(**kw)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(), "CUDA device"),
+    (dict(act="tanh"), "act must be one of"),
+    (dict(gate_mode="sigmoid"), "gate_mode must be one of"),
+    (dict(x=torch.zeros(65, 16, dtype=BF16)), "at most 64 tokens"),
+    (dict(router_w=torch.zeros(256, 16, dtype=BF16)), "1 to 255 experts"),
+    (dict(router_w=torch.zeros(0, 16, dtype=BF16)), "1 to 255 experts"),
+    (dict(top_k=0), "top_k"),
+    (dict(top_k=5), "top_k"),
+    (dict(w1=torch.zeros(4, 12, 16, dtype=BF16)), "shapes differ"),
+    (dict(w2=torch.zeros(3, 10, 12, dtype=BF16)), "shapes differ"),
+    (dict(w1=torch.zeros(4, 24, 15, dtype=BF16)), "shapes differ"),
+    (dict(w2=torch.zeros(4, 10, 0, dtype=BF16), w1=torch.zeros(4, 0, 16, dtype=BF16)), "widths"),
+    (dict(w1=torch.zeros(4, 24, 16)), "all be bf16 or all be fp32"),
+    (dict(w1=torch.zeros(4, 16, 24, dtype=BF16).transpose(1, 2)), "contiguous rows"),
+    (dict(router_b=torch.zeros(3)), "router_b"),
+    (dict(b1=torch.zeros(4, 12)), "b1"),
+    (dict(b2=torch.zeros(4, 10, dtype=BF16)), "b2"),
+    (dict(block_mask=torch.zeros(4)), "block_mask"),
+    (dict(block_mask=torch.zeros(2, 4, dtype=torch.bool)), "block_mask"),
+    (dict(residual=torch.zeros(3, 12)), "shape of the output"),
+    (dict(out=torch.zeros(3, 11)), "out must have shape"),
+])
+def test_moe_refuses(kw, words):
+    with pytest.raises(ValueError, match=words):
+        _moe(**kw)
+
+
+def test_gradients_are_refused():
+    with pytest.raises(RuntimeError, match="no backward"):
+        _linear(weight=torch.zeros(8, 16, requires_grad=True), x=torch.zeros(3, 16))
+    with pytest.raises(RuntimeError, match="no backward"):
+        _moe(w2=torch.zeros(4, 10, 12, dtype=BF16, requires_grad=True))
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):
+        _linear(weight=torch.zeros(8, 16, requires_grad=True), x=torch.zeros(3, 16))
+
+
+def test_shared_memory_is_refused():
+    buf = torch.zeros(3, 24, dtype=BF16)
+    with pytest.raises(ValueError, match="shares memory with an input"):
+        _linear(x=buf[:, :16], out=buf[:, 16:])
+    r = torch.zeros(4, 8, dtype=BF16)
+    with pytest.raises(ValueError, match="shares memory with residual"):
+        _linear(residual=r[:3], out=r[1:])
+    with pytest.raises(ValueError, match="CUDA device"):
+        _linear(residual=r[:3], out=r[:3])
