@@ -1,0 +1,632 @@
+// Experts of a few-token mixture-of-experts layer on the tensor cores: the
+// chosen experts' weights are read once, at the rate that memory gives them.
+//
+// Both products run with the weights as the 128-row operand of tcgen05.mma and
+// the tokens as its narrow N side, so a weight goes from memory to shared
+// memory (TMA) to the tensor core without passing through registers.
+//
+// Split.  The hidden rows of all chosen experts, in units of 16, are dealt to
+// the CTAs (one per SM) as contiguous ranges of equal size; a range may span
+// experts.  Hidden row f needs row f of W1 (rows f and F + f for SwiGLU) and
+// column f of W2, so a CTA makes its rows' activations for the expert's tokens,
+// keeps them in shared memory, and multiplies them by its columns of W2: no
+// CTA waits for another between the two products, and every CTA has the same
+// number of weights to read.  What remains is a sum over the CTAs of an expert
+// and over the experts of a token.  Each CTA writes its part of the expert's
+// result; for each 128 columns, the expert's last CTA to arrive adds the parts
+// in CTA order, and the layer's last expert to arrive adds the experts in the
+// order of the token's choices, applies the gates and adds the residual.  The
+// order of the additions never depends on the order of arrival, and nobody waits.
+//
+// Steps of a CTA's range (roles: one TMA thread, one MMA thread, four epilogue
+// warps; fp32 also four splitting warps), for each expert in it:
+//   product 1   tiles of 128 rows of W1 (64 gate + 64 up rows, 16 by 16), K = D
+//               in 128-byte steps, against all T tokens; the epilogue applies
+//               bias and activation and keeps the expert's own tokens, rounded
+//               to bf16 (fp32: as two tf32 parts) in the swizzled layout that
+//               product 2 reads
+//   product 2   tiles of 128 rows of W2, K = the range's hidden rows
+//
+// fp32 weights are split into two tf32 parts of 11 bits each in shared memory,
+// h + l; x and the activations too.  h h' + h l' + l h' is the product to 2^-21:
+// the tokens' parts are stacked as 2N columns, so that is two instructions.
+#pragma once
+
+#include "serving.h"
+#include "serving_device.cuh"
+#include "sm100_ptx.cuh"
+
+namespace raiccl {
+
+constexpr int kFewTile = 128 * 128;           // bytes of a weight tile: 128 rows of 128 bytes
+constexpr unsigned long long kFewWaitNs = 2000000000ull;
+constexpr int kFewKernelId = 600;
+
+// What the launch fixes.
+struct FewTcParams {
+  FewExpertParams e;
+  float* part;        // [rows, Op] the CTAs' parts of the experts' results
+  float* y;           // [T k, Op] the experts' results, by expert, then token
+  int* count;         // [min(E, T k) + 1][nO] arrivals, zeroed by the routing kernel
+  int Op;             // O rounded up to 128
+  int Tp;             // T rounded up to 16
+  int stages;
+  int hbytes;         // shared memory of the activations
+};
+
+template <bool FP32>
+struct FewTc {
+  static constexpr int EB = FP32 ? 4 : 2;
+  static constexpr int BK = 128 / EB;              // elements of a 128-byte row
+  static constexpr int PARTS = FP32 ? 2 : 1;
+  static constexpr int UPS = BK / 16;              // units of 16 hidden rows in a 128-byte row of activations
+  static constexpr int TAIL = 16 * EB;             // bytes of one unit in a row
+  static constexpr int THREADS = FP32 ? 320 : 192;
+  static constexpr uint32_t FORMAT = FP32 ? 2u : 1u;
+  static __host__ __device__ int stage_bytes(int Tp) { return PARTS * kFewTile + PARTS * Tp * 128; }
+};
+
+// fp32 as two tf32 numbers of 11 significant bits, rounded to nearest; what
+// would round to infinity is cut instead, and an infinity has no low part.
+__device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
+  const uint32_t b = __float_as_uint(v);
+  uint32_t h = (b + 0x1000u) & ~0x1fffu;
+  if ((h & 0x7f800000u) == 0x7f800000u) h = b & ~0x1fffu;
+  hi = __uint_as_float(h);
+  const float l = v == hi ? 0.f : v - hi;
+  lo = l != l ? l : __uint_as_float((__float_as_uint(l) + 0x1000u) & ~0x1fffu);
+}
+
+// The plan that every CTA makes of the routed tokens.
+struct FewPlan {
+  unsigned long long mask[kFewExperts + 1];  // by expert: its tokens
+  int used[kFewExperts + 1];                 // the chosen experts, by number
+  int index[kFewExperts + 1];                // their place in used, by expert
+  int part0[kFewExperts + 1];                // by place: first row in part
+  int y0[kFewExperts + 1];                   // by place: first row in y
+  int yrow[kFewTokens * kFewTopK];           // by (token, choice): row in y, -1 without an expert
+  int ne;
+};
+
+// CTA of unit u where U units are dealt to G <= U CTAs: CTA c has units [U c / G, U (c + 1) / G).
+__device__ __forceinline__ int few_cta(long long u, long long U, int G) { return (int)(((u + 1) * G - 1) / U); }
+
+__device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, int UE, int grid) {
+  const int pairs = p.T * p.k;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) s.mask[e] = 0ull;
+  __syncthreads();
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    const int e = __ldcg(p.ids + i);
+    if (e >= 0) atomicOr(&s.mask[e], 1ull << (i / p.k));
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int ne = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const bool has = e0 + lane < p.E && s.mask[e0 + lane] != 0ull;
+      const unsigned b = __ballot_sync(0xffffffffu, has);
+      if (has) {
+        const int at = ne + __popc(b & ((1u << lane) - 1u));
+        s.used[at] = e0 + lane;
+        s.index[e0 + lane] = at;
+      }
+      ne += __popc(b);
+    }
+    __syncwarp();
+    const long long U = (long long)ne * UE;
+    const int G = U < grid ? (int)U : grid;
+    int part = 0, y = 0;
+    for (int i0 = 0; i0 < ne; i0 += 32) {
+      const int i = i0 + lane;
+      int t = 0, rows = 0;
+      if (i < ne) {
+        t = __popcll(s.mask[s.used[i]]);
+        rows = t * (few_cta((long long)(i + 1) * UE - 1, U, G) - few_cta((long long)i * UE, U, G) + 1);
+      }
+      int ts = t, rs = rows;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, ts, o), b = __shfl_up_sync(0xffffffffu, rs, o);
+        if (lane >= o) { ts += a; rs += b; }
+      }
+      if (i < ne) { s.y0[i] = y + ts - t; s.part0[i] = part + rs - rows; }
+      y += __shfl_sync(0xffffffffu, ts, 31);
+      part += __shfl_sync(0xffffffffu, rs, 31);
+    }
+    if (lane == 0) s.ne = ne;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+    const int e = __ldcg(p.ids + i);
+    s.yrow[i] = e < 0 ? -1 : s.y0[s.index[e]] + __popcll(s.mask[e] & ((1ull << (i / p.k)) - 1ull));
+  }
+  __syncthreads();
+}
+
+// A run of units of one expert whose activations fit in shared memory; the
+// roles walk the same runs.
+struct FewRun {
+  int place, expert, tokens, np;   // place in used, expert, its tokens, their number rounded up to 16
+  int f0, units;                   // first hidden row, units of 16
+  bool first, last;                // of the CTA's runs of this expert
+};
+
+struct FewWalk {
+  long long u, u1, U;
+  int UE, G, cap, s, n, a, place;  // cap: 128-byte rows of activations that fit, over all tokens' rows
+  __device__ void start(const FewPlan& plan, int UE_, int grid) {
+    UE = UE_;
+    U = (long long)plan.ne * UE;
+    G = U < grid ? (int)U : grid;
+    const int c = blockIdx.x;
+    u = c < G ? U * c / G : 0;
+    u1 = c < G ? U * (c + 1) / G : 0;
+    s = n = 0;
+  }
+  __device__ bool next(const FewPlan& plan, int hrows, int parts, int ups, FewRun& r) {
+    if (s >= n) {
+      if (u >= u1) return false;
+      place = (int)(u / UE);
+      a = (int)(u - (long long)place * UE);
+      n = (int)(u1 - u < UE - a ? u1 - u : UE - a);
+      u += n;
+      s = 0;
+    }
+    r.place = place;
+    r.expert = plan.used[place];
+    r.tokens = __popcll(plan.mask[r.expert]);
+    r.np = (r.tokens + 15) & ~15;
+    const int cap = hrows / (r.np * parts) * ups;
+    r.units = n - s < cap ? n - s : cap;
+    r.f0 = (a + s) * 16;
+    r.first = s == 0;
+    s += r.units;
+    r.last = s >= n;
+    return true;
+  }
+};
+
+// Adds the parts of expert `place` for 128 columns, in CTA order, plus the
+// bias, into y.  The four epilogue warps; each thread has four columns.
+__device__ __forceinline__ void few_join_parts(const FewTcParams& p, const FewPlan& s, int place, int expert, int tokens,
+                                               int n, int o0, float (*red)[128]) {
+  const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int o = o0 + lane * 4;
+  const float4* src = (const float4*)(p.part + (long long)s.part0[place] * p.Op + o);
+  float4* dst = (float4*)(p.y + (long long)s.y0[place] * p.Op + o);
+  const long long row = p.Op / 4, step = row * tokens;
+  float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.e.b2) {
+    const float* b2 = p.e.b2 + (long long)expert * p.e.O;
+    b.x = o < p.e.O ? b2[o] : 0.f;
+    b.y = o + 1 < p.e.O ? b2[o + 1] : 0.f;
+    b.z = o + 2 < p.e.O ? b2[o + 2] : 0.f;
+    b.w = o + 3 < p.e.O ? b2[o + 3] : 0.f;
+  }
+  if (tokens >= 4) {  // a token per warp
+    for (int t = w; t < tokens; t += 4) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int c = 0; c < n; ++c) {
+        const float4 a = __ldcg(src + t * row + c * step);
+        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+      }
+      dst[t * row] = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+    }
+  } else {            // few tokens, many parts: a quarter of the parts per warp
+    for (int t = 0; t < tokens; ++t) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int c = w; c < n; c += 4) {
+        const float4 a = __ldcg(src + t * row + c * step);
+        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+      }
+      *(float4*)&red[w][lane * 4] = v;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (w == 0) {
+#pragma unroll
+        for (int q = 1; q < 4; ++q) {
+          const float4 a = *(const float4*)&red[q][lane * 4];
+          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+        }
+        dst[t * row] = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+    }
+  }
+}
+
+// The tokens' results for 128 columns: their experts in the order of choice, gates, residual.
+__device__ __forceinline__ void few_join_experts(const FewTcParams& p, const FewPlan& s, int o0) {
+  const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  const int o = o0 + lane * 4;
+  const FewExpertParams& e = p.e;
+  for (int t = w; t < e.T; t += 4) {
+    float4 a[kFewTopK];
+    float g[kFewTopK];
+#pragma unroll
+    for (int j = 0; j < kFewTopK; ++j) {
+      const int row = j < e.k ? s.yrow[t * e.k + j] : -1;
+      g[j] = 0.f;
+      a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (row >= 0) {
+        g[j] = __ldcg(e.gates + t * e.k + j);
+        a[j] = __ldcg((const float4*)(p.y + (long long)row * p.Op + o));
+      }
+    }
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < kFewTopK; ++j) {
+      v[0] = fmaf(g[j], a[j].x, v[0]);
+      v[1] = fmaf(g[j], a[j].y, v[1]);
+      v[2] = fmaf(g[j], a[j].z, v[2]);
+      v[3] = fmaf(g[j], a[j].w, v[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (o + i >= e.O) break;
+      if (e.residual) v[i] += load_elem(e.residual, (long long)t * e.res_stride + o + i, e.res_bf16);
+      store_elem(e.out, (long long)t * e.out_stride + o + i, v[i], e.out_bf16);
+    }
+  }
+}
+
+// Maps: x [T, D] in boxes of 128 bytes x Tp rows (fp32: [2 Tp, D] parts, 2 Tp
+// rows); W1 in boxes of 128 bytes x 16 rows (SwiGLU: x 2, gate and up); W2 in
+// boxes of 128 bytes x 128 rows and of one unit x 128 rows.
+template <bool FP32, bool GLU>
+__global__ void __launch_bounds__(FewTc<FP32>::THREADS, 1)
+few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap t1,
+                   const __grid_constant__ CUtensorMap t2, const __grid_constant__ CUtensorMap t2u, FewTcParams p,
+                   DeviceStatus* status) {
+  using C = FewTc<FP32>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ FewPlan plan;
+  __shared__ uint64_t full[16], empty[16], parted[16], acc1_full[2], acc1_empty[2], acc2_full[2], acc2_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int arrived;
+  __shared__ __align__(16) float red[4][128];
+  const int SB = C::stage_bytes(p.Tp), S = p.stages;
+  uint8_t* const hbuf = smem + S * SB;
+  const FewExpertParams& e = p.e;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n1 = C::PARTS * p.Tp;                       // columns of product 1's accumulator
+  const int cols = 4 * n1 <= 64 ? 64 : 4 * n1 <= 128 ? 128 : 4 * n1 <= 256 ? 256 : 512;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], 4); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc1_full[i], 1); mbar_init(&acc1_empty[i], 4);
+      mbar_init(&acc2_full[i], 1); mbar_init(&acc2_empty[i], 4);
+    }
+    mbar_init(&drained, 1);
+    fence_mbarrier_init();
+    tma_prefetch_desc(&tx); tma_prefetch_desc(&t1); tma_prefetch_desc(&t2); tma_prefetch_desc(&t2u);
+  }
+  if (warp == 1) { tmem_alloc(&tmem_slot, cols); tmem_relinquish(); }
+  tc_fence_before_sync();
+  griddep_wait();
+  const int UE = (e.F + 15) / 16;
+  few_plan(e, plan, UE, gridDim.x);   // holds __syncthreads
+  griddep_launch_dependents();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const int KB = (e.D + C::BK - 1) / C::BK;             // 128-byte steps of product 1
+  const int nO = p.Op / 128;
+  const int TU = GLU ? 4 : 8;                           // units of a product-1 tile
+  const int hrows = p.hbytes / 128;
+  const int rot = (int)(((long long)blockIdx.x * nO) / gridDim.x);  // so that the last arrivals of a column are spread
+  FewWalk walk;
+  walk.start(plan, UE, gridDim.x);
+  FewRun r;
+  int stage = 0;
+  uint32_t phase = 0;
+  auto advance = [&]() { if (++stage == S) { stage = 0; phase ^= 1u; } };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads
+    if (elect_one_sync()) {
+      bool ok = true;
+      while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
+        for (int u0 = 0; ok && u0 < r.units; u0 += TU) {
+          const int nu = r.units - u0 < TU ? r.units - u0 : TU;
+          for (int kb = 0; kb < KB; ++kb) {
+            if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+            uint8_t* w = smem + stage * SB;
+            mbar_arrive_expect_tx(&full[stage], nu * (GLU ? 4096 : 2048) + n1 * 128);
+            for (int u = 0; u < nu; ++u) {
+              const int f = r.f0 + (u0 + u) * 16;
+              if constexpr (GLU) tma_load_4d(w + u * 4096, &t1, &full[stage], kb * C::BK, f, 0, r.expert);
+              else tma_load_3d(w + u * 2048, &t1, &full[stage], kb * C::BK, f, r.expert);
+            }
+            tma_load_2d(w + C::PARTS * kFewTile, &tx, &full[stage], kb * C::BK, 0);
+            advance();
+          }
+        }
+        const int slices = r.units / C::UPS, tail = r.units % C::UPS;
+        for (int i = 0; ok && i < nO; ++i) {
+          const int o = (i + rot) % nO * 128;
+          for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
+            if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+            uint8_t* w = smem + stage * SB;
+            const int f = r.f0 + s * C::BK;
+            if (s < slices) {
+              mbar_arrive_expect_tx(&full[stage], kFewTile);
+              tma_load_3d(w, &t2, &full[stage], f, o, r.expert);
+            } else {
+              mbar_arrive_expect_tx(&full[stage], tail * 128 * C::TAIL);
+              for (int u = 0; u < tail; ++u) tma_load_3d(w + u * 128 * C::TAIL, &t2u, &full[stage], f + u * 16, o, r.expert);
+            }
+            advance();
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products
+    if (elect_one_sync()) {
+      uint64_t* ready = FP32 ? parted : full;
+      int i1 = 0, i2 = 0;
+      bool ok = true;
+      // one 128-byte K step: 32 bytes at a time, weights [hi | lo] against token rows [hi; lo]
+      auto step = [&](uint32_t d, uint64_t a, uint64_t alo, uint64_t b, int n, uint32_t more) {
+        if constexpr (FP32) {
+          umma_tf32(d, a, b, umma_idesc(2u, 128, 2 * n), more);
+          umma_tf32(d, alo, b, umma_idesc(2u, 128, n), 1u);
+        } else {
+          umma_f16(d, a, b, umma_idesc(1u, 128, n), more);
+        }
+      };
+      while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
+        for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
+          const int b = i1 & 1;
+          if (!(ok = mbar_wait_bounded(&acc1_empty[b], ((i1 >> 1) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+          tc_fence_after_sync();
+          const uint32_t d = tmem + b * n1;
+          for (int kb = 0; kb < KB; ++kb) {
+            if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+            tc_fence_after_sync();
+            const uint32_t w = smem_u32(smem + stage * SB), x = w + C::PARTS * kFewTile;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(x + k * 32),
+                   p.Tp, (kb | k) ? 1u : 0u);
+            umma_commit(&empty[stage]);
+            advance();
+          }
+          umma_commit(&acc1_full[b]);
+        }
+        // the activations of every tile are in shared memory once its accumulator was released
+        for (int b = 0; ok && b < 2; ++b) {
+          const int uses = (i1 + 1 - b) >> 1;
+          if (uses > 0) ok = mbar_wait_bounded(&acc1_empty[b], (uses - 1) & 1, status, kFewKernelId, kFewWaitNs);
+        }
+        tc_fence_after_sync();
+        const int slices = r.units / C::UPS, tail = r.units % C::UPS;
+        const uint32_t hrow = C::PARTS * r.np * 128;   // bytes of a slice of activations
+        for (int i = 0; ok && i < nO; ++i, ++i2) {
+          const int b = i2 & 1;
+          if (!(ok = mbar_wait_bounded(&acc2_empty[b], ((i2 >> 1) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+          tc_fence_after_sync();
+          const uint32_t d = tmem + 2 * n1 + b * n1;
+          for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
+            if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+            tc_fence_after_sync();
+            const uint32_t w = smem_u32(smem + stage * SB), h = smem_u32(hbuf) + s * hrow;
+            if (s < slices) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(h + k * 32),
+                     r.np, (s | k) ? 1u : 0u);
+            } else {
+              constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
+              for (int u = 0; u < tail; ++u)
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                  const uint32_t a = w + u * 128 * C::TAIL + k * 32;
+                  step(d, umma_desc_k_narrow(a, C::TAIL), umma_desc_k_narrow(a + kFewTile, C::TAIL),
+                       umma_desc_k_sw128(h + (u * KS + k) * 32), r.np, (s | u | k) ? 1u : 0u);
+                }
+            }
+            umma_commit(&empty[stage]);
+            advance();
+          }
+          umma_commit(&acc2_full[b]);
+        }
+      }
+      // every product has finished before the accumulators are freed
+      umma_commit(&drained);
+      mbar_wait_bounded(&drained, 0, status, kFewKernelId, kFewWaitNs);
+    }
+  } else if (warp < 6) {
+    // ---------------------------------------------------------------- epilogues
+    const int q = warp & 3;                               // TMEM lanes 32 q .. 32 q + 31
+    const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16);
+    int i1 = 0, i2 = 0;
+    // A wait that runs out is carried to the next vote: the four warps share
+    // named barriers, so they only leave together.
+    bool ok = true, alive = true;
+    while (alive && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
+      const unsigned long long mask = plan.mask[r.expert];
+      const float* b1 = e.b1 ? e.b1 + (long long)r.expert * (GLU ? 2 : 1) * e.F : nullptr;
+      const uint32_t hrow = C::PARTS * r.np * 128;
+      for (int u0 = 0; u0 < r.units; u0 += TU, ++i1) {
+        const int b = i1 & 1;
+        const int unit = u0 + (GLU ? q : 2 * q + (lane >> 4));  // of the run
+        const int fl = unit * 16 + (lane & 15);           // hidden row of the run
+        const int f = r.f0 + fl;
+        const bool real = f < e.F;
+        float bias = 0.f, bias_up = 0.f;
+        if (b1 && real && unit < r.units) {
+          bias = __ldg(b1 + f);
+          if constexpr (GLU) bias_up = __ldg(b1 + e.F + f);
+        }
+        ok = mbar_wait_bounded(&acc1_full[b], (i1 >> 1) & 1, status, kFewKernelId, kFewWaitNs) && ok;
+        tc_fence_after_sync();
+        const uint32_t base = lane_addr + b * n1;
+        uint8_t* hcol = hbuf + (fl / C::BK) * hrow;
+        const int byte = (fl % C::BK) * C::EB;
+        const bool any = u0 + (GLU ? q : 2 * q) < r.units;  // this warp has a unit of the tile
+        for (int c = 0; any && c < p.Tp; c += 16) {
+          const unsigned take = (unsigned)(mask >> c) & 0xffffu;   // the expert's tokens among these 16
+          if (take == 0u) continue;
+          uint32_t v[16];
+          tmem_ld16(base + c, v);
+          if constexpr (FP32) {
+            uint32_t l[16];
+            tmem_ld16(base + p.Tp + c, l);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(l[i]));
+          } else {
+            tmem_ld_wait();
+          }
+          const int below = __popcll(mask & ((1ull << c) - 1ull));
+          auto put = [&](int i, float val) {   // activation of token c + i
+            const int n = below + __popc(take & ((1u << i) - 1u));
+            const float h = real ? val : 0.f;
+            uint8_t* at = hcol + (n >> 3) * 1024 + (n & 7) * 128 + (byte ^ ((n & 7) << 4));
+            if constexpr (FP32) {
+              float hi, lo;
+              split_tf32(h, hi, lo);
+              *(float*)at = hi;
+              *(float*)(at + r.np * 128) = lo;
+            } else {
+              *(__nv_bfloat16*)at = __float2bfloat16_rn(h);
+            }
+          };
+          if constexpr (GLU) {
+            // lanes 0-15 hold gate rows, 16-31 the up rows of the same f: each half takes eight of the columns
+            const bool up = lane >= 16;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float mine = __uint_as_float(up ? v[8 + i] : v[i]);
+              const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(up ? v[i] : v[8 + i]), 16);
+              const int col = up ? 8 + i : i;
+              const float gate = (up ? other : mine) + bias, lin = (up ? mine : other) + bias_up;
+              if (take >> col & 1u) put(col, serving_swiglu(gate, lin));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if ((take >> i & 1u) && unit < r.units) put(i, serving_act(__uint_as_float(v[i]) + bias, e.act));
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc1_empty[b]);
+      }
+      // product 2: this CTA's part of the expert's result, or the result where no other CTA has a part
+      const int first = few_cta((long long)r.place * UE, walk.U, walk.G);
+      const int n = few_cta((long long)(r.place + 1) * UE - 1, walk.U, walk.G) - first + 1;
+      const bool alone = n == 1;
+      float* dst = alone ? p.y + (long long)plan.y0[r.place] * p.Op
+                         : p.part + (long long)(plan.part0[r.place] + ((int)blockIdx.x - first) * r.tokens) * p.Op;
+      for (int i = 0; i < nO; ++i, ++i2) {
+        const int b = i2 & 1;
+        const int ot = (i + rot) % nO, o = ot * 128 + q * 32 + lane;
+        float bias = 0.f;
+        if (alone && r.first && e.b2 && o < e.O) bias = __ldg(e.b2 + (long long)r.expert * e.O + o);
+        ok = mbar_wait_bounded(&acc2_full[b], (i2 >> 1) & 1, status, kFewKernelId, kFewWaitNs) && ok;
+        tc_fence_after_sync();
+        const uint32_t base = lane_addr + 2 * n1 + b * n1;
+        for (int c = 0; c < r.tokens; c += 16) {
+          uint32_t v[16];
+          tmem_ld16(base + c, v);
+          if constexpr (FP32) {
+            uint32_t l[16];
+            tmem_ld16(base + r.np + c, l);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(l[j]));
+          } else {
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (c + j >= r.tokens) break;
+            float* at = dst + (long long)(c + j) * p.Op + o;
+            float out = __uint_as_float(v[j]) + bias;
+            if (!r.first) out += *at;   // written by this thread
+            *at = out;
+          }
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc2_empty[b]);
+        if (!r.last) continue;
+        // arrivals: the expert's parts, then the layer's experts
+        __threadfence();
+        int go;
+        asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %1, 0;\n\tbar.red.and.pred b, 1, 128, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
+                     : "=r"(go) : "r"((int)ok) : "memory");
+        alive = go != 0;
+        if (!alive) break;
+        bool join = alone;
+        if (!alone) {
+          if (warp == 2 && lane == 0) arrived = atom_add_acq_rel_gpu(p.count + (long long)(1 + r.place) * nO + ot, 1);
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          join = arrived == n - 1;
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (join) {
+            __threadfence();
+            few_join_parts(p, plan, r.place, r.expert, r.tokens, n, ot * 128, red);
+            __threadfence();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+          }
+        }
+        if (join) {
+          if (warp == 2 && lane == 0) arrived = atom_add_acq_rel_gpu(p.count + ot, 1);
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          const bool whole = arrived == plan.ne - 1;
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (whole) {
+            __threadfence();
+            few_join_experts(p, plan, ot * 128);
+          }
+        }
+      }
+    }
+    if (plan.ne == 0)   // no token has an expert: the residual, or zeros
+      for (int ot = blockIdx.x; ot < nO; ot += gridDim.x) few_join_experts(p, plan, ot * 128);
+  } else if constexpr (FP32) {
+    // ---------------------------------------------------------------- weights into tf32 parts
+    const int tid = threadIdx.x - 192;
+    bool ok = true;
+    auto part = [&](int bytes) {
+      if (!(ok = mbar_wait_bounded(&full[stage], phase, status, kFewKernelId, kFewWaitNs))) return;
+      uint8_t* w = smem + stage * SB;
+      for (int i = tid * 16; i < bytes; i += 128 * 16) {
+        float4 v = *(float4*)(w + i), h, l;
+        split_tf32(v.x, h.x, l.x);
+        split_tf32(v.y, h.y, l.y);
+        split_tf32(v.z, h.z, l.z);
+        split_tf32(v.w, h.w, l.w);
+        *(float4*)(w + i) = h;
+        *(float4*)(w + kFewTile + i) = l;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&parted[stage]);
+      advance();
+    };
+    while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
+      for (int u0 = 0; ok && u0 < r.units; u0 += TU) {
+        const int nu = r.units - u0 < TU ? r.units - u0 : TU;
+        for (int kb = 0; ok && kb < KB; ++kb) part(nu * (GLU ? 4096 : 2048));
+      }
+      const int slices = r.units / C::UPS, tail = r.units % C::UPS;
+      for (int i = 0; ok && i < nO; ++i)
+        for (int s = 0; ok && s < slices + (tail ? 1 : 0); ++s) part(s < slices ? kFewTile : tail * 128 * C::TAIL);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, cols);
+}
+
+}  // namespace raiccl

@@ -32,6 +32,11 @@ struct FewRouteParams {
   int vec;                // rows of x and w are 16-byte aligned multiples of 16 bytes
   int* ids;               // [T, k], -1 where no expert was left
   float* gates;           // [T, k], 0 there
+  int* zero;              // zeroed for the experts' kernel
+  int n_zero;
+  void* packed;           // x for the experts' kernel, or nullptr: bf16 rows [T, packed_stride] as they are;
+  long long packed_stride;  // fp32 [2][packed_rows, packed_stride] as two tf32 parts
+  int packed_rows;
 };
 
 // The experts' MLPs and the weighted sum of the routed tokens.
@@ -50,15 +55,28 @@ struct FewExpertParams {
   long long out_stride;
   const int* ids;         // [T, k]
   const float* gates;     // [T, k]
-  float* h;               // [T k, F] scratch
-  float* y;               // [T k, O] scratch
   int T, D, E, k, F, O;
   int act;
   int bf16, out_bf16, res_bf16;
 };
 
+// How the experts of a call run, and the device memory that they need besides.
+struct FewExpertPlan {
+  int tensor;             // on the tensor cores (else one warp per weight row)
+  int grid, stages, hbytes, Op, Tp;
+  int pack;               // x is packed by the routing kernel
+  int packed_stride;
+  int n_zero;             // ints zeroed by the routing kernel
+  long long zero_bytes, packed_bytes, a_bytes, b_bytes;  // multiples of 256; in this order in the workspace
+  long long bytes() const { return zero_bytes + packed_bytes + a_bytes + b_bytes; }
+};
+
+FewExpertPlan plan_few_experts(const FewExpertParams& p);
 void launch_few_route(const FewRouteParams& p, cudaStream_t s);
-void launch_few_experts(const FewExpertParams& p, cudaStream_t s);
+void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s);
+
+// The current device's record of a wait that ran out in a serving operator (device memory).
+DeviceStatus* serving_status();
 
 // out = act(x w^T + bias) + residual; SwiGLU: w holds F gate rows, then F up
 // rows, and N = F is the width of out.

@@ -9,15 +9,38 @@
 //   out[t]  = sum_j g[t, j] (W2[e] act(W1[e] x[t] + b1[e]) + b2[e]) + residual[t],  e = ids[t, j]
 #include <cooperative_groups.h>
 
+#include <algorithm>
+#include <atomic>
 #include <stdexcept>
 
+#include "moe_few_tc.cuh"
 #include "serving.h"
 #include "serving_device.cuh"
+#include "serving_tma.h"
 #include "sm100_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace raiccl {
+
+__device__ DeviceStatus g_serving_status;
+
+static int current_device() {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  return dev & 63;
+}
+
+DeviceStatus* serving_status() {
+  static std::atomic<void*> at[64];
+  const int dev = current_device();
+  void* p = at[dev].load();
+  if (p == nullptr) {
+    if (cudaGetSymbolAddress(&p, g_serving_status) != cudaSuccess) throw std::runtime_error("serving operators: no device status");
+    at[dev].store(p);
+  }
+  return (DeviceStatus*)p;
+}
 
 // ---------------------------------------------------------------------------
 // Routing: one cluster per token, its CTAs and their warps share the experts.
@@ -70,6 +93,20 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* x = (const T*)p.x + (long long)t * p.x_stride;
   float* lead = cluster.map_shared_rank(logits, 0);
+  griddep_wait();
+  griddep_launch_dependents();
+  const int share = rank * kRouteThreads + threadIdx.x, shares = ranks * kRouteThreads;
+  for (int i = t * shares + share; i < p.n_zero; i += p.T * shares) p.zero[i] = 0;
+  if (p.packed) {
+    for (int d = share; d < p.D; d += shares) {
+      if constexpr (sizeof(T) == 4) {
+        float* at = (float*)p.packed + (long long)t * p.packed_stride + d;
+        split_tf32(x[d], at[0], at[(long long)p.packed_rows * p.packed_stride]);
+      } else {
+        ((T*)p.packed)[(long long)t * p.packed_stride + d] = x[d];
+      }
+    }
+  }
   for (int e = warp * ranks + rank; e < p.E; e += kRouteWarps * ranks) {
     float v = route_dot(x, (const T*)p.w + (long long)e * p.w_stride, p.D, p.vec);
     if (lane == 0) {
@@ -133,13 +170,15 @@ void launch_few_route(const FewRouteParams& p, cudaStream_t s) {
   cfg.gridDim = dim3(ranks, p.T);
   cfg.blockDim = dim3(kRouteThreads);
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = ranks;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (p.bf16) cudaLaunchKernelEx(&cfg, few_route_kernel<__nv_bfloat16>, p);
   else cudaLaunchKernelEx(&cfg, few_route_kernel<float>, p);
 }
@@ -167,7 +206,7 @@ __device__ __forceinline__ int few_pairs(const int* ids, int T, int k, int e, in
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams p) {
+__global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams p, float* h) {
   __shared__ int list[kFewTokens];
   const int e = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = few_pairs(p.ids, p.T, p.k, e, list);
@@ -197,7 +236,7 @@ __global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams
       if (lane == 0 && i0 + i < n) {
         const float* b1 = p.b1 ? p.b1 + (long long)e * (glu ? 2 : 1) * p.F : nullptr;
         const float z = g[i] + (b1 ? b1[f] : 0.f);
-        p.h[(long long)list[i0 + i] * p.F + f] =
+        h[(long long)list[i0 + i] * p.F + f] =
             glu ? serving_swiglu(z, u[i] + (b1 ? b1[p.F + f] : 0.f)) : serving_act(z, p.act);
       }
     }
@@ -205,7 +244,7 @@ __global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams p) {
+__global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams p, const float* hidden, float* y) {
   __shared__ int list[kFewTokens];
   const int e = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = few_pairs(p.ids, p.T, p.k, e, list);
@@ -215,7 +254,7 @@ __global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams
   for (int i0 = 0; i0 < n; i0 += kRowTokens) {
     float acc[kRowTokens] = {};
     const float* h[kRowTokens];
-    for (int i = 0; i < kRowTokens; ++i) h[i] = p.h + (long long)list[min(i0 + i, n - 1)] * p.F;
+    for (int i = 0; i < kRowTokens; ++i) h[i] = hidden + (long long)list[min(i0 + i, n - 1)] * p.F;
     for (int f = lane; f < p.F; f += 32) {
       const float a = as_float(w[f]);
 #pragma unroll
@@ -225,33 +264,158 @@ __global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams
     for (int i = 0; i < kRowTokens; ++i) {
       acc[i] = warp_sum(acc[i]);
       if (lane == 0 && i0 + i < n)
-        p.y[(long long)list[i0 + i] * p.O + o] = acc[i] + (p.b2 ? p.b2[(long long)e * p.O + o] : 0.f);
+        y[(long long)list[i0 + i] * p.O + o] = acc[i] + (p.b2 ? p.b2[(long long)e * p.O + o] : 0.f);
     }
   }
 }
 
-__global__ void __launch_bounds__(kRowThreads) few_join_kernel(FewExpertParams p) {
+__global__ void __launch_bounds__(kRowThreads) few_join_kernel(FewExpertParams p, const float* y) {
   const long long i = (long long)blockIdx.x * kRowThreads + threadIdx.x;
   if (i >= (long long)p.T * p.O) return;
   const int t = (int)(i / p.O), o = (int)(i % p.O);
   float acc = 0.f;
   for (int j = 0; j < p.k; ++j)
-    if (p.ids[t * p.k + j] >= 0) acc = fmaf(p.gates[t * p.k + j], p.y[(long long)(t * p.k + j) * p.O + o], acc);
+    if (p.ids[t * p.k + j] >= 0) acc = fmaf(p.gates[t * p.k + j], y[(long long)(t * p.k + j) * p.O + o], acc);
   if (p.residual) acc += load_elem(p.residual, (long long)t * p.res_stride + o, p.res_bf16);
   store_elem(p.out, (long long)t * p.out_stride + o, acc, p.out_bf16);
 }
 
 template <typename T>
-static void launch_rows(const FewExpertParams& p, cudaStream_t s) {
+static void launch_rows(const FewExpertParams& p, float* h, float* y, cudaStream_t s) {
   constexpr int W = kRowThreads / 32;
-  few_hidden_kernel<T><<<dim3((p.F + W - 1) / W, p.E), kRowThreads, 0, s>>>(p);
-  few_output_kernel<T><<<dim3((p.O + W - 1) / W, p.E), kRowThreads, 0, s>>>(p);
-  few_join_kernel<<<(unsigned)(((long long)p.T * p.O + kRowThreads - 1) / kRowThreads), kRowThreads, 0, s>>>(p);
+  few_hidden_kernel<T><<<dim3((p.F + W - 1) / W, p.E), kRowThreads, 0, s>>>(p, h);
+  few_output_kernel<T><<<dim3((p.O + W - 1) / W, p.E), kRowThreads, 0, s>>>(p, h, y);
+  few_join_kernel<<<(unsigned)(((long long)p.T * p.O + kRowThreads - 1) / kRowThreads), kRowThreads, 0, s>>>(p, y);
 }
 
-void launch_few_experts(const FewExpertParams& p, cudaStream_t s) {
-  if (p.bf16) launch_rows<__nv_bfloat16>(p, s);
-  else launch_rows<float>(p, s);
+// ---------------------------------------------------------------------------
+// Launch
+// ---------------------------------------------------------------------------
+static int sm_count() {
+  static std::atomic<int> n[64];
+  const int dev = current_device();
+  int v = n[dev].load();
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1)
+      throw std::runtime_error("serving operators: no SM count");
+    n[dev].store(v);
+  }
+  return v;
+}
+
+static long long up256(long long v) { return (v + 255) / 256 * 256; }
+
+constexpr int kFewShared = 232448 - 12 * 1024 - 1024;  // dynamic shared memory besides the kernel's own and the alignment
+
+FewExpertPlan plan_few_experts(const FewExpertParams& p) {
+  FewExpertPlan r{};
+  const int eb = p.bf16 ? 2 : 4, parts = p.bf16 ? 1 : 2;
+  auto aligned = [&](const void* base, long long row, long long expert) {
+    return ((uintptr_t)base & 15) == 0 && (row * eb) % 16 == 0 && (p.E == 1 || (expert * eb) % 16 == 0);
+  };
+  // TMA reads rows that start on 16 bytes
+  r.tensor = aligned(p.w1, p.w1_stride, p.w1_estride) && aligned(p.w2, p.w2_stride, p.w2_estride);
+  const int pairs = p.T * p.k;
+  if (!r.tensor) {
+    r.a_bytes = up256((long long)pairs * p.F * 4);
+    r.b_bytes = up256((long long)pairs * p.O * 4);
+    return r;
+  }
+  r.grid = sm_count();
+  r.Op = (p.O + 127) / 128 * 128;
+  r.Tp = (p.T + 15) / 16 * 16;
+  const int nO = r.Op / 128, UE = (p.F + 15) / 16, ups = 128 / eb / 16;
+  r.n_zero = (1 + std::min(p.E, pairs)) * nO;
+  r.zero_bytes = up256(4ll * r.n_zero);
+  r.pack = !p.bf16 || !aligned(p.x, p.T > 1 ? p.x_stride : 0, 0);
+  r.packed_stride = (p.D + 7) / 8 * 8;
+  if (r.pack) r.packed_bytes = up256((long long)parts * r.Tp * r.packed_stride * eb);
+  // An expert's tokens times the CTAs that share it, over all experts: n experts have at most min(T k, n T) tokens
+  // and (grid / n + 2) CTAs each, so T (grid + 2 k) rows at most, whatever n is.
+  r.a_bytes = up256((long long)p.T * (r.grid + 2 * p.k) * r.Op * 4);
+  r.b_bytes = up256((long long)pairs * r.Op * 4);
+  // activations: what the longest range of a CTA needs, at most a quarter of shared memory; the rest holds stages
+  const long long most = ((long long)std::min(p.E, pairs) * UE + r.grid - 1) / r.grid;
+  const long long rows = (std::min<long long>(most, UE) + ups - 1) / ups + 1;
+  r.hbytes = (int)std::min<long long>(rows * parts * r.Tp * 128, p.bf16 ? 56 * 1024 : 24 * 1024);
+  r.hbytes = std::max(r.hbytes, parts * r.Tp * 128);
+  const int sb = p.bf16 ? FewTc<false>::stage_bytes(r.Tp) : FewTc<true>::stage_bytes(r.Tp);
+  r.stages = std::min(16, (kFewShared - r.hbytes) / sb);
+  return r;
+}
+
+template <bool FP32, bool GLU>
+static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CUtensorMap& t2, const CUtensorMap& t2u,
+                          const FewTcParams& tp, int grid, cudaStream_t s) {
+  auto kern = few_experts_kernel<FP32, GLU>;
+  static std::atomic<unsigned long long> configured;  // by device
+  const unsigned long long bit = 1ull << current_device();
+  if (!(configured.load() & bit)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewShared + 1024) != cudaSuccess)
+      throw std::runtime_error("moe_few_tokens: shared memory");
+    configured.fetch_or(bit);
+  }
+  const size_t smem = 1024 + (size_t)tp.stages * FewTc<FP32>::stage_bytes(tp.Tp) + tp.hbytes;
+  launch_with_pdl(kern, dim3(grid), dim3(FewTc<FP32>::THREADS), smem, s, true, tx, t1, t2, t2u, tp, serving_status());
+}
+
+void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
+  char* ws = (char*)workspace;
+  float* a = (float*)(ws + plan.zero_bytes + plan.packed_bytes);
+  float* b = (float*)(ws + plan.zero_bytes + plan.packed_bytes + plan.a_bytes);
+  if (!plan.tensor) {
+    if (p.bf16) launch_rows<__nv_bfloat16>(p, a, b, s);
+    else launch_rows<float>(p, a, b, s);
+    return;
+  }
+  const cuuint64_t eb = p.bf16 ? 2 : 4;
+  const cuuint32_t bk = 128 / eb;
+  const int parts = p.bf16 ? 1 : 2;
+  const bool glu = p.act == (int)Act::kSwiGLU;
+  const cuuint64_t D = p.D, F = p.F, O = p.O, E = p.E;
+  // a stride along a single expert or token is never used
+  const cuuint64_t e1 = p.E > 1 ? p.w1_estride * eb : 16, e2 = p.E > 1 ? p.w2_estride * eb : 16;
+  CUtensorMap tx, t1, t2, t2u;
+  {
+    const cuuint64_t dims[2] = {D, plan.pack ? (cuuint64_t)parts * plan.Tp : (cuuint64_t)p.T};
+    const cuuint64_t strides[1] = {plan.pack ? plan.packed_stride * eb : p.T > 1 ? p.x_stride * eb : (D * eb + 15) / 16 * 16};
+    const cuuint32_t box[2] = {bk, (cuuint32_t)(parts * plan.Tp)};
+    tx = make_tmap(plan.pack ? ws + plan.zero_bytes : p.x, p.bf16, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  if (glu) {
+    const cuuint64_t dims[4] = {D, F, 2, E};
+    const cuuint64_t strides[3] = {p.w1_stride * eb, F * p.w1_stride * eb, e1};
+    const cuuint32_t box[4] = {bk, 16, 2, 1};
+    t1 = make_tmap(p.w1, p.bf16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  } else {
+    const cuuint64_t dims[3] = {D, F, E};
+    const cuuint64_t strides[2] = {p.w1_stride * eb, e1};
+    const cuuint32_t box[3] = {bk, 16, 1};
+    t1 = make_tmap(p.w1, p.bf16, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  }
+  {
+    const cuuint64_t dims[3] = {F, O, E};
+    const cuuint64_t strides[2] = {p.w2_stride * eb, e2};
+    const cuuint32_t box[3] = {bk, 128, 1}, unit[3] = {16, 128, 1};
+    t2 = make_tmap(p.w2, p.bf16, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    t2u = make_tmap(p.w2, p.bf16, 3, dims, strides, unit, p.bf16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
+  }
+  FewTcParams tp{};
+  tp.e = p;
+  tp.part = a;
+  tp.y = b;
+  tp.count = (int*)ws;
+  tp.Op = plan.Op;
+  tp.Tp = plan.Tp;
+  tp.stages = plan.stages;
+  tp.hbytes = plan.hbytes;
+  if (p.bf16) {
+    if (glu) launch_tensor<false, true>(tx, t1, t2, t2u, tp, plan.grid, s);
+    else launch_tensor<false, false>(tx, t1, t2, t2u, tp, plan.grid, s);
+  } else {
+    if (glu) launch_tensor<true, true>(tx, t1, t2, t2u, tp, plan.grid, s);
+    else launch_tensor<true, false>(tx, t1, t2, t2u, tp, plan.grid, s);
+  }
 }
 
 }  // namespace raiccl

@@ -169,9 +169,6 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   r.vec = (D * eb) % 16 == 0 && rows16(x) && rows16(router_w);
   r.ids = ids.data_ptr<int>();
   r.gates = gates.data_ptr<float>();
-  raiccl::launch_few_route(r, stream);
-
-  torch::Tensor ws = torch::empty({T * top_k * (F + O)}, x.options().dtype(torch::kFloat32));
   raiccl::FewExpertParams e{};
   e.x = x.data_ptr();
   e.x_stride = x.stride(0);
@@ -189,8 +186,6 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   e.out_stride = res.stride(0);
   e.ids = r.ids;
   e.gates = r.gates;
-  e.h = ws.data_ptr<float>();
-  e.y = e.h + T * top_k * F;
   e.T = r.T;
   e.D = r.D;
   e.E = r.E;
@@ -201,7 +196,16 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   e.bf16 = bf16;
   e.out_bf16 = res.scalar_type() == torch::kBFloat16;
   e.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
-  raiccl::launch_few_experts(e, stream);
+  const raiccl::FewExpertPlan plan = raiccl::plan_few_experts(e);
+  torch::Tensor ws = torch::empty({plan.bytes()}, x.options().dtype(torch::kUInt8));
+  char* base = (char*)ws.data_ptr();
+  r.zero = (int*)base;
+  r.n_zero = plan.n_zero;
+  r.packed = plan.pack ? base + plan.zero_bytes : nullptr;
+  r.packed_stride = plan.packed_stride;
+  r.packed_rows = plan.Tp;
+  raiccl::launch_few_route(r, stream);
+  raiccl::launch_few_experts(e, plan, base, stream);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {res, ids, gates};
 }
