@@ -12,11 +12,12 @@
 // keeps them in shared memory, and multiplies them by its columns of W2: no
 // CTA waits for another between the two products, and every CTA has the same
 // number of weights to read.  What remains is a sum over the CTAs of an expert
-// and over the experts of a token.  Each CTA writes its part of the expert's
-// result; for each 128 columns, the expert's last CTA to arrive adds the parts
-// in CTA order, and the layer's last expert to arrive adds the experts in the
-// order of the token's choices, applies the gates and adds the residual.  The
-// order of the additions never depends on the order of arrival, and nobody waits.
+// and over the experts of a token: each CTA writes its part of the expert's
+// result, and a third, small kernel adds a token's parts in a fixed order (by
+// choice, then CTA), applies the gates and adds the residual.  Adding them in
+// this kernel by the last CTA to arrive was tried first: a fence and an atomic
+// round trip for each 128 columns made the epilogue, not memory, set the pace
+// (64 experts, 1 token: 149 us).
 //
 // Steps of a CTA's range (roles: one TMA thread, one MMA thread, four epilogue
 // warps; fp32 also four splitting warps), for each expert in it:
@@ -46,8 +47,7 @@ constexpr int kFewKernelId = 600;
 struct FewTcParams {
   FewExpertParams e;
   float* part;        // [rows, Op] the CTAs' parts of the experts' results
-  float* y;           // [T k, Op] the experts' results, by expert, then token
-  int* count;         // [min(E, T k) + 1][nO] arrivals, zeroed by the routing kernel
+  int4* terms;        // [T, k] a choice's first row in part, rows to the next part, parts; expert
   int Op;             // O rounded up to 128
   int Tp;             // T rounded up to 16
   int stages;
@@ -83,15 +83,15 @@ struct FewPlan {
   int used[kFewExperts + 1];                 // the chosen experts, by number
   int index[kFewExperts + 1];                // their place in used, by expert
   int part0[kFewExperts + 1];                // by place: first row in part
-  int y0[kFewExperts + 1];                   // by place: first row in y
-  int yrow[kFewTokens * kFewTopK];           // by (token, choice): row in y, -1 without an expert
+  int parts[kFewExperts + 1];                // by place: CTAs with a part
   int ne;
 };
 
 // CTA of unit u where U units are dealt to G <= U CTAs: CTA c has units [U c / G, U (c + 1) / G).
 __device__ __forceinline__ int few_cta(long long u, long long U, int G) { return (int)(((u + 1) * G - 1) / U); }
 
-__device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, int UE, int grid) {
+__device__ __forceinline__ void few_plan(const FewTcParams& tp, FewPlan& s, int UE, int grid) {
+  const FewExpertParams& p = tp.e;
   const int pairs = p.T * p.k;
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) s.mask[e] = 0ull;
   __syncthreads();
@@ -116,32 +116,37 @@ __device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, i
     __syncwarp();
     const long long U = (long long)ne * UE;
     const int G = U < grid ? (int)U : grid;
-    int part = 0, y = 0;
+    int part = 0;
     for (int i0 = 0; i0 < ne; i0 += 32) {
       const int i = i0 + lane;
-      int t = 0, rows = 0;
+      int n = 0, rows = 0;
       if (i < ne) {
-        t = __popcll(s.mask[s.used[i]]);
-        rows = t * (few_cta((long long)(i + 1) * UE - 1, U, G) - few_cta((long long)i * UE, U, G) + 1);
+        n = few_cta((long long)(i + 1) * UE - 1, U, G) - few_cta((long long)i * UE, U, G) + 1;
+        rows = n * __popcll(s.mask[s.used[i]]);
       }
-      int ts = t, rs = rows;
+      int rs = rows;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, ts, o), b = __shfl_up_sync(0xffffffffu, rs, o);
-        if (lane >= o) { ts += a; rs += b; }
+        const int a = __shfl_up_sync(0xffffffffu, rs, o);
+        if (lane >= o) rs += a;
       }
-      if (i < ne) { s.y0[i] = y + ts - t; s.part0[i] = part + rs - rows; }
-      y += __shfl_sync(0xffffffffu, ts, 31);
+      if (i < ne) { s.part0[i] = part + rs - rows; s.parts[i] = n; }
       part += __shfl_sync(0xffffffffu, rs, 31);
     }
     if (lane == 0) s.ne = ne;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-    const int e = __ldcg(p.ids + i);
-    s.yrow[i] = e < 0 ? -1 : s.y0[s.index[e]] + __popcll(s.mask[e] & ((1ull << (i / p.k)) - 1ull));
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+      const int e = __ldcg(p.ids + i);
+      int4 t = make_int4(0, 0, 0, 0);
+      if (e >= 0) {
+        const unsigned long long m = s.mask[e];
+        t = make_int4(s.part0[s.index[e]] + __popcll(m & ((1ull << (i / p.k)) - 1ull)), __popcll(m), s.parts[s.index[e]], e);
+      }
+      tp.terms[i] = t;
+    }
   }
-  __syncthreads();
 }
 
 // A run of units of one expert whose activations fit in shared memory; the
@@ -149,7 +154,7 @@ __device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, i
 struct FewRun {
   int place, expert, tokens, np;   // place in used, expert, its tokens, their number rounded up to 16
   int f0, units;                   // first hidden row, units of 16
-  bool first, last;                // of the CTA's runs of this expert
+  bool first;                      // of the CTA's runs of this expert
 };
 
 struct FewWalk {
@@ -182,94 +187,52 @@ struct FewWalk {
     r.f0 = (a + s) * 16;
     r.first = s == 0;
     s += r.units;
-    r.last = s >= n;
     return true;
   }
 };
 
-// Adds the parts of expert `place` for 128 columns, in CTA order, plus the
-// bias, into y.  The four epilogue warps; each thread has four columns.
-__device__ __forceinline__ void few_join_parts(const FewTcParams& p, const FewPlan& s, int place, int expert, int tokens,
-                                               int n, int o0, float (*red)[128]) {
-  const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  const int o = o0 + lane * 4;
-  const float4* src = (const float4*)(p.part + (long long)s.part0[place] * p.Op + o);
-  float4* dst = (float4*)(p.y + (long long)s.y0[place] * p.Op + o);
-  const long long row = p.Op / 4, step = row * tokens;
-  float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (p.e.b2) {
-    const float* b2 = p.e.b2 + (long long)expert * p.e.O;
-    b.x = o < p.e.O ? b2[o] : 0.f;
-    b.y = o + 1 < p.e.O ? b2[o + 1] : 0.f;
-    b.z = o + 2 < p.e.O ? b2[o + 2] : 0.f;
-    b.w = o + 3 < p.e.O ? b2[o + 3] : 0.f;
-  }
-  if (tokens >= 4) {  // a token per warp
-    for (int t = w; t < tokens; t += 4) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int c = 0; c < n; ++c) {
-        const float4 a = __ldcg(src + t * row + c * step);
-        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-      }
-      dst[t * row] = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
-    }
-  } else {            // few tokens, many parts: a quarter of the parts per warp
-    for (int t = 0; t < tokens; ++t) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int c = w; c < n; c += 4) {
-        const float4 a = __ldcg(src + t * row + c * step);
-        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-      }
-      *(float4*)&red[w][lane * 4] = v;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (w == 0) {
-#pragma unroll
-        for (int q = 1; q < 4; ++q) {
-          const float4 a = *(const float4*)&red[q][lane * 4];
-          v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-        }
-        dst[t * row] = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
-      }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-    }
-  }
-}
+// out[t, o0 .. o0 + 128) of one token: its parts by choice, then CTA, dealt to
+// the eight warps in turn, each times its choice's gate; the warps' sums are
+// added in order.  A few hundred loads in all, so that many in flight count.
+constexpr int kFewJoinThreads = 256;
 
-// The tokens' results for 128 columns: their experts in the order of choice, gates, residual.
-__device__ __forceinline__ void few_join_experts(const FewTcParams& p, const FewPlan& s, int o0) {
-  const int w = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
-  const int o = o0 + lane * 4;
+__global__ void __launch_bounds__(kFewJoinThreads) few_join_parts_kernel(FewTcParams p) {
+  constexpr int W = kFewJoinThreads / 32;
+  __shared__ __align__(16) float red[W][128];
   const FewExpertParams& e = p.e;
-  for (int t = w; t < e.T; t += 4) {
-    float4 a[kFewTopK];
-    float g[kFewTopK];
-#pragma unroll
-    for (int j = 0; j < kFewTopK; ++j) {
-      const int row = j < e.k ? s.yrow[t * e.k + j] : -1;
-      g[j] = 0.f;
-      a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row >= 0) {
-        g[j] = __ldcg(e.gates + t * e.k + j);
-        a[j] = __ldcg((const float4*)(p.y + (long long)row * p.Op + o));
-      }
+  const int t = blockIdx.y, o0 = blockIdx.x * 128;
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float* col = p.part + o0 + lane * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float bias = 0.f;
+  griddep_wait();
+  int at = w;   // this warp's next item of the choice
+  for (int j = 0; j < e.k; ++j) {
+    const int4 term = __ldcg(p.terms + t * e.k + j);
+    if (term.z == 0) continue;
+    const float g = __ldcg(e.gates + t * e.k + j);
+    if (e.b2 && threadIdx.x < 128 && o0 + threadIdx.x < e.O)
+      bias = fmaf(g, __ldg(e.b2 + (long long)term.w * e.O + o0 + threadIdx.x), bias);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    int c = at;
+#pragma unroll 8
+    for (; c < term.z; c += W) {
+      const float4 a = __ldcg((const float4*)(col + ((long long)term.x + (long long)c * term.y) * p.Op));
+      s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
     }
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < kFewTopK; ++j) {
-      v[0] = fmaf(g[j], a[j].x, v[0]);
-      v[1] = fmaf(g[j], a[j].y, v[1]);
-      v[2] = fmaf(g[j], a[j].z, v[2]);
-      v[3] = fmaf(g[j], a[j].w, v[3]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (o + i >= e.O) break;
-      if (e.residual) v[i] += load_elem(e.residual, (long long)t * e.res_stride + o + i, e.res_bf16);
-      store_elem(e.out, (long long)t * e.out_stride + o + i, v[i], e.out_bf16);
-    }
+    at = c - term.z;
+    v.x = fmaf(g, s.x, v.x); v.y = fmaf(g, s.y, v.y); v.z = fmaf(g, s.z, v.z); v.w = fmaf(g, s.w, v.w);
   }
+  *(float4*)&red[w][lane * 4] = v;
+  __syncthreads();
+  const int o = o0 + threadIdx.x;
+  if (threadIdx.x >= 128 || o >= e.O) return;
+  float out = red[0][threadIdx.x];
+#pragma unroll
+  for (int i = 1; i < W; ++i) out += red[i][threadIdx.x];
+  out += bias;
+  if (e.residual) out += load_elem(e.residual, (long long)t * e.res_stride + o, e.res_bf16);
+  store_elem(e.out, (long long)t * e.out_stride + o, out, e.out_bf16);
 }
 
 // Maps: x [T, D] in boxes of 128 bytes x Tp rows (fp32: [2 Tp, D] parts, 2 Tp
@@ -286,8 +249,6 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   __shared__ FewPlan plan;
   __shared__ uint64_t full[16], empty[16], parted[16], acc1_full[2], acc1_empty[2], acc2_full[2], acc2_empty[2], drained;
   __shared__ uint32_t tmem_slot;
-  __shared__ int arrived;
-  __shared__ __align__(16) float red[4][128];
   const int SB = C::stage_bytes(p.Tp), S = p.stages;
   uint8_t* const hbuf = smem + S * SB;
   const FewExpertParams& e = p.e;
@@ -309,7 +270,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   tc_fence_before_sync();
   griddep_wait();
   const int UE = (e.F + 15) / 16;
-  few_plan(e, plan, UE, gridDim.x);   // holds __syncthreads
+  few_plan(p, plan, UE, gridDim.x);   // holds __syncthreads
   griddep_launch_dependents();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
@@ -317,7 +278,6 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   const int nO = p.Op / 128;
   const int TU = GLU ? 4 : 8;                           // units of a product-1 tile
   const int hrows = p.hbytes / 128;
-  const int rot = (int)(((long long)blockIdx.x * nO) / gridDim.x);  // so that the last arrivals of a column are spread
   FewWalk walk;
   walk.start(plan, UE, gridDim.x);
   FewRun r;
@@ -347,7 +307,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         }
         const int slices = r.units / C::UPS, tail = r.units % C::UPS;
         for (int i = 0; ok && i < nO; ++i) {
-          const int o = (i + rot) % nO * 128;
+          const int o = i * 128;
           for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
             if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             uint8_t* w = smem + stage * SB;
@@ -445,14 +405,12 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
     const int q = warp & 3;                               // TMEM lanes 32 q .. 32 q + 31
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16);
     int i1 = 0, i2 = 0;
-    // A wait that runs out is carried to the next vote: the four warps share
-    // named barriers, so they only leave together.
-    bool ok = true, alive = true;
-    while (alive && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
+    bool ok = true;
+    while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
       const unsigned long long mask = plan.mask[r.expert];
       const float* b1 = e.b1 ? e.b1 + (long long)r.expert * (GLU ? 2 : 1) * e.F : nullptr;
       const uint32_t hrow = C::PARTS * r.np * 128;
-      for (int u0 = 0; u0 < r.units; u0 += TU, ++i1) {
+      for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
         const int b = i1 & 1;
         const int unit = u0 + (GLU ? q : 2 * q + (lane >> 4));  // of the run
         const int fl = unit * 16 + (lane & 15);           // hidden row of the run
@@ -463,7 +421,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           bias = __ldg(b1 + f);
           if constexpr (GLU) bias_up = __ldg(b1 + e.F + f);
         }
-        ok = mbar_wait_bounded(&acc1_full[b], (i1 >> 1) & 1, status, kFewKernelId, kFewWaitNs) && ok;
+        ok = mbar_wait_bounded(&acc1_full[b], (i1 >> 1) & 1, status, kFewKernelId, kFewWaitNs);
         tc_fence_after_sync();
         const uint32_t base = lane_addr + b * n1;
         uint8_t* hcol = hbuf + (fl / C::BK) * hrow;
@@ -519,18 +477,12 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc1_empty[b]);
       }
-      // product 2: this CTA's part of the expert's result, or the result where no other CTA has a part
-      const int first = few_cta((long long)r.place * UE, walk.U, walk.G);
-      const int n = few_cta((long long)(r.place + 1) * UE - 1, walk.U, walk.G) - first + 1;
-      const bool alone = n == 1;
-      float* dst = alone ? p.y + (long long)plan.y0[r.place] * p.Op
-                         : p.part + (long long)(plan.part0[r.place] + ((int)blockIdx.x - first) * r.tokens) * p.Op;
-      for (int i = 0; i < nO; ++i, ++i2) {
+      // product 2: this CTA's part of the expert's result
+      const int mine = (int)blockIdx.x - few_cta((long long)r.place * UE, walk.U, walk.G);
+      float* dst = p.part + (long long)(plan.part0[r.place] + mine * r.tokens) * p.Op + q * 32 + lane;
+      for (int i = 0; ok && i < nO; ++i, ++i2) {
         const int b = i2 & 1;
-        const int ot = (i + rot) % nO, o = ot * 128 + q * 32 + lane;
-        float bias = 0.f;
-        if (alone && r.first && e.b2 && o < e.O) bias = __ldg(e.b2 + (long long)r.expert * e.O + o);
-        ok = mbar_wait_bounded(&acc2_full[b], (i2 >> 1) & 1, status, kFewKernelId, kFewWaitNs) && ok;
+        ok = mbar_wait_bounded(&acc2_full[b], (i2 >> 1) & 1, status, kFewKernelId, kFewWaitNs);
         tc_fence_after_sync();
         const uint32_t base = lane_addr + 2 * n1 + b * n1;
         for (int c = 0; c < r.tokens; c += 16) {
@@ -548,8 +500,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             if (c + j >= r.tokens) break;
-            float* at = dst + (long long)(c + j) * p.Op + o;
-            float out = __uint_as_float(v[j]) + bias;
+            float* at = dst + (long long)(c + j) * p.Op + i * 128;
+            float out = __uint_as_float(v[j]);
             if (!r.first) out += *at;   // written by this thread
             *at = out;
           }
@@ -557,41 +509,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive(&acc2_empty[b]);
-        if (!r.last) continue;
-        // arrivals: the expert's parts, then the layer's experts
-        __threadfence();
-        int go;
-        asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.s32 a, %1, 0;\n\tbar.red.and.pred b, 1, 128, a;\n\tselp.s32 %0, 1, 0, b;\n\t}"
-                     : "=r"(go) : "r"((int)ok) : "memory");
-        alive = go != 0;
-        if (!alive) break;
-        bool join = alone;
-        if (!alone) {
-          if (warp == 2 && lane == 0) arrived = atom_add_acq_rel_gpu(p.count + (long long)(1 + r.place) * nO + ot, 1);
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          join = arrived == n - 1;
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (join) {
-            __threadfence();
-            few_join_parts(p, plan, r.place, r.expert, r.tokens, n, ot * 128, red);
-            __threadfence();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-          }
-        }
-        if (join) {
-          if (warp == 2 && lane == 0) arrived = atom_add_acq_rel_gpu(p.count + ot, 1);
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          const bool whole = arrived == plan.ne - 1;
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (whole) {
-            __threadfence();
-            few_join_experts(p, plan, ot * 128);
-          }
-        }
       }
     }
-    if (plan.ne == 0)   // no token has an expert: the residual, or zeros
-      for (int ot = blockIdx.x; ot < nO; ot += gridDim.x) few_join_experts(p, plan, ot * 128);
   } else if constexpr (FP32) {
     // ---------------------------------------------------------------- weights into tf32 parts
     const int tid = threadIdx.x - 192;

@@ -32,8 +32,6 @@ struct FewRouteParams {
   int vec;                // rows of x and w are 16-byte aligned multiples of 16 bytes
   int* ids;               // [T, k], -1 where no expert was left
   float* gates;           // [T, k], 0 there
-  int* zero;              // zeroed for the experts' kernel
-  int n_zero;
   void* packed;           // x for the experts' kernel, or nullptr: bf16 rows [T, packed_stride] as they are;
   long long packed_stride;  // fp32 [2][packed_rows, packed_stride] as two tf32 parts
   int packed_rows;
@@ -66,9 +64,8 @@ struct FewExpertPlan {
   int grid, stages, hbytes, Op, Tp;
   int pack;               // x is packed by the routing kernel
   int packed_stride;
-  int n_zero;             // ints zeroed by the routing kernel
-  long long zero_bytes, packed_bytes, a_bytes, b_bytes;  // multiples of 256; in this order in the workspace
-  long long bytes() const { return zero_bytes + packed_bytes + a_bytes + b_bytes; }
+  long long packed_bytes, a_bytes, b_bytes;  // multiples of 256; in this order in the workspace
+  long long bytes() const { return packed_bytes + a_bytes + b_bytes; }
 };
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p);

@@ -96,7 +96,6 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams
   griddep_wait();
   griddep_launch_dependents();
   const int share = rank * kRouteThreads + threadIdx.x, shares = ranks * kRouteThreads;
-  for (int i = t * shares + share; i < p.n_zero; i += p.T * shares) p.zero[i] = 0;
   if (p.packed) {
     for (int d = share; d < p.D; d += shares) {
       if constexpr (sizeof(T) == 4) {
@@ -324,16 +323,14 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   r.grid = sm_count();
   r.Op = (p.O + 127) / 128 * 128;
   r.Tp = (p.T + 15) / 16 * 16;
-  const int nO = r.Op / 128, UE = (p.F + 15) / 16, ups = 128 / eb / 16;
-  r.n_zero = (1 + std::min(p.E, pairs)) * nO;
-  r.zero_bytes = up256(4ll * r.n_zero);
+  const int UE = (p.F + 15) / 16, ups = 128 / eb / 16;
   r.pack = !p.bf16 || !aligned(p.x, p.T > 1 ? p.x_stride : 0, 0);
   r.packed_stride = (p.D + 7) / 8 * 8;
   if (r.pack) r.packed_bytes = up256((long long)parts * r.Tp * r.packed_stride * eb);
   // An expert's tokens times the CTAs that share it, over all experts: n experts have at most min(T k, n T) tokens
   // and (grid / n + 2) CTAs each, so T (grid + 2 k) rows at most, whatever n is.
   r.a_bytes = up256((long long)p.T * (r.grid + 2 * p.k) * r.Op * 4);
-  r.b_bytes = up256((long long)pairs * r.Op * 4);
+  r.b_bytes = up256(16ll * pairs);
   // activations: what the longest range of a CTA needs, at most a quarter of shared memory; the rest holds stages
   const long long most = ((long long)std::min(p.E, pairs) * UE + r.grid - 1) / r.grid;
   const long long rows = (std::min<long long>(most, UE) + ups - 1) / ups + 1;
@@ -361,8 +358,8 @@ static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CU
 
 void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
   char* ws = (char*)workspace;
-  float* a = (float*)(ws + plan.zero_bytes + plan.packed_bytes);
-  float* b = (float*)(ws + plan.zero_bytes + plan.packed_bytes + plan.a_bytes);
+  float* a = (float*)(ws + plan.packed_bytes);
+  float* b = (float*)(ws + plan.packed_bytes + plan.a_bytes);
   if (!plan.tensor) {
     if (p.bf16) launch_rows<__nv_bfloat16>(p, a, b, s);
     else launch_rows<float>(p, a, b, s);
@@ -380,7 +377,7 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
     const cuuint64_t dims[2] = {D, plan.pack ? (cuuint64_t)parts * plan.Tp : (cuuint64_t)p.T};
     const cuuint64_t strides[1] = {plan.pack ? plan.packed_stride * eb : p.T > 1 ? p.x_stride * eb : (D * eb + 15) / 16 * 16};
     const cuuint32_t box[2] = {bk, (cuuint32_t)(parts * plan.Tp)};
-    tx = make_tmap(plan.pack ? ws + plan.zero_bytes : p.x, p.bf16, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    tx = make_tmap(plan.pack ? ws : p.x, p.bf16, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   }
   if (glu) {
     const cuuint64_t dims[4] = {D, F, 2, E};
@@ -403,8 +400,7 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
   FewTcParams tp{};
   tp.e = p;
   tp.part = a;
-  tp.y = b;
-  tp.count = (int*)ws;
+  tp.terms = (int4*)b;
   tp.Op = plan.Op;
   tp.Tp = plan.Tp;
   tp.stages = plan.stages;
@@ -416,6 +412,7 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
     if (glu) launch_tensor<true, true>(tx, t1, t2, t2u, tp, plan.grid, s);
     else launch_tensor<true, false>(tx, t1, t2, t2u, tp, plan.grid, s);
   }
+  launch_with_pdl(few_join_parts_kernel, dim3(plan.Op / 128, p.T), dim3(kFewJoinThreads), 0, s, true, tp);
 }
 
 }  // namespace raiccl

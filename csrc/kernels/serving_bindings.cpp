@@ -199,9 +199,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   const raiccl::FewExpertPlan plan = raiccl::plan_few_experts(e);
   torch::Tensor ws = torch::empty({plan.bytes()}, x.options().dtype(torch::kUInt8));
   char* base = (char*)ws.data_ptr();
-  r.zero = (int*)base;
-  r.n_zero = plan.n_zero;
-  r.packed = plan.pack ? base + plan.zero_bytes : nullptr;
+  r.packed = plan.pack ? base : nullptr;
   r.packed_stride = plan.packed_stride;
   r.packed_rows = plan.Tp;
   raiccl::launch_few_route(r, stream);
