@@ -19,8 +19,11 @@
 // round trip for each 128 columns made the epilogue, not memory, set the pace
 // (64 experts, 1 token: 149 us).
 //
-// Steps of a CTA's range (roles: one TMA thread, one MMA thread, four epilogue
-// warps; fp32 also four splitting warps), for each expert in it:
+// Steps of a CTA's range (roles: one TMA thread, one MMA thread, two groups of
+// four epilogue warps that take tiles in turn; fp32 also eight splitting
+// warps).  The range is worked off in batches of runs, each of one expert,
+// whose activations fit in shared memory together: first product 1 of all its
+// runs, then product 2 of all, so that the wait for the activations comes once:
 //   product 1   tiles of 128 rows of W1 (64 gate + 64 up rows, 16 by 16), K = D
 //               in 128-byte steps, against all T tokens; the epilogue applies
 //               bias and activation and keeps the expert's own tokens, rounded
@@ -40,6 +43,8 @@
 namespace raiccl {
 
 constexpr int kFewTile = 128 * 128;           // bytes of a weight tile: 128 rows of 128 bytes
+constexpr int kFewSlack = 12 * 1024;          // behind the last tile: rows that an instruction reads past a short one
+constexpr int kFewMaxStages = 12;
 constexpr unsigned long long kFewWaitNs = 2000000000ull;
 constexpr int kFewKernelId = 600;
 
@@ -51,6 +56,7 @@ struct FewTcParams {
   int Op;             // O rounded up to 128
   int Tp;             // T rounded up to 16
   int stages;
+  int wide;           // whole tiles of W1 in one copy
   int hbytes;         // shared memory of the activations
 };
 
@@ -61,9 +67,12 @@ struct FewTc {
   static constexpr int PARTS = FP32 ? 2 : 1;
   static constexpr int UPS = BK / 16;              // units of 16 hidden rows in a 128-byte row of activations
   static constexpr int TAIL = 16 * EB;             // bytes of one unit in a row
-  static constexpr int THREADS = FP32 ? 320 : 192;
-  static constexpr uint32_t FORMAT = FP32 ? 2u : 1u;
-  static __host__ __device__ int stage_bytes(int Tp) { return PARTS * kFewTile + PARTS * Tp * 128; }
+  static constexpr int THREADS = FP32 ? 576 : 320;
+  static constexpr int SPLITTERS = 256;
+  // K steps of 128 bytes that share a stage where a tile has few rows: a step
+  // costs its waits and its commit, 0.2 us, whatever it holds
+  static __host__ __device__ int packs(int Tp) { const int n = (FP32 ? 128 : 64) / (PARTS * Tp); return n > 4 ? 4 : n < 1 ? 1 : n; }
+  static __host__ __device__ int stage_bytes(int Tp) { return PARTS * kFewTile + packs(Tp) * PARTS * Tp * 128; }
 };
 
 // fp32 as two tf32 numbers of 11 significant bits, rounded to nearest; what
@@ -77,7 +86,7 @@ __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
   lo = l != l ? l : __uint_as_float((__float_as_uint(l) + 0x1000u) & ~0x1fffu);
 }
 
-// The plan that every CTA makes of the routed tokens.
+// The plan that every CTA makes of the routed tokens; mask is zero on entry.
 struct FewPlan {
   unsigned long long mask[kFewExperts + 1];  // by expert: its tokens
   int used[kFewExperts + 1];                 // the chosen experts, by number
@@ -93,8 +102,6 @@ __device__ __forceinline__ int few_cta(long long u, long long U, int G) { return
 __device__ __forceinline__ void few_plan(const FewTcParams& tp, FewPlan& s, int UE, int grid) {
   const FewExpertParams& p = tp.e;
   const int pairs = p.T * p.k;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) s.mask[e] = 0ull;
-  __syncthreads();
   for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
     const int e = __ldcg(p.ids + i);
     if (e >= 0) atomicOr(&s.mask[e], 1ull << (i / p.k));
@@ -149,17 +156,17 @@ __device__ __forceinline__ void few_plan(const FewTcParams& tp, FewPlan& s, int 
   }
 }
 
-// A run of units of one expert whose activations fit in shared memory; the
-// roles walk the same runs.
+// A run of units of one expert; the roles walk the same runs.
 struct FewRun {
   int place, expert, tokens, np;   // place in used, expert, its tokens, their number rounded up to 16
   int f0, units;                   // first hidden row, units of 16
+  int h;                           // its activations' first 128-byte row in shared memory
   bool first;                      // of the CTA's runs of this expert
 };
 
 struct FewWalk {
   long long u, u1, U;
-  int UE, G, cap, s, n, a, place;  // cap: 128-byte rows of activations that fit, over all tokens' rows
+  int UE, G, s, n, a, place;
   __device__ void start(const FewPlan& plan, int UE_, int grid) {
     UE = UE_;
     U = (long long)plan.ne * UE;
@@ -167,107 +174,161 @@ struct FewWalk {
     const int c = blockIdx.x;
     u = c < G ? U * c / G : 0;
     u1 = c < G ? U * (c + 1) / G : 0;
-    s = n = 0;
+    s = n = a = place = 0;
   }
-  __device__ bool next(const FewPlan& plan, int hrows, int parts, int ups, FewRun& r) {
+  // The next run of a batch that has used `off` of the hrows rows of activations so far; false at its end.
+  // Only a batch's first run may be cut to fit, and it is then the only one.
+  __device__ bool next(const FewPlan& plan, int hrows, int parts, int ups, int& off, FewRun& r) {
     if (s >= n) {
       if (u >= u1) return false;
-      place = (int)(u / UE);
-      a = (int)(u - (long long)place * UE);
-      n = (int)(u1 - u < UE - a ? u1 - u : UE - a);
-      u += n;
+      const int pl = (int)(u / UE), first = (int)(u - (long long)pl * UE);
+      const int count = (int)(u1 - u < UE - first ? u1 - u : UE - first);
+      const int np = (__popcll(plan.mask[plan.used[pl]]) + 15) & ~15;
+      if (off > 0 && off + (count + ups - 1) / ups * np * parts > hrows) return false;
+      place = pl;
+      a = first;
+      n = count;
       s = 0;
+      u += n;
+    } else if (off > 0) {
+      return false;
     }
     r.place = place;
     r.expert = plan.used[place];
     r.tokens = __popcll(plan.mask[r.expert]);
     r.np = (r.tokens + 15) & ~15;
-    const int cap = hrows / (r.np * parts) * ups;
+    const int cap = (hrows - off) / (r.np * parts) * ups;
     r.units = n - s < cap ? n - s : cap;
     r.f0 = (a + s) * 16;
+    r.h = off;
     r.first = s == 0;
+    off += (r.units + ups - 1) / ups * r.np * parts;
     s += r.units;
     return true;
   }
 };
 
-// out[t, o0 .. o0 + 128) of one token: its parts by choice, then CTA, dealt to
-// the eight warps in turn, each times its choice's gate; the warps' sums are
-// added in order.  A few hundred loads in all, so that many in flight count.
+// Accumulators in TMEM, n1 columns each, for two epilogue groups: nA buffers
+// of product 1 and nB of product 2 per group.
+struct FewAcc {
+  int n1, nA, nB;
+  __device__ FewAcc(int n1_) : n1(n1_) {
+    const int per = 512 / (2 * n1);
+    nA = per >= 4 ? 2 : 1;
+    nB = per - nA < 1 ? 1 : per - nA > 6 ? 6 : per - nA;
+  }
+  __device__ uint32_t first(int g, int b) const { return (g * nA + b) * n1; }
+  __device__ uint32_t second(int g, int b) const { return ((2 * nA) + g * nB + b) * n1; }
+  __device__ int columns() const {
+    const int c = 2 * (nA + nB) * n1;
+    return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512;
+  }
+};
+
+// out[t, o0 .. o0 + 128) of one token: the parts of all its choices, by choice,
+// then CTA, are dealt to the eight warps in turn, each times its choice's
+// gate; the warps' sums are added in order.  A few hundred loads in all, so
+// what counts is how many are in flight.
 constexpr int kFewJoinThreads = 256;
 
 __global__ void __launch_bounds__(kFewJoinThreads) few_join_parts_kernel(FewTcParams p) {
-  constexpr int W = kFewJoinThreads / 32;
+  constexpr int W = kFewJoinThreads / 32, U = 8;
   __shared__ __align__(16) float red[W][128];
   const FewExpertParams& e = p.e;
   const int t = blockIdx.y, o0 = blockIdx.x * 128;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* col = p.part + o0 + lane * 4;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  float bias = 0.f;
+  const int o = o0 + threadIdx.x;
+  const bool writes = threadIdx.x < 128 && o < e.O;
   griddep_wait();
-  int at = w;   // this warp's next item of the choice
-  for (int j = 0; j < e.k; ++j) {
-    const int4 term = __ldcg(p.terms + t * e.k + j);
-    if (term.z == 0) continue;
-    const float g = __ldcg(e.gates + t * e.k + j);
-    if (e.b2 && threadIdx.x < 128 && o0 + threadIdx.x < e.O)
-      bias = fmaf(g, __ldg(e.b2 + (long long)term.w * e.O + o0 + threadIdx.x), bias);
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    int c = at;
-#pragma unroll 8
-    for (; c < term.z; c += W) {
-      const float4 a = __ldcg((const float4*)(col + ((long long)term.x + (long long)c * term.y) * p.Op));
-      s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
+  griddep_launch_dependents();
+  float res = 0.f;
+  if (writes && e.residual) res = load_elem(e.residual, (long long)t * e.res_stride + o, e.res_bf16);
+  int4 term[kFewTopK];
+  float gate[kFewTopK];
+#pragma unroll
+  for (int j = 0; j < kFewTopK; ++j) {
+    term[j] = j < e.k ? __ldcg(p.terms + t * e.k + j) : make_int4(0, 0, 0, 0);
+    gate[j] = j < e.k ? __ldcg(e.gates + t * e.k + j) : 0.f;
+  }
+  int items = 0;
+  float bias = 0.f;
+#pragma unroll
+  for (int j = 0; j < kFewTopK; ++j) {
+    items += term[j].z;
+    if (e.b2 && writes && term[j].z > 0) bias = fmaf(gate[j], __ldg(e.b2 + (long long)term[j].w * e.O + o), bias);
+  }
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = w; i0 < items; i0 += W * U) {
+    float4 a[U];
+    float g[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      int c = i0 + i * W;
+      const float4* at = nullptr;
+      g[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kFewTopK; ++j) {
+        if (c >= 0 && c < term[j].z) {
+          at = (const float4*)(col + ((long long)term[j].x + (long long)c * term[j].y) * p.Op);
+          g[i] = gate[j];
+        }
+        c = c < term[j].z ? -1 : c - term[j].z;
+        c = c < 0 ? -1 : c;
+      }
+      a[i] = at ? __ldcg(at) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    at = c - term.z;
-    v.x = fmaf(g, s.x, v.x); v.y = fmaf(g, s.y, v.y); v.z = fmaf(g, s.z, v.z); v.w = fmaf(g, s.w, v.w);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      v.x = fmaf(g[i], a[i].x, v.x);
+      v.y = fmaf(g[i], a[i].y, v.y);
+      v.z = fmaf(g[i], a[i].z, v.z);
+      v.w = fmaf(g[i], a[i].w, v.w);
+    }
   }
   *(float4*)&red[w][lane * 4] = v;
   __syncthreads();
-  const int o = o0 + threadIdx.x;
-  if (threadIdx.x >= 128 || o >= e.O) return;
+  if (!writes) return;
   float out = red[0][threadIdx.x];
 #pragma unroll
   for (int i = 1; i < W; ++i) out += red[i][threadIdx.x];
-  out += bias;
-  if (e.residual) out += load_elem(e.residual, (long long)t * e.res_stride + o, e.res_bf16);
-  store_elem(e.out, (long long)t * e.out_stride + o, out, e.out_bf16);
+  store_elem(e.out, (long long)t * e.out_stride + o, out + bias + res, e.out_bf16);
 }
 
 // Maps: x [T, D] in boxes of 128 bytes x Tp rows (fp32: [2 Tp, D] parts, 2 Tp
-// rows); W1 in boxes of 128 bytes x 16 rows (SwiGLU: x 2, gate and up); W2 in
-// boxes of 128 bytes x 128 rows and of one unit x 128 rows.
+// rows); W1 in boxes of 128 bytes x 16 rows (SwiGLU: x 2, gate and up) and of a
+// whole tile; W2 in boxes of 128 bytes x 128 rows and of one unit x 128 rows.
 template <bool FP32, bool GLU>
 __global__ void __launch_bounds__(FewTc<FP32>::THREADS, 1)
 few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap t1,
-                   const __grid_constant__ CUtensorMap t2, const __grid_constant__ CUtensorMap t2u, FewTcParams p,
-                   DeviceStatus* status) {
+                   const __grid_constant__ CUtensorMap t1w, const __grid_constant__ CUtensorMap t2,
+                   const __grid_constant__ CUtensorMap t2u, FewTcParams p, DeviceStatus* status) {
   using C = FewTc<FP32>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ FewPlan plan;
-  __shared__ uint64_t full[16], empty[16], parted[16], acc1_full[2], acc1_empty[2], acc2_full[2], acc2_empty[2], drained;
+  __shared__ uint64_t full[kFewMaxStages], empty[kFewMaxStages], parted[kFewMaxStages];
+  __shared__ uint64_t acc1_full[4], acc1_empty[4], acc2_full[12], acc2_empty[12], drained;
   __shared__ uint32_t tmem_slot;
   const int SB = C::stage_bytes(p.Tp), S = p.stages;
   uint8_t* const hbuf = smem + S * SB;
   const FewExpertParams& e = p.e;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n1 = C::PARTS * p.Tp;                       // columns of product 1's accumulator
-  const int cols = 4 * n1 <= 64 ? 64 : 4 * n1 <= 128 ? 128 : 4 * n1 <= 256 ? 256 : 512;
+  const int n1 = C::PARTS * p.Tp;                       // columns of an accumulator
+  const FewAcc acc(n1);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], 4); }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc1_full[i], 1); mbar_init(&acc1_empty[i], 4);
-      mbar_init(&acc2_full[i], 1); mbar_init(&acc2_empty[i], 4);
-    }
+    for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], C::SPLITTERS / 32); }
+    for (int i = 0; i < 4; ++i) { mbar_init(&acc1_full[i], 1); mbar_init(&acc1_empty[i], 4); }
+    for (int i = 0; i < 12; ++i) { mbar_init(&acc2_full[i], 1); mbar_init(&acc2_empty[i], 4); }
     mbar_init(&drained, 1);
     fence_mbarrier_init();
-    tma_prefetch_desc(&tx); tma_prefetch_desc(&t1); tma_prefetch_desc(&t2); tma_prefetch_desc(&t2u);
+    tma_prefetch_desc(&tx); tma_prefetch_desc(&t1); tma_prefetch_desc(&t1w); tma_prefetch_desc(&t2); tma_prefetch_desc(&t2u);
   }
-  if (warp == 1) { tmem_alloc(&tmem_slot, cols); tmem_relinquish(); }
+  for (int i = threadIdx.x; i < e.E; i += blockDim.x) plan.mask[i] = 0ull;
+  if (warp == 1) { tmem_alloc(&tmem_slot, acc.columns()); tmem_relinquish(); }
   tc_fence_before_sync();
+  __syncthreads();
   griddep_wait();
   const int UE = (e.F + 15) / 16;
   few_plan(p, plan, UE, gridDim.x);   // holds __syncthreads
@@ -276,50 +337,71 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   const uint32_t tmem = tmem_slot;
   const int KB = (e.D + C::BK - 1) / C::BK;             // 128-byte steps of product 1
   const int nO = p.Op / 128;
-  const int TU = GLU ? 4 : 8;                           // units of a product-1 tile
+  constexpr int TU = GLU ? 4 : 8;                       // units of a product-1 tile
+  constexpr int UB = GLU ? 4096 : 2048;                 // bytes of one in a step
   const int hrows = p.hbytes / 128;
+  const int packs = C::packs(p.Tp);
   FewWalk walk;
   walk.start(plan, UE, gridDim.x);
   FewRun r;
   int stage = 0;
   uint32_t phase = 0;
   auto advance = [&]() { if (++stage == S) { stage = 0; phase ^= 1u; } };
+  // K steps that share a stage for a tile of nu units
+  auto pack_of = [&](int nu) { const int n = TU / nu; return n < packs ? n : packs; };
 
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     if (elect_one_sync()) {
       bool ok = true;
-      while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
-        for (int u0 = 0; ok && u0 < r.units; u0 += TU) {
-          const int nu = r.units - u0 < TU ? r.units - u0 : TU;
-          for (int kb = 0; kb < KB; ++kb) {
-            if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
-            uint8_t* w = smem + stage * SB;
-            mbar_arrive_expect_tx(&full[stage], nu * (GLU ? 4096 : 2048) + n1 * 128);
-            for (int u = 0; u < nu; ++u) {
-              const int f = r.f0 + (u0 + u) * 16;
-              if constexpr (GLU) tma_load_4d(w + u * 4096, &t1, &full[stage], kb * C::BK, f, 0, r.expert);
-              else tma_load_3d(w + u * 2048, &t1, &full[stage], kb * C::BK, f, r.expert);
+      while (ok) {
+        FewWalk again = walk;
+        int off = 0, runs = 0;
+        for (; ok && walk.next(plan, hrows, C::PARTS, C::UPS, off, r); ++runs) {
+          for (int u0 = 0; ok && u0 < r.units; u0 += TU) {
+            const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu), f0 = r.f0 + u0 * 16;
+            for (int kb = 0; kb < KB; kb += pack) {
+              if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+              uint8_t* w = smem + stage * SB;
+              uint8_t* x = w + C::PARTS * kFewTile;
+              const int n = KB - kb < pack ? KB - kb : pack;
+              mbar_arrive_expect_tx(&full[stage], n * (nu * UB + n1 * 128));
+              for (int k = 0; k < n; ++k, w += nu * UB, x += n1 * 128) {
+                const int d = (kb + k) * C::BK;
+                if (nu == TU && p.wide) {
+                  if constexpr (GLU) tma_load_5d(w, &t1w, &full[stage], d, 0, 0, f0 / 16, r.expert);
+                  else tma_load_3d(w, &t1w, &full[stage], d, f0, r.expert);
+                } else {
+                  for (int u = 0; u < nu; ++u) {
+                    if constexpr (GLU) tma_load_4d(w + u * UB, &t1, &full[stage], d, f0 + u * 16, 0, r.expert);
+                    else tma_load_3d(w + u * UB, &t1, &full[stage], d, f0 + u * 16, r.expert);
+                  }
+                }
+                tma_load_2d(x, &tx, &full[stage], d, 0);
+              }
+              advance();
             }
-            tma_load_2d(w + C::PARTS * kFewTile, &tx, &full[stage], kb * C::BK, 0);
-            advance();
           }
         }
-        const int slices = r.units / C::UPS, tail = r.units % C::UPS;
-        for (int i = 0; ok && i < nO; ++i) {
-          const int o = i * 128;
-          for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
-            if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
-            uint8_t* w = smem + stage * SB;
-            const int f = r.f0 + s * C::BK;
-            if (s < slices) {
-              mbar_arrive_expect_tx(&full[stage], kFewTile);
-              tma_load_3d(w, &t2, &full[stage], f, o, r.expert);
-            } else {
-              mbar_arrive_expect_tx(&full[stage], tail * 128 * C::TAIL);
-              for (int u = 0; u < tail; ++u) tma_load_3d(w + u * 128 * C::TAIL, &t2u, &full[stage], f + u * 16, o, r.expert);
+        if (runs == 0) break;
+        off = 0;
+        for (; ok && runs > 0; --runs) {
+          again.next(plan, hrows, C::PARTS, C::UPS, off, r);
+          const int slices = r.units / C::UPS, tail = r.units % C::UPS;
+          for (int i = 0; ok && i < nO; ++i) {
+            for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
+              if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+              uint8_t* w = smem + stage * SB;
+              const int f = r.f0 + s * C::BK;
+              if (s < slices) {
+                mbar_arrive_expect_tx(&full[stage], kFewTile);
+                tma_load_3d(w, &t2, &full[stage], f, i * 128, r.expert);
+              } else {
+                mbar_arrive_expect_tx(&full[stage], tail * 128 * C::TAIL);
+                for (int u = 0; u < tail; ++u) tma_load_3d(w + u * 128 * C::TAIL, &t2u, &full[stage], f + u * 16, i * 128, r.expert);
+              }
+              advance();
             }
-            advance();
           }
         }
       }
@@ -328,9 +410,9 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
     // ---------------------------------------------------------------- products
     if (elect_one_sync()) {
       uint64_t* ready = FP32 ? parted : full;
-      int i1 = 0, i2 = 0;
+      int i1 = 0, j2[2] = {0, 0};   // tiles of product 1; tiles of product 2 by group
       bool ok = true;
-      // one 128-byte K step: 32 bytes at a time, weights [hi | lo] against token rows [hi; lo]
+      // 32 bytes of K: weights [hi | lo] against token rows [hi; lo]
       auto step = [&](uint32_t d, uint64_t a, uint64_t alo, uint64_t b, int n, uint32_t more) {
         if constexpr (FP32) {
           umma_tf32(d, a, b, umma_idesc(2u, 128, 2 * n), more);
@@ -339,213 +421,254 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           umma_f16(d, a, b, umma_idesc(1u, 128, n), more);
         }
       };
-      while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
-        for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
-          const int b = i1 & 1;
-          if (!(ok = mbar_wait_bounded(&acc1_empty[b], ((i1 >> 1) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
-          tc_fence_after_sync();
-          const uint32_t d = tmem + b * n1;
-          for (int kb = 0; kb < KB; ++kb) {
-            if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+      while (ok) {
+        FewWalk again = walk;
+        int off = 0, runs = 0;
+        for (; ok && walk.next(plan, hrows, C::PARTS, C::UPS, off, r); ++runs) {
+          for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
+            const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu);
+            const int g = i1 & 1, j = i1 >> 1, b = j % acc.nA;
+            if (!(ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], ((j / acc.nA) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
-            const uint32_t w = smem_u32(smem + stage * SB), x = w + C::PARTS * kFewTile;
+            const uint32_t d = tmem + acc.first(g, b);
+            for (int kb = 0; kb < KB; kb += pack) {
+              if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+              tc_fence_after_sync();
+              uint32_t w = smem_u32(smem + stage * SB), x = w + C::PARTS * kFewTile;
+              const int n = KB - kb < pack ? KB - kb : pack;
+              for (int kk = 0; kk < n; ++kk, w += nu * UB, x += n1 * 128) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(x + k * 32),
-                   p.Tp, (kb | k) ? 1u : 0u);
-            umma_commit(&empty[stage]);
-            advance();
-          }
-          umma_commit(&acc1_full[b]);
-        }
-        // the activations of every tile are in shared memory once its accumulator was released
-        for (int b = 0; ok && b < 2; ++b) {
-          const int uses = (i1 + 1 - b) >> 1;
-          if (uses > 0) ok = mbar_wait_bounded(&acc1_empty[b], (uses - 1) & 1, status, kFewKernelId, kFewWaitNs);
-        }
-        tc_fence_after_sync();
-        const int slices = r.units / C::UPS, tail = r.units % C::UPS;
-        const uint32_t hrow = C::PARTS * r.np * 128;   // bytes of a slice of activations
-        for (int i = 0; ok && i < nO; ++i, ++i2) {
-          const int b = i2 & 1;
-          if (!(ok = mbar_wait_bounded(&acc2_empty[b], ((i2 >> 1) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
-          tc_fence_after_sync();
-          const uint32_t d = tmem + 2 * n1 + b * n1;
-          for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
-            if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
-            tc_fence_after_sync();
-            const uint32_t w = smem_u32(smem + stage * SB), h = smem_u32(hbuf) + s * hrow;
-            if (s < slices) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(h + k * 32),
-                     r.np, (s | k) ? 1u : 0u);
-            } else {
-              constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
-              for (int u = 0; u < tail; ++u)
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                  const uint32_t a = w + u * 128 * C::TAIL + k * 32;
-                  step(d, umma_desc_k_narrow(a, C::TAIL), umma_desc_k_narrow(a + kFewTile, C::TAIL),
-                       umma_desc_k_sw128(h + (u * KS + k) * 32), r.np, (s | u | k) ? 1u : 0u);
-                }
+                for (int k = 0; k < 4; ++k)
+                  step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(x + k * 32),
+                       p.Tp, (kb | kk | k) ? 1u : 0u);
+              }
+              umma_commit(&empty[stage]);
+              advance();
             }
-            umma_commit(&empty[stage]);
-            advance();
+            umma_commit(&acc1_full[g * 2 + b]);
           }
-          umma_commit(&acc2_full[b]);
+        }
+        if (runs == 0) break;
+        // a tile's activations are in shared memory once its accumulator was released
+        for (int g = 0; g < 2; ++g)
+          for (int b = 0; ok && b < acc.nA; ++b) {
+            const int tiles = (i1 + 1 - g) >> 1, uses = (tiles + acc.nA - 1 - b) / acc.nA;
+            if (uses > 0) ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], (uses - 1) & 1, status, kFewKernelId, kFewWaitNs);
+          }
+        tc_fence_after_sync();
+        off = 0;
+        for (; ok && runs > 0; --runs) {
+          again.next(plan, hrows, C::PARTS, C::UPS, off, r);
+          const int slices = r.units / C::UPS, tail = r.units % C::UPS;
+          const uint32_t hrow = C::PARTS * r.np * 128;   // bytes of a slice of activations
+          for (int i = 0; ok && i < nO; ++i) {
+            const int g = i & 1, j = j2[g]++, b = j % acc.nB;
+            if (!(ok = mbar_wait_bounded(&acc2_empty[g * 6 + b], ((j / acc.nB) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+            tc_fence_after_sync();
+            const uint32_t d = tmem + acc.second(g, b);
+            for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
+              if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+              tc_fence_after_sync();
+              const uint32_t w = smem_u32(smem + stage * SB), h = smem_u32(hbuf) + r.h * 128 + s * hrow;
+              if (s < slices) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(h + k * 32),
+                       r.np, (s | k) ? 1u : 0u);
+              } else {
+                constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
+                for (int u = 0; u < tail; ++u)
+#pragma unroll
+                  for (int k = 0; k < KS; ++k) {
+                    const uint32_t a = w + u * 128 * C::TAIL + k * 32;
+                    step(d, umma_desc_k_narrow(a, C::TAIL), umma_desc_k_narrow(a + kFewTile, C::TAIL),
+                         umma_desc_k_sw128(h + (u * KS + k) * 32), r.np, (s | u | k) ? 1u : 0u);
+                  }
+              }
+              umma_commit(&empty[stage]);
+              advance();
+            }
+            umma_commit(&acc2_full[g * 6 + b]);
+          }
         }
       }
       // every product has finished before the accumulators are freed
       umma_commit(&drained);
       mbar_wait_bounded(&drained, 0, status, kFewKernelId, kFewWaitNs);
     }
-  } else if (warp < 6) {
+  } else if (warp < 10) {
     // ---------------------------------------------------------------- epilogues
-    const int q = warp & 3;                               // TMEM lanes 32 q .. 32 q + 31
+    const int q = warp & 3, g = (warp - 2) >> 2;          // TMEM lanes 32 q .. 32 q + 31; group
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16);
-    int i1 = 0, i2 = 0;
+    int i1 = 0, j2 = 0;
     bool ok = true;
-    while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
-      const unsigned long long mask = plan.mask[r.expert];
-      const float* b1 = e.b1 ? e.b1 + (long long)r.expert * (GLU ? 2 : 1) * e.F : nullptr;
-      const uint32_t hrow = C::PARTS * r.np * 128;
-      for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
-        const int b = i1 & 1;
-        const int unit = u0 + (GLU ? q : 2 * q + (lane >> 4));  // of the run
-        const int fl = unit * 16 + (lane & 15);           // hidden row of the run
-        const int f = r.f0 + fl;
-        const bool real = f < e.F;
-        float bias = 0.f, bias_up = 0.f;
-        if (b1 && real && unit < r.units) {
-          bias = __ldg(b1 + f);
-          if constexpr (GLU) bias_up = __ldg(b1 + e.F + f);
-        }
-        ok = mbar_wait_bounded(&acc1_full[b], (i1 >> 1) & 1, status, kFewKernelId, kFewWaitNs);
-        tc_fence_after_sync();
-        const uint32_t base = lane_addr + b * n1;
-        uint8_t* hcol = hbuf + (fl / C::BK) * hrow;
-        const int byte = (fl % C::BK) * C::EB;
-        const bool any = u0 + (GLU ? q : 2 * q) < r.units;  // this warp has a unit of the tile
-        for (int c = 0; any && c < p.Tp; c += 16) {
-          const unsigned take = (unsigned)(mask >> c) & 0xffffu;   // the expert's tokens among these 16
-          if (take == 0u) continue;
-          uint32_t v[16];
-          tmem_ld16(base + c, v);
-          if constexpr (FP32) {
-            uint32_t l[16];
-            tmem_ld16(base + p.Tp + c, l);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(l[i]));
-          } else {
-            tmem_ld_wait();
+    while (ok) {
+      FewWalk again = walk;
+      int off = 0, runs = 0;
+      for (; ok && walk.next(plan, hrows, C::PARTS, C::UPS, off, r); ++runs) {
+        const unsigned long long mask = plan.mask[r.expert];
+        const float* b1 = e.b1 ? e.b1 + (long long)r.expert * (GLU ? 2 : 1) * e.F : nullptr;
+        const uint32_t hrow = C::PARTS * r.np * 128;
+        for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
+          if ((i1 & 1) != g) continue;
+          const int j = i1 >> 1, b = j % acc.nA;
+          const int unit = u0 + (GLU ? q : 2 * q + (lane >> 4));  // of the run
+          const int fl = unit * 16 + (lane & 15);           // hidden row of the run
+          const int f = r.f0 + fl;
+          const bool real = f < e.F;
+          float bias = 0.f, bias_up = 0.f;
+          if (b1 && real && unit < r.units) {
+            bias = __ldg(b1 + f);
+            if constexpr (GLU) bias_up = __ldg(b1 + e.F + f);
           }
-          const int below = __popcll(mask & ((1ull << c) - 1ull));
-          auto put = [&](int i, float val) {   // activation of token c + i
-            const int n = below + __popc(take & ((1u << i) - 1u));
-            const float h = real ? val : 0.f;
-            uint8_t* at = hcol + (n >> 3) * 1024 + (n & 7) * 128 + (byte ^ ((n & 7) << 4));
+          ok = mbar_wait_bounded(&acc1_full[g * 2 + b], (j / acc.nA) & 1, status, kFewKernelId, kFewWaitNs);
+          tc_fence_after_sync();
+          const uint32_t base = lane_addr + acc.first(g, b);
+          uint8_t* hcol = hbuf + r.h * 128 + (fl / C::BK) * hrow;
+          const int byte = (fl % C::BK) * C::EB;
+          const bool any = u0 + (GLU ? q : 2 * q) < r.units;  // this warp has a unit of the tile
+          for (int c = 0; any && c < p.Tp; c += 16) {
+            const unsigned take = (unsigned)(mask >> c) & 0xffffu;   // the expert's tokens among these 16
+            if (take == 0u) continue;
+            uint32_t v[16];
+            tmem_ld16(base + c, v);
             if constexpr (FP32) {
-              float hi, lo;
-              split_tf32(h, hi, lo);
-              *(float*)at = hi;
-              *(float*)(at + r.np * 128) = lo;
+              uint32_t l[16];
+              tmem_ld16(base + p.Tp + c, l);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(l[i]));
             } else {
-              *(__nv_bfloat16*)at = __float2bfloat16_rn(h);
+              tmem_ld_wait();
             }
-          };
-          if constexpr (GLU) {
-            // lanes 0-15 hold gate rows, 16-31 the up rows of the same f: each half takes eight of the columns
-            const bool up = lane >= 16;
+            const int below = __popcll(mask & ((1ull << c) - 1ull));
+            auto put = [&](int i, float val) {   // activation of token c + i
+              const int n = below + __popc(take & ((1u << i) - 1u));
+              const float h = real ? val : 0.f;
+              uint8_t* at = hcol + (n >> 3) * 1024 + (n & 7) * 128 + (byte ^ ((n & 7) << 4));
+              if constexpr (FP32) {
+                float hi, lo;
+                split_tf32(h, hi, lo);
+                *(float*)at = hi;
+                *(float*)(at + r.np * 128) = lo;
+              } else {
+                *(__nv_bfloat16*)at = __float2bfloat16_rn(h);
+              }
+            };
+            if constexpr (GLU) {
+              // lanes 0-15 hold gate rows, 16-31 the up rows of the same f: each half takes eight of the columns
+              const bool up = lane >= 16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float mine = __uint_as_float(up ? v[8 + i] : v[i]);
-              const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(up ? v[i] : v[8 + i]), 16);
-              const int col = up ? 8 + i : i;
-              const float gate = (up ? other : mine) + bias, lin = (up ? mine : other) + bias_up;
-              if (take >> col & 1u) put(col, serving_swiglu(gate, lin));
+              for (int i = 0; i < 8; ++i) {
+                const float mine = __uint_as_float(up ? v[8 + i] : v[i]);
+                const float other = __shfl_xor_sync(0xffffffffu, __uint_as_float(up ? v[i] : v[8 + i]), 16);
+                const int col = up ? 8 + i : i;
+                const float gate = (up ? other : mine) + bias, lin = (up ? mine : other) + bias_up;
+                if (take >> col & 1u) put(col, serving_swiglu(gate, lin));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if ((take >> i & 1u) && unit < r.units) put(i, serving_act(__uint_as_float(v[i]) + bias, e.act));
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if ((take >> i & 1u) && unit < r.units) put(i, serving_act(__uint_as_float(v[i]) + bias, e.act));
           }
+          fence_proxy_async_smem();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc1_empty[g * 2 + b]);
         }
-        fence_proxy_async_smem();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc1_empty[b]);
       }
-      // product 2: this CTA's part of the expert's result
-      const int mine = (int)blockIdx.x - few_cta((long long)r.place * UE, walk.U, walk.G);
-      float* dst = p.part + (long long)(plan.part0[r.place] + mine * r.tokens) * p.Op + q * 32 + lane;
-      for (int i = 0; ok && i < nO; ++i, ++i2) {
-        const int b = i2 & 1;
-        ok = mbar_wait_bounded(&acc2_full[b], (i2 >> 1) & 1, status, kFewKernelId, kFewWaitNs);
-        tc_fence_after_sync();
-        const uint32_t base = lane_addr + 2 * n1 + b * n1;
-        for (int c = 0; c < r.tokens; c += 16) {
-          uint32_t v[16];
-          tmem_ld16(base + c, v);
-          if constexpr (FP32) {
-            uint32_t l[16];
-            tmem_ld16(base + r.np + c, l);
-            tmem_ld_wait();
+      if (runs == 0) break;
+      off = 0;
+      for (; ok && runs > 0; --runs) {
+        again.next(plan, hrows, C::PARTS, C::UPS, off, r);
+        // product 2: this CTA's part of the expert's result.  Columns 128 i belong to group i % 2, so a cut
+        // run's later pieces are added by the thread that wrote the first.
+        const int mine = (int)blockIdx.x - few_cta((long long)r.place * UE, walk.U, walk.G);
+        float* dst = p.part + (long long)(plan.part0[r.place] + mine * r.tokens) * p.Op + q * 32 + lane;
+        for (int i = g; ok && i < nO; i += 2, ++j2) {
+          const int b = j2 % acc.nB;
+          ok = mbar_wait_bounded(&acc2_full[g * 6 + b], (j2 / acc.nB) & 1, status, kFewKernelId, kFewWaitNs);
+          tc_fence_after_sync();
+          const uint32_t base = lane_addr + acc.second(g, b);
+          for (int c = 0; c < r.tokens; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(base + c, v);
+            if constexpr (FP32) {
+              uint32_t l[16];
+              tmem_ld16(base + r.np + c, l);
+              tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(l[j]));
-          } else {
-            tmem_ld_wait();
-          }
+              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(l[j]));
+            } else {
+              tmem_ld_wait();
+            }
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (c + j >= r.tokens) break;
-            float* at = dst + (long long)(c + j) * p.Op + i * 128;
-            float out = __uint_as_float(v[j]);
-            if (!r.first) out += *at;   // written by this thread
-            *at = out;
+            for (int j = 0; j < 16; ++j) {
+              if (c + j >= r.tokens) break;
+              float* at = dst + (long long)(c + j) * p.Op + i * 128;
+              float out = __uint_as_float(v[j]);
+              if (!r.first) out += *at;
+              *at = out;
+            }
           }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&acc2_empty[g * 6 + b]);
         }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc2_empty[b]);
       }
     }
   } else if constexpr (FP32) {
     // ---------------------------------------------------------------- weights into tf32 parts
-    const int tid = threadIdx.x - 192;
+    const int tid = threadIdx.x - 320;
     bool ok = true;
     auto part = [&](int bytes) {
       if (!(ok = mbar_wait_bounded(&full[stage], phase, status, kFewKernelId, kFewWaitNs))) return;
-      uint8_t* w = smem + stage * SB;
-      for (int i = tid * 16; i < bytes; i += 128 * 16) {
-        float4 v = *(float4*)(w + i), h, l;
-        split_tf32(v.x, h.x, l.x);
-        split_tf32(v.y, h.y, l.y);
-        split_tf32(v.z, h.z, l.z);
-        split_tf32(v.w, h.w, l.w);
-        *(float4*)(w + i) = h;
-        *(float4*)(w + kFewTile + i) = l;
+      uint8_t* w = smem + stage * SB + tid * 16;
+      constexpr int N = kFewTile / (C::SPLITTERS * 16);
+      float4 v[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (tid * 16 + i * C::SPLITTERS * 16 < bytes) v[i] = *(const float4*)(w + i * C::SPLITTERS * 16);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (tid * 16 + i * C::SPLITTERS * 16 >= bytes) break;
+        float4 h, l;
+        split_tf32(v[i].x, h.x, l.x);
+        split_tf32(v[i].y, h.y, l.y);
+        split_tf32(v[i].z, h.z, l.z);
+        split_tf32(v[i].w, h.w, l.w);
+        *(float4*)(w + i * C::SPLITTERS * 16) = h;
+        *(float4*)(w + i * C::SPLITTERS * 16 + kFewTile) = l;
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&parted[stage]);
       advance();
     };
-    while (ok && walk.next(plan, hrows, C::PARTS, C::UPS, r)) {
-      for (int u0 = 0; ok && u0 < r.units; u0 += TU) {
-        const int nu = r.units - u0 < TU ? r.units - u0 : TU;
-        for (int kb = 0; ok && kb < KB; ++kb) part(nu * (GLU ? 4096 : 2048));
+    while (ok) {
+      FewWalk again = walk;
+      int off = 0, runs = 0;
+      for (; ok && walk.next(plan, hrows, C::PARTS, C::UPS, off, r); ++runs) {
+        for (int u0 = 0; ok && u0 < r.units; u0 += TU) {
+          const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu);
+          for (int kb = 0; ok && kb < KB; kb += pack) part((KB - kb < pack ? KB - kb : pack) * nu * UB);
+        }
       }
-      const int slices = r.units / C::UPS, tail = r.units % C::UPS;
-      for (int i = 0; ok && i < nO; ++i)
-        for (int s = 0; ok && s < slices + (tail ? 1 : 0); ++s) part(s < slices ? kFewTile : tail * 128 * C::TAIL);
+      if (runs == 0) break;
+      off = 0;
+      for (; ok && runs > 0; --runs) {
+        again.next(plan, hrows, C::PARTS, C::UPS, off, r);
+        const int slices = r.units / C::UPS, tail = r.units % C::UPS;
+        for (int i = 0; ok && i < nO; ++i)
+          for (int s = 0; ok && s < slices + (tail ? 1 : 0); ++s) part(s < slices ? kFewTile : tail * 128 * C::TAIL);
+      }
     }
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (warp == 1) tmem_dealloc(tmem, cols);
+  if (warp == 1) tmem_dealloc(tmem, acc.columns());
 }
 
 }  // namespace raiccl

@@ -35,6 +35,7 @@ struct FewRouteParams {
   void* packed;           // x for the experts' kernel, or nullptr: bf16 rows [T, packed_stride] as they are;
   long long packed_stride;  // fp32 [2][packed_rows, packed_stride] as two tf32 parts
   int packed_rows;
+  int cuts;               // pieces of a row, by the launch
 };
 
 // The experts' MLPs and the weighted sum of the routed tokens.

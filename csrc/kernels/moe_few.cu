@@ -47,6 +47,8 @@ DeviceStatus* serving_status() {
 // ---------------------------------------------------------------------------
 constexpr int kRouteThreads = 256;
 constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kRouteCuts = 8;
+static_assert(kRouteThreads > kFewExperts, "a thread per expert");
 
 // Sort key, larger = preferred: 0 for no candidate (blocked, or a logit of
 // -inf), then NaN, then numbers by value (an order-preserving map of the float
@@ -59,17 +61,17 @@ __device__ __forceinline__ unsigned long long few_key(float v, int e) {
   return (2ull << 40) | ((unsigned long long)u << 8) | (unsigned long long)(255 - e);
 }
 
-// x . w of one row pair by one warp, in 32 bits: each lane sums its vectors'
-// partial sums, a butterfly adds the lanes.
+// x . w over vectors (elements where rows are not aligned) [i0, i1) by one
+// warp, in 32 bits: each lane adds its vectors' partial sums, a butterfly adds
+// the lanes.
 template <typename T>
-__device__ __forceinline__ float route_dot(const T* x, const T* w, int D, int vec) {
+__device__ __forceinline__ float route_dot(const T* x, const T* w, int i0, int i1, int vec) {
   const int lane = threadIdx.x & 31;
   float acc = 0.f;
   if (vec) {
     constexpr int V = 16 / sizeof(T);
-    const int n = D / V;
 #pragma unroll 8
-    for (int i = lane; i < n; i += 32) {
+    for (int i = i0 + lane; i < i1; i += 32) {
       const uint4 xr = __ldg((const uint4*)x + i);
       const uint4 wr = __ldg((const uint4*)w + i);
       float s = 0.f;
@@ -79,24 +81,31 @@ __device__ __forceinline__ float route_dot(const T* x, const T* w, int D, int ve
     }
   } else {
 #pragma unroll 8
-    for (int i = lane; i < D; i += 32) acc = fmaf(as_float(x[i]), as_float(w[i]), acc);
+    for (int i = i0 + lane; i < i1; i += 32) acc = fmaf(as_float(x[i]), as_float(w[i]), acc);
   }
   return warp_sum(acc);
 }
 
+// One cluster per token.  The experts' rows, cut into `cuts` pieces each, are
+// dealt to the warps of its CTAs; the first CTA adds the pieces in order and
+// finds each expert's rank among all (the number of experts with a larger key),
+// so the choices need no rounds.
 template <typename T>
 __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams p) {
+  __shared__ float piece[kRouteCuts][kFewExperts + 1];
   __shared__ float logits[kFewExperts + 1];
+  __shared__ unsigned long long keys[kFewExperts + 1];
+  __shared__ int chosen[kFewTopK];
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int t = blockIdx.y;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* x = (const T*)p.x + (long long)t * p.x_stride;
-  float* lead = cluster.map_shared_rank(logits, 0);
+  float* lead = cluster.map_shared_rank(&piece[0][0], 0);
   griddep_wait();
   griddep_launch_dependents();
-  const int share = rank * kRouteThreads + threadIdx.x, shares = ranks * kRouteThreads;
   if (p.packed) {
+    const int share = rank * kRouteThreads + threadIdx.x, shares = ranks * kRouteThreads;
     for (int d = share; d < p.D; d += shares) {
       if constexpr (sizeof(T) == 4) {
         float* at = (float*)p.packed + (long long)t * p.packed_stride + d;
@@ -106,64 +115,63 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams
       }
     }
   }
-  for (int e = warp * ranks + rank; e < p.E; e += kRouteWarps * ranks) {
-    float v = route_dot(x, (const T*)p.w + (long long)e * p.w_stride, p.D, p.vec);
-    if (lane == 0) {
-      if (p.bias) v += p.bias[e];
-      if (p.mask && p.mask[(long long)t * p.mask_stride + e]) v = -INFINITY;
-      lead[e] = v;
-    }
+  const int n = p.vec ? p.D * (int)sizeof(T) / 16 : p.D;   // vectors (elements) of a row
+  const int per = (n + p.cuts - 1) / p.cuts;
+  for (int i = warp * ranks + rank; i < p.E * p.cuts; i += kRouteWarps * ranks) {
+    const int e = i / p.cuts, c = i - e * p.cuts;
+    const int i0 = c * per, i1 = i0 + per < n ? i0 + per : n;
+    const float v = route_dot(x, (const T*)p.w + (long long)e * p.w_stride, i0, i1, p.vec);
+    if (lane == 0) lead[c * (kFewExperts + 1) + e] = v;
   }
   cluster.sync();
-  if (rank != 0 || warp != 0) return;
-  // k rounds of a warp-wide maximum; lane l holds experts l, l + 32, ...
-  constexpr int PER = (kFewExperts + 32) / 32;
-  unsigned long long key[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = i * 32 + lane;
-    key[i] = e < p.E ? few_key(logits[e], e) : 0ull;
+  if (rank != 0) return;
+  const int e = threadIdx.x;   // kRouteThreads > kFewExperts
+  unsigned long long key = 0ull;
+  if (e < p.E) {
+    float v = piece[0][e];
+    for (int c = 1; c < p.cuts; ++c) v += piece[c][e];
+    if (p.bias) v += p.bias[e];
+    if (p.mask && p.mask[(long long)t * p.mask_stride + e]) v = -INFINITY;
+    logits[e] = v;
+    keys[e] = key = few_key(v, e);
   }
-  int chosen = -1;      // lane j: choice j
-  float top = 0.f;
-#pragma unroll 1
-  for (int j = 0; j < p.k; ++j) {
-    unsigned long long best = 0ull;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) best = key[i] > best ? key[i] : best;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
-    }
-    if (best == 0ull) break;  // the same on every lane
-    const int e = 255 - (int)(best & 255ull);
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (key[i] == best) key[i] = 0ull;
-    if (lane == j) { chosen = e; top = logits[e]; }
+  if (e < kFewTopK) chosen[e] = -1;
+  __syncthreads();
+  if (key != 0ull) {
+    int above = 0;
+#pragma unroll 8
+    for (int o = 0; o < p.E; ++o) above += keys[o] > key ? 1 : 0;
+    if (above < p.k) chosen[above] = e;
   }
-  float gate = chosen < 0 ? 0.f : 1.f;
+  __syncthreads();
+  if (warp != 0) return;
+  const int mine = lane < p.k ? chosen[lane] : -1;   // lane j: choice j
+  const float top = mine < 0 ? 0.f : logits[mine];
+  float gate = mine < 0 ? 0.f : 1.f;
   if (p.gate_mode != 0) {
     const float peak = __shfl_sync(0xffffffffu, top, 0);  // the largest number, or NaN if there is none
     float part = 0.f;
     if (p.gate_mode == 1) {
-      part = chosen < 0 ? 0.f : expf(top - peak);
+      part = mine < 0 ? 0.f : expf(top - peak);
     } else {
-      for (int e = lane; e < p.E; e += 32) part += logits[e] == -INFINITY ? 0.f : expf(logits[e] - peak);
+      for (int o = lane; o < p.E; o += 32) part += logits[o] == -INFINITY ? 0.f : expf(logits[o] - peak);
     }
     const float total = warp_sum(part);
-    if (chosen >= 0) gate = expf(top - peak) / total;
+    if (mine >= 0) gate = expf(top - peak) / total;
   }
   if (lane < p.k) {
-    p.ids[(long long)t * p.k + lane] = chosen;
+    p.ids[(long long)t * p.k + lane] = mine;
     p.gates[(long long)t * p.k + lane] = gate;
   }
 }
 
-void launch_few_route(const FewRouteParams& p, cudaStream_t s) {
-  // enough CTAs that each warp has one or two experts
-  const int want = (p.E + 2 * kRouteWarps - 1) / (2 * kRouteWarps);
+void launch_few_route(const FewRouteParams& params, cudaStream_t s) {
+  // Pieces of a row so that the cluster's warps have one each, down to one
+  // vector per lane; clusters of eight CTAs at most.
+  FewRouteParams p = params;
+  const int n = p.vec ? p.D * (p.bf16 ? 2 : 4) / 16 : p.D;
+  p.cuts = std::max(1, std::min({kRouteCuts, 8 * kRouteWarps / p.E, n / 32}));
+  const int want = (p.E * p.cuts + kRouteWarps - 1) / kRouteWarps;
   const int ranks = want > 4 ? 8 : want > 2 ? 4 : want;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ranks, p.T);
@@ -304,7 +312,7 @@ static int sm_count() {
 
 static long long up256(long long v) { return (v + 255) / 256 * 256; }
 
-constexpr int kFewShared = 232448 - 12 * 1024 - 1024;  // dynamic shared memory besides the kernel's own and the alignment
+constexpr int kFewShared = 232448 - 10 * 1024 - 1024;  // dynamic shared memory besides the kernel's own and the alignment
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   FewExpertPlan r{};
@@ -335,15 +343,15 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   const long long most = ((long long)std::min(p.E, pairs) * UE + r.grid - 1) / r.grid;
   const long long rows = (std::min<long long>(most, UE) + ups - 1) / ups + 1;
   r.hbytes = (int)std::min<long long>(rows * parts * r.Tp * 128, p.bf16 ? 56 * 1024 : 24 * 1024);
-  r.hbytes = std::max(r.hbytes, parts * r.Tp * 128);
+  r.hbytes = std::max({r.hbytes, parts * r.Tp * 128, kFewSlack});
   const int sb = p.bf16 ? FewTc<false>::stage_bytes(r.Tp) : FewTc<true>::stage_bytes(r.Tp);
-  r.stages = std::min(16, (kFewShared - r.hbytes) / sb);
+  r.stages = std::min(kFewMaxStages, (kFewShared - r.hbytes) / sb);
   return r;
 }
 
 template <bool FP32, bool GLU>
-static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CUtensorMap& t2, const CUtensorMap& t2u,
-                          const FewTcParams& tp, int grid, cudaStream_t s) {
+static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CUtensorMap& t1w, const CUtensorMap& t2,
+                          const CUtensorMap& t2u, const FewTcParams& tp, int grid, cudaStream_t s) {
   auto kern = few_experts_kernel<FP32, GLU>;
   static std::atomic<unsigned long long> configured;  // by device
   const unsigned long long bit = 1ull << current_device();
@@ -353,7 +361,7 @@ static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CU
     configured.fetch_or(bit);
   }
   const size_t smem = 1024 + (size_t)tp.stages * FewTc<FP32>::stage_bytes(tp.Tp) + tp.hbytes;
-  launch_with_pdl(kern, dim3(grid), dim3(FewTc<FP32>::THREADS), smem, s, true, tx, t1, t2, t2u, tp, serving_status());
+  launch_with_pdl(kern, dim3(grid), dim3(FewTc<FP32>::THREADS), smem, s, true, tx, t1, t1w, t2, t2u, tp, serving_status());
 }
 
 void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
@@ -368,11 +376,11 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
   const cuuint64_t eb = p.bf16 ? 2 : 4;
   const cuuint32_t bk = 128 / eb;
   const int parts = p.bf16 ? 1 : 2;
-  const bool glu = p.act == (int)Act::kSwiGLU;
+  const bool glu = p.act == (int)Act::kSwiGLU, wide = !glu || p.F % 16 == 0;
   const cuuint64_t D = p.D, F = p.F, O = p.O, E = p.E;
   // a stride along a single expert or token is never used
   const cuuint64_t e1 = p.E > 1 ? p.w1_estride * eb : 16, e2 = p.E > 1 ? p.w2_estride * eb : 16;
-  CUtensorMap tx, t1, t2, t2u;
+  CUtensorMap tx, t1, t1w, t2, t2u;
   {
     const cuuint64_t dims[2] = {D, plan.pack ? (cuuint64_t)parts * plan.Tp : (cuuint64_t)p.T};
     const cuuint64_t strides[1] = {plan.pack ? plan.packed_stride * eb : p.T > 1 ? p.x_stride * eb : (D * eb + 15) / 16 * 16};
@@ -383,12 +391,19 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
     const cuuint64_t dims[4] = {D, F, 2, E};
     const cuuint64_t strides[3] = {p.w1_stride * eb, F * p.w1_stride * eb, e1};
     const cuuint32_t box[4] = {bk, 16, 2, 1};
-    t1 = make_tmap(p.w1, p.bf16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    t1 = t1w = make_tmap(p.w1, p.bf16, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (wide) {  // 16 rows of F by gate and up by four of these groups: the order of a tile's rows
+      const cuuint64_t dims[5] = {D, 16, 2, F / 16, E};
+      const cuuint64_t strides[4] = {p.w1_stride * eb, F * p.w1_stride * eb, 16 * p.w1_stride * eb, e1};
+      const cuuint32_t box[5] = {bk, 16, 2, 4, 1};
+      t1w = make_tmap(p.w1, p.bf16, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    }
   } else {
     const cuuint64_t dims[3] = {D, F, E};
     const cuuint64_t strides[2] = {p.w1_stride * eb, e1};
-    const cuuint32_t box[3] = {bk, 16, 1};
+    const cuuint32_t box[3] = {bk, 16, 1}, tile[3] = {bk, 128, 1};
     t1 = make_tmap(p.w1, p.bf16, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    t1w = make_tmap(p.w1, p.bf16, 3, dims, strides, tile, CU_TENSOR_MAP_SWIZZLE_128B);
   }
   {
     const cuuint64_t dims[3] = {F, O, E};
@@ -405,12 +420,13 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
   tp.Tp = plan.Tp;
   tp.stages = plan.stages;
   tp.hbytes = plan.hbytes;
+  tp.wide = wide;
   if (p.bf16) {
-    if (glu) launch_tensor<false, true>(tx, t1, t2, t2u, tp, plan.grid, s);
-    else launch_tensor<false, false>(tx, t1, t2, t2u, tp, plan.grid, s);
+    if (glu) launch_tensor<false, true>(tx, t1, t1w, t2, t2u, tp, plan.grid, s);
+    else launch_tensor<false, false>(tx, t1, t1w, t2, t2u, tp, plan.grid, s);
   } else {
-    if (glu) launch_tensor<true, true>(tx, t1, t2, t2u, tp, plan.grid, s);
-    else launch_tensor<true, false>(tx, t1, t2, t2u, tp, plan.grid, s);
+    if (glu) launch_tensor<true, true>(tx, t1, t1w, t2, t2u, tp, plan.grid, s);
+    else launch_tensor<true, false>(tx, t1, t1w, t2, t2u, tp, plan.grid, s);
   }
   launch_with_pdl(few_join_parts_kernel, dim3(plan.Op / 128, p.T), dim3(kFewJoinThreads), 0, s, true, tp);
 }
