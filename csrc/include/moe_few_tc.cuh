@@ -68,7 +68,6 @@ struct FewTc {
   static constexpr int UPS = BK / 16;              // units of 16 hidden rows in a 128-byte row of activations
   static constexpr int TAIL = 16 * EB;             // bytes of one unit in a row
   static constexpr int THREADS = FP32 ? 576 : 320;
-  static constexpr int SPLITTERS = 256;
   // K steps of 128 bytes that share a stage where a tile has few rows: a step
   // costs its waits and its commit, 0.2 us, whatever it holds
   static __host__ __device__ int packs(int Tp) { const int n = (FP32 ? 128 : 64) / (PARTS * Tp); return n > 4 ? 4 : n < 1 ? 1 : n; }
@@ -208,19 +207,16 @@ struct FewWalk {
   }
 };
 
-// Accumulators in TMEM, n1 columns each, for two epilogue groups: nA buffers
-// of product 1 and nB of product 2 per group.
+// Accumulators in TMEM for two epilogue groups, two buffers each where 512
+// columns allow: of product 1 one tile (n1 columns), of product 2 a group of
+// `tiles` tiles of 128 outputs, so that a few tokens' tiles share a hand-over.
 struct FewAcc {
-  int n1, nA, nB;
-  __device__ FewAcc(int n1_) : n1(n1_) {
-    const int per = 512 / (2 * n1);
-    nA = per >= 4 ? 2 : 1;
-    nB = per - nA < 1 ? 1 : per - nA > 6 ? 6 : per - nA;
-  }
-  __device__ uint32_t first(int g, int b) const { return (g * nA + b) * n1; }
-  __device__ uint32_t second(int g, int b) const { return ((2 * nA) + g * nB + b) * n1; }
+  int n1, nbuf, tiles;
+  __device__ explicit FewAcc(int n1_) : n1(n1_), nbuf(n1_ <= 64 ? 2 : 1), tiles(n1_ <= 16 ? 4 : n1_ <= 32 ? 2 : 1) {}
+  __device__ uint32_t first(int g, int b) const { return (g * nbuf + b) * n1; }
+  __device__ uint32_t second(int g, int b) const { return (2 * nbuf + (g * nbuf + b) * tiles) * n1; }
   __device__ int columns() const {
-    const int c = 2 * (nA + nB) * n1;
+    const int c = 2 * nbuf * (1 + tiles) * n1;
     return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512;
   }
 };
@@ -232,8 +228,11 @@ struct FewAcc {
 constexpr int kFewJoinThreads = 256;
 
 __global__ void __launch_bounds__(kFewJoinThreads) few_join_parts_kernel(FewTcParams p) {
-  constexpr int W = kFewJoinThreads / 32, U = 8;
+  constexpr int W = kFewJoinThreads / 32;
   __shared__ __align__(16) float red[W][128];
+  __shared__ int4 term[kFewTopK];
+  __shared__ float gate[kFewTopK], weight[kFewJoinThreads];
+  __shared__ int row[kFewJoinThreads];
   const FewExpertParams& e = p.e;
   const int t = blockIdx.y, o0 = blockIdx.x * 128;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -244,46 +243,35 @@ __global__ void __launch_bounds__(kFewJoinThreads) few_join_parts_kernel(FewTcPa
   griddep_launch_dependents();
   float res = 0.f;
   if (writes && e.residual) res = load_elem(e.residual, (long long)t * e.res_stride + o, e.res_bf16);
-  int4 term[kFewTopK];
-  float gate[kFewTopK];
-#pragma unroll
-  for (int j = 0; j < kFewTopK; ++j) {
-    term[j] = j < e.k ? __ldcg(p.terms + t * e.k + j) : make_int4(0, 0, 0, 0);
-    gate[j] = j < e.k ? __ldcg(e.gates + t * e.k + j) : 0.f;
+  if (threadIdx.x < kFewTopK) {
+    term[threadIdx.x] = threadIdx.x < e.k ? __ldcg(p.terms + t * e.k + threadIdx.x) : make_int4(0, 0, 0, 0);
+    gate[threadIdx.x] = threadIdx.x < e.k ? __ldcg(e.gates + t * e.k + threadIdx.x) : 0.f;
   }
+  __syncthreads();
   int items = 0;
+  for (int j = 0; j < e.k; ++j) items += term[j].z;
   float bias = 0.f;
-#pragma unroll
-  for (int j = 0; j < kFewTopK; ++j) {
-    items += term[j].z;
-    if (e.b2 && writes && term[j].z > 0) bias = fmaf(gate[j], __ldg(e.b2 + (long long)term[j].w * e.O + o), bias);
-  }
+  if (e.b2 && writes)
+    for (int j = 0; j < e.k; ++j)
+      if (term[j].z > 0) bias = fmaf(gate[j], __ldg(e.b2 + (long long)term[j].w * e.O + o), bias);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = w; i0 < items; i0 += W * U) {
-    float4 a[U];
-    float g[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      int c = i0 + i * W;
-      const float4* at = nullptr;
-      g[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < kFewTopK; ++j) {
-        if (c >= 0 && c < term[j].z) {
-          at = (const float4*)(col + ((long long)term[j].x + (long long)c * term[j].y) * p.Op);
-          g[i] = gate[j];
-        }
-        c = c < term[j].z ? -1 : c - term[j].z;
-        c = c < 0 ? -1 : c;
-      }
-      a[i] = at ? __ldcg(at) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      v.x = fmaf(g[i], a[i].x, v.x);
-      v.y = fmaf(g[i], a[i].y, v.y);
-      v.z = fmaf(g[i], a[i].z, v.z);
-      v.w = fmaf(g[i], a[i].w, v.w);
+  // kFewJoinThreads items at a time: each thread looks one up, then the warps read theirs
+  for (int i0 = 0; i0 < items; i0 += kFewJoinThreads) {
+    int c = i0 + threadIdx.x, j = 0;
+    while (j + 1 < e.k && c >= term[j].z) c -= term[j++].z;
+    if (i0 > 0) __syncthreads();
+    row[threadIdx.x] = term[j].x + c * term[j].y;
+    weight[threadIdx.x] = gate[j];
+    __syncthreads();
+    const int n = items - i0 < kFewJoinThreads ? items - i0 : kFewJoinThreads;
+#pragma unroll 8
+    for (int i = w; i < n; i += W) {
+      const float4 a = __ldcg((const float4*)(col + (long long)row[i] * p.Op));
+      const float g = weight[i];
+      v.x = fmaf(g, a.x, v.x);
+      v.y = fmaf(g, a.y, v.y);
+      v.z = fmaf(g, a.z, v.z);
+      v.w = fmaf(g, a.w, v.w);
     }
   }
   *(float4*)&red[w][lane * 4] = v;
@@ -308,7 +296,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ FewPlan plan;
   __shared__ uint64_t full[kFewMaxStages], empty[kFewMaxStages], parted[kFewMaxStages];
-  __shared__ uint64_t acc1_full[4], acc1_empty[4], acc2_full[12], acc2_empty[12], drained;
+  __shared__ uint64_t acc1_full[4], acc1_empty[4], acc2_full[4], acc2_empty[4], drained;
   __shared__ uint32_t tmem_slot;
   const int SB = C::stage_bytes(p.Tp), S = p.stages;
   uint8_t* const hbuf = smem + S * SB;
@@ -318,9 +306,11 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   const FewAcc acc(n1);
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], C::SPLITTERS / 32); }
-    for (int i = 0; i < 4; ++i) { mbar_init(&acc1_full[i], 1); mbar_init(&acc1_empty[i], 4); }
-    for (int i = 0; i < 12; ++i) { mbar_init(&acc2_full[i], 1); mbar_init(&acc2_empty[i], 4); }
+    for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], 4); }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&acc1_full[i], 1); mbar_init(&acc1_empty[i], 4);
+      mbar_init(&acc2_full[i], 1); mbar_init(&acc2_empty[i], 4);
+    }
     mbar_init(&drained, 1);
     fence_mbarrier_init();
     tma_prefetch_desc(&tx); tma_prefetch_desc(&t1); tma_prefetch_desc(&t1w); tma_prefetch_desc(&t2); tma_prefetch_desc(&t2u);
@@ -339,6 +329,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   const int nO = p.Op / 128;
   constexpr int TU = GLU ? 4 : 8;                       // units of a product-1 tile
   constexpr int UB = GLU ? 4096 : 2048;                 // bytes of one in a step
+  constexpr int UPT = kFewTile / (128 * C::TAIL);       // units of 128 rows of W2 in a tile's bytes
   const int hrows = p.hbytes / 128;
   const int packs = C::packs(p.Tp);
   FewWalk walk;
@@ -388,18 +379,24 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         for (; ok && runs > 0; --runs) {
           again.next(plan, hrows, C::PARTS, C::UPS, off, r);
           const int slices = r.units / C::UPS, tail = r.units % C::UPS;
-          for (int i = 0; ok && i < nO; ++i) {
-            for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
-              if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
-              uint8_t* w = smem + stage * SB;
-              const int f = r.f0 + s * C::BK;
-              if (s < slices) {
+          const int share = tail ? UPT / tail : 1;   // tiles whose last units share a stage
+          for (int i0 = 0; ok && i0 < nO; i0 += acc.tiles) {
+            const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
+            for (int s = 0; ok && s < slices; ++s)
+              for (int i = 0; i < nt; ++i) {
+                if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
                 mbar_arrive_expect_tx(&full[stage], kFewTile);
-                tma_load_3d(w, &t2, &full[stage], f, i * 128, r.expert);
-              } else {
-                mbar_arrive_expect_tx(&full[stage], tail * 128 * C::TAIL);
-                for (int u = 0; u < tail; ++u) tma_load_3d(w + u * 128 * C::TAIL, &t2u, &full[stage], f + u * 16, i * 128, r.expert);
+                tma_load_3d(smem + stage * SB, &t2, &full[stage], r.f0 + s * C::BK, (i0 + i) * 128, r.expert);
+                advance();
               }
+            for (int i = 0; ok && tail && i < nt; i += share) {
+              const int n = nt - i < share ? nt - i : share;
+              if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+              mbar_arrive_expect_tx(&full[stage], n * tail * 128 * C::TAIL);
+              uint8_t* w = smem + stage * SB;
+              for (int m = 0; m < n; ++m)
+                for (int u = 0; u < tail; ++u, w += 128 * C::TAIL)
+                  tma_load_3d(w, &t2u, &full[stage], r.f0 + slices * C::BK + u * 16, (i0 + i + m) * 128, r.expert);
               advance();
             }
           }
@@ -427,8 +424,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         for (; ok && walk.next(plan, hrows, C::PARTS, C::UPS, off, r); ++runs) {
           for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
             const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu);
-            const int g = i1 & 1, j = i1 >> 1, b = j % acc.nA;
-            if (!(ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], ((j / acc.nA) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+            const int g = i1 & 1, j = i1 >> 1, b = j & (acc.nbuf - 1);
+            if (!(ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
             const uint32_t d = tmem + acc.first(g, b);
             for (int kb = 0; kb < KB; kb += pack) {
@@ -451,8 +448,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         if (runs == 0) break;
         // a tile's activations are in shared memory once its accumulator was released
         for (int g = 0; g < 2; ++g)
-          for (int b = 0; ok && b < acc.nA; ++b) {
-            const int tiles = (i1 + 1 - g) >> 1, uses = (tiles + acc.nA - 1 - b) / acc.nA;
+          for (int b = 0; ok && b < acc.nbuf; ++b) {
+            const int tiles = (i1 + 1 - g) >> 1, uses = (tiles + acc.nbuf - 1 - b) / acc.nbuf;
             if (uses > 0) ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], (uses - 1) & 1, status, kFewKernelId, kFewWaitNs);
           }
         tc_fence_after_sync();
@@ -461,34 +458,43 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           again.next(plan, hrows, C::PARTS, C::UPS, off, r);
           const int slices = r.units / C::UPS, tail = r.units % C::UPS;
           const uint32_t hrow = C::PARTS * r.np * 128;   // bytes of a slice of activations
-          for (int i = 0; ok && i < nO; ++i) {
-            const int g = i & 1, j = j2[g]++, b = j % acc.nB;
-            if (!(ok = mbar_wait_bounded(&acc2_empty[g * 6 + b], ((j / acc.nB) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+          const int share = tail ? UPT / tail : 1;
+          for (int i0 = 0, g = 0; ok && i0 < nO; i0 += acc.tiles, g ^= 1) {
+            const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
+            const int j = j2[g]++, b = j & (acc.nbuf - 1);
+            if (!(ok = mbar_wait_bounded(&acc2_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
-            const uint32_t d = tmem + acc.second(g, b);
-            for (int s = 0; s < slices + (tail ? 1 : 0); ++s) {
-              if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
-              tc_fence_after_sync();
-              const uint32_t w = smem_u32(smem + stage * SB), h = smem_u32(hbuf) + r.h * 128 + s * hrow;
-              if (s < slices) {
+            const uint32_t d = tmem + acc.second(g, b), dn = C::PARTS * r.np;
+            const uint32_t h0 = smem_u32(hbuf) + r.h * 128;
+            for (int s = 0; ok && s < slices; ++s)
+              for (int i = 0; i < nt; ++i) {
+                if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+                tc_fence_after_sync();
+                const uint32_t w = smem_u32(smem + stage * SB), h = h0 + s * hrow;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(h + k * 32),
-                       r.np, (s | k) ? 1u : 0u);
-              } else {
-                constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
-                for (int u = 0; u < tail; ++u)
-#pragma unroll
-                  for (int k = 0; k < KS; ++k) {
-                    const uint32_t a = w + u * 128 * C::TAIL + k * 32;
-                    step(d, umma_desc_k_narrow(a, C::TAIL), umma_desc_k_narrow(a + kFewTile, C::TAIL),
-                         umma_desc_k_sw128(h + (u * KS + k) * 32), r.np, (s | u | k) ? 1u : 0u);
-                  }
+                  step(d + i * dn, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32),
+                       umma_desc_k_sw128(h + k * 32), r.np, (s | k) ? 1u : 0u);
+                umma_commit(&empty[stage]);
+                advance();
               }
+            for (int i = 0; ok && tail && i < nt; i += share) {
+              const int n = nt - i < share ? nt - i : share;
+              if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+              tc_fence_after_sync();
+              constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
+              uint32_t w = smem_u32(smem + stage * SB);
+              const uint32_t h = h0 + slices * hrow;
+              for (int m = 0; m < n; ++m)
+                for (int u = 0; u < tail; ++u, w += 128 * C::TAIL)
+#pragma unroll
+                  for (int k = 0; k < KS; ++k)
+                    step(d + (i + m) * dn, umma_desc_k_narrow(w + k * 32, C::TAIL), umma_desc_k_narrow(w + kFewTile + k * 32, C::TAIL),
+                         umma_desc_k_sw128(h + (u * KS + k) * 32), r.np, (slices | u | k) ? 1u : 0u);
               umma_commit(&empty[stage]);
               advance();
             }
-            umma_commit(&acc2_full[g * 6 + b]);
+            umma_commit(&acc2_full[g * 2 + b]);
           }
         }
       }
@@ -511,7 +517,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         const uint32_t hrow = C::PARTS * r.np * 128;
         for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
           if ((i1 & 1) != g) continue;
-          const int j = i1 >> 1, b = j % acc.nA;
+          const int j = i1 >> 1, b = j & (acc.nbuf - 1);
           const int unit = u0 + (GLU ? q : 2 * q + (lane >> 4));  // of the run
           const int fl = unit * 16 + (lane & 15);           // hidden row of the run
           const int f = r.f0 + fl;
@@ -521,7 +527,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             bias = __ldg(b1 + f);
             if constexpr (GLU) bias_up = __ldg(b1 + e.F + f);
           }
-          ok = mbar_wait_bounded(&acc1_full[g * 2 + b], (j / acc.nA) & 1, status, kFewKernelId, kFewWaitNs);
+          ok = mbar_wait_bounded(&acc1_full[g * 2 + b], (j / acc.nbuf) & 1, status, kFewKernelId, kFewWaitNs);
           tc_fence_after_sync();
           const uint32_t base = lane_addr + acc.first(g, b);
           uint8_t* hcol = hbuf + r.h * 128 + (fl / C::BK) * hrow;
@@ -582,68 +588,68 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       off = 0;
       for (; ok && runs > 0; --runs) {
         again.next(plan, hrows, C::PARTS, C::UPS, off, r);
-        // product 2: this CTA's part of the expert's result.  Columns 128 i belong to group i % 2, so a cut
-        // run's later pieces are added by the thread that wrote the first.
+        // product 2: this CTA's part of the expert's result.  A group of tiles always belongs to the same epilogue
+        // group, so a cut run's later pieces are added by the thread that wrote the first.
         const int mine = (int)blockIdx.x - few_cta((long long)r.place * UE, walk.U, walk.G);
         float* dst = p.part + (long long)(plan.part0[r.place] + mine * r.tokens) * p.Op + q * 32 + lane;
-        for (int i = g; ok && i < nO; i += 2, ++j2) {
-          const int b = j2 % acc.nB;
-          ok = mbar_wait_bounded(&acc2_full[g * 6 + b], (j2 / acc.nB) & 1, status, kFewKernelId, kFewWaitNs);
+        for (int i0 = g * acc.tiles; ok && i0 < nO; i0 += 2 * acc.tiles, ++j2) {
+          const int b = j2 & (acc.nbuf - 1), nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
+          ok = mbar_wait_bounded(&acc2_full[g * 2 + b], (j2 / acc.nbuf) & 1, status, kFewKernelId, kFewWaitNs);
           tc_fence_after_sync();
-          const uint32_t base = lane_addr + acc.second(g, b);
-          for (int c = 0; c < r.tokens; c += 16) {
-            uint32_t v[16];
-            tmem_ld16(base + c, v);
-            if constexpr (FP32) {
-              uint32_t l[16];
-              tmem_ld16(base + r.np + c, l);
-              tmem_ld_wait();
+          for (int i = 0; i < nt; ++i) {
+            const uint32_t base = lane_addr + acc.second(g, b) + i * C::PARTS * r.np;
+            for (int c = 0; c < r.tokens; c += 16) {
+              uint32_t v[16];
+              tmem_ld16(base + c, v);
+              if constexpr (FP32) {
+                uint32_t l[16];
+                tmem_ld16(base + r.np + c, l);
+                tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(l[j]));
-            } else {
-              tmem_ld_wait();
-            }
+                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(l[j]));
+              } else {
+                tmem_ld_wait();
+              }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (c + j >= r.tokens) break;
-              float* at = dst + (long long)(c + j) * p.Op + i * 128;
-              float out = __uint_as_float(v[j]);
-              if (!r.first) out += *at;
-              *at = out;
+              for (int j = 0; j < 16; ++j) {
+                if (c + j >= r.tokens) break;
+                float* at = dst + (long long)(c + j) * p.Op + (i0 + i) * 128;
+                float out = __uint_as_float(v[j]);
+                if (!r.first) out += *at;
+                *at = out;
+              }
             }
           }
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&acc2_empty[g * 6 + b]);
+          if (lane == 0) mbar_arrive(&acc2_empty[g * 2 + b]);
         }
       }
     }
   } else if constexpr (FP32) {
     // ---------------------------------------------------------------- weights into tf32 parts
-    const int tid = threadIdx.x - 320;
+    const int tid = (threadIdx.x - 320) & 127, g = (threadIdx.x - 320) >> 7;   // two groups take stages in turn
+    int turn = 0;
     bool ok = true;
     auto part = [&](int bytes) {
-      if (!(ok = mbar_wait_bounded(&full[stage], phase, status, kFewKernelId, kFewWaitNs))) return;
-      uint8_t* w = smem + stage * SB + tid * 16;
-      constexpr int N = kFewTile / (C::SPLITTERS * 16);
-      float4 v[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (tid * 16 + i * C::SPLITTERS * 16 < bytes) v[i] = *(const float4*)(w + i * C::SPLITTERS * 16);
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (tid * 16 + i * C::SPLITTERS * 16 >= bytes) break;
-        float4 h, l;
-        split_tf32(v[i].x, h.x, l.x);
-        split_tf32(v[i].y, h.y, l.y);
-        split_tf32(v[i].z, h.z, l.z);
-        split_tf32(v[i].w, h.w, l.w);
-        *(float4*)(w + i * C::SPLITTERS * 16) = h;
-        *(float4*)(w + i * C::SPLITTERS * 16 + kFewTile) = l;
+      if (turn++ % 2 == g) {
+        ok = mbar_wait_bounded(&full[stage], phase, status, kFewKernelId, kFewWaitNs);
+        uint8_t* w = smem + stage * SB + tid * 16;
+#pragma unroll 4
+        for (int i = 0; i < bytes - tid * 16; i += 128 * 16) {
+          const float4 v = *(const float4*)(w + i);
+          float4 h, l;
+          split_tf32(v.x, h.x, l.x);
+          split_tf32(v.y, h.y, l.y);
+          split_tf32(v.z, h.z, l.z);
+          split_tf32(v.w, h.w, l.w);
+          *(float4*)(w + i) = h;
+          *(float4*)(w + i + kFewTile) = l;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&parted[stage]);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&parted[stage]);
       advance();
     };
     while (ok) {
@@ -660,8 +666,12 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       for (; ok && runs > 0; --runs) {
         again.next(plan, hrows, C::PARTS, C::UPS, off, r);
         const int slices = r.units / C::UPS, tail = r.units % C::UPS;
-        for (int i = 0; ok && i < nO; ++i)
-          for (int s = 0; ok && s < slices + (tail ? 1 : 0); ++s) part(s < slices ? kFewTile : tail * 128 * C::TAIL);
+        const int share = tail ? UPT / tail : 1;
+        for (int i0 = 0; ok && i0 < nO; i0 += acc.tiles) {
+          const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
+          for (int s = 0; ok && s < slices * nt; ++s) part(kFewTile);
+          for (int i = 0; ok && tail && i < nt; i += share) part((nt - i < share ? nt - i : share) * tail * 128 * C::TAIL);
+        }
       }
     }
   }
