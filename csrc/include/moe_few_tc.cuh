@@ -74,17 +74,6 @@ struct FewTc {
   static __host__ __device__ int stage_bytes(int Tp) { return PARTS * kFewTile + packs(Tp) * PARTS * Tp * 128; }
 };
 
-// fp32 as two tf32 numbers of 11 significant bits, rounded to nearest; what
-// would round to infinity is cut instead, and an infinity has no low part.
-__device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
-  const uint32_t b = __float_as_uint(v);
-  uint32_t h = (b + 0x1000u) & ~0x1fffu;
-  if ((h & 0x7f800000u) == 0x7f800000u) h = b & ~0x1fffu;
-  hi = __uint_as_float(h);
-  const float l = v == hi ? 0.f : v - hi;
-  lo = l != l ? l : __uint_as_float((__float_as_uint(l) + 0x1000u) & ~0x1fffu);
-}
-
 // The plan that every CTA makes of the routed tokens; mask is zero on entry.
 struct FewPlan {
   unsigned long long mask[kFewExperts + 1];  // by expert: its tokens

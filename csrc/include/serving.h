@@ -94,6 +94,18 @@ struct LinearParams {
   int bf16, out_bf16, res_bf16;
 };
 
-void launch_linear(const LinearParams& p, cudaStream_t s);
+// How a product runs, and the device memory that it needs besides.
+struct LinearPlan {
+  int Mp, ranks, stages;   // rows of x of a tile, CTAs that share K, stages
+  int pack_x, pack_w;      // rows that TMA cannot read are copied to aligned ones first
+  int packed_stride;
+  long long x_bytes, w_bytes;
+  long long bytes() const { return x_bytes + w_bytes; }
+};
+
+LinearPlan plan_linear(const LinearParams& p);
+void launch_linear(const LinearParams& p, const LinearPlan& plan, void* workspace, cudaStream_t s);
+
+int serving_sm_count();   // of the current device
 
 }  // namespace raiccl

@@ -36,6 +36,17 @@ __device__ __forceinline__ float serving_act(float z, int act) {
 
 __device__ __forceinline__ float serving_swiglu(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
 
+// fp32 as two tf32 numbers of 11 significant bits, rounded to nearest; what
+// would round to infinity is cut instead, and an infinity has no low part.
+__device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
+  const uint32_t b = __float_as_uint(v);
+  uint32_t h = (b + 0x1000u) & ~0x1fffu;
+  if ((h & 0x7f800000u) == 0x7f800000u) h = b & ~0x1fffu;
+  hi = __uint_as_float(h);
+  const float l = v == hi ? 0.f : v - hi;
+  lo = l != l ? l : __uint_as_float((__float_as_uint(l) + 0x1000u) & ~0x1fffu);
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

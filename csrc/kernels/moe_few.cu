@@ -298,7 +298,7 @@ static void launch_rows(const FewExpertParams& p, float* h, float* y, cudaStream
 // ---------------------------------------------------------------------------
 // Launch
 // ---------------------------------------------------------------------------
-static int sm_count() {
+int serving_sm_count() {
   static std::atomic<int> n[64];
   const int dev = current_device();
   int v = n[dev].load();
@@ -328,7 +328,7 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
     r.b_bytes = up256((long long)pairs * p.O * 4);
     return r;
   }
-  r.grid = sm_count();
+  r.grid = serving_sm_count();
   r.Op = (p.O + 127) / 128 * 128;
   r.Tp = (p.T + 15) / 16 * 16;
   const int UE = (p.F + 15) / 16, ups = 128 / eb / 16;

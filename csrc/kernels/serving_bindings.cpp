@@ -244,7 +244,10 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   p.bf16 = x.scalar_type() == torch::kBFloat16;
   p.out_bf16 = res.scalar_type() == torch::kBFloat16;
   p.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
-  raiccl::launch_linear(p, at::cuda::getCurrentCUDAStream());
+  const raiccl::LinearPlan plan = raiccl::plan_linear(p);
+  torch::Tensor ws;
+  if (plan.bytes() > 0) ws = torch::empty({plan.bytes()}, x.options().dtype(torch::kUInt8));
+  raiccl::launch_linear(p, plan, plan.bytes() > 0 ? ws.data_ptr() : nullptr, at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return res;
 }
