@@ -1,0 +1,362 @@
+// Dense product for many rows: persistent CTA pairs (tcgen05 cta_group::2), a
+// 256 x BN tile of sums per pair, two accumulators in TMEM so that one tile's
+// epilogue runs under the next tile's products.
+//
+// Each CTA of a pair stages its 128 rows of x and half of the tile's BN weight
+// rows; the pair's first CTA issues M = 256 products that read both.  SwiGLU:
+// the first CTA's half are gate rows and the second's the up rows of the same
+// outputs, so a thread finds both in its accumulator row and the weights need
+// no other order than gate rows, then up rows.
+//
+// fp32: x and w come as two tf32 parts each (linear_split_kernel), h + l.  The
+// tensor core cuts what does not fit its accumulator, which drifts with the
+// length of the chain (2e-6 of the result for each 1024 of K), so K is taken
+// 256 at a time, each into an accumulator of its own; the epilogue warps add
+// the chains in registers, rounded to nearest, while the next one runs.  A
+// stage holds both parts of both operands for the three products l h', h l',
+// h h': two thirds of the bytes that three walks over K would fetch.
+//
+// Tiles go by groups of eight row tiles, so that the pairs at work share rows
+// of x and of w in L2.  Every wait is bounded.
+#pragma once
+
+#include "serving.h"
+#include "serving_device.cuh"
+#include "sm100_ptx.cuh"
+
+namespace raiccl {
+
+constexpr int kDenseThreads = 320;         // TMA, MMA, eight epilogue warps
+constexpr int kDenseKernelId = 620;
+constexpr int kDenseGroup = 8;
+constexpr int kDenseChain = 8;             // fp32: 128-byte steps of K of a chain
+constexpr unsigned long long kDenseWaitNs = 2000000000ull;
+
+struct LinearDenseParams {
+  LinearParams l;
+  int mt, nt;      // tiles
+  int vec_out, vec_res, vec_bias;   // rows may be read and written 16 bytes at a time
+};
+
+template <int BN, bool FP32>
+struct LinearDense {
+  static constexpr int BK = FP32 ? 32 : 64;
+  static constexpr int HALF = BN / 2;
+  static constexpr int PARTS = FP32 ? 2 : 1;
+  static constexpr int X_BYTES = 128 * 128, W_BYTES = HALF * 128;
+  static constexpr int STAGE = PARTS * (X_BYTES + W_BYTES);   // x parts, then w parts
+  static constexpr int STAGES_FIT = 216 * 1024 / STAGE;
+  static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
+  static constexpr int SMEM = 1024 + STAGES * STAGE;
+  static constexpr int COLS = 2 * BN;
+};
+
+__device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* desc, uint32_t bar_cluster_addr, int32_t x, int32_t y,
+                                                 int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(desc), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void dense_tile(const LinearDenseParams& p, int t, int& mb, int& nb) {
+  const int per = kDenseGroup * p.nt, g = t / per, first = g * kDenseGroup;
+  const int rows = p.mt - first < kDenseGroup ? p.mt - first : kDenseGroup;
+  const int local = t - g * per;
+  mb = first + local % rows;
+  nb = local / rows;
+}
+
+// Sixteen consecutive outputs of one row: residual, rounding, store.
+__device__ __forceinline__ void dense_store16(const LinearDenseParams& p, long long m, int n, float (&v)[16]) {
+  const LinearParams& l = p.l;
+  const bool whole = n + 16 <= l.N;
+  if (l.residual) {
+    const long long at = m * l.res_stride + n;
+    if (whole && p.vec_res) {
+      if (l.res_bf16) {
+        const uint4* r = (const uint4*)((const __nv_bfloat16*)l.residual + at);
+        const uint4 a = r[0], b = r[1];
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[2 * i] += __uint_as_float(w[i] << 16);
+          v[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
+        }
+      } else {
+        const float4* r = (const float4*)((const float*)l.residual + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 a = r[i];
+          v[4 * i] += a.x; v[4 * i + 1] += a.y; v[4 * i + 2] += a.z; v[4 * i + 3] += a.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (n + i < l.N) v[i] += load_elem(l.residual, at + i, l.res_bf16);
+    }
+  }
+  const long long at = m * l.out_stride + n;
+  if (whole && p.vec_out) {
+    if (l.out_bf16) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *(const uint32_t*)&h;
+      }
+      uint4* o = (uint4*)((__nv_bfloat16*)l.out + at);
+      o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+      o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+      float4* o = (float4*)((float*)l.out + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (n + i < l.N) store_elem(l.out, at + i, v[i], l.out_bf16);
+  }
+}
+
+// bias[n .. n + 16), zeros behind the last
+__device__ __forceinline__ void dense_bias16(const float* bias, int n, int N, int vec, float (&b)[16]) {
+  if (bias == nullptr) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) b[i] = 0.f;
+  } else if (n + 16 <= N && vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = __ldg((const float4*)(bias + n) + i);
+      b[4 * i] = a.x; b[4 * i + 1] = a.y; b[4 * i + 2] = a.z; b[4 * i + 3] = a.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) b[i] = n + i < N ? __ldg(bias + n + i) : 0.f;
+  }
+}
+
+template <int BN, bool FP32, bool GLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kDenseThreads, 1)
+linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, LinearDenseParams p,
+                    DeviceStatus* status) {
+  using C = LinearDense<BN, FP32>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ uint32_t tmem_slot;
+  const LinearParams& l = p.l;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 16); }
+    mbar_init(&drained, 1);
+    fence_mbarrier_init();
+    tma_prefetch_desc(&tx); tma_prefetch_desc(&tw);
+  }
+  if (warp == 1) { tmem_alloc_pair(&tmem_slot, C::COLS); tmem_relinquish_pair(); }
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  constexpr int W = GLU ? BN / 2 : BN;      // outputs of a tile
+  const int KB = (l.K + C::BK - 1) / C::BK;
+  const int chain = FP32 ? kDenseChain : KB;             // 128-byte steps of K of an accumulator
+  const int tiles = p.mt * p.nt;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads, both CTAs
+    if (elect_one_sync()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += npairs) {
+        int mb, nb;
+        dense_tile(p, t, mb, nb);
+        const int xrow = mb * 256 + (int)rank * 128;
+        const int wrow = GLU ? nb * W + (int)rank * l.N : nb * W + (int)rank * C::HALF;
+        for (int kb = 0; kb < KB; ++kb) {
+          if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE);
+          const uint32_t lead = mapa_shared(smem_u32(&full[stage]), 0);
+          uint8_t* s = smem + stage * C::STAGE;
+#pragma unroll
+          for (int part = 0; part < C::PARTS; ++part) {
+            tma_load_3d_pair(s + part * C::X_BYTES, &tx, lead, kb * C::BK, xrow, part);
+            tma_load_3d_pair(s + C::PARTS * C::X_BYTES + part * C::W_BYTES, &tw, lead, kb * C::BK, wrow, part);
+          }
+          if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products, first CTA
+    if (rank == 0 && elect_one_sync()) {
+      int stage = 0, iter = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      constexpr uint32_t idesc = umma_idesc(FP32 ? 2u : 1u, 256, BN);
+      for (int t = pair; ok && t < tiles; t += npairs) {
+        for (int k0 = 0; ok && k0 < KB; k0 += chain, ++iter) {
+          const int steps = k0 + chain < KB ? chain : KB - k0;
+          const int b = iter & 1;
+          if (!(ok = mbar_wait_bounded(&acc_empty[b], ((iter >> 1) & 1) ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
+          tc_fence_after_sync();
+          const uint32_t d = tmem + b * BN;
+          for (int kb = 0; kb < steps; ++kb) {
+            if (!(ok = mbar_wait_bounded(&full[stage], phase, status, kDenseKernelId, kDenseWaitNs))) break;
+            tc_fence_after_sync();
+            const uint32_t x = smem_u32(smem + stage * C::STAGE), w = x + C::PARTS * C::X_BYTES;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint64_t a = umma_desc_k_sw128(x + k * 32), bb = umma_desc_k_sw128(w + k * 32);
+              if constexpr (FP32) {
+                umma_tf32_pair(d, umma_desc_k_sw128(x + C::X_BYTES + k * 32), bb, idesc, (kb | k) ? 1u : 0u);
+                umma_tf32_pair(d, a, umma_desc_k_sw128(w + C::W_BYTES + k * 32), idesc, 1u);
+                umma_tf32_pair(d, a, bb, idesc, 1u);
+              } else {
+                umma_f16_pair(d, a, bb, idesc, (kb | k) ? 1u : 0u);
+              }
+            }
+            const uint32_t e = smem_u32(&empty[stage]);
+            umma_commit_pair(mapa_shared(e, 0));
+            umma_commit_pair(mapa_shared(e, 1));
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+          }
+          if (!ok) break;
+          const uint32_t f = smem_u32(&acc_full[b]);
+          umma_commit_pair(mapa_shared(f, 0));
+          umma_commit_pair(mapa_shared(f, 1));
+        }
+      }
+      umma_commit_pair(mapa_shared(smem_u32(&drained), 0));
+      mbar_wait_bounded(&drained, 0, status, kDenseKernelId, kDenseWaitNs);
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue, both CTAs
+    const int q = warp & 3, side = (warp - 2) >> 2;   // TMEM lanes 32 q ..; half of the tile's columns
+    constexpr int OUT = W / 2;                        // outputs of a thread
+    int iter = 0;
+    bool ok = true;
+    auto finish = [&](long long m, int n, const float (&z)[16], const float (&zu)[16]) {
+      float bias[16], up[16], v[16];
+      dense_bias16(l.bias, n, l.N, p.vec_bias, bias);
+      if constexpr (GLU) dense_bias16(l.bias ? l.bias + l.N : nullptr, n, l.N, p.vec_bias, up);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        if constexpr (GLU) v[i] = serving_swiglu(z[i] + bias[i], zu[i] + up[i]);
+        else v[i] = serving_act(z[i] + bias[i], l.act);
+      }
+      if (m < l.M && n < l.N) dense_store16(p, m, n, v);
+      __syncwarp();
+    };
+    for (int t = pair; ok && t < tiles; t += npairs) {
+      int mb, nb;
+      dense_tile(p, t, mb, nb);
+      const long long m = (long long)mb * 256 + rank * 128 + q * 32 + lane;
+      const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
+      const int c0 = side * OUT, n0 = nb * W + c0;
+      if constexpr (FP32) {
+        float sum[OUT], sum_up[GLU ? OUT : 16];
+#pragma unroll
+        for (int i = 0; i < OUT; ++i) sum[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < (GLU ? OUT : 16); ++i) sum_up[i] = 0.f;
+        for (int k0 = 0; k0 < KB; k0 += chain, ++iter) {
+          const int b = iter & 1;
+          if (!(ok = mbar_wait_warp(&acc_full[b], (iter >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
+          tc_fence_after_sync();
+          const uint32_t base = lanes + b * BN + c0;
+#pragma unroll
+          for (int c = 0; c < OUT; c += 16) {
+            uint32_t r[16];
+            tmem_ld16(base + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[c + i] += __uint_as_float(r[i]);
+            if constexpr (GLU) {
+              tmem_ld16(base + C::HALF + c, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sum_up[c + i] += __uint_as_float(r[i]);
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[b]), 0));
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < OUT; c += 16) {
+          float z[16], zu[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) { z[i] = sum[c + i]; zu[i] = sum_up[GLU ? c + i : i]; }
+          finish(m, n0 + c, z, zu);
+        }
+      } else {
+        const int b = iter & 1;
+        if (!(ok = mbar_wait_warp(&acc_full[b], (iter >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
+        ++iter;
+        tc_fence_after_sync();
+        const uint32_t base = lanes + b * BN + c0;
+#pragma unroll 1
+        for (int c = 0; c < OUT; c += 16) {
+          if (n0 + c >= l.N) break;
+          uint32_t r[16], u[16];
+          tmem_ld16(base + c, r);
+          if constexpr (GLU) tmem_ld16(base + C::HALF + c, u);
+          tmem_ld_wait();
+          float z[16], zu[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) { z[i] = __uint_as_float(r[i]); zu[i] = GLU ? __uint_as_float(u[i]) : 0.f; }
+          finish(m, n0 + c, z, zu);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[b]), 0));
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  cluster_sync_all();   // both CTAs have finished before the pair frees its memory
+  __syncwarp();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc_pair(tmem, C::COLS);
+}
+
+// fp32 rows as two tf32 parts, [2][rows, packed]: what linear_dense_kernel reads.
+__global__ void __launch_bounds__(256) linear_split_kernel(const float* src, long long stride, float* dst, int packed, long long rows,
+                                                           int K, int vec) {
+  griddep_wait();
+  griddep_launch_dependents();
+  float* low = dst + rows * packed;
+  if (vec) {   // four at a time over all rows
+    const long long per = K / 4, n = rows * per;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+      const long long r = i / per, k = (i - r * per) * 4;
+      const float4 v = *(const float4*)(src + r * stride + k);
+      float4 h, lo;
+      split_tf32(v.x, h.x, lo.x);
+      split_tf32(v.y, h.y, lo.y);
+      split_tf32(v.z, h.z, lo.z);
+      split_tf32(v.w, h.w, lo.w);
+      *(float4*)(dst + r * packed + k) = h;
+      *(float4*)(low + r * packed + k) = lo;
+    }
+  } else {
+    for (long long r = blockIdx.x; r < rows; r += gridDim.x)
+      for (int k = threadIdx.x; k < K; k += 256) split_tf32(src[r * stride + k], dst[r * packed + k], low[r * packed + k]);
+  }
+}
+
+}  // namespace raiccl

@@ -13,7 +13,12 @@
 //
 // fp32: eight warps split the staged tiles into two tf32 parts of 11 bits (see
 // split_tf32), in place and into a short ring for the weights' low parts;
-// h h' + h l' + l h' is the product to 2^-21.
+// h h' + h l' + l h' is the product to 2^-21.  The tensor core cuts what does
+// not fit its accumulator instead of rounding, which drifts toward zero with
+// the length of the chain (2e-6 of the result for each 1024 of K): every 512 of
+// K the sums go to registers and are added there, rounded to nearest, while the
+// next 512 run into the other of two accumulators.  bf16 results are rounded to
+// 2^-8, where the drift of a whole K does not show.
 #pragma once
 
 #include "serving.h"
@@ -23,8 +28,9 @@
 namespace raiccl {
 
 constexpr int kRowsTile = 128 * 128;       // bytes of a weight tile: 128 rows of 128 bytes
+constexpr int kRowsPack = 2;               // 128-byte steps of K in a stage: a stage costs its waits and its commit, 0.15 us
 constexpr int kRowsMaxStages = 12;
-constexpr int kRowsLow = 3;                // weight tiles of low parts in flight
+constexpr int kRowsChain = 8;              // fp32: stages into one accumulator
 constexpr int kRowsKernelId = 610;
 constexpr unsigned long long kServingWaitNs = 2000000000ull;
 
@@ -32,6 +38,8 @@ struct LinearRowsParams {
   LinearParams l;
   int Mp;        // rows of x of a tile: a multiple of 16, at most 256 (fp32: 128)
   int stages;
+  int vec_out;   // four outputs of a row may be written at once
+  int low;       // fp32: stages whose low parts of the weights are kept, at most as many as stages
 };
 
 template <bool FP32>
@@ -39,18 +47,18 @@ struct LinearRows {
   static constexpr int PARTS = FP32 ? 2 : 1;
   static constexpr int BK = FP32 ? 32 : 64;          // elements of 128 bytes
   static constexpr int THREADS = FP32 ? 448 : 192;
-  static __host__ __device__ int stage_bytes(int Mp) { return kRowsTile + PARTS * Mp * 128; }
-  static __host__ __device__ int low_bytes() { return FP32 ? kRowsLow * kRowsTile : 0; }
+  static __host__ __device__ int stage_bytes(int Mp) { return kRowsPack * (kRowsTile + PARTS * Mp * 128); }   // weight tiles, then x tiles (h rows, l rows)
 };
 
-template <bool FP32, bool GLU>
+// MP: rows of x of a tile where the sums are kept in registers (fp32), else 0.
+template <bool FP32, bool GLU, int MP>
 __global__ void __launch_bounds__(LinearRows<FP32>::THREADS)
 linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, LinearRowsParams p,
                    DeviceStatus* status) {
   using C = LinearRows<FP32>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[kRowsMaxStages], empty[kRowsMaxStages], parted[kRowsMaxStages], done;
+  __shared__ uint64_t full[kRowsMaxStages], empty[kRowsMaxStages], parted[kRowsMaxStages], done, acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   const LinearParams& l = p.l;
   const int SB = C::stage_bytes(p.Mp), S = p.stages;
@@ -62,14 +70,15 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   constexpr int W = GLU ? 64 : 128;                     // output columns of a tile
   const int n0 = (int)(blockIdx.x / ranks) * W;
   const long long m0 = (long long)blockIdx.y * p.Mp;
-  const int cols0 = C::PARTS * p.Mp;
-  const int cols = cols0 <= 32 ? 32 : cols0 <= 64 ? 64 : cols0 <= 128 ? 128 : 256;
+  const int cols0 = FP32 ? 4 * p.Mp : p.Mp;             // fp32: two accumulators of [h | l] columns
+  const int cols = cols0 <= 32 ? 32 : cols0 <= 64 ? 64 : cols0 <= 128 ? 128 : cols0 <= 256 ? 256 : 512;
   const int KB = (l.K + C::BK - 1) / C::BK;
   const int kb0 = (int)((long long)KB * rank / ranks), kb1 = (int)((long long)KB * (rank + 1) / ranks);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], 4); }
     mbar_init(&done, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
     fence_mbarrier_init();
     tma_prefetch_desc(&tx); tma_prefetch_desc(&tw);
   }
@@ -80,141 +89,198 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   const uint32_t tmem = tmem_slot;
   griddep_wait();
   griddep_launch_dependents();
+  [[maybe_unused]] float acc[MP > 0 ? MP : 1];
+  [[maybe_unused]] bool added = true;
+#pragma unroll
+  for (int i = 0; i < MP; ++i) acc[i] = 0.f;
+
+  const int steps = kb1 - kb0;
+  const int count = (steps + kRowsPack - 1) / kRowsPack;   // stages' worth
+  int stage = 0;
+  uint32_t phase = 0;
+  auto advance = [&]() { if (++stage == S) { stage = 0; phase ^= 1u; } };
 
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     if (elect_one_sync()) {
-      for (int i = 0; kb0 + i < kb1; ++i) {
-        const int s = i % S;
-        if (!mbar_wait_bounded(&empty[s], ((i / S) & 1) ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
-        uint8_t* w = smem + s * SB;
-        const int k = (kb0 + i) * C::BK;
-        mbar_arrive_expect_tx(&full[s], kRowsTile + p.Mp * 128);
-        if constexpr (GLU) {
-          tma_load_2d(w, &tw, &full[s], k, n0);
-          tma_load_2d(w + kRowsTile / 2, &tw, &full[s], k, l.N + n0);
-        } else {
-          tma_load_2d(w, &tw, &full[s], k, n0);
+      for (int i = 0; i < count; ++i, advance()) {
+        if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
+        uint8_t* w = smem + stage * SB;
+        uint8_t* x = w + kRowsPack * kRowsTile;
+        const int n = steps - i * kRowsPack < kRowsPack ? steps - i * kRowsPack : kRowsPack;
+        int k = (kb0 + i * kRowsPack) * C::BK;
+        mbar_arrive_expect_tx(&full[stage], n * (kRowsTile + p.Mp * 128));
+        for (int j = 0; j < n; ++j, k += C::BK, w += kRowsTile, x += C::PARTS * p.Mp * 128) {
+          tma_load_2d(w, &tw, &full[stage], k, n0);
+          if constexpr (GLU) tma_load_2d(w + kRowsTile / 2, &tw, &full[stage], k, l.N + n0);
+          tma_load_2d(x, &tx, &full[stage], k, (int)m0);
         }
-        tma_load_2d(w + kRowsTile, &tx, &full[s], k, (int)m0);
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products
     if (elect_one_sync()) {
       uint64_t* ready = FP32 ? parted : full;
-      for (int i = 0; kb0 + i < kb1; ++i) {
-        const int s = i % S;
-        if (!mbar_wait_bounded(&ready[s], (i / S) & 1, status, kRowsKernelId, kServingWaitNs)) break;
+      int lo = 0;
+      for (int i = 0; i < count; ++i, advance()) {
+        if (FP32 && i % kRowsChain == 0) {
+          const int c = i / kRowsChain;
+          if (!mbar_wait_bounded(&acc_empty[c & 1], ((c >> 1) & 1) ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
+        }
+        if (!mbar_wait_bounded(&ready[stage], phase, status, kRowsKernelId, kServingWaitNs)) break;
         tc_fence_after_sync();
-        const uint32_t w = smem_u32(smem + s * SB), x = w + kRowsTile, wl = smem_u32(low) + i % kRowsLow * kRowsTile;
+        const uint32_t d = tmem + (FP32 ? (i / kRowsChain & 1) * 2 * p.Mp : 0);
+        uint32_t w = smem_u32(smem + stage * SB), x = w + kRowsPack * kRowsTile, wl = smem_u32(low) + lo * kRowsPack * kRowsTile;
+        const int n = steps - i * kRowsPack < kRowsPack ? steps - i * kRowsPack : kRowsPack;
+        for (int j = 0; j < n; ++j, w += kRowsTile, x += C::PARTS * p.Mp * 128, wl += kRowsTile) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint64_t a = umma_desc_k_sw128(w + k * 32), b = umma_desc_k_sw128(x + k * 32);
-          const uint32_t more = (i | k) ? 1u : 0u;
-          if constexpr (FP32) {
-            umma_tf32(tmem, a, b, umma_idesc(2u, 128, 2 * p.Mp), more);
-            umma_tf32(tmem, umma_desc_k_sw128(wl + k * 32), b, umma_idesc(2u, 128, p.Mp), 1u);
-          } else {
-            umma_f16(tmem, a, b, umma_idesc(1u, 128, p.Mp), more);
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t a = umma_desc_k_sw128(w + k * 32), b = umma_desc_k_sw128(x + k * 32);
+            const uint32_t more = ((FP32 ? i % kRowsChain : i) | j | k) ? 1u : 0u;
+            if constexpr (FP32) {
+              umma_tf32(d, a, b, umma_idesc(2u, 128, 2 * p.Mp), more);
+              umma_tf32(d, umma_desc_k_sw128(wl + k * 32), b, umma_idesc(2u, 128, p.Mp), 1u);
+            } else {
+              umma_f16(d, a, b, umma_idesc(1u, 128, p.Mp), more);
+            }
           }
         }
-        umma_commit(&empty[s]);
+        umma_commit(&empty[stage]);
+        if (FP32 && (i % kRowsChain == kRowsChain - 1 || i + 1 == count)) umma_commit(&acc_full[i / kRowsChain & 1]);
+        if (++lo == p.low) lo = 0;
       }
       umma_commit(&done);
+    }
+  } else if (FP32 && warp < 6) {
+    // ---------------------------------------------------------------- fp32: a chain's sums into registers
+    const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    for (int c = 0; c * kRowsChain < count; ++c) {
+      added = mbar_wait_warp(&acc_full[c & 1], (c >> 1) & 1, status, kRowsKernelId, kServingWaitNs);
+      if (!added) break;
+      tc_fence_after_sync();
+#pragma unroll
+      for (int i = 0; i < MP; i += 16) {
+        uint32_t v[16], u[16];
+        tmem_ld16(base + (c & 1) * 2 * MP + i, v);
+        tmem_ld16(base + (c & 1) * 2 * MP + MP + i, u);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[i + j] += __uint_as_float(v[j]) + __uint_as_float(u[j]);
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[c & 1]);
     }
   } else if (FP32 && warp >= 6) {
     // ---------------------------------------------------------------- tf32 parts: two groups take stages in turn
     const int tid = (threadIdx.x - 192) & 127, g = (threadIdx.x - 192) >> 7;
-    for (int i = g; kb0 + i < kb1; i += 2) {
-      const int s = i % S;
-      if (!mbar_wait_bounded(&full[s], (i / S) & 1, status, kRowsKernelId, kServingWaitNs)) break;
-      if (i >= kRowsLow) {  // the products that read this tile of low parts
-        const int j = i - kRowsLow;
-        if (!mbar_wait_bounded(&empty[j % S], (j / S) & 1, status, kRowsKernelId, kServingWaitNs)) break;
-      }
-      uint8_t* w = smem + s * SB;
-      uint8_t* wl = low + i % kRowsLow * kRowsTile;
-      auto part = [&](float4* at, float4* lo_at) {
-        const float4 v = *at;
-        float4 h, lo;
-        split_tf32(v.x, h.x, lo.x);
-        split_tf32(v.y, h.y, lo.y);
-        split_tf32(v.z, h.z, lo.z);
-        split_tf32(v.w, h.w, lo.w);
-        *at = h;
-        *lo_at = lo;
-      };
-#pragma unroll 4
-      for (int o = tid * 16; o < kRowsTile; o += 128 * 16) part((float4*)(w + o), (float4*)(wl + o));
-      uint8_t* x = w + kRowsTile;
-      for (int o = tid * 16; o < p.Mp * 128; o += 128 * 16) part((float4*)(x + o), (float4*)(x + p.Mp * 128 + o));
+    int lo = 0, old = 0;          // slot of low parts; stage of the products that read it last, and their phase
+    uint32_t old_phase = 0;
+    for (int i = 0; i < count; ++i, advance()) {
+      const int slot = lo;
+      if (++lo == p.low) lo = 0;
+      const int was = old;
+      const uint32_t was_phase = old_phase;
+      if (i >= p.low && ++old == S) { old = 0; old_phase ^= 1u; }
+      if ((i & 1) != g) continue;
+      if (!mbar_wait_warp(&full[stage], phase, status, kRowsKernelId, kServingWaitNs)) break;
+      if (i >= p.low && !mbar_wait_warp(&empty[was], was_phase, status, kRowsKernelId, kServingWaitNs)) break;
+      uint8_t* w = smem + stage * SB;
+      uint8_t* x = w + kRowsPack * kRowsTile;
+      const int n = steps - i * kRowsPack < kRowsPack ? steps - i * kRowsPack : kRowsPack;
+      split_tile(w, low + slot * kRowsPack * kRowsTile, tid, n * kRowsTile);
+      for (int j = 0; j < n; ++j, x += C::PARTS * p.Mp * 128) split_tile(x, x + p.Mp * 128, tid, p.Mp * 128);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&parted[s]);
+      if (lane == 0) mbar_arrive(&parted[stage]);
     }
   }
   __syncwarp();
   // -------------------------------------------------------------------- the CTA's sums to shared memory
   float* const sums = (float*)smem;   // [Mp][128], over the stages
-  const bool ok = mbar_wait_bounded(&done, 0, status, kRowsKernelId, kServingWaitNs);
+  const bool ok = mbar_wait_warp(&done, 0, status, kRowsKernelId, kServingWaitNs) && added;
   const int rows = (int)(l.M - m0 < p.Mp ? l.M - m0 : p.Mp);
   __syncthreads();                    // every role has left the stages
+  __syncwarp();
   if (warp >= 2 && warp < 6) {
     const int q = warp & 3;
-    tc_fence_after_sync();
-    const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);
-    for (int c = 0; c < rows; c += 16) {
-      uint32_t v[16];
-      tmem_ld16(base + c, v);
-      if constexpr (FP32) {
-        uint32_t u[16];
-        tmem_ld16(base + p.Mp + c, u);
+    if constexpr (FP32) {
+#pragma unroll
+      for (int i = 0; i < MP; ++i)
+        if (i < rows) sums[i * 128 + q * 32 + lane] = acc[i];
+    } else {
+      tc_fence_after_sync();
+      const uint32_t base = tmem + ((uint32_t)(q * 32) << 16);
+      for (int c = 0; c < rows; c += 16) {
+        uint32_t v[16];
+        tmem_ld16(base + c, v);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
-      } else {
-        tmem_ld_wait();
+        for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + q * 32 + lane] = kb0 < kb1 ? __uint_as_float(v[j]) : 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + q * 32 + lane] = kb0 < kb1 ? __uint_as_float(v[j]) : 0.f;
+      tc_fence_before_sync();
     }
-    tc_fence_before_sync();
   }
+  __syncwarp();
   if (ranks > 1) cluster_sync_all();
   else __syncthreads();
+  __syncwarp();
   tc_fence_after_sync();
   if (warp == 1) tmem_dealloc(tmem, cols);
   // -------------------------------------------------------------------- add the cluster's sums, finish
   if (ok) {
     const uint32_t own = smem_u32(sums);
-    auto total = [&](int at) {
-      if (ranks == 1) return sums[at];
-      float v = 0.f;
+    // four columns at a time, added over the cluster in rank order
+    auto total = [&](int at, float (&v)[4]) {
+      if (ranks == 1) {
+        const float4 a = *(const float4*)(sums + at);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        return;
+      }
+      v[0] = v[1] = v[2] = v[3] = 0.f;
 #pragma unroll 4
       for (uint32_t r = 0; r < ranks; ++r) {
-        float a;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a) : "r"(mapa_shared(own + at * 4, r)));
-        v += a;
+        float a, b, c, d;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(a), "=f"(b), "=f"(c), "=f"(d) : "r"(mapa_shared(own + at * 4, r)));
+        v[0] += a; v[1] += b; v[2] += c; v[3] += d;
       }
-      return v;
     };
-    for (int i = (int)rank * C::THREADS + threadIdx.x; i < rows * W; i += (int)ranks * C::THREADS) {
+    for (int i = ((int)rank * C::THREADS + threadIdx.x) * 4; i < rows * W; i += (int)ranks * C::THREADS * 4) {
       const int m = i / W, c = i % W, n = n0 + c;
       if (n >= l.N) continue;
-      float v = total(m * 128 + c);
-      if (l.bias) v += __ldg(l.bias + n);
-      if constexpr (GLU) {
-        float up = total(m * 128 + 64 + c);
-        if (l.bias) up += __ldg(l.bias + l.N + n);
-        v = serving_swiglu(v, up);
-      } else {
-        v = serving_act(v, l.act);
+      float v[4], up[4];
+      total(m * 128 + c, v);
+      if constexpr (GLU) total(m * 128 + 64 + c, up);
+      const bool whole = n + 4 <= l.N;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = whole || n + j < l.N;
+        if (l.bias && in) v[j] += __ldg(l.bias + n + j);
+        if constexpr (GLU) {
+          if (l.bias && in) up[j] += __ldg(l.bias + l.N + n + j);
+          v[j] = serving_swiglu(v[j], up[j]);
+        } else {
+          v[j] = serving_act(v[j], l.act);
+        }
+        if (l.residual && in) v[j] += load_elem(l.residual, (m0 + m) * l.res_stride + n + j, l.res_bf16);
       }
-      if (l.residual) v += load_elem(l.residual, (m0 + m) * l.res_stride + n, l.res_bf16);
-      store_elem(l.out, (m0 + m) * l.out_stride + n, v, l.out_bf16);
+      const long long at = (m0 + m) * l.out_stride + n;
+      if (whole && p.vec_out) {
+        if (l.out_bf16) {
+          const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+          *(uint2*)((__nv_bfloat16*)l.out + at) = make_uint2(*(const uint32_t*)&a, *(const uint32_t*)&b);
+        } else {
+          *(float4*)((float*)l.out + at) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (whole || n + j < l.N) store_elem(l.out, at + j, v[j], l.out_bf16);
+      }
     }
   }
+  __syncwarp();
   if (ranks > 1) cluster_sync_all();   // nobody leaves while its sums may be read
 }
 

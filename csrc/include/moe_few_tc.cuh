@@ -33,7 +33,10 @@
 //
 // fp32 weights are split into two tf32 parts of 11 bits each in shared memory,
 // h + l; x and the activations too.  h h' + h l' + l h' is the product to 2^-21:
-// the tokens' parts are stacked as 2N columns, so that is two instructions.
+// the tokens' parts are stacked as 2N columns, so that is two instructions.  The
+// tensor core cuts what does not fit its accumulator, which drifts with the
+// length of the chain (2e-6 of the result for each 1024 of K), so product 1 of
+// fp32 runs into up to four accumulators in turn along K, added in registers.
 #pragma once
 
 #include "serving.h"
@@ -196,16 +199,29 @@ struct FewWalk {
   }
 };
 
-// Accumulators in TMEM for two epilogue groups, two buffers each where 512
-// columns allow: of product 1 one tile (n1 columns), of product 2 a group of
-// `tiles` tiles of 128 outputs, so that a few tokens' tiles share a hand-over.
+// Accumulators in TMEM, n1 columns each, for one or two epilogue groups with
+// one or two sets of buffers: `chains` of product 1 for one tile (fp32 cuts K
+// into so many), and of product 2 `tiles` tiles of 128 outputs, so that a few
+// tokens' tiles share a hand-over.  At most 512 columns in all.
 struct FewAcc {
-  int n1, nbuf, tiles;
-  __device__ explicit FewAcc(int n1_) : n1(n1_), nbuf(n1_ <= 64 ? 2 : 1), tiles(n1_ <= 16 ? 4 : n1_ <= 32 ? 2 : 1) {}
-  __device__ uint32_t first(int g, int b) const { return (g * nbuf + b) * n1; }
-  __device__ uint32_t second(int g, int b) const { return (2 * nbuf + (g * nbuf + b) * tiles) * n1; }
+  int n1, groups, nbuf, chains, tiles;
+  __device__ FewAcc(int n1_, bool fp32) : n1(n1_) {
+    if (fp32) {
+      groups = n1 <= 64 ? 2 : 1;
+      nbuf = 1;
+      chains = n1 <= 32 ? 4 : n1 <= 64 ? 3 : n1 <= 96 ? 4 : 3;
+      tiles = n1 <= 32 ? 4 : 1;
+    } else {
+      groups = 2;
+      nbuf = 2;
+      chains = 1;
+      tiles = n1 <= 16 ? 4 : n1 <= 32 ? 2 : 1;
+    }
+  }
+  __device__ uint32_t first(int g, int b) const { return (g * nbuf + b) * chains * n1; }
+  __device__ uint32_t second(int g, int b) const { return (groups * nbuf * chains + (g * nbuf + b) * tiles) * n1; }
   __device__ int columns() const {
-    const int c = 2 * nbuf * (1 + tiles) * n1;
+    const int c = groups * nbuf * (chains + tiles) * n1;
     return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512;
   }
 };
@@ -292,7 +308,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   const FewExpertParams& e = p.e;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n1 = C::PARTS * p.Tp;                       // columns of an accumulator
-  const FewAcc acc(n1);
+  const FewAcc acc(n1, FP32);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], 4); }
@@ -315,6 +331,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
   const int KB = (e.D + C::BK - 1) / C::BK;             // 128-byte steps of product 1
+  const int per = (KB + acc.chains - 1) / acc.chains;   // of them to an accumulator
   const int nO = p.Op / 128;
   constexpr int TU = GLU ? 4 : 8;                       // units of a product-1 tile
   constexpr int UB = GLU ? 4096 : 2048;                 // bytes of one in a step
@@ -413,7 +430,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         for (; ok && walk.next(plan, hrows, C::PARTS, C::UPS, off, r); ++runs) {
           for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
             const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu);
-            const int g = i1 & 1, j = i1 >> 1, b = j & (acc.nbuf - 1);
+            const int g = i1 % acc.groups, j = i1 / acc.groups, b = j & (acc.nbuf - 1);
             if (!(ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
             const uint32_t d = tmem + acc.first(g, b);
@@ -423,10 +440,11 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               uint32_t w = smem_u32(smem + stage * SB), x = w + C::PARTS * kFewTile;
               const int n = KB - kb < pack ? KB - kb : pack;
               for (int kk = 0; kk < n; ++kk, w += nu * UB, x += n1 * 128) {
+                const int chain = FP32 ? (kb + kk) / per : 0, at = FP32 ? (kb + kk) - chain * per : kb + kk;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  step(d, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32), umma_desc_k_sw128(x + k * 32),
-                       p.Tp, (kb | kk | k) ? 1u : 0u);
+                  step(d + chain * n1, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32),
+                       umma_desc_k_sw128(x + k * 32), p.Tp, (at | k) ? 1u : 0u);
               }
               umma_commit(&empty[stage]);
               advance();
@@ -436,9 +454,9 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         }
         if (runs == 0) break;
         // a tile's activations are in shared memory once its accumulator was released
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < acc.groups; ++g)
           for (int b = 0; ok && b < acc.nbuf; ++b) {
-            const int tiles = (i1 + 1 - g) >> 1, uses = (tiles + acc.nbuf - 1 - b) / acc.nbuf;
+            const int tiles = (i1 + acc.groups - 1 - g) / acc.groups, uses = (tiles + acc.nbuf - 1 - b) / acc.nbuf;
             if (uses > 0) ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], (uses - 1) & 1, status, kFewKernelId, kFewWaitNs);
           }
         tc_fence_after_sync();
@@ -448,7 +466,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           const int slices = r.units / C::UPS, tail = r.units % C::UPS;
           const uint32_t hrow = C::PARTS * r.np * 128;   // bytes of a slice of activations
           const int share = tail ? UPT / tail : 1;
-          for (int i0 = 0, g = 0; ok && i0 < nO; i0 += acc.tiles, g ^= 1) {
+          for (int i0 = 0, g = 0; ok && i0 < nO; i0 += acc.tiles, g = acc.groups - 1 - g) {
             const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
             const int j = j2[g]++, b = j & (acc.nbuf - 1);
             if (!(ok = mbar_wait_bounded(&acc2_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
@@ -497,7 +515,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16);
     int i1 = 0, j2 = 0;
     bool ok = true;
-    while (ok) {
+    while (ok && g < acc.groups) {
       FewWalk again = walk;
       int off = 0, runs = 0;
       for (; ok && walk.next(plan, hrows, C::PARTS, C::UPS, off, r); ++runs) {
@@ -505,8 +523,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         const float* b1 = e.b1 ? e.b1 + (long long)r.expert * (GLU ? 2 : 1) * e.F : nullptr;
         const uint32_t hrow = C::PARTS * r.np * 128;
         for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
-          if ((i1 & 1) != g) continue;
-          const int j = i1 >> 1, b = j & (acc.nbuf - 1);
+          if (i1 % acc.groups != g) continue;
+          const int j = i1 / acc.groups, b = j & (acc.nbuf - 1);
           const int unit = u0 + (GLU ? q : 2 * q + (lane >> 4));  // of the run
           const int fl = unit * 16 + (lane & 15);           // hidden row of the run
           const int f = r.f0 + fl;
@@ -516,13 +534,14 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             bias = __ldg(b1 + f);
             if constexpr (GLU) bias_up = __ldg(b1 + e.F + f);
           }
-          ok = mbar_wait_bounded(&acc1_full[g * 2 + b], (j / acc.nbuf) & 1, status, kFewKernelId, kFewWaitNs);
+          ok = mbar_wait_warp(&acc1_full[g * 2 + b], (j / acc.nbuf) & 1, status, kFewKernelId, kFewWaitNs);
           tc_fence_after_sync();
           const uint32_t base = lane_addr + acc.first(g, b);
           uint8_t* hcol = hbuf + r.h * 128 + (fl / C::BK) * hrow;
           const int byte = (fl % C::BK) * C::EB;
           const bool any = u0 + (GLU ? q : 2 * q) < r.units;  // this warp has a unit of the tile
           for (int c = 0; any && c < p.Tp; c += 16) {
+            __syncwarp();
             const unsigned take = (unsigned)(mask >> c) & 0xffffu;   // the expert's tokens among these 16
             if (take == 0u) continue;
             uint32_t v[16];
@@ -533,6 +552,15 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               tmem_ld_wait();
 #pragma unroll
               for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(l[i]));
+              for (int q1 = 1; q1 * per < KB; ++q1) {
+                uint32_t h[16];
+                tmem_ld16(base + q1 * n1 + c, h);
+                tmem_ld16(base + q1 * n1 + p.Tp + c, l);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  v[i] = __float_as_uint(__uint_as_float(v[i]) + (__uint_as_float(h[i]) + __uint_as_float(l[i])));
+              }
             } else {
               tmem_ld_wait();
             }
@@ -581,13 +609,14 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         // group, so a cut run's later pieces are added by the thread that wrote the first.
         const int mine = (int)blockIdx.x - few_cta((long long)r.place * UE, walk.U, walk.G);
         float* dst = p.part + (long long)(plan.part0[r.place] + mine * r.tokens) * p.Op + q * 32 + lane;
-        for (int i0 = g * acc.tiles; ok && i0 < nO; i0 += 2 * acc.tiles, ++j2) {
+        for (int i0 = g * acc.tiles; ok && i0 < nO; i0 += acc.groups * acc.tiles, ++j2) {
           const int b = j2 & (acc.nbuf - 1), nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
-          ok = mbar_wait_bounded(&acc2_full[g * 2 + b], (j2 / acc.nbuf) & 1, status, kFewKernelId, kFewWaitNs);
+          ok = mbar_wait_warp(&acc2_full[g * 2 + b], (j2 / acc.nbuf) & 1, status, kFewKernelId, kFewWaitNs);
           tc_fence_after_sync();
           for (int i = 0; i < nt; ++i) {
             const uint32_t base = lane_addr + acc.second(g, b) + i * C::PARTS * r.np;
             for (int c = 0; c < r.tokens; c += 16) {
+              __syncwarp();
               uint32_t v[16];
               tmem_ld16(base + c, v);
               if constexpr (FP32) {
@@ -622,19 +651,9 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
     bool ok = true;
     auto part = [&](int bytes) {
       if (turn++ % 2 == g) {
-        ok = mbar_wait_bounded(&full[stage], phase, status, kFewKernelId, kFewWaitNs);
-        uint8_t* w = smem + stage * SB + tid * 16;
-#pragma unroll 4
-        for (int i = 0; i < bytes - tid * 16; i += 128 * 16) {
-          const float4 v = *(const float4*)(w + i);
-          float4 h, l;
-          split_tf32(v.x, h.x, l.x);
-          split_tf32(v.y, h.y, l.y);
-          split_tf32(v.z, h.z, l.z);
-          split_tf32(v.w, h.w, l.w);
-          *(float4*)(w + i) = h;
-          *(float4*)(w + i + kFewTile) = l;
-        }
+        ok = mbar_wait_warp(&full[stage], phase, status, kFewKernelId, kFewWaitNs);
+        uint8_t* w = smem + stage * SB;
+        split_tile(w, w + kFewTile, tid, bytes);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&parted[stage]);
@@ -664,8 +683,10 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       }
     }
   }
+  __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
+  __syncwarp();
   tc_fence_after_sync();
   if (warp == 1) tmem_dealloc(tmem, acc.columns());
 }

@@ -96,7 +96,8 @@ struct LinearParams {
 
 // How a product runs, and the device memory that it needs besides.
 struct LinearPlan {
-  int Mp, ranks, stages;   // rows of x of a tile, CTAs that share K, stages
+  int dense;               // CTA pairs with tiles of 256 x dense sums; 0: few rows
+  int Mp, ranks, stages, low;   // few rows: rows of x of a tile, CTAs that share K, stages, tiles of low parts
   int pack_x, pack_w;      // rows that TMA cannot read are copied to aligned ones first
   int packed_stride;
   long long x_bytes, w_bytes;

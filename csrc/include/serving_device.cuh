@@ -5,9 +5,45 @@
 
 #include <cstdint>
 
+#include "sm100_ptx.cuh"
 #include "types.h"
 
 namespace raiccl {
+
+// One try with a time hint: the thread may be put aside for so long instead of
+// polling, which takes issue and shared-memory slots from the warps at work.
+__device__ __forceinline__ bool mbar_try_wait_hint(uint64_t* bar, uint32_t parity, uint32_t ns) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P1;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2, %3;\n\t"
+      "selp.b32 %0, 1, 0, P1;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(ns)
+      : "memory");
+  return ok != 0;
+}
+
+// A wait of a whole warp, bounded like mbar_wait_bounded.  The lanes may leave
+// the loop apart, and the aligned instructions that follow (tcgen05.ld, cluster
+// barriers) need the warp in one piece; all lanes return the same.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, DeviceStatus* st, int kernel_id, uint64_t limit_ns) {
+  bool ok = mbar_try_wait_hint(bar, parity, 20000u);
+  if (!ok) {
+    const uint64_t start = globaltimer_ns();
+    uint32_t polls = 0;
+#pragma unroll 1
+    while (!(ok = mbar_try_wait_hint(bar, parity, 20000u))) {
+      if ((++polls & 63u) != 0) continue;
+      if (globaltimer_ns() - start > limit_ns) {
+        record_status(st, kTimeoutPipeline, kernel_id, (long long)parity, (long long)limit_ns);
+        break;
+      }
+      if (status_failed(st)) break;
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
 
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -36,15 +72,42 @@ __device__ __forceinline__ float serving_act(float z, int act) {
 
 __device__ __forceinline__ float serving_swiglu(float gate, float up) { return gate / (1.f + expf(-gate)) * up; }
 
-// fp32 as two tf32 numbers of 11 significant bits, rounded to nearest; what
-// would round to infinity is cut instead, and an infinity has no low part.
+// fp32 as two tf32 numbers: hi is v rounded to 11 significant bits, lo what is
+// left (at most 12 bits, of which the tensor core reads 11: 2^-23 of v is lost).
+// An infinity has no low part; the last 2^-12 of the range below it counts as
+// infinite.  No branches: with one this took twice as long.
 __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
-  const uint32_t b = __float_as_uint(v);
-  uint32_t h = (b + 0x1000u) & ~0x1fffu;
-  if ((h & 0x7f800000u) == 0x7f800000u) h = b & ~0x1fffu;
+  uint32_t h;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(h) : "f"(v));
   hi = __uint_as_float(h);
-  const float l = v == hi ? 0.f : v - hi;
-  lo = l != l ? l : __uint_as_float((__float_as_uint(l) + 0x1000u) & ~0x1fffu);
+  lo = fabsf(hi) == INFINITY ? 0.f : v - hi;
+}
+
+// Sixteen bytes of a tile in place into high parts, the low parts to `low`.
+__device__ __forceinline__ void split_store(uint8_t* at, uint8_t* low, const float4& v) {
+  float4 h, l;
+  split_tf32(v.x, h.x, l.x);
+  split_tf32(v.y, h.y, l.y);
+  split_tf32(v.z, h.z, l.z);
+  split_tf32(v.w, h.w, l.w);
+  *(float4*)at = h;
+  *(float4*)low = l;
+}
+
+// `bytes` of a tile (a multiple of 16) by the 128 threads of a group: eight
+// loads in flight, without a test while whole rounds of 16 KB are left.
+__device__ __forceinline__ void split_tile(uint8_t* at, uint8_t* low, int tid, int bytes) {
+  constexpr int STEP = 128 * 16;
+  at += tid * 16;
+  low += tid * 16;
+  for (; bytes >= 8 * STEP; bytes -= 8 * STEP, at += 8 * STEP, low += 8 * STEP) {
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = *(const float4*)(at + i * STEP);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) split_store(at + i * STEP, low + i * STEP, v[i]);
+  }
+  for (bytes -= tid * 16; bytes > 0; bytes -= STEP, at += STEP, low += STEP) split_store(at, low, *(const float4*)at);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {

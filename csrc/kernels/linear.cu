@@ -3,7 +3,9 @@
 #include <algorithm>
 #include <atomic>
 #include <stdexcept>
+#include <type_traits>
 
+#include "linear_dense.cuh"
 #include "linear_rows.cuh"
 #include "serving.h"
 #include "serving_device.cuh"
@@ -30,9 +32,15 @@ constexpr int kRowsShared = 232448 - 2048;   // dynamic shared memory of a CTA, 
 
 static long long up256(long long v) { return (v + 255) / 256 * 256; }
 
+// Which kernel, by what each was measured to take on one B200 (us; sizes 1 to 2048 rows, 512 to 16384 outputs, K 1024 and
+// 4096; the sums below are within a tenth of most).  Beside what memory takes for the operands:
+//   rows       3 + 4 Mp / (64 ranks) for each round of CTAs, and for each 128 bytes of its K 0.14 to 0.24 (fp32: 0.55 to 0.9)
+//   dense 128  5 + 1.2 for each round of pairs and 0.21 for each 128 bytes of K; fp32 0.5, and 8 for the split operands
+//   dense 256  6 + 2.5 and 0.31: fewer rounds, each longer
+// So one row of 4096 x 4096 takes 7 us by rows and 19 by dense tiles; 256 rows 22 and 19; 2048 rows 122, 61 and 50.
 LinearPlan plan_linear(const LinearParams& p) {
   LinearPlan r{};
-  const int eb = p.bf16 ? 2 : 4;
+  const int eb = p.bf16 ? 2 : 4, sms = serving_sm_count();
   const bool glu = p.act == (int)Act::kSwiGLU;
   const long long wrows = glu ? 2ll * p.N : p.N;
   auto aligned = [&](const void* base, long long rows, long long stride) {
@@ -41,28 +49,57 @@ LinearPlan plan_linear(const LinearParams& p) {
   r.packed_stride = (std::max(p.K, 1) + 7) / 8 * 8;
   r.pack_x = p.K > 0 && !aligned(p.x, p.M, p.x_stride);
   r.pack_w = p.K > 0 && !aligned(p.w, wrows, p.w_stride);
+  const int KB = (p.K + 128 / eb - 1) / (128 / eb);   // 128-byte steps of K
+
+  // rows: CTAs that share K
+  r.Mp = (int)std::min<long long>(64, (p.M + 15) / 16 * 16);
+  if (!p.bf16 && r.Mp == 48) r.Mp = 64;
+  const long long mt = (p.M + r.Mp - 1) / r.Mp, tiles = (p.N + (glu ? 63 : 127)) / (glu ? 64 : 128) * mt;
+  const int per = p.bf16 ? 2 : 1;   // CTAs per SM; fp32 holds a stage through splitting and product, so one with as many as fit
+  double best = 0;
+  for (int ranks = 1; ranks <= 8; ranks *= 2) {
+    if (ranks > 1 && KB < 2 * ranks) break;
+    const long long slots = (long long)per * sms * (ranks == 8 ? 81 : ranks == 4 ? 89 : 100) / 100;   // clusters leave SMs empty
+    const long long rounds = (tiles * ranks + slots - 1) / slots;
+    const double step = p.bf16 ? 0.14 + 0.1 * r.Mp / 64 : 0.55 + 0.35 * r.Mp / 64;
+    const double cost = rounds * (3.0 + 4.0 * r.Mp / 64 / ranks + (KB + ranks - 1) / ranks * step) + 0.1 * ranks;
+    if (r.ranks == 0 || cost < best) {
+      best = cost;
+      r.ranks = ranks;
+    }
+  }
+  // dense tiles
+  if (p.K > 0 && p.M < (1ll << 30)) {
+    for (int bn = 128; bn <= (p.bf16 ? 256 : 128); bn *= 2) {
+      const int w = glu ? bn / 2 : bn;
+      const long long t = (p.M + 255) / 256 * ((p.N + w - 1) / w), rounds = (t + sms / 2 - 1) / (sms / 2);
+      const double cost = p.bf16 ? (bn == 256 ? 6 + rounds * (2.5 + 0.31 * KB) : 5 + rounds * (1.2 + 0.21 * KB))
+                                 : 13 + rounds * (1.2 + 0.5 * KB) + (double)(p.M + wrows) * p.K * 2e-6;
+      if (cost < best) {
+        best = cost;
+        r.dense = bn;
+      }
+    }
+  }
+  if (p.K == 0) r.x_bytes = 256;   // an address for the maps; nothing is read
+  if (r.dense && !p.bf16) {        // both operands as two tf32 parts
+    r.x_bytes = up256(2ll * p.M * r.packed_stride * eb);
+    r.w_bytes = up256(2ll * wrows * r.packed_stride * eb);
+    return r;
+  }
   if (r.pack_x) r.x_bytes = up256(p.M * r.packed_stride * eb);
   if (r.pack_w) r.w_bytes = up256(wrows * r.packed_stride * eb);
-  if (p.K == 0) r.x_bytes = 256;   // an address for the maps; nothing is read
-  const int most = p.bf16 ? 256 : 128;
-  r.Mp = (int)std::min<long long>(most, (p.M + 15) / 16 * 16);
-  const long long mt = (p.M + r.Mp - 1) / r.Mp, tiles = (p.N + (glu ? 63 : 127)) / (glu ? 64 : 128) * mt;
-  const int KB = (p.K + 128 / eb - 1) / (128 / eb), slots = 2 * serving_sm_count();
-  r.ranks = 1;
-  while (r.ranks < 8 && tiles * r.ranks * 2 <= slots && KB >= r.ranks * 2 * 4) r.ranks *= 2;
   const int sb = p.bf16 ? LinearRows<false>::stage_bytes(r.Mp) : LinearRows<true>::stage_bytes(r.Mp);
-  const int low = p.bf16 ? 0 : LinearRows<true>::low_bytes();
-  // two CTAs per SM where four stages fit in half of its shared memory
-  const int half = kRowsShared / 2 - 2048;
-  const int room = (half - 1024 - low) / sb >= 4 ? half : kRowsShared;
-  r.stages = std::max(2, std::min({kRowsMaxStages, (room - 1024 - low) / sb, std::max(4, (KB + r.ranks - 1) / r.ranks)}));
+  r.low = p.bf16 ? 0 : 2;
+  const int fit = std::min(kRowsMaxStages, (kRowsShared / per - (per - 1) * 2048 - 1024 - r.low * kRowsPack * kRowsTile) / sb);
+  r.stages = std::max(2, std::min(fit, ((KB + r.ranks - 1) / r.ranks + kRowsPack - 1) / kRowsPack));
   return r;
 }
 
-template <bool FP32, bool GLU>
+template <bool FP32, bool GLU, int MP>
 static void launch_rows(const LinearParams& p, const LinearPlan& plan, cudaStream_t s) {
   using C = LinearRows<FP32>;
-  auto kern = linear_rows_kernel<FP32, GLU>;
+  auto kern = linear_rows_kernel<FP32, GLU, MP>;
   static std::atomic<unsigned long long> configured;  // by device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -89,11 +126,14 @@ static void launch_rows(const LinearParams& p, const LinearPlan& plan, cudaStrea
   rp.l = p;
   rp.Mp = plan.Mp;
   rp.stages = plan.stages;
+  rp.low = plan.low;
+  const int ob = p.out_bf16 ? 2 : 4;
+  rp.vec_out = ((uintptr_t)p.out & (4 * ob - 1)) == 0 && p.out_stride % 4 == 0;
   cudaLaunchConfig_t cfg = {};
   const int W = GLU ? 64 : 128;
   cfg.gridDim = dim3((unsigned)((p.N + W - 1) / W * plan.ranks), (unsigned)((p.M + plan.Mp - 1) / plan.Mp));
   cfg.blockDim = dim3(C::THREADS);
-  cfg.dynamicSmemBytes = 1024 + (size_t)std::max(plan.stages * C::stage_bytes(plan.Mp) + C::low_bytes(), plan.Mp * 512);
+  cfg.dynamicSmemBytes = 1024 + (size_t)std::max(plan.stages * C::stage_bytes(plan.Mp) + plan.low * kRowsPack * kRowsTile, plan.Mp * 512);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -105,6 +145,57 @@ static void launch_rows(const LinearParams& p, const LinearPlan& plan, cudaStrea
   cfg.attrs = attr;
   cfg.numAttrs = 2;
   cudaLaunchKernelEx(&cfg, kern, tx, tw, rp, serving_status());
+}
+
+template <int BN, bool FP32, bool GLU>
+static void launch_dense(const LinearParams& p, cudaStream_t s) {
+  using C = LinearDense<BN, FP32>;
+  auto kern = linear_dense_kernel<BN, FP32, GLU>;
+  static std::atomic<unsigned long long> configured;  // by device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+      throw std::runtime_error("linear: shared memory");
+    configured.fetch_or(bit);
+  }
+  const cuuint64_t eb = FP32 ? 4 : 2, K = p.K, parts = FP32 ? 2 : 1, wrows = GLU ? 2ull * p.N : p.N;
+  auto map = [&](const void* base, cuuint64_t rows, cuuint64_t stride, cuuint32_t box_rows) {
+    const cuuint64_t row = rows > 1 ? stride * eb : (K * eb + 15) / 16 * 16;
+    const cuuint64_t dims[3] = {K, rows, parts}, strides[2] = {row, FP32 ? rows * stride * eb : row};
+    const cuuint32_t box[3] = {C::BK, box_rows, 1};
+    return make_tmap(base, !FP32, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  const CUtensorMap tx = map(p.x, p.M, p.x_stride, 128), tw = map(p.w, wrows, p.w_stride, C::HALF);
+  LinearDenseParams dp{};
+  dp.l = p;
+  dp.mt = (int)((p.M + 255) / 256);
+  const int W = GLU ? BN / 2 : BN;
+  dp.nt = (p.N + W - 1) / W;
+  const int ob = p.out_bf16 ? 2 : 4, rb = p.res_bf16 ? 2 : 4;
+  dp.vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * ob) % 16 == 0;
+  dp.vec_res = ((uintptr_t)p.residual & 15) == 0 && (p.res_stride * rb) % 16 == 0;
+  dp.vec_bias = ((uintptr_t)p.bias & 15) == 0 && (!GLU || p.N % 4 == 0);
+  const long long tiles = (long long)dp.mt * dp.nt;
+  const int pairs = (int)std::min<long long>(tiles, serving_sm_count() / 2);
+  launch_with_pdl(kern, dim3(2 * pairs), dim3(kDenseThreads), C::SMEM, s, true, tx, tw, dp, serving_status());
+}
+
+// fp32 stages hold four tiles: at 256 columns three stages of 64 KB, at 128 four of 48 KB, which is what it takes
+// (2048 x 4096 x 4096: 340 against 275 us).
+static void launch_dense_any(const LinearParams& p, int bn, cudaStream_t s) {
+  const bool glu = p.act == (int)Act::kSwiGLU;
+  if (!p.bf16) {
+    if (glu) launch_dense<128, true, true>(p, s);
+    else launch_dense<128, true, false>(p, s);
+  } else if (bn == 256) {
+    if (glu) launch_dense<256, false, true>(p, s);
+    else launch_dense<256, false, false>(p, s);
+  } else {
+    if (glu) launch_dense<128, false, true>(p, s);
+    else launch_dense<128, false, false>(p, s);
+  }
 }
 
 static void pack(const void* src, long long stride, void* dst, int packed, long long rows, int K, int bf16, cudaStream_t s) {
@@ -124,22 +215,41 @@ void launch_linear(const LinearParams& params, const LinearPlan& plan, void* wor
     p.x = p.w = ws;
     p.x_stride = p.w_stride = 8;
   }
-  if (plan.pack_x) {
+  if (plan.dense && !p.bf16) {
+    const long long wrows = glu ? 2ll * p.N : p.N;
+    auto split = [&](const void* src, long long stride, void* dst, long long rows) {
+      const int vec = p.K % 4 == 0 && ((uintptr_t)src & 15) == 0 && stride % 4 == 0;
+      launch_with_pdl(linear_split_kernel, dim3((unsigned)(8 * serving_sm_count())), dim3(256), 0, s, true, (const float*)src, stride,
+                      (float*)dst, plan.packed_stride, rows, p.K, vec);
+    };
+    split(p.x, p.x_stride, ws, p.M);
+    split(p.w, p.w_stride, ws + plan.x_bytes, wrows);
+    p.x = ws;
+    p.w = ws + plan.x_bytes;
+    p.x_stride = p.w_stride = plan.packed_stride;
+  }
+  if (plan.pack_x && !(plan.dense && !p.bf16)) {
     pack(p.x, p.x_stride, ws, plan.packed_stride, p.M, p.K, p.bf16, s);
     p.x = ws;
     p.x_stride = plan.packed_stride;
   }
-  if (plan.pack_w) {
+  if (plan.pack_w && !(plan.dense && !p.bf16)) {
     pack(p.w, p.w_stride, ws + plan.x_bytes, plan.packed_stride, glu ? 2ll * p.N : p.N, p.K, p.bf16, s);
     p.w = ws + plan.x_bytes;
     p.w_stride = plan.packed_stride;
   }
+  if (plan.dense) return launch_dense_any(p, plan.dense, s);
   if (p.bf16) {
-    if (glu) launch_rows<false, true>(p, plan, s);
-    else launch_rows<false, false>(p, plan, s);
+    if (glu) launch_rows<false, true, 0>(p, plan, s);
+    else launch_rows<false, false, 0>(p, plan, s);
   } else {
-    if (glu) launch_rows<true, true>(p, plan, s);
-    else launch_rows<true, false>(p, plan, s);
+    auto rows = [&](auto mp) {
+      if (glu) launch_rows<true, true, decltype(mp)::value>(p, plan, s);
+      else launch_rows<true, false, decltype(mp)::value>(p, plan, s);
+    };
+    if (plan.Mp == 16) rows(std::integral_constant<int, 16>{});
+    else if (plan.Mp == 32) rows(std::integral_constant<int, 32>{});
+    else rows(std::integral_constant<int, 64>{});
   }
 }
 

@@ -74,6 +74,16 @@ def test_fp32_results_are_not_tf32(m, dtype):
     check_norm(got, want, U * (1024 ** 0.5 + 8) + PARTS)
 
 
+@pytest.mark.parametrize("m,n,k", [(64, 12288, 4096), (1, 256, 14336), (20, 512, 8192), (300, 1024, 8192), (1100, 4096, 4096)])
+def test_long_sums(m, n, k):
+    """Chains of thousands of products, over several waves of tiles: the error of fp32 sums grows with the root of K."""
+    x, w, _, _ = _make(m, k, n, "none", FP32, False, False)
+    got = _linear(x, w)
+    want, bound = linear64(x, w)
+    check_close(got, want, bound)
+    check_norm(got, want, U * (k ** 0.5 / 2 + 8) + PARTS)
+
+
 @pytest.mark.parametrize("m", [1, 37, 300])
 @pytest.mark.parametrize("offset,pad", [(0, 8), (1, 0), (4, 3), (8, 64)])
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
