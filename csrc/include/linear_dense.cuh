@@ -12,9 +12,10 @@
 // tensor core cuts what does not fit its accumulator, which drifts with the
 // length of the chain (2e-6 of the result for each 1024 of K), so K is taken
 // 256 at a time, each into an accumulator of its own; the epilogue warps add
-// the chains in registers, rounded to nearest, while the next one runs.  A
-// stage holds both parts of both operands for the three products l h', h l',
-// h h': two thirds of the bytes that three walks over K would fetch.
+// the chains in registers, rounded to nearest, while the next one runs.  The
+// small products l h' and h l' have an accumulator for the whole tile.  A stage
+// holds both parts of both operands for the three products: two thirds of the
+// bytes that three walks over K would fetch.
 //
 // Tiles go by groups of eight row tiles, so that the pairs at work share rows
 // of x and of w in L2.  Every wait is bounded.
@@ -48,7 +49,7 @@ struct LinearDense {
   static constexpr int STAGES_FIT = 216 * 1024 / STAGE;
   static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
   static constexpr int SMEM = 1024 + STAGES * STAGE;
-  static constexpr int COLS = 2 * BN;
+  static constexpr int COLS = FP32 ? 4 * BN : 2 * BN;   // fp32: two for chains, two for small products
 };
 
 __device__ __forceinline__ void tma_load_3d_pair(void* smem_dst, const void* desc, uint32_t bar_cluster_addr, int32_t x, int32_t y,
@@ -146,7 +147,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
   using C = LinearDense<BN, FP32>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], acc_full[2], acc_empty[2], drained;
+  __shared__ uint64_t full[C::STAGES], empty[C::STAGES], acc_full[2], acc_empty[2], low_full[2], low_empty[2], drained;
   __shared__ uint32_t tmem_slot;
   const LinearParams& l = p.l;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -154,7 +155,10 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 16); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 16);
+      mbar_init(&low_full[i], 1); mbar_init(&low_empty[i], 16);
+    }
     mbar_init(&drained, 1);
     fence_mbarrier_init();
     tma_prefetch_desc(&tx); tma_prefetch_desc(&tw);
@@ -205,7 +209,11 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
       uint32_t phase = 0;
       bool ok = true;
       constexpr uint32_t idesc = umma_idesc(FP32 ? 2u : 1u, 256, BN);
-      for (int t = pair; ok && t < tiles; t += npairs) {
+      int nth = 0;
+      for (int t = pair; ok && t < tiles; t += npairs, ++nth) {
+        const int lb = nth & 1;
+        const uint32_t dl = tmem + (2 + lb) * BN;
+        if (FP32 && !(ok = mbar_wait_bounded(&low_empty[lb], ((nth >> 1) & 1) ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
         for (int k0 = 0; ok && k0 < KB; k0 += chain, ++iter) {
           const int steps = k0 + chain < KB ? chain : KB - k0;
           const int b = iter & 1;
@@ -220,9 +228,9 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
             for (int k = 0; k < 4; ++k) {
               const uint64_t a = umma_desc_k_sw128(x + k * 32), bb = umma_desc_k_sw128(w + k * 32);
               if constexpr (FP32) {
-                umma_tf32_pair(d, umma_desc_k_sw128(x + C::X_BYTES + k * 32), bb, idesc, (kb | k) ? 1u : 0u);
-                umma_tf32_pair(d, a, umma_desc_k_sw128(w + C::W_BYTES + k * 32), idesc, 1u);
-                umma_tf32_pair(d, a, bb, idesc, 1u);
+                umma_tf32_pair(dl, umma_desc_k_sw128(x + C::X_BYTES + k * 32), bb, idesc, (k0 | kb | k) ? 1u : 0u);
+                umma_tf32_pair(dl, a, umma_desc_k_sw128(w + C::W_BYTES + k * 32), idesc, 1u);
+                umma_tf32_pair(d, a, bb, idesc, (kb | k) ? 1u : 0u);
               } else {
                 umma_f16_pair(d, a, bb, idesc, (kb | k) ? 1u : 0u);
               }
@@ -237,6 +245,11 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
           umma_commit_pair(mapa_shared(f, 0));
           umma_commit_pair(mapa_shared(f, 1));
         }
+        if (FP32 && ok) {
+          const uint32_t f = smem_u32(&low_full[lb]);
+          umma_commit_pair(mapa_shared(f, 0));
+          umma_commit_pair(mapa_shared(f, 1));
+        }
       }
       umma_commit_pair(mapa_shared(smem_u32(&drained), 0));
       mbar_wait_bounded(&drained, 0, status, kDenseKernelId, kDenseWaitNs);
@@ -246,6 +259,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
     const int q = warp & 3, side = (warp - 2) >> 2;   // TMEM lanes 32 q ..; half of the tile's columns
     constexpr int OUT = W / 2;                        // outputs of a thread
     int iter = 0;
+    [[maybe_unused]] int nth = 0;
     bool ok = true;
     auto finish = [&](long long m, int n, const float (&z)[16], const float (&zu)[16]) {
       float bias[16], up[16], v[16];
@@ -271,30 +285,38 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
         for (int i = 0; i < OUT; ++i) sum[i] = 0.f;
 #pragma unroll
         for (int i = 0; i < (GLU ? OUT : 16); ++i) sum_up[i] = 0.f;
-        for (int k0 = 0; k0 < KB; k0 += chain, ++iter) {
-          const int b = iter & 1;
-          if (!(ok = mbar_wait_warp(&acc_full[b], (iter >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
-          tc_fence_after_sync();
-          const uint32_t base = lanes + b * BN + c0;
+        auto add = [&](uint32_t base) {
 #pragma unroll
           for (int c = 0; c < OUT; c += 16) {
             uint32_t r[16];
             tmem_ld16(base + c, r);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum[c + i] += __uint_as_float(r[i]);
             if constexpr (GLU) {
-              tmem_ld16(base + C::HALF + c, r);
+              uint32_t u[16];
+              tmem_ld16(base + C::HALF + c, u);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) sum_up[c + i] += __uint_as_float(r[i]);
+              for (int i = 0; i < 16; ++i) sum_up[c + i] += __uint_as_float(u[i]);
+            } else {
+              tmem_ld_wait();
             }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[c + i] += __uint_as_float(r[i]);
           }
           tc_fence_before_sync();
           __syncwarp();
+        };
+        for (int k0 = 0; k0 < KB; k0 += chain, ++iter) {
+          const int b = iter & 1;
+          if (!(ok = mbar_wait_warp(&acc_full[b], (iter >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
+          tc_fence_after_sync();
+          add(lanes + b * BN + c0);
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[b]), 0));
         }
-        if (!ok) break;
+        if (!ok || !(ok = mbar_wait_warp(&low_full[nth & 1], (nth >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
+        tc_fence_after_sync();
+        add(lanes + (2 + (nth & 1)) * BN + c0);
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&low_empty[nth & 1]), 0));
+        ++nth;
 #pragma unroll
         for (int c = 0; c < OUT; c += 16) {
           float z[16], zu[16];

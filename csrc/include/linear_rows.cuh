@@ -139,7 +139,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             const uint32_t more = ((FP32 ? i % kRowsChain : i) | j | k) ? 1u : 0u;
             if constexpr (FP32) {
               umma_tf32(d, a, b, umma_idesc(2u, 128, 2 * p.Mp), more);
-              umma_tf32(d, umma_desc_k_sw128(wl + k * 32), b, umma_idesc(2u, 128, p.Mp), 1u);
+              umma_tf32(d + p.Mp, umma_desc_k_sw128(wl + k * 32), b, umma_idesc(2u, 128, p.Mp), 1u);   // with the other small products
             } else {
               umma_f16(d, a, b, umma_idesc(1u, 128, p.Mp), more);
             }

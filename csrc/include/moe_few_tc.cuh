@@ -419,7 +419,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       auto step = [&](uint32_t d, uint64_t a, uint64_t alo, uint64_t b, int n, uint32_t more) {
         if constexpr (FP32) {
           umma_tf32(d, a, b, umma_idesc(2u, 128, 2 * n), more);
-          umma_tf32(d, alo, b, umma_idesc(2u, 128, n), 1u);
+          umma_tf32(d + n, alo, b, umma_idesc(2u, 128, n), 1u);   // with the other small products
         } else {
           umma_f16(d, a, b, umma_idesc(1u, 128, n), more);
         }
