@@ -36,7 +36,7 @@
 // the tokens' parts are stacked as 2N columns, so that is two instructions.  The
 // tensor core cuts what does not fit its accumulator, which drifts with the
 // length of the chain (2e-6 of the result for each 1024 of K), so product 1 of
-// fp32 runs into up to four accumulators in turn along K, added in registers.
+// fp32 runs into three to six accumulators in turn along K, added in registers.
 #pragma once
 
 #include "serving.h"
@@ -48,6 +48,7 @@ namespace raiccl {
 constexpr int kFewTile = 128 * 128;           // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kFewSlack = 12 * 1024;          // behind the last tile: rows that an instruction reads past a short one
 constexpr int kFewMaxStages = 12;
+constexpr int kFewLow = 3;                    // fp32: stages whose low parts of the weights are kept
 constexpr unsigned long long kFewWaitNs = 2000000000ull;
 constexpr int kFewKernelId = 600;
 
@@ -71,10 +72,10 @@ struct FewTc {
   static constexpr int UPS = BK / 16;              // units of 16 hidden rows in a 128-byte row of activations
   static constexpr int TAIL = 16 * EB;             // bytes of one unit in a row
   static constexpr int THREADS = FP32 ? 576 : 320;
-  // K steps of 128 bytes that share a stage where a tile has few rows: a step
-  // costs its waits and its commit, 0.2 us, whatever it holds
-  static __host__ __device__ int packs(int Tp) { const int n = (FP32 ? 128 : 64) / (PARTS * Tp); return n > 4 ? 4 : n < 1 ? 1 : n; }
-  static __host__ __device__ int stage_bytes(int Tp) { return PARTS * kFewTile + packs(Tp) * PARTS * Tp * 128; }
+  // A stage holds a weight tile and its tile of tokens, or, where the weight tile has few rows, several K steps of
+  // both (weights first, tokens at the end): a stage costs its waits and its commit, 0.2 us, whatever it holds.
+  static __host__ __device__ int stage_bytes(int Tp) { return kFewTile + (PARTS * Tp * 128 < 4096 ? 4096 : PARTS * Tp * 128); }
+  static __host__ __device__ int low_bytes() { return FP32 ? kFewLow * kFewTile : 0; }
 };
 
 // The plan that every CTA makes of the routed tokens; mask is zero on entry.
@@ -209,8 +210,8 @@ struct FewAcc {
     if (fp32) {
       groups = n1 <= 64 ? 2 : 1;
       nbuf = 1;
-      chains = n1 <= 32 ? 4 : n1 <= 64 ? 3 : n1 <= 96 ? 4 : 3;
-      tiles = n1 <= 32 ? 4 : 1;
+      chains = n1 <= 32 ? 6 : n1 <= 64 ? 3 : n1 <= 96 ? 4 : 3;
+      tiles = n1 <= 32 ? 2 : 1;
     } else {
       groups = 2;
       nbuf = 2;
@@ -304,7 +305,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   __shared__ uint64_t acc1_full[4], acc1_empty[4], acc2_full[4], acc2_empty[4], drained;
   __shared__ uint32_t tmem_slot;
   const int SB = C::stage_bytes(p.Tp), S = p.stages;
-  uint8_t* const hbuf = smem + S * SB;
+  uint8_t* const low = smem + S * SB;
+  uint8_t* const hbuf = low + C::low_bytes();
   const FewExpertParams& e = p.e;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n1 = C::PARTS * p.Tp;                       // columns of an accumulator
@@ -337,7 +339,6 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   constexpr int UB = GLU ? 4096 : 2048;                 // bytes of one in a step
   constexpr int UPT = kFewTile / (128 * C::TAIL);       // units of 128 rows of W2 in a tile's bytes
   const int hrows = p.hbytes / 128;
-  const int packs = C::packs(p.Tp);
   FewWalk walk;
   walk.start(plan, UE, gridDim.x);
   FewRun r;
@@ -345,7 +346,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   uint32_t phase = 0;
   auto advance = [&]() { if (++stage == S) { stage = 0; phase ^= 1u; } };
   // K steps that share a stage for a tile of nu units
-  auto pack_of = [&](int nu) { const int n = TU / nu; return n < packs ? n : packs; };
+  auto pack_of = [&](int nu) { const int n = SB / (nu * UB + n1 * 128); return n < 4 ? n : 4; };
 
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
@@ -360,7 +361,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             for (int kb = 0; kb < KB; kb += pack) {
               if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
               uint8_t* w = smem + stage * SB;
-              uint8_t* x = w + C::PARTS * kFewTile;
+              uint8_t* x = w + SB - pack * n1 * 128;
               const int n = KB - kb < pack ? KB - kb : pack;
               mbar_arrive_expect_tx(&full[stage], n * (nu * UB + n1 * 128));
               for (int k = 0; k < n; ++k, w += nu * UB, x += n1 * 128) {
@@ -414,6 +415,11 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
     if (elect_one_sync()) {
       uint64_t* ready = FP32 ? parted : full;
       int i1 = 0, j2[2] = {0, 0};   // tiles of product 1; tiles of product 2 by group
+      int lo = 0;                   // slot of low parts
+      auto next = [&]() {
+        advance();
+        if (++lo == kFewLow) lo = 0;
+      };
       bool ok = true;
       // 32 bytes of K: weights [hi | lo] against token rows [hi; lo]
       auto step = [&](uint32_t d, uint64_t a, uint64_t alo, uint64_t b, int n, uint32_t more) {
@@ -437,17 +443,17 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             for (int kb = 0; kb < KB; kb += pack) {
               if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
               tc_fence_after_sync();
-              uint32_t w = smem_u32(smem + stage * SB), x = w + C::PARTS * kFewTile;
+              uint32_t w = smem_u32(smem + stage * SB), x = w + SB - pack * n1 * 128, wl = smem_u32(low) + lo * kFewTile;
               const int n = KB - kb < pack ? KB - kb : pack;
-              for (int kk = 0; kk < n; ++kk, w += nu * UB, x += n1 * 128) {
+              for (int kk = 0; kk < n; ++kk, w += nu * UB, wl += nu * UB, x += n1 * 128) {
                 const int chain = FP32 ? (kb + kk) / per : 0, at = FP32 ? (kb + kk) - chain * per : kb + kk;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  step(d + chain * n1, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32),
+                  step(d + chain * n1, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(wl + k * 32),
                        umma_desc_k_sw128(x + k * 32), p.Tp, (at | k) ? 1u : 0u);
               }
               umma_commit(&empty[stage]);
-              advance();
+              next();
             }
             umma_commit(&acc1_full[g * 2 + b]);
           }
@@ -477,29 +483,29 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               for (int i = 0; i < nt; ++i) {
                 if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
                 tc_fence_after_sync();
-                const uint32_t w = smem_u32(smem + stage * SB), h = h0 + s * hrow;
+                const uint32_t w = smem_u32(smem + stage * SB), wl = smem_u32(low) + lo * kFewTile, h = h0 + s * hrow;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  step(d + i * dn, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(w + kFewTile + k * 32),
+                  step(d + i * dn, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(wl + k * 32),
                        umma_desc_k_sw128(h + k * 32), r.np, (s | k) ? 1u : 0u);
                 umma_commit(&empty[stage]);
-                advance();
+                next();
               }
             for (int i = 0; ok && tail && i < nt; i += share) {
               const int n = nt - i < share ? nt - i : share;
               if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
               tc_fence_after_sync();
               constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
-              uint32_t w = smem_u32(smem + stage * SB);
+              uint32_t w = smem_u32(smem + stage * SB), wl = smem_u32(low) + lo * kFewTile;
               const uint32_t h = h0 + slices * hrow;
               for (int m = 0; m < n; ++m)
-                for (int u = 0; u < tail; ++u, w += 128 * C::TAIL)
+                for (int u = 0; u < tail; ++u, w += 128 * C::TAIL, wl += 128 * C::TAIL)
 #pragma unroll
                   for (int k = 0; k < KS; ++k)
-                    step(d + (i + m) * dn, umma_desc_k_narrow(w + k * 32, C::TAIL), umma_desc_k_narrow(w + kFewTile + k * 32, C::TAIL),
+                    step(d + (i + m) * dn, umma_desc_k_narrow(w + k * 32, C::TAIL), umma_desc_k_narrow(wl + k * 32, C::TAIL),
                          umma_desc_k_sw128(h + (u * KS + k) * 32), r.np, (slices | u | k) ? 1u : 0u);
               umma_commit(&empty[stage]);
-              advance();
+              next();
             }
             umma_commit(&acc2_full[g * 2 + b]);
           }
@@ -618,6 +624,10 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             for (int c = 0; c < r.tokens; c += 16) {
               __syncwarp();
               uint32_t v[16];
+              float was[16];   // of the run's earlier pieces: all loads before the first store
+              float* at = dst + (long long)c * p.Op + (i0 + i) * 128;
+#pragma unroll
+              for (int j = 0; j < 16; ++j) was[j] = !r.first && c + j < r.tokens ? __ldcg(at + (long long)j * p.Op) : 0.f;
               tmem_ld16(base + c, v);
               if constexpr (FP32) {
                 uint32_t l[16];
@@ -629,13 +639,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
                 tmem_ld_wait();
               }
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                if (c + j >= r.tokens) break;
-                float* at = dst + (long long)(c + j) * p.Op + (i0 + i) * 128;
-                float out = __uint_as_float(v[j]);
-                if (!r.first) out += *at;
-                *at = out;
-              }
+              for (int j = 0; j < 16; ++j)
+                if (c + j < r.tokens) __stcg(at + (long long)j * p.Op, __uint_as_float(v[j]) + was[j]);
             }
           }
           tc_fence_before_sync();
@@ -647,17 +652,23 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   } else if constexpr (FP32) {
     // ---------------------------------------------------------------- weights into tf32 parts
     const int tid = (threadIdx.x - 320) & 127, g = (threadIdx.x - 320) >> 7;   // two groups take stages in turn
-    int turn = 0;
+    int turn = 0, lo = 0, old = 0;   // slot of low parts; stage of the products that read it last, and their phase
+    uint32_t old_phase = 0;
     bool ok = true;
     auto part = [&](int bytes) {
-      if (turn++ % 2 == g) {
-        ok = mbar_wait_warp(&full[stage], phase, status, kFewKernelId, kFewWaitNs);
-        uint8_t* w = smem + stage * SB;
-        split_tile(w, w + kFewTile, tid, bytes);
+      const int slot = lo, was = old;
+      const uint32_t was_phase = old_phase;
+      if (++lo == kFewLow) lo = 0;
+      if (turn >= kFewLow && ++old == S) { old = 0; old_phase ^= 1u; }
+      if (turn % 2 == g) {
+        ok = mbar_wait_warp(&full[stage], phase, status, kFewKernelId, kFewWaitNs) &&
+             (turn < kFewLow || mbar_wait_warp(&empty[was], was_phase, status, kFewKernelId, kFewWaitNs));
+        split_tile(smem + stage * SB, low + slot * kFewTile, tid, bytes);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&parted[stage]);
       }
+      ++turn;
       advance();
     };
     while (ok) {

@@ -339,13 +339,15 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   // and (grid / n + 2) CTAs each, so T (grid + 2 k) rows at most, whatever n is.
   r.a_bytes = up256((long long)p.T * (r.grid + 2 * p.k) * r.Op * 4);
   r.b_bytes = up256(16ll * pairs);
-  // activations: what the longest range of a CTA needs, at most a quarter of shared memory; the rest holds stages
+  // Activations of the longest range of a CTA, if that leaves four stages; else the range is worked off in pieces, which
+  // costs a sum in memory each.  The rest holds stages.
+  const int sb = p.bf16 ? FewTc<false>::stage_bytes(r.Tp) : FewTc<true>::stage_bytes(r.Tp);
+  const int room = kFewShared - (p.bf16 ? 0 : FewTc<true>::low_bytes());
   const long long most = ((long long)std::min(p.E, pairs) * UE + r.grid - 1) / r.grid;
   const long long rows = (std::min<long long>(most, UE) + ups - 1) / ups + 1;
-  r.hbytes = (int)std::min<long long>(rows * parts * r.Tp * 128, p.bf16 ? 56 * 1024 : 24 * 1024);
+  r.hbytes = (int)std::min<long long>(rows * parts * r.Tp * 128, room - 4 * sb);
   r.hbytes = std::max({r.hbytes, parts * r.Tp * 128, kFewSlack});
-  const int sb = p.bf16 ? FewTc<false>::stage_bytes(r.Tp) : FewTc<true>::stage_bytes(r.Tp);
-  r.stages = std::min(kFewMaxStages, (kFewShared - r.hbytes) / sb);
+  r.stages = std::min(kFewMaxStages, (room - r.hbytes) / sb);
   return r;
 }
 
@@ -360,7 +362,7 @@ static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CU
       throw std::runtime_error("moe_few_tokens: shared memory");
     configured.fetch_or(bit);
   }
-  const size_t smem = 1024 + (size_t)tp.stages * FewTc<FP32>::stage_bytes(tp.Tp) + tp.hbytes;
+  const size_t smem = 1024 + (size_t)tp.stages * FewTc<FP32>::stage_bytes(tp.Tp) + FewTc<FP32>::low_bytes() + tp.hbytes;
   launch_with_pdl(kern, dim3(grid), dim3(FewTc<FP32>::THREADS), smem, s, true, tx, t1, t1w, t2, t2u, tp, serving_status());
 }
 
