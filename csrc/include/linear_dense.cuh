@@ -209,6 +209,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
       uint32_t phase = 0;
       bool ok = true;
       constexpr uint32_t idesc = umma_idesc(FP32 ? 2u : 1u, 256, BN);
+      const uint64_t row = umma_desc_k_sw128(0);
       int nth = 0;
       for (int t = pair; ok && t < tiles; t += npairs, ++nth) {
         const int lb = nth & 1;
@@ -223,16 +224,15 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
           for (int kb = 0; kb < steps; ++kb) {
             if (!(ok = mbar_wait_bounded(&full[stage], phase, status, kDenseKernelId, kDenseWaitNs))) break;
             tc_fence_after_sync();
-            const uint32_t x = smem_u32(smem + stage * C::STAGE), w = x + C::PARTS * C::X_BYTES;
+            const uint64_t dx = desc_at(row, smem_u32(smem + stage * C::STAGE)), dw = dx + C::PARTS * C::X_BYTES / 16;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint64_t a = umma_desc_k_sw128(x + k * 32), bb = umma_desc_k_sw128(w + k * 32);
               if constexpr (FP32) {
-                umma_tf32_pair(dl, umma_desc_k_sw128(x + C::X_BYTES + k * 32), bb, idesc, (k0 | kb | k) ? 1u : 0u);
-                umma_tf32_pair(dl, a, umma_desc_k_sw128(w + C::W_BYTES + k * 32), idesc, 1u);
-                umma_tf32_pair(d, a, bb, idesc, (kb | k) ? 1u : 0u);
+                umma_tf32_pair(dl, dx + C::X_BYTES / 16 + 2 * k, dw + 2 * k, idesc, (k0 | kb | k) ? 1u : 0u);
+                umma_tf32_pair(dl, dx + 2 * k, dw + C::W_BYTES / 16 + 2 * k, idesc, 1u);
+                umma_tf32_pair(d, dx + 2 * k, dw + 2 * k, idesc, (kb | k) ? 1u : 0u);
               } else {
-                umma_f16_pair(d, a, bb, idesc, (kb | k) ? 1u : 0u);
+                umma_f16_pair(d, dx + 2 * k, dw + 2 * k, idesc, (kb | k) ? 1u : 0u);
               }
             }
             const uint32_t e = smem_u32(&empty[stage]);

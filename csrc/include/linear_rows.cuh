@@ -121,6 +121,8 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
     // ---------------------------------------------------------------- products
     if (elect_one_sync()) {
       uint64_t* ready = FP32 ? parted : full;
+      const uint64_t row = umma_desc_k_sw128(0);
+      const uint32_t id = umma_idesc(FP32 ? 2u : 1u, 128, (uint32_t)(C::PARTS * p.Mp)), idl = umma_idesc(2u, 128, (uint32_t)p.Mp);
       int lo = 0;
       for (int i = 0; i < count; ++i, advance()) {
         if (FP32 && i % kRowsChain == 0) {
@@ -130,18 +132,18 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         if (!mbar_wait_bounded(&ready[stage], phase, status, kRowsKernelId, kServingWaitNs)) break;
         tc_fence_after_sync();
         const uint32_t d = tmem + (FP32 ? (i / kRowsChain & 1) * 2 * p.Mp : 0);
-        uint32_t w = smem_u32(smem + stage * SB), x = w + kRowsPack * kRowsTile, wl = smem_u32(low) + lo * kRowsPack * kRowsTile;
+        const uint32_t w = smem_u32(smem + stage * SB);
+        uint64_t da = desc_at(row, w), dx = desc_at(row, w + kRowsPack * kRowsTile), dl = desc_at(row, smem_u32(low) + lo * kRowsPack * kRowsTile);
         const int n = steps - i * kRowsPack < kRowsPack ? steps - i * kRowsPack : kRowsPack;
-        for (int j = 0; j < n; ++j, w += kRowsTile, x += C::PARTS * p.Mp * 128, wl += kRowsTile) {
+        for (int j = 0; j < n; ++j, da += kRowsTile / 16, dx += C::PARTS * p.Mp * 8, dl += kRowsTile / 16) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint64_t a = umma_desc_k_sw128(w + k * 32), b = umma_desc_k_sw128(x + k * 32);
             const uint32_t more = ((FP32 ? i % kRowsChain : i) | j | k) ? 1u : 0u;
             if constexpr (FP32) {
-              umma_tf32(d, a, b, umma_idesc(2u, 128, 2 * p.Mp), more);
-              umma_tf32(d + p.Mp, umma_desc_k_sw128(wl + k * 32), b, umma_idesc(2u, 128, p.Mp), 1u);   // with the other small products
+              umma_tf32(d, da + 2 * k, dx + 2 * k, id, more);
+              umma_tf32(d + p.Mp, dl + 2 * k, dx + 2 * k, idl, 1u);   // with the other small products
             } else {
-              umma_f16(d, a, b, umma_idesc(1u, 128, p.Mp), more);
+              umma_f16(d, da + 2 * k, dx + 2 * k, id, more);
             }
           }
         }

@@ -72,6 +72,7 @@ struct FewTc {
   static constexpr int UPS = BK / 16;              // units of 16 hidden rows in a 128-byte row of activations
   static constexpr int TAIL = 16 * EB;             // bytes of one unit in a row
   static constexpr int THREADS = FP32 ? 576 : 320;
+  static constexpr uint32_t FORMAT = FP32 ? 2u : 1u;
   // A stage holds a weight tile and its tile of tokens, or, where the weight tile has few rows, several K steps of
   // both (weights first, tokens at the end): a stage costs its waits and its commit, 0.2 us, whatever it holds.
   static __host__ __device__ int stage_bytes(int Tp) { return kFewTile + (PARTS * Tp * 128 < 4096 ? 4096 : PARTS * Tp * 128); }
@@ -421,13 +422,15 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         if (++lo == kFewLow) lo = 0;
       };
       bool ok = true;
+      const uint64_t wide_row = umma_desc_k_sw128(0), unit_row = umma_desc_k_narrow(0, C::TAIL);
+      const uint32_t id1 = umma_idesc(C::FORMAT, 128, (uint32_t)n1), id1l = umma_idesc(C::FORMAT, 128, (uint32_t)p.Tp);
       // 32 bytes of K: weights [hi | lo] against token rows [hi; lo]
-      auto step = [&](uint32_t d, uint64_t a, uint64_t alo, uint64_t b, int n, uint32_t more) {
+      auto step = [&](uint32_t d, uint32_t dl, uint64_t a, uint64_t al, uint64_t b, uint32_t id, uint32_t idl, uint32_t more) {
         if constexpr (FP32) {
-          umma_tf32(d, a, b, umma_idesc(2u, 128, 2 * n), more);
-          umma_tf32(d + n, alo, b, umma_idesc(2u, 128, n), 1u);   // with the other small products
+          umma_tf32(d, a, b, id, more);
+          umma_tf32(dl, al, b, idl, 1u);   // with the other small products
         } else {
-          umma_f16(d, a, b, umma_idesc(1u, 128, n), more);
+          umma_f16(d, a, b, id, more);
         }
       };
       while (ok) {
@@ -439,18 +442,19 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             const int g = i1 % acc.groups, j = i1 / acc.groups, b = j & (acc.nbuf - 1);
             if (!(ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
-            const uint32_t d = tmem + acc.first(g, b);
+            uint32_t dc = tmem + acc.first(g, b);
+            int at = 0;   // steps of the chain
             for (int kb = 0; kb < KB; kb += pack) {
               if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
               tc_fence_after_sync();
-              uint32_t w = smem_u32(smem + stage * SB), x = w + SB - pack * n1 * 128, wl = smem_u32(low) + lo * kFewTile;
+              const uint32_t w = smem_u32(smem + stage * SB), x = w + SB - pack * n1 * 128, wl = smem_u32(low) + lo * kFewTile;
               const int n = KB - kb < pack ? KB - kb : pack;
-              for (int kk = 0; kk < n; ++kk, w += nu * UB, wl += nu * UB, x += n1 * 128) {
-                const int chain = FP32 ? (kb + kk) / per : 0, at = FP32 ? (kb + kk) - chain * per : kb + kk;
+              uint64_t da = desc_at(wide_row, w), dl = desc_at(wide_row, wl), dx = desc_at(wide_row, x);
+              for (int kk = 0; kk < n; ++kk, da += nu * UB / 16, dl += nu * UB / 16, dx += n1 * 8) {
+                if (FP32 && at == per) { at = 0; dc += n1; }   // the next chain
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  step(d + chain * n1, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(wl + k * 32),
-                       umma_desc_k_sw128(x + k * 32), p.Tp, (at | k) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) step(dc, dc + p.Tp, da + 2 * k, dl + 2 * k, dx + 2 * k, id1, id1l, (at | k) ? 1u : 0u);
+                ++at;
               }
               umma_commit(&empty[stage]);
               next();
@@ -471,6 +475,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           again.next(plan, hrows, C::PARTS, C::UPS, off, r);
           const int slices = r.units / C::UPS, tail = r.units % C::UPS;
           const uint32_t hrow = C::PARTS * r.np * 128;   // bytes of a slice of activations
+          const uint32_t id2 = umma_idesc(C::FORMAT, 128, (uint32_t)(C::PARTS * r.np)), id2l = umma_idesc(C::FORMAT, 128, (uint32_t)r.np);
           const int share = tail ? UPT / tail : 1;
           for (int i0 = 0, g = 0; ok && i0 < nO; i0 += acc.tiles, g = acc.groups - 1 - g) {
             const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
@@ -483,11 +488,11 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               for (int i = 0; i < nt; ++i) {
                 if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
                 tc_fence_after_sync();
-                const uint32_t w = smem_u32(smem + stage * SB), wl = smem_u32(low) + lo * kFewTile, h = h0 + s * hrow;
+                const uint64_t da = desc_at(wide_row, smem_u32(smem + stage * SB)), dl = desc_at(wide_row, smem_u32(low) + lo * kFewTile);
+                const uint64_t dh = desc_at(wide_row, h0 + s * hrow);
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  step(d + i * dn, umma_desc_k_sw128(w + k * 32), umma_desc_k_sw128(wl + k * 32),
-                       umma_desc_k_sw128(h + k * 32), r.np, (s | k) ? 1u : 0u);
+                  step(d + i * dn, d + i * dn + r.np, da + 2 * k, dl + 2 * k, dh + 2 * k, id2, id2l, (s | k) ? 1u : 0u);
                 umma_commit(&empty[stage]);
                 next();
               }
@@ -496,14 +501,14 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
               tc_fence_after_sync();
               constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
-              uint32_t w = smem_u32(smem + stage * SB), wl = smem_u32(low) + lo * kFewTile;
-              const uint32_t h = h0 + slices * hrow;
+              uint64_t da = desc_at(unit_row, smem_u32(smem + stage * SB)), dl = desc_at(unit_row, smem_u32(low) + lo * kFewTile);
+              const uint64_t dh = desc_at(wide_row, h0 + slices * hrow);
               for (int m = 0; m < n; ++m)
-                for (int u = 0; u < tail; ++u, w += 128 * C::TAIL, wl += 128 * C::TAIL)
+                for (int u = 0; u < tail; ++u, da += 8 * C::TAIL, dl += 8 * C::TAIL)
 #pragma unroll
                   for (int k = 0; k < KS; ++k)
-                    step(d + (i + m) * dn, umma_desc_k_narrow(w + k * 32, C::TAIL), umma_desc_k_narrow(wl + k * 32, C::TAIL),
-                         umma_desc_k_sw128(h + (u * KS + k) * 32), r.np, (slices | u | k) ? 1u : 0u);
+                    step(d + (i + m) * dn, d + (i + m) * dn + r.np, da + 2 * k, dl + 2 * k, dh + 2 * (u * KS + k), id2, id2l,
+                         (slices | u | k) ? 1u : 0u);
               umma_commit(&empty[stage]);
               next();
             }

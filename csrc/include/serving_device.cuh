@@ -45,6 +45,11 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, D
   return __all_sync(0xffffffffu, ok);
 }
 
+// Shared-memory descriptors by addition: the fields of umma_desc_k_sw128 (or
+// umma_desc_k_narrow) without an address, plus the address in 16-byte units.
+// A product issues four to twelve of them for each 128 bytes of K.
+__device__ __forceinline__ uint64_t desc_at(uint64_t fields, uint32_t smem_addr) { return fields + (smem_addr >> 4); }
+
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
