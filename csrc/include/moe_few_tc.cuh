@@ -352,6 +352,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     if (elect_one_sync()) {
+      // weights are read once: they leave the rest of L2 (code, router, tokens, parts) alone
+      const uint64_t once = l2_evict_first();
       bool ok = true;
       while (ok) {
         FewWalk again = walk;
@@ -368,12 +370,12 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               for (int k = 0; k < n; ++k, w += nu * UB, x += n1 * 128) {
                 const int d = (kb + k) * C::BK;
                 if (nu == TU && p.wide) {
-                  if constexpr (GLU) tma_load_5d(w, &t1w, &full[stage], d, 0, 0, f0 / 16, r.expert);
-                  else tma_load_3d(w, &t1w, &full[stage], d, f0, r.expert);
+                  if constexpr (GLU) tma_load_5d_hint(w, &t1w, &full[stage], d, 0, 0, f0 / 16, r.expert, once);
+                  else tma_load_3d_hint(w, &t1w, &full[stage], d, f0, r.expert, once);
                 } else {
                   for (int u = 0; u < nu; ++u) {
-                    if constexpr (GLU) tma_load_4d(w + u * UB, &t1, &full[stage], d, f0 + u * 16, 0, r.expert);
-                    else tma_load_3d(w + u * UB, &t1, &full[stage], d, f0 + u * 16, r.expert);
+                    if constexpr (GLU) tma_load_4d_hint(w + u * UB, &t1, &full[stage], d, f0 + u * 16, 0, r.expert, once);
+                    else tma_load_3d_hint(w + u * UB, &t1, &full[stage], d, f0 + u * 16, r.expert, once);
                   }
                 }
                 tma_load_2d(x, &tx, &full[stage], d, 0);
@@ -394,7 +396,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               for (int i = 0; i < nt; ++i) {
                 if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
                 mbar_arrive_expect_tx(&full[stage], kFewTile);
-                tma_load_3d(smem + stage * SB, &t2, &full[stage], r.f0 + s * C::BK, (i0 + i) * 128, r.expert);
+                tma_load_3d_hint(smem + stage * SB, &t2, &full[stage], r.f0 + s * C::BK, (i0 + i) * 128, r.expert, once);
                 advance();
               }
             for (int i = 0; ok && tail && i < nt; i += share) {
@@ -404,7 +406,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               uint8_t* w = smem + stage * SB;
               for (int m = 0; m < n; ++m)
                 for (int u = 0; u < tail; ++u, w += 128 * C::TAIL)
-                  tma_load_3d(w, &t2u, &full[stage], r.f0 + slices * C::BK + u * 16, (i0 + i + m) * 128, r.expert);
+                  tma_load_3d_hint(w, &t2u, &full[stage], r.f0 + slices * C::BK + u * 16, (i0 + i + m) * 128, r.expert, once);
               advance();
             }
           }
