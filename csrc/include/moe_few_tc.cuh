@@ -56,7 +56,7 @@ constexpr int kFewKernelId = 600;
 struct FewTcParams {
   FewExpertParams e;
   float* part;        // [rows, Op] the CTAs' parts of the experts' results
-  int4* terms;        // [T, k] a choice's first row in part, rows to the next part, parts; expert
+  int grid;           // CTAs of the experts' kernel
   int Op;             // O rounded up to 128
   int Tp;             // T rounded up to 16
   int stages;
@@ -79,7 +79,7 @@ struct FewTc {
   static __host__ __device__ int low_bytes() { return FP32 ? kFewLow * kFewTile : 0; }
 };
 
-// The plan that every CTA makes of the routed tokens; mask is zero on entry.
+// The plan that every CTA makes of the routed tokens.
 struct FewPlan {
   unsigned long long mask[kFewExperts + 1];  // by expert: its tokens
   int used[kFewExperts + 1];                 // the chosen experts, by number
@@ -92,9 +92,8 @@ struct FewPlan {
 // CTA of unit u where U units are dealt to G <= U CTAs: CTA c has units [U c / G, U (c + 1) / G).
 __device__ __forceinline__ int few_cta(long long u, long long U, int G) { return (int)(((u + 1) * G - 1) / U); }
 
-__device__ __forceinline__ void few_plan(const FewTcParams& tp, FewPlan& s, int UE, int grid) {
-  const FewExpertParams& p = tp.e;
-  const int pairs = p.T * p.k;
+__device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, int UE, int grid) {
+  const int pairs = p.T * p.k;   // mask is zero on entry
   for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
     const int e = __ldcg(p.ids + i);
     if (e >= 0) atomicOr(&s.mask[e], 1ull << (i / p.k));
@@ -136,17 +135,6 @@ __device__ __forceinline__ void few_plan(const FewTcParams& tp, FewPlan& s, int 
     if (lane == 0) s.ne = ne;
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
-      const int e = __ldcg(p.ids + i);
-      int4 t = make_int4(0, 0, 0, 0);
-      if (e >= 0) {
-        const unsigned long long m = s.mask[e];
-        t = make_int4(s.part0[s.index[e]] + __popcll(m & ((1ull << (i / p.k)) - 1ull)), __popcll(m), s.parts[s.index[e]], e);
-      }
-      tp.terms[i] = t;
-    }
-  }
 }
 
 // A run of units of one expert; the roles walk the same runs.
@@ -229,57 +217,69 @@ struct FewAcc {
 };
 
 // out[t, o0 .. o0 + 128) of one token: the parts of all its choices, by choice,
-// then CTA, are dealt to the eight warps in turn, each times its choice's
-// gate; the warps' sums are added in order.  A few hundred loads in all, so
-// what counts is how many are in flight.
-constexpr int kFewJoinThreads = 256;
+// then CTA, are dealt to the warps in turn, each times its choice's gate; the
+// warps' sums are added in order.  At most grid + 2 k loads of a column in all,
+// so what counts is how many are in flight, and that all but these loads is
+// done before the experts' kernel ends: its CTAs leave room for these beside
+// them, and which rows to add follows from the routing alone, whose kernel had
+// ended before the experts' kernel allowed this launch.
+constexpr int kFewJoinThreads = 512;
 
 __global__ void __launch_bounds__(kFewJoinThreads) few_join_parts_kernel(FewTcParams p) {
   constexpr int W = kFewJoinThreads / 32;
+  __shared__ FewPlan plan;
   __shared__ __align__(16) float red[W][128];
-  __shared__ int4 term[kFewTopK];
-  __shared__ float gate[kFewTopK], weight[kFewJoinThreads];
   __shared__ int row[kFewJoinThreads];
+  __shared__ float weight[kFewJoinThreads];
+  __shared__ int4 term[kFewTopK];     // a choice's first row in part, rows to the next part, parts, expert
+  __shared__ float gate[kFewTopK];
   const FewExpertParams& e = p.e;
   const int t = blockIdx.y, o0 = blockIdx.x * 128;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float* col = p.part + o0 + lane * 4;
   const int o = o0 + threadIdx.x;
   const bool writes = threadIdx.x < 128 && o < e.O;
-  griddep_wait();
-  griddep_launch_dependents();
   float res = 0.f;
   if (writes && e.residual) res = load_elem(e.residual, (long long)t * e.res_stride + o, e.res_bf16);
+  for (int i = threadIdx.x; i < e.E; i += kFewJoinThreads) plan.mask[i] = 0ull;
+  __syncthreads();
+  few_plan(e, plan, (e.F + 15) / 16, p.grid);
   if (threadIdx.x < kFewTopK) {
-    term[threadIdx.x] = threadIdx.x < e.k ? __ldcg(p.terms + t * e.k + threadIdx.x) : make_int4(0, 0, 0, 0);
-    gate[threadIdx.x] = threadIdx.x < e.k ? __ldcg(e.gates + t * e.k + threadIdx.x) : 0.f;
+    const int j = threadIdx.x, x = j < e.k ? __ldcg(e.ids + t * e.k + j) : -1;
+    int4 v = make_int4(0, 0, 0, 0);
+    if (x >= 0) {
+      const unsigned long long m = plan.mask[x];
+      const int place = plan.index[x];
+      v = make_int4(plan.part0[place] + __popcll(m & ((1ull << t) - 1ull)), __popcll(m), plan.parts[place], x);
+    }
+    term[j] = v;
+    gate[j] = j < e.k ? __ldcg(e.gates + t * e.k + j) : 0.f;
   }
   __syncthreads();
   int items = 0;
   for (int j = 0; j < e.k; ++j) items += term[j].z;
+  {
+    int c = threadIdx.x, j = 0;      // items <= kFewJoinThreads: a token's choices have at most grid + 2 k parts
+    while (j + 1 < e.k && c >= term[j].z) c -= term[j++].z;
+    row[threadIdx.x] = term[j].x + c * term[j].y;
+    weight[threadIdx.x] = gate[j];
+  }
   float bias = 0.f;
   if (e.b2 && writes)
     for (int j = 0; j < e.k; ++j)
       if (term[j].z > 0) bias = fmaf(gate[j], __ldg(e.b2 + (long long)term[j].w * e.O + o), bias);
+  __syncthreads();
+  griddep_wait();
+  griddep_launch_dependents();
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  // kFewJoinThreads items at a time: each thread looks one up, then the warps read theirs
-  for (int i0 = 0; i0 < items; i0 += kFewJoinThreads) {
-    int c = i0 + threadIdx.x, j = 0;
-    while (j + 1 < e.k && c >= term[j].z) c -= term[j++].z;
-    if (i0 > 0) __syncthreads();
-    row[threadIdx.x] = term[j].x + c * term[j].y;
-    weight[threadIdx.x] = gate[j];
-    __syncthreads();
-    const int n = items - i0 < kFewJoinThreads ? items - i0 : kFewJoinThreads;
 #pragma unroll 8
-    for (int i = w; i < n; i += W) {
-      const float4 a = __ldcg((const float4*)(col + (long long)row[i] * p.Op));
-      const float g = weight[i];
-      v.x = fmaf(g, a.x, v.x);
-      v.y = fmaf(g, a.y, v.y);
-      v.z = fmaf(g, a.z, v.z);
-      v.w = fmaf(g, a.w, v.w);
-    }
+  for (int i = w; i < items; i += W) {
+    const float4 a = __ldcg((const float4*)(col + (long long)row[i] * p.Op));
+    const float g = weight[i];
+    v.x = fmaf(g, a.x, v.x);
+    v.y = fmaf(g, a.y, v.y);
+    v.z = fmaf(g, a.z, v.z);
+    v.w = fmaf(g, a.w, v.w);
   }
   *(float4*)&red[w][lane * 4] = v;
   __syncthreads();
@@ -329,7 +329,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   __syncthreads();
   griddep_wait();
   const int UE = (e.F + 15) / 16;
-  few_plan(p, plan, UE, gridDim.x);   // holds __syncthreads
+  few_plan(e, plan, UE, gridDim.x);   // holds __syncthreads
   griddep_launch_dependents();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;

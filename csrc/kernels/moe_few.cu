@@ -313,6 +313,7 @@ int serving_sm_count() {
 static long long up256(long long v) { return (v + 255) / 256 * 256; }
 
 constexpr int kFewShared = 232448 - 10 * 1024 - 1024;  // dynamic shared memory besides the kernel's own and the alignment
+constexpr int kFewJoinRoom = 24 * 1024;                // of the join's CTA beside it
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   FewExpertPlan r{};
@@ -338,11 +339,12 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   // An expert's tokens times the CTAs that share it, over all experts: n experts have at most min(T k, n T) tokens
   // and (grid / n + 2) CTAs each, so T (grid + 2 k) rows at most, whatever n is.
   r.a_bytes = up256((long long)p.T * (r.grid + 2 * p.k) * r.Op * 4);
-  r.b_bytes = up256(16ll * pairs);
   // Activations of the longest range of a CTA, if that leaves four stages; else the range is worked off in pieces, which
   // costs a sum in memory each.  The rest holds stages.
   const int sb = p.bf16 ? FewTc<false>::stage_bytes(r.Tp) : FewTc<true>::stage_bytes(r.Tp);
-  const int room = kFewShared - (p.bf16 ? 0 : FewTc<true>::low_bytes());
+  // Up to 16 tokens the join's CTAs find room beside the experts' (64 experts, 1 token: 49.7 -> 43.5 us); with more, the
+  // stages are worth more (37 tokens: 193 against 196 us).
+  const int room = kFewShared - (p.T <= 16 ? kFewJoinRoom : 0) - (p.bf16 ? 0 : FewTc<true>::low_bytes());
   const long long most = ((long long)std::min(p.E, pairs) * UE + r.grid - 1) / r.grid;
   const long long rows = (std::min<long long>(most, UE) + ups - 1) / ups + 1;
   r.hbytes = (int)std::min<long long>(rows * parts * r.Tp * 128, room - 4 * sb);
@@ -417,7 +419,7 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
   FewTcParams tp{};
   tp.e = p;
   tp.part = a;
-  tp.terms = (int4*)b;
+  tp.grid = plan.grid;
   tp.Op = plan.Op;
   tp.Tp = plan.Tp;
   tp.stages = plan.stages;
