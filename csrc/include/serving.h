@@ -61,12 +61,13 @@ struct FewExpertParams {
 
 // How the experts of a call run, and the device memory that they need besides.
 struct FewExpertPlan {
-  int tensor;             // on the tensor cores (else one warp per weight row)
+  int tensor;             // on the tensor cores (else by rows, on CUDA cores)
+  int vec;                // by rows: 16 bytes at a time
   int grid, stages, hbytes, Op, Tp;
   int pack;               // x is packed by the routing kernel
   int packed_stride;
-  long long packed_bytes, a_bytes, b_bytes;  // multiples of 256; in this order in the workspace
-  long long bytes() const { return packed_bytes + a_bytes + b_bytes; }
+  long long packed_bytes, a_bytes;  // multiples of 256; in this order in the workspace
+  long long bytes() const { return packed_bytes + a_bytes; }
 };
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p);

@@ -191,108 +191,201 @@ void launch_few_route(const FewRouteParams& params, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------------------
-// Experts: one warp per weight row and expert; a row is read once for up to
-// eight of the expert's tokens at a time.
+// Experts by rows, on CUDA cores: for the smallest calls, where a pipeline's
+// start costs more than it brings, and for weights that TMA cannot read.  One
+// warp per pair of W1 rows and per row of W2; fp32 sums, activations in fp32.
+// What bounds it is memory: 24 loads of 16 bytes in flight per lane and four
+// CTAs per SM.  64 experts, 1 token (104 MB): MEASURE_FINE us, against MEASURE_TC by
+// tensor cores; the R4 layer, 1 token: MEASURE_R4 against MEASURE_R4TC.
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
-constexpr int kRowTokens = 8;
+constexpr int kRowWarps = kRowThreads / 32;
 
-// The expert's (token, choice) pairs t k + j in token order -> list; returns their number.
-__device__ __forceinline__ int few_pairs(const int* ids, int T, int k, int e, int* list) {
+// An expert's (token, choice) pairs in token order go four to a CTA: that of the
+// pair `y` takes list[0 .. n) if it is the first of its four, else none.
+constexpr int kRowTokens = 4;
+
+__device__ __forceinline__ int few_pairs(const int* ids, int T, int k, int y, int* list, int& e) {
   __shared__ unsigned long long mask;
   if (threadIdx.x == 0) mask = 0ull;
+  e = __ldcg(ids + y);
+  if (e < 0) return 0;
   __syncthreads();
   for (int i = threadIdx.x; i < T * k; i += blockDim.x)
-    if (ids[i] == e) atomicOr(&mask, 1ull << (i / k));
+    if (__ldcg(ids + i) == e) atomicOr(&mask, 1ull << (i / k));
   __syncthreads();
   const unsigned long long m = mask;
+  const int first = __popcll(m & ((1ull << (y / k)) - 1ull)), n = __popcll(m) - first;
+  if (first % kRowTokens != 0) return 0;
   for (int i = threadIdx.x; i < T * k; i += blockDim.x)
-    if (ids[i] == e) list[__popcll(m & ((1ull << (i / k)) - 1ull))] = i;
+    if (__ldcg(ids + i) == e) {
+      const int at = __popcll(m & ((1ull << (i / k)) - 1ull)) - first;
+      if (at >= 0 && at < kRowTokens) list[at] = i;
+    }
   __syncthreads();
-  return __popcll(m);
+  return n < kRowTokens ? n : kRowTokens;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams p, float* h) {
-  __shared__ int list[kFewTokens];
-  const int e = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = few_pairs(p.ids, p.T, p.k, e, list);
-  const int f = blockIdx.x * (kRowThreads / 32) + warp;
-  if (n == 0 || f >= p.F) return;
-  const bool glu = p.act == (int)Act::kSwiGLU;
-  const T* wg = (const T*)p.w1 + (long long)e * p.w1_estride + (long long)f * p.w1_stride;
-  const T* wu = wg + (long long)p.F * p.w1_stride;
-  for (int i0 = 0; i0 < n; i0 += kRowTokens) {
-    float g[kRowTokens] = {}, u[kRowTokens] = {};
-    const T* x[kRowTokens];
-    for (int i = 0; i < kRowTokens; ++i)
-      x[i] = (const T*)p.x + (long long)(list[min(i0 + i, n - 1)] / p.k) * p.x_stride;
+__device__ __forceinline__ void unpack16(const uint4& v, float (&f)[16 / sizeof(T)]) {
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = as_float(((const T*)&v)[i]);
+}
+
+// Two rows of W1 against NT of the expert's tokens, pairs list[0 .. n): h[pair, f] = act(W1[e] x + b1).
+template <typename T, bool VEC, int NT>
+__device__ __forceinline__ void few_hidden_rows(const FewExpertParams& p, float* h, const int* list, int n, int e, int f, bool glu) {
+  const int lane = threadIdx.x & 31;
+  const bool two = glu || f + 1 < p.F;
+  const T* wa = (const T*)p.w1 + (long long)e * p.w1_estride + (long long)f * p.w1_stride;
+  const T* wb = !two ? wa : wa + (glu ? p.F : 1) * p.w1_stride;
+  float a[NT] = {}, b[NT] = {};
+  const T* x[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) x[i] = (const T*)p.x + (long long)(list[i < n ? i : n - 1] / p.k) * p.x_stride;
+  if constexpr (VEC) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll(NT == 1 ? 8 : 4)
+    for (int d = lane * V; d < p.D; d += 32 * V) {
+      float fa[V], fb[V], fx[V];
+      unpack16<T>(__ldg((const uint4*)(wa + d)), fa);
+      unpack16<T>(__ldg((const uint4*)(wb + d)), fb);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        unpack16<T>(__ldg((const uint4*)(x[i] + d)), fx);
+        float sa = 0.f, sb = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          sa = fmaf(fa[v], fx[v], sa);
+          sb = fmaf(fb[v], fx[v], sb);
+        }
+        a[i] += sa;
+        b[i] += sb;
+      }
+    }
+  } else {
+#pragma unroll(NT == 1 ? 8 : 4)
     for (int d = lane; d < p.D; d += 32) {
-      const float a = as_float(wg[d]), b = glu ? as_float(wu[d]) : 0.f;
+      const float fa = as_float(wa[d]), fb = as_float(wb[d]);
 #pragma unroll
-      for (int i = 0; i < kRowTokens; ++i) {
-        const float v = as_float(x[i][d]);
-        g[i] = fmaf(a, v, g[i]);
-        if (glu) u[i] = fmaf(b, v, u[i]);
+      for (int i = 0; i < NT; ++i) {
+        const float fx = as_float(x[i][d]);
+        a[i] = fmaf(fa, fx, a[i]);
+        b[i] = fmaf(fb, fx, b[i]);
       }
     }
+  }
 #pragma unroll
-    for (int i = 0; i < kRowTokens; ++i) {
-      g[i] = warp_sum(g[i]);
-      u[i] = warp_sum(u[i]);
-      if (lane == 0 && i0 + i < n) {
-        const float* b1 = p.b1 ? p.b1 + (long long)e * (glu ? 2 : 1) * p.F : nullptr;
-        const float z = g[i] + (b1 ? b1[f] : 0.f);
-        h[(long long)list[i0 + i] * p.F + f] =
-            glu ? serving_swiglu(z, u[i] + (b1 ? b1[p.F + f] : 0.f)) : serving_act(z, p.act);
-      }
+  for (int i = 0; i < NT; ++i) {
+    a[i] = warp_sum(a[i]);
+    b[i] = warp_sum(b[i]);
+    if (lane == 0 && i < n) {
+      const float* b1 = p.b1 ? p.b1 + (long long)e * (glu ? 2 : 1) * p.F : nullptr;
+      float* at = h + (long long)list[i] * p.F + f;
+      const float za = a[i] + (b1 ? b1[f] : 0.f);
+      const float zb = b[i] + (b1 && two ? b1[glu ? p.F + f : f + 1] : 0.f);
+      at[0] = glu ? serving_swiglu(za, zb) : serving_act(za, p.act);
+      if (!glu && two) at[1] = serving_act(zb, p.act);
     }
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams p, const float* hidden, float* y) {
-  __shared__ int list[kFewTokens];
-  const int e = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = few_pairs(p.ids, p.T, p.k, e, list);
-  const int o = blockIdx.x * (kRowThreads / 32) + warp;
-  if (n == 0 || o >= p.O) return;
-  const T* w = (const T*)p.w2 + (long long)e * p.w2_estride + (long long)o * p.w2_stride;
-  for (int i0 = 0; i0 < n; i0 += kRowTokens) {
-    float acc[kRowTokens] = {};
-    const float* h[kRowTokens];
-    for (int i = 0; i < kRowTokens; ++i) h[i] = hidden + (long long)list[min(i0 + i, n - 1)] * p.F;
-    for (int f = lane; f < p.F; f += 32) {
-      const float a = as_float(w[f]);
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams p, float* h) {
+  __shared__ int list[kRowTokens];
+  const bool glu = p.act == (int)Act::kSwiGLU;
+  griddep_wait();
+  griddep_launch_dependents();
+  int e;
+  const int n = few_pairs(p.ids, p.T, p.k, blockIdx.y, list, e);
+  const int f = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * (glu ? 1 : 2);   // rows f and F + f, or f and f + 1
+  if (n == 0 || f >= p.F) return;
+  if (n == 1) few_hidden_rows<T, VEC, 1>(p, h, list, 1, e, f, glu);
+  else few_hidden_rows<T, VEC, kRowTokens>(p, h, list, n, e, f, glu);
+}
+
+// out[t, o] = sum_j gate (W2[e] h[t, j] + b2[e]) + residual, four o to a CTA: its
+// warps share the choices and, where these are fewer than the warps, their F.
+constexpr int kOutRows = 4;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams p, const float* h) {
+  __shared__ float part[kRowWarps][kOutRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = blockIdx.y;
+  const int o0 = blockIdx.x * kOutRows;
+  const int pieces = kRowWarps / p.k, j = warp % p.k, piece = warp / p.k;
+  griddep_wait();
+  griddep_launch_dependents();
+  float acc[kOutRows] = {};
+  const int e = piece < pieces ? __ldcg(p.ids + t * p.k + j) : -1;
+  if (e >= 0) {
+    const T* w = (const T*)p.w2 + (long long)e * p.w2_estride;
+    const T* row[kOutRows];
 #pragma unroll
-      for (int i = 0; i < kRowTokens; ++i) acc[i] = fmaf(a, h[i][f], acc[i]);
-    }
+    for (int r = 0; r < kOutRows; ++r) row[r] = w + (long long)(o0 + r < p.O ? o0 + r : p.O - 1) * p.w2_stride;
+    const float* hj = h + (long long)(t * p.k + j) * p.F;
+    constexpr int V = VEC ? 16 / sizeof(T) : 1;
+    const int n = p.F / V, i1 = (int)((long long)n * (piece + 1) / pieces);
+    if constexpr (VEC) {
+#pragma unroll 4
+      for (int i = (int)((long long)n * piece / pieces) + lane; i < i1; i += 32) {
+        float fh[V];
 #pragma unroll
-    for (int i = 0; i < kRowTokens; ++i) {
-      acc[i] = warp_sum(acc[i]);
-      if (lane == 0 && i0 + i < n)
-        y[(long long)list[i0 + i] * p.O + o] = acc[i] + (p.b2 ? p.b2[(long long)e * p.O + o] : 0.f);
+        for (int q = 0; q < V / 4; ++q) {
+          const float4 v = __ldcg((const float4*)(hj + i * V) + q);
+          fh[4 * q] = v.x; fh[4 * q + 1] = v.y; fh[4 * q + 2] = v.z; fh[4 * q + 3] = v.w;
+        }
+#pragma unroll
+        for (int r = 0; r < kOutRows; ++r) {
+          float fw[V], s = 0.f;
+          unpack16<T>(__ldg((const uint4*)row[r] + i), fw);
+#pragma unroll
+          for (int v = 0; v < V; ++v) s = fmaf(fw[v], fh[v], s);
+          acc[r] += s;
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int i = (int)((long long)n * piece / pieces) + lane; i < i1; i += 32) {
+        const float fh = __ldcg(hj + i);
+#pragma unroll
+        for (int r = 0; r < kOutRows; ++r) acc[r] = fmaf(as_float(row[r][i]), fh, acc[r]);
+      }
     }
   }
+  const float g = e >= 0 ? __ldcg(p.gates + t * p.k + j) : 0.f;
+#pragma unroll
+  for (int r = 0; r < kOutRows; ++r) {
+    acc[r] = warp_sum(acc[r]);
+    if (lane == r) {
+      float v = acc[r];
+      if (e >= 0 && piece == 0 && p.b2 && o0 + r < p.O) v += __ldg(p.b2 + (long long)e * p.O + o0 + r);
+      part[warp][r] = e >= 0 ? g * v : 0.f;
+    }
+  }
+  __syncthreads();
+  const int o = o0 + threadIdx.x;
+  if (threadIdx.x >= kOutRows || o >= p.O) return;
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < kRowWarps; ++i) v += part[i][threadIdx.x];
+  if (p.residual) v += load_elem(p.residual, (long long)t * p.res_stride + o, p.res_bf16);
+  store_elem(p.out, (long long)t * p.out_stride + o, v, p.out_bf16);
 }
 
-__global__ void __launch_bounds__(kRowThreads) few_join_kernel(FewExpertParams p, const float* y) {
-  const long long i = (long long)blockIdx.x * kRowThreads + threadIdx.x;
-  if (i >= (long long)p.T * p.O) return;
-  const int t = (int)(i / p.O), o = (int)(i % p.O);
-  float acc = 0.f;
-  for (int j = 0; j < p.k; ++j)
-    if (p.ids[t * p.k + j] >= 0) acc = fmaf(p.gates[t * p.k + j], y[(long long)(t * p.k + j) * p.O + o], acc);
-  if (p.residual) acc += load_elem(p.residual, (long long)t * p.res_stride + o, p.res_bf16);
-  store_elem(p.out, (long long)t * p.out_stride + o, acc, p.out_bf16);
+template <typename T, bool VEC>
+static void launch_rows_vec(const FewExpertParams& p, float* h, cudaStream_t s) {
+  const int per = kRowWarps * (p.act == (int)Act::kSwiGLU ? 1 : 2);
+  const dim3 grid((p.F + per - 1) / per, p.T * p.k);
+  launch_with_pdl(few_hidden_kernel<T, VEC>, grid, dim3(kRowThreads), 0, s, true, p, h);
+  launch_with_pdl(few_output_kernel<T, VEC>, dim3((p.O + kOutRows - 1) / kOutRows, p.T), dim3(kRowThreads), 0, s, true, p,
+                  (const float*)h);
 }
 
 template <typename T>
-static void launch_rows(const FewExpertParams& p, float* h, float* y, cudaStream_t s) {
-  constexpr int W = kRowThreads / 32;
-  few_hidden_kernel<T><<<dim3((p.F + W - 1) / W, p.E), kRowThreads, 0, s>>>(p, h);
-  few_output_kernel<T><<<dim3((p.O + W - 1) / W, p.E), kRowThreads, 0, s>>>(p, h, y);
-  few_join_kernel<<<(unsigned)(((long long)p.T * p.O + kRowThreads - 1) / kRowThreads), kRowThreads, 0, s>>>(p, y);
+static void launch_rows(const FewExpertParams& p, float* h, bool vec, cudaStream_t s) {
+  if (vec) launch_rows_vec<T, true>(p, h, s);
+  else launch_rows_vec<T, false>(p, h, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -313,6 +406,10 @@ int serving_sm_count() {
 static long long up256(long long v) { return (v + 255) / 256 * 256; }
 
 constexpr int kFewShared = 232448 - 10 * 1024 - 1024;  // dynamic shared memory besides the kernel's own and the alignment
+// By rows up to so many bytes of weights, counted once for each (token, choice).  Measured, rows against tensor cores (us):
+// bf16 64 experts 512 x 352, 1 token (6.5 MB) 11 / 17, 4 tokens (26 MB) 21 / 21, 32 experts 1024 x 1024, 2 tokens (50 MB)
+// 29 / 26; fp32 8 experts 1024 x 4096, 1 token (67 MB) 24 / 49, 4 (268 MB) 52 / 76, 8 (537 MB) 82 / 86, 16 130 / 89.
+constexpr double kFewRowBytes = 30e6, kFewRowBytesFp32 = 400e6;
 constexpr int kFewJoinRoom = 24 * 1024;                // of the join's CTA beside it
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p) {
@@ -322,11 +419,13 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
     return ((uintptr_t)base & 15) == 0 && (row * eb) % 16 == 0 && (p.E == 1 || (expert * eb) % 16 == 0);
   };
   // TMA reads rows that start on 16 bytes
-  r.tensor = aligned(p.w1, p.w1_stride, p.w1_estride) && aligned(p.w2, p.w2_stride, p.w2_estride);
+  const bool rows16 = aligned(p.w1, p.w1_stride, p.w1_estride) && aligned(p.w2, p.w2_stride, p.w2_estride);
   const int pairs = p.T * p.k;
+  const double bytes = (double)pairs * eb * ((p.act == (int)Act::kSwiGLU ? 2.0 : 1.0) * p.F * p.D + (double)p.O * p.F);
+  r.tensor = rows16 && bytes > (p.bf16 ? kFewRowBytes : kFewRowBytesFp32);
   if (!r.tensor) {
+    r.vec = rows16 && (p.D * eb) % 16 == 0 && (p.F * eb) % 16 == 0 && aligned(p.x, p.T > 1 ? p.x_stride : 0, 0);
     r.a_bytes = up256((long long)pairs * p.F * 4);
-    r.b_bytes = up256((long long)pairs * p.O * 4);
     return r;
   }
   r.grid = serving_sm_count();
@@ -371,10 +470,9 @@ static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CU
 void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
   char* ws = (char*)workspace;
   float* a = (float*)(ws + plan.packed_bytes);
-  float* b = (float*)(ws + plan.packed_bytes + plan.a_bytes);
   if (!plan.tensor) {
-    if (p.bf16) launch_rows<__nv_bfloat16>(p, a, b, s);
-    else launch_rows<float>(p, a, b, s);
+    if (p.bf16) launch_rows<__nv_bfloat16>(p, a, plan.vec != 0, s);
+    else launch_rows<float>(p, a, plan.vec != 0, s);
     return;
   }
   const cuuint64_t eb = p.bf16 ? 2 : 4;
