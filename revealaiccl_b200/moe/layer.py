@@ -31,6 +31,7 @@ import torch.distributed as dist
 from ..ops import status as _status
 from ..ops._native import host, kernels
 from ..ops.grouped_gemm import ACT_IDS, pick_bn, swiglu_interleave, swiglu_interleave_bias
+from ..ops.moe_few import MAX_TOKENS as FEW_TOKENS, moe_few_tokens
 from ..parallel.peer import PeerChannel, device_view
 from ..scheduling.compiled import StaticPlanCompiler, _plan_flat
 from ..topology.loader import load_rear4_topology
@@ -83,6 +84,10 @@ class ProgressiveMoELayer:
         # ---- inputs and weights (deterministic)
         self.inputs = make_rank_inputs(cfg, self.rank, W, dev, seed=seed)
         self.weights = make_weights(cfg, dev, seed=seed)
+        # few_tokens: the topology mask of the first positions
+        pos = torch.arange(FEW_TOKENS, device=dev)
+        self._few_mask = torch.zeros((FEW_TOKENS, E), dtype=torch.bool, device=dev)
+        self._few_mask[pos, pos % E] = True
         swiglu = cfg.activation == "swiglu"
         self.bn1 = pick_bn(cfg.gemm1_n, swiglu)
         self.bn2 = pick_bn(cfg.out_dim)
@@ -372,6 +377,31 @@ class ProgressiveMoELayer:
             host_out.copy_(self.out, non_blocking=True)
         torch.cuda.current_stream(self.device).wait_stream(self.comm_stream)
         return host_out
+
+    def few_tokens(self, x: torch.Tensor, *, block_mask: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """This layer on a decode step: x [T, D] of the layer's type, T <= 64, on
+        its device; returns (out [T, out_dim], expert ids [T, top_k], gates).
+
+        Runs on the current stream with the weights that every rank holds, in
+        three launches and without the progressive machinery (no chunks, no
+        dispatch, no peers), so it needs no other rank and leaves the layer's
+        buffers alone.  Router, masks and gates are the layer's, row t taking
+        position t of the topology mask; the synthetic per-chunk logit bias of a
+        batch does not apply.  fp32 layers are computed to fp32 accuracy here,
+        where the batch path uses tf32 products.  ``block_mask`` ([E] or [T, E])
+        replaces the layer's own masks; ``residual`` is added to the result.
+        """
+        if block_mask is None:
+            own = self.inputs.block_mask
+            if self.cfg.mask_mode == "topology_source":
+                rows = self._few_mask[: x.shape[0]]
+                block_mask = rows if own is None else rows | own.bool()
+            else:
+                block_mask = own
+        w, cfg = self.weights, self.cfg
+        return moe_few_tokens(x, w.router_w, w.w1, w.w2, top_k=cfg.top_k, act=cfg.activation, gate_mode=cfg.gate_mode,
+                              router_b=w.router_b, b1=w.b1, b2=w.b2, block_mask=block_mask, residual=residual, out=out)
 
     def clear_returns(self) -> None:
         """Zero this rank's return rows and return identity rows (so a lost

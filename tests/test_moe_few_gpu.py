@@ -30,6 +30,17 @@ def _make(T, D, E, F, O, act, dtype, seed=0, bias=False):
     return a
 
 
+def _sizes(tensor, dtype, pairs, O=None):
+    """(D, F, O): widths whose (token, choice) pairs read few bytes of weights (by rows, on CUDA cores) or many (on the tensor
+    cores, from 30 MB in bf16 and 400 MB in fp32), as csrc/kernels/moe_few.cu chooses."""
+    if not tensor:
+        return 256, 96, O or 128
+    D, F = (512, 1000) if dtype == BF16 else (1024, 1400)
+    while pairs * (2 if dtype == BF16 else 4) * 3 * D * F < (32e6 if dtype == BF16 else 420e6):
+        F += 1000
+    return D, F, O or D
+
+
 def _check(a, k, act, gate_mode, norm=True, **kw):
     out, ids, gates = _moe(**a, top_k=k, act=act, gate_mode=gate_mode, **kw)
     kw = {n: v for n, v in kw.items() if n != "out"}
@@ -64,31 +75,42 @@ def test_sizes(T, D, E, k, F, O, dtype):
     _check(_make(T, D, E, F, O, act, dtype, seed=T + D, bias=(T + k) % 2 == 0), k, act, mode)
 
 
-@pytest.mark.parametrize("act", ["swiglu", "relu", "gelu", "silu", "none"])
-@pytest.mark.parametrize("mode", ["topk_softmax", "softmax", "none"])
+@pytest.mark.parametrize("tensor", [False, True], ids=["rows", "tensor"])
+@pytest.mark.parametrize("act,mode", [("swiglu", "topk_softmax"), ("relu", "softmax"), ("gelu", "none"), ("silu", "topk_softmax"),
+                                      ("none", "softmax"), ("swiglu", "none"), ("swiglu", "softmax")])
 @pytest.mark.parametrize("dtype,out_dtype,res_dtype", [(BF16, BF16, BF16), (BF16, FP32, BF16), (BF16, BF16, FP32), (FP32, FP32, FP32),
                                                        (FP32, FP32, BF16)])
-def test_acts_gates_types(act, mode, dtype, out_dtype, res_dtype):
-    a = _make(9, 256, 12, 160, 192, act, dtype, seed=3, bias=True)
-    r = torch.randn(9, 192, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(res_dtype)
+def test_acts_gates_types(act, mode, dtype, out_dtype, res_dtype, tensor):
+    D, F, O = _sizes(tensor, dtype, 9 if act != "swiglu" else 18, 192)
+    a = _make(9, D, 12, F, O, act, dtype, seed=3, bias=True)
+    r = torch.randn(9, O, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).to(res_dtype)
     out, _, _ = _check(a, 3, act, mode, residual=r, out_dtype=out_dtype)
     assert out.dtype == out_dtype
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
-@pytest.mark.parametrize("T", [1, 6, 64])
-def test_every_token_on_one_expert(T, dtype):
-    a = _make(T, 256, 16, 512, 256, "swiglu", dtype, bias=True)
+@pytest.mark.parametrize("T", [1, 6, 17, 33, 49, 64])
+@pytest.mark.parametrize("tensor", [False, True], ids=["rows", "tensor"])
+def test_every_token_on_one_expert(T, dtype, tensor):
+    D, F, O = _sizes(tensor, dtype, T, 256)
+    a = _make(T, D, 16 if T > 1 else 2, F, O, "swiglu", dtype, bias=True)
+    if T == 1:
+        a["router_b"][1] += 100.0
+        _, ids, _ = _check(a, 1, "swiglu", "softmax")
+        assert (ids == 1).all()
+        return
     a["router_b"][11] += 100.0
     _, ids, _ = _check(a, 1, "swiglu", "softmax")
     assert (ids == 11).all()
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
-def test_masks(dtype):
+@pytest.mark.parametrize("tensor", [False, True], ids=["rows", "tensor"])
+def test_masks(dtype, tensor):
     """Blocked experts, tokens with fewer free experts than choices, tokens with none; what is blocked is not read."""
     T, E = 12, 8
-    a = _make(T, 256, E, 96, 128, "swiglu", dtype, bias=True)
+    D, F, O = _sizes(tensor, dtype, T * 2, 128)
+    a = _make(T, D, E, F, O, "swiglu", dtype, bias=True)
     g = torch.Generator(DEV).manual_seed(5)
     mask = torch.rand(T, E, generator=g, device=DEV) < 0.4
     mask[0] = True            # none left
@@ -136,9 +158,11 @@ def test_ties_go_to_the_lower_expert():
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
-def test_special_values_stay_where_they_are(dtype):
+@pytest.mark.parametrize("tensor", [False, True], ids=["rows", "tensor"])
+def test_special_values_stay_where_they_are(dtype, tensor):
     """A NaN or infinite token, and weights of experts that nobody chose, leave the other tokens alone."""
-    a = _make(6, 128, 16, 80, 96, "swiglu", dtype)
+    D, F, O = _sizes(tensor, dtype, 12, 96)
+    a = _make(6, D, 16, F, O, "swiglu", dtype)
     base, ids, _ = _moe(**a, top_k=2, act="swiglu", gate_mode="topk_softmax")
     unused = [e for e in range(16) if not (ids == e).any()]
     b = {n: v.clone() for n, v in a.items()}
@@ -156,9 +180,11 @@ def test_special_values_stay_where_they_are(dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("offset,pad", [(0, 8), (1, 0), (8, 24)])
-def test_strides(dtype, offset, pad):
+@pytest.mark.parametrize("tensor", [False, True], ids=["rows", "tensor"])
+def test_strides(dtype, offset, pad, tensor):
     """Every tensor as a window of a wider buffer, every other expert of a larger bank; what lies around out stays."""
-    T, D, E, F, O = 5, 128, 6, 80, 72
+    T, E = 5, 6
+    D, F, O = _sizes(tensor, dtype, T * 2, 72)
     g = torch.Generator(DEV).manual_seed(2)
 
     def window(*shape, s):
@@ -209,7 +235,7 @@ def test_far_experts():
 
 def test_repeats_and_streams():
     """The same bits every time, on side streams too and while another call runs."""
-    sets = [_make(T, 512, E, F, 512, "swiglu", BF16, seed=T) for T, E, F in ((1, 64, 352), (30, 16, 512), (64, 8, 1000))]
+    sets = [_make(T, 512, E, F, 512, "swiglu", BF16, seed=T) for T, E, F in ((1, 64, 352), (30, 16, 512), (64, 8, 1000), (3, 4, 5000))]
     want = [_moe(**a, top_k=2) for a in sets]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in sets]
@@ -223,11 +249,12 @@ def test_repeats_and_streams():
         assert all(torch.equal(u, v) for u, v in zip(g, want[i % len(want)]))
 
 
-def test_a_block_of_a_served_model():
+@pytest.mark.parametrize("F", [96, 1000], ids=["rows", "tensor"])
+def test_a_block_of_a_served_model(F):
     """Attention output projection, experts and a shared expert as one decode step, eager and as two captured graphs
     replayed in turn, with new inputs each time."""
     from revealaiccl_b200.ops.linear import linear
-    T, D, E, F, S = 11, 256, 16, 96, 160
+    T, D, E, S = 11, 256, 16, 160
     a = _make(T, D, E, F, D, "swiglu", BF16, seed=8)
     g = torch.Generator(DEV).manual_seed(9)
     attn = torch.randn(T, D, generator=g, device=DEV).bfloat16()
@@ -267,3 +294,36 @@ def test_a_block_of_a_served_model():
         graph.replay()
         assert all(torch.equal(u, v) for u, v in zip(result, want))
         check(result)
+
+
+@pytest.mark.parametrize("dtype,act,k", [("bf16", "swiglu", 2), ("fp32", "gelu", 2), ("fp32", "relu", 1)])
+def test_layer_few_tokens(dtype, act, k):
+    """A layer's decode step beside its batches: same router, masks and experts, and the batch's results stay."""
+    from revealaiccl_b200.moe.config import MoELayerConfig
+    from revealaiccl_b200.moe.layer import ProgressiveMoELayer
+
+    cfg = MoELayerConfig(
+        name=f"few_{dtype}_{act}", tokens_per_rank=512, hidden=256, experts=8, top_k=k, chunk_sizes=(64,) * 8, ffn_hidden=128,
+        out_dim=256, activation=act, dtype=dtype, placement="contiguous", gate_mode="topk_softmax" if k > 1 else "none",
+        mask_mode="topology_source" if act == "relu" else "none", router_init="unit_logits", expert_init="normal002")
+    layer = ProgressiveMoELayer(cfg, device=torch.device("cuda", 0), timeout_s=5.0)
+    try:
+        before = layer.forward("early").clone()
+        w = layer.weights
+        for T in (1, 5, 64):
+            x = layer.inputs.tokens[:T].clone()
+            res = torch.randn(T, cfg.out_dim, device=DEV).to(x.dtype)
+            out, ids, gates = layer.few_tokens(x, residual=res)
+            mask = None
+            if cfg.mask_mode == "topology_source":
+                mask = torch.zeros(T, cfg.experts, dtype=torch.bool, device=DEV)
+                mask[torch.arange(T), torch.arange(T) % cfg.experts] = True
+            want, bound, rid, rg, grel, gap = moe64(x, w.router_w, w.w1, w.w2, top_k=k, act=act, gate_mode=cfg.gate_mode,
+                                                    router_b=w.router_b, b1=w.b1, b2=w.b2, block_mask=mask, residual=res)
+            assert gap > 4 * U * ((cfg.hidden / 32) ** 0.5 + 8)
+            assert torch.equal(ids.cpu(), rid) and torch.equal(ids, layer.expert_ids[:T])
+            check_close(out, want, bound)
+        assert torch.equal(layer.forward("early"), before)
+        assert layer.verify()["pass"]
+    finally:
+        layer.close()
