@@ -87,9 +87,10 @@ struct FewPlan {
   int part0[kFewExperts + 1];                // by place: first row in part
   int parts[kFewExperts + 1];                // by place: CTAs with a part
   int ne;
+  int q, groups;                             // units that stay together; of these to an expert
 };
 
-// CTA of unit u where U units are dealt to G <= U CTAs: CTA c has units [U c / G, U (c + 1) / G).
+// CTA of group u where U groups are dealt to G <= U CTAs: CTA c has groups [U c / G, U (c + 1) / G).
 __device__ __forceinline__ int few_cta(long long u, long long U, int G) { return (int)(((u + 1) * G - 1) / U); }
 
 __device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, int UE, int grid) {
@@ -113,14 +114,23 @@ __device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, i
       ne += __popc(b);
     }
     __syncwarp();
-    const long long U = (long long)ne * UE;
+    // Where a CTA has few units, they go by fours (64 hidden rows, whole 128-byte rows of W2) or pairs if no CTA gets more
+    // of them for that than a thirty-second: fewer CTAs then share two experts, and fewer loads are short (64 experts, 1
+    // token: 43.5 -> 31.7 us).
+    long long U = 0, least = ((long long)ne * UE + grid - 1) / grid;
+    int q = least <= 32 ? 4 : 1, groups = 0;
+    for (;; q >>= 1) {
+      groups = (UE + q - 1) / q;
+      U = (long long)ne * groups;
+      if (q == 1 || (U + grid - 1) / grid * q * 32 <= least * 33) break;
+    }
     const int G = U < grid ? (int)U : grid;
     int part = 0;
     for (int i0 = 0; i0 < ne; i0 += 32) {
       const int i = i0 + lane;
       int n = 0, rows = 0;
       if (i < ne) {
-        n = few_cta((long long)(i + 1) * UE - 1, U, G) - few_cta((long long)i * UE, U, G) + 1;
+        n = few_cta((long long)(i + 1) * groups - 1, U, G) - few_cta((long long)i * groups, U, G) + 1;
         rows = n * __popcll(s.mask[s.used[i]]);
       }
       int rs = rows;
@@ -132,7 +142,7 @@ __device__ __forceinline__ void few_plan(const FewExpertParams& p, FewPlan& s, i
       if (i < ne) { s.part0[i] = part + rs - rows; s.parts[i] = n; }
       part += __shfl_sync(0xffffffffu, rs, 31);
     }
-    if (lane == 0) s.ne = ne;
+    if (lane == 0) { s.ne = ne; s.q = q; s.groups = groups; }
   }
   __syncthreads();
 }
@@ -146,11 +156,11 @@ struct FewRun {
 };
 
 struct FewWalk {
-  long long u, u1, U;
+  long long u, u1, U;   // groups
   int UE, G, s, n, a, place;
   __device__ void start(const FewPlan& plan, int UE_, int grid) {
     UE = UE_;
-    U = (long long)plan.ne * UE;
+    U = (long long)plan.ne * plan.groups;
     G = U < grid ? (int)U : grid;
     const int c = blockIdx.x;
     u = c < G ? U * c / G : 0;
@@ -162,15 +172,16 @@ struct FewWalk {
   __device__ bool next(const FewPlan& plan, int hrows, int parts, int ups, int& off, FewRun& r) {
     if (s >= n) {
       if (u >= u1) return false;
-      const int pl = (int)(u / UE), first = (int)(u - (long long)pl * UE);
-      const int count = (int)(u1 - u < UE - first ? u1 - u : UE - first);
+      const int pl = (int)(u / plan.groups), first = (int)(u - (long long)pl * plan.groups);
+      const int take = (int)(u1 - u < plan.groups - first ? u1 - u : plan.groups - first);
+      const int count = take * plan.q < UE - first * plan.q ? take * plan.q : UE - first * plan.q;   // units
       const int np = (__popcll(plan.mask[plan.used[pl]]) + 15) & ~15;
       if (off > 0 && off + (count + ups - 1) / ups * np * parts > hrows) return false;
       place = pl;
-      a = first;
+      a = first * plan.q;
       n = count;
       s = 0;
-      u += n;
+      u += take;
     } else if (off > 0) {
       return false;
     }
@@ -216,66 +227,83 @@ struct FewAcc {
   }
 };
 
-// out[t, o0 .. o0 + 128) of one token: the parts of all its choices, by choice,
-// then CTA, are dealt to the warps in turn, each times its choice's gate; the
-// warps' sums are added in order.  At most grid + 2 k loads of a column in all,
-// so what counts is how many are in flight, and that all but these loads is
-// done before the experts' kernel ends: its CTAs leave room for these beside
+// out[t, o0 .. o0 + 128) of a token: the parts of all its choices, by choice,
+// then CTA, are dealt to its warps in turn, each times its choice's gate; the
+// warps' sums are added in order.  A CTA has one token, or from five on four of
+// them.  At most grid + 2 k loads of a column for each, so what counts is how
+// many are in flight, and, up to 16 tokens, that all but these loads is done
+// before the experts' kernel ends: its CTAs then leave room for these beside
 // them, and which rows to add follows from the routing alone, whose kernel had
 // ended before the experts' kernel allowed this launch.
 constexpr int kFewJoinThreads = 512;
+constexpr int kFewJoinItems = 192;       // of a token at most; the launch checks grid + 2 k
 
+template <int TOKENS>
 __global__ void __launch_bounds__(kFewJoinThreads) few_join_parts_kernel(FewTcParams p) {
-  constexpr int W = kFewJoinThreads / 32;
+  constexpr int W = kFewJoinThreads / 32, tokens = TOKENS;
   __shared__ FewPlan plan;
   __shared__ __align__(16) float red[W][128];
-  __shared__ int row[kFewJoinThreads];
-  __shared__ float weight[kFewJoinThreads];
-  __shared__ int4 term[kFewTopK];     // a choice's first row in part, rows to the next part, parts, expert
-  __shared__ float gate[kFewTopK];
+  __shared__ int row[TOKENS * kFewJoinItems];
+  __shared__ float weight[TOKENS * kFewJoinItems];
+  __shared__ int4 term[TOKENS][kFewTopK];     // a choice's first row in part, rows to the next part, parts, expert
+  __shared__ float gate[TOKENS][kFewTopK];
+  __shared__ int items[TOKENS];
   const FewExpertParams& e = p.e;
-  const int t = blockIdx.y, o0 = blockIdx.x * 128;
+  const int t0 = blockIdx.y * tokens, o0 = blockIdx.x * 128;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float* col = p.part + o0 + lane * 4;
-  const int o = o0 + threadIdx.x;
-  const bool writes = threadIdx.x < 128 && o < e.O;
-  float res = 0.f;
+  // this thread's output
+  const int sub = threadIdx.x >> 7, t = t0 + sub, o = o0 + (threadIdx.x & 127);
+  const bool writes = sub < tokens && t < e.T && o < e.O;
+  float res = 0.f, bias = 0.f;
   if (writes && e.residual) res = load_elem(e.residual, (long long)t * e.res_stride + o, e.res_bf16);
   for (int i = threadIdx.x; i < e.E; i += kFewJoinThreads) plan.mask[i] = 0ull;
   __syncthreads();
   few_plan(e, plan, (e.F + 15) / 16, p.grid);
-  if (threadIdx.x < kFewTopK) {
-    const int j = threadIdx.x, x = j < e.k ? __ldcg(e.ids + t * e.k + j) : -1;
+  if (threadIdx.x < TOKENS * kFewTopK) {
+    const int s = threadIdx.x / kFewTopK, j = threadIdx.x % kFewTopK, tt = t0 + s;
+    const bool in = tt < e.T && j < e.k;
+    const int x = in ? __ldcg(e.ids + tt * e.k + j) : -1;
     int4 v = make_int4(0, 0, 0, 0);
     if (x >= 0) {
       const unsigned long long m = plan.mask[x];
       const int place = plan.index[x];
-      v = make_int4(plan.part0[place] + __popcll(m & ((1ull << t) - 1ull)), __popcll(m), plan.parts[place], x);
+      v = make_int4(plan.part0[place] + __popcll(m & ((1ull << tt) - 1ull)), __popcll(m), plan.parts[place], x);
     }
-    term[j] = v;
-    gate[j] = j < e.k ? __ldcg(e.gates + t * e.k + j) : 0.f;
+    term[s][j] = v;
+    gate[s][j] = in ? __ldcg(e.gates + tt * e.k + j) : 0.f;
   }
   __syncthreads();
-  int items = 0;
-  for (int j = 0; j < e.k; ++j) items += term[j].z;
-  {
-    int c = threadIdx.x, j = 0;      // items <= kFewJoinThreads: a token's choices have at most grid + 2 k parts
-    while (j + 1 < e.k && c >= term[j].z) c -= term[j++].z;
-    row[threadIdx.x] = term[j].x + c * term[j].y;
-    weight[threadIdx.x] = gate[j];
+  for (int i = threadIdx.x; i < tokens * kFewJoinItems; i += kFewJoinThreads) {
+    const int s = i / kFewJoinItems;
+    int c = i - s * kFewJoinItems, j = 0;
+    while (j < e.k && c >= term[s][j].z) c -= term[s][j++].z;
+    if (j < e.k) {
+      row[i] = term[s][j].x + c * term[s][j].y;
+      weight[i] = gate[s][j];
+    }
   }
-  float bias = 0.f;
+  if (threadIdx.x < tokens) {
+    int n = 0;
+    for (int j = 0; j < e.k; ++j) n += term[threadIdx.x][j].z;
+    items[threadIdx.x] = n;
+  }
   if (e.b2 && writes)
     for (int j = 0; j < e.k; ++j)
-      if (term[j].z > 0) bias = fmaf(gate[j], __ldg(e.b2 + (long long)term[j].w * e.O + o), bias);
+      if (term[sub][j].z > 0) bias = fmaf(gate[sub][j], __ldg(e.b2 + (long long)term[sub][j].w * e.O + o), bias);
   __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
+  constexpr int per = W / tokens;
+  const int mine = w / per;
+  const float* col = p.part + o0 + lane * 4;
+  const int* rows = row + mine * kFewJoinItems;
+  const float* weights = weight + mine * kFewJoinItems;
+  const int n = items[mine];
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-  for (int i = w; i < items; i += W) {
-    const float4 a = __ldcg((const float4*)(col + (long long)row[i] * p.Op));
-    const float g = weight[i];
+  for (int i = w % per; i < n; i += per) {
+    const float4 a = __ldcg((const float4*)(col + (long long)rows[i] * p.Op));
+    const float g = weights[i];
     v.x = fmaf(g, a.x, v.x);
     v.y = fmaf(g, a.y, v.y);
     v.z = fmaf(g, a.z, v.z);
@@ -284,9 +312,9 @@ __global__ void __launch_bounds__(kFewJoinThreads) few_join_parts_kernel(FewTcPa
   *(float4*)&red[w][lane * 4] = v;
   __syncthreads();
   if (!writes) return;
-  float out = red[0][threadIdx.x];
+  float out = 0.f;
 #pragma unroll
-  for (int i = 1; i < W; ++i) out += red[i][threadIdx.x];
+  for (int i = 0; i < per; ++i) out += red[sub * per + i][threadIdx.x & 127];
   store_elem(e.out, (long long)t * e.out_stride + o, out + bias + res, e.out_bf16);
 }
 
@@ -620,7 +648,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         again.next(plan, hrows, C::PARTS, C::UPS, off, r);
         // product 2: this CTA's part of the expert's result.  A group of tiles always belongs to the same epilogue
         // group, so a cut run's later pieces are added by the thread that wrote the first.
-        const int mine = (int)blockIdx.x - few_cta((long long)r.place * UE, walk.U, walk.G);
+        const int mine = (int)blockIdx.x - few_cta((long long)r.place * plan.groups, walk.U, walk.G);
         float* dst = p.part + (long long)(plan.part0[r.place] + mine * r.tokens) * p.Op + q * 32 + lane;
         for (int i0 = g * acc.tiles; ok && i0 < nO; i0 += acc.groups * acc.tiles, ++j2) {
           const int b = j2 & (acc.nbuf - 1), nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;

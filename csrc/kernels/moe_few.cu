@@ -428,7 +428,7 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
     r.a_bytes = up256((long long)pairs * p.F * 4);
     return r;
   }
-  r.grid = serving_sm_count();
+  r.grid = std::min(serving_sm_count(), kFewJoinItems - 2 * kFewTopK);
   r.Op = (p.O + 127) / 128 * 128;
   r.Tp = (p.T + 15) / 16 * 16;
   const int UE = (p.F + 15) / 16, ups = 128 / eb / 16;
@@ -530,7 +530,8 @@ void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, voi
     if (glu) launch_tensor<true, true>(tx, t1, t1w, t2, t2u, tp, plan.grid, s);
     else launch_tensor<true, false>(tx, t1, t1w, t2, t2u, tp, plan.grid, s);
   }
-  launch_with_pdl(few_join_parts_kernel, dim3(plan.Op / 128, p.T), dim3(kFewJoinThreads), 0, s, true, tp);
+  if (p.T >= 5) launch_with_pdl(few_join_parts_kernel<4>, dim3(plan.Op / 128, (p.T + 3) / 4), dim3(kFewJoinThreads), 0, s, true, tp);
+  else launch_with_pdl(few_join_parts_kernel<1>, dim3(plan.Op / 128, p.T), dim3(kFewJoinThreads), 0, s, true, tp);
 }
 
 }  // namespace raiccl
