@@ -217,13 +217,12 @@ void launch_linear(const LinearParams& params, const LinearPlan& plan, void* wor
   }
   if (plan.dense && !p.bf16) {
     const long long wrows = glu ? 2ll * p.N : p.N;
-    auto split = [&](const void* src, long long stride, void* dst, long long rows) {
-      const int vec = p.K % 4 == 0 && ((uintptr_t)src & 15) == 0 && stride % 4 == 0;
-      launch_with_pdl(linear_split_kernel, dim3((unsigned)(8 * serving_sm_count())), dim3(256), 0, s, true, (const float*)src, stride,
-                      (float*)dst, plan.packed_stride, rows, p.K, vec);
+    auto operand = [&](const void* src, long long stride, void* dst, long long rows) {
+      return SplitOperand{(const float*)src, stride, (float*)dst, rows,
+                          p.K % 4 == 0 && ((uintptr_t)src & 15) == 0 && (rows <= 1 || stride % 4 == 0)};
     };
-    split(p.x, p.x_stride, ws, p.M);
-    split(p.w, p.w_stride, ws + plan.x_bytes, wrows);
+    launch_with_pdl(linear_split_kernel, dim3((unsigned)(8 * serving_sm_count())), dim3(256), 0, s, true,
+                    operand(p.x, p.x_stride, ws, p.M), operand(p.w, p.w_stride, ws + plan.x_bytes, wrows), plan.packed_stride, p.K);
     p.x = ws;
     p.w = ws + plan.x_bytes;
     p.x_stride = p.w_stride = plan.packed_stride;
