@@ -194,9 +194,10 @@ void launch_few_route(const FewRouteParams& params, cudaStream_t s) {
 // Experts by rows, on CUDA cores: for the smallest calls, where a pipeline's
 // start costs more than it brings, and for weights that TMA cannot read.  One
 // warp per pair of W1 rows and per row of W2; fp32 sums, activations in fp32.
-// What bounds it is memory: 24 loads of 16 bytes in flight per lane and four
-// CTAs per SM.  64 experts, 1 token (104 MB): MEASURE_FINE us, against MEASURE_TC by
-// tensor cores; the R4 layer, 1 token: MEASURE_R4 against MEASURE_R4TC.
+// What bounds the large ones is memory (24 loads of 16 bytes in flight per
+// lane): 64 experts, 1 token (104 MB) 42 us, against 34 by tensor cores; the
+// small ones are three launches and their first loads: R4 layer, 1 token 10 us
+// in a graph, against 32.
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;

@@ -252,12 +252,27 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   return res;
 }
 
+// The device's record of the first wait that ran out in a serving operator
+// since the last call (eight words, DeviceStatus); waits for the device and
+// clears the record.
+torch::Tensor serving_status(int64_t device) {
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  torch::Tensor words = torch::zeros({(int64_t)(sizeof(raiccl::DeviceStatus) / 4)}, torch::kInt32);
+  raiccl::DeviceStatus* at = raiccl::serving_status();
+  C10_CUDA_CHECK(cudaDeviceSynchronize());
+  C10_CUDA_CHECK(cudaMemcpy(words.data_ptr(), at, sizeof(raiccl::DeviceStatus), cudaMemcpyDeviceToHost));
+  C10_CUDA_CHECK(cudaMemset(at, 0, sizeof(raiccl::DeviceStatus)));
+  C10_CUDA_CHECK(cudaDeviceSynchronize());
+  return words;
+}
+
 }  // namespace
 
 void register_serving(py::module_& m) {
   m.def("moe_few_tokens", &moe_few_tokens, py::arg("x"), py::arg("router_w"), py::arg("w1"), py::arg("w2"), py::arg("top_k"),
         py::arg("act"), py::arg("gate_mode"), py::arg("router_b"), py::arg("b1"), py::arg("b2"), py::arg("block_mask"),
         py::arg("residual"), py::arg("out"), py::arg("out_dtype"));
+  m.def("serving_status", &serving_status, py::arg("device"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("residual"),
         py::arg("out"), py::arg("out_dtype"));
 }

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 
+from . import status as _status
 from ._native import kernels
 from .grouped_gemm import ACT_IDS
 
@@ -37,6 +38,7 @@ def moe_few_tokens(
     residual: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
     out_dtype: torch.dtype | None = None,
+    check: bool = False,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """out[t] = sum_j gate[t, j] * (w2[e] @ act(w1[e] @ x[t] + b1[e]) + b2[e]) + residual[t], e = ids[t, j].
 
@@ -49,17 +51,23 @@ def moe_few_tokens(
     (or zeros).  residual [T, O]: fp32 or bf16; ``out`` may be the same tensor.
 
     Sums are kept in fp32; bf16 layers keep the hidden activation in bf16, as
-    the large layer does.  Returns (out [T, O] in out_dtype or x's type,
-    expert ids int32 [T, top_k], gates fp32 [T, top_k]).  Enqueues on the
-    current stream without synchronising and can be captured in a CUDA graph.
-    There is no backward.
+    the large layer does, except in the smallest calls, which keep it in fp32.
+    Returns (out [T, O] in out_dtype or x's type, expert ids int32 [T, top_k],
+    gates fp32 [T, top_k]).  Enqueues three launches on the current stream
+    without synchronising and can be captured in a CUDA graph; outputs and
+    workspace come from torch's allocator on that stream.  Expert rows that do
+    not start on 16 bytes are read element by element.  ``check=True`` waits
+    and raises on a recorded device status.  There is no backward.
     """
     if act not in ACT_IDS:
         raise ValueError(f"moe_few_tokens: act must be one of {sorted(ACT_IDS)}")
     if gate_mode not in GATE_IDS:
         raise ValueError(f"moe_few_tokens: gate_mode must be one of {sorted(GATE_IDS)}")
-    return kernels().moe_few_tokens(x, router_w, w1, w2, top_k, ACT_IDS[act], GATE_IDS[gate_mode], router_b, b1, b2,
-                                    block_mask, residual, out, out_dtype)
+    res = kernels().moe_few_tokens(x, router_w, w1, w2, top_k, ACT_IDS[act], GATE_IDS[gate_mode], router_b, b1, b2,
+                                   block_mask, residual, out, out_dtype)
+    if check:
+        _status.check_serving(x.device)
+    return res
 
 
 __all__ = ["GATE_IDS", "MAX_EXPERTS", "MAX_TOKENS", "MAX_TOP_K", "moe_few_tokens"]

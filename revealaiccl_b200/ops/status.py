@@ -52,3 +52,14 @@ def check(status: torch.Tensor) -> None:
     rec = decode(status)
     if rec["code"] != 0:
         raise DeviceStatusError(rec)
+
+
+def check_serving(device: torch.device | str | int | None = None) -> None:
+    """Wait for ``device`` and raise if a bounded wait ran out in one of its
+    ``linear`` / ``moe_few_tokens`` calls since the last check; the record is
+    cleared.  Until then the calls behind a failed one may give up early too."""
+    from ._native import kernels
+
+    dev = torch.device("cuda" if device is None else device if not isinstance(device, int) else f"cuda:{device}")
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    check(kernels().serving_status(index))

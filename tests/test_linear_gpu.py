@@ -186,3 +186,11 @@ def test_graph_replay(m, k):
         x.copy_(x2), w.copy_(w2), r.copy_(r2)
         graph.replay()
         assert torch.equal(out, _linear(x, w, b, act="silu", residual=r))
+
+
+def test_check_reads_and_clears_the_status():
+    from revealaiccl_b200.ops import status
+    x, w, b, r = _make(3, 256, 64, "silu", BF16, True, True)
+    assert torch.equal(_linear(x, w, b, act="silu", residual=r, check=True), _linear(x, w, b, act="silu", residual=r))
+    status.check_serving()
+    status.check_serving(x.device)
