@@ -97,6 +97,7 @@ struct LinearParams {
 
 // How a product runs, and the device memory that it needs besides.
 struct LinearPlan {
+  int vector, vec;         // very few rows, on CUDA cores; 16 bytes at a time
   int dense;               // CTA pairs with tiles of 256 x dense sums; 0: few rows
   int Mp, ranks, stages, low;   // few rows: rows of x of a tile, CTAs that share K, stages, tiles of low parts
   int pack_x, pack_w;      // rows that TMA cannot read are copied to aligned ones first

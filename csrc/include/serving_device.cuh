@@ -53,6 +53,13 @@ __device__ __forceinline__ uint64_t desc_at(uint64_t fields, uint32_t smem_addr)
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
+// The elements of sixteen bytes as fp32.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& v, float (&f)[16 / sizeof(T)]) {
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = as_float(((const T*)&v)[i]);
+}
+
 // One element of a tensor of either type, by element offset.
 __device__ __forceinline__ float load_elem(const void* p, long long i, int bf16) {
   return bf16 ? __bfloat162float(((const __nv_bfloat16*)p)[i]) : ((const float*)p)[i];

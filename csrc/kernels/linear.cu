@@ -7,6 +7,7 @@
 
 #include "linear_dense.cuh"
 #include "linear_rows.cuh"
+#include "linear_vector.cuh"
 #include "serving.h"
 #include "serving_device.cuh"
 #include "serving_tma.h"
@@ -61,6 +62,7 @@ static long long up256(long long v) { return (v + 255) / 256 * 256; }
 //   rows       3 + 4 Mp / (64 ranks) for each round of CTAs, and for each 128 bytes of its K 0.14 to 0.24 (fp32: 0.55 to 0.9)
 //   dense 128  5 + 1.2 for each round of pairs and 0.21 for each 128 bytes of K; fp32 0.5, and 8 for the split operands
 //   dense 256  6 + 2.5 and 0.31: fewer rounds, each longer
+//   vector     very few rows, see below
 // So one row of 4096 x 4096 takes 7 us by rows and 19 by dense tiles; 256 rows 22 and 19; 2048 rows 122, 61 and 50.
 LinearPlan plan_linear(const LinearParams& p) {
   LinearPlan r{};
@@ -104,6 +106,23 @@ LinearPlan plan_linear(const LinearParams& p) {
         r.dense = bn;
       }
     }
+  }
+  // Very few rows: without pipelines, splits and copies.  Up to so many weights (millions), by where the two cross; us, here
+  // against there: bf16 1 row 1024 x 1024 2.4 / 4.0, 4096 x 4096 9.1 / 9.7, 16384 x 4096 26.5 / 23.5, 4 rows 1024 x 1024
+  // 3.1 / 4.1, 4096 x 1024 9.0 / 4.6; fp32 1 row 16384 x 4096 43 / 74, 4 rows 68 / 75, 8 rows 1024 x 1024 4.9 / 7.7; SwiGLU
+  // holds twice the sums: 2 rows 2 x 4096 x 4096 fp32 45 / 42.  Off 16 bytes: bf16 4 rows 1728 x 9097 18 / 20, fp32 8 rows
+  // 23 / 49.
+  const bool packs = r.pack_x || r.pack_w;
+  const double weights = 1e-6 * wrows * p.K, all = 1e30;
+  double most = 0;
+  if (packs && p.K > 0) most = p.M <= (p.bf16 ? 4 : 8) ? all : 0;
+  else if (p.bf16) most = p.M == 1 ? (glu ? 2.5 : 17) : p.M == 2 ? 2.5 : p.M <= 4 ? 1.2 : p.M <= 8 ? 0.2 : 0;
+  else most = p.M == 1 ? all : p.M == 2 ? (glu ? 9 : all) : p.M <= 4 ? (glu ? 2.5 : all) : p.M <= 8 ? 2.5 : 0;
+  if (p.M <= 8 && weights <= most) {
+    r.vector = 1;
+    r.vec = !packs && (p.K * eb) % 16 == 0;
+    r.dense = r.pack_x = r.pack_w = 0;
+    return r;
   }
   if (p.K == 0) r.x_bytes = 256;   // an address for the maps; nothing is read
   if (r.dense && !p.bf16) {        // both operands as two tf32 parts
@@ -222,6 +241,33 @@ static void launch_dense_any(const LinearParams& p, int bn, cudaStream_t s) {
   }
 }
 
+template <typename T, bool VEC, bool GLU>
+static void launch_vector(const LinearParams& p, cudaStream_t s) {
+  auto run = [&](auto kern, int nt) {
+    launch_with_pdl(kern, dim3((p.N + kVectorOut - 1) / kVectorOut, (unsigned)((p.M + nt - 1) / nt)), dim3(kVectorThreads), 0, s, true, p);
+  };
+  if (p.M == 1) run(linear_vector_kernel<T, VEC, GLU, 1>, 1);
+  else if (p.M == 2) run(linear_vector_kernel<T, VEC, GLU, 2>, 2);
+  else if (p.M <= 4) run(linear_vector_kernel<T, VEC, GLU, 4>, 4);
+  else run(linear_vector_kernel<T, VEC, GLU, 8>, 8);
+}
+
+static void launch_vector_any(const LinearParams& p, bool vec, cudaStream_t s) {
+  const bool glu = p.act == (int)Act::kSwiGLU;
+  auto run = [&](auto type, auto v) {
+    using T = decltype(type);
+    if (glu) launch_vector<T, decltype(v)::value, true>(p, s);
+    else launch_vector<T, decltype(v)::value, false>(p, s);
+  };
+  if (p.bf16) {
+    if (vec) run(__nv_bfloat16{}, std::true_type{});
+    else run(__nv_bfloat16{}, std::false_type{});
+  } else {
+    if (vec) run(float{}, std::true_type{});
+    else run(float{}, std::false_type{});
+  }
+}
+
 static void pack(const void* src, long long stride, void* dst, int packed, long long rows, int K, int bf16, cudaStream_t s) {
   const dim3 grid((unsigned)(8 * serving_sm_count()));
   if (bf16)
@@ -235,6 +281,7 @@ void launch_linear(const LinearParams& params, const LinearPlan& plan, void* wor
   LinearParams p = params;
   const bool glu = p.act == (int)Act::kSwiGLU;
   char* ws = (char*)workspace;
+  if (plan.vector) return launch_vector_any(p, plan.vec != 0, s);
   if (p.K == 0) {
     p.x = p.w = ws;
     p.x_stride = p.w_stride = 8;

@@ -227,12 +227,6 @@ __device__ __forceinline__ int few_pairs(const int* ids, int T, int k, int y, in
   return n < kRowTokens ? n : kRowTokens;
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack16(const uint4& v, float (&f)[16 / sizeof(T)]) {
-#pragma unroll
-  for (int i = 0; i < (int)(16 / sizeof(T)); ++i) f[i] = as_float(((const T*)&v)[i]);
-}
-
 // Two rows of W1 against NT of the expert's tokens, pairs list[0 .. n): h[pair, f] = act(W1[e] x + b1).
 template <typename T, bool VEC, int NT>
 __device__ __forceinline__ void few_hidden_rows(const FewExpertParams& p, float* h, const int* list, int n, int e, int f, bool glu) {
