@@ -1,5 +1,5 @@
 // Dense product for few rows, and for problems with few tiles: every weight is
-// read once for up to 256 rows of x, and the K axis is split over a cluster
+// read once for up to 64 rows of x, and the K axis is split over a cluster
 // when the tiles alone would leave SMs idle.
 //
 // The weights are the 128-row operand of tcgen05.mma (SwiGLU: 64 gate and 64 up
@@ -36,7 +36,7 @@ constexpr unsigned long long kServingWaitNs = 2000000000ull;
 
 struct LinearRowsParams {
   LinearParams l;
-  int Mp;        // rows of x of a tile: a multiple of 16, at most 256 (fp32: 128)
+  int Mp;        // rows of x of a tile: a multiple of 16, at most 64 (fp32: 16, 32 or 64)
   int stages;
   int vec_out;   // four outputs of a row may be written at once
   int low;       // fp32: stages whose low parts of the weights are kept, at most as many as stages

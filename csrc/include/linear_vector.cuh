@@ -5,6 +5,10 @@
 // A CTA has four outputs (SwiGLU: their gate and up rows) and up to eight rows
 // of x; its eight warps share K.  Each lane adds products of 16 bytes at a time
 // in 32 bits, a butterfly adds the lanes, shared memory the warps in order.
+// Four outputs for a CTA: fewer read x more often, more leave SMs empty at the
+// smallest widths.  Loads bound it: one row of 4096 x 4096 bf16 takes 9.1 us
+// (33.6 MB from L2, 3.7 TB/s), of 16384 x 4096 fp32 43 us (268 MB, 6.2 TB/s),
+// 7 rows of 2048 x 33 fp32 5.3 us, nearly all of it the launch.
 #pragma once
 
 #include "serving.h"

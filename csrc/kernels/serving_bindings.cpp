@@ -3,6 +3,8 @@
 // its tensors' device; outputs and workspaces come from torch's allocator on
 // that stream, so nothing is shared between calls or captured graphs.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -30,6 +32,12 @@ bool inner_contiguous(const torch::Tensor& t) { return t.size(-1) <= 1 || t.stri
 
 bool is_float_type(const torch::Tensor& t) {
   return t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16;
+}
+
+// A new tensor without the dispatcher's rounds, which cost the smallest calls as
+// much as a launch.
+torch::Tensor fresh(at::IntArrayRef shape, torch::ScalarType dt, const torch::Device& dev) {
+  return at::detail::empty_cuda(shape, dt, dev, c10::nullopt);
 }
 
 // [first, last) bytes that the tensor's elements lie in.
@@ -83,7 +91,7 @@ torch::Tensor check_out(const char* op, const OptTensor& out, const OptTensor& r
   }
   if (!out) {
     check_cuda(op, dev);
-    return torch::empty({rows, width}, like.options().dtype(dt));
+    return fresh({rows, width}, dt, dev);
   }
   check_input(op, "out", *out, dev);
   TORCH_CHECK_VALUE(out->dim() == 2 && out->size(0) == rows && out->size(1) == width, op, ": out must have shape ",
@@ -142,9 +150,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
                       op, ": block_mask must be bool or uint8 of shape [E] or [T, E] with contiguous rows");
   }
   torch::Tensor res = check_out(op, out, residual, x, out_dtype, T, O, {&x, &router_w, &w1, &w2});
-  c10::cuda::CUDAGuard guard(dev);
-  torch::Tensor ids = torch::empty({T, top_k}, x.options().dtype(torch::kInt32));
-  torch::Tensor gates = torch::empty({T, top_k}, x.options().dtype(torch::kFloat32));
+  const c10::cuda::CUDAGuard guard(dev);
+  torch::Tensor ids = fresh({T, top_k}, torch::kInt32, dev);
+  torch::Tensor gates = fresh({T, top_k}, torch::kFloat32, dev);
   if (T == 0) return {res, ids, gates};
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
 
@@ -197,8 +205,8 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   e.out_bf16 = res.scalar_type() == torch::kBFloat16;
   e.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
   const raiccl::FewExpertPlan plan = raiccl::plan_few_experts(e);
-  torch::Tensor ws = torch::empty({plan.bytes()}, x.options().dtype(torch::kUInt8));
-  char* base = (char*)ws.data_ptr();
+  const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)plan.bytes());   // of the current stream
+  char* base = (char*)ws.get();
   r.packed = plan.pack ? base : nullptr;
   r.packed_stride = plan.packed_stride;
   r.packed_rows = plan.Tp;
@@ -220,6 +228,7 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   TORCH_CHECK_VALUE(weight.size(1) == K, op, ": weight has ", text(weight.size(1)), " columns, x has ", text(K));
   TORCH_CHECK_VALUE(!glu || rows % 2 == 0, op, ": SwiGLU needs as many up rows as gate rows in weight");
   TORCH_CHECK_VALUE(M < (1ll << 30) && rows < (1 << 24) && K < (1 << 24), op, ": at most 2^30 rows and 2^24 columns");
+  TORCH_CHECK_VALUE(K > 0 || M <= (1 << 22), op, ": at most 2^22 rows without columns");
   TORCH_CHECK_VALUE(is_float_type(x) && weight.scalar_type() == x.scalar_type(), op, ": x and weight must both be bf16 or both be fp32");
   TORCH_CHECK_VALUE(inner_contiguous(x) && inner_contiguous(weight), op, ": x and weight must have contiguous rows");
   const int64_t N = glu ? rows / 2 : rows;
@@ -245,9 +254,9 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   p.out_bf16 = res.scalar_type() == torch::kBFloat16;
   p.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
   const raiccl::LinearPlan plan = raiccl::plan_linear(p);
-  torch::Tensor ws;
-  if (plan.bytes() > 0) ws = torch::empty({plan.bytes()}, x.options().dtype(torch::kUInt8));
-  raiccl::launch_linear(p, plan, plan.bytes() > 0 ? ws.data_ptr() : nullptr, at::cuda::getCurrentCUDAStream());
+  c10::DataPtr ws;   // of the current stream
+  if (plan.bytes() > 0) ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)plan.bytes());
+  raiccl::launch_linear(p, plan, ws.get(), at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return res;
 }

@@ -52,6 +52,23 @@ def test_sizes(m, k, n, dtype):
         check_norm(got, want, 2 * _norm_bound(k, dtype, dtype))
 
 
+FEW = [  # on both sides of where very few rows go to CUDA cores: many weights, and odd widths
+    (1, 4096, 4104), (1, 2048, 9000), (2, 4096, 2048), (3, 1000, 3001), (4, 1024, 2048), (5, 2048, 520), (6, 264, 4096),
+    (7, 1408, 1000), (8, 2048, 2048), (8, 4097, 129), (9, 1024, 512),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("act", ["none", "swiglu"])
+@pytest.mark.parametrize("m,k,n", FEW)
+def test_few_rows(m, k, n, act, dtype):
+    x, w, b, r = _make(m, k, n, act, dtype, True, n % 2 == 0, seed=n)
+    got = _linear(x, w, b, act=act, residual=r)
+    want, bound = linear64(x, w, b, act, r)
+    check_close(got, want, bound)
+    check_norm(got, want, 2 * _norm_bound(k, dtype, dtype))
+
+
 @pytest.mark.parametrize("m", [1, 4, 40, 130, 600])
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu", "swiglu"])
 @pytest.mark.parametrize("dtype,out_dtype,res_dtype", [(BF16, BF16, FP32), (BF16, FP32, BF16), (BF16, FP32, FP32),
@@ -129,6 +146,9 @@ def test_empty():
     b, r = torch.randn(8, device=DEV), torch.randn(3, 8, device=DEV)
     got = _linear(torch.empty(3, 0, device=DEV), torch.empty(8, 0, device=DEV), b, act="relu", residual=r)
     assert torch.equal(got, b.clamp_min(0) + r)
+    r = torch.randn(20, 8, device=DEV)
+    got = _linear(torch.empty(20, 0, device=DEV, dtype=BF16), torch.empty(8, 0, device=DEV, dtype=BF16), b, residual=r, out_dtype=FP32)
+    assert torch.equal(got, b + r)
 
 
 @pytest.mark.parametrize("m", [4, 200])
