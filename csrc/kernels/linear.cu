@@ -94,6 +94,7 @@ LinearPlan plan_linear(const LinearParams& p) {
       r.ranks = ranks;
     }
   }
+  if (mt > 65535) best = 1e30;   // more tiles than a grid has rows
   // dense tiles
   if (p.K > 0 && p.M < (1ll << 30)) {
     for (int bn = 128; bn <= (p.bf16 ? 256 : 128); bn *= 2) {

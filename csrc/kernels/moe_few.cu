@@ -102,6 +102,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* x = (const T*)p.x + (long long)t * p.x_stride;
   float* lead = cluster.map_shared_rank(&piece[0][0], 0);
+  cluster.barrier_arrive();   // of the CTAs that write to the first one's shared memory: it has begun
   griddep_wait();
   griddep_launch_dependents();
   if (p.packed) {
@@ -117,6 +118,7 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams
   }
   const int n = p.vec ? p.D * (int)sizeof(T) / 16 : p.D;   // vectors (elements) of a row
   const int per = (n + p.cuts - 1) / p.cuts;
+  cluster.barrier_wait();
   for (int i = warp * ranks + rank; i < p.E * p.cuts; i += kRouteWarps * ranks) {
     const int e = i / p.cuts, c = i - e * p.cuts;
     const int i0 = c * per, i1 = i0 + per < n ? i0 + per : n;

@@ -228,7 +228,7 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   TORCH_CHECK_VALUE(weight.size(1) == K, op, ": weight has ", text(weight.size(1)), " columns, x has ", text(K));
   TORCH_CHECK_VALUE(!glu || rows % 2 == 0, op, ": SwiGLU needs as many up rows as gate rows in weight");
   TORCH_CHECK_VALUE(M < (1ll << 30) && rows < (1 << 24) && K < (1 << 24), op, ": at most 2^30 rows and 2^24 columns");
-  TORCH_CHECK_VALUE(K > 0 || M <= (1 << 22), op, ": at most 2^22 rows without columns");
+  TORCH_CHECK_VALUE(K > 0 || M <= (1 << 21), op, ": at most 2^21 rows without columns");
   TORCH_CHECK_VALUE(is_float_type(x) && weight.scalar_type() == x.scalar_type(), op, ": x and weight must both be bf16 or both be fp32");
   TORCH_CHECK_VALUE(inner_contiguous(x) && inner_contiguous(weight), op, ": x and weight must have contiguous rows");
   const int64_t N = glu ? rows / 2 : rows;

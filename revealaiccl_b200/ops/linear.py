@@ -41,7 +41,7 @@ def linear(
     synchronising and can be captured in a CUDA graph.  Rows of x or weight
     that do not start on 16 bytes are copied first (not for up to 4 rows of x,
     8 in fp32), which costs up to twice the product's own reads.  At most 2^30
-    rows and 2^24 columns and weight rows; 2^22 rows when there are no columns.  ``check=True`` waits and raises on a recorded device
+    rows and 2^24 columns and weight rows; 2^21 rows when there are no columns.  ``check=True`` waits and raises on a recorded device
     status.  There is no backward.
     """
     if act not in ACT_IDS:

@@ -47,7 +47,7 @@ X = torch.zeros(3, 16, dtype=BF16)
     (dict(out=torch.zeros(8, dtype=BF16).expand(3, 8)), "do not overlap"),
     (dict(out_dtype=torch.float16), "the output is fp32"),
     (dict(x=X.float(), weight=torch.zeros(8, 16), out_dtype=BF16), "the output is fp32"),
-    (dict(x=torch.zeros(2 ** 22 + 1, 0, dtype=BF16), weight=torch.zeros(8, 0, dtype=BF16)), r"at most 2\^22 rows"),
+    (dict(x=torch.zeros(2 ** 21 + 1, 0, dtype=BF16), weight=torch.zeros(8, 0, dtype=BF16)), r"at most 2\^21 rows"),
 ])
 def test_linear_refuses(kw, words):
     with pytest.raises(ValueError, match=words):
