@@ -63,6 +63,7 @@ struct FewExpertParams {
 struct FewExpertPlan {
   int tensor;             // on the tensor cores (else by rows, on CUDA cores)
   int vec;                // by rows: 16 bytes at a time
+  int route;              // by rows: the experts' kernel routes too
   int grid, stages, hbytes, Op, Tp;
   int pack;               // x is packed by the routing kernel
   int packed_stride;
@@ -71,8 +72,7 @@ struct FewExpertPlan {
 };
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p);
-void launch_few_route(const FewRouteParams& p, cudaStream_t s);
-void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s);
+void launch_few(const FewRouteParams& r, const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s);
 
 // The current device's record of a wait that ran out in a serving operator (device memory).
 DeviceStatus* serving_status();

@@ -86,22 +86,83 @@ __device__ __forceinline__ float route_dot(const T* x, const T* w, int i0, int i
   return warp_sum(acc);
 }
 
-// One cluster per token.  The experts' rows, cut into `cuts` pieces each, are
-// dealt to the warps of its CTAs; the first CTA adds the pieces in order and
-// finds each expert's rank among all (the number of experts with a larger key),
-// so the choices need no rounds.
+// What a CTA holds of a token's routing.
+struct FewRoute {
+  float piece[kRouteCuts][kFewExperts + 1];
+  float logits[kFewExperts + 1];
+  unsigned long long keys[kFewExperts + 1];
+  int chosen[kFewTopK];
+};
+
+// The experts' rows, cut into `cuts` pieces each, are dealt to warps: warp `at` of `of`.
+template <typename T>
+__device__ __forceinline__ void route_pieces(const FewRouteParams& p, const T* x, float* piece, int at, int of) {
+  const int n = p.vec ? p.D * (int)sizeof(T) / 16 : p.D;   // vectors (elements) of a row
+  const int per = (n + p.cuts - 1) / p.cuts;
+  for (int i = at; i < p.E * p.cuts; i += of) {
+    const int e = i / p.cuts, c = i - e * p.cuts;
+    const int i0 = c * per, i1 = i0 + per < n ? i0 + per : n;
+    const float v = route_dot(x, (const T*)p.w + (long long)e * p.w_stride, i0, i1, p.vec);
+    if ((threadIdx.x & 31) == 0) piece[c * (kFewExperts + 1) + e] = v;
+  }
+}
+
+// Adds the pieces in order and finds each expert's rank among all (the number
+// of experts with a larger key), so the choices need no rounds.
+__device__ __forceinline__ void route_choose(const FewRouteParams& p, FewRoute& s, int t) {
+  const int e = threadIdx.x;   // kRouteThreads > kFewExperts
+  unsigned long long key = 0ull;
+  if (e < p.E) {
+    float v = s.piece[0][e];
+    for (int c = 1; c < p.cuts; ++c) v += s.piece[c][e];
+    if (p.bias) v += p.bias[e];
+    if (p.mask && p.mask[(long long)t * p.mask_stride + e]) v = -INFINITY;
+    s.logits[e] = v;
+    s.keys[e] = key = few_key(v, e);
+  }
+  if (e < kFewTopK) s.chosen[e] = -1;
+  __syncthreads();
+  if (key != 0ull) {
+    int above = 0;
+#pragma unroll 8
+    for (int o = 0; o < p.E; ++o) above += s.keys[o] > key ? 1 : 0;
+    if (above < p.k) s.chosen[above] = e;
+  }
+  __syncthreads();
+}
+
+// By one warp: the choices and gates of the token.
+__device__ __forceinline__ void route_write(const FewRouteParams& p, const FewRoute& s, int t) {
+  const int lane = threadIdx.x & 31;
+  const int mine = lane < p.k ? s.chosen[lane] : -1;   // lane j: choice j
+  const float top = mine < 0 ? 0.f : s.logits[mine];
+  float gate = mine < 0 ? 0.f : 1.f;
+  if (p.gate_mode != 0) {
+    const float peak = __shfl_sync(0xffffffffu, top, 0);  // the largest number, or NaN if there is none
+    float part = 0.f;
+    if (p.gate_mode == 1) {
+      part = mine < 0 ? 0.f : expf(top - peak);
+    } else {
+      for (int o = lane; o < p.E; o += 32) part += s.logits[o] == -INFINITY ? 0.f : expf(s.logits[o] - peak);
+    }
+    const float total = warp_sum(part);
+    if (mine >= 0) gate = expf(top - peak) / total;
+  }
+  if (lane < p.k) {
+    p.ids[(long long)t * p.k + lane] = mine;
+    p.gates[(long long)t * p.k + lane] = gate;
+  }
+}
+
+// One cluster per token: its CTAs share the pieces, the first one chooses.
 template <typename T>
 __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams p) {
-  __shared__ float piece[kRouteCuts][kFewExperts + 1];
-  __shared__ float logits[kFewExperts + 1];
-  __shared__ unsigned long long keys[kFewExperts + 1];
-  __shared__ int chosen[kFewTopK];
+  __shared__ FewRoute s;
   cg::cluster_group cluster = cg::this_cluster();
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int t = blockIdx.y;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* x = (const T*)p.x + (long long)t * p.x_stride;
-  float* lead = cluster.map_shared_rank(&piece[0][0], 0);
+  float* lead = cluster.map_shared_rank(&s.piece[0][0], 0);
   cluster.barrier_arrive();   // of the CTAs that write to the first one's shared memory: it has begun
   griddep_wait();
   griddep_launch_dependents();
@@ -116,63 +177,23 @@ __global__ void __launch_bounds__(kRouteThreads) few_route_kernel(FewRouteParams
       }
     }
   }
-  const int n = p.vec ? p.D * (int)sizeof(T) / 16 : p.D;   // vectors (elements) of a row
-  const int per = (n + p.cuts - 1) / p.cuts;
   cluster.barrier_wait();
-  for (int i = warp * ranks + rank; i < p.E * p.cuts; i += kRouteWarps * ranks) {
-    const int e = i / p.cuts, c = i - e * p.cuts;
-    const int i0 = c * per, i1 = i0 + per < n ? i0 + per : n;
-    const float v = route_dot(x, (const T*)p.w + (long long)e * p.w_stride, i0, i1, p.vec);
-    if (lane == 0) lead[c * (kFewExperts + 1) + e] = v;
-  }
+  route_pieces(p, x, lead, (threadIdx.x >> 5) * ranks + rank, kRouteWarps * ranks);
   cluster.sync();
   if (rank != 0) return;
-  const int e = threadIdx.x;   // kRouteThreads > kFewExperts
-  unsigned long long key = 0ull;
-  if (e < p.E) {
-    float v = piece[0][e];
-    for (int c = 1; c < p.cuts; ++c) v += piece[c][e];
-    if (p.bias) v += p.bias[e];
-    if (p.mask && p.mask[(long long)t * p.mask_stride + e]) v = -INFINITY;
-    logits[e] = v;
-    keys[e] = key = few_key(v, e);
-  }
-  if (e < kFewTopK) chosen[e] = -1;
-  __syncthreads();
-  if (key != 0ull) {
-    int above = 0;
-#pragma unroll 8
-    for (int o = 0; o < p.E; ++o) above += keys[o] > key ? 1 : 0;
-    if (above < p.k) chosen[above] = e;
-  }
-  __syncthreads();
-  if (warp != 0) return;
-  const int mine = lane < p.k ? chosen[lane] : -1;   // lane j: choice j
-  const float top = mine < 0 ? 0.f : logits[mine];
-  float gate = mine < 0 ? 0.f : 1.f;
-  if (p.gate_mode != 0) {
-    const float peak = __shfl_sync(0xffffffffu, top, 0);  // the largest number, or NaN if there is none
-    float part = 0.f;
-    if (p.gate_mode == 1) {
-      part = mine < 0 ? 0.f : expf(top - peak);
-    } else {
-      for (int o = lane; o < p.E; o += 32) part += logits[o] == -INFINITY ? 0.f : expf(logits[o] - peak);
-    }
-    const float total = warp_sum(part);
-    if (mine >= 0) gate = expf(top - peak) / total;
-  }
-  if (lane < p.k) {
-    p.ids[(long long)t * p.k + lane] = mine;
-    p.gates[(long long)t * p.k + lane] = gate;
-  }
+  route_choose(p, s, t);
+  if (threadIdx.x < 32) route_write(p, s, t);
 }
 
-void launch_few_route(const FewRouteParams& params, cudaStream_t s) {
-  // Pieces of a row so that the cluster's warps have one each, down to one
-  // vector per lane; clusters of eight CTAs at most.
-  FewRouteParams p = params;
+// Pieces of a row so that `warps` warps have one each, down to one vector per lane.
+static int route_cuts(const FewRouteParams& p, int warps) {
   const int n = p.vec ? p.D * (p.bf16 ? 2 : 4) / 16 : p.D;
-  p.cuts = std::max(1, std::min({kRouteCuts, 8 * kRouteWarps / p.E, n / 32}));
+  return std::max(1, std::min({kRouteCuts, warps / p.E, n / 32}));
+}
+
+static void launch_route(const FewRouteParams& params, cudaStream_t s) {
+  FewRouteParams p = params;
+  p.cuts = route_cuts(p, 8 * kRouteWarps);   // clusters of eight CTAs at most
   const int want = (p.E * p.cuts + kRouteWarps - 1) / kRouteWarps;
   const int ranks = want > 4 ? 8 : want > 2 ? 4 : want;
   cudaLaunchConfig_t cfg = {};
@@ -198,8 +219,8 @@ void launch_few_route(const FewRouteParams& params, cudaStream_t s) {
 // warp per pair of W1 rows and per row of W2; fp32 sums, activations in fp32.
 // What bounds the large ones is memory (24 loads of 16 bytes in flight per
 // lane): 64 experts, 1 token (104 MB) 42 us, against 34 by tensor cores; the
-// small ones are three launches and their first loads: R4 layer, 1 token 10 us
-// in a graph, against 32.
+// small ones are two or three launches and their first loads: 4 experts, 2048 to
+// 32 to 16 fp32, 1 token 8.3 us in a graph, against 32.
 // ---------------------------------------------------------------------------
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
@@ -287,17 +308,29 @@ __device__ __forceinline__ void few_hidden_rows(const FewExpertParams& p, float*
   }
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams p, float* h) {
+// ROUTE: every CTA routes the call's one token for itself, and the first one writes its choices and gates.
+template <typename T, bool VEC, bool ROUTE>
+__global__ void __launch_bounds__(kRowThreads) few_hidden_kernel(FewExpertParams p, float* h, FewRouteParams r) {
   __shared__ int list[kRowTokens];
   const bool glu = p.act == (int)Act::kSwiGLU;
   griddep_wait();
   griddep_launch_dependents();
-  int e;
-  const int n = few_pairs(p.ids, p.T, p.k, blockIdx.y, list, e);
+  int e, n;
+  if constexpr (ROUTE) {
+    __shared__ FewRoute s;
+    route_pieces(r, (const T*)r.x, &s.piece[0][0], threadIdx.x >> 5, kRowWarps);
+    __syncthreads();
+    if (threadIdx.x == 0) list[0] = blockIdx.y;
+    route_choose(r, s, 0);
+    if ((blockIdx.x | blockIdx.y) == 0 && threadIdx.x < 32) route_write(r, s, 0);
+    e = s.chosen[blockIdx.y];
+    n = e < 0 ? 0 : 1;
+  } else {
+    n = few_pairs(p.ids, p.T, p.k, blockIdx.y, list, e);
+  }
   const int f = (blockIdx.x * kRowWarps + (threadIdx.x >> 5)) * (glu ? 1 : 2);   // rows f and F + f, or f and f + 1
   if (n == 0 || f >= p.F) return;
-  if (n == 1) few_hidden_rows<T, VEC, 1>(p, h, list, 1, e, f, glu);
+  if (ROUTE || n == 1) few_hidden_rows<T, VEC, 1>(p, h, list, 1, e, f, glu);
   else few_hidden_rows<T, VEC, kRowTokens>(p, h, list, n, e, f, glu);
 }
 
@@ -371,18 +404,21 @@ __global__ void __launch_bounds__(kRowThreads) few_output_kernel(FewExpertParams
 }
 
 template <typename T, bool VEC>
-static void launch_rows_vec(const FewExpertParams& p, float* h, cudaStream_t s) {
+static void launch_rows_vec(const FewExpertParams& p, const FewRouteParams& route, bool own, float* h, cudaStream_t s) {
   const int per = kRowWarps * (p.act == (int)Act::kSwiGLU ? 1 : 2);
   const dim3 grid((p.F + per - 1) / per, p.T * p.k);
-  launch_with_pdl(few_hidden_kernel<T, VEC>, grid, dim3(kRowThreads), 0, s, true, p, h);
+  FewRouteParams r = route;
+  r.cuts = route_cuts(r, kRowWarps);
+  if (own) launch_with_pdl(few_hidden_kernel<T, VEC, true>, grid, dim3(kRowThreads), 0, s, true, p, h, r);
+  else launch_with_pdl(few_hidden_kernel<T, VEC, false>, grid, dim3(kRowThreads), 0, s, true, p, h, r);
   launch_with_pdl(few_output_kernel<T, VEC>, dim3((p.O + kOutRows - 1) / kOutRows, p.T), dim3(kRowThreads), 0, s, true, p,
                   (const float*)h);
 }
 
 template <typename T>
-static void launch_rows(const FewExpertParams& p, float* h, bool vec, cudaStream_t s) {
-  if (vec) launch_rows_vec<T, true>(p, h, s);
-  else launch_rows_vec<T, false>(p, h, s);
+static void launch_rows(const FewExpertParams& p, const FewRouteParams& r, const FewExpertPlan& plan, float* h, cudaStream_t s) {
+  if (plan.vec) launch_rows_vec<T, true>(p, r, plan.route != 0, h, s);
+  else launch_rows_vec<T, false>(p, r, plan.route != 0, h, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -407,6 +443,10 @@ constexpr int kFewShared = 232448 - 10 * 1024 - 1024;  // dynamic shared memory 
 // bf16 64 experts 512 x 352, 1 token (6.5 MB) 11 / 17, 4 tokens (26 MB) 21 / 21, 32 experts 1024 x 1024, 2 tokens (50 MB)
 // 29 / 26; fp32 8 experts 1024 x 4096, 1 token (67 MB) 24 / 49, 4 (268 MB) 52 / 76, 8 (537 MB) 82 / 86, 16 130 / 89.
 constexpr double kFewRowBytes = 30e6, kFewRowBytesFp32 = 400e6;
+// One token: with few experts every CTA routes for itself and a launch is saved (us, apart against together): 4 experts, rows
+// of 2048 fp32 9.4 / 8.3 in a graph, 11.7 / 9.3 outside one; 16 experts, 2048 bf16 9.3 / 9.4 and 11.8 / 9.8; 64 experts, 512
+// bf16 10.1 / 13.1, since a warp takes its experts one after the other; 32 experts, 2048 bf16 9.6 / 11.3.
+constexpr int kFewOwnExperts = 16, kFewOwnBytes = 65536;
 constexpr int kFewJoinRoom = 24 * 1024;                // of the join's CTA beside it
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p) {
@@ -423,6 +463,7 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   if (!r.tensor) {
     r.vec = rows16 && (p.D * eb) % 16 == 0 && (p.F * eb) % 16 == 0 && aligned(p.x, p.T > 1 ? p.x_stride : 0, 0);
     r.a_bytes = up256((long long)pairs * p.F * 4);
+    r.route = p.T == 1 && p.E <= kFewOwnExperts && (long long)p.E * p.D * eb <= kFewOwnBytes;
     return r;
   }
   r.grid = std::min(serving_sm_count(), kFewJoinItems - 2 * kFewTopK);
@@ -464,12 +505,13 @@ static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CU
   launch_with_pdl(kern, dim3(grid), dim3(FewTc<FP32>::THREADS), smem, s, true, tx, t1, t1w, t2, t2u, tp, serving_status());
 }
 
-void launch_few_experts(const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
+void launch_few(const FewRouteParams& r, const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
   char* ws = (char*)workspace;
   float* a = (float*)(ws + plan.packed_bytes);
+  if (!plan.route) launch_route(r, s);
   if (!plan.tensor) {
-    if (p.bf16) launch_rows<__nv_bfloat16>(p, a, plan.vec != 0, s);
-    else launch_rows<float>(p, a, plan.vec != 0, s);
+    if (p.bf16) launch_rows<__nv_bfloat16>(p, r, plan, a, s);
+    else launch_rows<float>(p, r, plan, a, s);
     return;
   }
   const cuuint64_t eb = p.bf16 ? 2 : 4;

@@ -210,8 +210,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   r.packed = plan.pack ? base : nullptr;
   r.packed_stride = plan.packed_stride;
   r.packed_rows = plan.Tp;
-  raiccl::launch_few_route(r, stream);
-  raiccl::launch_few_experts(e, plan, base, stream);
+  raiccl::launch_few(r, e, plan, base, stream);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {res, ids, gates};
 }

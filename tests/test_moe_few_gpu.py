@@ -137,6 +137,29 @@ def test_masks(dtype, tensor):
     assert (out == 0).all() and (ids == -1).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("D,E,k", [(2048, 4, 1), (77, 1, 1), (256, 8, 8), (2048, 16, 3), (1000, 16, 2), (256, 17, 2), (4096, 8, 2)])
+def test_one_token(D, E, k, dtype):
+    """One token, on both sides of where its few experts are routed by the experts' kernel: masks, no expert left, NaN, ties."""
+    a = _make(1, D, E, 72, 40, "swiglu", dtype, seed=E, bias=True)
+    r = torch.randn(1, 40, device=DEV).to(dtype)
+    for mode in ("topk_softmax", "softmax", "none"):
+        _, ids, _ = _check(a, k, "swiglu", mode, residual=r)
+        mask = torch.zeros(E, device=DEV, dtype=torch.bool)
+        mask[ids[0, 0]] = True
+        _, ids, gates = _check(a, k, "swiglu", mode, residual=r, block_mask=mask)
+        assert not (ids == int(mask.nonzero())).any() and (k < E or ids[0, -1] == -1 and gates[0, -1] == 0)
+        out, ids, gates = _moe(**a, top_k=k, act="swiglu", gate_mode=mode, residual=r, block_mask=~torch.zeros_like(mask))
+        assert (ids == -1).all() and (gates == 0).all() and torch.equal(out, r)
+    b = dict(a, router_w=a["router_w"][:1].expand(E, D), router_b=a["router_b"][:1].expand(E).contiguous())
+    _, ids, _ = _moe(**b, top_k=k, act="swiglu", gate_mode="softmax")
+    assert ids[0].tolist() == list(range(k))
+    b = dict(a, x=a["x"].clone())
+    b["x"][0, D // 2] = float("nan")
+    out, ids, _ = _moe(**b, top_k=k, act="swiglu", gate_mode="topk_softmax")
+    assert out.isnan().all() and ids[0].tolist() == list(range(k))
+
+
 @pytest.mark.parametrize("mode", ["topk_softmax", "softmax", "none"])
 def test_bias_as_mask(mode):
     """A bias of -inf blocks; the type's lowest value is a number like any other and comes last."""
