@@ -53,7 +53,7 @@ def moe_few_tokens(
     Sums are kept in fp32; bf16 layers keep the hidden activation in bf16, as
     the large layer does, except in the smallest calls, which keep it in fp32.
     Returns (out [T, O] in out_dtype or x's type, expert ids int32 [T, top_k],
-    gates fp32 [T, top_k]).  Enqueues three launches on the current stream
+    gates fp32 [T, top_k]).  Enqueues two or three launches on the current stream
     without synchronising and can be captured in a CUDA graph; outputs and
     workspace come from torch's allocator on that stream.  Expert rows that do
     not start on 16 bytes are read element by element.  ``check=True`` waits
