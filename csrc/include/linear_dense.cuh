@@ -36,7 +36,7 @@ constexpr unsigned long long kDenseWaitNs = 2000000000ull;
 struct LinearDenseParams {
   LinearParams l;
   int mt, nt;      // tiles
-  int vec_out, vec_res, vec_bias;   // rows may be read and written 16 bytes at a time
+  int vec_out, vec_res;   // rows may be read and written 16 bytes at a time
 };
 
 template <int BN, bool FP32>
@@ -69,16 +69,31 @@ __device__ __forceinline__ void dense_tile(const LinearDenseParams& p, int t, in
   nb = local / rows;
 }
 
-// Sixteen consecutive outputs of one row: residual, rounding, store.
-__device__ __forceinline__ void dense_store16(const LinearDenseParams& p, long long m, int n, float (&v)[16]) {
+// residual[m, n .. n + 16) as it lies, where it may be read 16 bytes at a time
+__device__ __forceinline__ void dense_residual16(const LinearDenseParams& p, long long m, int n, uint4 (&r)[4]) {
+  const LinearParams& l = p.l;
+  if (l.residual == nullptr || !p.vec_res || m >= l.M || n + 16 > l.N) return;
+  const long long at = m * l.res_stride + n;
+  if (l.res_bf16) {
+    const uint4* s = (const uint4*)((const __nv_bfloat16*)l.residual + at);
+    r[0] = s[0]; r[1] = s[1];
+  } else {
+    const uint4* s = (const uint4*)((const float*)l.residual + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = s[i];
+  }
+}
+
+// Sixteen consecutive outputs of one row: residual (`ahead` is what
+// dense_residual16 read), rounding, store.
+__device__ __forceinline__ void dense_store16(const LinearDenseParams& p, long long m, int n, const uint4 (&ahead)[4], float (&v)[16]) {
   const LinearParams& l = p.l;
   const bool whole = n + 16 <= l.N;
   if (l.residual) {
     const long long at = m * l.res_stride + n;
     if (whole && p.vec_res) {
       if (l.res_bf16) {
-        const uint4* r = (const uint4*)((const __nv_bfloat16*)l.residual + at);
-        const uint4 a = r[0], b = r[1];
+        const uint4 a = ahead[0], b = ahead[1];
         const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -86,11 +101,11 @@ __device__ __forceinline__ void dense_store16(const LinearDenseParams& p, long l
           v[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
         }
       } else {
-        const float4* r = (const float4*)((const float*)l.residual + at);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 a = r[i];
-          v[4 * i] += a.x; v[4 * i + 1] += a.y; v[4 * i + 2] += a.z; v[4 * i + 3] += a.w;
+          const uint4 a = ahead[i];
+          v[4 * i] += __uint_as_float(a.x); v[4 * i + 1] += __uint_as_float(a.y);
+          v[4 * i + 2] += __uint_as_float(a.z); v[4 * i + 3] += __uint_as_float(a.w);
         }
       }
     } else {
@@ -123,21 +138,22 @@ __device__ __forceinline__ void dense_store16(const LinearDenseParams& p, long l
   }
 }
 
-// bias[n .. n + 16), zeros behind the last
-__device__ __forceinline__ void dense_bias16(const float* bias, int n, int N, int vec, float (&b)[16]) {
-  if (bias == nullptr) {
+// bias[n .. n + 32 NB), a lane has every 32nd of them; zeros behind the last.
+template <int NB>
+__device__ __forceinline__ void dense_bias(const float* bias, int n, int N, float (&b)[NB]) {
+  const int at = n + (int)(threadIdx.x & 31);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = 0.f;
-  } else if (n + 16 <= N && vec) {
+  for (int i = 0; i < NB; ++i) b[i] = bias != nullptr && at + 32 * i < N ? __ldg(bias + at + 32 * i) : 0.f;
+}
+
+// b[c .. c + 16) of them in every lane, added to v; c a multiple of 16.
+template <int NB>
+__device__ __forceinline__ void dense_add_bias16(const float (&b)[NB], int c, float (&v)[16]) {
+  float mine = b[0];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float4 a = __ldg((const float4*)(bias + n) + i);
-      b[4 * i] = a.x; b[4 * i + 1] = a.y; b[4 * i + 2] = a.z; b[4 * i + 3] = a.w;
-    }
-  } else {
+  for (int i = 1; i < NB; ++i) mine = (c >> 5) == i ? b[i] : mine;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) b[i] = n + i < N ? __ldg(bias + n + i) : 0.f;
-  }
+  for (int i = 0; i < 16; ++i) v[i] += __shfl_sync(0xffffffffu, mine, (c & 16) + i);
 }
 
 template <int BN, bool FP32, bool GLU>
@@ -261,16 +277,37 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
     int iter = 0;
     [[maybe_unused]] int nth = 0;
     bool ok = true;
-    auto finish = [&](long long m, int n, const float (&z)[16], const float (&zu)[16]) {
-      float bias[16], up[16], v[16];
-      dense_bias16(l.bias, n, l.N, p.vec_bias, bias);
-      if constexpr (GLU) dense_bias16(l.bias ? l.bias + l.N : nullptr, n, l.N, p.vec_bias, up);
+    // Biases and the first pieces (16 columns) of the residual are read before the sums are waited for, the others as many
+    // pieces ahead.
+    constexpr int AHEAD = FP32 ? 2 : 4;
+    constexpr int NB = (OUT + 31) / 32;
+    float bias[NB], up[NB];
+    uint4 ahead[AHEAD][4];
+    auto begin = [&](long long m, int n) {
+      dense_bias(l.bias, n, l.N, bias);
+      if constexpr (GLU) dense_bias(l.bias ? l.bias + l.N : nullptr, n, l.N, up);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if constexpr (GLU) v[i] = serving_swiglu(z[i] + bias[i], zu[i] + up[i]);
-        else v[i] = serving_act(z[i] + bias[i], l.act);
+      for (int j = 0; j < AHEAD; ++j)
+        if (16 * j < OUT) dense_residual16(p, m, n + 16 * j, ahead[j]);
+    };
+    // columns c .. c + 16 of the thread's OUT, which begin at n0
+    auto finish = [&](long long m, int n0, int c, float (&v)[16], float (&vu)[16]) {
+      if (l.bias) {
+        dense_add_bias16(bias, c, v);
+        if constexpr (GLU) dense_add_bias16(up, c, vu);
       }
-      if (m < l.M && n < l.N) dense_store16(p, m, n, v);
+      if constexpr (GLU) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = serving_swiglu(v[i], vu[i]);
+      } else {
+        serving_act_each(v, l.act);
+      }
+      if (m < l.M && n0 + c < l.N) dense_store16(p, m, n0 + c, ahead[0], v);
+#pragma unroll
+      for (int j = 1; j < AHEAD; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ahead[j - 1][i] = ahead[j][i];
+      if (c + 16 * AHEAD < OUT) dense_residual16(p, m, n0 + c + 16 * AHEAD, ahead[AHEAD - 1]);
       __syncwarp();
     };
     for (int t = pair; ok && t < tiles; t += npairs) {
@@ -312,6 +349,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
           add(lanes + b * BN + c0);
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[b]), 0));
         }
+        if (ok) begin(m, n0);
         if (!ok || !(ok = mbar_wait_warp(&low_full[nth & 1], (nth >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
         tc_fence_after_sync();
         add(lanes + (2 + (nth & 1)) * BN + c0);
@@ -322,15 +360,16 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
           float z[16], zu[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) { z[i] = sum[c + i]; zu[i] = sum_up[GLU ? c + i : i]; }
-          finish(m, n0 + c, z, zu);
+          finish(m, n0, c, z, zu);
         }
       } else {
         const int b = iter & 1;
+        begin(m, n0);
         if (!(ok = mbar_wait_warp(&acc_full[b], (iter >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
         ++iter;
         tc_fence_after_sync();
         const uint32_t base = lanes + b * BN + c0;
-#pragma unroll 1
+#pragma unroll 1   // code that a launch's only tile runs once is fetched while it waits: unrolled four times, 2.4 us more
         for (int c = 0; c < OUT; c += 16) {
           if (n0 + c >= l.N) break;
           uint32_t r[16], u[16];
@@ -340,7 +379,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
           float z[16], zu[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) { z[i] = __uint_as_float(r[i]); zu[i] = GLU ? __uint_as_float(u[i]) : 0.f; }
-          finish(m, n0 + c, z, zu);
+          finish(m, n0, c, z, zu);
         }
         tc_fence_before_sync();
         __syncwarp();

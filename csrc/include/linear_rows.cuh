@@ -248,6 +248,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         v[0] += a; v[1] += b; v[2] += c; v[3] += d;
       }
     };
+#pragma unroll 1
     for (int i = ((int)rank * C::THREADS + threadIdx.x) * 4; i < rows * W; i += (int)ranks * C::THREADS * 4) {
       const int m = i / W, c = i % W, n = n0 + c;
       if (n >= l.N) continue;
@@ -255,17 +256,25 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       total(m * 128 + c, v);
       if constexpr (GLU) total(m * 128 + 64 + c, up);
       const bool whole = n + 4 <= l.N;
+      if (l.bias) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool in = whole || n + j < l.N;
-        if (l.bias && in) v[j] += __ldg(l.bias + n + j);
-        if constexpr (GLU) {
-          if (l.bias && in) up[j] += __ldg(l.bias + l.N + n + j);
-          v[j] = serving_swiglu(v[j], up[j]);
-        } else {
-          v[j] = serving_act(v[j], l.act);
-        }
-        if (l.residual && in) v[j] += load_elem(l.residual, (m0 + m) * l.res_stride + n + j, l.res_bf16);
+        for (int j = 0; j < 4; ++j)
+          if (whole || n + j < l.N) {
+            v[j] += __ldg(l.bias + n + j);
+            if constexpr (GLU) up[j] += __ldg(l.bias + l.N + n + j);
+          }
+      }
+      if constexpr (GLU) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = serving_swiglu(v[j], up[j]);
+      } else {
+        serving_act_each(v, l.act);
+      }
+      if (l.residual) {
+        const long long at = (m0 + m) * l.res_stride + n;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (whole || n + j < l.N) v[j] += load_elem(l.residual, at + j, l.res_bf16);
       }
       const long long at = (m0 + m) * l.out_stride + n;
       if (whole && p.vec_out) {

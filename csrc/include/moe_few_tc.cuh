@@ -39,6 +39,8 @@
 // fp32 runs into three to six accumulators in turn along K, added in registers.
 #pragma once
 
+#include <type_traits>
+
 #include "serving.h"
 #include "serving_device.cuh"
 #include "sm100_ptx.cuh"
@@ -631,9 +633,15 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
                 if (take >> col & 1u) put(col, serving_swiglu(gate, lin));
               }
             } else {
+              auto all = [&](auto act) {   // one loop to an activation: a launch fetches only the code of its own
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if ((take >> i & 1u) && unit < r.units) put(i, serving_act(__uint_as_float(v[i]) + bias, e.act));
+                for (int i = 0; i < 16; ++i)
+                  if ((take >> i & 1u) && unit < r.units) put(i, serving_act(__uint_as_float(v[i]) + bias, (int)decltype(act)::value));
+              };
+              if (e.act == (int)Act::kRelu) all(std::integral_constant<Act, Act::kRelu>{});
+              else if (e.act == (int)Act::kGelu) all(std::integral_constant<Act, Act::kGelu>{});
+              else if (e.act == (int)Act::kSilu) all(std::integral_constant<Act, Act::kSilu>{});
+              else all(std::integral_constant<Act, Act::kNone>{});
             }
           }
           fence_proxy_async_smem();

@@ -100,6 +100,21 @@ __device__ __forceinline__ float serving_act(float z, int act) {
   }
 }
 
+// Several at a time, one loop to an activation: a launch fetches only the code of its own.
+template <int N>
+__device__ __forceinline__ void serving_act_each(float (&v)[N], int act) {
+  if (act == (int)Act::kRelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = serving_act(v[i], (int)Act::kRelu);
+  } else if (act == (int)Act::kGelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = serving_act(v[i], (int)Act::kGelu);
+  } else if (act == (int)Act::kSilu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = serving_act(v[i], (int)Act::kSilu);
+  }
+}
+
 __device__ __forceinline__ float serving_swiglu(float gate, float up) { return gate * serving_sigmoid(gate) * up; }
 
 // fp32 as two tf32 numbers: hi is v rounded to 11 significant bits, lo what is

@@ -220,7 +220,6 @@ static void launch_dense(const LinearParams& p, cudaStream_t s) {
   const int ob = p.out_bf16 ? 2 : 4, rb = p.res_bf16 ? 2 : 4;
   dp.vec_out = ((uintptr_t)p.out & 15) == 0 && (p.out_stride * ob) % 16 == 0;
   dp.vec_res = ((uintptr_t)p.residual & 15) == 0 && (p.res_stride * rb) % 16 == 0;
-  dp.vec_bias = ((uintptr_t)p.bias & 15) == 0 && (!GLU || p.N % 4 == 0);
   const long long tiles = (long long)dp.mt * dp.nt;
   const int pairs = (int)std::min<long long>(tiles, serving_sm_count() / 2);
   launch_with_pdl(kern, dim3(2 * pairs), dim3(kDenseThreads), C::SMEM, s, true, tx, tw, dp, serving_status());
