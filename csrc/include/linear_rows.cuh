@@ -190,8 +190,8 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       uint8_t* w = smem + stage * SB;
       uint8_t* x = w + kRowsPack * kRowsTile;
       const int n = steps - i * kRowsPack < kRowsPack ? steps - i * kRowsPack : kRowsPack;
-      split_tile(w, low + slot * kRowsPack * kRowsTile, tid, n * kRowsTile);
-      for (int j = 0; j < n; ++j, x += C::PARTS * p.Mp * 128) split_tile(x, x + p.Mp * 128, tid, p.Mp * 128);
+      split_tile<false>(w, low + slot * kRowsPack * kRowsTile, tid, n * kRowsTile);
+      for (int j = 0; j < n; ++j, x += C::PARTS * p.Mp * 128) split_tile<true>(x, x + p.Mp * 128, tid, p.Mp * 128);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&parted[stage]);

@@ -706,7 +706,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       if (turn % 2 == g) {
         ok = mbar_wait_warp(&full[stage], phase, status, kFewKernelId, kFewWaitNs) &&
              (turn < kFewLow || mbar_wait_warp(&empty[was], was_phase, status, kFewKernelId, kFewWaitNs));
-        split_tile(smem + stage * SB, low + slot * kFewTile, tid, bytes);
+        split_tile<false>(smem + stage * SB, low + slot * kFewTile, tid, bytes);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&parted[stage]);

@@ -128,19 +128,35 @@ __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
   lo = fabsf(hi) == INFINITY ? 0.f : v - hi;
 }
 
-// Sixteen bytes of a tile in place into high parts, the low parts to `low`.
+// What the tensor core does not read of an fp32 number, which it takes by its
+// upper 19 bits: v less those, 13 bits rounded to 11 (2^-22 of v is lost at most).
+__device__ __forceinline__ float rest_tf32(float v) {
+  const float rest = fabsf(v) == INFINITY ? 0.f : v - __uint_as_float(__float_as_uint(v) & 0xffffe000u);
+  uint32_t l;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(l) : "f"(rest));
+  return __uint_as_float(l);
+}
+
+// Sixteen bytes of a tile: BOTH, in place into high parts, the low parts to
+// `low`; else only the rests to `low`, and the tile serves as the high parts.
+template <bool BOTH>
 __device__ __forceinline__ void split_store(uint8_t* at, uint8_t* low, const float4& v) {
   float4 h, l;
-  split_tf32(v.x, h.x, l.x);
-  split_tf32(v.y, h.y, l.y);
-  split_tf32(v.z, h.z, l.z);
-  split_tf32(v.w, h.w, l.w);
-  *(float4*)at = h;
+  if constexpr (BOTH) {
+    split_tf32(v.x, h.x, l.x);
+    split_tf32(v.y, h.y, l.y);
+    split_tf32(v.z, h.z, l.z);
+    split_tf32(v.w, h.w, l.w);
+    *(float4*)at = h;
+  } else {
+    l = make_float4(rest_tf32(v.x), rest_tf32(v.y), rest_tf32(v.z), rest_tf32(v.w));
+  }
   *(float4*)low = l;
 }
 
 // `bytes` of a tile (a multiple of 16) by the 128 threads of a group: eight
 // loads in flight, without a test while whole rounds of 16 KB are left.
+template <bool BOTH>
 __device__ __forceinline__ void split_tile(uint8_t* at, uint8_t* low, int tid, int bytes) {
   constexpr int STEP = 128 * 16;
   at += tid * 16;
@@ -150,9 +166,9 @@ __device__ __forceinline__ void split_tile(uint8_t* at, uint8_t* low, int tid, i
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = *(const float4*)(at + i * STEP);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) split_store(at + i * STEP, low + i * STEP, v[i]);
+    for (int i = 0; i < 8; ++i) split_store<BOTH>(at + i * STEP, low + i * STEP, v[i]);
   }
-  for (bytes -= tid * 16; bytes > 0; bytes -= STEP, at += STEP, low += STEP) split_store(at, low, *(const float4*)at);
+  for (bytes -= tid * 16; bytes > 0; bytes -= STEP, at += STEP, low += STEP) split_store<BOTH>(at, low, *(const float4*)at);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
