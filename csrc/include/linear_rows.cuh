@@ -11,9 +11,10 @@
 // shared memory, no global scratch and no counters, the same result every
 // time), then bias, activation and residual, and rounds once.
 //
-// fp32: eight warps split the staged tiles into two tf32 parts of 11 bits (see
-// split_tf32), in place and into a short ring for the weights' low parts;
-// h h' + h l' + l h' is the product to 2^-21.  The tensor core cuts what does
+// fp32: two tf32 parts of 11 bits each, made by eight warps from the staged
+// tiles: x in place and beside it (split_tf32), of the weights, whose upper 19
+// bits the tensor core reads, only the rests (rest_tf32), into a short ring;
+// h h' + h l' + l h' is the product to 2^-20.  The tensor core cuts what does
 // not fit its accumulator instead of rounding, which drifts toward zero with
 // the length of the chain (2e-6 of the result for each 1024 of K): every 512 of
 // K the sums go to registers and are added there, rounded to nearest, while the

@@ -31,12 +31,16 @@
 //               product 2 reads
 //   product 2   tiles of 128 rows of W2, K = the range's hidden rows
 //
-// fp32 weights are split into two tf32 parts of 11 bits each in shared memory,
-// h + l; x and the activations too.  h h' + h l' + l h' is the product to 2^-21:
-// the tokens' parts are stacked as 2N columns, so that is two instructions.  The
-// tensor core cuts what does not fit its accumulator, which drifts with the
-// length of the chain (2e-6 of the result for each 1024 of K), so product 1 of
-// fp32 runs into three to six accumulators in turn along K, added in registers.
+// fp32 numbers are taken as two tf32 parts of 11 bits each, h + l: x and the
+// activations as two copies, the weights as they lie (the tensor core reads
+// their upper 19 bits) with the rests written beside them in shared memory.
+// h h' + h l' + l h' is the product to 2^-20: the tokens' parts are stacked as
+// 2N columns, so that is two instructions.  The tensor core cuts what does not
+// fit its accumulator, which drifts with the length of the chain (2e-6 of the
+// result for each 1024 of K), so product 1 of fp32 runs into three to six
+// accumulators in turn along K, added in registers.  Two groups of splitting
+// warps set the pace of fp32 (8 experts 1024 x 4096, 16 tokens: 82 us; writing
+// the high parts too 90, writing nothing 68).
 #pragma once
 
 #include <type_traits>
@@ -50,7 +54,7 @@ namespace raiccl {
 constexpr int kFewTile = 128 * 128;           // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kFewSlack = 12 * 1024;          // behind the last tile: rows that an instruction reads past a short one
 constexpr int kFewMaxStages = 12;
-constexpr int kFewLow = 3;                    // fp32: stages whose low parts of the weights are kept
+constexpr int kFewLow = 2;                    // fp32: stages whose low parts of the weights are kept (3: a stage less, 84 against 82 us)
 constexpr unsigned long long kFewWaitNs = 2000000000ull;
 constexpr int kFewKernelId = 600;
 

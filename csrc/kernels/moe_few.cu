@@ -441,8 +441,8 @@ static long long up256(long long v) { return (v + 255) / 256 * 256; }
 constexpr int kFewShared = 232448 - 10 * 1024 - 1024;  // dynamic shared memory besides the kernel's own and the alignment
 // By rows up to so many bytes of weights, counted once for each (token, choice).  Measured, rows against tensor cores (us):
 // bf16 64 experts 512 x 352, 1 token (6.5 MB) 11 / 17, 4 tokens (26 MB) 21 / 21, 32 experts 1024 x 1024, 2 tokens (50 MB)
-// 29 / 26; fp32 8 experts 1024 x 4096, 1 token (67 MB) 24 / 49, 4 (268 MB) 52 / 76, 8 (537 MB) 82 / 86, 16 130 / 89.
-constexpr double kFewRowBytes = 30e6, kFewRowBytesFp32 = 400e6;
+// 29 / 26; fp32 8 experts 1024 x 4096, 1 token (67 MB) 20 / 42, 4 (268 MB) 46 / 72, 8 (537 MB) 77 / 80, 12 105 / 81.
+constexpr double kFewRowBytes = 30e6, kFewRowBytesFp32 = 540e6;
 // One token: with few experts every CTA routes for itself and a launch is saved (us, apart against together): 4 experts, rows
 // of 2048 fp32 9.4 / 8.3 in a graph, 11.7 / 9.3 outside one; 16 experts, 2048 bf16 9.3 / 9.4 and 11.8 / 9.8; 64 experts, 512
 // bf16 10.1 / 13.1, since a warp takes its experts one after the other; 32 experts, 2048 bf16 9.6 / 11.3.

@@ -32,11 +32,11 @@ def _make(T, D, E, F, O, act, dtype, seed=0, bias=False):
 
 def _sizes(tensor, dtype, pairs, O=None):
     """(D, F, O): widths whose (token, choice) pairs read few bytes of weights (by rows, on CUDA cores) or many (on the tensor
-    cores, from 30 MB in bf16 and 400 MB in fp32), as csrc/kernels/moe_few.cu chooses."""
+    cores, from 30 MB in bf16 and 540 MB in fp32), as csrc/kernels/moe_few.cu chooses."""
     if not tensor:
         return 256, 96, O or 128
     D, F = (512, 1000) if dtype == BF16 else (1024, 1400)
-    while pairs * (2 if dtype == BF16 else 4) * 3 * D * F < (32e6 if dtype == BF16 else 420e6):
+    while pairs * (2 if dtype == BF16 else 4) * 3 * D * F < (32e6 if dtype == BF16 else 560e6):
         F += 1000
     return D, F, O or D
 
