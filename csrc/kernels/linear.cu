@@ -57,13 +57,16 @@ constexpr int kRowsShared = 232448 - 2048;   // dynamic shared memory of a CTA, 
 
 static long long up256(long long v) { return (v + 255) / 256 * 256; }
 
-// Which kernel, by what each was measured to take on one B200 (us; sizes 1 to 2048 rows, 512 to 16384 outputs, K 1024 and
-// 4096; the sums below are within a tenth of most).  Beside what memory takes for the operands:
-//   rows       3 + 4 Mp / (64 ranks) for each round of CTAs, and for each 128 bytes of its K 0.14 to 0.24 (fp32: 0.55 to 0.9)
-//   dense 128  5 + 1.2 for each round of pairs and 0.21 for each 128 bytes of K; fp32 0.5, and 8 for the split operands
-//   dense 256  6 + 2.5 and 0.31: fewer rounds, each longer
+// Which kernel, by what each was measured to take on one B200 (us; sizes 32 to 2048 rows, 1024 to 5632 outputs, K 1024 to
+// 4096; the sums below are within a seventh of most):
+//   rows       3 + 4 Mp / (64 ranks) for each round of CTAs, and for each 128 bytes of its K 0.14 to 0.24 (fp32: 0.55 to
+//              0.9); a quarter more where clusters share SMs
+//   dense 128  3.2 + 0.9 for each round of pairs and 0.19 for each 128 bytes of K; fp32 7 + 0.5 and 0.44, and 1.6 for each
+//              million numbers that are split
+//   dense 256  4.2 + 1.8 and 0.29: fewer rounds, each longer
 //   vector     very few rows, see below
-// So one row of 4096 x 4096 takes 7 us by rows and 19 by dense tiles; 256 rows 22 and 19; 2048 rows 122, 61 and 50.
+// So 4096 x 4096 takes (rows, 128, 256) for 64 rows 11.9, 16.2, 24.1, for 384 rows 26.1, 17.5, 24.8, for 2048 rows 117, 60,
+// 50; 1024 x 4096 fp32 for 64 rows 13.4, 27.2, for 384 rows 60, 31.
 LinearPlan plan_linear(const LinearParams& p) {
   LinearPlan r{};
   const int eb = p.bf16 ? 2 : 4, sms = serving_sm_count();
@@ -88,7 +91,8 @@ LinearPlan plan_linear(const LinearParams& p) {
     const long long slots = (long long)per * sms * (ranks == 8 ? 81 : ranks == 4 ? 89 : 100) / 100;   // clusters leave SMs empty
     const long long rounds = (tiles * ranks + slots - 1) / slots;
     const double step = p.bf16 ? 0.14 + 0.1 * r.Mp / 64 : 0.55 + 0.35 * r.Mp / 64;
-    const double cost = rounds * (3.0 + 4.0 * r.Mp / 64 / ranks + (KB + ranks - 1) / ranks * step) + 0.1 * ranks;
+    const double shared = p.bf16 && ranks > 1 && tiles * ranks > sms ? 1.25 : 1.0;
+    const double cost = rounds * (3.0 + 4.0 * r.Mp / 64 / ranks + (KB + ranks - 1) / ranks * step) * shared + 0.1 * ranks;
     if (r.ranks == 0 || cost < best) {
       best = cost;
       r.ranks = ranks;
@@ -100,8 +104,8 @@ LinearPlan plan_linear(const LinearParams& p) {
     for (int bn = 128; bn <= (p.bf16 ? 256 : 128); bn *= 2) {
       const int w = glu ? bn / 2 : bn;
       const long long t = (p.M + 255) / 256 * ((p.N + w - 1) / w), rounds = (t + sms / 2 - 1) / (sms / 2);
-      const double cost = p.bf16 ? (bn == 256 ? 6 + rounds * (2.5 + 0.31 * KB) : 5 + rounds * (1.2 + 0.21 * KB))
-                                 : 13 + rounds * (1.2 + 0.5 * KB) + (double)(p.M + wrows) * p.K * 2e-6;
+      const double cost = p.bf16 ? (bn == 256 ? 4.2 + rounds * (1.8 + 0.29 * KB) : 3.2 + rounds * (0.9 + 0.19 * KB))
+                                 : 7 + rounds * (0.5 + 0.44 * KB) + (double)(p.M + wrows) * p.K * 1.6e-6;
       if (cost < best) {
         best = cost;
         r.dense = bn;

@@ -384,7 +384,7 @@ class ProgressiveMoELayer:
         its device; returns (out [T, out_dim], expert ids [T, top_k], gates).
 
         Runs on the current stream with the weights that every rank holds, in
-        three launches and without the progressive machinery (no chunks, no
+        two or three launches and without the progressive machinery (no chunks, no
         dispatch, no peers), so it needs no other rank and leaves the layer's
         buffers alone.  Router, masks and gates are the layer's, row t taking
         position t of the topology mask; the synthetic per-chunk logit bias of a
