@@ -35,7 +35,7 @@ def linear(
 
     Sums are kept in fp32 and rounded once, to out_dtype (default: x's type;
     fp32 inputs give fp32).  fp32 inputs are multiplied to fp32 accuracy, not
-    to tf32's (a value whose rounding to 11 bits overflows counts as infinite);
+    to tf32's (an infinite result may come out as NaN);
     bf16 inputs leave the tensor core's own sums, which over a K of 14336 drift
     by up to 3e-5 of an fp32 result.  Enqueues on the current stream without
     synchronising and can be captured in a CUDA graph.  Rows of x or weight

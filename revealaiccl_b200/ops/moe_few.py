@@ -51,7 +51,8 @@ def moe_few_tokens(
     (or zeros).  residual [T, O]: fp32 or bf16; ``out`` may be the same tensor.
 
     Sums are kept in fp32; bf16 layers keep the hidden activation in bf16, as
-    the large layer does, except in the smallest calls, which keep it in fp32.
+    the large layer does, except in the smallest calls, which keep it in fp32;
+    an fp32 result that is infinite may come out as NaN.
     Returns (out [T, O] in out_dtype or x's type, expert ids int32 [T, top_k],
     gates fp32 [T, top_k]).  Enqueues two or three launches on the current stream
     without synchronising and can be captured in a CUDA graph; outputs and
