@@ -67,12 +67,17 @@ struct FewExpertPlan {
   int grid, stages, hbytes, Op, Tp;
   int pack;               // x is packed by the routing kernel
   int packed_stride;
-  long long packed_bytes, a_bytes;  // multiples of 256; in this order in the workspace
-  long long bytes() const { return packed_bytes + a_bytes; }
+  int pack_w;             // the experts are copied to rows that TMA can read
+  long long packed_bytes, a_bytes, w1_bytes, w2_bytes;  // multiples of 256; in this order in the workspace
+  long long bytes() const { return packed_bytes + a_bytes + w1_bytes + w2_bytes; }
 };
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p);
 void launch_few(const FewRouteParams& r, const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s);
+
+// `groups` blocks of rows of K elements, `group` apart, to one block of rows that start on 16 bytes, `packed` apart.
+void launch_pack_rows(const void* src, long long stride, long long group, int groups, void* dst, int packed, long long rows, int K,
+                      int bf16, cudaStream_t s);
 
 // The current device's record of a wait that ran out in a serving operator (device memory).
 DeviceStatus* serving_status();

@@ -20,9 +20,13 @@ namespace raiccl {
 // bytes at a time from the two aligned words around them, shifted together; the
 // last word of a row, whose second neighbour may lie behind the tensor, by
 // elements.  (One element at a time took 35 us for 1728 x 9097 bf16.)
+// Groups of rows (experts) are a grid row each.
 template <typename T>
-__global__ void __launch_bounds__(256) linear_pack_kernel(const T* src, long long stride, T* dst, int packed, long long rows, int K) {
+__global__ void __launch_bounds__(256) linear_pack_kernel(const T* src, long long stride, long long group, T* dst, int packed,
+                                                          long long rows, int K) {
   constexpr int V = 16 / sizeof(T);
+  src += blockIdx.y * group;
+  dst += blockIdx.y * rows * packed;
   griddep_wait();
   griddep_launch_dependents();
   const int per = (K + V - 1) / V;   // 16-byte words of a row
@@ -272,13 +276,15 @@ static void launch_vector_any(const LinearParams& p, bool vec, cudaStream_t s) {
   }
 }
 
-static void pack(const void* src, long long stride, void* dst, int packed, long long rows, int K, int bf16, cudaStream_t s) {
-  const dim3 grid((unsigned)(8 * serving_sm_count()));
+void launch_pack_rows(const void* src, long long stride, long long group, int groups, void* dst, int packed, long long rows, int K,
+                      int bf16, cudaStream_t s) {
+  const dim3 grid((unsigned)((8 * serving_sm_count() + groups - 1) / groups), groups);
   if (bf16)
-    launch_with_pdl(linear_pack_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, (const __nv_bfloat16*)src, stride,
+    launch_with_pdl(linear_pack_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, (const __nv_bfloat16*)src, stride, group,
                     (__nv_bfloat16*)dst, packed, rows, K);
   else
-    launch_with_pdl(linear_pack_kernel<float>, grid, dim3(256), 0, s, true, (const float*)src, stride, (float*)dst, packed, rows, K);
+    launch_with_pdl(linear_pack_kernel<float>, grid, dim3(256), 0, s, true, (const float*)src, stride, group, (float*)dst, packed,
+                    rows, K);
 }
 
 void launch_linear(const LinearParams& params, const LinearPlan& plan, void* workspace, cudaStream_t s) {
@@ -303,12 +309,12 @@ void launch_linear(const LinearParams& params, const LinearPlan& plan, void* wor
     p.x_stride = p.w_stride = plan.packed_stride;
   }
   if (plan.pack_x && !(plan.dense && !p.bf16)) {
-    pack(p.x, p.x_stride, ws, plan.packed_stride, p.M, p.K, p.bf16, s);
+    launch_pack_rows(p.x, p.x_stride, 0, 1, ws, plan.packed_stride, p.M, p.K, p.bf16, s);
     p.x = ws;
     p.x_stride = plan.packed_stride;
   }
   if (plan.pack_w && !(plan.dense && !p.bf16)) {
-    pack(p.w, p.w_stride, ws + plan.x_bytes, plan.packed_stride, glu ? 2ll * p.N : p.N, p.K, p.bf16, s);
+    launch_pack_rows(p.w, p.w_stride, 0, 1, ws + plan.x_bytes, plan.packed_stride, glu ? 2ll * p.N : p.N, p.K, p.bf16, s);
     p.w = ws + plan.x_bytes;
     p.w_stride = plan.packed_stride;
   }

@@ -437,6 +437,7 @@ int serving_sm_count() {
 }
 
 static long long up256(long long v) { return (v + 255) / 256 * 256; }
+static long long up8(long long v) { return (v + 7) / 8 * 8; }
 
 constexpr int kFewShared = 232448 - 10 * 1024 - 1024;  // dynamic shared memory besides the kernel's own and the alignment
 // By rows up to so many bytes of weights, counted once for each (token, choice).  Measured, rows against tensor cores (us):
@@ -447,6 +448,10 @@ constexpr double kFewRowBytes = 30e6, kFewRowBytesFp32 = 540e6;
 // of 2048 fp32 9.4 / 8.3 in a graph, 11.7 / 9.3 outside one; 16 experts, 2048 bf16 9.3 / 9.4 and 11.8 / 9.8; 64 experts, 512
 // bf16 10.1 / 13.1, since a warp takes its experts one after the other; 32 experts, 2048 bf16 9.6 / 11.3.
 constexpr int kFewOwnExperts = 16, kFewOwnBytes = 65536;
+// Weights that TMA cannot read go by rows, element by element (bytes of (token, choice) pairs each us), or all experts are copied
+// first (bytes read and written each us) where that is less: few experts and many tokens (27 tokens top-3, 4 experts 1803 x
+// 1809 bf16, us: 298 by rows, 77 with the copy).
+constexpr double kFewOddRate = 4.5e6, kFewPackRate = 5e6;
 constexpr int kFewJoinRoom = 24 * 1024;                // of the join's CTA beside it
 
 FewExpertPlan plan_few_experts(const FewExpertParams& p) {
@@ -455,11 +460,19 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
   auto aligned = [&](const void* base, long long row, long long expert) {
     return ((uintptr_t)base & 15) == 0 && (row * eb) % 16 == 0 && (p.E == 1 || (expert * eb) % 16 == 0);
   };
+  const int n1 = (p.act == (int)Act::kSwiGLU ? 2 : 1) * p.F;
   // TMA reads rows that start on 16 bytes
-  const bool rows16 = aligned(p.w1, p.w1_stride, p.w1_estride) && aligned(p.w2, p.w2_stride, p.w2_estride);
+  const bool rows16 = aligned(p.w1, p.w1_stride, p.w1_estride) && aligned(p.w2, p.w2_stride, p.w2_estride) &&
+                      p.w1_stride > 0 && p.w2_stride > 0 && (p.E == 1 || (p.w1_estride > 0 && p.w2_estride > 0));
   const int pairs = p.T * p.k;
-  const double bytes = (double)pairs * eb * ((p.act == (int)Act::kSwiGLU ? 2.0 : 1.0) * p.F * p.D + (double)p.O * p.F);
-  r.tensor = rows16 && bytes > (p.bf16 ? kFewRowBytes : kFewRowBytesFp32);
+  const double expert = (double)eb * ((double)n1 * p.D + (double)p.O * p.F), bytes = pairs * expert;
+  if (rows16) {
+    r.tensor = bytes > (p.bf16 ? kFewRowBytes : kFewRowBytesFp32);
+  } else if (bytes / kFewOddRate > p.E * expert * 2 / kFewPackRate + std::min(p.E, pairs) * expert / (p.bf16 ? 5e6 : 3e6) + 20) {
+    r.tensor = r.pack_w = 1;
+    r.w1_bytes = up256((long long)p.E * n1 * up8(p.D) * eb);
+    r.w2_bytes = up256((long long)p.E * p.O * up8(p.F) * eb);
+  }
   if (!r.tensor) {
     r.vec = rows16 && (p.D * eb) % 16 == 0 && (p.F * eb) % 16 == 0 && aligned(p.x, p.T > 1 ? p.x_stride : 0, 0);
     r.a_bytes = up256((long long)pairs * p.F * 4);
@@ -505,7 +518,8 @@ static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CU
   launch_with_pdl(kern, dim3(grid), dim3(FewTc<FP32>::THREADS), smem, s, true, tx, t1, t1w, t2, t2u, tp, serving_status());
 }
 
-void launch_few(const FewRouteParams& r, const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
+void launch_few(const FewRouteParams& r, const FewExpertParams& params, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
+  FewExpertParams p = params;
   char* ws = (char*)workspace;
   float* a = (float*)(ws + plan.packed_bytes);
   if (!plan.route) launch_route(r, s);
@@ -513,6 +527,19 @@ void launch_few(const FewRouteParams& r, const FewExpertParams& p, const FewExpe
     if (p.bf16) launch_rows<__nv_bfloat16>(p, r, plan, a, s);
     else launch_rows<float>(p, r, plan, a, s);
     return;
+  }
+  if (plan.pack_w) {
+    char* const w1 = ws + plan.packed_bytes + plan.a_bytes;
+    char* const w2 = w1 + plan.w1_bytes;
+    const int n1 = (p.act == (int)Act::kSwiGLU ? 2 : 1) * p.F, s1 = (int)up8(p.D), s2 = (int)up8(p.F);
+    launch_pack_rows(p.w1, p.w1_stride, p.w1_estride, p.E, w1, s1, n1, p.D, p.bf16, s);
+    launch_pack_rows(p.w2, p.w2_stride, p.w2_estride, p.E, w2, s2, p.O, p.F, p.bf16, s);
+    p.w1 = w1;
+    p.w2 = w2;
+    p.w1_stride = s1;
+    p.w2_stride = s2;
+    p.w1_estride = (long long)n1 * s1;
+    p.w2_estride = (long long)p.O * s2;
   }
   const cuuint64_t eb = p.bf16 ? 2 : 4;
   const cuuint32_t bk = 128 / eb;

@@ -57,8 +57,10 @@ def moe_few_tokens(
     gates fp32 [T, top_k]).  Enqueues two or three launches on the current stream
     without synchronising and can be captured in a CUDA graph; outputs and
     workspace come from torch's allocator on that stream.  Expert rows that do
-    not start on 16 bytes are read element by element.  ``check=True`` waits
-    and raises on a recorded device status.  There is no backward.
+    not start on 16 bytes are read element by element or, where many tokens
+    share few experts, copied first, which takes as much memory as all experts.
+    ``check=True`` waits and raises on a recorded device status.  There is no
+    backward.
     """
     if act not in ACT_IDS:
         raise ValueError(f"moe_few_tokens: act must be one of {sorted(ACT_IDS)}")

@@ -224,6 +224,30 @@ def test_strides(dtype, offset, pad, tensor):
     assert torch.equal(ob, torch.full_like(ob, 7.0))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T,D,E,k,F,O,act", [(33, 401, 4, 4, 2203, 302, "swiglu"), (64, 515, 8, 8, 1777, 131, "gelu"), (20, 1803, 4, 3, 1809, 1803, "swiglu"),
+                                             (64, 2051, 1, 1, 1001, 77, "relu"), (40, 512, 3, 3, 2000, 520, "swiglu"), (12, 2050, 2, 2, 3001, 66, "silu")])
+def test_many_tokens_on_odd_rows(T, D, E, k, F, O, act, dtype):
+    """Weights off 16 bytes with enough tokens for a copy of the experts: odd widths, and windows at odd places."""
+    a = _make(T, D, E, F, O, act, dtype, bias=True)
+    if D % 8 == 0:
+        for n in ("w1", "w2"):
+            w = a[n]
+            wide = torch.full((2 * w.shape[0], w.shape[1] + 1, w.shape[2] + 3), float("nan"), device=DEV, dtype=dtype)
+            view = wide[1::2, 1:, 1:1 + w.shape[2]]
+            view.copy_(w)
+            a[n] = view
+    _check(a, k, act, "topk_softmax", residual=torch.randn(T, O, device=DEV).to(dtype))
+
+
+@pytest.mark.parametrize("T", [1, 4, 48])
+def test_experts_that_share_their_weights(T):
+    """Experts, or rows of an expert, that are one tensor expanded."""
+    a = _make(T, 512, 4, 1000, 256, "swiglu", BF16)
+    _check(dict(a, w1=a["w1"][:1].expand(4, -1, -1), w2=a["w2"][:1].expand(4, -1, -1)), 3, "swiglu", "softmax")
+    _check(dict(a, w2=a["w2"][:, :1].expand(-1, 256, -1)), 3, "swiglu", "softmax")
+
+
 def test_empty_batch_and_in_place():
     a = _make(4, 64, 4, 32, 64, "swiglu", BF16)
     e = dict(a, x=a["x"][:0])
