@@ -77,7 +77,7 @@ void check_vector(const char* op, const char* name, const torch::Tensor& t, cons
 // out and residual of [rows, width]; out is allocated where none is given.
 torch::Tensor check_out(const char* op, const OptTensor& out, const OptTensor& residual, const torch::Tensor& like,
                         c10::optional<torch::ScalarType> out_dtype, int64_t rows, int64_t width,
-                        std::initializer_list<const torch::Tensor*> inputs) {
+                        std::initializer_list<const torch::Tensor*> inputs, std::initializer_list<const OptTensor*> more) {
   const torch::Device dev = like.device();
   torch::ScalarType dt = out_dtype ? *out_dtype : out ? out->scalar_type() : like.scalar_type();
   TORCH_CHECK_VALUE(dt == torch::kFloat32 || (dt == torch::kBFloat16 && like.scalar_type() == torch::kBFloat16), op,
@@ -101,6 +101,8 @@ torch::Tensor check_out(const char* op, const OptTensor& out, const OptTensor& r
                     ": out must have contiguous rows that do not overlap");
   for (const torch::Tensor* t : inputs)
     TORCH_CHECK_VALUE(!overlap(*out, *t), op, ": out shares memory with an input");
+  for (const OptTensor* t : more)
+    TORCH_CHECK_VALUE(!*t || !overlap(*out, **t), op, ": out shares memory with an input");
   if (residual && overlap(*out, *residual))  // in place: each element is read and written by one thread
     TORCH_CHECK_VALUE(out->data_ptr() == residual->data_ptr() && out->scalar_type() == residual->scalar_type() &&
                           (rows <= 1 || out->stride(0) == residual->stride(0)),
@@ -149,7 +151,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
                           inner_contiguous(*block_mask),
                       op, ": block_mask must be bool or uint8 of shape [E] or [T, E] with contiguous rows");
   }
-  torch::Tensor res = check_out(op, out, residual, x, out_dtype, T, O, {&x, &router_w, &w1, &w2});
+  torch::Tensor res = check_out(op, out, residual, x, out_dtype, T, O, {&x, &router_w, &w1, &w2}, {&router_b, &b1, &b2, &block_mask});
   const c10::cuda::CUDAGuard guard(dev);
   torch::Tensor ids = fresh({T, top_k}, torch::kInt32, dev);
   torch::Tensor gates = fresh({T, top_k}, torch::kFloat32, dev);
@@ -232,7 +234,7 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   TORCH_CHECK_VALUE(inner_contiguous(x) && inner_contiguous(weight), op, ": x and weight must have contiguous rows");
   const int64_t N = glu ? rows / 2 : rows;
   if (bias) check_vector(op, "bias", *bias, dev, {rows});
-  torch::Tensor res = check_out(op, out, residual, x, out_dtype, M, N, {&x, &weight});
+  torch::Tensor res = check_out(op, out, residual, x, out_dtype, M, N, {&x, &weight}, {&bias});
   c10::cuda::CUDAGuard guard(dev);
   if (M == 0 || N == 0) return res;
   raiccl::LinearParams p{};

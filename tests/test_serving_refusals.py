@@ -100,3 +100,11 @@ def test_shared_memory_is_refused():
         _linear(residual=r[:3], out=r[1:])
     with pytest.raises(ValueError, match="CUDA device"):
         _linear(residual=r[:3], out=r[:3])
+
+
+def test_out_apart_from_biases_and_mask():
+    buf = torch.zeros(64)
+    with pytest.raises(ValueError, match="shares memory with an input"):
+        _linear(bias=buf[4:12], out=buf[:24].view(3, 8), out_dtype=torch.float32)
+    with pytest.raises(ValueError, match="shares memory with an input"):
+        _moe(router_b=buf[28:32], out=buf[:30].view(3, 10), out_dtype=torch.float32)
