@@ -30,7 +30,7 @@ namespace raiccl {
 constexpr int kDenseThreads = 320;         // TMA, MMA, eight epilogue warps
 constexpr int kDenseKernelId = 620;
 constexpr int kDenseGroup = 8;
-constexpr int kDenseChain = 8;             // fp32: 128-byte steps of K of a chain
+constexpr int kDenseChain = 4;             // fp32: 128-byte steps of K of a chain
 constexpr unsigned long long kDenseWaitNs = 2000000000ull;
 
 struct LinearDenseParams {

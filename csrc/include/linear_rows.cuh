@@ -31,7 +31,7 @@ namespace raiccl {
 constexpr int kRowsTile = 128 * 128;       // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kRowsPack = 2;               // 128-byte steps of K in a stage: a stage costs its waits and its commit, 0.15 us
 constexpr int kRowsMaxStages = 12;
-constexpr int kRowsChain = 4;              // fp32: stages into one accumulator
+constexpr int kRowsChain = 2;              // fp32: stages into one accumulator
 constexpr int kRowsKernelId = 610;
 constexpr unsigned long long kServingWaitNs = 2000000000ull;
 

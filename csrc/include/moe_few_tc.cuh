@@ -54,6 +54,7 @@ namespace raiccl {
 constexpr int kFewTile = 128 * 128;           // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kFewSlack = 12 * 1024;          // behind the last tile: rows that an instruction reads past a short one
 constexpr int kFewMaxStages = 12;
+constexpr int kFewChain = 11;                 // fp32: 128-byte steps of K of an accumulator
 constexpr int kFewLow = 2;                    // fp32: stages whose low parts of the weights are kept (3: a stage less, 84 against 82 us)
 constexpr unsigned long long kFewWaitNs = 2000000000ull;
 constexpr int kFewKernelId = 600;
@@ -212,11 +213,13 @@ struct FewWalk {
 // tokens' tiles share a hand-over.  At most 512 columns in all.
 struct FewAcc {
   int n1, groups, nbuf, chains, tiles;
-  __device__ FewAcc(int n1_, bool fp32) : n1(n1_) {
+  // fp32: chains of 512 of K (kFewChain steps) at most, where that many accumulators fit; one epilogue group has more of
+  // them (16 tokens, D 4096: error 3.4e-6 with six).
+  __host__ __device__ FewAcc(int n1_, bool fp32, int steps) : n1(n1_) {
     if (fp32) {
-      groups = n1 <= 64 ? 2 : 1;
+      groups = n1 <= 64 && steps <= (n1 <= 32 ? 6 : 3) * kFewChain ? 2 : 1;
       nbuf = 1;
-      chains = n1 <= 32 ? 6 : n1 <= 64 ? 3 : n1 <= 96 ? 4 : 3;
+      chains = n1 <= 32 ? (groups == 2 ? 6 : 14) : n1 <= 64 ? (groups == 2 ? 3 : 7) : n1 <= 96 ? 4 : 3;
       tiles = n1 <= 32 ? 2 : 1;
     } else {
       groups = 2;
@@ -345,7 +348,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   const FewExpertParams& e = p.e;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n1 = C::PARTS * p.Tp;                       // columns of an accumulator
-  const FewAcc acc(n1, FP32);
+  const FewAcc acc(n1, FP32, (e.D + C::BK - 1) / C::BK);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], 4); }

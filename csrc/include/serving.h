@@ -67,6 +67,7 @@ struct FewExpertPlan {
   int grid, stages, hbytes, Op, Tp;
   int pack;               // x is packed by the routing kernel
   int packed_stride;
+  int slice;              // fp32 on the tensor cores: tokens that go together
   int pack_w;             // the experts are copied to rows that TMA can read
   long long packed_bytes, a_bytes, w1_bytes, w2_bytes;  // multiples of 256; in this order in the workspace
   long long bytes() const { return packed_bytes + a_bytes + w1_bytes + w2_bytes; }

@@ -479,23 +479,35 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
     r.route = p.T == 1 && p.E <= kFewOwnExperts && (long long)p.E * p.D * eb <= kFewOwnBytes;
     return r;
   }
+  // fp32: so many tokens at a time that no accumulator takes more than 512 of K, if 16 can (D 7168), since it is cut at each
+  // step (64 tokens, D 4096, SwiGLU: error 6.6e-6 all at once); the weights are then read again for each.
+  r.slice = p.T;
+  if (!p.bf16) {
+    const int steps = (p.D + 31) / 32;
+    auto fits = [&](int T) {
+      const int n1 = 2 * ((T + 15) / 16 * 16);
+      return steps <= FewAcc(n1, true, steps).chains * kFewChain;
+    };
+    if (!fits(p.T)) r.slice = std::min(p.T, fits(32) ? 32 : 16);
+  }
+  const int T = r.slice;
   r.grid = std::min(serving_sm_count(), kFewJoinItems - 2 * kFewTopK);
   r.Op = (p.O + 127) / 128 * 128;
-  r.Tp = (p.T + 15) / 16 * 16;
+  r.Tp = (T + 15) / 16 * 16;
   const int UE = (p.F + 15) / 16, ups = 128 / eb / 16;
   r.pack = !p.bf16 || !aligned(p.x, p.T > 1 ? p.x_stride : 0, 0);
   r.packed_stride = (p.D + 7) / 8 * 8;
   if (r.pack) r.packed_bytes = up256((long long)parts * r.Tp * r.packed_stride * eb);
   // An expert's tokens times the CTAs that share it, over all experts: n experts have at most min(T k, n T) tokens
   // and (grid / n + 2) CTAs each, so T (grid + 2 k) rows at most, whatever n is.
-  r.a_bytes = up256((long long)p.T * (r.grid + 2 * p.k) * r.Op * 4);
+  r.a_bytes = up256((long long)T * (r.grid + 2 * p.k) * r.Op * 4);
   // Activations of the longest range of a CTA, if that leaves four stages; else the range is worked off in pieces, which
   // costs a sum in memory each.  The rest holds stages.
   const int sb = p.bf16 ? FewTc<false>::stage_bytes(r.Tp) : FewTc<true>::stage_bytes(r.Tp);
   // Up to 16 tokens the join's CTAs find room beside the experts' (64 experts, 1 token: 49.7 -> 43.5 us); with more, the
   // stages are worth more (37 tokens: 193 against 196 us).
-  const int room = kFewShared - (p.T <= 16 ? kFewJoinRoom : 0) - (p.bf16 ? 0 : FewTc<true>::low_bytes());
-  const long long most = ((long long)std::min(p.E, pairs) * UE + r.grid - 1) / r.grid;
+  const int room = kFewShared - (T <= 16 ? kFewJoinRoom : 0) - (p.bf16 ? 0 : FewTc<true>::low_bytes());
+  const long long most = ((long long)std::min(p.E, T * p.k) * UE + r.grid - 1) / r.grid;
   const long long rows = (std::min<long long>(most, UE) + ups - 1) / ups + 1;
   r.hbytes = (int)std::min<long long>(rows * parts * r.Tp * 128, room - 4 * sb);
   r.hbytes = std::max({r.hbytes, parts * r.Tp * 128, kFewSlack});
@@ -518,12 +530,15 @@ static void launch_tensor(const CUtensorMap& tx, const CUtensorMap& t1, const CU
   launch_with_pdl(kern, dim3(grid), dim3(FewTc<FP32>::THREADS), smem, s, true, tx, t1, t1w, t2, t2u, tp, serving_status());
 }
 
-void launch_few(const FewRouteParams& r, const FewExpertParams& params, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
+static void launch_few_tensor(const FewExpertParams& p, const FewExpertPlan& plan, char* ws, cudaStream_t s);
+
+void launch_few(const FewRouteParams& route, const FewExpertParams& params, const FewExpertPlan& plan, void* workspace, cudaStream_t s) {
+  FewRouteParams r = route;
   FewExpertParams p = params;
   char* ws = (char*)workspace;
   float* a = (float*)(ws + plan.packed_bytes);
-  if (!plan.route) launch_route(r, s);
   if (!plan.tensor) {
+    if (!plan.route) launch_route(r, s);
     if (p.bf16) launch_rows<__nv_bfloat16>(p, r, plan, a, s);
     else launch_rows<float>(p, r, plan, a, s);
     return;
@@ -541,6 +556,24 @@ void launch_few(const FewRouteParams& r, const FewExpertParams& params, const Fe
     p.w1_estride = (long long)n1 * s1;
     p.w2_estride = (long long)p.O * s2;
   }
+  const int eb = p.bf16 ? 2 : 4, ob = p.out_bf16 ? 2 : 4, rb = p.res_bf16 ? 2 : 4;
+  for (int t = 0; t < params.T; t += plan.slice) {   // each uses the workspace when the one before has ended
+    r.T = p.T = std::min(plan.slice, params.T - t);
+    r.x = p.x = (const char*)params.x + t * params.x_stride * eb;
+    r.ids = route.ids + t * p.k;
+    r.gates = route.gates + t * p.k;
+    if (route.mask) r.mask = route.mask + t * route.mask_stride;
+    p.ids = r.ids;
+    p.gates = r.gates;
+    p.out = (char*)params.out + t * params.out_stride * ob;
+    if (params.residual) p.residual = (const char*)params.residual + t * params.res_stride * rb;
+    launch_route(r, s);
+    launch_few_tensor(p, plan, ws, s);
+  }
+}
+
+static void launch_few_tensor(const FewExpertParams& p, const FewExpertPlan& plan, char* ws, cudaStream_t s) {
+  float* const a = (float*)(ws + plan.packed_bytes);
   const cuuint64_t eb = p.bf16 ? 2 : 4;
   const cuuint32_t bk = 128 / eb;
   const int parts = p.bf16 ? 1 : 2;
