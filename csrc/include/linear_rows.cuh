@@ -16,9 +16,9 @@
 // bits the tensor core reads, only the rests (rest_tf32), into a short ring;
 // h h' + h l' + l h' is the product to 2^-20.  The tensor core cuts what does
 // not fit its accumulator instead of rounding, which drifts toward zero with
-// the length of the chain (2e-6 of the result for each 1024 of K): every 512 of
+// the length of the chain (2e-6 of the result for each 1024 of K): every 128 of
 // K the sums go to registers and are added there, rounded to nearest, while the
-// next 512 run into the other of two accumulators.  bf16 results are rounded to
+// next 128 run into the other of two accumulators.  bf16 results are rounded to
 // 2^-8, where the drift of a whole K does not show.
 #pragma once
 

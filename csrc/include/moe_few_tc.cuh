@@ -37,8 +37,8 @@
 // h h' + h l' + l h' is the product to 2^-20: the tokens' parts are stacked as
 // 2N columns, so that is two instructions.  The tensor core cuts what does not
 // fit its accumulator, which drifts with the length of the chain (2e-6 of the
-// result for each 1024 of K), so product 1 of fp32 runs into three to six
-// accumulators in turn along K, added in registers.  Two groups of splitting
+// result for each 1024 of K), so product 1 of fp32 runs into three to
+// fourteen accumulators in turn along K, added in registers.  Two groups of splitting
 // warps set the pace of fp32 (8 experts 1024 x 4096, 16 tokens: 82 us; writing
 // the high parts too 90, writing nothing 68).
 #pragma once
@@ -213,7 +213,7 @@ struct FewWalk {
 // tokens' tiles share a hand-over.  At most 512 columns in all.
 struct FewAcc {
   int n1, groups, nbuf, chains, tiles;
-  // fp32: chains of 512 of K (kFewChain steps) at most, where that many accumulators fit; one epilogue group has more of
+  // fp32: chains of 352 of K (kFewChain steps) at most, where that many accumulators fit; one epilogue group has more of
   // them (16 tokens, D 4096: error 3.4e-6 with six).
   __host__ __device__ FewAcc(int n1_, bool fp32, int steps) : n1(n1_) {
     if (fp32) {

@@ -54,7 +54,8 @@ def moe_few_tokens(
     the large layer does, except in the smallest calls, which keep it in fp32;
     an fp32 result that is infinite may come out as NaN.
     Returns (out [T, O] in out_dtype or x's type, expert ids int32 [T, top_k],
-    gates fp32 [T, top_k]).  Enqueues two or three launches on the current stream
+    gates fp32 [T, top_k]).  Enqueues two or three launches (wide fp32 layers: for
+    each 16 or 32 tokens) on the current stream
     without synchronising and can be captured in a CUDA graph; outputs and
     workspace come from torch's allocator on that stream.  Expert rows that do
     not start on 16 bytes are read element by element or, where many tokens
