@@ -103,13 +103,19 @@ LinearPlan plan_linear(const LinearParams& p) {
     }
   }
   if (mt > 65535) best = 1e30;   // more tiles than a grid has rows
+  // Rows of out or residual off 16 bytes: a thread of a dense tile has a row of its own and goes through it element by
+  // element, 20 us for a tile of 128 columns (bf16, dense / rows, us: 269 x 64 x 10735 71 / 16, 4096 x 1024 x 4097 281 / 127).
+  const int ob = p.out_bf16 ? 2 : 4, rb = p.res_bf16 ? 2 : 4;
+  const bool odd = (((uintptr_t)p.out | (uintptr_t)(p.out_stride * ob)) & 15) != 0 ||
+                   (p.residual != nullptr && (((uintptr_t)p.residual | (uintptr_t)(p.res_stride * rb)) & 15) != 0);
   // dense tiles
   if (p.K > 0 && p.M < (1ll << 30)) {
     for (int bn = 128; bn <= (p.bf16 ? 256 : 128); bn *= 2) {
       const int w = glu ? bn / 2 : bn;
       const long long t = (p.M + 255) / 256 * ((p.N + w - 1) / w), rounds = (t + sms / 2 - 1) / (sms / 2);
-      const double cost = p.bf16 ? (bn == 256 ? 4.2 + rounds * (1.8 + 0.29 * KB) : 3.2 + rounds * (0.9 + 0.19 * KB))
-                                 : 7 + rounds * (0.5 + 0.44 * KB) + (double)(p.M + wrows) * p.K * 1.6e-6;
+      const double cost = p.bf16 ? (bn == 256 ? 4.2 + rounds * std::max(1.8 + 0.29 * KB, odd ? 40.0 : 0.0)
+                                               : 3.2 + rounds * std::max(0.9 + 0.19 * KB, odd ? 20.0 : 0.0))
+                                 : 7 + rounds * std::max(0.5 + 0.44 * KB, odd ? 20.0 : 0.0) + (double)(p.M + wrows) * p.K * 1.6e-6;
       if (cost < best) {
         best = cost;
         r.dense = bn;
