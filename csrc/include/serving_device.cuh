@@ -119,21 +119,25 @@ __device__ __forceinline__ float serving_swiglu(float gate, float up) { return g
 
 // fp32 as two tf32 numbers: hi is v rounded to 11 significant bits, lo what is
 // left (at most 12 bits, of which the tensor core reads 11: 2^-23 of v is lost).
-// An infinity has no low part; the last 2^-12 of the range below it counts as
-// infinite.  No branches: with one this took twice as long.
+// Rounding up from the last 2^-12 of the range would give an infinity, so v is
+// cut there (lo then has 13 bits: 2^-21 of v is lost).  An infinity has no low
+// part.  No branches: with one this took twice as long.
 __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
   uint32_t h;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(h) : "f"(v));
-  hi = __uint_as_float(h);
-  lo = fabsf(hi) == INFINITY ? 0.f : v - hi;
+  hi = fabsf(__uint_as_float(h)) == INFINITY ? __uint_as_float(__float_as_uint(v) & 0xffffe000u) : __uint_as_float(h);
+  lo = fabsf(v) == INFINITY ? 0.f : v - hi;
 }
 
 // What the tensor core does not read of an fp32 number, which it takes by its
 // upper 19 bits: v less those, 13 bits rounded to 11 (2^-22 of v is lost at most).
+// Numbers behind the last one of 22 bits, infinities too, count as that one, so
+// that rounding never carries the two parts into an infinity.
 __device__ __forceinline__ float rest_tf32(float v) {
-  const float rest = fabsf(v) == INFINITY ? 0.f : v - __uint_as_float(__float_as_uint(v) & 0xffffe000u);
+  float c;
+  asm("min.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(c) : "f"(v), "f"(__uint_as_float(0x7f7ffffcu)));
   uint32_t l;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(l) : "f"(rest));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(l) : "f"(c - __uint_as_float(__float_as_uint(c) & 0xffffe000u)));
   return __uint_as_float(l);
 }
 

@@ -214,3 +214,23 @@ def test_check_reads_and_clears_the_status():
     assert torch.equal(_linear(x, w, b, act="silu", residual=r, check=True), _linear(x, w, b, act="silu", residual=r))
     status.check_serving()
     status.check_serving(x.device)
+
+
+LARGEST = torch.finfo(FP32).max
+
+
+@pytest.mark.parametrize("m", [4, 20, 300])
+def test_largest_numbers(m):
+    """Finite fp32 numbers up to the type's largest, in x and in the weights: the products are at most half as large."""
+    k, n = 100, 96
+    top = torch.tensor([LARGEST, -LARGEST, 3.4020e38, -3.4020e38, 3.4019e38, 3.3e38, 1e38], device=DEV)
+    i = torch.arange(m, device=DEV)
+    x = torch.zeros(m, k, device=DEV)
+    x[i, i % k] = top[i % len(top)]
+    w = torch.tensor([0.5, -0.5, 2.0 ** -30, 1 / 3, -0.3], device=DEV)[torch.arange(n * k, device=DEV) % 5].view(n, k)
+    want, bound = linear64(x, w)
+    check_close(_linear(x, w), want, bound)
+    x = torch.tensor([0.5, -0.25, 0.3], device=DEV)[torch.arange(m, device=DEV) % 3][:, None] * (torch.arange(k, device=DEV) == 7)
+    w = top[torch.arange(n * k, device=DEV) % len(top)].view(n, k)
+    want, bound = linear64(x, w)
+    check_close(_linear(x, w), want, bound)

@@ -374,3 +374,31 @@ def test_layer_few_tokens(dtype, act, k):
         assert layer.verify()["pass"]
     finally:
         layer.close()
+
+
+@pytest.mark.parametrize("where", ["x", "w1", "w2"])
+@pytest.mark.parametrize("T", [1, 64])
+def test_largest_numbers(T, where):
+    """Finite fp32 numbers up to the type's largest in the tokens, the weights and the activations, by rows and on the
+    tensor cores: what they are multiplied by keeps each result far below it."""
+    E, D, F, O = 4, 512, 1200, 512
+    top = torch.finfo(FP32).max
+    a = _make(T, D, E, F, O, "relu", FP32, seed=4)
+    a["router_w"].zero_()
+    a["router_b"] = torch.randn(E, device=DEV, generator=torch.Generator(DEV).manual_seed(5))
+    a["x"] = a["x"].sign() * (torch.arange(D, device=DEV) == 3)
+    if where == "x":          # z = top * w1
+        a["x"] *= top
+        a["w1"] *= 2.0 ** -100
+    elif where == "w1":       # z = +-top, and so are the activations
+        a["w1"] = a["w1"].sign() * top
+        a["w2"] *= 2.0 ** -100
+    else:
+        a["w1"] *= 2.0 ** -40
+        a["w2"] = a["w2"].sign() * top
+        a["w2"][:, :, F // 2:] = 0
+        a["w2"][:, :, ::3] = 0
+    out, ids, gates = _moe(**a, top_k=2, act="relu", gate_mode="topk_softmax")
+    want, bound, rid, rg, _, _ = moe64(**a, top_k=2, act="relu", gate_mode="topk_softmax")
+    assert torch.equal(ids.cpu(), rid) and out.isfinite().all()
+    check_close(out, want, bound)
