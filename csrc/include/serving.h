@@ -73,7 +73,7 @@ struct FewExpertPlan {
   long long bytes() const { return packed_bytes + a_bytes + w1_bytes + w2_bytes; }
 };
 
-FewExpertPlan plan_few_experts(const FewExpertParams& p);
+FewExpertPlan plan_few_experts(const FewExpertParams& p, int sms);
 void launch_few(const FewRouteParams& r, const FewExpertParams& p, const FewExpertPlan& plan, void* workspace, cudaStream_t s);
 
 // `groups` blocks of rows of K elements, `group` apart, to one block of rows that start on 16 bytes, `packed` apart.
@@ -112,7 +112,7 @@ struct LinearPlan {
   long long bytes() const { return x_bytes + w_bytes; }
 };
 
-LinearPlan plan_linear(const LinearParams& p);
+LinearPlan plan_linear(const LinearParams& p, int sms);
 void launch_linear(const LinearParams& p, const LinearPlan& plan, void* workspace, cudaStream_t s);
 
 int serving_sm_count();   // of the current device

@@ -71,9 +71,9 @@ static long long up256(long long v) { return (v + 255) / 256 * 256; }
 //   vector     very few rows, see below
 // So 4096 x 4096 takes (rows, 128, 256) for 64 rows 11.9, 16.2, 24.1, for 384 rows 26.1, 17.5, 24.8, for 2048 rows 117, 60,
 // 50; 1024 x 4096 fp32 for 64 rows 13.4, 27.2, for 384 rows 60, 31.
-LinearPlan plan_linear(const LinearParams& p) {
+LinearPlan plan_linear(const LinearParams& p, int sms) {
   LinearPlan r{};
-  const int eb = p.bf16 ? 2 : 4, sms = serving_sm_count();
+  const int eb = p.bf16 ? 2 : 4;
   const bool glu = p.act == (int)Act::kSwiGLU;
   const long long wrows = glu ? 2ll * p.N : p.N;
   auto aligned = [&](const void* base, long long rows, long long stride) {

@@ -454,16 +454,16 @@ constexpr int kFewOwnExperts = 16, kFewOwnBytes = 65536;
 constexpr double kFewOddRate = 4.5e6, kFewPackRate = 5e6;
 constexpr int kFewJoinRoom = 24 * 1024;                // of the join's CTA beside it
 
-FewExpertPlan plan_few_experts(const FewExpertParams& p) {
+FewExpertPlan plan_few_experts(const FewExpertParams& p, int sms) {
   FewExpertPlan r{};
   const int eb = p.bf16 ? 2 : 4, parts = p.bf16 ? 1 : 2;
   auto aligned = [&](const void* base, long long row, long long expert) {
     return ((uintptr_t)base & 15) == 0 && (row * eb) % 16 == 0 && (p.E == 1 || (expert * eb) % 16 == 0);
   };
   const int n1 = (p.act == (int)Act::kSwiGLU ? 2 : 1) * p.F;
-  // TMA reads rows that start on 16 bytes
+  // TMA reads rows that start on 16 bytes and do not overlap, of experts that lie apart
   const bool rows16 = aligned(p.w1, p.w1_stride, p.w1_estride) && aligned(p.w2, p.w2_stride, p.w2_estride) &&
-                      p.w1_stride > 0 && p.w2_stride > 0 && (p.E == 1 || (p.w1_estride > 0 && p.w2_estride > 0));
+                      p.w1_stride >= p.D && p.w2_stride >= p.F && (p.E == 1 || (p.w1_estride > 0 && p.w2_estride > 0));
   const int pairs = p.T * p.k;
   const double expert = (double)eb * ((double)n1 * p.D + (double)p.O * p.F), bytes = pairs * expert;
   if (rows16) {
@@ -492,11 +492,11 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p) {
     if (!fits(p.T)) r.slice = std::min(p.T, fits(32) ? 32 : 16);
   }
   const int T = r.slice;
-  r.grid = std::min(serving_sm_count(), kFewJoinItems - 2 * kFewTopK);
+  r.grid = std::min(sms, kFewJoinItems - 2 * kFewTopK);
   r.Op = (p.O + 127) / 128 * 128;
   r.Tp = (T + 15) / 16 * 16;
   const int UE = (p.F + 15) / 16, ups = 128 / eb / 16;
-  r.pack = !p.bf16 || !aligned(p.x, p.T > 1 ? p.x_stride : 0, 0);
+  r.pack = !p.bf16 || !aligned(p.x, p.T > 1 ? p.x_stride : 0, 0) || (p.T > 1 && p.x_stride < p.D);   // tokens that are one, expanded
   r.packed_stride = (p.D + 7) / 8 * 8;
   if (r.pack) r.packed_bytes = up256((long long)parts * r.Tp * r.packed_stride * eb);
   // An expert's tokens times the CTAs that share it, over all experts: n experts have at most min(T k, n T) tokens

@@ -111,6 +111,50 @@ torch::Tensor check_out(const char* op, const OptTensor& out, const OptTensor& r
   return *out;
 }
 
+// What the plan of a call goes by: shapes, types, addresses and strides.
+raiccl::FewExpertParams few_expert_params(const torch::Tensor& x, const torch::Tensor& w1, const torch::Tensor& w2, int64_t top_k,
+                                          int64_t act) {
+  raiccl::FewExpertParams e{};
+  e.x = x.data_ptr();
+  e.x_stride = x.stride(0);
+  e.w1 = w1.data_ptr();
+  e.w1_estride = w1.stride(0);
+  e.w1_stride = w1.stride(1);
+  e.w2 = w2.data_ptr();
+  e.w2_estride = w2.stride(0);
+  e.w2_stride = w2.stride(1);
+  e.T = (int)x.size(0);
+  e.D = (int)x.size(1);
+  e.E = (int)w1.size(0);
+  e.k = (int)top_k;
+  e.F = (int)w2.size(2);
+  e.O = (int)w2.size(1);
+  e.act = (int)act;
+  e.bf16 = x.scalar_type() == torch::kBFloat16;
+  return e;
+}
+
+raiccl::LinearParams linear_params(const torch::Tensor& x, const torch::Tensor& weight, int64_t act, const OptTensor& residual,
+                                   void* out, int64_t out_stride, torch::ScalarType out_type) {
+  raiccl::LinearParams p{};
+  p.x = x.data_ptr();
+  p.x_stride = x.stride(0);
+  p.w = weight.data_ptr();
+  p.w_stride = weight.stride(0);
+  p.residual = residual ? residual->data_ptr() : nullptr;
+  p.res_stride = residual ? residual->stride(0) : 0;
+  p.out = out;
+  p.out_stride = out_stride;
+  p.M = x.size(0);
+  p.N = (int)(act == (int64_t)raiccl::Act::kSwiGLU ? weight.size(0) / 2 : weight.size(0));
+  p.K = (int)x.size(1);
+  p.act = (int)act;
+  p.bf16 = x.scalar_type() == torch::kBFloat16;
+  p.out_bf16 = out_type == torch::kBFloat16;
+  p.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
+  return p;
+}
+
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
     torch::Tensor x, torch::Tensor router_w, torch::Tensor w1, torch::Tensor w2, int64_t top_k, int64_t act,
     int64_t gate_mode, OptTensor router_b, OptTensor b1, OptTensor b2, OptTensor block_mask, OptTensor residual,
@@ -179,15 +223,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   r.vec = (D * eb) % 16 == 0 && rows16(x) && rows16(router_w);
   r.ids = ids.data_ptr<int>();
   r.gates = gates.data_ptr<float>();
-  raiccl::FewExpertParams e{};
-  e.x = x.data_ptr();
-  e.x_stride = x.stride(0);
-  e.w1 = w1.data_ptr();
-  e.w1_estride = w1.stride(0);
-  e.w1_stride = w1.stride(1);
-  e.w2 = w2.data_ptr();
-  e.w2_estride = w2.stride(0);
-  e.w2_stride = w2.stride(1);
+  raiccl::FewExpertParams e = few_expert_params(x, w1, w2, top_k, act);
   e.b1 = b1 ? b1->data_ptr<float>() : nullptr;
   e.b2 = b2 ? b2->data_ptr<float>() : nullptr;
   e.residual = residual ? residual->data_ptr() : nullptr;
@@ -196,17 +232,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   e.out_stride = res.stride(0);
   e.ids = r.ids;
   e.gates = r.gates;
-  e.T = r.T;
-  e.D = r.D;
-  e.E = r.E;
-  e.k = r.k;
-  e.F = (int)F;
-  e.O = (int)O;
-  e.act = (int)act;
-  e.bf16 = bf16;
   e.out_bf16 = res.scalar_type() == torch::kBFloat16;
   e.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
-  const raiccl::FewExpertPlan plan = raiccl::plan_few_experts(e);
+  const raiccl::FewExpertPlan plan = raiccl::plan_few_experts(e, raiccl::serving_sm_count());
   const c10::DataPtr ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)plan.bytes());   // of the current stream
   char* base = (char*)ws.get();
   r.packed = plan.pack ? base : nullptr;
@@ -237,29 +265,45 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   torch::Tensor res = check_out(op, out, residual, x, out_dtype, M, N, {&x, &weight}, {&bias});
   c10::cuda::CUDAGuard guard(dev);
   if (M == 0 || N == 0) return res;
-  raiccl::LinearParams p{};
-  p.x = x.data_ptr();
-  p.x_stride = x.stride(0);
-  p.w = weight.data_ptr();
-  p.w_stride = weight.stride(0);
+  raiccl::LinearParams p = linear_params(x, weight, act, residual, res.data_ptr(), res.stride(0), res.scalar_type());
   p.bias = bias ? bias->data_ptr<float>() : nullptr;
-  p.residual = residual ? residual->data_ptr() : nullptr;
-  p.res_stride = residual ? residual->stride(0) : 0;
-  p.out = res.data_ptr();
-  p.out_stride = res.stride(0);
-  p.M = M;
-  p.N = (int)N;
-  p.K = (int)K;
-  p.act = (int)act;
-  p.bf16 = x.scalar_type() == torch::kBFloat16;
-  p.out_bf16 = res.scalar_type() == torch::kBFloat16;
-  p.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
-  const raiccl::LinearPlan plan = raiccl::plan_linear(p);
+  const raiccl::LinearPlan plan = raiccl::plan_linear(p, raiccl::serving_sm_count());
   c10::DataPtr ws;   // of the current stream
   if (plan.bytes() > 0) ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)plan.bytes());
   raiccl::launch_linear(p, plan, ws.get(), at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return res;
+}
+
+// Which kernels a call takes on a device of `sms` SMs: for tests, which name the path that they are about.  Launches
+// nothing; the tensors may lie on any device.
+py::dict moe_few_plan(torch::Tensor x, torch::Tensor w1, torch::Tensor w2, int64_t top_k, int64_t act, int64_t sms) {
+  const raiccl::FewExpertPlan plan = raiccl::plan_few_experts(few_expert_params(x, w1, w2, top_k, act), (int)sms);
+  py::dict d;
+  d["path"] = plan.tensor ? "tensor" : "rows";
+  d["vec"] = plan.vec != 0;
+  d["routes"] = plan.route != 0;
+  d["pack_x"] = plan.pack != 0;
+  d["pack_w"] = plan.pack_w != 0;
+  d["slice"] = plan.slice;
+  d["bytes"] = plan.bytes();
+  return d;
+}
+
+py::dict linear_plan(torch::Tensor x, torch::Tensor weight, int64_t act, OptTensor residual, OptTensor out, bool out_bf16,
+                     int64_t sms) {
+  raiccl::LinearParams p = linear_params(x, weight, act, residual, out ? out->data_ptr() : nullptr, out ? out->stride(0) : 0,
+                                         out_bf16 ? torch::kBFloat16 : torch::kFloat32);
+  if (!out) p.out_stride = p.N;
+  const raiccl::LinearPlan plan = raiccl::plan_linear(p, (int)sms);
+  py::dict d;
+  d["kernel"] = plan.vector ? "vector" : plan.dense ? "dense" : "rows";
+  d["tile"] = plan.dense;
+  d["ranks"] = plan.vector || plan.dense ? 0 : plan.ranks;
+  d["pack_x"] = plan.pack_x != 0;
+  d["pack_w"] = plan.pack_w != 0;
+  d["bytes"] = plan.bytes();
+  return d;
 }
 
 // The device's record of the first wait that ran out in a serving operator
@@ -282,6 +326,9 @@ void register_serving(py::module_& m) {
   m.def("moe_few_tokens", &moe_few_tokens, py::arg("x"), py::arg("router_w"), py::arg("w1"), py::arg("w2"), py::arg("top_k"),
         py::arg("act"), py::arg("gate_mode"), py::arg("router_b"), py::arg("b1"), py::arg("b2"), py::arg("block_mask"),
         py::arg("residual"), py::arg("out"), py::arg("out_dtype"));
+  m.def("moe_few_plan", &moe_few_plan, py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("top_k"), py::arg("act"), py::arg("sms"));
+  m.def("linear_plan", &linear_plan, py::arg("x"), py::arg("weight"), py::arg("act"), py::arg("residual"), py::arg("out"),
+        py::arg("out_bf16"), py::arg("sms"));
   m.def("serving_status", &serving_status, py::arg("device"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("residual"),
         py::arg("out"), py::arg("out_dtype"));

@@ -16,6 +16,12 @@ def _moe(*a, **k):
     return moe_few_tokens(*a, **k)
 
 
+def _plan(a, k, act):
+    from revealaiccl_b200.ops._native import kernels
+    from revealaiccl_b200.ops.grouped_gemm import ACT_IDS
+    return kernels().moe_few_plan(a["x"], a["w1"], a["w2"], k, ACT_IDS[act], torch.cuda.get_device_properties(DEV).multi_processor_count)
+
+
 def _make(T, D, E, F, O, act, dtype, seed=0, bias=False):
     g = torch.Generator(DEV).manual_seed(seed)
 
@@ -402,3 +408,18 @@ def test_largest_numbers(T, where):
     want, bound, rid, rg, _, _ = moe64(**a, top_k=2, act="relu", gate_mode="topk_softmax")
     assert torch.equal(ids.cpu(), rid) and out.isfinite().all()
     check_close(out, want, bound)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("tensor", [False, True], ids=["rows", "tensor"])
+def test_tokens_that_share_their_rows(dtype, tensor):
+    """Tokens that are one row expanded, or windows that overlap."""
+    E, D, O, T = 6, 512, 512, 9
+    F = 10000 if tensor else 96
+    a = _make(1, D, E, F, O, "swiglu", dtype, seed=6)
+    path = _plan(dict(a, x=a["x"].expand(T, D)), 2, "swiglu")
+    assert path["path"] == ("tensor" if tensor else "rows") and path["pack_x"] == tensor
+    out, ids, _ = _check(dict(a, x=a["x"].expand(T, D)), 2, "swiglu", "softmax")
+    assert (out == out[:1]).all() and (ids == ids[:1]).all()
+    long = torch.randn(T * 64 + D, device=DEV, generator=torch.Generator(DEV).manual_seed(7)).to(dtype)
+    _check(dict(a, x=long.as_strided((T, D), (64, 1))), 2, "swiglu", "softmax")
