@@ -5,6 +5,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -62,6 +63,8 @@ void check_input(const char* op, const char* name, const torch::Tensor& t, const
   TORCH_CHECK_VALUE(t.device() == dev, op, ": ", name, " must be on ", dev.str(), ", not on ", t.device().str());
   TORCH_CHECK(!(t.requires_grad() && c10::GradMode::is_enabled()), op, ": ", name,
               " requires a gradient, but the operator has no backward; call it under torch.no_grad()");
+  TORCH_CHECK(!(t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), op, ": ", name,
+              " carries a forward-mode tangent, but the operator has no derivative; take the primal of it");
 }
 
 void check_cuda(const char* op, const torch::Device& dev) {

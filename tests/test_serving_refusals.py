@@ -108,3 +108,20 @@ def test_out_apart_from_biases_and_mask():
         _linear(bias=buf[4:12], out=buf[:24].view(3, 8), out_dtype=torch.float32)
     with pytest.raises(ValueError, match="shares memory with an input"):
         _moe(router_b=buf[28:32], out=buf[:30].view(3, 10), out_dtype=torch.float32)
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        x = fwd.make_dual(torch.zeros(3, 16), torch.ones(3, 16))
+        with pytest.raises(RuntimeError, match="no derivative"):
+            _linear(x=x, weight=torch.zeros(8, 16))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no derivative"):
+            _linear(x=x, weight=torch.zeros(8, 16))
+        with pytest.raises(RuntimeError, match="no derivative"):
+            _linear(weight=torch.zeros(8, 16), x=torch.zeros(3, 16), residual=fwd.make_dual(torch.zeros(3, 8), torch.ones(3, 8)))
+        w2 = torch.zeros(4, 10, 12)
+        with pytest.raises(RuntimeError, match="no derivative"):
+            _moe(x=torch.zeros(3, 16), router_w=torch.zeros(4, 16), w1=torch.zeros(4, 24, 16), w2=fwd.make_dual(w2, w2 + 1))
+        with pytest.raises(ValueError, match="CUDA device"):
+            _linear(x=fwd.unpack_dual(x).primal, weight=torch.zeros(8, 16))
