@@ -158,6 +158,11 @@ raiccl::LinearParams linear_params(const torch::Tensor& x, const torch::Tensor& 
   return p;
 }
 
+// A given out was written: an operation that saved it for its backward pass has to notice.
+void written(const OptTensor& out) {
+  if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
+
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
     torch::Tensor x, torch::Tensor router_w, torch::Tensor w1, torch::Tensor w2, int64_t top_k, int64_t act,
     int64_t gate_mode, OptTensor router_b, OptTensor b1, OptTensor b2, OptTensor block_mask, OptTensor residual,
@@ -245,6 +250,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
   r.packed_rows = plan.Tp;
   raiccl::launch_few(r, e, plan, base, stream);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  written(out);
   return {res, ids, gates};
 }
 
@@ -275,6 +281,7 @@ torch::Tensor linear(torch::Tensor x, torch::Tensor weight, OptTensor bias, int6
   if (plan.bytes() > 0) ws = c10::cuda::CUDACachingAllocator::get()->allocate((size_t)plan.bytes());
   raiccl::launch_linear(p, plan, ws.get(), at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  written(out);
   return res;
 }
 

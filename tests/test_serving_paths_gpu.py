@@ -224,3 +224,25 @@ def test_wide_fp32_layers(T, D, E, k, act):
     want, _, _, _, _, _ = moe64(**a, top_k=k, act=act, gate_mode="none", block_mask=mask)
     got, _, _ = _moe(**a, top_k=k, act=act, gate_mode="none", block_mask=mask)
     check_norm(got, want, 4 * PARTS + U * (D ** 0.5 + a["w2"].shape[2] ** 0.5 + 16 + 48))
+
+
+# ---------------------------------------------------------------------------- both
+
+def test_writing_to_out_is_seen_by_autograd():
+    """A tensor that an operation saved for its backward pass, then given as out: that pass has to fail, not use what was written."""
+    x, w, _, _ = _make_linear(3, 64, 32, "none", FP32, False, False)
+    a = _make(3, 64, 4, 32, 32, "relu", FP32)
+    for write in (lambda out: _linear(x, w, out=out), lambda out: _moe(**a, top_k=2, act="relu", out=out)):
+        scale = torch.ones(3, 32, device=DEV, requires_grad=True)
+        saved = torch.randn(3, 32, device=DEV)
+        before = saved._version
+        (scale * saved).sum().backward()
+        y = (scale * saved).sum()
+        write(saved)
+        assert saved._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with torch.inference_mode():
+            out = torch.empty(3, 32, device=DEV)
+            write(out)
+        write(out)   # an inference tensor has no counter
