@@ -57,6 +57,18 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
   return x.first < y.second && y.first < x.second;
 }
 
+// Behind a shape there may be no numbers to read: a sparse layout, a lazy zero or
+// negation, or a storage that was freed (sharded parameters between their uses).
+void check_memory(const char* op, const char* name, const torch::Tensor& t) {
+  TORCH_CHECK_VALUE(t.layout() == c10::kStrided && !t.is_neg() && !t._is_zerotensor(), op, ": ", name,
+                    " must be a dense tensor, without a pending negation or zero");
+  if (t.numel() == 0 || !t.has_storage()) return;   // without one, data_ptr raises
+  int64_t last = t.storage_offset();
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  TORCH_CHECK_VALUE((int64_t)t.storage().nbytes() >= (last + 1) * (int64_t)t.element_size(), op, ": ", name,
+                    " reaches behind its storage, which holds ", text((int64_t)t.storage().nbytes()), " bytes");
+}
+
 // Every tensor of a call lies on the CUDA device of x; checked behind the
 // shapes, types and strides, whose refusals need no device.
 void check_input(const char* op, const char* name, const torch::Tensor& t, const torch::Device& dev) {
@@ -65,6 +77,7 @@ void check_input(const char* op, const char* name, const torch::Tensor& t, const
               " requires a gradient, but the operator has no backward; call it under torch.no_grad()");
   TORCH_CHECK(!(t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), op, ": ", name,
               " carries a forward-mode tangent, but the operator has no derivative; take the primal of it");
+  check_memory(op, name, t);
 }
 
 void check_cuda(const char* op, const torch::Device& dev) {

@@ -125,3 +125,33 @@ def test_tangents_are_refused():
             _moe(x=torch.zeros(3, 16), router_w=torch.zeros(4, 16), w1=torch.zeros(4, 24, 16), w2=fwd.make_dual(w2, w2 + 1))
         with pytest.raises(ValueError, match="CUDA device"):
             _linear(x=fwd.unpack_dual(x).primal, weight=torch.zeros(8, 16))
+
+
+def _freed(*shape, dtype=BF16):
+    t = torch.zeros(*shape, dtype=dtype)
+    t.untyped_storage().resize_(0)
+    return t
+
+
+@pytest.mark.parametrize("t", [_freed(3, 16), torch.zeros(3, 16, dtype=BF16).to_sparse(), torch._neg_view(torch.zeros(3, 16, dtype=BF16)),
+                               torch._efficientzerotensor((3, 16), dtype=BF16)], ids=["freed", "sparse", "neg", "zero"])
+def test_tensors_without_their_numbers_are_refused(t):
+    with pytest.raises(ValueError, match="x (reaches behind its storage|must be a dense tensor)"):
+        _linear(x=t)
+    with pytest.raises(ValueError, match="x (reaches behind its storage|must be a dense tensor)"):
+        _moe(x=t)
+
+
+def test_freed_storages_are_refused():
+    for name, shape, dtype in (("weight", (8, 16), BF16), ("bias", (8,), torch.float32), ("residual", (3, 8), BF16), ("out", (3, 8), BF16)):
+        with pytest.raises(ValueError, match=f"{name} reaches behind its storage"):
+            _linear(**{name: _freed(*shape, dtype=dtype)})
+    for name, shape, dtype in (("router_w", (4, 16), BF16), ("w1", (4, 24, 16), BF16), ("w2", (4, 10, 12), BF16),
+                               ("router_b", (4,), torch.float32), ("b1", (4, 24), torch.float32), ("b2", (4, 10), torch.float32),
+                               ("block_mask", (3, 4), torch.bool), ("residual", (3, 10), BF16), ("out", (3, 10), BF16)):
+        with pytest.raises(ValueError, match=f"{name} reaches behind its storage"):
+            _moe(**{name: _freed(*shape, dtype=dtype)})
+    part = torch.zeros(6, 16, dtype=BF16)[3:]
+    part.untyped_storage().resize_(100)
+    with pytest.raises(ValueError, match="x reaches behind its storage, which holds 100 bytes"):
+        _linear(x=part)
