@@ -197,7 +197,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
   if (warp == 0) {
     // ---------------------------------------------------------------- loads, both CTAs
     if (elect_one_sync()) {
-      int stage = 0;
+      int stage = 0, filled = 0;
       uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; ok && t < tiles; t += npairs) {
@@ -215,9 +215,14 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
             tma_load_3d_pair(s + part * C::X_BYTES, &tx, lead, kb * C::BK, xrow, part);
             tma_load_3d_pair(s + C::PARTS * C::X_BYTES + part * C::W_BYTES, &tw, lead, kb * C::BK, wrow, part);
           }
+          ++filled;
           if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
       }
+      // Both CTAs' copies count on the first one's barriers, and the pair leaves together.  Where one thread gave up before
+      // the other, the second CTA may have filled a stage more than the first knows of: that one gets a millisecond.
+      if (rank == 0) await_loads(full, C::STAGES, stage, phase, filled, status, kDenseKernelId, kDenseWaitNs);
+      if (!ok) serving_hold(1000000ull);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products, first CTA

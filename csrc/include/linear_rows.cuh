@@ -104,7 +104,8 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     if (elect_one_sync()) {
-      for (int i = 0; i < count; ++i, advance()) {
+      int i = 0;
+      for (; i < count; ++i, advance()) {
         if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
         uint8_t* w = smem + stage * SB;
         uint8_t* x = w + kRowsPack * kRowsTile;
@@ -117,6 +118,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           tma_load_2d(x, &tx, &full[stage], k, (int)m0);
         }
       }
+      await_loads(full, S, stage, phase, i, status, kRowsKernelId, kServingWaitNs);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products

@@ -392,6 +392,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       // weights are read once: they leave the rest of L2 (code, router, tokens, parts) alone
       const uint64_t once = l2_evict_first();
       bool ok = true;
+      int filled = 0;
       while (ok) {
         FewWalk again = walk;
         int off = 0, runs = 0;
@@ -418,6 +419,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
                 tma_load_2d(x, &tx, &full[stage], d, 0);
               }
               advance();
+              ++filled;
             }
           }
         }
@@ -435,6 +437,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
                 mbar_arrive_expect_tx(&full[stage], kFewTile);
                 tma_load_3d_hint(smem + stage * SB, &t2, &full[stage], r.f0 + s * C::BK, (i0 + i) * 128, r.expert, once);
                 advance();
+                ++filled;
               }
             for (int i = 0; ok && tail && i < nt; i += share) {
               const int n = nt - i < share ? nt - i : share;
@@ -445,10 +448,12 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
                 for (int u = 0; u < tail; ++u, w += 128 * C::TAIL)
                   tma_load_3d_hint(w, &t2u, &full[stage], r.f0 + slices * C::BK + u * 16, (i0 + i + m) * 128, r.expert, once);
               advance();
+              ++filled;
             }
           }
         }
       }
+      await_loads(full, S, stage, phase, filled, status, kFewKernelId, kFewWaitNs);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products

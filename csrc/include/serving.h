@@ -17,6 +17,17 @@ constexpr int kFewTokens = 64;     // tokens of one call at most: an expert's to
 constexpr int kFewExperts = 255;   // experts at most (the routing key's byte for the expert)
 constexpr int kFewTopK = 8;
 
+// A ring of S stages is filled in turn, the phase of its barriers changes with
+// every round.  From the stage and phase of the next fill back to those of the
+// fill before it.
+__host__ __device__ inline void fill_before(int S, int& stage, uint32_t& phase) {
+  if (stage == 0) {
+    stage = S;
+    phase ^= 1u;
+  }
+  --stage;
+}
+
 // Routing of T tokens.  Element strides; mask_stride 0 for one mask of all tokens.
 struct FewRouteParams {
   const void* x;          // [T, D]

@@ -6,6 +6,7 @@
 #include <cstdint>
 
 #include "sm100_ptx.cuh"
+#include "serving.h"
 #include "types.h"
 
 namespace raiccl {
@@ -43,6 +44,25 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, D
     }
   }
   return __all_sync(0xffffffffu, ok);
+}
+
+// Lets so much time pass.
+__device__ __forceinline__ void serving_hold(uint64_t ns) {
+  const uint64_t start = globaltimer_ns();
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 20) && globaltimer_ns() - start < ns; ++i) __nanosleep(1000u);
+}
+
+// A loading thread's last step, whether its loop ended or gave up: the copies
+// that it has issued land before its CTA leaves and another one gets the shared
+// memory.  `filled` stages so far, the next one would be (stage, phase).  In a
+// call that went well all of them have landed or are about to.
+__device__ __forceinline__ void await_loads(uint64_t* full, int S, int stage, uint32_t phase, int filled, DeviceStatus* st, int kernel_id,
+                                            uint64_t limit_ns) {
+  for (int i = filled < S ? filled : S; i > 0; --i) {
+    fill_before(S, stage, phase);
+    if (!mbar_wait_bounded(&full[stage], phase, st, kernel_id, limit_ns)) return;
+  }
 }
 
 // Shared-memory descriptors by addition: the fields of umma_desc_k_sw128 (or

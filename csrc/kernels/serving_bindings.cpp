@@ -12,6 +12,8 @@
 
 #include <string>
 #include <tuple>
+#include <utility>
+#include <vector>
 
 #include "serving.h"
 
@@ -329,6 +331,18 @@ py::dict linear_plan(torch::Tensor x, torch::Tensor weight, int64_t act, OptTens
   return d;
 }
 
+// Stages and phases of the last fills of a ring of `stages`, newest first, after `filled` fills: what a loading thread waits for.
+std::vector<std::pair<int, int>> serving_last_fills(int64_t stages, int64_t filled) {
+  int stage = (int)(filled % stages);
+  uint32_t phase = (uint32_t)(filled / stages & 1);
+  std::vector<std::pair<int, int>> v;
+  for (int64_t i = std::min(stages, filled); i > 0; --i) {
+    raiccl::fill_before((int)stages, stage, phase);
+    v.emplace_back(stage, (int)phase);
+  }
+  return v;
+}
+
 // The device's record of the first wait that ran out in a serving operator
 // since the last call (eight words, DeviceStatus); waits for the device and
 // clears the record.
@@ -352,6 +366,7 @@ void register_serving(py::module_& m) {
   m.def("moe_few_plan", &moe_few_plan, py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("top_k"), py::arg("act"), py::arg("sms"));
   m.def("linear_plan", &linear_plan, py::arg("x"), py::arg("weight"), py::arg("act"), py::arg("residual"), py::arg("out"),
         py::arg("out_bf16"), py::arg("sms"));
+  m.def("serving_last_fills", &serving_last_fills, py::arg("stages"), py::arg("filled"));
   m.def("serving_status", &serving_status, py::arg("device"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("residual"),
         py::arg("out"), py::arg("out_dtype"));

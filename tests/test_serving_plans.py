@@ -37,3 +37,19 @@ def test_rows_that_overlap_are_no_operand_of_copies(F, path):
                  (w1, _empty(E * O * F).as_strided((E, O, F), (O * 16, 16, 1)))):
         p = _few(_empty(8, D), a, b)
         assert (p["path"] == "rows" and not p["vec"]) or p["pack_w"]
+
+
+@pytest.mark.parametrize("stages", [2, 3, 4, 9, 12])
+def test_last_fills_of_a_ring(stages):
+    """What a loading thread waits for before its CTA leaves: the last fill of every stage that was filled."""
+    stage, phase, fills = 0, 0, []
+    for filled in range(5 * stages + 2):
+        want = []
+        for s, f in reversed(fills):
+            if s not in [w[0] for w in want]:
+                want.append((s, f))
+        assert _native.kernels().serving_last_fills(stages, filled) == want
+        fills.append((stage, phase))
+        stage += 1
+        if stage == stages:
+            stage, phase = 0, phase ^ 1
