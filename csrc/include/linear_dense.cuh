@@ -206,7 +206,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
         const int xrow = mb * 256 + (int)rank * 128;
         const int wrow = GLU ? nb * W + (int)rank * l.N : nb * W + (int)rank * C::HALF;
         for (int kb = 0; kb < KB; ++kb) {
-          if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
+          if (!(ok = serving_wait(&empty[stage], phase ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * C::STAGE);
           const uint32_t lead = mapa_shared(smem_u32(&full[stage]), 0);
           uint8_t* s = smem + stage * C::STAGE;
@@ -236,15 +236,15 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
       for (int t = pair; ok && t < tiles; t += npairs, ++nth) {
         const int lb = nth & 1;
         const uint32_t dl = tmem + (2 + lb) * BN;
-        if (FP32 && !(ok = mbar_wait_bounded(&low_empty[lb], ((nth >> 1) & 1) ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
+        if (FP32 && !(ok = serving_wait(&low_empty[lb], ((nth >> 1) & 1) ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
         for (int k0 = 0; ok && k0 < KB; k0 += chain, ++iter) {
           const int steps = k0 + chain < KB ? chain : KB - k0;
           const int b = iter & 1;
-          if (!(ok = mbar_wait_bounded(&acc_empty[b], ((iter >> 1) & 1) ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
+          if (!(ok = serving_wait(&acc_empty[b], ((iter >> 1) & 1) ^ 1u, status, kDenseKernelId, kDenseWaitNs))) break;
           tc_fence_after_sync();
           const uint32_t d = tmem + b * BN;
           for (int kb = 0; kb < steps; ++kb) {
-            if (!(ok = mbar_wait_bounded(&full[stage], phase, status, kDenseKernelId, kDenseWaitNs))) break;
+            if (!(ok = serving_wait(&full[stage], phase, status, kDenseKernelId, kDenseWaitNs))) break;
             tc_fence_after_sync();
             const uint64_t dx = desc_at(row, smem_u32(smem + stage * C::STAGE)), dw = dx + C::PARTS * C::X_BYTES / 16;
 #pragma unroll
@@ -274,7 +274,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
         }
       }
       umma_commit_pair(mapa_shared(smem_u32(&drained), 0));
-      mbar_wait_bounded(&drained, 0, status, kDenseKernelId, kDenseWaitNs);
+      serving_wait(&drained, 0, status, kDenseKernelId, kDenseWaitNs);
     }
   } else {
     // ---------------------------------------------------------------- epilogue, both CTAs

@@ -106,7 +106,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
     if (elect_one_sync()) {
       int i = 0;
       for (; i < count; ++i, advance()) {
-        if (!mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
+        if (!serving_wait(&empty[stage], phase ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
         uint8_t* w = smem + stage * SB;
         uint8_t* x = w + kRowsPack * kRowsTile;
         const int n = steps - i * kRowsPack < kRowsPack ? steps - i * kRowsPack : kRowsPack;
@@ -130,9 +130,9 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       for (int i = 0; i < count; ++i, advance()) {
         if (FP32 && i % kRowsChain == 0) {
           const int c = i / kRowsChain;
-          if (!mbar_wait_bounded(&acc_empty[c & 1], ((c >> 1) & 1) ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
+          if (!serving_wait(&acc_empty[c & 1], ((c >> 1) & 1) ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
         }
-        if (!mbar_wait_bounded(&ready[stage], phase, status, kRowsKernelId, kServingWaitNs)) break;
+        if (!serving_wait(&ready[stage], phase, status, kRowsKernelId, kServingWaitNs)) break;
         tc_fence_after_sync();
         const uint32_t d = tmem + (FP32 ? (i / kRowsChain & 1) * 2 * p.Mp : 0);
         const uint32_t w = smem_u32(smem + stage * SB);

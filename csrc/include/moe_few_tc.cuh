@@ -400,7 +400,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           for (int u0 = 0; ok && u0 < r.units; u0 += TU) {
             const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu), f0 = r.f0 + u0 * 16;
             for (int kb = 0; kb < KB; kb += pack) {
-              if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+              if (!(ok = serving_wait(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
               uint8_t* w = smem + stage * SB;
               uint8_t* x = w + SB - pack * n1 * 128;
               const int n = KB - kb < pack ? KB - kb : pack;
@@ -433,7 +433,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
             for (int s = 0; ok && s < slices; ++s)
               for (int i = 0; i < nt; ++i) {
-                if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+                if (!(ok = serving_wait(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
                 mbar_arrive_expect_tx(&full[stage], kFewTile);
                 tma_load_3d_hint(smem + stage * SB, &t2, &full[stage], r.f0 + s * C::BK, (i0 + i) * 128, r.expert, once);
                 advance();
@@ -441,7 +441,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               }
             for (int i = 0; ok && tail && i < nt; i += share) {
               const int n = nt - i < share ? nt - i : share;
-              if (!(ok = mbar_wait_bounded(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+              if (!(ok = serving_wait(&empty[stage], phase ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
               mbar_arrive_expect_tx(&full[stage], n * tail * 128 * C::TAIL);
               uint8_t* w = smem + stage * SB;
               for (int m = 0; m < n; ++m)
@@ -484,12 +484,12 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
             const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu);
             const int g = i1 % acc.groups, j = i1 / acc.groups, b = j & (acc.nbuf - 1);
-            if (!(ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+            if (!(ok = serving_wait(&acc1_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
             uint32_t dc = tmem + acc.first(g, b);
             int at = 0;   // steps of the chain
             for (int kb = 0; kb < KB; kb += pack) {
-              if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+              if (!(ok = serving_wait(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
               tc_fence_after_sync();
               const uint32_t w = smem_u32(smem + stage * SB), x = w + SB - pack * n1 * 128, wl = smem_u32(low) + lo * kFewTile;
               const int n = KB - kb < pack ? KB - kb : pack;
@@ -511,7 +511,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         for (int g = 0; g < acc.groups; ++g)
           for (int b = 0; ok && b < acc.nbuf; ++b) {
             const int tiles = (i1 + acc.groups - 1 - g) / acc.groups, uses = (tiles + acc.nbuf - 1 - b) / acc.nbuf;
-            if (uses > 0) ok = mbar_wait_bounded(&acc1_empty[g * 2 + b], (uses - 1) & 1, status, kFewKernelId, kFewWaitNs);
+            if (uses > 0) ok = serving_wait(&acc1_empty[g * 2 + b], (uses - 1) & 1, status, kFewKernelId, kFewWaitNs);
           }
         tc_fence_after_sync();
         off = 0;
@@ -524,13 +524,13 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           for (int i0 = 0, g = 0; ok && i0 < nO; i0 += acc.tiles, g = acc.groups - 1 - g) {
             const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
             const int j = j2[g]++, b = j & (acc.nbuf - 1);
-            if (!(ok = mbar_wait_bounded(&acc2_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
+            if (!(ok = serving_wait(&acc2_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
             const uint32_t d = tmem + acc.second(g, b), dn = C::PARTS * r.np;
             const uint32_t h0 = smem_u32(hbuf) + r.h * 128;
             for (int s = 0; ok && s < slices; ++s)
               for (int i = 0; i < nt; ++i) {
-                if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+                if (!(ok = serving_wait(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
                 tc_fence_after_sync();
                 const uint64_t da = desc_at(wide_row, smem_u32(smem + stage * SB)), dl = desc_at(wide_row, smem_u32(low) + lo * kFewTile);
                 const uint64_t dh = desc_at(wide_row, h0 + s * hrow);
@@ -542,7 +542,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               }
             for (int i = 0; ok && tail && i < nt; i += share) {
               const int n = nt - i < share ? nt - i : share;
-              if (!(ok = mbar_wait_bounded(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
+              if (!(ok = serving_wait(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
               tc_fence_after_sync();
               constexpr int KS = C::TAIL / 32;   // 32-byte steps of a unit
               uint64_t da = desc_at(unit_row, smem_u32(smem + stage * SB)), dl = desc_at(unit_row, smem_u32(low) + lo * kFewTile);
@@ -562,7 +562,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       }
       // every product has finished before the accumulators are freed
       umma_commit(&drained);
-      mbar_wait_bounded(&drained, 0, status, kFewKernelId, kFewWaitNs);
+      serving_wait(&drained, 0, status, kFewKernelId, kFewWaitNs);
     }
   } else if (warp < 10) {
     // ---------------------------------------------------------------- epilogues

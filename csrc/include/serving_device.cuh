@@ -25,8 +25,24 @@ __device__ __forceinline__ bool mbar_try_wait_hint(uint64_t* bar, uint32_t parit
   return ok != 0;
 }
 
-// A wait of a whole warp, bounded like mbar_wait_bounded.  The lanes may leave
-// the loop apart, and the aligned instructions that follow (tcgen05.ld, cluster
+// A wait of one thread.  When `limit_ns` have passed it records that and gives
+// up.  Unlike mbar_wait_bounded it does not look at what others have recorded:
+// the record of a device stays until it is read, and the calls behind a failed
+// one must not end early for it.
+__device__ __forceinline__ bool serving_wait(uint64_t* bar, uint32_t parity, DeviceStatus* st, int kernel_id, uint64_t limit_ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = globaltimer_ns();
+  uint32_t polls = 0;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((++polls & 63u) == 0 && globaltimer_ns() - start > limit_ns) {
+      record_status(st, kTimeoutPipeline, kernel_id, (long long)parity, (long long)limit_ns);
+      return false;
+    }
+  }
+}
+
+// The same wait of a whole warp.  The lanes may leave the loop apart, and the aligned instructions that follow (tcgen05.ld, cluster
 // barriers) need the warp in one piece; all lanes return the same.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, DeviceStatus* st, int kernel_id, uint64_t limit_ns) {
   bool ok = mbar_try_wait_hint(bar, parity, 20000u);
@@ -35,12 +51,10 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, D
     uint32_t polls = 0;
 #pragma unroll 1
     while (!(ok = mbar_try_wait_hint(bar, parity, 20000u))) {
-      if ((++polls & 63u) != 0) continue;
-      if (globaltimer_ns() - start > limit_ns) {
+      if ((++polls & 63u) == 0 && globaltimer_ns() - start > limit_ns) {
         record_status(st, kTimeoutPipeline, kernel_id, (long long)parity, (long long)limit_ns);
         break;
       }
-      if (status_failed(st)) break;
     }
   }
   return __all_sync(0xffffffffu, ok);
@@ -61,7 +75,7 @@ __device__ __forceinline__ void await_loads(uint64_t* full, int S, int stage, ui
                                             uint64_t limit_ns) {
   for (int i = filled < S ? filled : S; i > 0; --i) {
     fill_before(S, stage, phase);
-    if (!mbar_wait_bounded(&full[stage], phase, st, kernel_id, limit_ns)) return;
+    if (!serving_wait(&full[stage], phase, st, kernel_id, limit_ns)) return;
   }
 }
 

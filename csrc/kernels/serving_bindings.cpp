@@ -331,6 +331,12 @@ py::dict linear_plan(torch::Tensor x, torch::Tensor weight, int64_t act, OptTens
   return d;
 }
 
+// Where the device's record lies.
+int64_t serving_status_address(int64_t device) {
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  return (int64_t)raiccl::serving_status();
+}
+
 // Stages and phases of the last fills of a ring of `stages`, newest first, after `filled` fills: what a loading thread waits for.
 std::vector<std::pair<int, int>> serving_last_fills(int64_t stages, int64_t filled) {
   int stage = (int)(filled % stages);
@@ -366,6 +372,7 @@ void register_serving(py::module_& m) {
   m.def("moe_few_plan", &moe_few_plan, py::arg("x"), py::arg("w1"), py::arg("w2"), py::arg("top_k"), py::arg("act"), py::arg("sms"));
   m.def("linear_plan", &linear_plan, py::arg("x"), py::arg("weight"), py::arg("act"), py::arg("residual"), py::arg("out"),
         py::arg("out_bf16"), py::arg("sms"));
+  m.def("serving_status_address", &serving_status_address, py::arg("device"));
   m.def("serving_last_fills", &serving_last_fills, py::arg("stages"), py::arg("filled"));
   m.def("serving_status", &serving_status, py::arg("device"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("residual"),

@@ -57,7 +57,8 @@ def check(status: torch.Tensor) -> None:
 def check_serving(device: torch.device | str | int | None = None) -> None:
     """Wait for ``device`` and raise if a bounded wait ran out in one of its
     ``linear`` / ``moe_few_tokens`` calls since the last check; the record is
-    cleared.  Until then the calls behind a failed one may give up early too."""
+    cleared.  The failed call's result is incomplete; the calls behind it are
+    not affected."""
     from ._native import kernels
 
     dev = torch.device("cuda" if device is None else device if not isinstance(device, int) else f"cuda:{device}")

@@ -246,3 +246,37 @@ def test_writing_to_out_is_seen_by_autograd():
             out = torch.empty(3, 32, device=DEV)
             write(out)
         write(out)   # an inference tensor has no counter
+
+
+def test_a_record_is_raised_once_and_leaves_other_calls_alone():
+    """The record of a wait that ran out, written here by the host: the next check raises it with its fields, the one after
+    passes, and calls made while it stands, with long waits in them, give the same bits as before."""
+    from revealaiccl_b200.ops import status
+    from revealaiccl_b200.ops._native import kernels
+    from revealaiccl_b200.parallel.peer import device_view
+
+    index = torch.cuda.current_device()
+    record = device_view(kernels().serving_status_address(index), (status.STATUS_WORDS,), torch.int32, torch.device(DEV, index))
+    fields = torch.tensor([1, 620, 17, 33, 5, 0, 2_000_000_000, 0], dtype=torch.int32, device=DEV)
+    calls = []
+    for m, k, n, act, dtype in ((64, 14336, 4096, "swiglu", BF16), (2048, 8192, 4096, "none", BF16), (64, 8192, 2048, "none", FP32),
+                                (1024, 4096, 4096, "gelu", FP32)):
+        x, w, b, r = _make_linear(m, k, n, act, dtype, True, True)
+        calls.append(lambda x=x, w=w, b=b, r=r, act=act, **kw: _linear(x, w, b, act=act, residual=r, **kw))
+    for dtype in (BF16, FP32):
+        a = _make(40, 1024, 8, 6000, 1024, "swiglu", dtype)
+        assert _plan(a, 2, "swiglu")["path"] == "tensor"
+        calls.append(lambda a=a, **kw: _moe(**a, top_k=2, **kw)[0])
+    want = [c() for c in calls]
+    status.check_serving()
+    for c, v in zip(calls, want):
+        record.copy_(fields)
+        assert torch.equal(c(), v)
+        with pytest.raises(status.DeviceStatusError, match="pipeline mbarrier wait timed out") as e:
+            c(check=True)
+        assert e.value.record == {"code": 1, "kernel_id": 620, "block": 17, "thread": 33, "index": 5, "bound": 2_000_000_000}
+        assert torch.equal(c(check=True), v) and (record == 0).all()
+        record.copy_(fields)
+        with pytest.raises(status.DeviceStatusError):
+            status.check_serving(index)
+        status.check_serving()
