@@ -163,6 +163,16 @@ __device__ __forceinline__ void split_tf32(float v, float& hi, float& lo) {
   lo = fabsf(v) == INFINITY ? 0.f : v - hi;
 }
 
+// fp32 as two bf16 numbers: hi is v rounded to 8 significant bits, or cut where
+// rounding would give an infinity, lo what is left, rounded (2^-16 of v is lost
+// at most).
+__device__ __forceinline__ void split_bf16(float v, __nv_bfloat16& hi, __nv_bfloat16& lo) {
+  const float r = __bfloat162float(__float2bfloat16_rn(v));
+  const float h = fabsf(r) == INFINITY ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : r;
+  hi = __float2bfloat16_rn(h);
+  lo = __float2bfloat16_rn(fabsf(v) == INFINITY ? 0.f : v - h);
+}
+
 // What the tensor core does not read of an fp32 number, which it takes by its
 // upper 19 bits: v less those, 13 bits rounded to 11 (2^-22 of v is lost at most).
 // Numbers behind the last one of 22 bits, infinities too, count as that one, so

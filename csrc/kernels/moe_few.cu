@@ -502,16 +502,19 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p, int sms) {
   // An expert's tokens times the CTAs that share it, over all experts: n experts have at most min(T k, n T) tokens
   // and (grid / n + 2) CTAs each, so T (grid + 2 k) rows at most, whatever n is.
   r.a_bytes = up256((long long)T * (r.grid + 2 * p.k) * r.Op * 4);
-  // Activations of the longest range of a CTA, if that leaves four stages; else the range is worked off in pieces, which
-  // costs a sum in memory each.  The rest holds stages.
+  // Activations of the longest range of a CTA (bf16: for an expert of four times the average tokens), if that leaves four
+  // stages; where there are more the range is worked off in pieces, which costs a sum in memory each.  The rest holds stages (64
+  // experts top-6, 37 tokens: 188 us with seven, 205 with the four that room for all tokens on one expert leaves).
   const int sb = p.bf16 ? FewTc<false>::stage_bytes(r.Tp) : FewTc<true>::stage_bytes(r.Tp);
   // Up to 16 tokens the join's CTAs find room beside the experts' (64 experts, 1 token: 49.7 -> 43.5 us); with more, the
   // stages are worth more (37 tokens: 193 against 196 us).
   const int room = kFewShared - (T <= 16 ? kFewJoinRoom : 0) - (p.bf16 ? 0 : FewTc<true>::low_bytes());
   const long long most = ((long long)std::min(p.E, T * p.k) * UE + r.grid - 1) / r.grid;
   const long long rows = (std::min<long long>(most, UE) + ups - 1) / ups + 1;
-  r.hbytes = (int)std::min<long long>(rows * parts * r.Tp * 128, room - 4 * sb);
-  r.hbytes = std::max({r.hbytes, parts * r.Tp * 128, kFewSlack});
+  constexpr int hparts = FewTc<false>::HPARTS;
+  const int crowd = p.bf16 ? std::min(r.Tp, (4 * T * p.k / p.E + 16) / 16 * 16) : r.Tp;
+  r.hbytes = (int)std::min<long long>(rows * hparts * crowd * 128, room - 4 * sb);
+  r.hbytes = std::max({r.hbytes, hparts * r.Tp * 128, kFewSlack});
   r.stages = std::min(kFewMaxStages, (room - r.hbytes) / sb);
   return r;
 }

@@ -50,9 +50,11 @@ def moe_few_tokens(
     for has id -1 and gate 0, and a token without any expert gets its residual
     (or zeros).  residual [T, O]: fp32 or bf16; ``out`` may be the same tensor.
 
-    Sums are kept in fp32; bf16 layers keep the hidden activation in bf16, as
-    the large layer does, except in the smallest calls, which keep it in fp32;
-    an fp32 result that is infinite may come out as NaN.
+    Sums are kept in fp32, and the hidden activations in fp32 or as two bf16
+    numbers (2^-16), whatever the size of the call; the result is rounded once.
+    A result that is infinite may come out as NaN.  bf16 layers leave the tensor
+    core's own sums over D, which drift by up to 2e-6 of the activation for each
+    1024 of it.
     Returns (out [T, O] in out_dtype or x's type, expert ids int32 [T, top_k],
     gates fp32 [T, top_k]).  Enqueues two or three launches (wide fp32 layers: for
     each 16 or 32 tokens) on the current stream

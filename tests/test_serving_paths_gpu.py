@@ -280,3 +280,41 @@ def test_a_record_is_raised_once_and_leaves_other_calls_alone():
         with pytest.raises(status.DeviceStatusError):
             status.check_serving(index)
         status.check_serving()
+
+
+@pytest.mark.parametrize("T,k,E,act", [(1, 4, 16, "swiglu"), (9, 2, 8, "gelu"), (30, 1, 2, "silu"), (64, 2, 4, "swiglu"), (64, 1, 1, "relu")])
+@pytest.mark.parametrize("tensor", [False, True], ids=["rows", "tensor"])
+def test_bf16_activations_keep_their_bits(T, k, E, act, tensor):
+    """A bf16 layer with an fp32 result: the activations between the products are not rounded to bf16, however the call runs.
+    Two bf16 parts hold one to 2^-16.  The tensor core cuts what it adds, 2^-23 at most for each 16 of D and, with both parts,
+    for each 8 of F."""
+    D, O = 512, 384
+    F = _widths(T, k, BF16, act, D, O) if tensor else 48
+    a = _make(T, D, E, F, O, act, BF16, seed=T)
+    assert _plan(a, k, act)["path"] == ("tensor" if tensor else "rows")
+    out, _, _ = _check(a, k, act, "none", out_dtype=FP32)
+    want = moe64(**a, top_k=k, act=act, gate_mode="none", out_dtype=FP32)[0]
+    check_norm(out, want, 2.0 ** -16 + 2 * U * (D / 16 + F / 8 + 16))
+
+
+def test_largest_bf16_activations():
+    """Activations that bf16 cannot round without an infinity, and infinite ones, which stay with their token."""
+    T, D, E, k, O = 8, 512, 4, 1, 256
+    a = _make(T, D, E, _widths(T, k, BF16, "relu", D, O), O, "relu", BF16, seed=3)
+    a["x"] = torch.zeros_like(a["x"])
+    a["x"][:, 3] = 1.0 + 2.0 ** -6
+    a["router_w"].zero_()
+    a["w1"] = a["w1"].sign() * 3.35e38          # in bf16, times 1 + 2^-6: 3.402e38, between the largest numbers of bf16 and fp32
+    a["b1"] = torch.zeros(E, a["w1"].shape[1], device=DEV)
+    top = float(a["w1"].abs().max()) * (1 + 2.0 ** -6)
+    assert torch.finfo(BF16).max < top < torch.finfo(FP32).max
+    a["w2"] *= 2.0 ** -100
+    assert _plan(a, k, "relu")["path"] == "tensor"
+    out, _, _ = _moe(**a, top_k=k, act="relu", gate_mode="none", out_dtype=FP32)
+    want, bound = moe64(**a, top_k=k, act="relu", gate_mode="none", out_dtype=FP32)[:2]
+    check_close(out, want, bound)
+    base = out
+    a["x"][5, 3] = 2.0
+    out, _, _ = _moe(**a, top_k=k, act="relu", gate_mode="none", out_dtype=FP32)
+    keep = [i for i in range(T) if i != 5]
+    assert torch.equal(out[keep], base[keep]) and not out[5].isfinite().any()
