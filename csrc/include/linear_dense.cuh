@@ -8,12 +8,16 @@
 // outputs, so a thread finds both in its accumulator row and the weights need
 // no other order than gate rows, then up rows.
 //
+// The tensor core cuts what does not fit its accumulator, which drifts with the
+// length of the chain (2e-6 of the result for each 1024 of K), so for fp32
+// results K is taken in chains, each into an accumulator of its own; the
+// epilogue warps add the chains in registers, rounded to nearest, while the
+// next one runs.  Chains of 1024 of K for bf16 operands (4096 x 8192 x 4096 to
+// fp32: 269 us, all of K in one 244 and 1.6e-5 off), of 128 for fp32 ones (4096
+// x 1024 x 4096: 199 us and 0.35e-6 off; 256 at a time 188 and 0.64e-6, twice
+// that behind SwiGLU).
+//
 // fp32: x and w come as two tf32 parts each (linear_split_kernel), h + l.  The
-// tensor core cuts what does not fit its accumulator, which drifts with the
-// length of the chain (2e-6 of the result for each 1024 of K), so K is taken
-// 128 at a time (4096 x 1024 x 4096: 199 us and 0.35e-6 off; 256 at a time 188
-// and 0.64e-6, twice that behind SwiGLU), each into an accumulator of its own; the epilogue warps add
-// the chains in registers, rounded to nearest, while the next one runs.  The
 // small products l h' and h l' have an accumulator for the whole tile.  A stage
 // holds both parts of both operands for the three products: two thirds of the
 // bytes that three walks over K would fetch.
@@ -31,7 +35,6 @@ namespace raiccl {
 constexpr int kDenseThreads = 320;         // TMA, MMA, eight epilogue warps
 constexpr int kDenseKernelId = 620;
 constexpr int kDenseGroup = 8;
-constexpr int kDenseChain = 4;             // fp32: 128-byte steps of K of a chain
 constexpr unsigned long long kDenseWaitNs = 2000000000ull;
 
 struct LinearDenseParams {
@@ -50,6 +53,7 @@ struct LinearDense {
   static constexpr int STAGES_FIT = 216 * 1024 / STAGE;
   static constexpr int STAGES = STAGES_FIT > 8 ? 8 : STAGES_FIT;
   static constexpr int SMEM = 1024 + STAGES * STAGE;
+  static constexpr int CHAIN = FP32 ? 4 : 16;   // 128-byte steps of K of a chain
   static constexpr int COLS = FP32 ? 4 * BN : 2 * BN;   // fp32: two for chains, two for small products
 };
 
@@ -157,7 +161,8 @@ __device__ __forceinline__ void dense_add_bias16(const float (&b)[NB], int c, fl
   for (int i = 0; i < 16; ++i) v[i] += __shfl_sync(0xffffffffu, mine, (c & 16) + i);
 }
 
-template <int BN, bool FP32, bool GLU>
+// CHAINED: the sums leave the tensor core after every chain, else after the whole of K.
+template <int BN, bool FP32, bool GLU, bool CHAINED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kDenseThreads, 1)
 linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, LinearDenseParams p,
                     DeviceStatus* status) {
@@ -191,7 +196,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
 
   constexpr int W = GLU ? BN / 2 : BN;      // outputs of a tile
   const int KB = (l.K + C::BK - 1) / C::BK;
-  const int chain = FP32 ? kDenseChain : KB;             // 128-byte steps of K of an accumulator
+  const int chain = CHAINED ? C::CHAIN : KB;             // 128-byte steps of K of an accumulator
   const int tiles = p.mt * p.nt;
 
   if (warp == 0) {
@@ -285,7 +290,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
     bool ok = true;
     // Biases and the first pieces (16 columns) of the residual are read before the sums are waited for, the others as many
     // pieces ahead.
-    constexpr int AHEAD = FP32 ? 2 : 4;
+    constexpr int AHEAD = CHAINED ? (BN == 256 ? 1 : 2) : 4;   // by the registers that the sums leave
     constexpr int NB = (OUT + 31) / 32;
     float bias[NB], up[NB];
     uint4 ahead[AHEAD][4];
@@ -322,7 +327,7 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
       const long long m = (long long)mb * 256 + rank * 128 + q * 32 + lane;
       const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16);
       const int c0 = side * OUT, n0 = nb * W + c0;
-      if constexpr (FP32) {
+      if constexpr (CHAINED) {
         float sum[OUT], sum_up[GLU ? OUT : 16];
 #pragma unroll
         for (int i = 0; i < OUT; ++i) sum[i] = 0.f;
@@ -355,12 +360,15 @@ linear_dense_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constan
           add(lanes + b * BN + c0);
           if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&acc_empty[b]), 0));
         }
-        if (ok) begin(m, n0);
-        if (!ok || !(ok = mbar_wait_warp(&low_full[nth & 1], (nth >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
-        tc_fence_after_sync();
-        add(lanes + (2 + (nth & 1)) * BN + c0);
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&low_empty[nth & 1]), 0));
-        ++nth;
+        if (!ok) break;
+        begin(m, n0);
+        if constexpr (FP32) {
+          if (!(ok = mbar_wait_warp(&low_full[nth & 1], (nth >> 1) & 1, status, kDenseKernelId, kDenseWaitNs))) break;
+          tc_fence_after_sync();
+          add(lanes + (2 + (nth & 1)) * BN + c0);
+          if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&low_empty[nth & 1]), 0));
+          ++nth;
+        }
 #pragma unroll
         for (int c = 0; c < OUT; c += 16) {
           float z[16], zu[16];

@@ -11,15 +11,17 @@
 // shared memory, no global scratch and no counters, the same result every
 // time), then bias, activation and residual, and rounds once.
 //
+// The tensor core cuts what does not fit its accumulator instead of rounding,
+// which drifts toward zero with the length of the chain (2e-6 of the result for
+// each 1024 of K).  For fp32 results the sums therefore go to registers after
+// every 128 of K (bf16 operands: 512) and are added there, rounded to nearest,
+// while the next piece runs into the other of two accumulators.  bf16 results
+// are rounded to 2^-8, where the drift of a whole K does not show.
+//
 // fp32: two tf32 parts of 11 bits each, made by eight warps from the staged
 // tiles: x in place and beside it (split_tf32), of the weights, whose upper 19
 // bits the tensor core reads, only the rests (rest_tf32), into a short ring;
-// h h' + h l' + l h' is the product to 2^-20.  The tensor core cuts what does
-// not fit its accumulator instead of rounding, which drifts toward zero with
-// the length of the chain (2e-6 of the result for each 1024 of K): every 128 of
-// K the sums go to registers and are added there, rounded to nearest, while the
-// next 128 run into the other of two accumulators.  bf16 results are rounded to
-// 2^-8, where the drift of a whole K does not show.
+// h h' + h l' + l h' is the product to 2^-20.
 #pragma once
 
 #include "serving.h"
@@ -31,7 +33,6 @@ namespace raiccl {
 constexpr int kRowsTile = 128 * 128;       // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kRowsPack = 2;               // 128-byte steps of K in a stage: a stage costs its waits and its commit, 0.15 us
 constexpr int kRowsMaxStages = 12;
-constexpr int kRowsChain = 2;              // fp32: stages into one accumulator
 constexpr int kRowsKernelId = 610;
 constexpr unsigned long long kServingWaitNs = 2000000000ull;
 
@@ -48,10 +49,11 @@ struct LinearRows {
   static constexpr int PARTS = FP32 ? 2 : 1;
   static constexpr int BK = FP32 ? 32 : 64;          // elements of 128 bytes
   static constexpr int THREADS = FP32 ? 448 : 192;
+  static constexpr int CHAIN = FP32 ? 2 : 4;         // stages into one accumulator, where sums are kept in registers
   static __host__ __device__ int stage_bytes(int Mp) { return kRowsPack * (kRowsTile + PARTS * Mp * 128); }   // weight tiles, then x tiles (h rows, l rows)
 };
 
-// MP: rows of x of a tile where the sums are kept in registers (fp32), else 0.
+// MP: rows of x of a tile where the sums are kept in registers (fp32 operands, fp32 results), else 0.
 template <bool FP32, bool GLU, int MP>
 __global__ void __launch_bounds__(LinearRows<FP32>::THREADS)
 linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, LinearRowsParams p,
@@ -71,7 +73,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   constexpr int W = GLU ? 64 : 128;                     // output columns of a tile
   const int n0 = (int)(blockIdx.x / ranks) * W;
   const long long m0 = (long long)blockIdx.y * p.Mp;
-  const int cols0 = FP32 ? 4 * p.Mp : p.Mp;             // fp32: two accumulators of [h | l] columns
+  const int cols0 = MP > 0 ? 2 * C::PARTS * MP : p.Mp;  // two accumulators where chains are cut; fp32: of [h | l] columns
   const int cols = cols0 <= 32 ? 32 : cols0 <= 64 ? 64 : cols0 <= 128 ? 128 : cols0 <= 256 ? 256 : 512;
   const int KB = (l.K + C::BK - 1) / C::BK;
   const int kb0 = (int)((long long)KB * rank / ranks), kb1 = (int)((long long)KB * (rank + 1) / ranks);
@@ -128,20 +130,20 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       const uint32_t id = umma_idesc(FP32 ? 2u : 1u, 128, (uint32_t)(C::PARTS * p.Mp)), idl = umma_idesc(2u, 128, (uint32_t)p.Mp);
       int lo = 0;
       for (int i = 0; i < count; ++i, advance()) {
-        if (FP32 && i % kRowsChain == 0) {
-          const int c = i / kRowsChain;
+        if (MP > 0 && i % C::CHAIN == 0) {
+          const int c = i / C::CHAIN;
           if (!serving_wait(&acc_empty[c & 1], ((c >> 1) & 1) ^ 1u, status, kRowsKernelId, kServingWaitNs)) break;
         }
         if (!serving_wait(&ready[stage], phase, status, kRowsKernelId, kServingWaitNs)) break;
         tc_fence_after_sync();
-        const uint32_t d = tmem + (FP32 ? (i / kRowsChain & 1) * 2 * p.Mp : 0);
+        const uint32_t d = tmem + (MP > 0 ? (i / C::CHAIN & 1) * C::PARTS * MP : 0);
         const uint32_t w = smem_u32(smem + stage * SB);
         uint64_t da = desc_at(row, w), dx = desc_at(row, w + kRowsPack * kRowsTile), dl = desc_at(row, smem_u32(low) + lo * kRowsPack * kRowsTile);
         const int n = steps - i * kRowsPack < kRowsPack ? steps - i * kRowsPack : kRowsPack;
         for (int j = 0; j < n; ++j, da += kRowsTile / 16, dx += C::PARTS * p.Mp * 8, dl += kRowsTile / 16) {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const uint32_t more = ((FP32 ? i % kRowsChain : i) | j | k) ? 1u : 0u;
+            const uint32_t more = ((MP > 0 ? i % C::CHAIN : i) | j | k) ? 1u : 0u;
             if constexpr (FP32) {
               umma_tf32(d, da + 2 * k, dx + 2 * k, id, more);
               umma_tf32(d + p.Mp, dl + 2 * k, dx + 2 * k, idl, 1u);   // with the other small products
@@ -151,26 +153,26 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           }
         }
         umma_commit(&empty[stage]);
-        if (FP32 && (i % kRowsChain == kRowsChain - 1 || i + 1 == count)) umma_commit(&acc_full[i / kRowsChain & 1]);
+        if (MP > 0 && (i % C::CHAIN == C::CHAIN - 1 || i + 1 == count)) umma_commit(&acc_full[i / C::CHAIN & 1]);
         if (++lo == p.low) lo = 0;
       }
       umma_commit(&done);
     }
-  } else if (FP32 && warp < 6) {
-    // ---------------------------------------------------------------- fp32: a chain's sums into registers
+  } else if (MP > 0 && warp < 6) {
+    // ---------------------------------------------------------------- a chain's sums into registers
     const uint32_t base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    for (int c = 0; c * kRowsChain < count; ++c) {
+    for (int c = 0; c * C::CHAIN < count; ++c) {
       added = mbar_wait_warp(&acc_full[c & 1], (c >> 1) & 1, status, kRowsKernelId, kServingWaitNs);
       if (!added) break;
       tc_fence_after_sync();
 #pragma unroll
       for (int i = 0; i < MP; i += 16) {
         uint32_t v[16], u[16];
-        tmem_ld16(base + (c & 1) * 2 * MP + i, v);
-        tmem_ld16(base + (c & 1) * 2 * MP + MP + i, u);
+        tmem_ld16(base + (c & 1) * C::PARTS * MP + i, v);
+        if constexpr (FP32) tmem_ld16(base + (c & 1) * 2 * MP + MP + i, u);
         tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[i + j] += __uint_as_float(v[j]) + __uint_as_float(u[j]);
+        for (int j = 0; j < 16; ++j) acc[i + j] += FP32 ? __uint_as_float(v[j]) + __uint_as_float(u[j]) : __uint_as_float(v[j]);
       }
       tc_fence_before_sync();
       __syncwarp();
@@ -209,7 +211,7 @@ linear_rows_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   __syncwarp();
   if (warp >= 2 && warp < 6) {
     const int q = warp & 3;
-    if constexpr (FP32) {
+    if constexpr (MP > 0) {
 #pragma unroll
       for (int i = 0; i < MP; ++i)
         if (i < rows) sums[i * 128 + q * 32 + lane] = acc[i];

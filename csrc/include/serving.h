@@ -117,6 +117,7 @@ struct LinearPlan {
   int vector, vec;         // very few rows, on CUDA cores; 16 bytes at a time
   int dense;               // CTA pairs with tiles of 256 x dense sums; 0: few rows
   int Mp, ranks, stages, low;   // few rows: rows of x of a tile, CTAs that share K, stages, tiles of low parts
+  int chained;             // bf16 operands, fp32 result: sums leave the tensor core in pieces of K
   int pack_x, pack_w;      // rows that TMA cannot read are copied to aligned ones first
   int packed_stride;
   long long x_bytes, w_bytes;

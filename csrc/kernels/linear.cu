@@ -61,6 +61,11 @@ constexpr int kRowsShared = 232448 - 2048;   // dynamic shared memory of a CTA, 
 
 static long long up256(long long v) { return (v + 255) / 256 * 256; }
 
+// bf16 operands with an fp32 result: so much of K goes into one accumulator at least, in dense tiles up to twice as much.
+constexpr int kLinearChain = 512;
+static_assert(kLinearChain == LinearRows<false>::CHAIN * kRowsPack * LinearRows<false>::BK &&
+              2 * kLinearChain == LinearDense<256, false>::CHAIN * LinearDense<256, false>::BK);
+
 // Which kernel, by what each was measured to take on one B200 (us; sizes 32 to 2048 rows, 1024 to 5632 outputs, K 1024 to
 // 4096; the sums below are within a seventh of most):
 //   rows       3 + 4 Mp / (64 ranks) for each round of CTAs, and for each 128 bytes of its K 0.14 to 0.24 (fp32: 0.55 to
@@ -86,7 +91,8 @@ LinearPlan plan_linear(const LinearParams& p, int sms) {
 
   // rows: CTAs that share K
   r.Mp = (int)std::min<long long>(64, (p.M + 15) / 16 * 16);
-  if (!p.bf16 && r.Mp == 48) r.Mp = 64;
+  r.chained = p.bf16 && !p.out_bf16 && p.K > kLinearChain;
+  if ((!p.bf16 || r.chained) && r.Mp == 48) r.Mp = 64;
   const long long mt = (p.M + r.Mp - 1) / r.Mp, tiles = (p.N + (glu ? 63 : 127)) / (glu ? 64 : 128) * mt;
   const int per = p.bf16 ? 2 : 1;   // CTAs per SM; fp32 holds a stage through splitting and product, so one with as many as fit
   double best = 0;
@@ -122,6 +128,7 @@ LinearPlan plan_linear(const LinearParams& p, int sms) {
       }
     }
   }
+  if (r.dense && p.K <= 2 * kLinearChain) r.chained = 0;
   // Very few rows: without pipelines, splits and copies.  Up to so many weights (millions), by where the two cross; us, here
   // against there: bf16 1 row 1024 x 1024 2.4 / 4.0, 4096 x 4096 9.1 / 9.7, 16384 x 4096 26.5 / 23.5, 4 rows 1024 x 1024
   // 3.1 / 4.1, 4096 x 1024 9.0 / 4.6; fp32 1 row 16384 x 4096 43 / 74, 4 rows 68 / 75, 8 rows 1024 x 1024 4.9 / 7.7; SwiGLU
@@ -205,10 +212,10 @@ static void launch_rows(const LinearParams& p, const LinearPlan& plan, cudaStrea
   cudaLaunchKernelEx(&cfg, kern, tx, tw, rp, serving_status());
 }
 
-template <int BN, bool FP32, bool GLU>
+template <int BN, bool FP32, bool GLU, bool CHAINED>
 static void launch_dense(const LinearParams& p, cudaStream_t s) {
   using C = LinearDense<BN, FP32>;
-  auto kern = linear_dense_kernel<BN, FP32, GLU>;
+  auto kern = linear_dense_kernel<BN, FP32, GLU, CHAINED>;
   static std::atomic<unsigned long long> configured;  // by device
   int dev = 0;
   cudaGetDevice(&dev);
@@ -241,18 +248,20 @@ static void launch_dense(const LinearParams& p, cudaStream_t s) {
 
 // fp32 stages hold four tiles: at 256 columns three stages of 64 KB, at 128 four of 48 KB, which is what it takes
 // (2048 x 4096 x 4096: 340 against 275 us).
-static void launch_dense_any(const LinearParams& p, int bn, cudaStream_t s) {
-  const bool glu = p.act == (int)Act::kSwiGLU;
-  if (!p.bf16) {
-    if (glu) launch_dense<128, true, true>(p, s);
-    else launch_dense<128, true, false>(p, s);
-  } else if (bn == 256) {
-    if (glu) launch_dense<256, false, true>(p, s);
-    else launch_dense<256, false, false>(p, s);
-  } else {
-    if (glu) launch_dense<128, false, true>(p, s);
-    else launch_dense<128, false, false>(p, s);
-  }
+static void launch_dense_any(const LinearParams& p, const LinearPlan& plan, cudaStream_t s) {
+  auto run = [&](auto bn, auto fp32, auto chained) {
+    constexpr int BN = decltype(bn)::value;
+    constexpr bool FP32 = decltype(fp32)::value, CHAINED = decltype(chained)::value;
+    if (p.act == (int)Act::kSwiGLU) launch_dense<BN, FP32, true, CHAINED>(p, s);
+    else launch_dense<BN, FP32, false, CHAINED>(p, s);
+  };
+  auto bf16 = [&](auto bn) {
+    if (plan.chained) run(bn, std::false_type{}, std::true_type{});
+    else run(bn, std::false_type{}, std::false_type{});
+  };
+  if (!p.bf16) run(std::integral_constant<int, 128>{}, std::true_type{}, std::true_type{});
+  else if (plan.dense == 256) bf16(std::integral_constant<int, 256>{});
+  else bf16(std::integral_constant<int, 128>{});
 }
 
 template <typename T, bool VEC, bool GLU>
@@ -324,19 +333,19 @@ void launch_linear(const LinearParams& params, const LinearPlan& plan, void* wor
     p.w = ws + plan.x_bytes;
     p.w_stride = plan.packed_stride;
   }
-  if (plan.dense) return launch_dense_any(p, plan.dense, s);
-  if (p.bf16) {
-    if (glu) launch_rows<false, true, 0>(p, plan, s);
-    else launch_rows<false, false, 0>(p, plan, s);
-  } else {
-    auto rows = [&](auto mp) {
-      if (glu) launch_rows<true, true, decltype(mp)::value>(p, plan, s);
-      else launch_rows<true, false, decltype(mp)::value>(p, plan, s);
-    };
-    if (plan.Mp == 16) rows(std::integral_constant<int, 16>{});
-    else if (plan.Mp == 32) rows(std::integral_constant<int, 32>{});
-    else rows(std::integral_constant<int, 64>{});
-  }
+  if (plan.dense) return launch_dense_any(p, plan, s);
+  auto rows = [&](auto fp32, auto mp) {
+    if (glu) launch_rows<decltype(fp32)::value, true, decltype(mp)::value>(p, plan, s);
+    else launch_rows<decltype(fp32)::value, false, decltype(mp)::value>(p, plan, s);
+  };
+  auto chained = [&](auto fp32) {
+    if (plan.Mp == 16) rows(fp32, std::integral_constant<int, 16>{});
+    else if (plan.Mp == 32) rows(fp32, std::integral_constant<int, 32>{});
+    else rows(fp32, std::integral_constant<int, 64>{});
+  };
+  if (!p.bf16) chained(std::true_type{});
+  else if (plan.chained) chained(std::false_type{});
+  else rows(std::false_type{}, std::integral_constant<int, 0>{});
 }
 
 }  // namespace raiccl

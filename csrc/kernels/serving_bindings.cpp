@@ -324,6 +324,7 @@ py::dict linear_plan(torch::Tensor x, torch::Tensor weight, int64_t act, OptTens
   py::dict d;
   d["kernel"] = plan.vector ? "vector" : plan.dense ? "dense" : "rows";
   d["tile"] = plan.dense;
+  d["chained"] = !plan.vector && plan.chained;
   d["ranks"] = plan.vector || plan.dense ? 0 : plan.ranks;
   d["pack_x"] = plan.pack_x != 0;
   d["pack_w"] = plan.pack_w != 0;

@@ -35,9 +35,7 @@ def linear(
 
     Sums are kept in fp32 and rounded once, to out_dtype (default: x's type;
     fp32 inputs give fp32).  fp32 inputs are multiplied to fp32 accuracy, not
-    to tf32's (an infinite result may come out as NaN);
-    bf16 inputs leave the tensor core's own sums, which over a K of 14336 drift
-    by up to 3e-5 of an fp32 result.  Enqueues on the current stream without
+    to tf32's (an infinite result may come out as NaN).  Enqueues on the current stream without
     synchronising and can be captured in a CUDA graph.  Rows of x or weight
     that do not start on 16 bytes are copied first (not for up to 4 rows of x,
     8 in fp32), which costs up to twice the product's own reads.  At most 2^30

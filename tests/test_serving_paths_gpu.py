@@ -318,3 +318,20 @@ def test_largest_bf16_activations():
     out, _, _ = _moe(**a, top_k=k, act="relu", gate_mode="none", out_dtype=FP32)
     keep = [i for i in range(T) if i != 5]
     assert torch.equal(out[keep], base[keep]) and not out[5].isfinite().any()
+
+
+@pytest.mark.parametrize("m,k,n,act,kernel", [
+    (1, 14336, 256, "none", "vector"), (20, 8192, 512, "none", "rows"), (40, 14336, 12288, "none", "rows"), (64, 8192, 9000, "swiglu", "rows"),
+    (10, 520, 100, "none", "rows"), (300, 8192, 1032, "gelu", "rows"), (1100, 4104, 4096, "none", "dense"), (1100, 8192, 2600, "swiglu", "dense"),
+    (2100, 8192, 1200, "none", "dense"), (700, 1000, 2049, "none", "rows"),
+])
+def test_bf16_products_to_fp32(m, k, n, act, kernel):
+    """Exact products and 32-bit sums, over any K: errors of random sign, and the cuts of the tensor core in one chain of 512
+    (32 instructions; dense tiles 64); a whole K of 8192 without chains would be 1.6e-5 off."""
+    x, w, b, _ = _make_linear(m, k, n, act, BF16, True, False, seed=8)
+    plan = _linear_plan(x, w, act, out_dtype=FP32)
+    assert plan["kernel"] == kernel and plan["chained"] == (kernel != "vector")
+    got = _linear(x, w, b, act=act, out_dtype=FP32)
+    want, bound = linear64(x, w, b, act, None, FP32)
+    check_close(got, want, bound)
+    check_norm(got, want, (2 if act == "swiglu" else 1) * U * (k ** 0.5 / 2 + 8 + (64 if kernel == "dense" else 32)))
