@@ -60,7 +60,8 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
 }
 
 // Behind a shape there may be no numbers to read: a sparse layout, a lazy zero or
-// negation, or a storage that was freed (sharded parameters between their uses).
+// negation, a storage that was freed (sharded parameters between their uses), or
+// a wrapper of other tensors (distributed, quantised or fake ones).
 void check_memory(const char* op, const char* name, const torch::Tensor& t) {
   TORCH_CHECK_VALUE(t.layout() == c10::kStrided && !t.is_neg() && !t._is_zerotensor(), op, ": ", name,
                     " must be a dense tensor, without a pending negation or zero");
@@ -69,6 +70,7 @@ void check_memory(const char* op, const char* name, const torch::Tensor& t) {
   for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
   TORCH_CHECK_VALUE((int64_t)t.storage().nbytes() >= (last + 1) * (int64_t)t.element_size(), op, ": ", name,
                     " reaches behind its storage, which holds ", text((int64_t)t.storage().nbytes()), " bytes");
+  TORCH_CHECK_VALUE(t.is_meta() || t.data_ptr() != nullptr, op, ": ", name, " has no memory of its own (a wrapper of other tensors?)");
 }
 
 // Every tensor of a call lies on the CUDA device of x; checked behind the

@@ -155,3 +155,34 @@ def test_freed_storages_are_refused():
     part.untyped_storage().resize_(100)
     with pytest.raises(ValueError, match="x reaches behind its storage, which holds 100 bytes"):
         _linear(x=part)
+
+
+class _Wrapper(torch.Tensor):
+    """A shape without memory, as distributed and quantised tensors are."""
+
+    @staticmethod
+    def __new__(cls, *shape, dtype=BF16):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, dtype=dtype)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(func)
+
+
+def test_wrappers_are_refused():
+    for name, shape in (("x", (3, 16)), ("weight", (8, 16)), ("residual", (3, 8)), ("out", (3, 8))):
+        with pytest.raises(ValueError, match=f"{name} has no memory"):
+            _linear(**{name: _Wrapper(*shape)})
+    for name, shape in (("x", (3, 16)), ("router_w", (4, 16)), ("w1", (4, 24, 16)), ("w2", (4, 10, 12)), ("residual", (3, 10)),
+                        ("out", (3, 10))):
+        with pytest.raises(ValueError, match=f"{name} has no memory"):
+            _moe(**{name: _Wrapper(*shape)})
+    with pytest.raises(ValueError, match="b1 has no memory"):
+        _moe(b1=_Wrapper(4, 24, dtype=torch.float32))
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        fake = torch.zeros(3, 16, dtype=BF16)
+    with pytest.raises((ValueError, RuntimeError), match="memory|data pointer"):
+        _linear(x=fake)
+    with pytest.raises(ValueError, match="CUDA device"):
+        _linear(x=torch.zeros(3, 16, dtype=BF16, device="meta"), weight=torch.zeros(8, 16, dtype=BF16, device="meta"))
