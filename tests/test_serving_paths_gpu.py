@@ -335,3 +335,40 @@ def test_bf16_products_to_fp32(m, k, n, act, kernel):
     want, bound = linear64(x, w, b, act, None, FP32)
     check_close(got, want, bound)
     check_norm(got, want, (2 if act == "swiglu" else 1) * U * (k ** 0.5 / 2 + 8 + (64 if kernel == "dense" else 32)))
+
+
+FIRST_IN_A_CAPTURE = """
+import torch
+from revealaiccl_b200.ops.linear import linear
+from revealaiccl_b200.ops.moe_few import moe_few_tokens
+
+def make(*shape, dtype):
+    return (torch.randn(*shape, device="cuda") * 0.1).to(dtype)
+
+for dtype in (torch.bfloat16, torch.float32):
+    w, big = make(512, 256, dtype=dtype), make(2048, 1024, dtype=dtype)
+    layer = dict(router_w=make(8, 256, dtype=dtype), w1=make(8, 20000, 256, dtype=dtype), w2=make(8, 256, 10000, dtype=dtype))
+    small = dict(router_w=make(8, 256, dtype=dtype), w1=make(8, 64, 256, dtype=dtype), w2=make(8, 256, 32, dtype=dtype))
+    x1, x20, x999, odd = (make(m, k, dtype=dtype) for m, k in ((1, 256), (20, 256), (999, 1024), (20, 257)))
+    calls = (lambda: linear(x1, w), lambda: linear(x20, w, act="swiglu"), lambda: linear(x999, big), lambda: linear(odd[:, 1:], w),
+             lambda: moe_few_tokens(x1, **small, top_k=2)[0], lambda: moe_few_tokens(x20, **small, top_k=2)[0],
+             lambda: moe_few_tokens(x20, **layer, top_k=2)[0])
+    for call in calls:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graph.replay()
+        assert torch.equal(out, call())
+print("all captured")
+"""
+
+
+def test_first_calls_inside_captures():
+    """A process whose first call of each kernel is captured: nothing that a first call sets up breaks the capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    p = subprocess.run([sys.executable, "-c", FIRST_IN_A_CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0 and "all captured" in p.stdout, p.stderr[-2000:]
