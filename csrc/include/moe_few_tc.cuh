@@ -44,7 +44,7 @@
 // fit its accumulator, which drifts with the length of the chain (2e-6 of the
 // result for each 1024 of K), so product 1 of fp32 runs into three to
 // fourteen accumulators in turn along K, added in registers.  Two groups of splitting
-// warps set the pace of fp32 (8 experts 1024 x 4096, 16 tokens: 82 us; writing
+// warps set the pace of fp32 (8 experts 1024 x 4096, 16 tokens: 80 us; writing
 // the high parts too 90, writing nothing 68).
 #pragma once
 
@@ -60,7 +60,7 @@ constexpr int kFewTile = 128 * 128;           // bytes of a weight tile: 128 row
 constexpr int kFewSlack = 12 * 1024;          // behind the last tile: rows that an instruction reads past a short one
 constexpr int kFewMaxStages = 12;
 constexpr int kFewChain = 11;                 // fp32: 128-byte steps of K of an accumulator
-constexpr int kFewLow = 2;                    // fp32: stages whose low parts of the weights are kept (3: a stage less, 84 against 82 us)
+constexpr int kFewLow = 2;                    // fp32: stages whose low parts of the weights are kept (3: a stage less, 2 us more of 82)
 constexpr unsigned long long kFewWaitNs = 2000000000ull;
 constexpr int kFewKernelId = 600;
 

@@ -105,10 +105,14 @@ __device__ __forceinline__ void store_elem(void* p, long long i, float v, int bf
   else ((float*)p)[i] = v;
 }
 
-// Activations in 32 bits, by the approximate exponential and quotient (a few
-// units in the last place; an epilogue has 64 to 128 of them per thread, and
-// with expf, erfcf and exact quotients they took as long as the products: 4096
-// x 1024 x 4096 fp32 with GELU 212 us, without 159).  ReLU keeps a NaN.
+// Activations in 32 bits, by the approximate exponential and quotient.  Their
+// errors are small against the argument, not against a result near zero: the
+// exponential is off by 2 + 1.2 |z| units in the last place, and GELU's tail by
+// an absolute 0.75e-7 |z| (at -4 that is 5e-4 of the value, about what a sum 1 +
+// erf in 32 bits loses there too).  An epilogue has 64 to 128 of them per
+// thread, and with expf, erfcf and exact quotients they took as long as the
+// products: 4096 x 1024 x 4096 fp32 with GELU 212 us, without 159.  ReLU keeps a
+// NaN.
 __device__ __forceinline__ float serving_sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
 // z Phi(z), with the normal distribution's tail from the rational-exponential

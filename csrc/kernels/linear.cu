@@ -110,7 +110,7 @@ LinearPlan plan_linear(const LinearParams& p, int sms) {
   }
   if (mt > 65535) best = 1e30;   // more tiles than a grid has rows
   // Rows of out or residual off 16 bytes: a thread of a dense tile has a row of its own and goes through it element by
-  // element, 20 us for a tile of 128 columns (bf16, dense / rows, us: 269 x 64 x 10735 71 / 16, 4096 x 1024 x 4097 281 / 127).
+  // element, 20 us for a tile of 128 columns (bf16, dense / rows, us: 269 x 64 x 10735 71 / 16, 4096 x 1024 x 4097 281 / 106).
   const int ob = p.out_bf16 ? 2 : 4, rb = p.res_bf16 ? 2 : 4;
   const bool odd = (((uintptr_t)p.out | (uintptr_t)(p.out_stride * ob)) & 15) != 0 ||
                    (p.residual != nullptr && (((uintptr_t)p.residual | (uintptr_t)(p.res_stride * rb)) & 15) != 0);

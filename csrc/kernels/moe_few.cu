@@ -480,8 +480,8 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p, int sms) {
     return r;
   }
   // fp32: so many tokens at a time that no accumulator takes more than 352 of K, if 16 can (D 4928), since it is cut at each
-  // step (64 tokens, 4 experts 4096 x 1024 SwiGLU: error 6.6e-6 and 130 us all at once, 1.6e-6 and 371 us by 16); the weights are then
-  // read again for each.
+  // step (64 tokens, 4 experts 4096 x 1024 SwiGLU: error 6.6e-6 and 130 us all at once, 1.6e-6 and 371 to
+  // 480 us by 16); the weights are then read again for each.
   r.slice = p.T;
   if (!p.bf16) {
     const int steps = (p.D + 31) / 32;

@@ -48,22 +48,27 @@ def moe_few_tokens(
     block_mask: bool or uint8 [E] or [T, E], true where an expert may not be
     chosen; a logit of -inf counts as blocked.  A choice that no expert is left
     for has id -1 and gate 0, and a token without any expert gets its residual
-    (or zeros).  residual [T, O]: fp32 or bf16; ``out`` may be the same tensor.
+    (or zeros).  residual [T, O]: fp32 or bf16; ``out`` may be the same tensor,
+    but its range of memory may not overlap another input's.
 
     Sums are kept in fp32, and the hidden activations in fp32 or as two bf16
     numbers (2^-16), whatever the size of the call; the result is rounded once.
-    A result that is infinite may come out as NaN.  bf16 layers leave the tensor
+    A result that is infinite may come out as NaN, and fp32 numbers below 2^-113
+    are taken to 2^-137 of absolute error only.  bf16 layers leave the tensor
     core's own sums over D, which drift by up to 2e-6 of the activation for each
     1024 of it.
     Returns (out [T, O] in out_dtype or x's type, expert ids int32 [T, top_k],
-    gates fp32 [T, top_k]).  Enqueues two or three launches (wide fp32 layers: for
-    each 16 or 32 tokens) on the current stream
-    without synchronising and can be captured in a CUDA graph; outputs and
-    workspace come from torch's allocator on that stream.  Expert rows that do
-    not start on 16 bytes are read element by element or, where many tokens
-    share few experts, copied first, which takes as much memory as all experts.
-    ``check=True`` waits and raises on a recorded device status.  There is no
-    backward.
+    gates fp32 [T, top_k]).
+
+    Enqueues two or three launches (wide fp32 layers: for each 16 or 32 tokens)
+    on the current stream without synchronising and can be captured in a CUDA
+    graph.  Outputs and workspace come from torch's allocator on that stream;
+    the workspace is up to T (SMs + 2 top_k) rows of O fp32 numbers, 172 MB for
+    64 tokens at an O of 4096 and top_k 8.  Expert rows that do not start on 16
+    bytes are read element by element or, where many tokens share few experts,
+    copied first, which takes as much memory as all experts.  ``check=True``
+    waits and raises on a recorded device status.  There is no backward: tensors
+    that require a gradient or carry a tangent are refused.
     """
     if act not in ACT_IDS:
         raise ValueError(f"moe_few_tokens: act must be one of {sorted(ACT_IDS)}")
