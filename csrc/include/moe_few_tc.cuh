@@ -41,12 +41,14 @@
 // fp32 numbers are taken as two tf32 parts of 11 bits each, h + l: x and the
 // activations as two copies, the weights as they lie (the tensor core reads
 // their upper 19 bits) with the rests written beside them in shared memory.
-// h h' + h l' + l h' is the product to 2^-20: the tokens' parts are stacked as
-// 2N columns, so that is two instructions.  The tensor core cuts what does not
+// h h' + h l' + l h' is the product to 2^-20.  The tensor core cuts what does not
 // fit its accumulator, which drifts with the length of the chain (2e-6 of the
-// result for each 1024 of K), so product 1 of fp32 runs into three to
-// fourteen accumulators in turn along K, added in registers.  Two groups of splitting
-// warps set the pace of fp32 (8 experts 1024 x 4096, 16 tokens: 80 us; writing
+// result for each 1024 of K, twice that behind SwiGLU), so fp32 sums h h' in
+// chains, 128 to 160 of K in product 1 and about 128 hidden rows in product 2,
+// each into an accumulator of its own; they are added in registers.  The small
+// products, whose cuts do not show, have one accumulator for all of K.  Two
+// groups of splitting
+// warps set the pace of fp32 (8 experts 1024 x 4096, 16 tokens: 82 us; writing
 // the high parts too 90, writing nothing 68).
 #pragma once
 
@@ -61,7 +63,8 @@ namespace raiccl {
 constexpr int kFewTile = 128 * 128;           // bytes of a weight tile: 128 rows of 128 bytes
 constexpr int kFewSlack = 12 * 1024;          // behind the last tile: rows that an instruction reads past a short one
 constexpr int kFewMaxStages = 12;
-constexpr int kFewChain = 11;                 // fp32: 128-byte steps of K of an accumulator
+constexpr int kFewChain = 5;                  // fp32: 128-byte steps of K of an accumulator at most (160) ...
+constexpr int kFewShort = 4;                  // ... and at least (128): each one more is another read in the epilogue
 constexpr int kFewLow = 2;                    // fp32: stages whose low parts of the weights are kept (3: a stage less, 2 us more of 82)
 constexpr unsigned long long kFewWaitNs = 2000000000ull;
 constexpr int kFewKernelId = 600;
@@ -215,32 +218,46 @@ struct FewWalk {
   }
 };
 
-// Accumulators in TMEM, n1 columns each, for one or two epilogue groups with
-// one or two sets of buffers: `chains` of product 1 for one tile (fp32 cuts K
-// into so many), and of product 2 `tiles` tiles of 128 outputs, so that a few
-// tokens' tiles share a hand-over.  At most 512 columns in all.
+// Accumulators in TMEM, for one or two epilogue groups with one or two sets of
+// buffers: `chains` of product 1 for one tile, and of product 2 `tiles` tiles of
+// 128 outputs, `chains2` each, so that a few tokens' tiles share a hand-over.
+// fp32 cuts K into so many chains; the small products, whose own cuts do not
+// show, have one more for all of K (`small`), and product 2 has its accumulators
+// in product 1's place: neither begins in a batch before the other's have been
+// read.  At most 512 columns in all.
 struct FewAcc {
-  int n1, groups, nbuf, chains, tiles;
-  // fp32: chains of 352 of K (kFewChain steps) at most, where that many accumulators fit; one epilogue group has more of
-  // them (16 tokens, D 4096: error 3.4e-6 with six).
-  __host__ __device__ FewAcc(int n1_, bool fp32, int steps) : n1(n1_) {
+  int Tp, groups, nbuf, chains, chains2, tiles, small;
+  // fp32: one epilogue group has more accumulators; two where the chains stay within kFewChain steps (16 tokens, 8 experts
+  // 1536 x 4096: 113 us against 130 with one)
+  __host__ __device__ FewAcc(int Tp_, bool fp32, int steps) : Tp(Tp_) {
     if (fp32) {
-      groups = n1 <= 64 && steps <= (n1 <= 32 ? 6 : 3) * kFewChain ? 2 : 1;
       nbuf = 1;
-      chains = n1 <= 32 ? (groups == 2 ? 6 : 14) : n1 <= 64 ? (groups == 2 ? 3 : 7) : n1 <= 96 ? 4 : 3;
-      tiles = n1 <= 32 ? 2 : 1;
+      small = 1;
+      chains2 = 5;
+      tiles = Tp <= 16 ? 2 : 1;
+      const int two = 256 / Tp - small;
+      groups = Tp <= 32 && steps <= two * kFewChain ? 2 : 1;
+      chains = groups == 2 ? two : 512 / Tp - small;
     } else {
       groups = 2;
       nbuf = 2;
-      chains = 1;
-      tiles = n1 <= 16 ? 4 : n1 <= 32 ? 2 : 1;
+      small = 0;
+      chains = chains2 = 1;
+      tiles = Tp <= 16 ? 4 : Tp <= 32 ? 2 : 1;
     }
   }
-  __device__ uint32_t first(int g, int b) const { return (g * nbuf + b) * chains * n1; }
-  __device__ uint32_t second(int g, int b) const { return (groups * nbuf * chains + (g * nbuf + b) * tiles) * n1; }
+  __device__ uint32_t first(int g, int b) const { return (g * nbuf + b) * (chains + small) * Tp; }
+  __device__ uint32_t second(int g, int b) const {   // fp32: tiles * (chains2 + small) of at least 8
+    return small ? first(g, b) : (groups * nbuf * chains + (g * nbuf + b) * tiles * chains2) * Tp;
+  }
   __device__ int columns() const {
-    const int c = groups * nbuf * (chains + tiles) * n1;
+    const int c = groups * nbuf * (chains + small + (small ? 0 : tiles * chains2)) * Tp;
     return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512;
+  }
+  // Steps to a chain where `all` are dealt to n chains.
+  static __device__ int each(int all, int n) {
+    const int k = (all + n - 1) / n;
+    return k > kFewShort ? k : kFewShort;
   }
 };
 
@@ -355,8 +372,8 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   uint8_t* const hbuf = low + C::low_bytes();
   const FewExpertParams& e = p.e;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n1 = C::PARTS * p.Tp;                       // columns of an accumulator
-  const FewAcc acc(n1, FP32, (e.D + C::BK - 1) / C::BK);
+  const int n1 = C::PARTS * p.Tp;                       // rows of tokens in a step
+  const FewAcc acc(p.Tp, FP32, (e.D + C::BK - 1) / C::BK);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); mbar_init(&parted[i], 4); }
@@ -379,7 +396,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
   const int KB = (e.D + C::BK - 1) / C::BK;             // 128-byte steps of product 1
-  const int per = (KB + acc.chains - 1) / acc.chains;   // of them to an accumulator
+  const int per = FP32 ? FewAcc::each(KB, acc.chains) : KB;   // of them to an accumulator
   const int nO = p.Op / 128;
   constexpr int TU = GLU ? 4 : 8;                       // units of a product-1 tile
   constexpr int UB = GLU ? 4096 : 2048;                 // bytes of one in a step
@@ -475,25 +492,31 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
       };
       bool ok = true;
       const uint64_t wide_row = umma_desc_k_sw128(0), unit_row = umma_desc_k_narrow(0, C::TAIL);
-      const uint32_t id1 = umma_idesc(C::FORMAT, 128, (uint32_t)n1), id1l = umma_idesc(C::FORMAT, 128, (uint32_t)p.Tp);
-      // 32 bytes of K: weights [hi | lo] against token rows [hi; lo]
-      auto step = [&](uint32_t d, uint32_t dl, uint64_t a, uint64_t al, uint64_t b, uint32_t id, uint32_t idl, uint32_t more) {
-        if constexpr (FP32) {
-          umma_tf32(d, a, b, id, more);
-          umma_tf32(dl, al, b, idl, 1u);   // with the other small products
-        } else {
-          umma_f16(d, a, b, id, more);
-        }
+      const uint32_t id1 = umma_idesc(C::FORMAT, 128, (uint32_t)p.Tp);
+      // 32 bytes of K, fp32: weights a and their rests al against the high parts of tokens or activations, b, and the low
+      // parts, `lows` 16-byte units behind: into a chain's sum d, and the small products into ds
+      auto step = [&](uint32_t d, uint32_t ds, uint64_t a, uint64_t al, uint64_t b, uint32_t lows, uint32_t id, uint32_t more,
+                      uint32_t more_small) {
+        umma_tf32_twice(d, ds, a, b, b + lows, id, more, more_small);
+        umma_tf32(ds, al, b, id, 1u);
       };
-      // The same for product 2, with the activations' np rows of high parts, then np of low parts; bf16: both into one sum
-      // (no further columns), by two products that read the weights once.
-      auto step2 = [&](uint32_t d, int np, uint64_t a, uint64_t al, uint64_t b, uint32_t id, uint32_t idl, uint32_t more) {
-        if constexpr (FP32) step(d, d + np, a, al, b, id, idl, more);
-        else umma_f16_twice(d, a, b, b + np * 8, id, more);
+      // The same for product 2: step `at` of slice s of the run's hidden rows, whose activations are np rows of high parts,
+      // then np of low parts.  bf16: both parts into one sum (no further columns), by two products that read the weights once.
+      // fp32: the slice is number `nth` of a chain, whose sum lies `chain` columns behind d.
+      auto step2 = [&](uint32_t d, int s, uint32_t chain, int nth, int np, uint64_t a, uint64_t al, uint64_t b, uint32_t id, int at) {
+        if constexpr (FP32)
+          step(d + chain, d + acc.chains2 * np, a, al, b, np * 8, id, (nth | at) ? 1u : 0u, (s | at) ? 1u : 0u);
+        else
+          umma_f16_twice(d, a, b, b + np * 8, id, (s | at) ? 1u : 0u);
       };
       while (ok) {
         FewWalk again = walk;
         int off = 0, runs = 0;
+        if constexpr (FP32) {   // the batch before has been read: its product 2 in this product 1's place
+          for (int g = 0; ok && g < acc.groups; ++g)
+            if (j2[g] > 0) ok = serving_wait(&acc2_empty[g * 2], (j2[g] - 1) & 1, status, kFewKernelId, kFewWaitNs);
+          tc_fence_after_sync();
+        }
         for (; ok && walk.next(plan, hrows, C::HPARTS, C::UPS, off, r); ++runs) {
           for (int u0 = 0; ok && u0 < r.units; u0 += TU, ++i1) {
             const int nu = r.units - u0 < TU ? r.units - u0 : TU, pack = pack_of(nu);
@@ -501,6 +524,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             if (!(ok = serving_wait(&acc1_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
             uint32_t dc = tmem + acc.first(g, b);
+            [[maybe_unused]] const uint32_t ds = dc + acc.chains * p.Tp;
             int at = 0;   // steps of the chain
             for (int kb = 0; kb < KB; kb += pack) {
               if (!(ok = serving_wait(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
@@ -509,9 +533,12 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               const int n = KB - kb < pack ? KB - kb : pack;
               uint64_t da = desc_at(wide_row, w), dl = desc_at(wide_row, wl), dx = desc_at(wide_row, x);
               for (int kk = 0; kk < n; ++kk, da += nu * UB / 16, dl += nu * UB / 16, dx += n1 * 8) {
-                if (FP32 && at == per) { at = 0; dc += n1; }   // the next chain
+                if (FP32 && at == per) { at = 0; dc += p.Tp; }   // the next chain
 #pragma unroll
-                for (int k = 0; k < 4; ++k) step(dc, dc + p.Tp, da + 2 * k, dl + 2 * k, dx + 2 * k, id1, id1l, (at | k) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) {
+                  if constexpr (FP32) step(dc, ds, da + 2 * k, dl + 2 * k, dx + 2 * k, p.Tp * 8, id1, (at | k) ? 1u : 0u, (kb | kk | k) ? 1u : 0u);
+                  else umma_f16(dc, da + 2 * k, dx + 2 * k, id1, (at | k) ? 1u : 0u);
+                }
                 ++at;
               }
               umma_commit(&empty[stage]);
@@ -533,26 +560,31 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
           again.next(plan, hrows, C::HPARTS, C::UPS, off, r);
           const int slices = r.units / C::UPS, tail = r.units % C::UPS;
           const uint32_t hrow = C::HPARTS * r.np * 128;   // bytes of a slice of activations
-          const uint32_t id2 = umma_idesc(C::FORMAT, 128, (uint32_t)(C::PARTS * r.np)), id2l = umma_idesc(C::FORMAT, 128, (uint32_t)r.np);
+          const uint32_t id2 = umma_idesc(C::FORMAT, 128, (uint32_t)r.np);
+          [[maybe_unused]] const int each = FewAcc::each(slices + (tail ? 1 : 0), acc.chains2);
           const int share = tail ? UPT / tail : 1;
           for (int i0 = 0, g = 0; ok && i0 < nO; i0 += acc.tiles, g = acc.groups - 1 - g) {
             const int nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
             const int j = j2[g]++, b = j & (acc.nbuf - 1);
             if (!(ok = serving_wait(&acc2_empty[g * 2 + b], ((j / acc.nbuf) & 1) ^ 1u, status, kFewKernelId, kFewWaitNs))) break;
             tc_fence_after_sync();
-            const uint32_t d = tmem + acc.second(g, b), dn = C::PARTS * r.np;
+            const uint32_t d = tmem + acc.second(g, b), dn = (acc.chains2 + acc.small) * r.np;
             const uint32_t h0 = smem_u32(hbuf) + r.h * 128;
-            for (int s = 0; ok && s < slices; ++s)
+            uint32_t chain = 0;
+            int nth = 0;
+            for (int s = 0; ok && s < slices; ++s) {
               for (int i = 0; i < nt; ++i) {
                 if (!(ok = serving_wait(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
                 tc_fence_after_sync();
                 const uint64_t da = desc_at(wide_row, smem_u32(smem + stage * SB)), dl = desc_at(wide_row, smem_u32(low) + lo * kFewTile);
                 const uint64_t dh = desc_at(wide_row, h0 + s * hrow);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) step2(d + i * dn, r.np, da + 2 * k, dl + 2 * k, dh + 2 * k, id2, id2l, (s | k) ? 1u : 0u);
+                for (int k = 0; k < 4; ++k) step2(d + i * dn, s, chain, nth, r.np, da + 2 * k, dl + 2 * k, dh + 2 * k, id2, k);
                 umma_commit(&empty[stage]);
                 next();
               }
+              if (FP32 && ++nth == each) { nth = 0; chain += r.np; }
+            }
             for (int i = 0; ok && tail && i < nt; i += share) {
               const int n = nt - i < share ? nt - i : share;
               if (!(ok = serving_wait(&ready[stage], phase, status, kFewKernelId, kFewWaitNs))) break;
@@ -564,7 +596,7 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
                 for (int u = 0; u < tail; ++u, da += 8 * C::TAIL, dl += 8 * C::TAIL)
 #pragma unroll
                   for (int k = 0; k < KS; ++k)
-                    step2(d + (i + m) * dn, r.np, da + 2 * k, dl + 2 * k, dh + 2 * (u * KS + k), id2, id2l, (slices | u | k) ? 1u : 0u);
+                    step2(d + (i + m) * dn, slices, chain, nth, r.np, da + 2 * k, dl + 2 * k, dh + 2 * (u * KS + k), id2, u | k);
               umma_commit(&empty[stage]);
               next();
             }
@@ -614,19 +646,16 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
             uint32_t v[16];
             tmem_ld16(base + c, v);
             if constexpr (FP32) {
-              uint32_t l[16];
-              tmem_ld16(base + p.Tp + c, l);
+              uint32_t h[16];
+              tmem_ld16(base + acc.chains * p.Tp + c, h);   // the small products
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(l[i]));
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(h[i]));
               for (int q1 = 1; q1 * per < KB; ++q1) {
-                uint32_t h[16];
-                tmem_ld16(base + q1 * n1 + c, h);
-                tmem_ld16(base + q1 * n1 + p.Tp + c, l);
+                tmem_ld16(base + q1 * p.Tp + c, h);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  v[i] = __float_as_uint(__uint_as_float(v[i]) + (__uint_as_float(h[i]) + __uint_as_float(l[i])));
+                for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(h[i]));
               }
             } else {
               tmem_ld_wait();
@@ -681,13 +710,14 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
         // product 2: this CTA's part of the expert's result.  A group of tiles always belongs to the same epilogue
         // group, so a cut run's later pieces are added by the thread that wrote the first.
         const int mine = (int)blockIdx.x - few_cta((long long)r.place * plan.groups, walk.U, walk.G);
+        const int all = (r.units + C::UPS - 1) / C::UPS, each = FewAcc::each(all, acc.chains2);
         float* dst = p.part + (long long)(plan.part0[r.place] + mine * r.tokens) * p.Op + q * 32 + lane;
         for (int i0 = g * acc.tiles; ok && i0 < nO; i0 += acc.groups * acc.tiles, ++j2) {
           const int b = j2 & (acc.nbuf - 1), nt = nO - i0 < acc.tiles ? nO - i0 : acc.tiles;
           ok = mbar_wait_warp(&acc2_full[g * 2 + b], (j2 / acc.nbuf) & 1, status, kFewKernelId, kFewWaitNs);
           tc_fence_after_sync();
           for (int i = 0; i < nt; ++i) {
-            const uint32_t base = lane_addr + acc.second(g, b) + i * C::PARTS * r.np;
+            const uint32_t base = lane_addr + acc.second(g, b) + i * (acc.chains2 + acc.small) * r.np;
             for (int c = 0; c < r.tokens; c += 16) {
               __syncwarp();
               uint32_t v[16];
@@ -698,10 +728,16 @@ few_experts_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant
               tmem_ld16(base + c, v);
               if constexpr (FP32) {
                 uint32_t l[16];
-                tmem_ld16(base + r.np + c, l);
+                tmem_ld16(base + acc.chains2 * r.np + c, l);   // the small products
                 tmem_ld_wait();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(l[j]));
+                for (int q2 = 1; q2 * each < all; ++q2) {
+                  tmem_ld16(base + q2 * r.np + c, l);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(l[j]));
+                }
               } else {
                 tmem_ld_wait();
               }

@@ -426,6 +426,20 @@ __device__ __forceinline__ uint64_t umma_desc_k_narrow(uint32_t smem_addr, uint3
   return d;
 }
 
+// D0 (+)= A B0^T, D1 (+)= A B1^T, kind::tf32: two products with the same A, which
+// the second one finds in the collector buffer.
+__device__ __forceinline__ void umma_tf32_twice(uint32_t tmem_d0, uint32_t tmem_d1, uint64_t adesc, uint64_t bdesc0, uint64_t bdesc1,
+                                                uint32_t idesc, uint32_t accumulate0, uint32_t accumulate1) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32.collector::a::fill [%0], %2, %3, %5, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32.collector::a::lastuse [%1], %2, %4, %5, q;\n\t}" ::"r"(tmem_d0), "r"(tmem_d1),
+      "l"(adesc), "l"(bdesc0), "l"(bdesc1), "r"(idesc), "r"(accumulate0), "r"(accumulate1)
+      : "memory");
+}
+
 // Instruction descriptor for dense MMA with fp32 accumulation, both operands
 // K-major.  ab_format: 1 = BF16 (kind::f16), 2 = TF32 (kind::tf32).
 //   bits [4,6) D format (1 = F32); [7,10) A format; [10,13) B format;

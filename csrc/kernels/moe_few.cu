@@ -479,15 +479,14 @@ FewExpertPlan plan_few_experts(const FewExpertParams& p, int sms) {
     r.route = p.T == 1 && p.E <= kFewOwnExperts && (long long)p.E * p.D * eb <= kFewOwnBytes;
     return r;
   }
-  // fp32: so many tokens at a time that no accumulator takes more than 352 of K, if 16 can (D 4928), since it is cut at each
-  // step (64 tokens, 4 experts 4096 x 1024 SwiGLU: error 6.6e-6 and 130 us all at once, 1.6e-6 and 371 to
-  // 480 us by 16); the weights are then read again for each.
+  // fp32: so many tokens at a time that no accumulator takes more than 160 of K, if 16 can (D 4960), since it is cut at each
+  // step: 64 tokens to a D of 1120, 48 to 1440, 32 to 2400.  The weights are then read again for each (64 tokens, 4 experts
+  // 4096 x 1024 SwiGLU: error 0.9e-6 and 484 us by 16; all at once, with chains of 1024, it was 6.6e-6 and 130 us).
   r.slice = p.T;
   if (!p.bf16) {
     const int steps = (p.D + 31) / 32;
     auto fits = [&](int T) {
-      const int n1 = 2 * ((T + 15) / 16 * 16);
-      return steps <= FewAcc(n1, true, steps).chains * kFewChain;
+      return steps <= FewAcc((T + 15) / 16 * 16, true, steps).chains * kFewChain;
     };
     if (!fits(p.T)) r.slice = std::min(p.T, fits(32) ? 32 : 16);
   }

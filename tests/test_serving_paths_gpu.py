@@ -369,3 +369,18 @@ def test_first_calls_inside_captures():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     p = subprocess.run([sys.executable, "-c", FIRST_IN_A_CAPTURE], cwd=root, capture_output=True, text=True, timeout=300)
     assert p.returncode == 0 and "all captured" in p.stdout, p.stderr[-2000:]
+
+
+@pytest.mark.parametrize("T,D,E,k,F,act", [(22, 1024, 16, 4, 5888, "swiglu"), (23, 1046, 24, 5, 4672, "swiglu"), (5, 1792, 8, 4, 8000, "swiglu"),
+                                           (16, 2048, 8, 2, 4096, "gelu"), (40, 1440, 8, 3, 2500, "swiglu"), (64, 1120, 6, 2, 4000, "silu"),
+                                           (64, 4096, 3, 2, 1500, "swiglu"), (12, 640, 2, 1, 9000, "swiglu"), (1, 4960, 8, 8, 2000, "swiglu")])
+def test_fp32_layers_have_fp32_sums(T, D, E, k, F, act):
+    """The tensor core cuts its sums, 2e-6 of them for each 1024 of K, which one chain of K may not show: no chain of either
+    product is longer than 160.  SwiGLU multiplies two of them.  Beside that, numbers in parts are 2^-22 off, and a few dozen
+    sums of chains, tokens and choices are rounded."""
+    a = _make(T, D, E, F, D, act, FP32, seed=D)
+    assert _plan(a, k, act)["path"] == ("rows" if k * T * 4 * F * (D + (2 if act == "swiglu" else 1) * D) <= 540e6 else "tensor")
+    out, _, _ = _check(a, k, act, "none")
+    want = moe64(**a, top_k=k, act=act, gate_mode="none")[0]
+    once = 2.1 if act == "swiglu" else 1.1
+    check_norm(out, want, 2e-6 / 1024 * 160 * (once + 1) + 2.0 ** -22 * (once + 1) + 8 * U)
