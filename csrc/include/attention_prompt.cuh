@@ -1,0 +1,80 @@
+// What the kernels of attention over whole prompts share: which rows of which
+// sequence a CTA has, and numbers of values that are not finite.
+#pragma once
+
+#include "attention.h"
+#include "serving_device.cuh"
+#include "sm100_ptx.cuh"
+
+namespace raiccl {
+
+// A sequence's tokens in q and in k, v.
+struct PromptSeq {
+  int q0, nq, k0, nk;
+};
+
+// Ends outside of the tensors, or before their beginnings, are recorded and cut.
+__device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
+  const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1), k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
+  PromptSeq s;
+  s.q0 = q0 < 0 ? 0 : q0 > p.Nq ? (int)p.Nq : q0;
+  s.k0 = k0 < 0 ? 0 : k0 > p.Nk ? (int)p.Nk : k0;
+  const int qe = q1 < s.q0 ? s.q0 : q1 > p.Nq ? (int)p.Nq : q1, ke = k1 < s.k0 ? s.k0 : k1 > p.Nk ? (int)p.Nk : k1;
+  s.nq = qe - s.q0;
+  s.nk = ke - s.k0;
+  if (s.q0 != q0 || qe != q1) record_status(p.status, kBoundsViolation, kPromptKernelId, q1, p.Nq);
+  if (s.k0 != k0 || ke != k1) record_status(p.status, kBoundsViolation, kPromptKernelId, k1, p.Nk);
+  return s;
+}
+
+// The tile `index` of all sequences' tiles of `tokens` tokens of q; false behind the last.  A whole warp calls it.
+// Within a sequence the last tile, which sees the most keys, comes first.
+__device__ __forceinline__ bool prompt_tile(const PromptParams& p, int index, int tokens, PromptSeq& s, int& tile) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    PromptSeq mine{};
+    if (b0 + lane < p.B) mine = prompt_seq(p, b0 + lane);
+    const int n = (mine.nq + tokens - 1) / tokens;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const uint32_t in = __ballot_sync(0xffffffffu, index < before + sum);
+    if (in) {
+      const int at = __ffs(in) - 1;
+      s.q0 = __shfl_sync(0xffffffffu, mine.q0, at);
+      s.nq = __shfl_sync(0xffffffffu, mine.nq, at);
+      s.k0 = __shfl_sync(0xffffffffu, mine.k0, at);
+      s.nk = __shfl_sync(0xffffffffu, mine.nk, at);
+      tile = before + __shfl_sync(0xffffffffu, sum, at) - 1 - index;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return false;
+}
+
+// Keys that row `token` of q sees.
+__device__ __forceinline__ int prompt_visible(const PromptParams& p, const PromptSeq& s, int token) {
+  if (!p.causal) return s.nk;
+  const int n = s.nk - s.nq + token + 1;
+  return n < 0 ? 0 : n;
+}
+
+// Values that are not finite must not reach rows that do not see them, but a
+// product adds 0 * NaN there.  They go into the products as zeros, and for each
+// kind and dimension the first key that has one is kept; a row sees a prefix of
+// the keys, so that is enough to put them back.  first[0]: NaN, [1]: +inf, [2]: -inf.
+__device__ __forceinline__ int odd_kind(float v) { return v != v ? 0 : v > 0.f ? 1 : 2; }
+
+template <int D>
+__device__ __forceinline__ float put_back_odd(const int (*first)[D], int d, int visible, float v) {
+  const bool nan = first[0][d] < visible, up = first[1][d] < visible, down = first[2][d] < visible;
+  if (nan || (up && down)) return NAN;
+  return up ? INFINITY : down ? -INFINITY : v;
+}
+
+}  // namespace raiccl

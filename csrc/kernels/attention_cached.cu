@@ -1,0 +1,793 @@
+// Attention of one new token of each sequence over the paged cache in 4 bits.
+//
+//   z_j = scale q . k_j,   out = sum_j exp(z_j - m) v_j / sum_j exp(z_j - m)
+//
+// in one pass over the cache, with the running maximum m and sum l of a softmax.
+// The floor is the cache's own bytes, 9/16 of a byte a number.
+//
+// Work.  Tiles of 32 tokens of one sequence and one key head, in the order of
+// sequences and heads, are dealt to the CTAs in equal contiguous shares, and a
+// CTA's share to its warps.  A warp is on its own from the first tile to the
+// last: it copies its tiles to its own ring in shared memory (cp.async.bulk),
+// and meets no other warp before its share is done.  What it has of a sequence
+// whose tiles others have too is joined then, in a fixed order: within the CTA
+// through shared memory, between CTAs by a second, small kernel.
+//
+// Products.  Tokens are the 16-row operand of mma.sync (m16n8k16, f16, fp32
+// sums), the group's query heads its eight columns: the operand that comes from
+// the cache goes straight from its 4 bits into registers.  A lane takes D / 4
+// consecutive numbers of a key (the dimensions' order within the product is
+// free) and D / 8 of each of four values, so that both are read as they lie.  A
+// code times its scale has at most 6 bits and is exact in f16.  tcgen05 has no
+// mixed product of f16 by 4 bits with scales along the rows; the operand would
+// have to be written back to shared memory, twice the bytes that a tile reads.
+//
+// The sums S^T = K Q^T come out with tokens as rows; movmatrix turns two 8 x 8
+// blocks of exp(S) into the other operand of out^T = V^T P^T.
+//
+// Roundings.  Queries are scaled by a power of two and held in f16 (bf16 queries
+// exactly but for numbers 2^-14 below the row's largest, which lose bits below
+// 2^-25 of it), fp32 queries as two f16 parts (2^-22).  Probabilities go into
+// the second product in f16 (2^-12 of each, unbiased, small against a bf16
+// result's own 2^-9), for fp32 results in two parts.  Maxima, sums and outputs
+// are fp32.  Tensor-core sums are cut rather than rounded, so for fp32 results
+// they leave it every 32 tokens.
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <atomic>
+#include <stdexcept>
+
+#include "attention.h"
+#include "serving.h"
+#include "serving_device.cuh"
+#include "sm100_ptx.cuh"
+
+namespace raiccl {
+
+constexpr int kCachedTile = 32;
+constexpr unsigned long long kCachedWaitNs = 2000000000ull;
+// Probabilities are exp2(z - m + 7) and m follows the maximum once that passes 15: f16 holds them (below 2^15), and small
+// ones keep their bits down to 2^-21 of the largest.
+constexpr float kCachedHead = 7.f, kCachedRoom = 15.f;
+
+template <int D, int NT, int PARTS>
+struct Cached {
+  static constexpr int WARPS = 8, THREADS = 32 * WARPS;
+  static constexpr int HEADS = 8 * NT;                       // query heads of a chunk at most
+  static constexpr int CODES = kCachedTile * D / 2, SCALES = kCachedTile * D / 16;
+  static constexpr int STAGE = 2 * (CODES + SCALES);         // K codes, V codes, K scales, V scales
+  static constexpr int PART = HEADS * D * 4;                 // a warp's sums of a sequence that it shares
+  static constexpr int STAGES = NT == 1 ? 5 : 4;
+  static constexpr int SMEM = WARPS * (STAGES * STAGE + PART);   // a warp's last part goes into its ring, which is done then
+  static_assert(STAGES * STAGE >= PART && SMEM <= 222 * 1024, "shared memory");
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Four bytes of two codes each as f16 pairs, lower code first.
+__device__ __forceinline__ void codes_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+
+// Two e4m3 numbers (the lower sixteen bits) as an f16 pair.
+__device__ __forceinline__ uint32_t scales_f16(uint32_t two) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+  return h;
+}
+
+__device__ __forceinline__ uint32_t mul_f16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *(const uint32_t*)&h;
+}
+
+// What f16 rounding leaves of two numbers, in f16.
+__device__ __forceinline__ uint32_t rest_f16(float lo, float hi, uint32_t rounded) {
+  const float2 f = __half22float2(*(const __half2*)&rounded);
+  return pack_f16(lo - f.x, hi - f.y);
+}
+
+// Tokens of a sequence, within its row of the table.
+__device__ __forceinline__ int cached_length(const CachedParams& p, int b) {
+  const int n = __ldg(p.lengths + b);
+  const long long most = (long long)p.table_pages << p.c.page_shift;
+  return n < 0 ? 0 : (long long)n > most ? (int)most : n;
+}
+
+__device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) { return (cached_length(p, b) + kCachedTile - 1) / kCachedTile; }
+
+// CTAs that take part, the first tile of one, and the CTA of a tile.
+__device__ __forceinline__ int cached_ctas(long long tiles, int ctas, int warps) {
+  const long long most = (tiles + warps - 1) / warps;
+  return most < ctas ? (int)most : ctas;
+}
+__device__ __forceinline__ long long cached_first(long long tiles, int ctas, int c) { return tiles * c / ctas; }
+__device__ __forceinline__ int cached_cta(long long tiles, int ctas, long long tile) { return (int)(((tile + 1) * ctas - 1) / tiles); }
+
+// A sequence and chunk of heads, as a piece of the order of all tiles.
+struct CachedPiece {
+  int b, hc, n;        // tiles
+  long long first;     // its first tile
+};
+
+__device__ __forceinline__ void next_piece(const CachedParams& p, CachedPiece& s) {
+  s.first += s.n;
+  if (++s.hc < p.c.heads * p.chunks) return;
+  s.hc = 0;
+  do {
+    ++s.b;
+    s.n = s.b < p.B ? cached_tiles(p, s.b) : 1;
+  } while (s.n == 0);
+}
+
+__device__ __forceinline__ int piece_heads(const CachedParams& p, int hc, int& head) {
+  const int kv = hc / p.chunks, chunk = hc - kv * p.chunks;
+  head = kv * p.group + chunk * p.chunk;
+  const int left = p.group - chunk * p.chunk;
+  return left < p.chunk ? left : p.chunk;
+}
+
+__device__ __forceinline__ float cached_lse(float m, float l) { return (m + log2f(l)) * 0.69314718055994531f; }
+
+// Four outputs of a row from sums and the reciprocal of l.
+__device__ __forceinline__ void cached_store4(const CachedParams& p, int b, int head, int d, float4 v) {
+  const long long at = b * p.o_seq + head * p.o_head + d;
+  if (p.out_bf16) {
+    __nv_bfloat16* o = (__nv_bfloat16*)p.out + at;
+    const __nv_bfloat162 x = __floats2bfloat162_rn(v.x, v.y), y = __floats2bfloat162_rn(v.z, v.w);
+    if (p.o_vec) *(uint2*)o = make_uint2(*(const uint32_t*)&x, *(const uint32_t*)&y);
+    else { o[0] = x.x; o[1] = x.y; o[2] = y.x; o[3] = y.y; }
+  } else {
+    float* o = (float*)p.out + at;
+    if (p.o_vec) *(float4*)o = v;
+    else { o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w; }
+  }
+}
+
+// A warp's (or CTA's) piece of a sequence that is not whole: 0 it began before, 1 it ends after.
+struct CachedPart {
+  CachedPiece s;
+  int used;
+};
+
+template <int D, int NT, int PARTS>
+__global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kernel(CachedParams p) {
+  using C = Cached<D, NT, PARTS>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t full[C::WARPS][C::STAGES];
+  __shared__ int pages_ok[C::WARPS][C::STAGES];
+  __shared__ long long before[C::THREADS + 1];
+  __shared__ CachedPart part[C::WARPS][2];
+  __shared__ float2 stat[C::WARPS][2][C::HEADS];
+  __shared__ int nonempty[C::WARPS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
+  // a warp's part of a sequence: the one that began before its share, the one that ends after it
+  auto sums = [&](int w, int side) {
+    return (float*)(side == 0 ? smem + C::WARPS * C::STAGES * C::STAGE + w * C::PART : smem + w * C::STAGES * C::STAGE);
+  };
+  if (lane < C::STAGES) mbar_init(&full[warp][lane], 1);
+  fence_mbarrier_init();
+  __syncwarp();
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // ------------------------------------------------------------ all tiles, and this CTA's and this warp's
+  const int HC = p.c.heads * p.chunks, per = (p.B + C::THREADS - 1) / C::THREADS;
+  {
+    long long n = 0;
+    for (int b = tid * per; b < p.B && b < (tid + 1) * per; ++b) {
+      const int len = __ldg(p.lengths + b);
+      const long long most = (long long)p.table_pages << p.c.page_shift;
+      if (blockIdx.x == 0 && (len < 0 || (long long)len > most)) record_status(p.status, kBoundsViolation, kCachedKernelId, len, most);
+      n += cached_tiles(p, b);
+    }
+    long long sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    __shared__ long long warp_sum_of[C::WARPS];
+    if (lane == 31) warp_sum_of[warp] = sum;
+    __syncthreads();
+    long long base = 0;
+    for (int w = 0; w < warp; ++w) base += warp_sum_of[w];
+    before[tid + 1] = (base + sum) * HC;
+    if (tid == 0) before[0] = 0;
+    __syncthreads();
+  }
+  const long long tiles = before[C::THREADS];
+  if (tiles == 0) return;
+  const int ctas = cached_ctas(tiles, p.ctas, C::WARPS);
+  if ((int)blockIdx.x >= ctas) return;
+  const long long c0 = cached_first(tiles, ctas, blockIdx.x), c1 = cached_first(tiles, ctas, blockIdx.x + 1);
+  const long long u0 = c0 + (c1 - c0) * warp / C::WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
+  const int count = (int)(u1 - u0);
+  if (lane == 0) {
+    part[warp][0].used = part[warp][1].used = 0;
+    nonempty[warp] = count > 0;
+  }
+  __syncwarp();
+
+  if (count > 0) {
+    CachedPiece piece;
+    {
+      int lo = 0, hi = C::THREADS;   // before[lo] <= u0 < before[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (before[mid] <= u0) lo = mid; else hi = mid;
+      }
+      long long first = before[lo];
+      int b = lo * per, n = cached_tiles(p, b);
+      while (first + (long long)n * HC <= u0) {
+        first += (long long)n * HC;
+        n = cached_tiles(p, ++b);
+      }
+      const int hc = (int)((u0 - first) / n);
+      piece = {b, hc, n, first + (long long)hc * n};
+    }
+
+    // ---------------------------------------------------------- copies, STAGES tiles ahead
+    CachedPiece ahead = piece;
+    int issued = 0;
+    const int page_size = 1 << p.c.page_shift;
+    const bool whole = page_size >= kCachedTile;   // a tile lies in one page
+    auto issue = [&]() {
+      const long long u = u0 + issued;
+      while (u >= ahead.first + ahead.n) next_piece(p, ahead);
+      const int stage = issued % C::STAGES;
+      const int token = (int)(u - ahead.first) * kCachedTile, len = cached_length(p, ahead.b);
+      const int kv = ahead.hc / p.chunks;
+      // one copy to a lane: lanes 0 to 3 the four arrays, of the tile or of its first sixteen tokens, 4 to 7 of the others
+      const int half = (lane >> 2) & 1, what = lane & 3;
+      const int at = token + 16 * half;
+      int page = -1;
+      if (lane < 8 && at < len) {
+        page = __ldg(p.table + ahead.b * p.table_stride + (at >> p.c.page_shift));
+        if (page < 0 || page >= p.c.pages) {
+          if (what == 0) record_status(p.status, kBoundsViolation, kCachedKernelId, page, p.c.pages);
+          page = -1;
+        }
+      }
+      const uint32_t have = __ballot_sync(0xffffffffu, lane < 8 && page >= 0);
+      const int ok = (have & 1u ? 1 : 0) | (have & 16u ? 2 : 0);
+      const int rows = whole ? (ok & 1 ? kCachedTile : 0) : 16 * __popc(ok);
+      if (lane == 0) {
+        pages_ok[warp][stage] = ok;
+        mbar_arrive_expect_tx(&full[warp][stage], rows * (2 * (D / 2) + 2 * (D / 16)));
+      }
+      __syncwarp();
+      if (page >= 0 && lane < (whole ? 4 : 8)) {
+        const bool codes = what < 2;
+        const int width = codes ? D / 2 : D / 16;
+        const uint8_t* base = what == 0 ? p.c.k_codes : what == 1 ? p.c.v_codes : what == 2 ? p.c.k_scales : p.c.v_scales;
+        const long long row = ((((long long)page * p.c.heads + kv) << p.c.page_shift) + (at & (page_size - 1)));
+        uint8_t* dst = ring + stage * C::STAGE + (codes ? what * C::CODES : 2 * C::CODES + (what - 2) * C::SCALES) + 16 * half * width;
+        bulk_load_g2s(dst, base + row * width, (whole ? kCachedTile : 16) * width, &full[warp][stage]);
+      }
+      ++issued;
+    };
+    while (issued < count && issued < C::STAGES) issue();
+
+    // ---------------------------------------------------------- tiles
+    constexpr int KS = D / 16;         // products of a row of sixteen tokens over D
+    constexpr int DM = D / 16;         // blocks of sixteen dimensions of the output
+    uint32_t bq[PARTS][NT][KS][2];
+    float mult[NT][2];                 // from sums to logits in powers of two, heads 8 nt + 2t and 2t + 1
+    float m[NT][2], l[NT][2];
+    float o[DM][NT][4];
+    int head0 = 0, heads = 0;
+
+    auto begin = [&]() {
+      heads = piece_heads(p, piece.hc, head0);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int h = 8 * nt + g;
+        float x[D / 4];
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) x[i] = 0.f;
+        if (h < heads) {
+          const long long at = piece.b * p.q_seq + (head0 + h) * p.q_head + t * (D / 4);
+          if (p.bf16) {
+            const __nv_bfloat16* q = (const __nv_bfloat16*)p.q + at;
+            if (p.q_vec) {
+#pragma unroll
+              for (int i = 0; i < D / 4; i += 8) {
+                float f[8];
+                unpack16<__nv_bfloat16>(*(const uint4*)(q + i), f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[i + j] = f[j];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < D / 4; ++i) x[i] = __bfloat162float(q[i]);
+            }
+          } else {
+            const float* q = (const float*)p.q + at;
+            if (p.q_vec) {
+#pragma unroll
+              for (int i = 0; i < D / 4; i += 4) *(float4*)(x + i) = *(const float4*)(q + i);
+            } else {
+#pragma unroll
+              for (int i = 0; i < D / 4; ++i) x[i] = q[i];
+            }
+          }
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the power of two at or below the largest (1 for zeros and infinities), and its reciprocal
+        uint32_t e = __float_as_uint(top) >> 23;
+        if (e == 0 || e == 255) e = 127;
+        if (e > 253) e = 253;
+        const float down = __uint_as_float((254u - e) << 23);
+        const float up = __uint_as_float(e << 23) * p.c.k_unit * p.scale * 1.44269504088896341f;
+        mult[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t);
+        mult[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+#pragma unroll
+        for (int i = 0; i < D / 4; i += 2) {
+          const float a = x[i] * down, b = x[i + 1] * down;
+          const uint32_t w = pack_f16(a, b);
+          bq[0][nt][i / 4][(i / 2) & 1] = w;
+          if constexpr (PARTS == 2) bq[1][nt][i / 4][(i / 2) & 1] = rest_f16(a, b, w);
+        }
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < DM; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[i][nt][j] = 0.f;
+    };
+
+    // The piece's end, for this warp: written where all its tiles were this warp's, else left for the join.
+    auto finish = [&]() {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float s = l[nt][j];
+          s += __shfl_xor_sync(0xffffffffu, s, 4);
+          s += __shfl_xor_sync(0xffffffffu, s, 8);
+          s += __shfl_xor_sync(0xffffffffu, s, 16);
+          l[nt][j] = s;
+        }
+      const bool early = piece.first < u0, late = piece.first + piece.n > u1;
+      if (!early && !late) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int h = 8 * nt + 2 * t + j;
+            if (h >= heads) continue;
+            const float s = l[nt][j], r = s == 0.f ? 0.f : p.c.v_unit / s;
+#pragma unroll
+            for (int i = 0; i < DM; i += 2)
+              cached_store4(p, piece.b, head0 + h, g * (D / 8) + 2 * i,
+                            make_float4(o[i][nt][j] * r, o[i][nt][j + 2] * r, o[i + 1][nt][j] * r, o[i + 1][nt][j + 2] * r));
+            if (p.lse != nullptr && g == 0) p.lse[(long long)piece.b * p.Hq + head0 + h] = cached_lse(m[nt][j], s);
+          }
+        return;
+      }
+      const int side = early ? 0 : 1;
+      if (lane == 0) part[warp][side] = {piece, 1};
+      float* const at = sums(warp, side);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int h = 8 * nt + 2 * t + j;
+          if (g == 0) stat[warp][side][h] = make_float2(m[nt][j], l[nt][j]);
+#pragma unroll
+          for (int i = 0; i < DM; i += 2)
+            *(float4*)(at + h * D + g * (D / 8) + 2 * i) =
+                make_float4(o[i][nt][j], o[i][nt][j + 2], o[i + 1][nt][j], o[i + 1][nt][j + 2]);
+        }
+    };
+
+    begin();
+    int done = 0;
+    for (; done < count; ++done) {
+      const long long u = u0 + done;
+      if (u >= piece.first + piece.n) {
+        finish();
+        next_piece(p, piece);
+        begin();
+      }
+      const int stage = done % C::STAGES;
+      if (!mbar_wait_warp(&full[warp][stage], (done / C::STAGES) & 1, p.status, kCachedKernelId, kCachedWaitNs)) break;
+      const uint8_t* const s = ring + stage * C::STAGE;
+      const int ok = pages_ok[warp][stage];
+      const int left = cached_length(p, piece.b) - (int)(u - piece.first) * kCachedTile;
+      const bool all = left >= kCachedTile && (whole ? ok & 1 : ok == 3);
+      auto valid = [&](int row) { return all || (row < left && (ok >> (whole ? 0 : row >> 4) & 1)); };
+      if (ok != 0) {
+        float z[2][NT][4];
+        // -------------------------------------------------- S^T = K Q^T
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[mt][nt][j] = 0.f;
+          uint32_t w[2][D / 32], sc[2][D / 64];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int row = 16 * mt + 8 * r + g;
+            if constexpr (D == 128) {
+              const uint4 v = *(const uint4*)(s + row * 64 + 16 * t);
+              w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
+              const uint32_t two = scales_f16(*(const uint16_t*)(s + 2 * C::CODES + row * 8 + 2 * t));
+              sc[r][0] = __byte_perm(two, two, 0x1010);
+              sc[r][1] = __byte_perm(two, two, 0x3232);
+            } else {
+              const uint2 v = *(const uint2*)(s + row * 32 + 8 * t);
+              w[r][0] = v.x; w[r][1] = v.y;
+              const uint32_t two = scales_f16(s[2 * C::CODES + row * 4 + t]);
+              sc[r][0] = __byte_perm(two, two, 0x1010);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            uint32_t lo[4], hi[4];
+            codes_f16(w[0][j], lo);
+            codes_f16(w[1][j], hi);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              lo[i] = mul_f16(lo[i], sc[0][j / 2]);
+              hi[i] = mul_f16(hi[i], sc[1][j / 2]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t a[4] = {lo[2 * k], hi[2 * k], lo[2 * k + 1], hi[2 * k + 1]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = PARTS - 1; q >= 0; --q) mma_f16(z[mt][nt], a, bq[q][nt][2 * j + k][0], bq[q][nt][2 * j + k][1]);
+            }
+          }
+        }
+        // -------------------------------------------------- softmax
+        // x = z - m by one fma: off by a rounding of the difference, not of the logit
+        float x[2][NT][4];
+        bool grow = false;
+        auto below = [&]() {
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                x[mt][nt][j] = valid(16 * mt + 8 * (j >> 1) + g) ? fmaf(z[mt][nt][j], mult[nt][j & 1], -m[nt][j & 1]) : -INFINITY;
+                grow |= x[mt][nt][j] > kCachedRoom;
+              }
+        };
+        below();
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float top = -INFINITY;
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                  if (valid(16 * mt + 8 * r + g)) top = fmaxf(top, z[mt][nt][j + 2 * r] * mult[nt][j]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              const float now = fmaxf(m[nt][j], top - kCachedHead);
+              const float shrink = now == -INFINITY ? 1.f : exp2_fast(m[nt][j] - now);
+              m[nt][j] = now;
+              l[nt][j] *= shrink;
+#pragma unroll
+              for (int i = 0; i < DM; ++i) {
+                o[i][nt][j] *= shrink;
+                o[i][nt][j + 2] *= shrink;
+              }
+            }
+          below();
+        }
+        uint32_t bp[PARTS][2][NT][2];
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              e[j] = exp2_fast(x[mt][nt][j]);
+              l[nt][j & 1] += e[j];
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const uint32_t h = pack_f16(e[2 * r], e[2 * r + 1]);
+              bp[0][mt][nt][r] = transpose8(h);
+              if constexpr (PARTS == 2) bp[1][mt][nt][r] = transpose8(rest_f16(e[2 * r], e[2 * r + 1], h));
+            }
+          }
+        // -------------------------------------------------- out^T += V^T P^T
+        // words of four tokens; pairs of tokens to one register by their nibbles
+        constexpr int WV = D / 64;     // words of a lane's D / 8 numbers
+        float fresh[PARTS == 2 ? DM : 1][NT][4];
+        if constexpr (PARTS == 2) {
+#pragma unroll
+          for (int i = 0; i < DM; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) fresh[i][nt][j] = 0.f;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+          uint32_t pair[2][2][WV], sv[2];   // [tokens 2t, 2t + 1 / + 8][even, odd dimensions]
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            uint32_t x[2][WV], byte[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int row = 16 * mt + 8 * r + 2 * t + e;
+              if constexpr (D == 128) {
+                const uint2 v = *(const uint2*)(s + C::CODES + row * 64 + 8 * g);
+                x[e][0] = v.x; x[e][1] = v.y;
+                byte[e] = s[2 * C::CODES + C::SCALES + row * 8 + g];
+              } else {
+                x[e][0] = *(const uint32_t*)(s + C::CODES + row * 32 + 4 * g);
+                byte[e] = s[2 * C::CODES + C::SCALES + row * 4 + (g >> 1)];
+              }
+              byte[e] = valid(row) ? byte[e] : 0u;   // a page's rest may hold anything
+            }
+            sv[r] = scales_f16(byte[0] | byte[1] << 8);
+#pragma unroll
+            for (int i = 0; i < WV; ++i) {
+              pair[r][0][i] = (x[0][i] & 0x0f0f0f0fu) | ((x[1][i] << 4) & 0xf0f0f0f0u);
+              pair[r][1][i] = ((x[0][i] >> 4) & 0x0f0f0f0fu) | (x[1][i] & 0xf0f0f0f0u);
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < WV; ++i) {
+            uint32_t h[2][2][4];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                codes_f16(pair[r][e][i], h[r][e]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) h[r][e][x] = mul_f16(h[r][e][x], sv[r]);
+              }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const uint32_t a[4] = {h[0][0][x], h[0][1][x], h[1][0][x], h[1][1][x]};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int q = PARTS - 1; q >= 0; --q)
+                  mma_f16(PARTS == 2 ? fresh[PARTS == 2 ? 4 * i + x : 0][nt] : o[4 * i + x][nt], a, bp[q][mt][nt][0], bp[q][mt][nt][1]);
+            }
+          }
+        }
+        if constexpr (PARTS == 2) {
+#pragma unroll
+          for (int i = 0; i < DM; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) o[i][nt][j] += fresh[i][nt][j];
+        }
+      }
+      __syncwarp();   // every lane has read the stage
+      if (issued < count) issue();
+    }
+    for (int i = done; i < issued; ++i)   // after a wait that ran out: the copies in flight land before the ring is used again
+      mbar_wait_warp(&full[warp][i % C::STAGES], (i / C::STAGES) & 1, p.status, kCachedKernelId, kCachedWaitNs);
+    finish();
+  }
+
+  // ------------------------------------------------------------ the CTA's shared pieces
+  __syncthreads();
+  for (int w = 0; w < C::WARPS; ++w)
+    for (int side = 0; side < 2; ++side) {
+      if (!part[w][side].used) continue;
+      const CachedPiece s = part[w][side].s;
+      // a piece's parts: its first one (a tail, or the head of the CTA's first warp), then the heads of the warps behind it
+      bool first = side == 1;
+      if (side == 0) {
+        first = true;
+        for (int v = 0; v < w; ++v) first &= !nonempty[v];
+      }
+      if (!first) continue;
+      int head0;
+      const int heads = piece_heads(p, s.hc, head0);
+      const bool early = s.first < c0, late = s.first + s.n > c1;
+      for (int e = tid; e < heads * (D / 4); e += C::THREADS) {
+        const int h = e / (D / 4), d = 4 * (e - h * (D / 4));
+        float top = stat[w][side][h].x;
+        int end = w + 1;
+        for (; end < C::WARPS; ++end) {
+          if (!nonempty[end]) continue;
+          if (!part[end][0].used || part[end][0].s.first != s.first) break;
+          top = fmaxf(top, stat[end][0][h].x);
+        }
+        float l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int x = w; x < end; ++x) {
+          if (!nonempty[x]) continue;
+          const int y = x == w ? side : 0;
+          const float2 st = stat[x][y][h];
+          const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
+          const float4 a = *(const float4*)(sums(x, y) + h * D + d);
+          l = fmaf(st.y, f, l);
+          v.x = fmaf(a.x, f, v.x); v.y = fmaf(a.y, f, v.y); v.z = fmaf(a.z, f, v.z); v.w = fmaf(a.w, f, v.w);
+        }
+        if (!early && !late) {
+          const float r = l == 0.f ? 0.f : p.c.v_unit / l;
+          cached_store4(p, s.b, head0 + h, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+          if (p.lse != nullptr && d == 0) p.lse[(long long)s.b * p.Hq + head0 + h] = cached_lse(top, l);
+        } else {
+          const long long at = ((long long)blockIdx.x * 2 + (early ? 0 : 1)) * p.chunk + h;
+          *(float4*)(p.parts + at * D + d) = v;
+          if (d == 0) p.stats[at] = make_float2(top, l);
+        }
+      }
+    }
+}
+
+// Sequences that several CTAs share, one head to a CTA; a warp takes every
+// eighth part.  Empty sequences too, which no tile stands for.
+template <int D>
+__global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p, int warps) {
+  __shared__ long long sum_of[2][8];
+  __shared__ float4 acc[8][D / 4];
+  __shared__ float2 ml[8];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int HC = p.c.heads * p.chunks, b = blockIdx.x / HC, hc = blockIdx.x - b * HC, h = blockIdx.y;
+  int head0;
+  const int heads = piece_heads(p, hc, head0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (h >= heads) return;
+  long long all = 0, ahead = 0;
+  for (int i = threadIdx.x; i < p.B; i += 256) {
+    const int n = cached_tiles(p, i);
+    all += n;
+    if (i < b) ahead += n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+  }
+  if (lane == 0) { sum_of[0][warp] = all; sum_of[1][warp] = ahead; }
+  __syncthreads();
+  all = ahead = 0;
+  for (int w = 0; w < 8; ++w) { all += sum_of[0][w]; ahead += sum_of[1][w]; }
+  const int n = cached_tiles(p, b);
+  if (n == 0) {
+    if (threadIdx.x < D / 4) cached_store4(p, b, head0 + h, 4 * threadIdx.x, make_float4(0.f, 0.f, 0.f, 0.f));
+    if (p.lse != nullptr && threadIdx.x == 0) p.lse[(long long)b * p.Hq + head0 + h] = -INFINITY;
+    return;
+  }
+  const long long tiles = all * HC, first = ahead * HC + (long long)hc * n;
+  const int ctas = cached_ctas(tiles, p.ctas, warps);
+  const int c0 = cached_cta(tiles, ctas, first), c1 = cached_cta(tiles, ctas, first + n - 1);
+  if (c0 == c1) return;
+  float m = -INFINITY, l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  const bool mine = lane < D / 4;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += 8) {
+    const long long at = ((long long)c * 2 + (c == c0 ? 1 : 0)) * p.chunk + h;
+    const float2 st = p.stats[at];
+    const float4 a = mine ? *(const float4*)(p.parts + at * D + 4 * lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float top = fmaxf(m, st.x);
+    const float f0 = m == -INFINITY ? (l == 0.f ? 0.f : NAN) : exp2_fast(m - top);
+    const float f1 = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
+    m = top;
+    l = l * f0 + st.y * f1;
+    v.x = v.x * f0 + a.x * f1; v.y = v.y * f0 + a.y * f1; v.z = v.z * f0 + a.z * f1; v.w = v.w * f0 + a.w * f1;
+  }
+  if (mine) acc[warp][lane] = v;
+  if (lane == 0) ml[warp] = make_float2(m, l);
+  __syncthreads();
+  if (warp != 0 || !mine) return;
+  m = -INFINITY;
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, ml[w].x);
+  l = 0.f;
+  v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int w = 0; w < 8; ++w) {
+    const float f = ml[w].x == -INFINITY ? (ml[w].y == 0.f ? 0.f : NAN) : exp2_fast(ml[w].x - m);
+    const float4 a = acc[w][lane];
+    l = fmaf(ml[w].y, f, l);
+    v.x = fmaf(a.x, f, v.x); v.y = fmaf(a.y, f, v.y); v.z = fmaf(a.z, f, v.z); v.w = fmaf(a.w, f, v.w);
+  }
+  const float r = l == 0.f ? 0.f : p.c.v_unit / l;
+  cached_store4(p, b, head0 + h, 4 * lane, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+  if (p.lse != nullptr && lane == 0) p.lse[(long long)b * p.Hq + head0 + h] = cached_lse(m, l);
+}
+
+// Query heads that are worked on together: up to 16 of a group, 8 where queries and probabilities have two parts.
+CachedPlan plan_cached(const CachedParams& p, int sms) {
+  CachedPlan plan{};
+  const int most = p.bf16 && p.out_bf16 ? 16 : 8;
+  plan.chunks = (p.group + most - 1) / most;
+  plan.chunk = (p.group + plan.chunks - 1) / plan.chunks;
+  plan.ctas = sms;
+  plan.parts_bytes = (long long)plan.ctas * 2 * plan.chunk * p.c.D * 4;
+  plan.stats_bytes = ((long long)plan.ctas * 2 * plan.chunk * 8 + 255) / 256 * 256;
+  return plan;
+}
+
+template <int D, int NT, int PARTS>
+static void launch_cached_as(const CachedParams& p, cudaStream_t s) {
+  using C = Cached<D, NT, PARTS>;
+  auto kern = cached_kernel<D, NT, PARTS>;
+  static std::atomic<unsigned long long> configured;   // by device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+      throw std::runtime_error("attention_cached: shared memory");
+    configured.fetch_or(bit);
+  }
+  launch_with_pdl(kern, dim3(p.ctas), dim3(C::THREADS), C::SMEM, s, true, p);
+  launch_with_pdl(cached_join_kernel<D>, dim3(p.B * p.c.heads * p.chunks, p.chunk), dim3(256), 0, s, true, p, (int)C::WARPS);
+}
+
+void launch_cached(const CachedParams& params, const CachedPlan& plan, void* workspace, cudaStream_t s) {
+  CachedParams p = params;
+  p.chunk = plan.chunk;
+  p.chunks = plan.chunks;
+  p.ctas = plan.ctas;
+  p.parts = (float*)workspace;
+  p.stats = (float2*)((char*)workspace + plan.parts_bytes);
+  const bool two = !(p.bf16 && p.out_bf16);
+  if (p.c.D == 128) {
+    if (two) launch_cached_as<128, 1, 2>(p, s);
+    else if (p.chunk > 8) launch_cached_as<128, 2, 1>(p, s);
+    else launch_cached_as<128, 1, 1>(p, s);
+  } else {
+    if (two) launch_cached_as<64, 1, 2>(p, s);
+    else if (p.chunk > 8) launch_cached_as<64, 2, 1>(p, s);
+    else launch_cached_as<64, 1, 1>(p, s);
+  }
+}
+
+}  // namespace raiccl

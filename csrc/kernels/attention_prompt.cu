@@ -1,0 +1,253 @@
+// Attention over whole prompts: packed sequences, causal or not, grouped heads.
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <stdexcept>
+
+#include "attention.h"
+#include "attention_prompt.cuh"
+#include "serving.h"
+#include "serving_device.cuh"
+#include "sm100_ptx.cuh"
+
+namespace raiccl {
+
+constexpr int kRowsTile = 128, kRowsKeys = 32;
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int D>
+struct PromptRows {
+  static constexpr int KS = D + 8, VS = D + 4;   // strides of a key's and a value's row, without conflicts of the fragments' loads
+  static constexpr int SMEM = 4 * kRowsKeys * 2 * (KS + VS);
+};
+
+template <typename T>
+__device__ __forceinline__ void load4(const void* base, long long at, bool vec, float (&x)[4]) {
+  const T* p = (const T*)base + at;
+  if (vec) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 v = *(const float4*)p;
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const uint2 v = *(const uint2*)p;
+      x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+      x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = as_float(p[i]);
+  }
+}
+
+// One CTA: 128 rows (a token and a query head of the group), eight warps of
+// sixteen; 32 keys at a time, split into two tf32 parts as they are stored.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool vec) {
+  using C = PromptRows<D>;
+  extern __shared__ __align__(16) float sm[];
+  float* const kh = sm;
+  float* const kl = kh + kRowsKeys * C::KS;
+  float* const vh = kl + kRowsKeys * C::KS;
+  float* const vl = vh + kRowsKeys * C::VS;
+  __shared__ int odd[3][D], any_odd;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  for (int i = threadIdx.x; i < 3 * D; i += 256) odd[0][i] = INT_MAX;
+  if (threadIdx.x == 0) any_odd = 0;
+  griddep_wait();
+  griddep_launch_dependents();
+  const int tokens = kRowsTile / p.group, head = blockIdx.y;
+  PromptSeq s;
+  int tile;
+  if (!prompt_tile(p, blockIdx.x, tokens, s, tile)) return;
+  const int rows = min(tokens, s.nq - tile * tokens) * p.group;
+
+  int visible[2], token[2], hq[2];
+  bool row_in[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = 16 * warp + 8 * r + g;
+    row_in[r] = row < rows;
+    token[r] = tile * tokens + row / p.group;
+    hq[r] = head * p.group + row % p.group;
+    visible[r] = row_in[r] ? min(prompt_visible(p, s, token[r]), s.nk) : 0;
+  }
+  const int keys = prompt_visible(p, s, min(tile * tokens + tokens, s.nq) - 1);
+
+  float q[2][D / 4];   // dimensions 8 j + 2 t and + 1
+#pragma unroll
+  for (int r = 0; r < 2; ++r)
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      const long long at = (long long)(s.q0 + token[r]) * p.q_token + (long long)hq[r] * p.q_head + 8 * j + 2 * t;
+      q[r][2 * j] = row_in[r] ? as_float(((const T*)p.q)[at]) : 0.f;
+      q[r][2 * j + 1] = row_in[r] ? as_float(((const T*)p.q)[at + 1]) : 0.f;
+    }
+  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[n][j] = 0.f;
+  const float mult = p.scale * 1.44269504088896341f;
+
+  for (int k0 = 0; k0 < keys; k0 += kRowsKeys) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < kRowsKeys * D / 4; i += 256) {
+      const int row = i / (D / 4), d = 4 * (i - row * (D / 4));
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (k0 + row < s.nk) {
+        const long long token = s.k0 + k0 + row;
+        load4<T>(p.k, token * p.k_token + head * p.k_head + d, vec, x);
+        load4<T>(p.v, token * p.v_token + head * p.v_head + d, vec, y);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!(fabsf(y[j]) < INFINITY)) {
+          atomicMin(&odd[odd_kind(y[j])][d + j], k0 + row);
+          any_odd = 1;
+          y[j] = 0.f;
+        }
+        split_tf32(x[j], kh[row * C::KS + d + j], kl[row * C::KS + d + j]);
+        split_tf32(y[j], vh[row * C::VS + d + j], vl[row * C::VS + d + j]);
+      }
+    }
+    __syncthreads();
+    float z[kRowsKeys / 8][4];
+#pragma unroll
+    for (int n = 0; n < kRowsKeys / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[n][j] = 0.f;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) {
+      uint32_t ah[4], al[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float h, low;
+        split_tf32(q[i & 1][2 * j + (i >> 1)], h, low);
+        ah[i] = __float_as_uint(h);
+        al[i] = __float_as_uint(low);
+      }
+#pragma unroll
+      for (int n = 0; n < kRowsKeys / 8; ++n) {
+        const float2 h = *(const float2*)(kh + (8 * n + g) * C::KS + 8 * j + 2 * t);
+        if constexpr (sizeof(T) == 4) {
+          const float2 low = *(const float2*)(kl + (8 * n + g) * C::KS + 8 * j + 2 * t);
+          mma_tf32(z[n], ah, __float_as_uint(low.x), __float_as_uint(low.y));
+          mma_tf32(z[n], al, __float_as_uint(h.x), __float_as_uint(h.y));
+        }
+        mma_tf32(z[n], ah, __float_as_uint(h.x), __float_as_uint(h.y));
+      }
+    }
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < kRowsKeys / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + 8 * n + 2 * t + (j & 1);
+        if (key < visible[j >> 1]) top[j >> 1] = fmaxf(top[j >> 1], z[n][j] * mult);
+      }
+    float now[2], shrink[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+      now[r] = fmaxf(m[r], top[r]);
+      shrink[r] = now[r] == -INFINITY ? 1.f : exp2f(m[r] - now[r]);
+      m[r] = now[r];
+      l[r] *= shrink[r];
+    }
+#pragma unroll
+    for (int n = 0; n < kRowsKeys / 8; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // a masked key adds nothing, whatever m is; a row of -inf alone is NaN, as its formula is.  One fma: off by a
+        // rounding of the difference, not of the logit.
+        const int key = k0 + 8 * n + 2 * t + (j & 1);
+        z[n][j] = key < visible[j >> 1] ? exp2f(fmaf(z[n][j], mult, -m[j >> 1])) : 0.f;
+        l[j >> 1] += z[n][j];
+      }
+    uint32_t ph[kRowsKeys / 8][4], pl[kRowsKeys / 8][4];
+#pragma unroll
+    for (int n = 0; n < kRowsKeys / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float h, low;
+        split_tf32(z[n][(i & 1) * 2 + (i >> 1)], h, low);
+        ph[n][i] = __float_as_uint(h);
+        pl[n][i] = __float_as_uint(low);
+      }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      float fresh[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < kRowsKeys / 8; ++k) {
+        const int at = (8 * k + 2 * t) * C::VS + 8 * n + g;
+        if constexpr (sizeof(T) == 4) {
+          mma_tf32(fresh, ph[k], __float_as_uint(vl[at]), __float_as_uint(vl[at + C::VS]));
+          mma_tf32(fresh, pl[k], __float_as_uint(vh[at]), __float_as_uint(vh[at + C::VS]));
+        }
+        mma_tf32(fresh, ph[k], __float_as_uint(vh[at]), __float_as_uint(vh[at + C::VS]));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[n][j] = fmaf(o[n][j], shrink[j >> 1], fresh[j]);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    if (!row_in[r]) continue;
+    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const long long at = (long long)(s.q0 + token[r]) * p.o_token + (long long)hq[r] * p.o_head;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int d = 8 * n + 2 * t + e;
+        float v = o[n][2 * r + e] * inv;
+        if (any_odd) v = put_back_odd<D>(odd, d, visible[r], v);
+        store_elem(p.out, at + d, v, sizeof(T) == 2);
+      }
+    if (p.lse != nullptr && t == 0)
+      p.lse[(long long)(s.q0 + token[r]) * p.Hq + hq[r]] = (m[r] + log2f(l[r])) * 0.69314718055994531f;
+  }
+}
+
+PromptPlan plan_prompt(const PromptParams& p, int sms) { return PromptPlan{}; }
+
+template <typename T, int D>
+static void launch_prompt_rows(const PromptParams& p, cudaStream_t s) {
+  using C = PromptRows<D>;
+  auto kern = prompt_rows_kernel<T, D>;
+  static std::atomic<unsigned long long> configured;   // by device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (!(configured.load() & bit)) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+      throw std::runtime_error("attention_prompt: shared memory");
+    configured.fetch_or(bit);
+  }
+  const int tokens = kRowsTile / p.group;
+  auto aligned = [&](const void* t, long long a, long long b) { return (((uintptr_t)t | (a * sizeof(T)) | (b * sizeof(T))) & 15) == 0; };
+  const bool vec = aligned(p.k, p.k_token, p.k_head) && aligned(p.v, p.v_token, p.v_head);
+  const dim3 grid((unsigned)((p.Nq + tokens - 1) / tokens + p.B), (unsigned)p.Hk);
+  launch_with_pdl(kern, grid, dim3(256), C::SMEM, s, true, p, vec);
+}
+
+void launch_prompt(const PromptParams& p, const PromptPlan& plan, void* workspace, cudaStream_t s) {
+  if (p.D == 128) {
+    if (p.bf16) launch_prompt_rows<__nv_bfloat16, 128>(p, s);
+    else launch_prompt_rows<float, 128>(p, s);
+  } else {
+    if (p.bf16) launch_prompt_rows<__nv_bfloat16, 64>(p, s);
+    else launch_prompt_rows<float, 64>(p, s);
+  }
+}
+
+}  // namespace raiccl

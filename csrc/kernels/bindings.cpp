@@ -103,6 +103,7 @@ void grouped_gemm(torch::Tensor A, torch::Tensor B, torch::Tensor segs, torch::T
 
 void register_moe(py::module_& m);
 void register_serving(py::module_& m);
+void register_attention(py::module_& m);
 
 // Peer put + signal: copies src (a CUDA tensor, 16-byte aligned, bytes a
 // multiple of 16) to the device address dst_ptr (own or peer mapping), then
@@ -146,6 +147,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("grid"), py::arg("timeout_ns"), py::arg("pair") = false, py::arg("swap_max") = 0);
   register_moe(m);
   register_serving(m);
+  register_attention(m);
   m.def("peer_put_signal", &peer_put_signal, py::arg("src"), py::arg("dst_ptr"), py::arg("flag_ptr"), py::arg("seq"),
         py::arg("counter"), py::arg("grid") = 64);
   m.def("peer_wait", &peer_wait, py::arg("flag_ptr"), py::arg("seq"), py::arg("timeout_ns"), py::arg("status"),

@@ -2,97 +2,16 @@
 // workspaces and launches.  A call only enqueues work on the current stream of
 // its tensors' device; outputs and workspaces come from torch's allocator on
 // that stream, so nothing is shared between calls or captured graphs.
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDACachingAllocator.h>
-#include <c10/core/AutogradState.h>
-#include <c10/core/GradMode.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
-
-#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
 
 #include "serving.h"
+#include "serving_checks.h"
 
 namespace {
 
-using OptTensor = c10::optional<torch::Tensor>;
-
-// Numbers and shapes as text.  Messages are put together from texts alone:
-// streaming a number through the C++ library that this process has loaded ends it.
-std::string text(int64_t v) { return std::to_string(v); }
-
-std::string text(at::IntArrayRef v) {
-  std::string s = "[";
-  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
-  return s + "]";
-}
-
-bool inner_contiguous(const torch::Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1; }
-
-bool is_float_type(const torch::Tensor& t) {
-  return t.scalar_type() == torch::kFloat32 || t.scalar_type() == torch::kBFloat16;
-}
-
-// A new tensor without the dispatcher's rounds, which cost the smallest calls as
-// much as a launch.
-torch::Tensor fresh(at::IntArrayRef shape, torch::ScalarType dt, const torch::Device& dev) {
-  return at::detail::empty_cuda(shape, dt, dev, c10::nullopt);
-}
-
-// [first, last) bytes that the tensor's elements lie in.
-std::pair<const char*, const char*> extent(const torch::Tensor& t) {
-  int64_t last = 0;
-  for (int64_t d = 0; d < t.dim(); ++d) {
-    if (t.size(d) == 0) return {nullptr, nullptr};
-    last += (t.size(d) - 1) * t.stride(d);
-  }
-  const char* p = (const char*)t.data_ptr();
-  return {p, p + (last + 1) * t.element_size()};
-}
-
-bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
-  const auto x = extent(a), y = extent(b);
-  return x.first < y.second && y.first < x.second;
-}
-
-// Behind a shape there may be no numbers to read: a sparse layout, a lazy zero or
-// negation, a storage that was freed (sharded parameters between their uses), or
-// a wrapper of other tensors (distributed, quantised or fake ones).
-void check_memory(const char* op, const char* name, const torch::Tensor& t) {
-  TORCH_CHECK_VALUE(t.layout() == c10::kStrided && !t.is_neg() && !t._is_zerotensor(), op, ": ", name,
-                    " must be a dense tensor, without a pending negation or zero");
-  if (t.numel() == 0 || !t.has_storage()) return;   // without one, data_ptr raises
-  int64_t last = t.storage_offset();
-  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-  TORCH_CHECK_VALUE((int64_t)t.storage().nbytes() >= (last + 1) * (int64_t)t.element_size(), op, ": ", name,
-                    " reaches behind its storage, which holds ", text((int64_t)t.storage().nbytes()), " bytes");
-  TORCH_CHECK_VALUE(t.is_meta() || t.data_ptr() != nullptr, op, ": ", name, " has no memory of its own (a wrapper of other tensors?)");
-}
-
-// Every tensor of a call lies on the CUDA device of x; checked behind the
-// shapes, types and strides, whose refusals need no device.
-void check_input(const char* op, const char* name, const torch::Tensor& t, const torch::Device& dev) {
-  TORCH_CHECK_VALUE(t.device() == dev, op, ": ", name, " must be on ", dev.str(), ", not on ", t.device().str());
-  TORCH_CHECK(!(t.requires_grad() && c10::GradMode::is_enabled()), op, ": ", name,
-              " requires a gradient, but the operator has no backward; call it under torch.no_grad()");
-  TORCH_CHECK(!(t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), op, ": ", name,
-              " carries a forward-mode tangent, but the operator has no derivative; take the primal of it");
-  check_memory(op, name, t);
-}
-
-void check_cuda(const char* op, const torch::Device& dev) {
-  TORCH_CHECK_VALUE(dev.is_cuda(), op, ": the tensors must be on a CUDA device, not on ", dev.str());
-}
-
-void check_vector(const char* op, const char* name, const torch::Tensor& t, const torch::Device& dev, at::IntArrayRef shape) {
-  check_input(op, name, t, dev);
-  TORCH_CHECK_VALUE(t.scalar_type() == torch::kFloat32 && t.sizes() == shape && t.is_contiguous(), op, ": ", name,
-                    " must be a contiguous fp32 tensor of shape ", text(shape));
-}
+using namespace raiccl;
 
 // out and residual of [rows, width]; out is allocated where none is given.
 torch::Tensor check_out(const char* op, const OptTensor& out, const OptTensor& residual, const torch::Tensor& like,
@@ -173,11 +92,6 @@ raiccl::LinearParams linear_params(const torch::Tensor& x, const torch::Tensor& 
   p.out_bf16 = out_type == torch::kBFloat16;
   p.res_bf16 = residual && residual->scalar_type() == torch::kBFloat16;
   return p;
-}
-
-// A given out was written: an operation that saved it for its backward pass has to notice.
-void written(const OptTensor& out) {
-  if (out && !out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
 }
 
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> moe_few_tokens(
@@ -355,7 +269,7 @@ std::vector<std::pair<int, int>> serving_last_fills(int64_t stages, int64_t fill
 // The device's record of the first wait that ran out in a serving operator
 // since the last call (eight words, DeviceStatus); waits for the device and
 // clears the record.
-torch::Tensor serving_status(int64_t device) {
+torch::Tensor serving_status_words(int64_t device) {
   c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   torch::Tensor words = torch::zeros({(int64_t)(sizeof(raiccl::DeviceStatus) / 4)}, torch::kInt32);
   raiccl::DeviceStatus* at = raiccl::serving_status();
@@ -377,7 +291,7 @@ void register_serving(py::module_& m) {
         py::arg("out_bf16"), py::arg("sms"));
   m.def("serving_status_address", &serving_status_address, py::arg("device"));
   m.def("serving_last_fills", &serving_last_fills, py::arg("stages"), py::arg("filled"));
-  m.def("serving_status", &serving_status, py::arg("device"));
+  m.def("serving_status", &serving_status_words, py::arg("device"));
   m.def("linear", &linear, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("act"), py::arg("residual"),
         py::arg("out"), py::arg("out_dtype"));
 }
