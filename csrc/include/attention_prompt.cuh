@@ -72,7 +72,8 @@ __device__ __forceinline__ int odd_kind(float v) { return v != v ? 0 : v > 0.f ?
 
 template <int D>
 __device__ __forceinline__ float put_back_odd(const int (*first)[D], int d, int visible, float v) {
-  const bool nan = first[0][d] < visible, up = first[1][d] < visible, down = first[2][d] < visible;
+  // v may hold some already, of tiles that all rows saw whole
+  const bool nan = v != v || first[0][d] < visible, up = v == INFINITY || first[1][d] < visible, down = v == -INFINITY || first[2][d] < visible;
   if (nan || (up && down)) return NAN;
   return up ? INFINITY : down ? -INFINITY : v;
 }

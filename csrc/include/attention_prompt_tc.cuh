@@ -1,0 +1,409 @@
+// Attention over whole prompts on the tensor cores, bf16.
+//
+// A CTA has two tiles, A and B, of 128 rows each; a row is a token and a query
+// head of one key head's group, so that a group shares every key that is read.
+// It walks over the keys in tiles of 128 and keeps the running maximum m and sum
+// l of a softmax:
+//
+//   S = Q K^T,  P = exp2(c S - m),  O = O + P V,  l = l + sum P
+//
+// with O multiplied by exp2 of the change where m has to follow a maximum that
+// grew by more than 8 (powers of two); until then P stays below 2^8, which costs
+// no accuracy.
+//
+// One warp loads (TMA), one issues the products (tcgen05.mma, 128 x 128 sums in
+// TMEM), and a warpgroup to each tile does the softmax, one row to a thread: no
+// shuffles.  P goes back into TMEM as bf16 over S, as the operand of the second
+// product.  While tile A's softmax runs, the tensor core has B's products, and
+// the other way round; S of the next step is issued behind P V of this one, so
+// its arrival tells the softmax that O may be touched too.
+//
+// TMEM: S (and P) of A and B, O of A and B, 128 columns each.
+// Two more warps look through the tiles of values that some row does not see
+// whole (attention_prompt.cuh), and clear what lies behind the sequence's end.
+#pragma once
+
+#include "attention_prompt.cuh"
+
+namespace raiccl {
+
+constexpr int kPromptThreads = 384;   // two warpgroups of softmax; loads, products, two warps for masked tiles' values
+constexpr int kPromptKeys = 128;
+constexpr unsigned long long kPromptWaitNs = 2000000000ull;
+
+template <int D>
+struct PromptTc {
+  static constexpr int HALVES = D / 64;                       // 128-byte swizzled columns of 64 dimensions
+  static constexpr int TILE = 128 * D * 2;                    // bytes of 128 rows
+  static constexpr int STAGES = 2;                            // of keys, and as many of values
+  static constexpr int SMEM = 1024 + (2 + 2 * STAGES) * TILE;
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem], kind::f16: A's rows are lanes, two 16-bit elements to a column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* desc, uint64_t* bar, int32_t x, int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(desc), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// Shared-memory descriptor of an operand whose rows (of 128 bytes, swizzled) run
+// along the product's sum: 64 columns to a row, the next 64 `apart` bytes on,
+// eight rows 1024 bytes on.
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t apart) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((apart >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)(1024u >> 4) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+
+__device__ __forceinline__ float prompt_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                 PromptParams p) {
+  using C = PromptTc<D>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* const sq = smem;                                   // tiles A and B
+  uint8_t* const sk = smem + 2 * C::TILE;
+  uint8_t* const sv = sk + C::STAGES * C::TILE;
+  __shared__ uint64_t q_full[2], k_full[C::STAGES], k_empty[C::STAGES], v_full[C::STAGES], v_empty[C::STAGES], v_raw[C::STAGES],
+      v_ready[C::STAGES], s_full[2], p_full[2], o_full[2], drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int odd[3][D], any_odd;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int tokens = 128 / p.group;                           // of a tile
+  const int head = blockIdx.x % p.Hk;
+  PromptSeq s;
+  int pair;
+  if (!prompt_tile(p, blockIdx.x / p.Hk, 2 * tokens, s, pair)) return;
+  const int token0 = pair * 2 * tokens;                       // of the sequence, A's first
+  const int tiles = token0 + tokens < s.nq ? 2 : 1;
+  const int keys = prompt_visible(p, s, min(token0 + 2 * tokens, s.nq) - 1);
+  const int steps = (keys + kPromptKeys - 1) / kPromptKeys;
+  // Values of tiles from here on, which some row does not see whole, arrive on v_raw and go through two warps first.
+  const int first_fixed = min(prompt_visible(p, s, token0), s.nk) / kPromptKeys;
+  auto fixed_phase = [&](int i) { return (uint32_t)((i - first_fixed) / C::STAGES) & 1u; };   // of v_raw and v_ready
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); mbar_init(&v_raw[i], 1); mbar_init(&v_ready[i], 2);
+    }
+    mbar_init(&drained, 1);
+    fence_mbarrier_init();
+    any_odd = 0;
+    tma_prefetch_desc(&tq); tma_prefetch_desc(&tk); tma_prefetch_desc(&tv);
+  }
+  for (int i = threadIdx.x; i < 3 * D; i += kPromptThreads) ((int*)odd)[i] = INT_MAX;
+  if (warp == 9) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+
+  // 168 registers to a thread at launch: the warpgroups of the softmax, which hold a row of S, get 208, the other 88.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+      // -------------------------------------------------------------- loads
+      if (elect_one_sync()) {
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
+        auto load_q = [&](int x) {
+          mbar_arrive_expect_tx(&q_full[x], C::HALVES * tokens * p.group * 128);
+          for (int h = 0; h < C::HALVES; ++h)
+            tma_load_3d(sq + x * C::TILE + h * 128 * 128, &tq, &q_full[x], 64 * h, head * p.group, s.q0 + token0 + x * tokens);
+        };
+        auto load = [&](uint8_t* at, const CUtensorMap* map, uint64_t* full, int i) {
+          mbar_arrive_expect_tx(full, C::TILE);
+          for (int h = 0; h < C::HALVES; ++h)
+            tma_load_3d(at + (i % C::STAGES) * C::TILE + h * 128 * 128, map, full, 64 * h, head, s.k0 + i * kPromptKeys);
+        };
+        auto load_k = [&](int i) {
+          if ((ok = wait(&k_empty[i % C::STAGES], ((i / C::STAGES) & 1) ^ 1u))) load(sk, &tk, &k_full[i % C::STAGES], i);
+        };
+        if (steps > 0) {
+          load_q(0);
+          load_k(0);
+          if (tiles == 2) load_q(1);
+        }
+        int nk = steps > 0, nv = 0;
+        for (int i = 0; ok && i < steps; ++i) {
+          if (!(ok = wait(&v_empty[i % C::STAGES], ((i / C::STAGES) & 1) ^ 1u))) break;
+          load(sv, &tv, i < first_fixed ? &v_full[i % C::STAGES] : &v_raw[i % C::STAGES], i);
+          ++nv;
+          if (i + 1 < steps) {
+            load_k(i + 1);
+            nk += ok;
+          }
+        }
+        // the copies land before the CTA leaves
+        for (int x = 0; x < tiles && steps > 0; ++x) wait(&q_full[x], 0);
+        for (int i = max(0, nk - C::STAGES); i < nk; ++i) wait(&k_full[i % C::STAGES], (i / C::STAGES) & 1);
+        for (int i = max(0, nv - C::STAGES); i < nv; ++i)
+          if (i < first_fixed) wait(&v_full[i % C::STAGES], (i / C::STAGES) & 1);
+          else wait(&v_raw[i % C::STAGES], fixed_phase(i));
+      }
+    } else if (warp == 9) {
+      // -------------------------------------------------------------- products
+      if (steps > 0 && elect_one_sync()) {
+        constexpr uint32_t iqk = umma_idesc(1u, 128, 128), ipv = umma_idesc(1u, 128, D) | (1u << 16);
+        const uint64_t krow = umma_desc_k_sw128(0), vrow = umma_desc_mn_sw128(0, 128 * 128);
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
+        auto qk = [&](int x, int i) {
+          const uint64_t a = desc_at(krow, smem_u32(sq + x * C::TILE)), b = desc_at(krow, smem_u32(sk + (i % C::STAGES) * C::TILE));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k / 4) * (128 * 128 / 16) + (k % 4) * 2;
+            umma_f16(tmem + 128 * x, a + at, b + at, iqk, k > 0);
+          }
+          umma_commit(&s_full[x]);
+        };
+        bool ok = wait(&k_full[0], 0);
+        for (int x = 0; ok && x < tiles; ++x)
+          if ((ok = wait(&q_full[x], 0))) { tc_fence_after_sync(); qk(x, 0); }
+        if (ok) umma_commit(&k_empty[0]);
+        for (int i = 0; ok && i < steps; ++i) {
+          const int stage = i % C::STAGES;
+          const uint32_t phase = (i / C::STAGES) & 1;
+          for (int x = 0; ok && x < tiles; ++x) {
+            if (x == 0) {
+              if (!(ok = i < first_fixed ? wait(&v_full[stage], phase) : wait(&v_ready[stage], fixed_phase(i)))) break;
+            }
+            if (!(ok = wait(&p_full[x], i & 1))) break;
+            tc_fence_after_sync();
+            const uint64_t b = desc_at(vrow, smem_u32(sv + stage * C::TILE));
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, b + k * (16 * 128 / 16), ipv, i > 0 || k > 0);
+            if (x + 1 == tiles) umma_commit(&v_empty[stage]);
+            if (i + 1 == steps) {
+              umma_commit(&o_full[x]);
+              continue;
+            }
+            if (x == 0) {
+              if (!(ok = wait(&k_full[(i + 1) % C::STAGES], ((i + 1) / C::STAGES) & 1))) break;
+              tc_fence_after_sync();
+            }
+            qk(x, i + 1);
+            if (x + 1 == tiles) umma_commit(&k_empty[(i + 1) % C::STAGES]);
+          }
+        }
+        umma_commit(&drained);
+        wait(&drained, 0);
+      }
+    } else {
+      // -------------------------------------------------------------- values of tiles that some row does not see whole
+      for (int i = first_fixed; i < steps; ++i) {
+        const int stage = i % C::STAGES;
+        if (!mbar_wait_warp(&v_raw[stage], fixed_phase(i), p.status, kPromptKernelId, kPromptWaitNs)) break;
+        uint4* const at = (uint4*)(sv + stage * C::TILE);
+#pragma unroll 4
+        for (int c = (warp - 10) * 32 + lane; c < C::TILE / 16; c += 64) {
+          const int half = c / 1024, row = (c / 8) % 128;
+          const int key = i * kPromptKeys + row;
+          if (key >= s.nk) {
+            at[c] = make_uint4(0, 0, 0, 0);
+            continue;
+          }
+          uint4 v = at[c];
+          auto bad = [](uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; };   // an exponent of ones
+          if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            const int d = 64 * half + 8 * ((c & 7) ^ (row & 7));    // the swizzle's order of 16-byte pieces
+            for (int e = 0; e < 8; ++e) {
+              const float f = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+              if (fabsf(f) < INFINITY) continue;
+              atomicMin(&odd[odd_kind(f)][d + e], key);
+              w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+            }
+            any_odd = 1;
+            at[c] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_ready[stage]);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax, one row to a thread
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int x = warp >> 2, row = threadIdx.x & 127;
+    const int token = token0 + x * tokens + row / p.group, hq = head * p.group + row % p.group;
+    const bool mine = row < tokens * p.group && token < s.nq;
+    const int visible = mine ? min(prompt_visible(p, s, token), s.nk) : 0;
+    const int all = __reduce_min_sync(0xffffffffu, mine ? visible : INT_MAX);   // keys that the warp's rows all see
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;
+    // logits are turned positive multiples of S: a scale that is not positive goes into S itself
+    float mult = p.scale * 1.44269504088896341f;
+    const float turn = mult > 0.f ? 1.f : mult < 0.f ? -1.f : 0.f;
+    mult = turn == 0.f ? 1.f : fabsf(mult);
+    float m = -INFINITY, l = 0.f;
+    bool ok = x < tiles;
+    for (int i = 0; ok && i < steps; ++i) {
+      if (!(ok = mbar_wait_warp(&s_full[x], i & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+      tc_fence_after_sync();
+      uint32_t r[128];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
+      tmem_ld_wait();
+      if (turn != 1.f) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * turn);
+      }
+      const int k0 = i * kPromptKeys;
+      if (k0 + kPromptKeys > all) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c)
+          if (k0 + c >= visible) r[c] = __float_as_uint(-INFINITY);
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(r[c]));
+      const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
+      const bool grow = peak > m + 8.f;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float now = grow ? peak : m;
+        const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
+        m = now;
+        l *= shrink;
+        if (i > 0) {
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(to + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+            tmem_st32(to + c, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : -m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float a = prompt_exp2(fmaf(__uint_as_float(r[64 * h + 2 * c]), mult, base));
+          const float b = prompt_exp2(fmaf(__uint_as_float(r[64 * h + 2 * c + 1]), mult, base));
+          sum[(2 * c) & 3] += a;
+          sum[(2 * c + 1) & 3] += b;
+          w[c] = pack_bf16(a, b);
+        }
+        tmem_st32(ts + 32 * h, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[x]);
+    }
+    if (x < tiles) {
+      if (ok && steps > 0) {
+        ok = mbar_wait_warp(&o_full[x], 0, p.status, kPromptKernelId, kPromptWaitNs);
+        tc_fence_after_sync();
+      }
+      // a row that sees keys has a sum, unless all its logits are -inf
+      const float inv = l == 0.f ? (visible > 0 ? NAN : 0.f) : 1.f / l;
+      const bool put_back = any_odd != 0;
+      const long long at = (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (steps > 0) {
+          tmem_ld32(to + c, o);
+          tmem_ld_wait();
+        }
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = steps > 0 && visible > 0 ? __uint_as_float(o[e]) * inv : 0.f;
+        if (put_back) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] = put_back_odd<D>(odd, c + e, visible, v[e]);
+        }
+        if (mine) {
+          __nv_bfloat16* const dst = (__nv_bfloat16*)p.out + at + c;
+          if (p.o_vec) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              *(uint4*)(dst + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]), pack_bf16(v[e + 4], v[e + 5]),
+                                              pack_bf16(v[e + 6], v[e + 7]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) dst[e] = __float2bfloat16_rn(v[e]);
+          }
+        }
+        __syncwarp();
+      }
+      if (mine && p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace raiccl

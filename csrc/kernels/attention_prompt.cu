@@ -1,4 +1,6 @@
 // Attention over whole prompts: packed sequences, causal or not, grouped heads.
+// bf16 on tcgen05 (attention_prompt_tc.cuh); fp32 here, as two tf32 parts of each
+// number.
 #include <algorithm>
 #include <atomic>
 #include <climits>
@@ -6,8 +8,10 @@
 
 #include "attention.h"
 #include "attention_prompt.cuh"
+#include "attention_prompt_tc.cuh"
 #include "serving.h"
 #include "serving_device.cuh"
+#include "serving_tma.h"
 #include "sm100_ptx.cuh"
 
 namespace raiccl {
@@ -26,27 +30,20 @@ struct PromptRows {
   static constexpr int SMEM = 4 * kRowsKeys * 2 * (KS + VS);
 };
 
-template <typename T>
 __device__ __forceinline__ void load4(const void* base, long long at, bool vec, float (&x)[4]) {
-  const T* p = (const T*)base + at;
+  const float* p = (const float*)base + at;
   if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 v = *(const float4*)p;
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
-      const uint2 v = *(const uint2*)p;
-      x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
-      x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
-    }
+    const float4 v = *(const float4*)p;
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = as_float(p[i]);
+    for (int i = 0; i < 4; ++i) x[i] = p[i];
   }
 }
 
 // One CTA: 128 rows (a token and a query head of the group), eight warps of
 // sixteen; 32 keys at a time, split into two tf32 parts as they are stored.
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool vec) {
   using C = PromptRows<D>;
   extern __shared__ __align__(16) float sm[];
@@ -84,8 +81,8 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
 #pragma unroll
     for (int j = 0; j < D / 8; ++j) {
       const long long at = (long long)(s.q0 + token[r]) * p.q_token + (long long)hq[r] * p.q_head + 8 * j + 2 * t;
-      q[r][2 * j] = row_in[r] ? as_float(((const T*)p.q)[at]) : 0.f;
-      q[r][2 * j + 1] = row_in[r] ? as_float(((const T*)p.q)[at + 1]) : 0.f;
+      q[r][2 * j] = row_in[r] ? ((const float*)p.q)[at] : 0.f;
+      q[r][2 * j + 1] = row_in[r] ? ((const float*)p.q)[at + 1] : 0.f;
     }
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -101,8 +98,8 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
       float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
       if (k0 + row < s.nk) {
         const long long token = s.k0 + k0 + row;
-        load4<T>(p.k, token * p.k_token + head * p.k_head + d, vec, x);
-        load4<T>(p.v, token * p.v_token + head * p.v_head + d, vec, y);
+        load4(p.k, token * p.k_token + head * p.k_head + d, vec, x);
+        load4(p.v, token * p.v_token + head * p.v_head + d, vec, y);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -134,11 +131,9 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
 #pragma unroll
       for (int n = 0; n < kRowsKeys / 8; ++n) {
         const float2 h = *(const float2*)(kh + (8 * n + g) * C::KS + 8 * j + 2 * t);
-        if constexpr (sizeof(T) == 4) {
-          const float2 low = *(const float2*)(kl + (8 * n + g) * C::KS + 8 * j + 2 * t);
-          mma_tf32(z[n], ah, __float_as_uint(low.x), __float_as_uint(low.y));
-          mma_tf32(z[n], al, __float_as_uint(h.x), __float_as_uint(h.y));
-        }
+        const float2 low = *(const float2*)(kl + (8 * n + g) * C::KS + 8 * j + 2 * t);
+        mma_tf32(z[n], ah, __float_as_uint(low.x), __float_as_uint(low.y));
+        mma_tf32(z[n], al, __float_as_uint(h.x), __float_as_uint(h.y));
         mma_tf32(z[n], ah, __float_as_uint(h.x), __float_as_uint(h.y));
       }
     }
@@ -186,10 +181,8 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
 #pragma unroll
       for (int k = 0; k < kRowsKeys / 8; ++k) {
         const int at = (8 * k + 2 * t) * C::VS + 8 * n + g;
-        if constexpr (sizeof(T) == 4) {
-          mma_tf32(fresh, ph[k], __float_as_uint(vl[at]), __float_as_uint(vl[at + C::VS]));
-          mma_tf32(fresh, pl[k], __float_as_uint(vh[at]), __float_as_uint(vh[at + C::VS]));
-        }
+        mma_tf32(fresh, ph[k], __float_as_uint(vl[at]), __float_as_uint(vl[at + C::VS]));
+        mma_tf32(fresh, pl[k], __float_as_uint(vh[at]), __float_as_uint(vh[at + C::VS]));
         mma_tf32(fresh, ph[k], __float_as_uint(vh[at]), __float_as_uint(vh[at + C::VS]));
       }
 #pragma unroll
@@ -211,43 +204,98 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
         const int d = 8 * n + 2 * t + e;
         float v = o[n][2 * r + e] * inv;
         if (any_odd) v = put_back_odd<D>(odd, d, visible[r], v);
-        store_elem(p.out, at + d, v, sizeof(T) == 2);
+        ((float*)p.out)[at + d] = v;
       }
     if (p.lse != nullptr && t == 0)
       p.lse[(long long)(s.q0 + token[r]) * p.Hq + hq[r]] = (m[r] + log2f(l[r])) * 0.69314718055994531f;
   }
 }
 
-PromptPlan plan_prompt(const PromptParams& p, int sms) { return PromptPlan{}; }
+// Rows of a tensor [n, heads, D] that TMA can read: on 16 bytes, and apart.
+static bool tma_rows(const void* t, long long token, long long head, long long n, int heads) {
+  return ((uintptr_t)t & 15) == 0 && (n <= 1 || (token > 0 && token % 8 == 0)) && (heads <= 1 || (head > 0 && head % 8 == 0));
+}
 
-template <typename T, int D>
-static void launch_prompt_rows(const PromptParams& p, cudaStream_t s) {
-  using C = PromptRows<D>;
-  auto kern = prompt_rows_kernel<T, D>;
-  static std::atomic<unsigned long long> configured;   // by device
+PromptPlan plan_prompt(const PromptParams& p, int sms) {
+  PromptPlan plan{};
+  if (!p.bf16) return plan;
+  auto bytes = [&](long long n, int heads) { return (n * heads * p.D * 2 + 255) / 256 * 256; };
+  plan.pack_q = !tma_rows(p.q, p.q_token, p.q_head, p.Nq, p.Hq);
+  plan.pack_k = p.Nk > 0 && !tma_rows(p.k, p.k_token, p.k_head, p.Nk, p.Hk);
+  plan.pack_v = p.Nk > 0 && !tma_rows(p.v, p.v_token, p.v_head, p.Nk, p.Hk);
+  if (plan.pack_q) plan.q_bytes = bytes(p.Nq, p.Hq);
+  if (plan.pack_k) plan.k_bytes = bytes(p.Nk, p.Hk);
+  if (plan.pack_v) plan.v_bytes = bytes(p.Nk, p.Hk);
+  return plan;
+}
+
+template <typename K>
+static void configure(K kern, int smem, std::atomic<unsigned long long>& configured) {
   int dev = 0;
   cudaGetDevice(&dev);
   const unsigned long long bit = 1ull << (dev & 63);
-  if (!(configured.load() & bit)) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
-      throw std::runtime_error("attention_prompt: shared memory");
-    configured.fetch_or(bit);
-  }
+  if (configured.load() & bit) return;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    throw std::runtime_error("attention_prompt: shared memory");
+  configured.fetch_or(bit);
+}
+
+template <int D>
+static void launch_prompt_rows(const PromptParams& p, cudaStream_t s) {
+  using C = PromptRows<D>;
+  auto kern = prompt_rows_kernel<D>;
+  static std::atomic<unsigned long long> configured;   // by device
+  configure(kern, C::SMEM, configured);
   const int tokens = kRowsTile / p.group;
-  auto aligned = [&](const void* t, long long a, long long b) { return (((uintptr_t)t | (a * sizeof(T)) | (b * sizeof(T))) & 15) == 0; };
+  auto aligned = [&](const void* t, long long a, long long b) { return (((uintptr_t)t | (a * 4) | (b * 4)) & 15) == 0; };
   const bool vec = aligned(p.k, p.k_token, p.k_head) && aligned(p.v, p.v_token, p.v_head);
   const dim3 grid((unsigned)((p.Nq + tokens - 1) / tokens + p.B), (unsigned)p.Hk);
   launch_with_pdl(kern, grid, dim3(256), C::SMEM, s, true, p, vec);
 }
 
-void launch_prompt(const PromptParams& p, const PromptPlan& plan, void* workspace, cudaStream_t s) {
-  if (p.D == 128) {
-    if (p.bf16) launch_prompt_rows<__nv_bfloat16, 128>(p, s);
-    else launch_prompt_rows<float, 128>(p, s);
-  } else {
-    if (p.bf16) launch_prompt_rows<__nv_bfloat16, 64>(p, s);
-    else launch_prompt_rows<float, 64>(p, s);
+// [tokens, heads, D] as TMA reads it: boxes of 64 dimensions, `heads_box` heads and `tokens_box` tokens.
+static CUtensorMap prompt_map(const void* base, long long token, long long head, long long n, int heads, int D, int heads_box, int tokens_box) {
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)n};
+  const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? head * 2 : D * 2), (cuuint64_t)(n > 1 ? token * 2 : D * 2)};
+  const cuuint32_t box[3] = {64, (cuuint32_t)heads_box, (cuuint32_t)tokens_box};
+  return make_tmap(base, true, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <int D>
+static void launch_prompt_tc(const PromptParams& p, cudaStream_t s) {
+  using C = PromptTc<D>;
+  auto kern = prompt_tc_kernel<D>;
+  static std::atomic<unsigned long long> configured;   // by device
+  configure(kern, C::SMEM, configured);
+  const int tokens = 128 / p.group;
+  const CUtensorMap tq = prompt_map(p.q, p.q_token, p.q_head, p.Nq, p.Hq, D, p.group, tokens);
+  // without keys nothing is loaded; a map has to name something
+  const CUtensorMap tk = p.Nk > 0 ? prompt_map(p.k, p.k_token, p.k_head, p.Nk, p.Hk, D, 1, kPromptKeys) : tq;
+  const CUtensorMap tv = p.Nk > 0 ? prompt_map(p.v, p.v_token, p.v_head, p.Nk, p.Hk, D, 1, kPromptKeys) : tq;
+  const long long tiles = (p.Nq + 2 * tokens - 1) / (2 * tokens) + p.B;   // at most
+  launch_with_pdl(kern, dim3((unsigned)(tiles * p.Hk)), dim3(kPromptThreads), C::SMEM, s, true, tq, tk, tv, p);
+}
+
+void launch_prompt(const PromptParams& params, const PromptPlan& plan, void* workspace, cudaStream_t s) {
+  PromptParams p = params;
+  if (!p.bf16) {
+    if (p.D == 128) launch_prompt_rows<128>(p, s);
+    else launch_prompt_rows<64>(p, s);
+    return;
   }
+  char* ws = (char*)workspace;
+  auto pack = [&](const void*& t, long long& token, long long& head, long long n, int heads, long long bytes) {
+    launch_pack_rows(t, token, head, heads, ws, p.D, n, p.D, 1, s);   // [heads, tokens, D]
+    t = ws;
+    token = p.D;
+    head = n * p.D;
+    ws += bytes;
+  };
+  if (plan.pack_q) pack(p.q, p.q_token, p.q_head, p.Nq, p.Hq, plan.q_bytes);
+  if (plan.pack_k) pack(p.k, p.k_token, p.k_head, p.Nk, p.Hk, plan.k_bytes);
+  if (plan.pack_v) pack(p.v, p.v_token, p.v_head, p.Nk, p.Hk, plan.v_bytes);
+  if (p.D == 128) launch_prompt_tc<128>(p, s);
+  else launch_prompt_tc<64>(p, s);
 }
 
 }  // namespace raiccl
