@@ -39,7 +39,7 @@ struct CacheWriteParams {
   const void* slots;                 // [N] int32 or int64
   int slots64, bf16, vec;            // vec: rows may be read 16 bytes at a time
   long long N;
-  int per;                           // tokens of a CTA, by the launch
+  int per_shift;                     // a CTA has 1 << per_shift tokens, by the launch
   DeviceStatus* status;
 };
 
@@ -79,13 +79,14 @@ struct CachedParams {
   int ctas;                          // that share the work
   float* parts;                      // [ctas][2][chunk][D] sums of sequences that several CTAs share
   float2* stats;                     // [ctas][2][chunk] their maxima and sums of exponentials
+  float* spill;                      // [ctas][warps][8 or 16][D] sums that a warp puts aside
   DeviceStatus* status;
 };
 
 struct CachedPlan {
   int chunk, chunks, ctas;
-  long long parts_bytes, stats_bytes;
-  long long bytes() const { return parts_bytes + stats_bytes; }
+  long long parts_bytes, stats_bytes, spill_bytes;
+  long long bytes() const { return parts_bytes + stats_bytes + spill_bytes; }
 };
 
 CachedPlan plan_cached(const CachedParams& p, int sms);

@@ -53,16 +53,20 @@ constexpr unsigned long long kCachedWaitNs = 2000000000ull;
 // ones keep their bits down to 2^-21 of the largest.
 constexpr float kCachedHead = 7.f, kCachedRoom = 15.f;
 
+// Warps of a CTA, by the registers that queries, sums and the operands in flight take.
+template <int D, int NT, int PARTS>
+constexpr int kCachedWarps = NT == 1 && PARTS == 1 ? 16 : 8;
+
 template <int D, int NT, int PARTS>
 struct Cached {
-  static constexpr int WARPS = 8, THREADS = 32 * WARPS;
+  static constexpr int WARPS = kCachedWarps<D, NT, PARTS>, THREADS = 32 * WARPS;
   static constexpr int HEADS = 8 * NT;                       // query heads of a chunk at most
   static constexpr int CODES = kCachedTile * D / 2, SCALES = kCachedTile * D / 16;
   static constexpr int STAGE = 2 * (CODES + SCALES);         // K codes, V codes, K scales, V scales
   static constexpr int PART = HEADS * D * 4;                 // a warp's sums of a sequence that it shares
-  static constexpr int STAGES = NT == 1 ? 5 : 4;
-  static constexpr int SMEM = WARPS * (STAGES * STAGE + PART);   // a warp's last part goes into its ring, which is done then
-  static_assert(STAGES * STAGE >= PART && SMEM <= 222 * 1024, "shared memory");
+  static constexpr int STAGES = 216 * 1024 / (WARPS * STAGE) < 6 ? 216 * 1024 / (WARPS * STAGE) : 6;
+  static constexpr int SMEM = WARPS * STAGES * STAGE;
+  static_assert(STAGES >= 3 && STAGES * STAGE >= PART, "the ring holds the warp's last part too");
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -128,9 +132,9 @@ __device__ __forceinline__ int cached_length(const CachedParams& p, int b) {
 
 __device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) { return (cached_length(p, b) + kCachedTile - 1) / kCachedTile; }
 
-// CTAs that take part, the first tile of one, and the CTA of a tile.
-__device__ __forceinline__ int cached_ctas(long long tiles, int ctas, int warps) {
-  const long long most = (tiles + warps - 1) / warps;
+// CTAs that take part (four tiles to one at least), the first tile of one, and the CTA of a tile.
+__device__ __forceinline__ int cached_ctas(long long tiles, int ctas) {
+  const long long most = (tiles + 3) / 4;
   return most < ctas ? (int)most : ctas;
 }
 __device__ __forceinline__ long long cached_first(long long tiles, int ctas, int c) { return tiles * c / ctas; }
@@ -176,7 +180,7 @@ __device__ __forceinline__ void cached_store4(const CachedParams& p, int b, int 
   }
 }
 
-// A warp's (or CTA's) piece of a sequence that is not whole: 0 it began before, 1 it ends after.
+// A warp's part of a piece that it shares; used: 1 the sums are in its ring, 2 in device memory.
 struct CachedPart {
   CachedPiece s;
   int used;
@@ -188,16 +192,12 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t full[C::WARPS][C::STAGES];
   __shared__ int pages_ok[C::WARPS][C::STAGES];
-  __shared__ long long before[C::THREADS + 1];
+  __shared__ long long before[C::THREADS + 1], sum_of[C::WARPS];
   __shared__ CachedPart part[C::WARPS][2];
   __shared__ float2 stat[C::WARPS][2][C::HEADS];
   __shared__ int nonempty[C::WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
-  // a warp's part of a sequence: the one that began before its share, the one that ends after it
-  auto sums = [&](int w, int side) {
-    return (float*)(side == 0 ? smem + C::WARPS * C::STAGES * C::STAGE + w * C::PART : smem + w * C::STAGES * C::STAGE);
-  };
   if (lane < C::STAGES) mbar_init(&full[warp][lane], 1);
   fence_mbarrier_init();
   __syncwarp();
@@ -220,22 +220,25 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
       const long long up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
-    __shared__ long long warp_sum_of[C::WARPS];
-    if (lane == 31) warp_sum_of[warp] = sum;
+    if (lane == 31) sum_of[warp] = sum;
     __syncthreads();
     long long base = 0;
-    for (int w = 0; w < warp; ++w) base += warp_sum_of[w];
+    for (int w = 0; w < warp; ++w) base += sum_of[w];
     before[tid + 1] = (base + sum) * HC;
     if (tid == 0) before[0] = 0;
     __syncthreads();
   }
   const long long tiles = before[C::THREADS];
   if (tiles == 0) return;
-  const int ctas = cached_ctas(tiles, p.ctas, C::WARPS);
+  const int ctas = cached_ctas(tiles, p.ctas);
   if ((int)blockIdx.x >= ctas) return;
   const long long c0 = cached_first(tiles, ctas, blockIdx.x), c1 = cached_first(tiles, ctas, blockIdx.x + 1);
   const long long u0 = c0 + (c1 - c0) * warp / C::WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
   const int count = (int)(u1 - u0);
+  // A warp's part of a sequence: the one that began before its share (0), the one that ends after it (1).  The last that it
+  // works on goes into its ring, which is done then; a first one with others behind it to device memory.
+  auto spilled = [&](int w) { return p.spill + ((long long)blockIdx.x * C::WARPS + w) * (C::HEADS * D); };
+  auto ringed = [&](int w) { return (float*)(smem + w * C::STAGES * C::STAGE); };
   if (lane == 0) {
     part[warp][0].used = part[warp][1].used = 0;
     nonempty[warp] = count > 0;
@@ -261,44 +264,52 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
     }
 
     // ---------------------------------------------------------- copies, STAGES tiles ahead
-    CachedPiece ahead = piece;
-    int issued = 0;
+    // One copy to a lane: lanes 0 to 3 the four arrays, of the tile or of its first sixteen tokens, 4 to 7 of the others.
     const int page_size = 1 << p.c.page_shift;
     const bool whole = page_size >= kCachedTile;   // a tile lies in one page
+    const int what = lane & 3, half16 = 16 * ((lane >> 2) & 1);
+    const int width = what < 2 ? D / 2 : D / 16;
+    const uint8_t* const array = what == 0 ? p.c.k_codes : what == 1 ? p.c.v_codes : what == 2 ? p.c.k_scales : p.c.v_scales;
+    const uint32_t copy_at = (what < 2 ? what * C::CODES : 2 * C::CODES + (what - 2) * C::SCALES) + half16 * width;
+    const bool copier = lane < (whole ? 4 : 8);
+    CachedPiece ahead = piece;
+    int ahead_len = cached_length(p, piece.b), ahead_at = (int)(u0 - piece.first) * kCachedTile;   // the next copy's tokens
+    int ahead_end = (int)min((long long)count, piece.first + piece.n - u0);                         // tiles of the share up to the piece's end
+    const int* ahead_pages = p.table + (long long)piece.b * p.table_stride;
+    long long ahead_row = (long long)(piece.hc / p.chunks) << p.c.page_shift;
+    int issued = 0, fill = 0;
     auto issue = [&]() {
-      const long long u = u0 + issued;
-      while (u >= ahead.first + ahead.n) next_piece(p, ahead);
-      const int stage = issued % C::STAGES;
-      const int token = (int)(u - ahead.first) * kCachedTile, len = cached_length(p, ahead.b);
-      const int kv = ahead.hc / p.chunks;
-      // one copy to a lane: lanes 0 to 3 the four arrays, of the tile or of its first sixteen tokens, 4 to 7 of the others
-      const int half = (lane >> 2) & 1, what = lane & 3;
-      const int at = token + 16 * half;
+      if (issued == ahead_end) {
+        next_piece(p, ahead);
+        ahead_len = cached_length(p, ahead.b);
+        ahead_at = 0;
+        ahead_end = (int)min((long long)count, (long long)ahead_end + ahead.n);
+        ahead_pages = p.table + (long long)ahead.b * p.table_stride;
+        ahead_row = (long long)(ahead.hc / p.chunks) << p.c.page_shift;
+      }
+      const int at = ahead_at + half16;
       int page = -1;
-      if (lane < 8 && at < len) {
-        page = __ldg(p.table + ahead.b * p.table_stride + (at >> p.c.page_shift));
+      if (lane < 8 && at < ahead_len) {
+        page = __ldg(ahead_pages + (at >> p.c.page_shift));
         if (page < 0 || page >= p.c.pages) {
           if (what == 0) record_status(p.status, kBoundsViolation, kCachedKernelId, page, p.c.pages);
           page = -1;
         }
       }
-      const uint32_t have = __ballot_sync(0xffffffffu, lane < 8 && page >= 0);
-      const int ok = (have & 1u ? 1 : 0) | (have & 16u ? 2 : 0);
-      const int rows = whole ? (ok & 1 ? kCachedTile : 0) : 16 * __popc(ok);
+      const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
       if (lane == 0) {
-        pages_ok[warp][stage] = ok;
-        mbar_arrive_expect_tx(&full[warp][stage], rows * (2 * (D / 2) + 2 * (D / 16)));
+        const int ok = whole ? (have & 1u ? 3 : 0) : (have & 1u ? 1 : 0) | (have & 16u ? 2 : 0);
+        pages_ok[warp][fill] = ok;
+        mbar_arrive_expect_tx(&full[warp][fill], __popc(ok) * 16 * (2 * (D / 2) + 2 * (D / 16)));
       }
       __syncwarp();
-      if (page >= 0 && lane < (whole ? 4 : 8)) {
-        const bool codes = what < 2;
-        const int width = codes ? D / 2 : D / 16;
-        const uint8_t* base = what == 0 ? p.c.k_codes : what == 1 ? p.c.v_codes : what == 2 ? p.c.k_scales : p.c.v_scales;
-        const long long row = ((((long long)page * p.c.heads + kv) << p.c.page_shift) + (at & (page_size - 1)));
-        uint8_t* dst = ring + stage * C::STAGE + (codes ? what * C::CODES : 2 * C::CODES + (what - 2) * C::SCALES) + 16 * half * width;
-        bulk_load_g2s(dst, base + row * width, (whole ? kCachedTile : 16) * width, &full[warp][stage]);
+      if (copier && page >= 0) {
+        const long long row = ((long long)page * p.c.heads << p.c.page_shift) + ahead_row + (at & (page_size - 1));
+        bulk_load_g2s(ring + fill * C::STAGE + copy_at, array + row * width, (whole ? kCachedTile : 16) * width, &full[warp][fill]);
       }
       ++issued;
+      ahead_at += kCachedTile;
+      fill = fill + 1 == C::STAGES ? 0 : fill + 1;
     };
     while (issued < count && issued < C::STAGES) issue();
 
@@ -378,7 +389,7 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
     };
 
     // The piece's end, for this warp: written where all its tiles were this warp's, else left for the join.
-    auto finish = [&]() {
+    auto finish = [&](bool last) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -407,8 +418,8 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         return;
       }
       const int side = early ? 0 : 1;
-      if (lane == 0) part[warp][side] = {piece, 1};
-      float* const at = sums(warp, side);
+      if (lane == 0) part[warp][side] = {piece, last ? 1 : 2};
+      float* const at = last ? ringed(warp) : spilled(warp);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -423,22 +434,35 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
     };
 
     begin();
-    int done = 0;
+    int done = 0, stage = 0, end = (int)min((long long)count, piece.first + piece.n - u0);
+    int left = cached_length(p, piece.b) - (int)(u0 - piece.first) * kCachedTile;   // tokens of the piece from this tile on
+    uint32_t phase = 0;
+#pragma unroll 1
     for (; done < count; ++done) {
-      const long long u = u0 + done;
-      if (u >= piece.first + piece.n) {
-        finish();
+      if (done == end) {
+        finish(false);
         next_piece(p, piece);
         begin();
+        end = (int)min((long long)count, (long long)end + piece.n);
+        left = cached_length(p, piece.b);
       }
-      const int stage = done % C::STAGES;
-      if (!mbar_wait_warp(&full[warp][stage], (done / C::STAGES) & 1, p.status, kCachedKernelId, kCachedWaitNs)) break;
-      const uint8_t* const s = ring + stage * C::STAGE;
+      if (!mbar_wait_warp(&full[warp][stage], phase, p.status, kCachedKernelId, kCachedWaitNs)) break;
+      uint8_t* const s = ring + stage * C::STAGE;
       const int ok = pages_ok[warp][stage];
-      const int left = cached_length(p, piece.b) - (int)(u - piece.first) * kCachedTile;
-      const bool all = left >= kCachedTile && (whole ? ok & 1 : ok == 3);
-      auto valid = [&](int row) { return all || (row < left && (ok >> (whole ? 0 : row >> 4) & 1)); };
-      if (ok != 0) {
+      const bool all = left >= kCachedTile && ok == 3;
+      uint32_t rows = 0xffffffffu;     // tokens of the tile that the sequence has
+      if (!all) {
+        rows = left >= kCachedTile ? 0xffffffffu : (1u << left) - 1;
+        rows &= (ok & 1 ? 0xffffu : 0u) | (ok & 2 ? 0xffff0000u : 0u);
+        // a page's rest may hold anything: its values count as zeros
+        if (!(rows >> lane & 1)) {
+          if constexpr (D == 128) *(uint2*)(s + 2 * C::CODES + C::SCALES + lane * 8) = make_uint2(0, 0);
+          else *(uint32_t*)(s + 2 * C::CODES + C::SCALES + lane * 4) = 0;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (rows != 0) {
         float z[2][NT][4];
         // -------------------------------------------------- S^T = K Q^T
 #pragma unroll
@@ -487,20 +511,32 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         // -------------------------------------------------- softmax
         // x = z - m by one fma: off by a rounding of the difference, not of the logit
         float x[2][NT][4];
-        bool grow = false;
         auto below = [&]() {
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                x[mt][nt][j] = valid(16 * mt + 8 * (j >> 1) + g) ? fmaf(z[mt][nt][j], mult[nt][j & 1], -m[nt][j & 1]) : -INFINITY;
-                grow |= x[mt][nt][j] > kCachedRoom;
-              }
+              for (int j = 0; j < 4; ++j) x[mt][nt][j] = fmaf(z[mt][nt][j], mult[nt][j & 1], -m[nt][j & 1]);
+          if (!all) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (!(rows >> (16 * mt + 8 * (j >> 1) + g) & 1)) x[mt][nt][j] = -INFINITY;
+          }
         };
         below();
-        if (__any_sync(0xffffffffu, grow)) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = fmaxf(most, x[mt][nt][j]);
+        if (__any_sync(0xffffffffu, most > kCachedRoom)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -510,7 +546,7 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
               for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
-                  if (valid(16 * mt + 8 * r + g)) top = fmaxf(top, z[mt][nt][j + 2 * r] * mult[nt][j]);
+                  if (rows >> (16 * mt + 8 * r + g) & 1) top = fmaxf(top, z[mt][nt][j + 2 * r] * mult[nt][j]);
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -561,25 +597,24 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
           uint32_t pair[2][2][WV], sv[2];   // [tokens 2t, 2t + 1 / + 8][even, odd dimensions]
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            uint32_t x[2][WV], byte[2];
+            uint32_t y[2][WV], byte[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int row = 16 * mt + 8 * r + 2 * t + e;
               if constexpr (D == 128) {
                 const uint2 v = *(const uint2*)(s + C::CODES + row * 64 + 8 * g);
-                x[e][0] = v.x; x[e][1] = v.y;
+                y[e][0] = v.x; y[e][1] = v.y;
                 byte[e] = s[2 * C::CODES + C::SCALES + row * 8 + g];
               } else {
-                x[e][0] = *(const uint32_t*)(s + C::CODES + row * 32 + 4 * g);
+                y[e][0] = *(const uint32_t*)(s + C::CODES + row * 32 + 4 * g);
                 byte[e] = s[2 * C::CODES + C::SCALES + row * 4 + (g >> 1)];
               }
-              byte[e] = valid(row) ? byte[e] : 0u;   // a page's rest may hold anything
             }
             sv[r] = scales_f16(byte[0] | byte[1] << 8);
 #pragma unroll
             for (int i = 0; i < WV; ++i) {
-              pair[r][0][i] = (x[0][i] & 0x0f0f0f0fu) | ((x[1][i] << 4) & 0xf0f0f0f0u);
-              pair[r][1][i] = ((x[0][i] >> 4) & 0x0f0f0f0fu) | (x[1][i] & 0xf0f0f0f0u);
+              pair[r][0][i] = (y[0][i] & 0x0f0f0f0fu) | ((y[1][i] << 4) & 0xf0f0f0f0u);
+              pair[r][1][i] = ((y[0][i] >> 4) & 0x0f0f0f0fu) | (y[1][i] & 0xf0f0f0f0u);
             }
           }
 #pragma unroll
@@ -591,16 +626,16 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
               for (int e = 0; e < 2; ++e) {
                 codes_f16(pair[r][e][i], h[r][e]);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) h[r][e][x] = mul_f16(h[r][e][x], sv[r]);
+                for (int y = 0; y < 4; ++y) h[r][e][y] = mul_f16(h[r][e][y], sv[r]);
               }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const uint32_t a[4] = {h[0][0][x], h[0][1][x], h[1][0][x], h[1][1][x]};
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t a[4] = {h[0][0][y], h[0][1][y], h[1][0][y], h[1][1][y]};
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int q = PARTS - 1; q >= 0; --q)
-                  mma_f16(PARTS == 2 ? fresh[PARTS == 2 ? 4 * i + x : 0][nt] : o[4 * i + x][nt], a, bp[q][mt][nt][0], bp[q][mt][nt][1]);
+                  mma_f16(PARTS == 2 ? fresh[PARTS == 2 ? 4 * i + y : 0][nt] : o[4 * i + y][nt], a, bp[q][mt][nt][0], bp[q][mt][nt][1]);
             }
           }
         }
@@ -613,67 +648,66 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
               for (int j = 0; j < 4; ++j) o[i][nt][j] += fresh[i][nt][j];
         }
       }
+      left -= kCachedTile;
+      if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
       __syncwarp();   // every lane has read the stage
       if (issued < count) issue();
     }
     for (int i = done; i < issued; ++i)   // after a wait that ran out: the copies in flight land before the ring is used again
       mbar_wait_warp(&full[warp][i % C::STAGES], (i / C::STAGES) & 1, p.status, kCachedKernelId, kCachedWaitNs);
-    finish();
+    finish(true);
   }
 
   // ------------------------------------------------------------ the CTA's shared pieces
   __syncthreads();
-  for (int w = 0; w < C::WARPS; ++w)
-    for (int side = 0; side < 2; ++side) {
-      if (!part[w][side].used) continue;
-      const CachedPiece s = part[w][side].s;
-      // a piece's parts: its first one (a tail, or the head of the CTA's first warp), then the heads of the warps behind it
-      bool first = side == 1;
-      if (side == 0) {
-        first = true;
-        for (int v = 0; v < w; ++v) first &= !nonempty[v];
+  // a piece's parts: its first one (a tail, or the head of the CTA's first warp), then the heads of the warps behind it
+  const bool mine = lane < C::WARPS;
+  const uint32_t with = __ballot_sync(0xffffffffu, mine && nonempty[mine ? lane : 0]);
+  uint32_t tails = __ballot_sync(0xffffffffu, mine && part[mine ? lane : 0][1].used);
+  const uint32_t heads_at = __ballot_sync(0xffffffffu, mine && part[mine ? lane : 0][0].used);
+  uint32_t firsts = heads_at & with & -with;
+  while (firsts | tails) {
+    const int side = firsts ? 0 : 1, w = __ffs(firsts ? firsts : tails) - 1;
+    if (firsts) firsts = 0; else tails &= tails - 1;
+    const CachedPiece s = part[w][side].s;
+    int head0;
+    const int heads = piece_heads(p, s.hc, head0);
+    const bool early = s.first < c0, late = s.first + s.n > c1;
+    int end = w + 1;
+    while (end < C::WARPS && (!(with >> end & 1) || ((heads_at >> end & 1) && part[end][0].s.first == s.first))) ++end;
+    for (int e = tid; e < heads * (D / 4); e += C::THREADS) {
+      const int h = e / (D / 4), d = 4 * (e - h * (D / 4));
+      float top = stat[w][side][h].x;
+      for (int x = w + 1; x < end; ++x)
+        if (with >> x & 1) top = fmaxf(top, stat[x][0][h].x);
+      float l = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int x = w; x < end; ++x) {
+        if (!(with >> x & 1)) continue;
+        const int y = x == w ? side : 0;
+        const float2 st = stat[x][y][h];
+        const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
+        const float4 a = *(const float4*)((part[x][y].used == 1 ? ringed(x) : spilled(x)) + h * D + d);
+        l = fmaf(st.y, f, l);
+        v.x = fmaf(a.x, f, v.x); v.y = fmaf(a.y, f, v.y); v.z = fmaf(a.z, f, v.z); v.w = fmaf(a.w, f, v.w);
       }
-      if (!first) continue;
-      int head0;
-      const int heads = piece_heads(p, s.hc, head0);
-      const bool early = s.first < c0, late = s.first + s.n > c1;
-      for (int e = tid; e < heads * (D / 4); e += C::THREADS) {
-        const int h = e / (D / 4), d = 4 * (e - h * (D / 4));
-        float top = stat[w][side][h].x;
-        int end = w + 1;
-        for (; end < C::WARPS; ++end) {
-          if (!nonempty[end]) continue;
-          if (!part[end][0].used || part[end][0].s.first != s.first) break;
-          top = fmaxf(top, stat[end][0][h].x);
-        }
-        float l = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int x = w; x < end; ++x) {
-          if (!nonempty[x]) continue;
-          const int y = x == w ? side : 0;
-          const float2 st = stat[x][y][h];
-          const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
-          const float4 a = *(const float4*)(sums(x, y) + h * D + d);
-          l = fmaf(st.y, f, l);
-          v.x = fmaf(a.x, f, v.x); v.y = fmaf(a.y, f, v.y); v.z = fmaf(a.z, f, v.z); v.w = fmaf(a.w, f, v.w);
-        }
-        if (!early && !late) {
-          const float r = l == 0.f ? 0.f : p.c.v_unit / l;
-          cached_store4(p, s.b, head0 + h, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
-          if (p.lse != nullptr && d == 0) p.lse[(long long)s.b * p.Hq + head0 + h] = cached_lse(top, l);
-        } else {
-          const long long at = ((long long)blockIdx.x * 2 + (early ? 0 : 1)) * p.chunk + h;
-          *(float4*)(p.parts + at * D + d) = v;
-          if (d == 0) p.stats[at] = make_float2(top, l);
-        }
+      if (!early && !late) {
+        const float r = l == 0.f ? 0.f : p.c.v_unit / l;
+        cached_store4(p, s.b, head0 + h, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+        if (p.lse != nullptr && d == 0) p.lse[(long long)s.b * p.Hq + head0 + h] = cached_lse(top, l);
+      } else {
+        const long long at = ((long long)blockIdx.x * 2 + (early ? 0 : 1)) * p.chunk + h;
+        *(float4*)(p.parts + at * D + d) = v;
+        if (d == 0) p.stats[at] = make_float2(top, l);
       }
     }
+  }
 }
 
 // Sequences that several CTAs share, one head to a CTA; a warp takes every
 // eighth part.  Empty sequences too, which no tile stands for.
 template <int D>
-__global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p, int warps) {
+__global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p) {
   __shared__ long long sum_of[2][8];
   __shared__ float4 acc[8][D / 4];
   __shared__ float2 ml[8];
@@ -705,7 +739,7 @@ __global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p, int wa
     return;
   }
   const long long tiles = all * HC, first = ahead * HC + (long long)hc * n;
-  const int ctas = cached_ctas(tiles, p.ctas, warps);
+  const int ctas = cached_ctas(tiles, p.ctas);
   const int c0 = cached_cta(tiles, ctas, first), c1 = cached_cta(tiles, ctas, first + n - 1);
   if (c0 == c1) return;
   float m = -INFINITY, l = 0.f;
@@ -751,6 +785,8 @@ CachedPlan plan_cached(const CachedParams& p, int sms) {
   plan.ctas = sms;
   plan.parts_bytes = (long long)plan.ctas * 2 * plan.chunk * p.c.D * 4;
   plan.stats_bytes = ((long long)plan.ctas * 2 * plan.chunk * 8 + 255) / 256 * 256;
+  const int warps = most == 16 && plan.chunk <= 8 ? kCachedWarps<128, 1, 1> : most == 16 ? kCachedWarps<128, 2, 1> : kCachedWarps<128, 1, 2>;
+  plan.spill_bytes = (long long)plan.ctas * warps * (plan.chunk > 8 ? 16 : 8) * p.c.D * 4;
   return plan;
 }
 
@@ -768,7 +804,7 @@ static void launch_cached_as(const CachedParams& p, cudaStream_t s) {
     configured.fetch_or(bit);
   }
   launch_with_pdl(kern, dim3(p.ctas), dim3(C::THREADS), C::SMEM, s, true, p);
-  launch_with_pdl(cached_join_kernel<D>, dim3(p.B * p.c.heads * p.chunks, p.chunk), dim3(256), 0, s, true, p, (int)C::WARPS);
+  launch_with_pdl(cached_join_kernel<D>, dim3(p.B * p.c.heads * p.chunks, p.chunk), dim3(256), 0, s, true, p);
 }
 
 void launch_cached(const CachedParams& params, const CachedPlan& plan, void* workspace, cudaStream_t s) {
@@ -778,6 +814,7 @@ void launch_cached(const CachedParams& params, const CachedPlan& plan, void* wor
   p.ctas = plan.ctas;
   p.parts = (float*)workspace;
   p.stats = (float2*)((char*)workspace + plan.parts_bytes);
+  p.spill = (float*)((char*)workspace + plan.parts_bytes + plan.stats_bytes);
   const bool two = !(p.bf16 && p.out_bf16);
   if (p.c.D == 128) {
     if (two) launch_cached_as<128, 1, 2>(p, s);

@@ -28,8 +28,7 @@
 namespace raiccl {
 
 constexpr int kWriteThreads = 512;
-constexpr int kWriteTokens = 1024;         // of a CTA at most
-constexpr int kWriteTable = 2 * kWriteTokens;
+constexpr int kWriteTokens = 2048;         // of a CTA at most
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -73,59 +72,61 @@ __device__ __forceinline__ void load8(const T* p, int vec, float (&x)[8]) {
 }
 
 // Two lanes have a group of sixteen: its scale (both get it) and this lane's eight codes.
-__device__ __forceinline__ uint32_t quantise8(float (&x)[8], float per_unit, uint32_t& scale) {
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float unit, float per_unit, uint32_t& scale) {
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] *= per_unit;
-    top = max_nan(top, fabsf(x[i]));
-  }
-  top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
+  top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1)) * per_unit;
   scale = __nv_cvt_float_to_fp8(__fdiv_rn(top, 6.f), __NV_SATFINITE, __NV_E4M3);
   const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)scale, __NV_E4M3)));
-  const float r = s > 0.f ? __frcp_rn(s) : 0.f;
+  const float r = s > 0.f ? __frcp_rn(s) * per_unit : 0.f, back = s * unit;
+  // Behind 448 * 6 everything saturates; there numbers are cut, so that no infinities meet below.
+  const float most = 8192.f * unit;
+  const bool cut = top > 8192.f;
   uint32_t codes = 0;
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     float q[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      // Behind 448 * 6 everything saturates; infinities must not meet each other below.
-      const float v = fminf(fmaxf(x[i + j], -8192.f), 8192.f);
+      const float v = cut ? fminf(fmaxf(x[i + j], -most), most) : x[i + j];
       // x / s: the product by the rounded reciprocal, and one correction by its remainder, which is exact in an fma
       // (P. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990).
       q[j] = v * r;
-      q[j] = fmaf(fmaf(-s, q[j], v), r, q[j]);
+      q[j] = fmaf(fmaf(-back, q[j], v), r, q[j]);
     }
     codes |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(q[0], q[1]), __NV_E2M1, cudaRoundNearest) << (4 * i);
   }
   return codes;
 }
 
-// A CTA has `per` consecutive tokens.  Where several tokens of a call name one
-// slot, the last of them is kept: the CTA enters its tokens' slots into a hash
-// table, the highest token of each, and looks up all later tokens' slots in it.
-// With 2 CTAs to an SM that is at most 300 reads of the slots, in L2 (16384
-// tokens, 0.5 us).
+// A CTA has `per` consecutive tokens (a power of two).  Where several tokens of
+// a call name one slot, the last of them is kept: the CTA enters its tokens'
+// slots into a hash table, the highest token of each, and looks up all later
+// tokens' slots in it.
+//
+// A row of a head is D / 8 lanes; rows go by value or key, head and token, the
+// token fastest, so that no index needs a division.  Four rows to a thread are
+// loaded before the first is worked on.
 template <typename T>
 __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWriteParams p) {
-  __shared__ int slot_of[kWriteTokens], key[kWriteTable], last[kWriteTable];
+  extern __shared__ int table[];      // [per] slots, [size] keys, [size] last tokens
   const CacheView& c = p.c;
   griddep_wait();
   griddep_launch_dependents();
-  const long long first = (long long)blockIdx.x * p.per;
-  const int n = (int)(p.N - first < p.per ? p.N - first : p.per);
-  int size = 2;                       // of the table: a power of two, at most half full
-  while (size < 2 * n) size *= 2;
+  const int per = 1 << p.per_shift, size = 2 * per;
+  int *slot_of = table, *key = table + per, *last = key + size;
+  const long long first = (long long)blockIdx.x << p.per_shift;
+  const int n = (int)(p.N - first < per ? p.N - first : per);
   for (int i = threadIdx.x; i < size; i += kWriteThreads) { key[i] = -1; last[i] = -1; }
   __syncthreads();
   auto at = [&](int slot) { return (int)(((uint32_t)slot * 2654435761u) >> 16) & (size - 1); };
-  for (int i = threadIdx.x; i < n; i += kWriteThreads) {
-    const int s = cache_slot(p.slots, p.slots64, first + i, c, p.status, kCacheWriteKernelId);
+  for (int i = threadIdx.x; i < per; i += kWriteThreads) {
+    const int s = i < n ? cache_slot(p.slots, p.slots64, first + i, c, p.status, kCacheWriteKernelId) : -1;
     slot_of[i] = s;
     if (s < 0) continue;
     int e = at(s);
-    while (true) {                    // ends: the table has free places
+    while (true) {                    // ends: the table is at most half full
       const int old = atomicCAS(&key[e], -1, s);
       if (old == -1 || old == s) break;
       e = (e + 1) & (size - 1);
@@ -133,10 +134,11 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
     atomicMax(&last[e], i);
   }
   __syncthreads();
+  const long long bound = (long long)c.pages << c.page_shift;
 #pragma unroll 4
   for (long long i = first + n + threadIdx.x; i < p.N; i += kWriteThreads) {
     const long long wide = p.slots64 ? ((const long long*)p.slots)[i] : (long long)((const int*)p.slots)[i];
-    if (wide < 0 || wide >= (long long)c.pages << c.page_shift) continue;
+    if (wide < 0 || wide >= bound) continue;
     const int s = (int)wide;
     int e = at(s), k;
     while ((k = key[e]) != -1 && k != s) e = (e + 1) & (size - 1);
@@ -151,57 +153,84 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
     if (last[e] != i) slot_of[i] = -1;
   }
   __syncthreads();
-  // eight numbers to a thread; D is 64 or 128, so that the lanes of a group, and of a scales' word, are neighbours
-  const int lanes = c.D / 8, row = lanes * c.heads, total = 2 * row * n;
-  for (int i0 = 0; i0 < total; i0 += kWriteThreads) {
-    const int i = i0 + threadIdx.x;
-    const int t = i / (2 * row), rest = i - t * 2 * row, value = rest >= row, in = rest - value * row;
-    const int h = in / lanes, l = in - h * lanes;
-    const int slot = i < total ? slot_of[t] : -1;
-    float x[8] = {};
-    if (slot >= 0) {
-      const T* src = value ? (const T*)p.v + (first + t) * p.v_token + h * p.v_head : (const T*)p.k + (first + t) * p.k_token + h * p.k_head;
-      load8(src + 8 * l, p.vec, x);
+  const int lane_shift = c.D == 128 ? 4 : 3, l = threadIdx.x & ((1 << lane_shift) - 1);
+  const int step = kWriteThreads >> lane_shift, rows = 2 * c.heads << p.per_shift;
+  constexpr int U = 4;
+  for (int r0 = 0; r0 < rows; r0 += U * step) {
+    float x[U][8];
+    int slot[U], hv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * step + (int)(threadIdx.x >> lane_shift), t = r & (per - 1);
+      hv[u] = r >> p.per_shift;
+      slot[u] = r < rows ? slot_of[t] : -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+      if (slot[u] >= 0) {
+        const T* src = hv[u] < c.heads ? (const T*)p.k + (first + t) * p.k_token + hv[u] * p.k_head
+                                       : (const T*)p.v + (first + t) * p.v_token + (hv[u] - c.heads) * p.v_head;
+        load8(src + 8 * l, p.vec, x[u]);
+      }
     }
-    uint32_t scale;
-    const uint32_t codes = quantise8(x, value ? 1.f / c.v_unit : 1.f / c.k_unit, scale);
-    uint32_t word = scale << (8 * ((l >> 1) & 3));   // four groups' scales, eight lanes
-    word |= __shfl_xor_sync(0xffffffffu, word, 2);
-    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-    if (slot >= 0) {
-      const long long r = cache_row(c, slot, h);
-      *(uint32_t*)((value ? c.v_codes : c.k_codes) + r * (c.D / 2) + 4 * l) = codes;
-      if ((l & 7) == 0) *(uint32_t*)((value ? c.v_scales : c.k_scales) + r * (c.D / 16) + l / 2) = word;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (r0 + u * step >= rows) break;              // the same for all threads
+      const bool value = hv[u] >= c.heads;
+      const float unit = value ? c.v_unit : c.k_unit;
+      uint32_t scale;
+      const uint32_t codes = quantise8(x[u], unit, 1.f / unit, scale);
+      uint32_t word = scale << (8 * ((l >> 1) & 3));   // four groups' scales, eight lanes
+      word |= __shfl_xor_sync(0xffffffffu, word, 2);
+      word |= __shfl_xor_sync(0xffffffffu, word, 4);
+      if (slot[u] >= 0) {
+        const long long at_row = cache_row(c, slot[u], value ? hv[u] - c.heads : hv[u]);
+        *(uint32_t*)((value ? c.v_codes : c.k_codes) + at_row * (c.D / 2) + 4 * l) = codes;
+        if ((l & 7) == 0) *(uint32_t*)((value ? c.v_scales : c.k_scales) + at_row * (c.D / 16) + l / 2) = word;
+      }
     }
   }
 }
 
-// Eight numbers to a thread.  A code times its scale has at most 6 bits: nothing is rounded in bf16 either.
+// Eight numbers to a thread, of one head of four tokens in turn (all loads before
+// the first store).  A code times its scale has at most 6 bits: nothing is
+// rounded in bf16 either.
+constexpr int kReadTokens = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(256) kv_cache_read_kernel(CacheReadParams p) {
   const CacheView& c = p.c;
   griddep_wait();
   griddep_launch_dependents();
-  const int lanes = c.D / 8, row = lanes * c.heads;
-  const long long total = 2 * row * p.N;
-#pragma unroll 2
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-    const long long t = i / (2 * row);
-    const int rest = (int)(i - t * 2 * row), value = rest >= row, in = rest - value * row;
-    const int h = in / lanes, l = in - h * lanes;
-    const int slot = cache_slot(p.slots, p.slots64, t, c, p.status, kCacheReadKernelId);
-    float x[8] = {};
-    if (slot >= 0) {
-      const long long r = cache_row(c, slot, h);
-      const uint32_t codes = *(const uint32_t*)((value ? c.v_codes : c.k_codes) + r * (c.D / 2) + 4 * l);
-      const uint8_t byte = ((value ? c.v_scales : c.k_scales) + r * (c.D / 16))[l >> 1];
-      const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw(byte, __NV_E4M3))) * (value ? c.v_unit : c.k_unit);
+  const int lane_shift = c.D == 128 ? 4 : 3, l = threadIdx.x & ((1 << lane_shift) - 1), step = 256 >> lane_shift;
+  const bool value = blockIdx.y >= c.heads;
+  const int h = value ? blockIdx.y - c.heads : blockIdx.y;
+  const uint8_t* const codes_of = (value ? c.v_codes : c.k_codes) + 4 * l;
+  const uint8_t* const scales_of = (value ? c.v_scales : c.k_scales) + (l >> 1);
+  const float unit = value ? c.v_unit : c.k_unit;
+  const long long first = (long long)blockIdx.x * (kReadTokens * step) + (threadIdx.x >> lane_shift);
+  uint32_t codes[kReadTokens], scale[kReadTokens];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(codes >> (8 * j)), __NV_E2M1)));
-        x[2 * j] = f.x * s;
-        x[2 * j + 1] = f.y * s;
-      }
+  for (int u = 0; u < kReadTokens; ++u) {
+    const long long t = first + u * step;
+    const int slot = t < p.N ? cache_slot(p.slots, p.slots64, t, c, p.status, kCacheReadKernelId) : -1;
+    codes[u] = scale[u] = 0;
+    if (slot >= 0) {
+      const long long row = cache_row(c, slot, h);
+      codes[u] = __ldg((const uint32_t*)(codes_of + row * (c.D / 2)));
+      scale[u] = __ldg(scales_of + row * (c.D / 16));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kReadTokens; ++u) {
+    const long long t = first + u * step;
+    if (t >= p.N) return;
+    float x[8];
+    const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)scale[u], __NV_E4M3))) * unit;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(codes[u] >> (8 * j)), __NV_E2M1)));
+      x[2 * j] = f.x * s;
+      x[2 * j + 1] = f.y * s;
     }
     T* dst = value ? (T*)p.v + t * p.v_token + h * p.v_head + 8 * l : (T*)p.k + t * p.k_token + h * p.k_head + 8 * l;
     if (p.vec) {
@@ -224,18 +253,21 @@ __global__ void __launch_bounds__(256) kv_cache_read_kernel(CacheReadParams p) {
   }
 }
 
+// Tokens of a CTA: about three CTAs to an SM.
 void launch_cache_write(const CacheWriteParams& params, cudaStream_t s) {
   CacheWriteParams p = params;
-  const long long wave = 2ll * serving_sm_count();
-  p.per = (int)std::min<long long>((p.N + wave - 1) / wave, kWriteTokens);
-  const dim3 grid((unsigned)((p.N + p.per - 1) / p.per));
-  if (p.bf16) launch_with_pdl(kv_cache_write_kernel<__nv_bfloat16>, grid, dim3(kWriteThreads), 0, s, true, p);
-  else launch_with_pdl(kv_cache_write_kernel<float>, grid, dim3(kWriteThreads), 0, s, true, p);
+  const long long wave = 3ll * serving_sm_count();
+  while ((p.N >> p.per_shift) > wave && (1 << p.per_shift) < kWriteTokens) ++p.per_shift;
+  const int per = 1 << p.per_shift;
+  const dim3 grid((unsigned)((p.N + per - 1) / per));
+  const size_t smem = 5 * per * sizeof(int);
+  if (p.bf16) launch_with_pdl(kv_cache_write_kernel<__nv_bfloat16>, grid, dim3(kWriteThreads), smem, s, true, p);
+  else launch_with_pdl(kv_cache_write_kernel<float>, grid, dim3(kWriteThreads), smem, s, true, p);
 }
 
 void launch_cache_read(const CacheReadParams& p, cudaStream_t s) {
-  const long long total = 2ll * (p.c.D / 8) * p.c.heads * p.N;
-  const dim3 grid((unsigned)std::min<long long>((total + 255) / 256, 32ll * serving_sm_count()));
+  const int tokens = kReadTokens * 256 / (p.c.D / 8);
+  const dim3 grid((unsigned)((p.N + tokens - 1) / tokens), 2 * p.c.heads);
   if (p.bf16) launch_with_pdl(kv_cache_read_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, p);
   else launch_with_pdl(kv_cache_read_kernel<float>, grid, dim3(256), 0, s, true, p);
 }
