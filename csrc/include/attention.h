@@ -40,6 +40,7 @@ struct CacheWriteParams {
   int slots64, bf16, vec;            // vec: rows may be read 16 bytes at a time
   long long N;
   int per_shift;                     // a CTA has 1 << per_shift tokens, by the launch
+  float per_k_unit, per_v_unit;      // the units' reciprocals, by the launch
   DeviceStatus* status;
 };
 
@@ -50,7 +51,7 @@ struct CacheReadParams {
   void* v;
   long long k_token, k_head, v_token, v_head;
   const void* slots;
-  int slots64, bf16, vec;
+  int slots64, bf16, vec;            // vec: rows may be written 16 (1) or 32 (2) bytes at a time
   long long N;
   DeviceStatus* status;
 };

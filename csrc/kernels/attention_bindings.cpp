@@ -18,10 +18,11 @@ using namespace raiccl;
 
 bool aligned16(const torch::Tensor& t) { return ((uintptr_t)t.data_ptr() & 15) == 0; }
 
-// Rows of a tensor [n, heads, D] that start on 16 bytes.
-bool rows16(const torch::Tensor& t) {
+// Rows of a tensor [n, heads, D] that start on 16 (or 32) bytes.
+bool rows16(const torch::Tensor& t, int64_t bytes = 16) {
   const int64_t eb = t.element_size();
-  return aligned16(t) && (t.size(0) <= 1 || (t.stride(0) * eb) % 16 == 0) && (t.size(1) <= 1 || (t.stride(1) * eb) % 16 == 0);
+  return (uintptr_t)t.data_ptr() % bytes == 0 && (t.size(0) <= 1 || (t.stride(0) * eb) % bytes == 0) &&
+         (t.size(1) <= 1 || (t.stride(1) * eb) % bytes == 0);
 }
 
 // A tensor to be written whose elements share no memory with each other: some order of its dimensions nests.
@@ -91,6 +92,7 @@ CacheView check_cache(const char* op, const Cache& c, const torch::Device& dev) 
   TORCH_CHECK_VALUE(page >= kCachePage && page <= 65536 && (page & (page - 1)) == 0, op, ": page_size must be a power of two from 16 to 65536, got ",
                     text(page));
   TORCH_CHECK_VALUE(heads >= 1 && heads <= 1024, op, ": 1 to 1024 kv_heads, got ", text(heads));
+  TORCH_CHECK_VALUE(heads * page <= (1 << 24), op, ": kv_heads times page_size must be at most 2^24");
   TORCH_CHECK_VALUE(pages < (1ll << 31) / page, op, ": the cache must have less than 2^31 places");
   codes("k_codes", c.k_codes);
   codes("v_codes", c.v_codes);
@@ -197,7 +199,7 @@ std::tuple<torch::Tensor, torch::Tensor> kv_cache_read(torch::Tensor k_codes, to
   p.slots = slots.data_ptr();
   p.slots64 = slots.scalar_type() == torch::kInt64;
   p.bf16 = dt == torch::kBFloat16;
-  p.vec = rows16(k) && rows16(v);
+  p.vec = rows16(k, 32) && rows16(v, 32) ? 2 : rows16(k) && rows16(v) ? 1 : 0;
   p.N = N;
   p.status = serving_status();
   launch_cache_read(p, at::cuda::getCurrentCUDAStream());

@@ -5,11 +5,11 @@
 // in one pass over the cache, with the running maximum m and sum l of a softmax.
 // The floor is the cache's own bytes, 9/16 of a byte a number.
 //
-// Work.  Tiles of 32 tokens of one sequence and one key head, in the order of
+// Work.  Tiles of 64 tokens of one sequence and one key head, in the order of
 // sequences and heads, are dealt to the CTAs in equal contiguous shares, and a
 // CTA's share to its warps.  A warp is on its own from the first tile to the
-// last: it copies its tiles to its own ring in shared memory (cp.async.bulk),
-// and meets no other warp before its share is done.  What it has of a sequence
+// last: it copies its tiles to its own ring in shared memory (cp.async), and meets
+// no other before its share is done.  What it has of a sequence
 // whose tiles others have too is joined then, in a fixed order: within the CTA
 // through shared memory, between CTAs by a second, small kernel.
 //
@@ -39,6 +39,7 @@
 #include <algorithm>
 #include <atomic>
 #include <stdexcept>
+#include <type_traits>
 
 #include "attention.h"
 #include "serving.h"
@@ -47,27 +48,35 @@
 
 namespace raiccl {
 
-constexpr int kCachedTile = 32;
-constexpr unsigned long long kCachedWaitNs = 2000000000ull;
+constexpr int kCachedTile = 64;
 // Probabilities are exp2(z - m + 7) and m follows the maximum once that passes 15: f16 holds them (below 2^15), and small
 // ones keep their bits down to 2^-21 of the largest.
 constexpr float kCachedHead = 7.f, kCachedRoom = 15.f;
 
 // Warps of a CTA, by the registers that queries, sums and the operands in flight take.
-template <int D, int NT, int PARTS>
-constexpr int kCachedWarps = NT == 1 && PARTS == 1 ? 16 : 8;
+template <int NT, int PARTS>
+constexpr int kCachedWarps = NT == 1 && PARTS == 1 ? 12 : 8;
 
 template <int D, int NT, int PARTS>
 struct Cached {
-  static constexpr int WARPS = kCachedWarps<D, NT, PARTS>, THREADS = 32 * WARPS;
+  static constexpr int WARPS = kCachedWarps<NT, PARTS>, THREADS = 32 * WARPS;
   static constexpr int HEADS = 8 * NT;                       // query heads of a chunk at most
   static constexpr int CODES = kCachedTile * D / 2, SCALES = kCachedTile * D / 16;
   static constexpr int STAGE = 2 * (CODES + SCALES);         // K codes, V codes, K scales, V scales
   static constexpr int PART = HEADS * D * 4;                 // a warp's sums of a sequence that it shares
-  static constexpr int STAGES = 216 * 1024 / (WARPS * STAGE) < 6 ? 216 * 1024 / (WARPS * STAGE) : 6;
+  static constexpr int STAGES = 216 * 1024 / (WARPS * STAGE) < 4 ? 216 * 1024 / (WARPS * STAGE) : 4;
   static constexpr int SMEM = WARPS * STAGES * STAGE;
-  static_assert(STAGES >= 3 && STAGES * STAGE >= PART, "the ring holds the warp's last part too");
+  static_assert(STAGES >= 2 && STAGES * STAGE >= PART, "the ring holds the warp's last part too");
 };
+
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -190,17 +199,11 @@ template <int D, int NT, int PARTS>
 __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kernel(CachedParams p) {
   using C = Cached<D, NT, PARTS>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t full[C::WARPS][C::STAGES];
-  __shared__ int pages_ok[C::WARPS][C::STAGES];
   __shared__ long long before[C::THREADS + 1], sum_of[C::WARPS];
   __shared__ CachedPart part[C::WARPS][2];
   __shared__ float2 stat[C::WARPS][2][C::HEADS];
   __shared__ int nonempty[C::WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
-  if (lane < C::STAGES) mbar_init(&full[warp][lane], 1);
-  fence_mbarrier_init();
-  __syncwarp();
   griddep_wait();
   griddep_launch_dependents();
 
@@ -233,12 +236,29 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
   const int ctas = cached_ctas(tiles, p.ctas);
   if ((int)blockIdx.x >= ctas) return;
   const long long c0 = cached_first(tiles, ctas, blockIdx.x), c1 = cached_first(tiles, ctas, blockIdx.x + 1);
-  const long long u0 = c0 + (c1 - c0) * warp / C::WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
-  const int count = (int)(u1 - u0);
   // A warp's part of a sequence: the one that began before its share (0), the one that ends after it (1).  The last that it
   // works on goes into its ring, which is done then; a first one with others behind it to device memory.
   auto spilled = [&](int w) { return p.spill + ((long long)blockIdx.x * C::WARPS + w) * (C::HEADS * D); };
   auto ringed = [&](int w) { return (float*)(smem + w * C::STAGES * C::STAGE); };
+  auto piece_at = [&](long long u) {
+    int lo = 0, hi = C::THREADS;     // before[lo] <= u < before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (before[mid] <= u) lo = mid; else hi = mid;
+    }
+    long long first = before[lo];
+    int b = lo * per, n = cached_tiles(p, b);
+    while (first + (long long)n * HC <= u) {
+      first += (long long)n * HC;
+      n = cached_tiles(p, ++b);
+    }
+    const int hc = (int)((u - first) / n);
+    return CachedPiece{b, hc, n, first + (long long)hc * n};
+  };
+
+  const long long u0 = c0 + (c1 - c0) * warp / C::WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
+  const int count = (int)(u1 - u0);
+  uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
   if (lane == 0) {
     part[warp][0].used = part[warp][1].used = 0;
     nonempty[warp] = count > 0;
@@ -246,38 +266,37 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
   __syncwarp();
 
   if (count > 0) {
-    CachedPiece piece;
-    {
-      int lo = 0, hi = C::THREADS;   // before[lo] <= u0 < before[hi]
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (before[mid] <= u0) lo = mid; else hi = mid;
-      }
-      long long first = before[lo];
-      int b = lo * per, n = cached_tiles(p, b);
-      while (first + (long long)n * HC <= u0) {
-        first += (long long)n * HC;
-        n = cached_tiles(p, ++b);
-      }
-      const int hc = (int)((u0 - first) / n);
-      piece = {b, hc, n, first + (long long)hc * n};
-    }
+    CachedPiece piece = piece_at(u0);
 
     // ---------------------------------------------------------- copies, STAGES tiles ahead
-    // One copy to a lane: lanes 0 to 3 the four arrays, of the tile or of its first sixteen tokens, 4 to 7 of the others.
-    const int page_size = 1 << p.c.page_shift;
-    const bool whole = page_size >= kCachedTile;   // a tile lies in one page
-    const int what = lane & 3, half16 = 16 * ((lane >> 2) & 1);
-    const int width = what < 2 ? D / 2 : D / 16;
-    const uint8_t* const array = what == 0 ? p.c.k_codes : what == 1 ? p.c.v_codes : what == 2 ? p.c.k_scales : p.c.v_scales;
-    const uint32_t copy_at = (what < 2 ? what * C::CODES : 2 * C::CODES + (what - 2) * C::SCALES) + half16 * width;
-    const bool copier = lane < (whole ? 4 : 8);
+    // Sixteen bytes to a lane and copy.  Of a tile, or of the page that is a part of it: K codes, V codes, the scales of both.
+    const uint32_t page_mask = (1u << p.c.page_shift) - 1, page_bytes = ((uint32_t)p.c.heads << p.c.page_shift) * (D / 2);
+    const uint32_t ring_at = smem_u32(ring);
+    auto copy = [&](uint32_t stage_at, int row_to, int page, uint32_t row, auto rows_of) {
+      constexpr int ROWS = decltype(rows_of)::value, SCALES = ROWS * (D / 16), N = SCALES / 16;
+      const unsigned long long off = (unsigned long long)(uint32_t)page * page_bytes + row * (D / 2);
+      const uint8_t *k = p.c.k_codes + off + lane * 16, *v = p.c.v_codes + off + lane * 16;
+      const uint32_t to = stage_at + row_to * (D / 2) + lane * 16;
+#pragma unroll
+      for (int i = 0; i < ROWS * (D / 2); i += 512) {
+        cp_async16(to + i, k + i);
+        cp_async16(to + C::CODES + i, v + i);
+      }
+      const uint32_t mine = (lane & (N - 1)) * 16, st = stage_at + 2 * C::CODES + row_to * (D / 16) + mine;
+      if constexpr (N == 32) {
+        cp_async16(st, p.c.k_scales + (off >> 3) + mine);
+        cp_async16(st + C::SCALES, p.c.v_scales + (off >> 3) + mine);
+      } else if (lane < 2 * N) {                   // both in one copy
+        cp_async16(st + (lane < N ? 0 : C::SCALES), (lane < N ? p.c.k_scales : p.c.v_scales) + (off >> 3) + mine);
+      }
+    };
     CachedPiece ahead = piece;
     int ahead_len = cached_length(p, piece.b), ahead_at = (int)(u0 - piece.first) * kCachedTile;   // the next copy's tokens
     int ahead_end = (int)min((long long)count, piece.first + piece.n - u0);                         // tiles of the share up to the piece's end
     const int* ahead_pages = p.table + (long long)piece.b * p.table_stride;
-    long long ahead_row = (long long)(piece.hc / p.chunks) << p.c.page_shift;
+    uint32_t ahead_row = (uint32_t)(piece.hc / p.chunks) << p.c.page_shift;
     int issued = 0, fill = 0;
+    uint32_t missing = 0;                          // sixteens of tokens without a page of the cache: four bits to a stage
     auto issue = [&]() {
       if (issued == ahead_end) {
         next_piece(p, ahead);
@@ -285,33 +304,39 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         ahead_at = 0;
         ahead_end = (int)min((long long)count, (long long)ahead_end + ahead.n);
         ahead_pages = p.table + (long long)ahead.b * p.table_stride;
-        ahead_row = (long long)(ahead.hc / p.chunks) << p.c.page_shift;
+        ahead_row = (uint32_t)(ahead.hc / p.chunks) << p.c.page_shift;
       }
-      const int at = ahead_at + half16;
-      int page = -1;
-      if (lane < 8 && at < ahead_len) {
-        page = __ldg(ahead_pages + (at >> p.c.page_shift));
-        if (page < 0 || page >= p.c.pages) {
-          if (what == 0) record_status(p.status, kBoundsViolation, kCachedKernelId, page, p.c.pages);
-          page = -1;
+      const uint32_t stage_at = ring_at + fill * C::STAGE;
+      uint32_t lost = 0;
+      auto part = [&](int row_to, auto rows_of) {  // as many of the tile's tokens as lie in one page
+        constexpr int ROWS = decltype(rows_of)::value;
+        const int at = ahead_at + row_to;
+        const int page = at < ahead_len ? __ldg(ahead_pages + (at >> p.c.page_shift)) : -1;
+        if ((uint32_t)page < (uint32_t)p.c.pages) {
+          copy(stage_at, row_to, page, ahead_row + (at & page_mask), rows_of);
+          return;
         }
+        lost |= ((1u << ROWS / 16) - 1) << (row_to / 16);
+        if (at < ahead_len && lane == 0) record_status(p.status, kBoundsViolation, kCachedKernelId, page, p.c.pages);
+      };
+      if (p.c.page_shift >= 6) {
+        part(0, std::integral_constant<int, 64>{});
+      } else if (p.c.page_shift == 5) {
+#pragma unroll 1
+        for (int r = 0; r < kCachedTile; r += 32) part(r, std::integral_constant<int, 32>{});
+      } else {
+#pragma unroll 1
+        for (int r = 0; r < kCachedTile; r += 16) part(r, std::integral_constant<int, 16>{});
       }
-      const uint32_t have = __ballot_sync(0xffffffffu, page >= 0);
-      if (lane == 0) {
-        const int ok = whole ? (have & 1u ? 3 : 0) : (have & 1u ? 1 : 0) | (have & 16u ? 2 : 0);
-        pages_ok[warp][fill] = ok;
-        mbar_arrive_expect_tx(&full[warp][fill], __popc(ok) * 16 * (2 * (D / 2) + 2 * (D / 16)));
-      }
-      __syncwarp();
-      if (copier && page >= 0) {
-        const long long row = ((long long)page * p.c.heads << p.c.page_shift) + ahead_row + (at & (page_size - 1));
-        bulk_load_g2s(ring + fill * C::STAGE + copy_at, array + row * width, (whole ? kCachedTile : 16) * width, &full[warp][fill]);
-      }
+      missing = (missing & ~(15u << (4 * fill))) | lost << (4 * fill);
       ++issued;
       ahead_at += kCachedTile;
       fill = fill + 1 == C::STAGES ? 0 : fill + 1;
     };
-    while (issued < count && issued < C::STAGES) issue();
+    for (int i = 0; i < C::STAGES; ++i) {
+      if (issued < count) issue();
+      cp_async_commit();
+    }
 
     // ---------------------------------------------------------- tiles
     constexpr int KS = D / 16;         // products of a row of sixteen tokens over D
@@ -436,7 +461,6 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
     begin();
     int done = 0, stage = 0, end = (int)min((long long)count, piece.first + piece.n - u0);
     int left = cached_length(p, piece.b) - (int)(u0 - piece.first) * kCachedTile;   // tokens of the piece from this tile on
-    uint32_t phase = 0;
 #pragma unroll 1
     for (; done < count; ++done) {
       if (done == end) {
@@ -446,23 +470,34 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         end = (int)min((long long)count, (long long)end + piece.n);
         left = cached_length(p, piece.b);
       }
-      if (!mbar_wait_warp(&full[warp][stage], phase, p.status, kCachedKernelId, kCachedWaitNs)) break;
+      cp_async_wait<C::STAGES - 1>();
+      __syncwarp();
       uint8_t* const s = ring + stage * C::STAGE;
-      const int ok = pages_ok[warp][stage];
-      const bool all = left >= kCachedTile && ok == 3;
-      uint32_t rows = 0xffffffffu;     // tokens of the tile that the sequence has
+      const uint32_t lost = missing >> (4 * stage) & 15;
+      const bool all = left >= kCachedTile && lost == 0;
+      auto seen_at = [&](int row) -> uint32_t {      // tokens row .. row + 31 of the tile that the sequence has
+        const int n = left - row;
+        uint32_t has = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+        if (lost >> (row / 16) & 1) has &= 0xffff0000u;
+        if (lost >> (row / 16) & 2) has &= 0x0000ffffu;
+        return has;
+      };
       if (!all) {
-        rows = left >= kCachedTile ? 0xffffffffu : (1u << left) - 1;
-        rows &= (ok & 1 ? 0xffffu : 0u) | (ok & 2 ? 0xffff0000u : 0u);
         // a page's rest may hold anything: its values count as zeros
-        if (!(rows >> lane & 1)) {
-          if constexpr (D == 128) *(uint2*)(s + 2 * C::CODES + C::SCALES + lane * 8) = make_uint2(0, 0);
-          else *(uint32_t*)(s + 2 * C::CODES + C::SCALES + lane * 4) = 0;
+#pragma unroll
+        for (int row = 0; row < kCachedTile; row += 32) {
+          if (seen_at(row) >> lane & 1) continue;
+          uint8_t* const scales = s + 2 * C::CODES + C::SCALES + (row + lane) * (D / 16);
+          if constexpr (D == 128) *(uint2*)scales = make_uint2(0, 0);
+          else *(uint32_t*)scales = 0;
         }
-        fence_proxy_async_smem();
         __syncwarp();
       }
-      if (rows != 0) {
+#pragma unroll 1
+      for (int half = 0; half < kCachedTile; half += 32) {   // 32 tokens at a time, by the registers that more would take
+        const uint32_t seen = all ? 0xffffffffu : seen_at(half);
+        if (seen == 0) continue;
+        const uint8_t *const sk = s + half * (D / 2), *const ss = s + 2 * C::CODES + half * (D / 16);
         float z[2][NT][4];
         // -------------------------------------------------- S^T = K Q^T
 #pragma unroll
@@ -476,15 +511,15 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
           for (int r = 0; r < 2; ++r) {
             const int row = 16 * mt + 8 * r + g;
             if constexpr (D == 128) {
-              const uint4 v = *(const uint4*)(s + row * 64 + 16 * t);
+              const uint4 v = *(const uint4*)(sk + row * 64 + 16 * t);
               w[r][0] = v.x; w[r][1] = v.y; w[r][2] = v.z; w[r][3] = v.w;
-              const uint32_t two = scales_f16(*(const uint16_t*)(s + 2 * C::CODES + row * 8 + 2 * t));
+              const uint32_t two = scales_f16(*(const uint16_t*)(ss + row * 8 + 2 * t));
               sc[r][0] = __byte_perm(two, two, 0x1010);
               sc[r][1] = __byte_perm(two, two, 0x3232);
             } else {
-              const uint2 v = *(const uint2*)(s + row * 32 + 8 * t);
+              const uint2 v = *(const uint2*)(sk + row * 32 + 8 * t);
               w[r][0] = v.x; w[r][1] = v.y;
-              const uint32_t two = scales_f16(s[2 * C::CODES + row * 4 + t]);
+              const uint32_t two = scales_f16(ss[row * 4 + t]);
               sc[r][0] = __byte_perm(two, two, 0x1010);
             }
           }
@@ -525,7 +560,7 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
               for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  if (!(rows >> (16 * mt + 8 * (j >> 1) + g) & 1)) x[mt][nt][j] = -INFINITY;
+                  if (!(seen >> (16 * mt + 8 * (j >> 1) + g) & 1)) x[mt][nt][j] = -INFINITY;
           }
         };
         below();
@@ -546,7 +581,7 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
               for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int r = 0; r < 2; ++r)
-                  if (rows >> (16 * mt + 8 * r + g) & 1) top = fmaxf(top, z[mt][nt][j + 2 * r] * mult[nt][j]);
+                  if (seen >> (16 * mt + 8 * r + g) & 1) top = fmaxf(top, z[mt][nt][j + 2 * r] * mult[nt][j]);
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
               top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -602,12 +637,12 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
             for (int e = 0; e < 2; ++e) {
               const int row = 16 * mt + 8 * r + 2 * t + e;
               if constexpr (D == 128) {
-                const uint2 v = *(const uint2*)(s + C::CODES + row * 64 + 8 * g);
+                const uint2 v = *(const uint2*)(sk + C::CODES + row * 64 + 8 * g);
                 y[e][0] = v.x; y[e][1] = v.y;
-                byte[e] = s[2 * C::CODES + C::SCALES + row * 8 + g];
+                byte[e] = ss[C::SCALES + row * 8 + g];
               } else {
-                y[e][0] = *(const uint32_t*)(s + C::CODES + row * 32 + 4 * g);
-                byte[e] = s[2 * C::CODES + C::SCALES + row * 4 + (g >> 1)];
+                y[e][0] = *(const uint32_t*)(sk + C::CODES + row * 32 + 4 * g);
+                byte[e] = ss[C::SCALES + row * 4 + (g >> 1)];
               }
             }
             sv[r] = scales_f16(byte[0] | byte[1] << 8);
@@ -649,12 +684,11 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         }
       }
       left -= kCachedTile;
-      if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
-      __syncwarp();   // every lane has read the stage
+      if (++stage == C::STAGES) stage = 0;
+      __syncwarp();   // every lane has read the tile
       if (issued < count) issue();
+      cp_async_commit();
     }
-    for (int i = done; i < issued; ++i)   // after a wait that ran out: the copies in flight land before the ring is used again
-      mbar_wait_warp(&full[warp][i % C::STAGES], (i / C::STAGES) & 1, p.status, kCachedKernelId, kCachedWaitNs);
     finish(true);
   }
 
@@ -785,7 +819,7 @@ CachedPlan plan_cached(const CachedParams& p, int sms) {
   plan.ctas = sms;
   plan.parts_bytes = (long long)plan.ctas * 2 * plan.chunk * p.c.D * 4;
   plan.stats_bytes = ((long long)plan.ctas * 2 * plan.chunk * 8 + 255) / 256 * 256;
-  const int warps = most == 16 && plan.chunk <= 8 ? kCachedWarps<128, 1, 1> : most == 16 ? kCachedWarps<128, 2, 1> : kCachedWarps<128, 1, 2>;
+  const int warps = most == 8 ? kCachedWarps<1, 2> : plan.chunk <= 8 ? kCachedWarps<1, 1> : kCachedWarps<2, 1>;
   plan.spill_bytes = (long long)plan.ctas * warps * (plan.chunk > 8 ? 16 : 8) * p.c.D * 4;
   return plan;
 }

@@ -12,13 +12,14 @@
 // 2 m' / T' > 1.06 remains between them (T' < 2 the leading digits of T, at most
 // 15/8 where m' is 1).  The same holds for the scale, with 6 in the place of s.
 //
-// Both kernels only move memory: eight numbers to a thread, 16 bytes in and 4
-// out for bf16.
+// Both kernels only move memory: a scale's sixteen numbers to a thread, 32 bytes
+// of bf16 on one side and 9 on the other.
 #include <cuda_fp16.h>
-#include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <climits>
+#include <type_traits>
 
 #include "attention.h"
 #include "serving.h"
@@ -27,7 +28,7 @@
 
 namespace raiccl {
 
-constexpr int kWriteThreads = 512;
+constexpr int kWriteThreads = 256;
 constexpr int kWriteTokens = 2048;         // of a CTA at most
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -48,56 +49,88 @@ __device__ __forceinline__ int cache_slot(const void* slots, int wide, long long
   return (int)s;
 }
 
-// Row (of D numbers) of a head's token in the cache.
-__device__ __forceinline__ long long cache_row(const CacheView& c, int slot, int head) {
-  const int page = slot >> c.page_shift, at = slot & ((1 << c.page_shift) - 1);
-  return ((((long long)page * c.heads + head) << c.page_shift) + at);
+// Byte offset of a head's token in the codes; its scales lie at an eighth of it.  A page has less than 2^31 bytes.
+template <int D>
+__device__ __forceinline__ long long cache_offset(const CacheView& c, int slot, int head) {
+  const uint32_t page = slot >> c.page_shift, at = slot & ((1 << c.page_shift) - 1);
+  return (long long)((unsigned long long)page * (((uint32_t)c.heads << c.page_shift) * (uint32_t)(D / 2))) +
+         (((uint32_t)head << c.page_shift) + at) * (uint32_t)(D / 2);
 }
 
+// Sixteen numbers of one row.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int vec, float (&x)[8]) {
+__device__ __forceinline__ void load16(const T* p, int vec, float (&x)[16]) {
   if (vec) {
     constexpr int W = 16 / sizeof(T);
+    uint4 v[16 / W];
 #pragma unroll
-    for (int i = 0; i < 8; i += W) {
+    for (int i = 0; i < 16 / W; ++i) v[i] = __ldg((const uint4*)p + i);
+#pragma unroll
+    for (int i = 0; i < 16 / W; ++i) {
       float f[W];
-      unpack16<T>(*(const uint4*)(p + i), f);
+      unpack16<T>(v[i], f);
 #pragma unroll
-      for (int j = 0; j < W; ++j) x[i + j] = f[j];
+      for (int j = 0; j < W; ++j) x[W * i + j] = f[j];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = as_float(p[i]);
+    for (int i = 0; i < 16; ++i) x[i] = as_float(p[i]);
   }
 }
 
-// Two lanes have a group of sixteen: its scale (both get it) and this lane's eight codes.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float unit, float per_unit, uint32_t& scale) {
+// x / s from the rounded reciprocal r of s: the product, and one correction by its remainder, which is exact in an fma
+// (P. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990).  At x = m s it is m: the
+// remainder is (m - q) s, and what it adds is off by 2^-24 of a step.  Where it underflows the code is 0 anyway.
+__device__ __forceinline__ float divide(float x, float s, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-s, q, x), r, q);
+}
+
+// Four bytes of two codes each as f16 pairs, and eight fp32 numbers as codes; lower code first.
+__device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+}
+
+__device__ __forceinline__ uint32_t codes_from_f32(const float* q) {
+  uint32_t w;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(w)
+      : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+  return w;
+}
+
+// The scale (returned, a byte) and the codes of sixteen numbers.
+__device__ __forceinline__ uint32_t quantise16(float (&x)[16], float unit, float per_unit, uint32_t (&codes)[2]) {
   float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(x[i]));
-  top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, 1)) * per_unit;
-  scale = __nv_cvt_float_to_fp8(__fdiv_rn(top, 6.f), __NV_SATFINITE, __NV_E4M3);
+  for (int i = 0; i < 16; ++i) top = max_nan(top, fabsf(x[i]));
+  top *= per_unit;
+  if (top > 8192.f) {                 // behind 448 * 6 everything saturates; cut here, infinities do not meet below
+    const float most = 8192.f * unit;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = fminf(fmaxf(x[i], -most), most);
+    top = 8192.f;
+  }
+  const uint32_t scale = __nv_cvt_float_to_fp8(divide(top, 6.f, 1.f / 6.f), __NV_SATFINITE, __NV_E4M3);
   const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)scale, __NV_E4M3)));
   const float r = s > 0.f ? __frcp_rn(s) * per_unit : 0.f, back = s * unit;
-  // Behind 448 * 6 everything saturates; there numbers are cut, so that no infinities meet below.
-  const float most = 8192.f * unit;
-  const bool cut = top > 8192.f;
-  uint32_t codes = 0;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    float q[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float v = cut ? fminf(fmaxf(x[i + j], -most), most) : x[i + j];
-      // x / s: the product by the rounded reciprocal, and one correction by its remainder, which is exact in an fma
-      // (P. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990).
-      q[j] = v * r;
-      q[j] = fmaf(fmaf(-back, q[j], v), r, q[j]);
-    }
-    codes |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(q[0], q[1]), __NV_E2M1, cudaRoundNearest) << (4 * i);
-  }
-  return codes;
+  for (int i = 0; i < 16; ++i) x[i] = divide(x[i], back, r);
+  codes[0] = codes_from_f32(x);
+  codes[1] = codes_from_f32(x + 8);
+  return scale;
 }
 
 // A CTA has `per` consecutive tokens (a power of two).  Where several tokens of
@@ -105,10 +138,10 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], float unit, f
 // slots into a hash table, the highest token of each, and looks up all later
 // tokens' slots in it.
 //
-// A row of a head is D / 8 lanes; rows go by value or key, head and token, the
-// token fastest, so that no index needs a division.  Four rows to a thread are
-// loaded before the first is worked on.
-template <typename T>
+// Sixteen numbers to a thread, D / 16 lanes to a row of a head; rows go by value
+// or key, head and token, the token fastest, so that no index needs a division.
+// Two rows to a thread are loaded before the first is worked on.
+template <typename T, int D>
 __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWriteParams p) {
   extern __shared__ int table[];      // [per] slots, [size] keys, [size] last tokens
   const CacheView& c = p.c;
@@ -118,6 +151,8 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
   int *slot_of = table, *key = table + per, *last = key + size;
   const long long first = (long long)blockIdx.x << p.per_shift;
   const int n = (int)(p.N - first < per ? p.N - first : per);
+  __shared__ int range[2];            // the least and the largest slot of the CTA's tokens
+  if (threadIdx.x == 0) { range[0] = INT_MAX; range[1] = -1; }
   for (int i = threadIdx.x; i < size; i += kWriteThreads) { key[i] = -1; last[i] = -1; }
   __syncthreads();
   auto at = [&](int slot) { return (int)(((uint32_t)slot * 2654435761u) >> 16) & (size - 1); };
@@ -132,17 +167,42 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
       e = (e + 1) & (size - 1);
     }
     atomicMax(&last[e], i);
+    atomicMin(&range[0], s);
+    atomicMax(&range[1], s);
   }
   __syncthreads();
-  const long long bound = (long long)c.pages << c.page_shift;
-#pragma unroll 4
-  for (long long i = first + n + threadIdx.x; i < p.N; i += kWriteThreads) {
-    const long long wide = p.slots64 ? ((const long long*)p.slots)[i] : (long long)((const int*)p.slots)[i];
-    if (wide < 0 || wide >= bound) continue;
+  const long long low = range[0], high = range[1];
+  auto look = [&](long long wide) {
+    if (wide < low || wide > high) return;     // most of them: a CTA's tokens are neighbours in few pages
     const int s = (int)wide;
     int e = at(s), k;
     while ((k = key[e]) != -1 && k != s) e = (e + 1) & (size - 1);
-    if (k == s) last[e] = 1 << 30;    // a later CTA has it
+    if (k == s) last[e] = 1 << 30;             // a later CTA has it
+  };
+  auto scan = [&](auto* slots) {
+    // four at a time, eight such loads in flight; the tensor starts on the type's alignment only, and ends anywhere
+    using S = std::remove_cv_t<std::remove_pointer_t<decltype(slots)>>;
+    long long from = first + n;
+    while (from < p.N && ((uintptr_t)(slots + from) & 15)) ++from;
+    for (long long i = first + n + threadIdx.x; i < from; i += kWriteThreads) look(slots[i]);
+    constexpr int V = 16 / sizeof(S), L = 8;
+    const long long words = from < p.N ? (p.N - from) / V : 0;
+    const uint4* const w = (const uint4*)(slots + from);
+    for (long long i = threadIdx.x; i < words; i += L * kWriteThreads) {
+      uint4 v[L];
+#pragma unroll
+      for (int u = 0; u < L; ++u)
+        v[u] = i + u * kWriteThreads < words ? __ldg(w + i + u * kWriteThreads) : make_uint4(~0u, ~0u, ~0u, ~0u);   // -1: none
+#pragma unroll
+      for (int u = 0; u < L; ++u)
+#pragma unroll
+        for (int e = 0; e < V; ++e) look(((const S*)&v[u])[e]);
+    }
+    for (long long i = from + words * V + threadIdx.x; i < p.N; i += kWriteThreads) look(slots[i]);
+  };
+  if (high >= 0) {
+    if (p.slots64) scan((const long long*)p.slots);
+    else scan((const int*)p.slots);
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kWriteThreads) {
@@ -153,11 +213,11 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
     if (last[e] != i) slot_of[i] = -1;
   }
   __syncthreads();
-  const int lane_shift = c.D == 128 ? 4 : 3, l = threadIdx.x & ((1 << lane_shift) - 1);
-  const int step = kWriteThreads >> lane_shift, rows = 2 * c.heads << p.per_shift;
-  constexpr int U = 4;
+  constexpr int lane_shift = D == 128 ? 3 : 2, step = kWriteThreads >> lane_shift;
+  const int l = threadIdx.x & ((1 << lane_shift) - 1), rows = 2 * c.heads << p.per_shift;
+  constexpr int U = 2;
   for (int r0 = 0; r0 < rows; r0 += U * step) {
-    float x[U][8];
+    float x[U][16];
     int slot[U], hv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -165,90 +225,108 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
       hv[u] = r >> p.per_shift;
       slot[u] = r < rows ? slot_of[t] : -1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+      for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
       if (slot[u] >= 0) {
         const T* src = hv[u] < c.heads ? (const T*)p.k + (first + t) * p.k_token + hv[u] * p.k_head
                                        : (const T*)p.v + (first + t) * p.v_token + (hv[u] - c.heads) * p.v_head;
-        load8(src + 8 * l, p.vec, x[u]);
+        load16(src + 16 * l, p.vec, x[u]);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (r0 + u * step >= rows) break;              // the same for all threads
       const bool value = hv[u] >= c.heads;
-      const float unit = value ? c.v_unit : c.k_unit;
-      uint32_t scale;
-      const uint32_t codes = quantise8(x[u], unit, 1.f / unit, scale);
-      uint32_t word = scale << (8 * ((l >> 1) & 3));   // four groups' scales, eight lanes
+      uint32_t codes[2], word = 0;
+      if (slot[u] >= 0) word = quantise16(x[u], value ? c.v_unit : c.k_unit, value ? p.per_v_unit : p.per_k_unit, codes);
+      word <<= 8 * (l & 3);             // four lanes' scales to a word; a row's lanes have one slot
+      word |= __shfl_xor_sync(0xffffffffu, word, 1);
       word |= __shfl_xor_sync(0xffffffffu, word, 2);
-      word |= __shfl_xor_sync(0xffffffffu, word, 4);
       if (slot[u] >= 0) {
-        const long long at_row = cache_row(c, slot[u], value ? hv[u] - c.heads : hv[u]);
-        *(uint32_t*)((value ? c.v_codes : c.k_codes) + at_row * (c.D / 2) + 4 * l) = codes;
-        if ((l & 7) == 0) *(uint32_t*)((value ? c.v_scales : c.k_scales) + at_row * (c.D / 16) + l / 2) = word;
+        const long long off = cache_offset<D>(c, slot[u], value ? hv[u] - c.heads : hv[u]);
+        *(uint2*)((value ? c.v_codes : c.k_codes) + off + 8 * l) = make_uint2(codes[0], codes[1]);
+        if ((l & 3) == 0) *(uint32_t*)((value ? c.v_scales : c.k_scales) + (off >> 3) + l) = word;
       }
     }
   }
 }
 
-// Eight numbers to a thread, of one head of four tokens in turn (all loads before
-// the first store).  A code times its scale has at most 6 bits: nothing is
+// Sixteen numbers to a thread, of one head of four tokens in turn (all loads
+// before the first store).  A code times its scale has at most 6 bits: nothing is
 // rounded in bf16 either.
 constexpr int kReadTokens = 4;
 
-template <typename T>
+template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_cache_read_kernel(CacheReadParams p) {
   const CacheView& c = p.c;
   griddep_wait();
   griddep_launch_dependents();
-  const int lane_shift = c.D == 128 ? 4 : 3, l = threadIdx.x & ((1 << lane_shift) - 1), step = 256 >> lane_shift;
+  constexpr int lane_shift = D == 128 ? 3 : 2, step = 256 >> lane_shift;
+  const int l = threadIdx.x & ((1 << lane_shift) - 1);
   const bool value = blockIdx.y >= c.heads;
   const int h = value ? blockIdx.y - c.heads : blockIdx.y;
-  const uint8_t* const codes_of = (value ? c.v_codes : c.k_codes) + 4 * l;
-  const uint8_t* const scales_of = (value ? c.v_scales : c.k_scales) + (l >> 1);
+  const uint8_t* const codes_of = (value ? c.v_codes : c.k_codes) + 8 * l;
+  const uint8_t* const scales_of = (value ? c.v_scales : c.k_scales) + l;
   const float unit = value ? c.v_unit : c.k_unit;
   const long long first = (long long)blockIdx.x * (kReadTokens * step) + (threadIdx.x >> lane_shift);
-  uint32_t codes[kReadTokens], scale[kReadTokens];
+  uint2 codes[kReadTokens];
+  uint32_t scale[kReadTokens];
 #pragma unroll
   for (int u = 0; u < kReadTokens; ++u) {
     const long long t = first + u * step;
     const int slot = t < p.N ? cache_slot(p.slots, p.slots64, t, c, p.status, kCacheReadKernelId) : -1;
-    codes[u] = scale[u] = 0;
+    codes[u] = make_uint2(0, 0);
+    scale[u] = 0;
     if (slot >= 0) {
-      const long long row = cache_row(c, slot, h);
-      codes[u] = __ldg((const uint32_t*)(codes_of + row * (c.D / 2)));
-      scale[u] = __ldg(scales_of + row * (c.D / 16));
+      const long long off = cache_offset<D>(c, slot, h);
+      codes[u] = __ldg((const uint2*)(codes_of + off));
+      scale[u] = __ldg(scales_of + (off >> 3));
     }
   }
+  const long long token = value ? p.v_token : p.k_token;
+  T* dst = (value ? (T*)p.v + h * p.v_head : (T*)p.k + h * p.k_head) + first * token + 16 * l;
 #pragma unroll
-  for (int u = 0; u < kReadTokens; ++u) {
-    const long long t = first + u * step;
-    if (t >= p.N) return;
-    float x[8];
-    const float s = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)scale[u], __NV_E4M3))) * unit;
+  for (int u = 0; u < kReadTokens; ++u, dst += step * token) {
+    if (first + u * step >= p.N) return;
+    uint32_t s = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)scale[u], __NV_E4M3).x;
+    s |= s << 16;
+    uint32_t half[2][4];
+    codes_to_f16(codes[u].x, half[0]);
+    codes_to_f16(codes[u].y, half[1]);
+    float x[16];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(codes[u] >> (8 * j)), __NV_E2M1)));
-      x[2 * j] = f.x * s;
-      x[2 * j + 1] = f.y * s;
+    for (int j = 0; j < 8; ++j) {
+      const float2 f = __half22float2(__hmul2(*(const __half2*)&half[j / 4][j % 4], *(const __half2*)&s));   // exact
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
     }
-    T* dst = value ? (T*)p.v + t * p.v_token + h * p.v_head + 8 * l : (T*)p.k + t * p.k_token + h * p.k_head + 8 * l;
+    if (unit != 1.f) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] *= unit;
+    }
     if (p.vec) {
       if constexpr (sizeof(T) == 2) {
-        uint32_t w[4];
+        uint32_t w[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 8; ++j) {
           const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
           w[j] = *(const uint32_t*)&b;
         }
-        *(uint4*)dst = make_uint4(w[0], w[1], w[2], w[3]);
+        // all 32 bytes in one instruction where they are a sector: in two, each of which has a half of every sector of its
+        // warp, the load-store unit was the limit (65536 tokens: 80 us)
+        if (p.vec == 2) {
+          asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                       "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                       : "memory");
+        } else {
+          ((uint4*)dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+          ((uint4*)dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        }
       } else {
-        ((float4*)dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-        ((float4*)dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ((float4*)dst)[j] = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) store_elem(dst, j, x[j], sizeof(T) == 2);
+      for (int j = 0; j < 16; ++j) store_elem(dst, j, x[j], sizeof(T) == 2);
     }
   }
 }
@@ -261,15 +339,19 @@ void launch_cache_write(const CacheWriteParams& params, cudaStream_t s) {
   const int per = 1 << p.per_shift;
   const dim3 grid((unsigned)((p.N + per - 1) / per));
   const size_t smem = 5 * per * sizeof(int);
-  if (p.bf16) launch_with_pdl(kv_cache_write_kernel<__nv_bfloat16>, grid, dim3(kWriteThreads), smem, s, true, p);
-  else launch_with_pdl(kv_cache_write_kernel<float>, grid, dim3(kWriteThreads), smem, s, true, p);
+  p.per_k_unit = 1.f / p.c.k_unit;
+  p.per_v_unit = 1.f / p.c.v_unit;
+  auto run = [&](auto kern) { launch_with_pdl(kern, grid, dim3(kWriteThreads), smem, s, true, p); };
+  if (p.c.D == 128) p.bf16 ? run(kv_cache_write_kernel<__nv_bfloat16, 128>) : run(kv_cache_write_kernel<float, 128>);
+  else p.bf16 ? run(kv_cache_write_kernel<__nv_bfloat16, 64>) : run(kv_cache_write_kernel<float, 64>);
 }
 
 void launch_cache_read(const CacheReadParams& p, cudaStream_t s) {
-  const int tokens = kReadTokens * 256 / (p.c.D / 8);
+  const int tokens = kReadTokens * 256 / (p.c.D / 16);
   const dim3 grid((unsigned)((p.N + tokens - 1) / tokens), 2 * p.c.heads);
-  if (p.bf16) launch_with_pdl(kv_cache_read_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, true, p);
-  else launch_with_pdl(kv_cache_read_kernel<float>, grid, dim3(256), 0, s, true, p);
+  auto run = [&](auto kern) { launch_with_pdl(kern, grid, dim3(256), 0, s, true, p); };
+  if (p.c.D == 128) p.bf16 ? run(kv_cache_read_kernel<__nv_bfloat16, 128>) : run(kv_cache_read_kernel<float, 128>);
+  else p.bf16 ? run(kv_cache_read_kernel<__nv_bfloat16, 64>) : run(kv_cache_read_kernel<float, 64>);
 }
 
 }  // namespace raiccl

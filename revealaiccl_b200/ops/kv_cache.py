@@ -34,7 +34,8 @@ class KVCache4:
     k_codes, v_codes: uint8 [pages, kv_heads, page_size, head_dim / 2], the even
     dimension in the low four bits.  k_scales, v_scales: float8_e4m3fn [pages,
     kv_heads, page_size, head_dim / 16].  Contiguous, on 16 bytes.  A token's
-    place ("slot") is page * page_size + its row in the page.
+    place ("slot") is page * page_size + its row in the page.  page_size: a power
+    of two from 16 to 65536, at most 2^24 / kv_heads; less than 2^31 places.
     """
 
     k_codes: torch.Tensor
