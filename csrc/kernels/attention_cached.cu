@@ -141,9 +141,9 @@ __device__ __forceinline__ int cached_length(const CachedParams& p, int b) {
 
 __device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) { return (cached_length(p, b) + kCachedTile - 1) / kCachedTile; }
 
-// CTAs that take part (four tiles to one at least), the first tile of one, and the CTA of a tile.
+// CTAs that take part (two tiles to one at least), the first tile of one, and the CTA of a tile.
 __device__ __forceinline__ int cached_ctas(long long tiles, int ctas) {
-  const long long most = (tiles + 3) / 4;
+  const long long most = (tiles + 1) / 2;
   return most < ctas ? (int)most : ctas;
 }
 __device__ __forceinline__ long long cached_first(long long tiles, int ctas, int c) { return tiles * c / ctas; }
@@ -308,25 +308,37 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
       }
       const uint32_t stage_at = ring_at + fill * C::STAGE;
       uint32_t lost = 0;
-      auto part = [&](int row_to, auto rows_of) {  // as many of the tile's tokens as lie in one page
-        constexpr int ROWS = decltype(rows_of)::value;
-        const int at = ahead_at + row_to;
-        const int page = at < ahead_len ? __ldg(ahead_pages + (at >> p.c.page_shift)) : -1;
-        if ((uint32_t)page < (uint32_t)p.c.pages) {
-          copy(stage_at, row_to, page, ahead_row + (at & page_mask), rows_of);
-          return;
-        }
-        lost |= ((1u << ROWS / 16) - 1) << (row_to / 16);
-        if (at < ahead_len && lane == 0) record_status(p.status, kBoundsViolation, kCachedKernelId, page, p.c.pages);
-      };
       if (p.c.page_shift >= 6) {
-        part(0, std::integral_constant<int, 64>{});
-      } else if (p.c.page_shift == 5) {
-#pragma unroll 1
-        for (int r = 0; r < kCachedTile; r += 32) part(r, std::integral_constant<int, 32>{});
-      } else {
-#pragma unroll 1
-        for (int r = 0; r < kCachedTile; r += 16) part(r, std::integral_constant<int, 16>{});
+        const int page = __ldg(ahead_pages + (ahead_at >> p.c.page_shift));
+        if ((uint32_t)page < (uint32_t)p.c.pages) {
+          copy(stage_at, 0, page, ahead_row + (ahead_at & page_mask), std::integral_constant<int, 64>{});
+        } else {
+          lost = 15;
+          if (lane == 0) record_status(p.status, kBoundsViolation, kCachedKernelId, page, p.c.pages);
+        }
+      } else {                                     // several pages: their numbers first, by a lane each
+        const int at = ahead_at + ((lane & 3) << p.c.page_shift);
+        const bool is = lane < (kCachedTile >> p.c.page_shift) && at < ahead_len;
+        int page = is ? __ldg(ahead_pages + (at >> p.c.page_shift)) : -1;
+        if (is && (uint32_t)page >= (uint32_t)p.c.pages) {
+          record_status(p.status, kBoundsViolation, kCachedKernelId, page, p.c.pages);
+          page = -1;
+        }
+        if (p.c.page_shift == 5) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int one = __shfl_sync(0xffffffffu, page, r);
+            if (one >= 0) copy(stage_at, 32 * r, one, ahead_row, std::integral_constant<int, 32>{});
+            else lost |= 3u << (2 * r);
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int one = __shfl_sync(0xffffffffu, page, r);
+            if (one >= 0) copy(stage_at, 16 * r, one, ahead_row, std::integral_constant<int, 16>{});
+            else lost |= 1u << r;
+          }
+        }
       }
       missing = (missing & ~(15u << (4 * fill))) | lost << (4 * fill);
       ++issued;
@@ -694,46 +706,53 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
 
   // ------------------------------------------------------------ the CTA's shared pieces
   __syncthreads();
-  // a piece's parts: its first one (a tail, or the head of the CTA's first warp), then the heads of the warps behind it
+  // A piece's parts: its first one (a tail, or the head of the CTA's first warp), then the heads of the warps behind it.
+  // All pieces' numbers, four to a thread; every thread finds its piece by the bits of the warps that begin one.
   const bool mine = lane < C::WARPS;
   const uint32_t with = __ballot_sync(0xffffffffu, mine && nonempty[mine ? lane : 0]);
-  uint32_t tails = __ballot_sync(0xffffffffu, mine && part[mine ? lane : 0][1].used);
+  const uint32_t tails = __ballot_sync(0xffffffffu, mine && part[mine ? lane : 0][1].used);
   const uint32_t heads_at = __ballot_sync(0xffffffffu, mine && part[mine ? lane : 0][0].used);
-  uint32_t firsts = heads_at & with & -with;
-  while (firsts | tails) {
-    const int side = firsts ? 0 : 1, w = __ffs(firsts ? firsts : tails) - 1;
-    if (firsts) firsts = 0; else tails &= tails - 1;
+  const uint32_t first_head = heads_at & with & -with;
+  const int pieces = __popc(tails) + (first_head != 0);
+  for (int i = tid; i < pieces * p.chunk * (D / 4); i += C::THREADS) {
+    const int h = i / (D / 4) % p.chunk, d = 4 * (i % (D / 4));
+    int nth = i / (p.chunk * (D / 4)), side = 1, w;
+    if (first_head && nth == 0) {
+      side = 0;
+      w = __ffs(first_head) - 1;
+    } else {
+      w = (int)__fns(tails, 0, nth + (first_head ? 0 : 1));
+    }
     const CachedPiece s = part[w][side].s;
     int head0;
-    const int heads = piece_heads(p, s.hc, head0);
+    if (h >= piece_heads(p, s.hc, head0)) continue;
     const bool early = s.first < c0, late = s.first + s.n > c1;
+    float top = stat[w][side][h].x;
     int end = w + 1;
-    while (end < C::WARPS && (!(with >> end & 1) || ((heads_at >> end & 1) && part[end][0].s.first == s.first))) ++end;
-    for (int e = tid; e < heads * (D / 4); e += C::THREADS) {
-      const int h = e / (D / 4), d = 4 * (e - h * (D / 4));
-      float top = stat[w][side][h].x;
-      for (int x = w + 1; x < end; ++x)
-        if (with >> x & 1) top = fmaxf(top, stat[x][0][h].x);
-      float l = 0.f;
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int x = w; x < end; ++x) {
-        if (!(with >> x & 1)) continue;
-        const int y = x == w ? side : 0;
-        const float2 st = stat[x][y][h];
-        const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
-        const float4 a = *(const float4*)((part[x][y].used == 1 ? ringed(x) : spilled(x)) + h * D + d);
-        l = fmaf(st.y, f, l);
-        v.x = fmaf(a.x, f, v.x); v.y = fmaf(a.y, f, v.y); v.z = fmaf(a.z, f, v.z); v.w = fmaf(a.w, f, v.w);
-      }
-      if (!early && !late) {
-        const float r = l == 0.f ? 0.f : p.c.v_unit / l;
-        cached_store4(p, s.b, head0 + h, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
-        if (p.lse != nullptr && d == 0) p.lse[(long long)s.b * p.Hq + head0 + h] = cached_lse(top, l);
-      } else {
-        const long long at = ((long long)blockIdx.x * 2 + (early ? 0 : 1)) * p.chunk + h;
-        *(float4*)(p.parts + at * D + d) = v;
-        if (d == 0) p.stats[at] = make_float2(top, l);
-      }
+    for (; end < C::WARPS; ++end) {
+      if (!(with >> end & 1)) continue;
+      if (!(heads_at >> end & 1) || part[end][0].s.first != s.first) break;
+      top = fmaxf(top, stat[end][0][h].x);
+    }
+    float l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int x = w; x < end; ++x) {
+      if (!(with >> x & 1)) continue;
+      const int y = x == w ? side : 0;
+      const float2 st = stat[x][y][h];
+      const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
+      const float4 a = *(const float4*)((part[x][y].used == 1 ? ringed(x) : spilled(x)) + h * D + d);
+      l = fmaf(st.y, f, l);
+      v.x = fmaf(a.x, f, v.x); v.y = fmaf(a.y, f, v.y); v.z = fmaf(a.z, f, v.z); v.w = fmaf(a.w, f, v.w);
+    }
+    if (!early && !late) {
+      const float r = l == 0.f ? 0.f : p.c.v_unit / l;
+      cached_store4(p, s.b, head0 + h, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
+      if (p.lse != nullptr && d == 0) p.lse[(long long)s.b * p.Hq + head0 + h] = cached_lse(top, l);
+    } else {
+      const long long at = ((long long)blockIdx.x * 2 + (early ? 0 : 1)) * p.chunk + h;
+      *(float4*)(p.parts + at * D + d) = v;
+      if (d == 0) p.stats[at] = make_float2(top, l);
     }
   }
 }

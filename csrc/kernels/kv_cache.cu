@@ -57,24 +57,32 @@ __device__ __forceinline__ long long cache_offset(const CacheView& c, int slot, 
          (((uint32_t)head << c.page_shift) + at) * (uint32_t)(D / 2);
 }
 
-// Sixteen numbers of one row.
+// Sixteen numbers of one row, as they lie.
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, int vec, float (&x)[16]) {
+struct Sixteen {
+  uint4 w[16 * sizeof(T) / 16];
+};
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, int vec, Sixteen<T>& x) {
   if (vec) {
-    constexpr int W = 16 / sizeof(T);
-    uint4 v[16 / W];
 #pragma unroll
-    for (int i = 0; i < 16 / W; ++i) v[i] = __ldg((const uint4*)p + i);
-#pragma unroll
-    for (int i = 0; i < 16 / W; ++i) {
-      float f[W];
-      unpack16<T>(v[i], f);
-#pragma unroll
-      for (int j = 0; j < W; ++j) x[W * i + j] = f[j];
-    }
+    for (int i = 0; i < (int)sizeof(T); ++i) x.w[i] = __ldg((const uint4*)p + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = as_float(p[i]);
+    for (int i = 0; i < 16; ++i) ((T*)x.w)[i] = p[i];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void as_floats(const Sixteen<T>& x, float (&f)[16]) {
+  constexpr int W = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) {
+    float part[W];
+    unpack16<T>(x.w[i], part);
+#pragma unroll
+    for (int j = 0; j < W; ++j) f[W * i + j] = part[j];
   }
 }
 
@@ -140,7 +148,8 @@ __device__ __forceinline__ uint32_t quantise16(float (&x)[16], float unit, float
 //
 // Sixteen numbers to a thread, D / 16 lanes to a row of a head; rows go by value
 // or key, head and token, the token fastest, so that no index needs a division.
-// Two rows to a thread are loaded before the first is worked on.
+// Two rows to a thread are loaded ahead, the first ones before the slots are
+// looked through.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWriteParams p) {
   extern __shared__ int table[];      // [per] slots, [size] keys, [size] last tokens
@@ -154,6 +163,20 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
   __shared__ int range[2];            // the least and the largest slot of the CTA's tokens
   if (threadIdx.x == 0) { range[0] = INT_MAX; range[1] = -1; }
   for (int i = threadIdx.x; i < size; i += kWriteThreads) { key[i] = -1; last[i] = -1; }
+  constexpr int lane_shift = D == 128 ? 3 : 2, step = kWriteThreads >> lane_shift, U = 2;
+  const int l = threadIdx.x & ((1 << lane_shift) - 1), rows = 2 * c.heads << p.per_shift;
+  Sixteen<T> ahead[U];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * step + (int)(threadIdx.x >> lane_shift), t = r & (per - 1), hv = r >> p.per_shift;
+      if (r >= rows || t >= n) continue;
+      const T* src = hv < c.heads ? (const T*)p.k + (first + t) * p.k_token + hv * p.k_head
+                                  : (const T*)p.v + (first + t) * p.v_token + (hv - c.heads) * p.v_head;
+      load16(src + 16 * l, p.vec, ahead[u]);
+    }
+  };
+  load(0);
   __syncthreads();
   auto at = [&](int slot) { return (int)(((uint32_t)slot * 2654435761u) >> 16) & (size - 1); };
   for (int i = threadIdx.x; i < per; i += kWriteThreads) {
@@ -213,35 +236,27 @@ __global__ void __launch_bounds__(kWriteThreads) kv_cache_write_kernel(CacheWrit
     if (last[e] != i) slot_of[i] = -1;
   }
   __syncthreads();
-  constexpr int lane_shift = D == 128 ? 3 : 2, step = kWriteThreads >> lane_shift;
-  const int l = threadIdx.x & ((1 << lane_shift) - 1), rows = 2 * c.heads << p.per_shift;
-  constexpr int U = 2;
   for (int r0 = 0; r0 < rows; r0 += U * step) {
-    float x[U][16];
-    int slot[U], hv[U];
+    Sixteen<T> now[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = ahead[u];
+    load(r0 + U * step);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * step + (int)(threadIdx.x >> lane_shift), t = r & (per - 1);
-      hv[u] = r >> p.per_shift;
-      slot[u] = r < rows ? slot_of[t] : -1;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
-      if (slot[u] >= 0) {
-        const T* src = hv[u] < c.heads ? (const T*)p.k + (first + t) * p.k_token + hv[u] * p.k_head
-                                       : (const T*)p.v + (first + t) * p.v_token + (hv[u] - c.heads) * p.v_head;
-        load16(src + 16 * l, p.vec, x[u]);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool value = hv[u] >= c.heads;
+      const int r = r0 + u * step + (int)(threadIdx.x >> lane_shift), hv = r >> p.per_shift;
+      const int slot = r < rows ? slot_of[r & (per - 1)] : -1;
+      const bool value = hv >= c.heads;
       uint32_t codes[2], word = 0;
-      if (slot[u] >= 0) word = quantise16(x[u], value ? c.v_unit : c.k_unit, value ? p.per_v_unit : p.per_k_unit, codes);
+      if (slot >= 0) {
+        float x[16];
+        as_floats(now[u], x);
+        word = quantise16(x, value ? c.v_unit : c.k_unit, value ? p.per_v_unit : p.per_k_unit, codes);
+      }
       word <<= 8 * (l & 3);             // four lanes' scales to a word; a row's lanes have one slot
       word |= __shfl_xor_sync(0xffffffffu, word, 1);
       word |= __shfl_xor_sync(0xffffffffu, word, 2);
-      if (slot[u] >= 0) {
-        const long long off = cache_offset<D>(c, slot[u], value ? hv[u] - c.heads : hv[u]);
+      if (slot >= 0) {
+        const long long off = cache_offset<D>(c, slot, value ? hv - c.heads : hv);
         *(uint2*)((value ? c.v_codes : c.k_codes) + off + 8 * l) = make_uint2(codes[0], codes[1]);
         if ((l & 3) == 0) *(uint32_t*)((value ? c.v_scales : c.k_scales) + (off >> 3) + l) = word;
       }
@@ -331,10 +346,10 @@ __global__ void __launch_bounds__(256) kv_cache_read_kernel(CacheReadParams p) {
   }
 }
 
-// Tokens of a CTA: about three CTAs to an SM.
+// Tokens of a CTA: up to four CTAs to an SM, which all fit.
 void launch_cache_write(const CacheWriteParams& params, cudaStream_t s) {
   CacheWriteParams p = params;
-  const long long wave = 3ll * serving_sm_count();
+  const long long wave = 4ll * serving_sm_count();
   while ((p.N >> p.per_shift) > wave && (1 << p.per_shift) < kWriteTokens) ++p.per_shift;
   const int per = 1 << p.per_shift;
   const dim3 grid((unsigned)((p.N + per - 1) / per));
