@@ -146,8 +146,18 @@ __device__ __forceinline__ int cached_ctas(long long tiles, int ctas) {
   const long long most = (tiles + 1) / 2;
   return most < ctas ? (int)most : ctas;
 }
-__device__ __forceinline__ long long cached_first(long long tiles, int ctas, int c) { return tiles * c / ctas; }
-__device__ __forceinline__ int cached_cta(long long tiles, int ctas, long long tile) { return (int)(((tile + 1) * ctas - 1) / tiles); }
+// The first tiles % ctas CTAs have one tile more than the others.
+__device__ __forceinline__ long long divide_tiles(long long a, long long b) {
+  return (a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+__device__ __forceinline__ long long cached_first(long long tiles, int ctas, int c) {
+  const long long each = divide_tiles(tiles, ctas), more = tiles - each * ctas;
+  return each * c + (c < more ? c : more);
+}
+__device__ __forceinline__ int cached_cta(long long tiles, int ctas, long long tile) {
+  const long long each = divide_tiles(tiles, ctas), more = tiles - each * ctas, behind = tile - more * (each + 1);
+  return (int)(behind < 0 ? divide_tiles(tile, each + 1) : more + divide_tiles(behind, each));
+}
 
 // A sequence and chunk of heads, as a piece of the order of all tiles.
 struct CachedPiece {
@@ -189,17 +199,101 @@ __device__ __forceinline__ void cached_store4(const CachedParams& p, int b, int 
   }
 }
 
+// A row of D numbers over a warp: lane i has numbers D / 32 * i and on.
+template <int D>
+__device__ __forceinline__ void load_lanes(const float* p, float (&v)[D / 32]) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (D == 128) {
+    const float4 x = *(const float4*)(p + 4 * lane);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+  } else {
+    const float2 x = *(const float2*)(p + 2 * lane);
+    v[0] = x.x; v[1] = x.y;
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void store_lanes(float* p, const float (&v)[D / 32]) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (D == 128) *(float4*)(p + 4 * lane) = make_float4(v[0], v[1], v[2], v[3]);
+  else *(float2*)(p + 2 * lane) = make_float2(v[0], v[1]);
+}
+
+// n parts of a row, each with its own maximum and sum of exponentials, joined by a warp in their order.
+template <int D, typename Stat, typename Row>
+__device__ __forceinline__ void warp_join(int n, Stat stat, Row row, float& top, float& l, float (&v)[D / 32]) {
+  const int lane = threadIdx.x & 31;
+  top = -INFINITY;
+  for (int j = lane; j < n; j += 32) top = fmaxf(top, stat(j).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  l = 0.f;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) v[d] = 0.f;
+  for (int j0 = 0; j0 < n; j0 += 32) {
+    float f = 0.f, y = 0.f;
+    if (j0 + lane < n) {
+      const float2 st = stat(j0 + lane);
+      // no maximum: nothing there, or logits that are all NaN or -inf, whose sum is NaN
+      f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
+      y = st.y;
+    }
+    const int here = n - j0 < 32 ? n - j0 : 32;
+#pragma unroll 4
+    for (int j = 0; j < here; ++j) {
+      float a[D / 32];
+      load_lanes<D>(row(j0 + j), a);
+      const float fj = __shfl_sync(0xffffffffu, f, j);
+      l = fmaf(__shfl_sync(0xffffffffu, y, j), fj, l);
+      if (fj == 0.f) continue;             // (a part that is nothing holds anything)
+#pragma unroll
+      for (int d = 0; d < D / 32; ++d) v[d] = fmaf(a[d], fj, v[d]);
+    }
+  }
+}
+
+// The result's row from sums over a warp.
+template <int N>
+__device__ __forceinline__ void cached_row(const CachedParams& p, int b, int head, float top, float l, const float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  const float r = l == 0.f ? 0.f : p.c.v_unit / l;
+  const long long at = b * p.o_seq + head * p.o_head + N * lane;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    if (p.out_bf16) {
+      const __nv_bfloat162 x = __floats2bfloat162_rn(v[i] * r, v[i + 1] * r);
+      __nv_bfloat16* const o = (__nv_bfloat16*)p.out + at + i;
+      if (p.o_vec) *(__nv_bfloat162*)o = x;
+      else { o[0] = x.x; o[1] = x.y; }
+    } else {
+      float* const o = (float*)p.out + at + i;
+      if (p.o_vec) *(float2*)o = make_float2(v[i] * r, v[i + 1] * r);
+      else { o[0] = v[i] * r; o[1] = v[i + 1] * r; }
+    }
+  }
+  if (p.lse != nullptr && lane == 0) p.lse[(long long)b * p.Hq + head] = cached_lse(top, l);
+}
+
 // A warp's part of a piece that it shares; used: 1 the sums are in its ring, 2 in device memory.
 struct CachedPart {
   CachedPiece s;
   int used;
 };
 
+// A piece that warps of a CTA share: the first of them and the side of its part, the warp behind the last; where the sum goes:
+// the CTA's parts 0 (it began before the CTA's share) and 1 (it ends after it), 2 the output.
+struct CachedChain {
+  int warp, side, end, b, head0, heads, where;
+};
+
 template <int D, int NT, int PARTS>
 __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kernel(CachedParams p) {
   using C = Cached<D, NT, PARTS>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long before[C::THREADS + 1], sum_of[C::WARPS];
+  __shared__ long long before[C::THREADS + 1], sum_of[C::WARPS], base_of[C::WARPS];
+  __shared__ CachedChain chain[C::WARPS + 1];
+  __shared__ int chains;
+  __shared__ uint32_t all_with;
   __shared__ CachedPart part[C::WARPS][2];
   __shared__ float2 stat[C::WARPS][2][C::HEADS];
   __shared__ int nonempty[C::WARPS];
@@ -229,6 +323,7 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
     for (int w = 0; w < warp; ++w) base += sum_of[w];
     before[tid + 1] = (base + sum) * HC;
     if (tid == 0) before[0] = 0;
+    if (lane == 0) base_of[warp] = base * HC;
     __syncthreads();
   }
   const long long tiles = before[C::THREADS];
@@ -236,28 +331,30 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
   const int ctas = cached_ctas(tiles, p.ctas);
   if ((int)blockIdx.x >= ctas) return;
   const long long c0 = cached_first(tiles, ctas, blockIdx.x), c1 = cached_first(tiles, ctas, blockIdx.x + 1);
+  const int share = (int)(c1 - c0);
   // A warp's part of a sequence: the one that began before its share (0), the one that ends after it (1).  The last that it
   // works on goes into its ring, which is done then; a first one with others behind it to device memory.
   auto spilled = [&](int w) { return p.spill + ((long long)blockIdx.x * C::WARPS + w) * (C::HEADS * D); };
   auto ringed = [&](int w) { return (float*)(smem + w * C::STAGES * C::STAGE); };
   auto piece_at = [&](long long u) {
-    int lo = 0, hi = C::THREADS;     // before[lo] <= u < before[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (before[mid] <= u) lo = mid; else hi = mid;
-    }
+    // the last thread whose sequences begin at or before u: its warp, then itself
+    const uint32_t w = __ballot_sync(0xffffffffu, lane < C::WARPS && base_of[lane < C::WARPS ? lane : 0] <= u);
+    const int in = 31 - __clz(w);
+    const uint32_t m = __ballot_sync(0xffffffffu, before[32 * in + lane] <= u);
+    const int lo = 32 * in + 31 - __clz(m);
     long long first = before[lo];
     int b = lo * per, n = cached_tiles(p, b);
     while (first + (long long)n * HC <= u) {
       first += (long long)n * HC;
       n = cached_tiles(p, ++b);
     }
-    const int hc = (int)((u - first) / n);
+    const int hc = (int)((uint32_t)(u - first) / (uint32_t)n);
     return CachedPiece{b, hc, n, first + (long long)hc * n};
   };
 
-  const long long u0 = c0 + (c1 - c0) * warp / C::WARPS, u1 = c0 + (c1 - c0) * (warp + 1) / C::WARPS;
-  const int count = (int)(u1 - u0);
+  const long long u0 = c0 + share / C::WARPS * warp + min(warp, share % C::WARPS);
+  const int count = share / C::WARPS + (warp < share % C::WARPS);
+  const long long u1 = u0 + count;
   uint8_t* const ring = smem + warp * C::STAGES * C::STAGE;
   if (lane == 0) {
     part[warp][0].used = part[warp][1].used = 0;
@@ -345,10 +442,6 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
       ahead_at += kCachedTile;
       fill = fill + 1 == C::STAGES ? 0 : fill + 1;
     };
-    for (int i = 0; i < C::STAGES; ++i) {
-      if (issued < count) issue();
-      cp_async_commit();
-    }
 
     // ---------------------------------------------------------- tiles
     constexpr int KS = D / 16;         // products of a row of sixteen tokens over D
@@ -470,17 +563,17 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         }
     };
 
-    begin();
-    int done = 0, stage = 0, end = (int)min((long long)count, piece.first + piece.n - u0);
-    int left = cached_length(p, piece.b) - (int)(u0 - piece.first) * kCachedTile;   // tokens of the piece from this tile on
+    // One loop, in which copies, beginnings and ends have one place each: with two places the code was a fifth longer (64 x
+    // 16384 tokens 229 us, so 221).
+    int stage = 0, end = 0, left = 0;   // tiles up to the piece's end; tokens of the piece from this tile on
 #pragma unroll 1
-    for (; done < count; ++done) {
+    for (int done = -C::STAGES; done < count; ++done) {
+     if (done >= 0) {
       if (done == end) {
-        finish(false);
-        next_piece(p, piece);
+        if (done > 0) next_piece(p, piece);
         begin();
-        end = (int)min((long long)count, (long long)end + piece.n);
-        left = cached_length(p, piece.b);
+        end = (int)min((long long)count, piece.first + piece.n - u0);
+        left = cached_length(p, piece.b) - (done == 0 ? (int)(u0 - piece.first) * kCachedTile : 0);
       }
       cp_async_wait<C::STAGES - 1>();
       __syncwarp();
@@ -698,61 +791,59 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
       left -= kCachedTile;
       if (++stage == C::STAGES) stage = 0;
       __syncwarp();   // every lane has read the tile
-      if (issued < count) issue();
-      cp_async_commit();
+      if (done + 1 == end) finish(done + 1 == count);
+     }
+     if (issued < count) issue();
+     cp_async_commit();
     }
-    finish(true);
   }
 
   // ------------------------------------------------------------ the CTA's shared pieces
   __syncthreads();
-  // A piece's parts: its first one (a tail, or the head of the CTA's first warp), then the heads of the warps behind it.
-  // All pieces' numbers, four to a thread; every thread finds its piece by the bits of the warps that begin one.
-  const bool mine = lane < C::WARPS;
-  const uint32_t with = __ballot_sync(0xffffffffu, mine && nonempty[mine ? lane : 0]);
-  const uint32_t tails = __ballot_sync(0xffffffffu, mine && part[mine ? lane : 0][1].used);
-  const uint32_t heads_at = __ballot_sync(0xffffffffu, mine && part[mine ? lane : 0][0].used);
-  const uint32_t first_head = heads_at & with & -with;
-  const int pieces = __popc(tails) + (first_head != 0);
-  for (int i = tid; i < pieces * p.chunk * (D / 4); i += C::THREADS) {
-    const int h = i / (D / 4) % p.chunk, d = 4 * (i % (D / 4));
-    int nth = i / (p.chunk * (D / 4)), side = 1, w;
-    if (first_head && nth == 0) {
-      side = 0;
-      w = __ffs(first_head) - 1;
+  // A piece's parts: its first one (a tail, or the head of the CTA's first warp), then the heads of the warps behind it, up
+  // to the one that it ends in.  The warps between have shares, if the CTA has tiles for all of them.
+  if (warp == 0) {
+    const bool mine = lane < C::WARPS && nonempty[lane < C::WARPS ? lane : 0];
+    const uint32_t with = __ballot_sync(0xffffffffu, mine);
+    const bool tail = mine && part[lane][1].used, head = mine && part[lane][0].used && lane == __ffs(with) - 1;
+    const uint32_t tails = __ballot_sync(0xffffffffu, tail), heads = __ballot_sync(0xffffffffu, head);
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      if (!(side ? tail : head)) continue;
+      const CachedPiece s = part[lane][side].s;
+      int end = lane + 1, parts = 1;
+      for (; end < C::WARPS; ++end) {
+        if (!(with >> end & 1)) continue;
+        if (!part[end][0].used || part[end][0].s.first != s.first) break;
+        ++parts;
+      }
+      int head0;
+      const int nheads = piece_heads(p, s.hc, head0);
+      const bool early = s.first < c0, late = s.first + s.n > c1;
+      chain[(heads != 0) * side + (side ? __popc(tails & ((1u << lane) - 1)) : 0)] = {lane, side, end, s.b, head0, nheads, early ? 0 : late ? 1 : 2};
+    }
+    if (lane == 0) { chains = __popc(tails) + (heads != 0); all_with = with; }
+  }
+  __syncthreads();
+  for (int i = warp; i < chains * C::HEADS; i += C::WARPS) {   // a warp to a head of a piece
+    const CachedChain x = chain[i / C::HEADS];
+    const int h = i % C::HEADS;
+    if (h >= x.heads) continue;
+    auto side_of = [&](int w) { return w == x.warp ? x.side : 0; };
+    float top, l, v[D / 32];
+    warp_join<D>(
+        x.end - x.warp, [&](int j) { return all_with >> (x.warp + j) & 1 ? stat[x.warp + j][side_of(x.warp + j)][h] : make_float2(-INFINITY, 0.f); },
+        [&](int j) {
+          const int w = x.warp + j;
+          return (!(all_with >> w & 1) || part[w][side_of(w)].used == 1 ? ringed(w) : spilled(w)) + h * D;
+        },
+        top, l, v);
+    if (x.where == 2) {
+      cached_row(p, x.b, x.head0 + h, top, l, v);
     } else {
-      w = (int)__fns(tails, 0, nth + (first_head ? 0 : 1));
-    }
-    const CachedPiece s = part[w][side].s;
-    int head0;
-    if (h >= piece_heads(p, s.hc, head0)) continue;
-    const bool early = s.first < c0, late = s.first + s.n > c1;
-    float top = stat[w][side][h].x;
-    int end = w + 1;
-    for (; end < C::WARPS; ++end) {
-      if (!(with >> end & 1)) continue;
-      if (!(heads_at >> end & 1) || part[end][0].s.first != s.first) break;
-      top = fmaxf(top, stat[end][0][h].x);
-    }
-    float l = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int x = w; x < end; ++x) {
-      if (!(with >> x & 1)) continue;
-      const int y = x == w ? side : 0;
-      const float2 st = stat[x][y][h];
-      const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
-      const float4 a = *(const float4*)((part[x][y].used == 1 ? ringed(x) : spilled(x)) + h * D + d);
-      l = fmaf(st.y, f, l);
-      v.x = fmaf(a.x, f, v.x); v.y = fmaf(a.y, f, v.y); v.z = fmaf(a.z, f, v.z); v.w = fmaf(a.w, f, v.w);
-    }
-    if (!early && !late) {
-      const float r = l == 0.f ? 0.f : p.c.v_unit / l;
-      cached_store4(p, s.b, head0 + h, d, make_float4(v.x * r, v.y * r, v.z * r, v.w * r));
-      if (p.lse != nullptr && d == 0) p.lse[(long long)s.b * p.Hq + head0 + h] = cached_lse(top, l);
-    } else {
-      const long long at = ((long long)blockIdx.x * 2 + (early ? 0 : 1)) * p.chunk + h;
-      *(float4*)(p.parts + at * D + d) = v;
-      if (d == 0) p.stats[at] = make_float2(top, l);
+      const long long at = ((long long)blockIdx.x * 2 + x.where) * p.chunk + h;
+      store_lanes<D>(p.parts + at * D, v);
+      if (lane == 0) p.stats[at] = make_float2(top, l);
     }
   }
 }
