@@ -7,9 +7,7 @@
 //
 //   S = Q K^T,  P = exp2(c S - m),  O = O + P V,  l = l + sum P
 //
-// with O multiplied by exp2 of the change where m has to follow a maximum that
-// grew by more than 8 (powers of two); until then P stays below 2^8, which costs
-// no accuracy.
+// with O multiplied by exp2 of the change where m has to follow the maximum.
 //
 // One warp loads (TMA), one issues the products (tcgen05.mma, 128 x 128 sums in
 // TMEM), and a warpgroup to each tile does the softmax, one row to a thread: no
@@ -102,6 +100,29 @@ __device__ __forceinline__ float prompt_exp2(float x) {
   return y;
 }
 
+// Two fp32 numbers to an instruction.
+__device__ __forceinline__ uint64_t pair_f32(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair_f32(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -119,7 +140,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   uint8_t* const sk = smem + 2 * C::TILE;
   uint8_t* const sv = sk + C::STAGES * C::TILE;
   __shared__ uint64_t q_full[2], k_full[C::STAGES], k_empty[C::STAGES], v_full[C::STAGES], v_empty[C::STAGES], v_raw[C::STAGES],
-      v_ready[C::STAGES], s_full[2], p_full[2], o_full[2], drained;
+      v_ready[C::STAGES], s_full[2], p_half[2], p_full[2], o_full[2], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int odd[3][D], any_odd;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -140,7 +161,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   auto fixed_phase = [&](int i) { return (uint32_t)((i - first_fixed) / C::STAGES) & 1u; };   // of v_raw and v_ready
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); mbar_init(&v_raw[i], 1); mbar_init(&v_ready[i], 2);
@@ -227,12 +248,15 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
             if (x == 0) {
               if (!(ok = i < first_fixed ? wait(&v_full[stage], phase) : wait(&v_ready[stage], fixed_phase(i)))) break;
             }
-            if (!(ok = wait(&p_full[x], i & 1))) break;
-            tc_fence_after_sync();
             const uint64_t b = desc_at(vrow, smem_u32(sv + stage * C::TILE));
+            for (int h = 0; ok && h < 2; ++h) {              // the first half of P's columns, then the other
+              if (!(ok = wait(h ? &p_full[x] : &p_half[x], i & 1))) break;
+              tc_fence_after_sync();
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * k, b + k * (16 * 128 / 16), ipv, i > 0 || k > 0);
+              for (int k = 0; k < 4; ++k)
+                umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 32 * h + 8 * k, b + (4 * h + k) * (16 * 128 / 16), ipv, i > 0 || h > 0 || k > 0);
+            }
+            if (!ok) break;
             if (x + 1 == tiles) umma_commit(&v_empty[stage]);
             if (i + 1 == steps) {
               umma_commit(&o_full[x]);
@@ -316,48 +340,68 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         for (int c = 0; c < 128; ++c)
           if (k0 + c >= visible) r[c] = __float_as_uint(-INFINITY);
       }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < 128; ++c) top[c & 3] = fmaxf(top[c & 3], __uint_as_float(r[c]));
-      const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
-      const bool grow = peak > m + 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float now = grow ? peak : m;
-        const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
-        m = now;
-        l *= shrink;
-        if (i > 0) {
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(to + c, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-            tmem_st32(to + c, o);
-          }
-        }
-      }
-      const float base = m == -INFINITY ? 0.f : -m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
+      // Weights are exp2(c S - m) for any m that lets them neither overflow nor vanish: bf16 and fp32 hold 2^64 as exactly as
+      // 1.  So m follows the maximum only when that is 2^64 past it (and in the first tile), and the first half of the weights
+      // is worked out before it is known whether it is.  The product begins with that half.  (A quarter of the exponentials
+      // by a polynomial, to spare the special-function unit: no difference, 16384 tokens run into the power limit.)
+      uint64_t sum[2];
+      uint32_t w[32];
+      auto half = [&](int h, float base) {
+        const uint64_t mult2 = pair_f32(mult, mult), base2 = pair_f32(base, base);
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          const float a = prompt_exp2(fmaf(__uint_as_float(r[64 * h + 2 * c]), mult, base));
-          const float b = prompt_exp2(fmaf(__uint_as_float(r[64 * h + 2 * c + 1]), mult, base));
-          sum[(2 * c) & 3] += a;
-          sum[(2 * c + 1) & 3] += b;
+          float a, b;
+          unpair_f32(fma2(pair_f32(__uint_as_float(r[64 * h + 2 * c]), __uint_as_float(r[64 * h + 2 * c + 1])), mult2, base2), a, b);
+          a = prompt_exp2(a);
+          b = prompt_exp2(b);
+          sum[c & 1] = add2(sum[c & 1], pair_f32(a, b));
           w[c] = pack_bf16(a, b);
         }
+      };
+      auto store = [&](int h) {
         tmem_st32(ts + 32 * h, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(h ? &p_full[x] : &p_half[x]);
+      };
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      bool again;
+#pragma unroll 1
+      do {
+        sum[0] = sum[1] = 0;
+        half(0, m == -INFINITY ? 0.f : -m);
+#pragma unroll
+        for (int c = 0; c < 128; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
+        const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
+        const bool grow = peak > m + 64.f;
+        again = __any_sync(0xffffffffu, grow);
+        if (again) {
+          const float now = grow ? peak : m;
+          const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
+          m = now;
+          l *= shrink;
+          if (i > 0) {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+              tmem_st32(to + c, o);
+            }
+          }
+        }
+      } while (again);
+      store(0);
+      half(1, m == -INFINITY ? 0.f : -m);
+      store(1);
+      float s0, s1;
+      unpair_f32(add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
     }
     if (x < tiles) {
       if (ok && steps > 0) {

@@ -27,33 +27,38 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
 template <int D>
 struct PromptRows {
   static constexpr int KS = D + 8, VS = D + 4;   // strides of a key's and a value's row, without conflicts of the fragments' loads
-  static constexpr int SMEM = 4 * kRowsKeys * 2 * (KS + VS);
+  static constexpr int TILE = kRowsKeys * (KS + VS);        // numbers: keys, then values
+  static constexpr int SMEM = 4 * 3 * TILE;                 // two tiles as they lie, the rests of one
+  static constexpr int CTAS = D == 64 ? 2 : 1;              // to an SM, by registers
 };
 
-__device__ __forceinline__ void load4(const void* base, long long at, bool vec, float (&x)[4]) {
-  const float* p = (const float*)base + at;
+__device__ __forceinline__ void rows_copy(uint32_t to, const float* from, bool there, bool vec) {
+  const int n = there ? 16 : 0;      // what is not read is zeros
   if (vec) {
-    const float4 v = *(const float4*)p;
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = p[i];
+    for (int i = 0; i < 4; ++i)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4 * i), "l"(there ? from + i : from), "r"(n / 4) : "memory");
   }
 }
 
-// One CTA: 128 rows (a token and a query head of the group), eight warps of
-// sixteen; 32 keys at a time, split into two tf32 parts as they are stored.
+// fp32: every number is two tf32 parts, its upper 19 bits, which is what the
+// tensor core reads of it, and the rest; three products.  One CTA: 128 rows (a
+// token and a query head of the group), eight warps of sixteen; 32 keys at a time
+// by cp.async, a tile ahead; the rests are worked out in shared memory, once for
+// all warps.
+//
+// The tensor core cuts what does not fit its sums, so the products with a rest
+// have sums of their own, and those of the values leave it every 32 keys.
 template <int D>
-__global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool vec) {
+__global__ void __launch_bounds__(256, PromptRows<D>::CTAS) prompt_rows_kernel(PromptParams p, bool vec) {
   using C = PromptRows<D>;
   extern __shared__ __align__(16) float sm[];
-  float* const kh = sm;
-  float* const kl = kh + kRowsKeys * C::KS;
-  float* const vh = kl + kRowsKeys * C::KS;
-  float* const vl = vh + kRowsKeys * C::VS;
+  float* const rest = sm + 2 * C::TILE;
   __shared__ int odd[3][D], any_odd;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  for (int i = threadIdx.x; i < 3 * D; i += 256) odd[0][i] = INT_MAX;
+  for (int i = threadIdx.x; i < 3 * D; i += 256) ((int*)odd)[i] = INT_MAX;
   if (threadIdx.x == 0) any_odd = 0;
   griddep_wait();
   griddep_launch_dependents();
@@ -75,6 +80,19 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
   }
   const int keys = prompt_visible(p, s, min(tile * tokens + tokens, s.nq) - 1);
 
+  auto copy = [&](int k0, int stage) {
+    const uint32_t to = smem_u32(sm + stage * C::TILE);
+    for (int i = threadIdx.x; i < kRowsKeys * D / 4; i += 256) {
+      const int row = i / (D / 4), d = 4 * (i - row * (D / 4));
+      const bool there = k0 + row < s.nk;
+      const long long at = s.k0 + (there ? k0 + row : 0);
+      rows_copy(to + 4 * (row * C::KS + d), (const float*)p.k + at * p.k_token + head * p.k_head + d, there, vec);
+      rows_copy(to + 4 * (kRowsKeys * C::KS + row * C::VS + d), (const float*)p.v + at * p.v_token + head * p.v_head + d, there, vec);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (keys > 0) copy(0, 0);
+
   float q[2][D / 4];   // dimensions 8 j + 2 t and + 1
 #pragma unroll
   for (int r = 0; r < 2; ++r)
@@ -91,51 +109,63 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
     for (int j = 0; j < 4; ++j) o[n][j] = 0.f;
   const float mult = p.scale * 1.44269504088896341f;
 
-  for (int k0 = 0; k0 < keys; k0 += kRowsKeys) {
+  for (int k0 = 0, stage = 0; k0 < keys; k0 += kRowsKeys, stage ^= 1) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncthreads();
+    if (k0 + kRowsKeys < keys) copy(k0 + kRowsKeys, stage ^ 1);
+    float *const kh = sm + stage * C::TILE, *const vh = kh + kRowsKeys * C::KS;
+    float *const kl = rest, *const vl = rest + kRowsKeys * C::KS;
     for (int i = threadIdx.x; i < kRowsKeys * D / 4; i += 256) {
       const int row = i / (D / 4), d = 4 * (i - row * (D / 4));
-      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      if (k0 + row < s.nk) {
-        const long long token = s.k0 + k0 + row;
-        load4(p.k, token * p.k_token + head * p.k_head + d, vec, x);
-        load4(p.v, token * p.v_token + head * p.v_head + d, vec, y);
-      }
+      const float4 x = *(const float4*)(kh + row * C::KS + d);
+      *(float4*)(kl + row * C::KS + d) = make_float4(rest_tf32(x.x), rest_tf32(x.y), rest_tf32(x.z), rest_tf32(x.w));
+      const float4 v = *(const float4*)(vh + row * C::VS + d);
+      float y[4] = {v.x, v.y, v.z, v.w};
+      bool finite = true;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (!(fabsf(y[j]) < INFINITY)) {
-          atomicMin(&odd[odd_kind(y[j])][d + j], k0 + row);
-          any_odd = 1;
-          y[j] = 0.f;
-        }
-        split_tf32(x[j], kh[row * C::KS + d + j], kl[row * C::KS + d + j]);
-        split_tf32(y[j], vh[row * C::VS + d + j], vl[row * C::VS + d + j]);
+      for (int j = 0; j < 4; ++j) finite &= fabsf(y[j]) < INFINITY;
+      if (!finite) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!(fabsf(y[j]) < INFINITY)) {
+            atomicMin(&odd[odd_kind(y[j])][d + j], k0 + row);
+            any_odd = 1;
+            y[j] = 0.f;
+            vh[row * C::VS + d + j] = 0.f;
+          }
       }
+      *(float4*)(vl + row * C::VS + d) = make_float4(rest_tf32(y[0]), rest_tf32(y[1]), rest_tf32(y[2]), rest_tf32(y[3]));
     }
     __syncthreads();
     float z[kRowsKeys / 8][4];
+    {
+      float zl[kRowsKeys / 8][4];
 #pragma unroll
-    for (int n = 0; n < kRowsKeys / 8; ++n)
+      for (int n = 0; n < kRowsKeys / 8; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z[n][j] = 0.f;
+        for (int j = 0; j < 4; ++j) z[n][j] = zl[n][j] = 0.f;
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) {
-      uint32_t ah[4], al[4];
+      for (int j = 0; j < D / 8; ++j) {
+        uint32_t ah[4], al[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float h, low;
-        split_tf32(q[i & 1][2 * j + (i >> 1)], h, low);
-        ah[i] = __float_as_uint(h);
-        al[i] = __float_as_uint(low);
+        for (int i = 0; i < 4; ++i) {
+          const float v = q[i & 1][2 * j + (i >> 1)];
+          ah[i] = __float_as_uint(v);
+          al[i] = __float_as_uint(rest_tf32(v));
+        }
+#pragma unroll
+        for (int n = 0; n < kRowsKeys / 8; ++n) {
+          const float2 h = *(const float2*)(kh + (8 * n + g) * C::KS + 8 * j + 2 * t);
+          const float2 low = *(const float2*)(kl + (8 * n + g) * C::KS + 8 * j + 2 * t);
+          mma_tf32(zl[n], ah, __float_as_uint(low.x), __float_as_uint(low.y));
+          mma_tf32(zl[n], al, __float_as_uint(h.x), __float_as_uint(h.y));
+          mma_tf32(z[n], ah, __float_as_uint(h.x), __float_as_uint(h.y));
+        }
       }
 #pragma unroll
-      for (int n = 0; n < kRowsKeys / 8; ++n) {
-        const float2 h = *(const float2*)(kh + (8 * n + g) * C::KS + 8 * j + 2 * t);
-        const float2 low = *(const float2*)(kl + (8 * n + g) * C::KS + 8 * j + 2 * t);
-        mma_tf32(z[n], ah, __float_as_uint(low.x), __float_as_uint(low.y));
-        mma_tf32(z[n], al, __float_as_uint(h.x), __float_as_uint(h.y));
-        mma_tf32(z[n], ah, __float_as_uint(h.x), __float_as_uint(h.y));
-      }
+      for (int n = 0; n < kRowsKeys / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[n][j] += zl[n][j];
     }
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -155,6 +185,7 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
       m[r] = now[r];
       l[r] *= shrink[r];
     }
+    uint32_t ph[kRowsKeys / 8][4], pl[kRowsKeys / 8][4];
 #pragma unroll
     for (int n = 0; n < kRowsKeys / 8; ++n)
 #pragma unroll
@@ -162,31 +193,25 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
         // a masked key adds nothing, whatever m is; a row of -inf alone is NaN, as its formula is.  One fma: off by a
         // rounding of the difference, not of the logit.
         const int key = k0 + 8 * n + 2 * t + (j & 1);
-        z[n][j] = key < visible[j >> 1] ? exp2f(fmaf(z[n][j], mult, -m[j >> 1])) : 0.f;
-        l[j >> 1] += z[n][j];
-      }
-    uint32_t ph[kRowsKeys / 8][4], pl[kRowsKeys / 8][4];
-#pragma unroll
-    for (int n = 0; n < kRowsKeys / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float h, low;
-        split_tf32(z[n][(i & 1) * 2 + (i >> 1)], h, low);
-        ph[n][i] = __float_as_uint(h);
-        pl[n][i] = __float_as_uint(low);
+        const float e = key < visible[j >> 1] ? exp2f(fmaf(z[n][j], mult, -m[j >> 1])) : 0.f;
+        l[j >> 1] += e;
+        const int at = (j & 1) * 2 + (j >> 1);         // the other operand's order
+        ph[n][at] = __float_as_uint(e);
+        pl[n][at] = __float_as_uint(rest_tf32(e));
       }
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
-      float fresh[4] = {0.f, 0.f, 0.f, 0.f};
+      float fresh[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int k = 0; k < kRowsKeys / 8; ++k) {
         const int at = (8 * k + 2 * t) * C::VS + 8 * n + g;
-        mma_tf32(fresh, ph[k], __float_as_uint(vl[at]), __float_as_uint(vl[at + C::VS]));
-        mma_tf32(fresh, pl[k], __float_as_uint(vh[at]), __float_as_uint(vh[at + C::VS]));
-        mma_tf32(fresh, ph[k], __float_as_uint(vh[at]), __float_as_uint(vh[at + C::VS]));
+        const uint32_t h0 = __float_as_uint(vh[at]), h1 = __float_as_uint(vh[at + C::VS]);
+        mma_tf32(low, ph[k], __float_as_uint(vl[at]), __float_as_uint(vl[at + C::VS]));
+        mma_tf32(low, pl[k], h0, h1);
+        mma_tf32(fresh, ph[k], h0, h1);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[n][j] = fmaf(o[n][j], shrink[j >> 1], fresh[j]);
+      for (int j = 0; j < 4; ++j) o[n][j] = fmaf(o[n][j], shrink[j >> 1], fresh[j] + low[j]);
     }
   }
   __syncthreads();
@@ -198,14 +223,17 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(PromptParams p, bool v
     const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
     const long long at = (long long)(s.q0 + token[r]) * p.o_token + (long long)hq[r] * p.o_head;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
+    for (int n = 0; n < D / 8; ++n) {
+      float v[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int d = 8 * n + 2 * t + e;
-        float v = o[n][2 * r + e] * inv;
-        if (any_odd) v = put_back_odd<D>(odd, d, visible[r], v);
-        ((float*)p.out)[at + d] = v;
+        v[e] = o[n][2 * r + e] * inv;
+        if (any_odd) v[e] = put_back_odd<D>(odd, 8 * n + 2 * t + e, visible[r], v[e]);
       }
+      float* const out = (float*)p.out + at + 8 * n + 2 * t;
+      if (p.o_vec) *(float2*)out = make_float2(v[0], v[1]);
+      else { out[0] = v[0]; out[1] = v[1]; }
+    }
     if (p.lse != nullptr && t == 0)
       p.lse[(long long)(s.q0 + token[r]) * p.Hq + hq[r]] = (m[r] + log2f(l[r])) * 0.69314718055994531f;
   }
