@@ -153,14 +153,19 @@ __global__ void __launch_bounds__(256, PromptRows<D>::CTAS) prompt_rows_kernel(P
           ah[i] = __float_as_uint(v);
           al[i] = __float_as_uint(rest_tf32(v));
         }
+        // four products in a row that do not wait for one another
+        float2 h[kRowsKeys / 8], low[kRowsKeys / 8];
 #pragma unroll
         for (int n = 0; n < kRowsKeys / 8; ++n) {
-          const float2 h = *(const float2*)(kh + (8 * n + g) * C::KS + 8 * j + 2 * t);
-          const float2 low = *(const float2*)(kl + (8 * n + g) * C::KS + 8 * j + 2 * t);
-          mma_tf32(zl[n], ah, __float_as_uint(low.x), __float_as_uint(low.y));
-          mma_tf32(zl[n], al, __float_as_uint(h.x), __float_as_uint(h.y));
-          mma_tf32(z[n], ah, __float_as_uint(h.x), __float_as_uint(h.y));
+          h[n] = *(const float2*)(kh + (8 * n + g) * C::KS + 8 * j + 2 * t);
+          low[n] = *(const float2*)(kl + (8 * n + g) * C::KS + 8 * j + 2 * t);
         }
+#pragma unroll
+        for (int n = 0; n < kRowsKeys / 8; ++n) mma_tf32(z[n], ah, __float_as_uint(h[n].x), __float_as_uint(h[n].y));
+#pragma unroll
+        for (int n = 0; n < kRowsKeys / 8; ++n) mma_tf32(zl[n], al, __float_as_uint(h[n].x), __float_as_uint(h[n].y));
+#pragma unroll
+        for (int n = 0; n < kRowsKeys / 8; ++n) mma_tf32(zl[n], ah, __float_as_uint(low[n].x), __float_as_uint(low[n].y));
       }
 #pragma unroll
       for (int n = 0; n < kRowsKeys / 8; ++n)
@@ -200,18 +205,30 @@ __global__ void __launch_bounds__(256, PromptRows<D>::CTAS) prompt_rows_kernel(P
         pl[n][at] = __float_as_uint(rest_tf32(e));
       }
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      float fresh[4] = {0.f, 0.f, 0.f, 0.f}, low[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < D / 8; n += 2) {
+      float fresh[2][4] = {}, low[2][4] = {};
 #pragma unroll
       for (int k = 0; k < kRowsKeys / 8; ++k) {
-        const int at = (8 * k + 2 * t) * C::VS + 8 * n + g;
-        const uint32_t h0 = __float_as_uint(vh[at]), h1 = __float_as_uint(vh[at + C::VS]);
-        mma_tf32(low, ph[k], __float_as_uint(vl[at]), __float_as_uint(vl[at + C::VS]));
-        mma_tf32(low, pl[k], h0, h1);
-        mma_tf32(fresh, ph[k], h0, h1);
+        uint32_t h[2][2], v[2][2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int at = (8 * k + 2 * t) * C::VS + 8 * (n + e) + g;
+          h[e][0] = __float_as_uint(vh[at]);
+          h[e][1] = __float_as_uint(vh[at + C::VS]);
+          v[e][0] = __float_as_uint(vl[at]);
+          v[e][1] = __float_as_uint(vl[at + C::VS]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) mma_tf32(fresh[e], ph[k], h[e][0], h[e][1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) mma_tf32(low[e], pl[k], h[e][0], h[e][1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) mma_tf32(low[e], ph[k], v[e][0], v[e][1]);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[n][j] = fmaf(o[n][j], shrink[j >> 1], fresh[j] + low[j]);
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[n + e][j] = fmaf(o[n + e][j], shrink[j >> 1], fresh[e][j] + low[e][j]);
     }
   }
   __syncthreads();
