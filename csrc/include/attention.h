@@ -108,13 +108,18 @@ struct PromptParams {
   int B, Hq, Hk, group, D;
   int bf16, causal, o_vec;
   float scale;
+  // by the plan: CTAs that share a tile's keys, [splits][Nq][Hq][D] their sums, [splits][Nq][Hq] maxima and sums of exponentials
+  int splits;
+  float* parts;
+  float2* stats;
   DeviceStatus* status;
 };
 
 struct PromptPlan {
   int pack_q, pack_k, pack_v;        // rows that are copied to aligned ones first
-  long long q_bytes, k_bytes, v_bytes;
-  long long bytes() const { return q_bytes + k_bytes + v_bytes; }
+  int splits;                        // CTAs that share a tile's keys
+  long long q_bytes, k_bytes, v_bytes, parts_bytes, stats_bytes;
+  long long bytes() const { return q_bytes + k_bytes + v_bytes + parts_bytes + stats_bytes; }
 };
 
 PromptPlan plan_prompt(const PromptParams& p, int sms);

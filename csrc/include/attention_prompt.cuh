@@ -57,6 +57,15 @@ __device__ __forceinline__ bool prompt_tile(const PromptParams& p, int index, in
   return false;
 }
 
+// This CTA's share of a tile's `steps` steps of `width` keys, where several CTAs share them: the sequence is cut to it, so
+// that everything behind goes by the share alone.
+__device__ __forceinline__ int prompt_share(const PromptParams& p, int split, int steps, int width, PromptSeq& s) {
+  const int each = (steps + p.splits - 1) / p.splits, first = min(steps, split * each);
+  s.k0 += first * width;
+  s.nk -= first * width;
+  return min(each, steps - first);
+}
+
 // Keys that row `token` of q sees.
 __device__ __forceinline__ int prompt_visible(const PromptParams& p, const PromptSeq& s, int token) {
   if (!p.causal) return s.nk;

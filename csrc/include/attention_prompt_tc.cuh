@@ -155,7 +155,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   const int token0 = pair * 2 * tokens;                       // of the sequence, A's first
   const int tiles = token0 + tokens < s.nq ? 2 : 1;
   const int keys = prompt_visible(p, s, min(token0 + 2 * tokens, s.nq) - 1);
-  const int steps = (keys + kPromptKeys - 1) / kPromptKeys;
+  const int steps = prompt_share(p, blockIdx.y, (keys + kPromptKeys - 1) / kPromptKeys, kPromptKeys, s);
   // Values of tiles from here on, which some row does not see whole, arrive on v_raw and go through two warps first.
   const int first_fixed = min(prompt_visible(p, s, token0), s.nk) / kPromptKeys;
   auto fixed_phase = [&](int i) { return (uint32_t)((i - first_fixed) / C::STAGES) & 1u; };   // of v_raw and v_ready
@@ -409,7 +409,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         tc_fence_after_sync();
       }
       // a row that sees keys has a sum, unless all its logits are -inf
-      const float inv = l == 0.f ? (visible > 0 ? NAN : 0.f) : 1.f / l;
+      if (l == 0.f && visible > 0 && steps > 0) l = NAN;
+      const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       const bool put_back = any_odd != 0;
       const long long at = (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head;
 #pragma unroll 1
@@ -426,7 +427,11 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = put_back_odd<D>(odd, c + e, visible, v[e]);
         }
-        if (mine) {
+        if (mine && p.splits > 1) {
+          float4* const dst = (float4*)(p.parts + (((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq) * D + c);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) dst[e / 4] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        } else if (mine) {
           __nv_bfloat16* const dst = (__nv_bfloat16*)p.out + at + c;
           if (p.o_vec) {
 #pragma unroll
@@ -440,7 +445,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         }
         __syncwarp();
       }
-      if (mine && p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+      if (mine && p.splits > 1) p.stats[((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq] = make_float2(m, l);
+      else if (mine && p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
     }
   }
   __syncwarp();

@@ -280,6 +280,41 @@ std::tuple<torch::Tensor, OptTensor> attention_cached(torch::Tensor q, torch::Te
   return {res, lse};
 }
 
+// What the plan of a call goes by: shapes, types, addresses and strides.
+void prompt_tensors(PromptParams& p, const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v) {
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.q_token = q.stride(0);
+  p.q_head = q.stride(1);
+  p.k_token = k.stride(0);
+  p.k_head = k.stride(1);
+  p.v_token = v.stride(0);
+  p.v_head = v.stride(1);
+  p.Nq = q.size(0);
+  p.Nk = k.size(0);
+  p.Hq = (int)q.size(1);
+  p.Hk = (int)k.size(1);
+  p.group = p.Hq / p.Hk;
+  p.D = (int)q.size(2);
+  p.bf16 = q.scalar_type() == torch::kBFloat16;
+}
+
+// How a call runs on a device of `sms` SMs: for tests.  Launches nothing; the tensors may lie on any device.
+py::dict attention_prompt_plan(torch::Tensor q, torch::Tensor k, torch::Tensor v, int64_t seqs, int64_t sms) {
+  PromptParams p{};
+  prompt_tensors(p, q, k, v);
+  p.B = (int)seqs;
+  const PromptPlan plan = plan_prompt(p, (int)sms);
+  py::dict d;
+  d["splits"] = plan.splits;
+  d["pack_q"] = plan.pack_q != 0;
+  d["pack_k"] = plan.pack_k != 0;
+  d["pack_v"] = plan.pack_v != 0;
+  d["bytes"] = plan.bytes();
+  return d;
+}
+
 std::tuple<torch::Tensor, OptTensor> attention_prompt(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_seqlens_q,
                                                       torch::Tensor cu_seqlens_k, bool causal, c10::optional<double> scale, OptTensor out,
                                                       bool return_lse) {
@@ -308,29 +343,14 @@ std::tuple<torch::Tensor, OptTensor> attention_prompt(torch::Tensor q, torch::Te
   OptTensor lse;
   if (return_lse) lse = fresh({Nq, Hq}, torch::kFloat32, dev);
   if (Nq == 0 || B == 0) return {res, lse};
-  p.q = q.data_ptr();
-  p.k = k.data_ptr();
-  p.v = v.data_ptr();
-  p.q_token = q.stride(0);
-  p.q_head = q.stride(1);
-  p.k_token = k.stride(0);
-  p.k_head = k.stride(1);
-  p.v_token = v.stride(0);
-  p.v_head = v.stride(1);
+  prompt_tensors(p, q, k, v);
   p.out = res.data_ptr();
   p.o_token = res.stride(0);
   p.o_head = res.stride(1);
   p.lse = lse ? lse->data_ptr<float>() : nullptr;
   p.cu_q = cu_seqlens_q.data_ptr<int>();
   p.cu_k = cu_seqlens_k.data_ptr<int>();
-  p.Nq = Nq;
-  p.Nk = Nk;
   p.B = (int)B;
-  p.Hq = (int)Hq;
-  p.Hk = (int)Hk;
-  p.group = (int)(Hq / Hk);
-  p.D = (int)D;
-  p.bf16 = q.scalar_type() == torch::kBFloat16;
   p.causal = causal;
   p.o_vec = rows16(res);
   p.status = serving_status();
@@ -350,4 +370,5 @@ void register_attention(py::module_& m) {
   m.def("kv_cache_read", &kv_cache_read);
   m.def("attention_cached", &attention_cached);
   m.def("attention_prompt", &attention_prompt);
+  m.def("attention_prompt_plan", &attention_prompt_plan);
 }

@@ -7,6 +7,7 @@
 #include <stdexcept>
 
 #include "attention.h"
+#include "attention_join.cuh"
 #include "attention_prompt.cuh"
 #include "attention_prompt_tc.cuh"
 #include "serving.h"
@@ -68,6 +69,8 @@ __global__ void __launch_bounds__(256, PromptRows<D>::CTAS) prompt_rows_kernel(P
   if (!prompt_tile(p, blockIdx.x, tokens, s, tile)) return;
   const int rows = min(tokens, s.nq - tile * tokens) * p.group;
 
+  const int all = prompt_visible(p, s, min(tile * tokens + tokens, s.nq) - 1);
+  const int keys = kRowsKeys * prompt_share(p, blockIdx.z, (all + kRowsKeys - 1) / kRowsKeys, kRowsKeys, s);
   int visible[2], token[2], hq[2];
   bool row_in[2];
 #pragma unroll
@@ -78,7 +81,6 @@ __global__ void __launch_bounds__(256, PromptRows<D>::CTAS) prompt_rows_kernel(P
     hq[r] = head * p.group + row % p.group;
     visible[r] = row_in[r] ? min(prompt_visible(p, s, token[r]), s.nk) : 0;
   }
-  const int keys = prompt_visible(p, s, min(tile * tokens + tokens, s.nq) - 1);
 
   auto copy = [&](int k0, int stage) {
     const uint32_t to = smem_u32(sm + stage * C::TILE);
@@ -237,7 +239,8 @@ __global__ void __launch_bounds__(256, PromptRows<D>::CTAS) prompt_rows_kernel(P
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     if (!row_in[r]) continue;
-    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+    const long long row = ((long long)blockIdx.z * p.Nq + s.q0 + token[r]) * p.Hq + hq[r];   // of the parts
+    const float inv = p.splits > 1 ? 1.f : l[r] == 0.f ? 0.f : 1.f / l[r];
     const long long at = (long long)(s.q0 + token[r]) * p.o_token + (long long)hq[r] * p.o_head;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) {
@@ -247,13 +250,35 @@ __global__ void __launch_bounds__(256, PromptRows<D>::CTAS) prompt_rows_kernel(P
         v[e] = o[n][2 * r + e] * inv;
         if (any_odd) v[e] = put_back_odd<D>(odd, 8 * n + 2 * t + e, visible[r], v[e]);
       }
-      float* const out = (float*)p.out + at + 8 * n + 2 * t;
-      if (p.o_vec) *(float2*)out = make_float2(v[0], v[1]);
+      float* const out = (p.splits > 1 ? p.parts + row * D : (float*)p.out + at) + 8 * n + 2 * t;
+      if (p.o_vec || p.splits > 1) *(float2*)out = make_float2(v[0], v[1]);
       else { out[0] = v[0]; out[1] = v[1]; }
     }
-    if (p.lse != nullptr && t == 0)
+    if (p.splits > 1) {
+      if (t == 0) p.stats[row] = make_float2(m[r], l[r]);
+    } else if (p.lse != nullptr && t == 0)
       p.lse[(long long)(s.q0 + token[r]) * p.Hq + hq[r]] = (m[r] + log2f(l[r])) * 0.69314718055994531f;
   }
+}
+
+// The results of tiles whose keys several CTAs shared, a warp to a row.  Rows before the first sequence and behind the last
+// stay as they are.
+template <int D>
+__global__ void __launch_bounds__(256) prompt_join_kernel(PromptParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= p.Nq * p.Hq) return;
+  const long long token = row / p.Hq, hq = row - token * p.Hq;
+  if (token < __ldg(p.cu_q) || token >= __ldg(p.cu_q + p.B)) return;
+  float top, l, v[D / 32];
+  auto at = [&](int j) { return j * p.Nq * p.Hq + row; };
+  warp_join<D>(p.splits, [&](int j) { return p.stats[at(j)]; }, [&](int j) { return p.parts + at(j) * D; }, top, l, v);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) store_elem(p.out, token * p.o_token + hq * p.o_head + D / 32 * lane + i, v[i] * inv, p.bf16);
+  if (p.lse != nullptr && lane == 0) p.lse[row] = (top + log2f(l)) * 0.69314718055994531f;
 }
 
 // Rows of a tensor [n, heads, D] that TMA can read: on 16 bytes, and apart.
@@ -261,8 +286,16 @@ static bool tma_rows(const void* t, long long token, long long head, long long n
   return ((uintptr_t)t & 15) == 0 && (n <= 1 || (token > 0 && token % 8 == 0)) && (heads <= 1 || (head > 0 && head % 8 == 0));
 }
 
+// CTAs share a tile's keys where there are fewer tiles than SMs, at least 512 keys to one.
 PromptPlan plan_prompt(const PromptParams& p, int sms) {
   PromptPlan plan{};
+  const int tokens = (p.bf16 ? 2 * (128 / p.group) : kRowsTile / p.group);
+  const long long tiles = ((p.Nq + tokens - 1) / tokens + p.B - 1) * p.Hk;   // at most
+  plan.splits = (int)std::max<long long>(1, std::min<long long>({sms / tiles, p.Nk / 512, 32}));
+  if (plan.splits > 1) {
+    plan.parts_bytes = (long long)plan.splits * p.Nq * p.Hq * p.D * 4;
+    plan.stats_bytes = ((long long)plan.splits * p.Nq * p.Hq * 8 + 255) / 256 * 256;
+  }
   if (!p.bf16) return plan;
   auto bytes = [&](long long n, int heads) { return (n * heads * p.D * 2 + 255) / 256 * 256; };
   plan.pack_q = !tma_rows(p.q, p.q_token, p.q_head, p.Nq, p.Hq);
@@ -294,7 +327,7 @@ static void launch_prompt_rows(const PromptParams& p, cudaStream_t s) {
   const int tokens = kRowsTile / p.group;
   auto aligned = [&](const void* t, long long a, long long b) { return (((uintptr_t)t | (a * 4) | (b * 4)) & 15) == 0; };
   const bool vec = aligned(p.k, p.k_token, p.k_head) && aligned(p.v, p.v_token, p.v_head);
-  const dim3 grid((unsigned)((p.Nq + tokens - 1) / tokens + p.B), (unsigned)p.Hk);
+  const dim3 grid((unsigned)((p.Nq + tokens - 1) / tokens + p.B - 1), (unsigned)p.Hk, (unsigned)p.splits);
   launch_with_pdl(kern, grid, dim3(256), C::SMEM, s, true, p, vec);
 }
 
@@ -317,18 +350,28 @@ static void launch_prompt_tc(const PromptParams& p, cudaStream_t s) {
   // without keys nothing is loaded; a map has to name something
   const CUtensorMap tk = p.Nk > 0 ? prompt_map(p.k, p.k_token, p.k_head, p.Nk, p.Hk, D, 1, kPromptKeys) : tq;
   const CUtensorMap tv = p.Nk > 0 ? prompt_map(p.v, p.v_token, p.v_head, p.Nk, p.Hk, D, 1, kPromptKeys) : tq;
-  const long long tiles = (p.Nq + 2 * tokens - 1) / (2 * tokens) + p.B;   // at most
-  launch_with_pdl(kern, dim3((unsigned)(tiles * p.Hk)), dim3(kPromptThreads), C::SMEM, s, true, tq, tk, tv, p);
+  const long long tiles = (p.Nq + 2 * tokens - 1) / (2 * tokens) + p.B - 1;   // at most
+  launch_with_pdl(kern, dim3((unsigned)(tiles * p.Hk), (unsigned)p.splits), dim3(kPromptThreads), C::SMEM, s, true, tq, tk, tv, p);
 }
 
 void launch_prompt(const PromptParams& params, const PromptPlan& plan, void* workspace, cudaStream_t s) {
   PromptParams p = params;
+  char* ws = (char*)workspace;
+  p.splits = plan.splits;
+  p.parts = (float*)ws;
+  p.stats = (float2*)(ws + plan.parts_bytes);
+  ws += plan.parts_bytes + plan.stats_bytes;
+  auto join = [&] {
+    if (p.splits == 1) return;
+    const dim3 grid((unsigned)((p.Nq * p.Hq + 7) / 8));
+    if (p.D == 128) launch_with_pdl(prompt_join_kernel<128>, grid, dim3(256), 0, s, true, p);
+    else launch_with_pdl(prompt_join_kernel<64>, grid, dim3(256), 0, s, true, p);
+  };
   if (!p.bf16) {
     if (p.D == 128) launch_prompt_rows<128>(p, s);
     else launch_prompt_rows<64>(p, s);
-    return;
+    return join();
   }
-  char* ws = (char*)workspace;
   auto pack = [&](const void*& t, long long& token, long long& head, long long n, int heads, long long bytes) {
     launch_pack_rows(t, token, head, heads, ws, p.D, n, p.D, 1, s);   // [heads, tokens, D]
     t = ws;
@@ -341,6 +384,7 @@ void launch_prompt(const PromptParams& params, const PromptPlan& plan, void* wor
   if (plan.pack_v) pack(p.v, p.v_token, p.v_head, p.Nk, p.Hk, plan.v_bytes);
   if (p.D == 128) launch_prompt_tc<128>(p, s);
   else launch_prompt_tc<64>(p, s);
+  join();
 }
 
 }  // namespace raiccl

@@ -92,6 +92,38 @@ def test_longer(hk, group, lens, dim):
         _check(q, k, v, lens, lens)
 
 
+def _plan(q, k, v, seqs):
+    from revealaiccl_b200.ops._native import kernels
+    return kernels().attention_prompt_plan(q, k, v, seqs, torch.cuda.get_device_properties(DEV).multi_processor_count)
+
+
+@DTYPES
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("hk,group,dim,q_lens,k_lens", [
+    (1, 1, 64, [1], [9001]), (2, 4, 128, [3, 40], [5000, 4100]), (1, 8, 128, [130, 0, 2], [4000, 700, 0]), (2, 3, 64, [7, 5], [3, 8000]),
+])
+def test_keys_shared_by_ctas(hk, group, dim, q_lens, k_lens, causal, dtype):
+    """Few queries of many keys: several CTAs to a tile.  What no token sees stays outside, and rows around are left alone."""
+    q, k, v = _make(q_lens, k_lens, hk, group, dim, dtype, seed=27)
+    assert _plan(q, k, v, len(q_lens))["splits"] > 1
+    out, lse = _check(q, k, v, q_lens, k_lens, causal)
+    n = sum(q_lens)
+    big, wide = torch.zeros(n + 9, hk * group, dim, dtype=dtype, device=DEV), torch.full((n + 9, hk * group + 1, dim), 7.0, dtype=dtype, device=DEV)
+    big[4:4 + n] = q
+    k2, v2 = (torch.cat([x, torch.full_like(x[:50], NAN)]) for x in (k, v))
+    got, glse = _attend(big, k2, v2, _cu(q_lens) + 4, _cu(k_lens), causal=causal, out=wide[:, 1:], return_lse=True, check=True)
+    assert torch.equal(got[4:4 + n], out) and torch.equal(glse[4:4 + n], lse)
+    got[4:4 + n] = 7.0
+    assert (wide == 7.0).all()
+    v2[k_lens[0] - 1, 0, 3] = INF                   # the last key of the first sequence
+    if q_lens[0] <= k_lens[0]:
+        got = _attend(q, k2, v2, _cu(q_lens), _cu(k_lens), causal=causal, check=True)
+        last = q_lens[0] - 1 if causal else 0
+        assert (got[last:q_lens[0], :group, 3] == INF).all()
+        got[last:q_lens[0], :group, 3] = out[last:q_lens[0], :group, 3]
+        assert torch.equal(got, out)
+
+
 @DTYPES
 def test_many_sequences(dtype):
     lens = [(5 * i) % 23 for i in range(400)]
