@@ -1,0 +1,374 @@
+// Attention over whole prompts on the tensor cores, fp32.
+//
+// Every number is three bf16 parts, x = x0 + x1 + x2 (24 bits, fp32's range), and
+// a product the six of their products that fp32 can show: twelve bits below the
+// largest the others are lost in its rounding.  (Two f16 parts would take three
+// products, but their range is not fp32's; tf32 ones have half the rate and no
+// transposed values.)  The parts of q, k and v are written first, by
+// prompt_split_kernel, as TMA reads them; those of the weights P by the threads
+// that work them out, into TMEM.
+//
+// One tile of 128 rows to a CTA; KT keys a step.  S has two buffers, so that Q K^T
+// of the next step runs while the softmax has this one; the softmax waits for P V
+// of the last step before it writes P.  The tensor core cuts what does not fit its
+// sums: the small products come first, and P V leaves it after every step and is
+// added up in registers (with one sum for all steps 2048 keys were 4e-6 off).
+//
+// Values go through two warps that look for numbers that are not finite
+// (attention_prompt.cuh): an infinity times a part of a weight that is negative
+// would be NaN.
+#pragma once
+
+#include "attention_prompt_tc.cuh"
+
+namespace raiccl {
+
+constexpr int kFp32Threads = 256;   // the softmax's four warps; loads, products, two warps for the values
+
+template <int D>
+struct PromptFp32 {
+  static constexpr int KT = D == 64 ? 128 : 64;               // keys of a step
+  static constexpr int HALVES = D / 64;
+  static constexpr int Q_PART = 128 * D * 2, KV_PART = KT * D * 2;
+  static constexpr int KSTAGES = D == 64 ? 2 : 1;             // of keys; values have one
+  static constexpr int SMEM = 1024 + 3 * (Q_PART + (KSTAGES + 1) * KV_PART);
+  static constexpr uint32_t P_AT = 2 * KT, O_AT = D == 64 ? 448 : 256;   // columns of TMEM behind the two of S
+};
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* desc, uint64_t* bar, int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(desc), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// Three bf16 parts, each rounded to nearest, but cut where that would give an infinity; an infinity or NaN is its first part.
+__device__ __forceinline__ void split3(float v, float (&part)[3]) {
+  const float r = __bfloat162float(__float2bfloat16_rn(v));
+  part[0] = fabsf(r) == INFINITY ? __uint_as_float(__float_as_uint(v) & 0xffff0000u) : r;
+  if (!(fabsf(v) < INFINITY)) {
+    part[0] = v;
+    part[1] = part[2] = 0.f;
+    return;
+  }
+  part[1] = __bfloat162float(__float2bfloat16_rn(v - part[0]));
+  part[2] = v - part[0] - part[1];
+}
+
+struct SplitTensor {
+  const float* src;            // [n, heads, D]
+  long long token, head, n;
+  __nv_bfloat16* dst;          // [3][n][heads][D]
+  int heads, vec;
+};
+
+// One read, and three writes of half the size; eight numbers to a thread.
+template <int D>
+__global__ void __launch_bounds__(256) prompt_split_kernel(SplitTensor q, SplitTensor k, SplitTensor v) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const SplitTensor& s = blockIdx.y == 0 ? q : blockIdx.y == 1 ? k : v;
+  const long long numbers = s.n * s.heads * D;
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8; i < numbers; i += (long long)gridDim.x * 2048) {
+    const long long row = i / D, token = row / s.heads;
+    const float* const src = s.src + token * s.token + (row - token * s.heads) * s.head + i % D;
+    float x[8];
+    if (s.vec) {
+      *(float4*)x = __ldg((const float4*)src);
+      *(float4*)(x + 4) = __ldg((const float4*)src + 1);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = src[e];
+    }
+    float part[8][3];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) split3(x[e], part[e]);
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      *(uint4*)(s.dst + j * numbers + i) = make_uint4(pack_bf16(part[0][j], part[1][j]), pack_bf16(part[2][j], part[3][j]),
+                                                      pack_bf16(part[4][j], part[5][j]), pack_bf16(part[6][j], part[7][j]));
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kFp32Threads, 1)
+prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                   PromptParams p) {
+  using C = PromptFp32<D>;
+  constexpr int KT = C::KT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* const sq = smem;
+  uint8_t* const sk = smem + 3 * C::Q_PART;
+  uint8_t* const sv = sk + C::KSTAGES * 3 * C::KV_PART;
+  __shared__ uint64_t q_full, k_full[C::KSTAGES], k_empty[C::KSTAGES], v_raw, v_ready, v_empty, s_full[2], p_full, o_full, drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int odd[3][D], any_odd;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int tokens = 128 / p.group;
+  const int head = blockIdx.x % p.Hk;
+  PromptSeq s;
+  int tile;
+  if (!prompt_tile(p, blockIdx.x / p.Hk, tokens, s, tile)) return;
+  const int token0 = tile * tokens;
+  const int keys = prompt_visible(p, s, min(token0 + tokens, s.nq) - 1);
+  const int steps = prompt_share(p, blockIdx.y, (keys + KT - 1) / KT, KT, s);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&q_full, 1);
+    for (int i = 0; i < C::KSTAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+    mbar_init(&v_raw, 1); mbar_init(&v_ready, 2); mbar_init(&v_empty, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
+    mbar_init(&p_full, 4); mbar_init(&o_full, 1); mbar_init(&drained, 1);
+    fence_mbarrier_init();
+    any_odd = 0;
+    tma_prefetch_desc(&tq); tma_prefetch_desc(&tk); tma_prefetch_desc(&tv);
+  }
+  for (int i = threadIdx.x; i < 3 * D; i += kFp32Threads) ((int*)odd)[i] = INT_MAX;
+  if (warp == 5) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
+
+  if (warp == 4) {
+    // ---------------------------------------------------------------- loads
+    if (steps > 0 && elect_one_sync()) {
+      mbar_arrive_expect_tx(&q_full, 3 * C::HALVES * tokens * p.group * 128);
+      for (int part = 0; part < 3; ++part)
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_4d(sq + part * C::Q_PART + h * 128 * 128, &tq, &q_full, 64 * h, head * p.group, s.q0 + token0, part);
+      auto load = [&](uint8_t* at, const CUtensorMap* map, uint64_t* full, int i) {
+        mbar_arrive_expect_tx(full, 3 * C::KV_PART);
+        for (int part = 0; part < 3; ++part)
+          for (int h = 0; h < C::HALVES; ++h)
+            tma_load_4d(at + part * C::KV_PART + h * KT * 128, map, full, 64 * h, head, s.k0 + i * KT, part);
+      };
+      int nk = 0, nv = 0;
+      bool ok = true;
+      auto load_k = [&] {
+        const int st = nk % C::KSTAGES;
+        if (!(ok = wait(&k_empty[st], ((nk / C::KSTAGES) & 1) ^ 1u))) return;
+        load(sk + st * 3 * C::KV_PART, &tk, &k_full[st], nk);
+        ++nk;
+      };
+      load_k();
+      for (int i = 0; ok && i < steps; ++i) {
+        if (C::KSTAGES == 2 && nk < steps) load_k();
+        if (!ok || !(ok = wait(&v_empty, (i & 1) ^ 1u))) break;
+        load(sv, &tv, &v_raw, i);
+        ++nv;
+        if (C::KSTAGES == 1 && nk < steps) load_k();
+      }
+      // the copies land before the CTA leaves
+      wait(&q_full, 0);
+      for (int i = max(0, nk - C::KSTAGES); i < nk; ++i) wait(&k_full[i % C::KSTAGES], (i / C::KSTAGES) & 1);
+      if (nv > 0) wait(&v_raw, (nv - 1) & 1);
+    }
+  } else if (warp == 5) {
+    // ---------------------------------------------------------------- products
+    if (steps > 0 && elect_one_sync()) {
+      constexpr uint32_t iqk = umma_idesc(1u, 128, KT), ipv = umma_idesc(1u, 128, D) | (1u << 16);
+      constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};   // parts, the small products first
+      const uint64_t krow = umma_desc_k_sw128(0), vrow = umma_desc_mn_sw128(0, KT * 128);
+      auto qk = [&](int i) {
+        const uint64_t a = desc_at(krow, smem_u32(sq)), b = desc_at(krow, smem_u32(sk + (i % C::KSTAGES) * 3 * C::KV_PART));
+#pragma unroll
+        for (int j = 0; j < 6; ++j)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_f16(tmem + KT * (i & 1), a + (A[j] * C::Q_PART + (k / 4) * 128 * 128) / 16 + (k % 4) * 2,
+                     b + (B[j] * C::KV_PART + (k / 4) * KT * 128) / 16 + (k % 4) * 2, iqk, j > 0 || k > 0);
+        umma_commit(&s_full[i & 1]);
+        umma_commit(&k_empty[i % C::KSTAGES]);
+      };
+      bool ok = wait(&q_full, 0) && wait(&k_full[0], 0);
+      if (ok) {
+        tc_fence_after_sync();
+        qk(0);
+      }
+      for (int i = 0; ok && i < steps; ++i) {
+        // S of the step after this one goes where the one before was, which was read before its P came
+        if (i + 1 < steps) {
+          if (!(ok = wait(&k_full[(i + 1) % C::KSTAGES], ((i + 1) / C::KSTAGES) & 1))) break;
+          tc_fence_after_sync();
+          qk(i + 1);
+        }
+        if (!(ok = wait(&v_ready, i & 1) && wait(&p_full, i & 1))) break;
+        tc_fence_after_sync();
+        const uint64_t b = desc_at(vrow, smem_u32(sv));
+#pragma unroll
+        for (int j = 0; j < 6; ++j)
+#pragma unroll
+          for (int k = 0; k < KT / 16; ++k)
+            umma_f16_ts(tmem + C::O_AT, tmem + C::P_AT + A[j] * (KT / 2) + 8 * k, b + (B[j] * C::KV_PART + k * 16 * 128) / 16, ipv, j > 0 || k > 0);
+        umma_commit(&v_empty);
+        umma_commit(&o_full);
+      }
+      umma_commit(&drained);
+      wait(&drained, 0);
+    }
+  } else if (warp >= 6) {
+    // ---------------------------------------------------------------- values
+    for (int i = 0; i < steps; ++i) {
+      if (!mbar_wait_warp(&v_raw, i & 1, p.status, kPromptKernelId, kPromptWaitNs)) break;
+      uint4* const at = (uint4*)sv;
+#pragma unroll 4
+      for (int c = (warp - 6) * 32 + lane; c < C::KV_PART / 16; c += 64) {
+        const int half = c / (KT * 8), row = (c / 8) % KT, key = i * KT + row;
+        if (key >= s.nk) {           // behind the sequence's end
+#pragma unroll
+          for (int part = 0; part < 3; ++part) at[part * (C::KV_PART / 16) + c] = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        const uint4 v = at[c];       // the first part: what is not finite is there
+        auto bad = [](uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; };
+        if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          const int d = 64 * half + 8 * ((c & 7) ^ (row & 7));
+          for (int e = 0; e < 8; ++e) {
+            const float f = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+            if (fabsf(f) < INFINITY) continue;
+            atomicMin(&odd[odd_kind(f)][d + e], key);
+            w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+          }
+          any_odd = 1;
+          at[c] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&v_ready);
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax, one row to a thread
+    const int row = threadIdx.x, token = token0 + row / p.group, hq = head * p.group + row % p.group;
+    const bool mine = row < tokens * p.group && token < s.nq;
+    const int visible = mine ? min(prompt_visible(p, s, token), s.nk) : 0;
+    const int all = __reduce_min_sync(0xffffffffu, mine ? visible : INT_MAX);
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    float mult = p.scale * 1.44269504088896341f;
+    const float turn = mult > 0.f ? 1.f : mult < 0.f ? -1.f : 0.f;
+    mult = turn == 0.f ? 1.f : fabsf(mult);
+    float m = -INFINITY, l = 0.f, o[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) o[d] = 0.f;
+    // the sums of step i, once its products are done
+    auto add = [&](int i) {
+      if (!mbar_wait_warp(&o_full, i & 1, p.status, kPromptKernelId, kPromptWaitNs)) return false;
+      tc_fence_after_sync();
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(lanes + C::O_AT + c, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[c + e] += __uint_as_float(r[e]);
+      }
+      return true;
+    };
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+      if (!(ok = mbar_wait_warp(&s_full[i & 1], (i >> 1) & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+      tc_fence_after_sync();
+      uint32_t r[KT];
+#pragma unroll
+      for (int c = 0; c < KT; c += 32) tmem_ld32(lanes + KT * (i & 1) + c, r + c);
+      tmem_ld_wait();
+      if (turn != 1.f) {
+#pragma unroll
+        for (int c = 0; c < KT; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * turn);
+      }
+      const int k0 = i * KT;
+      if (k0 + KT > all) {
+#pragma unroll
+        for (int c = 0; c < KT; ++c)
+          if (k0 + c >= visible) r[c] = __float_as_uint(-INFINITY);
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < KT; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
+      const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
+      if (i > 0 && !(ok = add(i - 1))) break;    // before P is written where its operand was
+      const bool grow = peak > m + 8.f;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float now = grow ? peak : m;
+        const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
+        m = now;
+        l *= shrink;
+#pragma unroll
+        for (int d = 0; d < D; ++d) o[d] *= shrink;
+      }
+      const float base = m == -INFINITY ? 0.f : -m;
+      const uint64_t mult2 = pair_f32(mult, mult), base2 = pair_f32(base, base);
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int h = 0; h < KT; h += 64) {
+        uint32_t w[3][32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          float u, v;
+          unpair_f32(fma2(pair_f32(__uint_as_float(r[h + 2 * c]), __uint_as_float(r[h + 2 * c + 1])), mult2, base2), u, v);
+          uint64_t x = pair_f32(prompt_exp2(u), prompt_exp2(v));
+          sum[c & 1] = add2(sum[c & 1], x);
+#pragma unroll
+          for (int part = 0; part < 3; ++part) {
+            unpair_f32(x, u, v);
+            const uint32_t rounded = pack_bf16(u, v);
+            w[part][c] = rounded;
+            if (part < 2) x = add2(x, pair_f32(__uint_as_float((rounded << 16) ^ 0x80000000u), __uint_as_float((rounded & 0xffff0000u) ^ 0x80000000u)));
+          }
+        }
+#pragma unroll
+        for (int part = 0; part < 3; ++part) tmem_st32(lanes + C::P_AT + part * (KT / 2) + h / 2, w[part]);
+      }
+      float s0, s1;
+      unpair_f32(add2(sum[0], sum[1]), s0, s1);
+      l += s0 + s1;
+      tmem_st_wait();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full);
+    }
+    if (ok && steps > 0) ok = add(steps - 1);
+    // a row that sees keys has a sum, unless all its logits are -inf
+    if (l == 0.f && visible > 0 && steps > 0) l = NAN;
+    const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const long long at = ((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq;   // of the parts
+    float* const dst = p.splits > 1 ? p.parts + at * D : (float*)p.out + (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head;
+    if (any_odd) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) o[d] = put_back_odd<D>(odd, d, visible, o[d] * inv);
+    } else {
+#pragma unroll
+      for (int d = 0; d < D; ++d) o[d] *= inv;
+    }
+    if (mine) {
+      if (p.o_vec || p.splits > 1) {
+#pragma unroll
+        for (int d = 0; d < D; d += 4) *(float4*)(dst + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+      } else {
+#pragma unroll
+        for (int d = 0; d < D; ++d) dst[d] = o[d];
+      }
+      if (p.splits > 1) p.stats[at] = make_float2(m, l);
+      else if (p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+    }
+  }
+  __syncwarp();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 5) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace raiccl
