@@ -106,18 +106,8 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   __shared__ uint32_t tmem_slot;
   __shared__ int odd[3][D], any_odd;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_wait();
-  griddep_launch_dependents();
-
-  const int tokens = 128 / p.group;
-  const int head = blockIdx.x % p.Hk;
-  PromptSeq s;
-  int tile;
-  if (!prompt_tile(p, blockIdx.x / p.Hk, tokens, s, tile)) return;
-  const int token0 = tile * tokens;
-  const int keys = prompt_visible(p, s, min(token0 + tokens, s.nq) - 1);
-  const int steps = prompt_share(p, blockIdx.y, (keys + KT - 1) / KT, KT, s);
-
+  // Nothing of this needs what the kernels before wrote.  TMEM has to be taken before the next kernel may start: one that took
+  // it first would keep it until this CTA is done.
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
     for (int i = 0; i < C::KSTAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
@@ -135,6 +125,23 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int tokens = 128 / p.group;
+  const int head = blockIdx.x % p.Hk;
+  PromptSeq s;
+  int tile;
+  const bool some = prompt_tile(p, blockIdx.x / p.Hk, tokens, s, tile);
+  if (!some) {
+    __syncthreads();
+    if (warp == 5) tmem_dealloc(tmem, 512);
+    return;
+  }
+  const int token0 = tile * tokens;
+  const int keys = prompt_visible(p, s, min(token0 + tokens, s.nq) - 1);
+  const int steps = prompt_share(p, blockIdx.y, (keys + KT - 1) / KT, KT, s);
+
   auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
 
   if (warp == 4) {

@@ -144,22 +144,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   __shared__ uint32_t tmem_slot;
   __shared__ int odd[3][D], any_odd;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  griddep_wait();
-  griddep_launch_dependents();
-
-  const int tokens = 128 / p.group;                           // of a tile
-  const int head = blockIdx.x % p.Hk;
-  PromptSeq s;
-  int pair;
-  if (!prompt_tile(p, blockIdx.x / p.Hk, 2 * tokens, s, pair)) return;
-  const int token0 = pair * 2 * tokens;                       // of the sequence, A's first
-  const int tiles = token0 + tokens < s.nq ? 2 : 1;
-  const int keys = prompt_visible(p, s, min(token0 + 2 * tokens, s.nq) - 1);
-  const int steps = prompt_share(p, blockIdx.y, (keys + kPromptKeys - 1) / kPromptKeys, kPromptKeys, s);
-  // Values of tiles from here on, which some row does not see whole, arrive on v_raw and go through two warps first.
-  const int first_fixed = min(prompt_visible(p, s, token0), s.nk) / kPromptKeys;
-  auto fixed_phase = [&](int i) { return (uint32_t)((i - first_fixed) / C::STAGES) & 1u; };   // of v_raw and v_ready
-
+  // Nothing of this needs what the kernels before wrote.  TMEM has to be taken before the next kernel may start: one that took
+  // it first would keep it until this CTA is done.
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
     for (int i = 0; i < C::STAGES; ++i) {
@@ -178,6 +164,26 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const int tokens = 128 / p.group;                           // of a tile
+  const int head = blockIdx.x % p.Hk;
+  PromptSeq s;
+  int pair;
+  const bool some = prompt_tile(p, blockIdx.x / p.Hk, 2 * tokens, s, pair);
+  if (!some) {
+    __syncthreads();
+    if (warp == 9) tmem_dealloc(tmem, 512);
+    return;
+  }
+  const int token0 = pair * 2 * tokens;                       // of the sequence, A's first
+  const int tiles = token0 + tokens < s.nq ? 2 : 1;
+  const int keys = prompt_visible(p, s, min(token0 + 2 * tokens, s.nq) - 1);
+  const int steps = prompt_share(p, blockIdx.y, (keys + kPromptKeys - 1) / kPromptKeys, kPromptKeys, s);
+  // Values of tiles from here on, which some row does not see whole, arrive on v_raw and go through two warps first.
+  const int first_fixed = min(prompt_visible(p, s, token0), s.nk) / kPromptKeys;
+  auto fixed_phase = [&](int i) { return (uint32_t)((i - first_fixed) / C::STAGES) & 1u; };   // of v_raw and v_ready
 
   // 168 registers to a thread at launch: the warpgroups of the softmax, which hold a row of S, get 208, the other 88.
   if (warp >= 8) {
