@@ -13,7 +13,8 @@ struct PromptSeq {
   int q0, nq, k0, nk;
 };
 
-// Ends outside of the tensors, or before their beginnings, are recorded and cut.
+// Ends outside of the tensors, or before their beginnings, are cut, and recorded by one warp of the launch.
+template <bool RECORD = false>
 __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
   const int q0 = __ldg(p.cu_q + b), q1 = __ldg(p.cu_q + b + 1), k0 = __ldg(p.cu_k + b), k1 = __ldg(p.cu_k + b + 1);
   PromptSeq s;
@@ -22,39 +23,50 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int b) {
   const int qe = q1 < s.q0 ? s.q0 : q1 > p.Nq ? (int)p.Nq : q1, ke = k1 < s.k0 ? s.k0 : k1 > p.Nk ? (int)p.Nk : k1;
   s.nq = qe - s.q0;
   s.nk = ke - s.k0;
-  if (s.q0 != q0 || qe != q1) record_status(p.status, kBoundsViolation, kPromptKernelId, q1, p.Nq);
-  if (s.k0 != k0 || ke != k1) record_status(p.status, kBoundsViolation, kPromptKernelId, k1, p.Nk);
+  if (RECORD && (s.q0 != q0 || qe != q1)) record_status(p.status, kBoundsViolation, kPromptKernelId, q1, p.Nq);
+  if (RECORD && (s.k0 != k0 || ke != k1)) record_status(p.status, kBoundsViolation, kPromptKernelId, k1, p.Nk);
   return s;
 }
 
-// The tile `index` of all sequences' tiles of `tokens` tokens of q; false behind the last.  A whole warp calls it.
-// Within a sequence the last tile, which sees the most keys, comes first.
+__device__ __forceinline__ void prompt_record(const PromptParams& p) {
+  for (int b = threadIdx.x & 31; b < p.B; b += 32) prompt_seq<true>(p, b);
+}
+
+// Tiles of `tokens` tokens of q that sequence b has, by its cut ends.
+__device__ __forceinline__ int prompt_tiles(const PromptParams& p, int b, int tokens) {
+  const int n = (int)p.Nq, q0 = min(max(__ldg(p.cu_q + b), 0), n), q1 = min(max(__ldg(p.cu_q + b + 1), q0), n);
+  return (q1 - q0 + tokens - 1) / tokens;
+}
+
+// The tile `index` of all sequences' tiles of `tokens` tokens of q; false behind the last.  A whole warp calls it: every lane
+// counts an equal number of sequences, then the warp goes through those of the lane that has the tile.  Within a sequence the
+// last tile, which sees the most keys, comes first.
 __device__ __forceinline__ bool prompt_tile(const PromptParams& p, int index, int tokens, PromptSeq& s, int& tile) {
   const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    PromptSeq mine{};
-    if (b0 + lane < p.B) mine = prompt_seq(p, b0 + lane);
-    const int n = (mine.nq + tokens - 1) / tokens;
-    int sum = n;
+  int first = 0, each = p.B, before = 0;
+  while (true) {
+    const int per = (each + 31) / 32, b0 = first + lane * per, b1 = min(b0 + per, first + each);
+    int sum = 0;
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) sum += prompt_tiles(p, b, tokens);
+    const int mine = sum;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
       const int up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
     const uint32_t in = __ballot_sync(0xffffffffu, index < before + sum);
-    if (in) {
-      const int at = __ffs(in) - 1;
-      s.q0 = __shfl_sync(0xffffffffu, mine.q0, at);
-      s.nq = __shfl_sync(0xffffffffu, mine.nq, at);
-      s.k0 = __shfl_sync(0xffffffffu, mine.k0, at);
-      s.nk = __shfl_sync(0xffffffffu, mine.nk, at);
-      tile = before + __shfl_sync(0xffffffffu, sum, at) - 1 - index;
+    if (in == 0) return false;
+    const int at = __ffs(in) - 1;
+    before += __shfl_sync(0xffffffffu, sum - mine, at);
+    first += at * per;
+    if (per == 1) {
+      s = prompt_seq(p, first);
+      tile = before + __shfl_sync(0xffffffffu, mine, at) - 1 - index;
       return true;
     }
-    before += __shfl_sync(0xffffffffu, sum, 31);
+    each = min(per, p.B - first);
   }
-  return false;
 }
 
 // This CTA's share of a tile's `steps` steps of `width` keys, where several CTAs share them: the sequence is cut to it, so

@@ -127,6 +127,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   const uint32_t tmem = tmem_slot;
   griddep_wait();
   griddep_launch_dependents();
+  if (blockIdx.x + blockIdx.y == 0 && warp == 7) prompt_record(p);
 
   const int tokens = 128 / p.group;
   const int head = blockIdx.x % p.Hk;

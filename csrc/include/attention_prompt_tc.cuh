@@ -166,6 +166,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   const uint32_t tmem = tmem_slot;
   griddep_wait();
   griddep_launch_dependents();
+  if (blockIdx.x + blockIdx.y == 0 && warp == 11) prompt_record(p);
 
   const int tokens = 128 / p.group;                           // of a tile
   const int head = blockIdx.x % p.Hk;

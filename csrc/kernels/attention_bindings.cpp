@@ -326,14 +326,14 @@ std::tuple<torch::Tensor, OptTensor> attention_prompt(torch::Tensor q, torch::Te
   const int64_t Nq = q.size(0), Hq = q.size(1), D = q.size(2), Nk = k.size(0), Hk = k.size(1);
   check_head_dim(op, D);
   TORCH_CHECK_VALUE(k.size(2) == D && v.sizes() == k.sizes(), op, ": k and v must be [tokens, kv_heads, ", text(D), "], alike");
-  TORCH_CHECK_VALUE(Hk >= 1 && Hk <= 1024 && Hq >= 1 && Hq % Hk == 0 && Hq / Hk <= 128, op, ": q must have 1 to 128 heads for each of k's (1 to 1024), got ",
-                    text(Hq), " and ", text(Hk));
+  TORCH_CHECK_VALUE(Hk >= 1 && Hk <= 1024 && Hq >= 1 && Hq % Hk == 0 && Hq / Hk <= 128 && Hq < 65536, op,
+                    ": q must have 1 to 128 heads for each of k's (1 to 1024; less than 65536 in all), got ", text(Hq), " and ", text(Hk));
   TORCH_CHECK_VALUE(is_float_type(q) && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), op,
                     ": q, k and v must all be bf16 or all be fp32");
   TORCH_CHECK_VALUE(Nq < (1ll << 30) && Nk < (1ll << 30), op, ": less than 2^30 tokens");
   TORCH_CHECK_VALUE(cu_seqlens_q.dim() == 1 && cu_seqlens_q.size(0) >= 1, op, ": cu_seqlens_q must have one entry more than there are sequences");
   const int64_t B = cu_seqlens_q.size(0) - 1;
-  TORCH_CHECK_VALUE(B < (1 << 20), op, ": less than 2^20 sequences in one call");
+  TORCH_CHECK_VALUE(B <= (1 << 16), op, ": at most 2^16 sequences in one call");
   check_index(op, "cu_seqlens_q", cu_seqlens_q, dev, B + 1);
   check_index(op, "cu_seqlens_k", cu_seqlens_k, dev, B + 1);
   PromptParams p{};

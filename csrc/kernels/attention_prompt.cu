@@ -46,7 +46,7 @@ static bool tma_rows(const void* t, long long token, long long head, long long n
 PromptPlan plan_prompt(const PromptParams& p, int sms) {
   PromptPlan plan{};
   const int tokens = (p.bf16 ? 2 : 1) * (128 / p.group);
-  const long long tiles = ((p.Nq + tokens - 1) / tokens + p.B - 1) * p.Hk;   // at most
+  const long long tiles = std::max<long long>(1, ((p.Nq + tokens - 1) / tokens + p.B - 1) * p.Hk);   // at most
   plan.splits = (int)std::max<long long>(1, std::min<long long>({sms / tiles, p.Nk / 512, 32}));
   if (plan.splits > 1) {
     plan.parts_bytes = (long long)plan.splits * p.Nq * p.Hq * p.D * 4;

@@ -46,7 +46,7 @@ def attention_cached(
     A page that is not the cache's is left out, a length behind the table's row
     cut, and both are recorded: ``check=True`` waits and raises.  Enqueues two
     launches on the current stream without synchronising and can be captured in
-    a CUDA graph.  Workspace, of torch's allocator: up to 2.5 MB.  There is no
+    a CUDA graph.  Workspace, of torch's allocator: up to 20 MB.  There is no
     backward: tensors that require a gradient or carry a tangent are refused.
     """
     res, lse = kernels().attention_cached(q, *cache._parts(), block_table, lengths, scale, out, out_dtype, return_lse)
@@ -77,17 +77,24 @@ def attention_prompt(
     cu_seqlens_k[b + 1] of k and v (int32, default: the same).  ``causal``: the
     last token of a sequence in q sees all its keys, every one before it one
     less, so k and v may begin with earlier tokens of a chunked prompt.  A token
-    that sees nothing gets zeros, and rows of ``out`` behind the last sequence
-    are left as they were.  What a token does not see does not enter its result,
-    infinities and NaN included.  scale: default head_dim ** -0.5.
+    that sees nothing gets zeros, and rows of ``out`` before the first and behind
+    the last sequence are left as they were.  What a token does not see does not
+    enter its result, infinities and NaN included.  scale: default head_dim **
+    -0.5.  At most 2^16 sequences.
 
     Sums, maxima and the result are kept in fp32 and rounded once, to q's type.
-    fp32 inputs are multiplied to fp32 accuracy.  ``return_lse``: also log sum
-    exp(scale * q K^T), fp32 [tokens, heads], -inf where a token sees nothing.
+    With bf16 inputs the probabilities enter their product as bf16 numbers; fp32
+    inputs and their probabilities are three bf16 numbers each, which is fp32's
+    accuracy (an infinite logit may come out as NaN).  ``return_lse``: also log
+    sum exp(scale * q K^T), fp32 [tokens, heads], -inf where a token sees nothing,
+    undefined outside of the sequences.
 
     Offsets that lie outside of the tensors or fall are cut and recorded:
-    ``check=True`` waits and raises.  Enqueues on the current stream without
-    synchronising and can be captured in a CUDA graph.  There is no backward:
+    ``check=True`` waits and raises.  Enqueues one to three launches on the
+    current stream without synchronising and can be captured in a CUDA graph;
+    rows that do not start on 16 bytes are copied first.  Workspace, of torch's
+    allocator: those copies, one and a half times the inputs in fp32, and with few
+    tiles of many keys up to 32 times the result in fp32.  There is no backward:
     tensors that require a gradient or carry a tangent are refused.
     """
     res, lse = kernels().attention_prompt(q, k, v, cu_seqlens_q, cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k,

@@ -55,10 +55,11 @@ def check(status: torch.Tensor) -> None:
 
 
 def check_serving(device: torch.device | str | int | None = None) -> None:
-    """Wait for ``device`` and raise if a bounded wait ran out in one of its
-    ``linear`` / ``moe_few_tokens`` calls since the last check; the record is
-    cleared.  The failed call's result is incomplete; the calls behind it are
-    not affected."""
+    """Wait for ``device`` and raise if, in one of its serving operators' calls
+    (``linear``, ``moe_few_tokens``, attention and its cache) since the last
+    check, a bounded wait ran out or a page, slot or offset lay outside; the
+    record is cleared.  The failed call's result is incomplete, or without what
+    lay outside; the calls behind it are not affected."""
     from ._native import kernels
 
     dev = torch.device("cuda" if device is None else device if not isinstance(device, int) else f"cuda:{device}")

@@ -125,8 +125,10 @@ def test_keys_shared_by_ctas(hk, group, dim, q_lens, k_lens, causal, dtype):
 
 
 @DTYPES
-def test_many_sequences(dtype):
-    lens = [(5 * i) % 23 for i in range(400)]
+@pytest.mark.parametrize("seqs", [33, 400, 2100])
+def test_many_sequences(seqs, dtype):
+    lens = [(5 * i) % 23 for i in range(seqs)]
+    lens[seqs // 2] = 300                        # of many tiles, between others
     q, k, v = _make(lens, lens, 2, 2, 64, dtype, seed=13)
     _check(q, k, v, lens, lens)
 

@@ -174,6 +174,8 @@ def test_cached_refuses(kw, words):
     (dict(q=_t(9, 6, 64, dtype=FP32)), "all be bf16 or all be fp32"),
     (dict(q=_t(9, 6, 64).half(), k=_t(9, 2, 64).half(), v=_t(9, 2, 64).half()), "all be bf16 or all be fp32"),
     (dict(k=_t(9, 64, 2).transpose(1, 2)), "contiguous rows"),
+    (dict(q=_t(1, 65536, 64), k=_t(9, 1024, 64), v=_t(9, 1024, 64)), "less than 65536 in all"),
+    (dict(cu_seqlens_q=_t(2 ** 16 + 2, dtype=INT)), r"at most 2\^16 sequences"),
     (dict(cu_seqlens_q=_t(0, dtype=INT)), "one entry more"),
     (dict(cu_seqlens_q=_t(3, dtype=torch.int64)), "cu_seqlens_q must be"),
     (dict(cu_seqlens_k=_t(2, dtype=INT)), "cu_seqlens_k must be"),
