@@ -17,6 +17,15 @@
 // its arrival tells the softmax that O may be touched too.
 //
 // TMEM: S (and P) of A and B, O of A and B, 128 columns each.
+//
+// What bounds it.  16384 tokens, causal, 32 heads of 128 over 8 key heads: 1.87 to
+// 2.06 ms, 1.07 to 1.18 PFLOP/s, where cuBLAS sustains 1.36 under the same power
+// limit (clocks near 1.45 GHz).  A step of both tiles takes 3000 clocks, 2048 of
+// them products: softmax 1750 (loads 90, the first half of the weights with the
+// maxima 1100, the other 600), then the rest of P V and Q K^T behind it.  Short
+// prompts: about 4 us of a CTA are its beginning and end (eight chunks of 512
+// tokens on average: 170 us, 3.7 CTAs to an SM).
+//
 // Two more warps look through the tiles of values that some row does not see
 // whole (attention_prompt.cuh), and clear what lies behind the sequence's end.
 #pragma once
