@@ -135,12 +135,12 @@ __device__ __forceinline__ uint32_t rest_f16(float lo, float hi, uint32_t rounde
   return pack_f16(lo - f.x, hi - f.y);
 }
 
-// Tokens of a sequence, within its row of the table.
-__device__ __forceinline__ int cached_length(const CachedParams& p, int b) {
-  const int n = __ldg(p.lengths + b);
+// Tokens of a sequence, within its row of the table, from the length read.
+__device__ __forceinline__ int cached_tokens(const CachedParams& p, int n) {
   const long long most = (long long)p.table_pages << p.c.page_shift;
   return n < 0 ? 0 : (long long)n > most ? (int)most : n;
 }
+__device__ __forceinline__ int cached_length(const CachedParams& p, int b) { return cached_tokens(p, __ldg(p.lengths + b)); }
 
 __device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) { return (cached_length(p, b) + kCachedTile - 1) / kCachedTile; }
 
@@ -805,15 +805,17 @@ __global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p) {
   __shared__ long long sum_of[2][8];
   __shared__ float4 acc[8][D / 4];
   __shared__ float2 ml[8];
-  griddep_wait();
-  griddep_launch_dependents();
+  // Whose parts these are goes by the lengths.  They are final once this kernel runs at all, since every CTA of the
+  // kernel before lets it start only after its own wait, so this is worked out ahead of the wait for the parts (one
+  // sequence of 1000 tokens 13.5 -> 11.0 us, 37 ragged ones 25.0 -> 22.8).  Read from L2, which the lengths' writer has
+  // reached: no wait of this kernel's has dropped what this SM's L1 may hold of them.
+  const auto tiles_of = [&](int i) { return (cached_tokens(p, __ldcg(p.lengths + i)) + kCachedTile - 1) / kCachedTile; };
   const int HC = p.c.heads * p.chunks, b = blockIdx.x / HC, hc = blockIdx.x - b * HC, h = blockIdx.y;
   int head0;
   const int heads = piece_heads(p, hc, head0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (h >= heads) return;
   long long all = 0, ahead = 0;
   for (int i = threadIdx.x; i < p.B; i += 256) {
-    const int n = cached_tiles(p, i);
+    const int n = tiles_of(i);
     all += n;
     if (i < b) ahead += n;
   }
@@ -826,15 +828,22 @@ __global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p) {
   __syncthreads();
   all = ahead = 0;
   for (int w = 0; w < 8; ++w) { all += sum_of[0][w]; ahead += sum_of[1][w]; }
-  const int n = cached_tiles(p, b);
+  const int n = tiles_of(b);
+  int c0 = 0, c1 = 0;
+  if (n > 0) {
+    const long long tiles = all * HC, first = ahead * HC + (long long)hc * n;
+    const int ctas = cached_ctas(tiles, p.ctas);
+    c0 = cached_cta(tiles, ctas, first);
+    c1 = cached_cta(tiles, ctas, first + n - 1);
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  if (h >= heads) return;
   if (n == 0) {
     if (threadIdx.x < D / 4) cached_store4(p, b, head0 + h, 4 * threadIdx.x, make_float4(0.f, 0.f, 0.f, 0.f));
     if (p.lse != nullptr && threadIdx.x == 0) p.lse[(long long)b * p.Hq + head0 + h] = -INFINITY;
     return;
   }
-  const long long tiles = all * HC, first = ahead * HC + (long long)hc * n;
-  const int ctas = cached_ctas(tiles, p.ctas);
-  const int c0 = cached_cta(tiles, ctas, first), c1 = cached_cta(tiles, ctas, first + n - 1);
   if (c0 == c1) return;
   float m = -INFINITY, l = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
