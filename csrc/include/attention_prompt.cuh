@@ -38,11 +38,33 @@ __device__ __forceinline__ int prompt_tiles(const PromptParams& p, int b, int to
   return (q1 - q0 + tokens - 1) / tokens;
 }
 
-// The tile `index` of all sequences' tiles of `tokens` tokens of q; false behind the last.  A whole warp calls it: every lane
-// counts an equal number of sequences, then the warp goes through those of the lane that has the tile.  Within a sequence the
-// last tile, which sees the most keys, comes first.
+// The tile `index` of all sequences' tiles of `tokens` tokens of q; false behind the last.  A whole warp calls it.  Within a
+// sequence the last tile, which sees the most keys, comes first.
+//
+// Up to 32 sequences, one to a lane, go by their number of keys, the longest first, so that no long tile begins when the
+// others are done.  More of them even that out by themselves and go in their order: every lane counts an equal number of
+// sequences, then the warp goes through those of the lane that has the tile.
 __device__ __forceinline__ bool prompt_tile(const PromptParams& p, int index, int tokens, PromptSeq& s, int& tile) {
   const int lane = threadIdx.x & 31;
+  if (p.B <= 32) {
+    PromptSeq mine{0, 0, 0, 0};
+    if (lane < p.B) mine = prompt_seq(p, lane);
+    const int tiles = (mine.nq + tokens - 1) / tokens;
+    int ahead = 0;
+    for (int b = 0; b < p.B; ++b) {
+      const int nk = __shfl_sync(0xffffffffu, mine.nk, b), n = __shfl_sync(0xffffffffu, tiles, b);
+      if (nk > mine.nk || (nk == mine.nk && b < lane)) ahead += n;
+    }
+    const uint32_t in = __ballot_sync(0xffffffffu, index >= ahead && index - ahead < tiles);
+    if (in == 0) return false;
+    const int at = __ffs(in) - 1;
+    s.q0 = __shfl_sync(0xffffffffu, mine.q0, at);
+    s.nq = __shfl_sync(0xffffffffu, mine.nq, at);
+    s.k0 = __shfl_sync(0xffffffffu, mine.k0, at);
+    s.nk = __shfl_sync(0xffffffffu, mine.nk, at);
+    tile = __shfl_sync(0xffffffffu, ahead + tiles - 1, at) - index;
+    return true;
+  }
   int first = 0, each = p.B, before = 0;
   while (true) {
     const int per = (each + 31) / 32, b0 = first + lane * per, b1 = min(b0 + per, first + each);
