@@ -22,9 +22,13 @@
 // 2.06 ms, 1.07 to 1.18 PFLOP/s, where cuBLAS sustains 1.36 under the same power
 // limit (clocks near 1.45 GHz).  A step of both tiles takes 3000 clocks, 2048 of
 // them products: softmax 1750 (loads 90, the first half of the weights with the
-// maxima 1100, the other 600), then the rest of P V and Q K^T behind it.  Short
-// prompts: about 4 us of a CTA are its beginning and end (eight chunks of 512
-// tokens on average: 170 us, 3.7 CTAs to an SM).
+// maxima 1100, the other 600), then the rest of P V and Q K^T behind it.
+//
+// A CTA that has loaded all of its pair of tiles takes over one that has not
+// begun yet (cluster launch control), and loads that while the last two steps and
+// the results of the first are worked on: beginnings and ends, about 4 us of every
+// pair, are hidden, and the last ones spread over the SMs as they become free.
+// Eight chunks of 512 tokens on average, 3.7 pairs to an SM: 161 -> 150 us.
 //
 // Two more warps look through the tiles of values that some row does not see
 // whole (attention_prompt.cuh), and clear what lies behind the sequence's end.
@@ -138,6 +142,40 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return r;
 }
 
+// Asks for a CTA of the grid that has not begun: this one will do its work.  The answer arrives at `at` (16 bytes), and on `bar`.
+__device__ __forceinline__ void ask_next_cta(void* at, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(at)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+
+// The answer: false where no CTA is left.
+__device__ __forceinline__ bool next_cta(const void* at, int& x, int& y) {
+  uint32_t some, cx, cy;
+  asm volatile(
+      "{\n\t.reg .b128 answer;\n\t.reg .pred some;\n\t.reg .b32 z, none;\n\t"
+      "ld.shared.b128 answer, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 some, answer;\n\t"
+      "selp.u32 %0, 1, 0, some;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "mov.u32 %2, 0;\n\t"
+      "@some clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, z, none}, answer;\n\t}"
+      : "=r"(some), "=r"(cx), "=r"(cy)
+      : "r"(smem_u32(at))
+      : "memory");
+  x = (int)cx;
+  y = (int)cy;
+  return some != 0;
+}
+
+// A pair of tiles: which rows, and how far over the keys.
+struct PromptItem {
+  PromptSeq s;
+  int token0, head, split;       // A's first token, of the sequence; the key head; which share of the keys
+  int tiles, steps;              // steps -1: there are no more
+  int first_fixed;               // tiles of values from here on, which some row does not see whole, go through two warps first
+};
+
 template <int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
 prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -148,25 +186,32 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   uint8_t* const sq = smem;                                   // tiles A and B
   uint8_t* const sk = smem + 2 * C::TILE;
   uint8_t* const sv = sk + C::STAGES * C::TILE;
-  __shared__ uint64_t q_full[2], k_full[C::STAGES], k_empty[C::STAGES], v_full[C::STAGES], v_empty[C::STAGES], v_raw[C::STAGES],
-      v_ready[C::STAGES], s_full[2], p_half[2], p_full[2], o_full[2], drained;
+  __shared__ uint64_t q_full[2], q_empty[2], k_full[C::STAGES], k_empty[C::STAGES], v_full[C::STAGES], v_empty[C::STAGES],
+      v_raw[C::STAGES], v_ready[C::STAGES], s_full[2], p_half[2], p_full[2], o_full[2], item_full[2], item_empty[2], answered, drained;
+  __shared__ __align__(16) uint4 answer;
+  __shared__ PromptItem items[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int odd[3][D], any_odd;
+  __shared__ int odd[2][3][D], any_odd[2];                    // of both items
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Nothing of this needs what the kernels before wrote.  TMEM has to be taken before the next kernel may start: one that took
   // it first would keep it until this CTA is done.
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); mbar_init(&s_full[i], 1);
+      mbar_init(&p_half[i], 4); mbar_init(&p_full[i], 4); mbar_init(&o_full[i], 1);
+      mbar_init(&item_full[i], 1); mbar_init(&item_empty[i], 11);     // 8 warps of softmax, the products, two for values
+      any_odd[i] = 0;
+    }
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); mbar_init(&v_raw[i], 1); mbar_init(&v_ready[i], 2);
     }
+    mbar_init(&answered, 1);
     mbar_init(&drained, 1);
     fence_mbarrier_init();
-    any_odd = 0;
     tma_prefetch_desc(&tq); tma_prefetch_desc(&tk); tma_prefetch_desc(&tv);
   }
-  for (int i = threadIdx.x; i < 3 * D; i += kPromptThreads) ((int*)odd)[i] = INT_MAX;
+  for (int i = threadIdx.x; i < 2 * 3 * D; i += kPromptThreads) ((int*)odd)[i] = INT_MAX;
   if (warp == 9) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
   __syncwarp();
   tc_fence_before_sync();
@@ -176,76 +221,125 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
   griddep_wait();
   griddep_launch_dependents();
   if (blockIdx.x + blockIdx.y == 0 && warp == 11) prompt_record(p);
-
   const int tokens = 128 / p.group;                           // of a tile
-  const int head = blockIdx.x % p.Hk;
-  PromptSeq s;
-  int pair;
-  const bool some = prompt_tile(p, blockIdx.x / p.Hk, 2 * tokens, s, pair);
-  if (!some) {
-    __syncthreads();
-    if (warp == 9) tmem_dealloc(tmem, 512);
-    return;
-  }
-  const int token0 = pair * 2 * tokens;                       // of the sequence, A's first
-  const int tiles = token0 + tokens < s.nq ? 2 : 1;
-  const int keys = prompt_visible(p, s, min(token0 + 2 * tokens, s.nq) - 1);
-  const int steps = prompt_share(p, blockIdx.y, (keys + kPromptKeys - 1) / kPromptKeys, kPromptKeys, s);
-  // Values of tiles from here on, which some row does not see whole, arrive on v_raw and go through two warps first.
-  const int first_fixed = min(prompt_visible(p, s, token0), s.nk) / kPromptKeys;
-  auto fixed_phase = [&](int i) { return (uint32_t)((i - first_fixed) / C::STAGES) & 1u; };   // of v_raw and v_ready
 
-  // 168 registers to a thread at launch: the warpgroups of the softmax, which hold a row of S, get 208, the other 88.
+  // Barriers are waited for by what went through them before: items n by turns through two places, all steps of all items by
+  // turns through the stages.  168 registers to a thread at launch: the warpgroups of the softmax, which hold a row of S, get
+  // 224, the other 56.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {
-      // -------------------------------------------------------------- loads
-      if (elect_one_sync()) {
-        bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
-        auto load_q = [&](int x) {
-          mbar_arrive_expect_tx(&q_full[x], C::HALVES * tokens * p.group * 128);
-          for (int h = 0; h < C::HALVES; ++h)
-            tma_load_3d(sq + x * C::TILE + h * 128 * 128, &tq, &q_full[x], 64 * h, head * p.group, s.q0 + token0 + x * tokens);
-        };
-        auto load = [&](uint8_t* at, const CUtensorMap* map, uint64_t* full, int i) {
-          mbar_arrive_expect_tx(full, C::TILE);
-          for (int h = 0; h < C::HALVES; ++h)
-            tma_load_3d(at + (i % C::STAGES) * C::TILE + h * 128 * 128, map, full, 64 * h, head, s.k0 + i * kPromptKeys);
-        };
-        auto load_k = [&](int i) {
-          if ((ok = wait(&k_empty[i % C::STAGES], ((i / C::STAGES) & 1) ^ 1u))) load(sk, &tk, &k_full[i % C::STAGES], i);
-        };
-        if (steps > 0) {
-          load_q(0);
-          load_k(0);
-          if (tiles == 2) load_q(1);
+      // -------------------------------------------------------------- items, and their loads
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
+      int n = 0, asked = 0, x = blockIdx.x, y = blockIdx.y, base = 0;
+      uint32_t q_phase = 0, k_phase = 0, raw_phase = 0, full_phase = 0;   // bits: of what comes next
+      auto load_q = [&](const PromptItem& it, int t) {
+        if (!(ok = wait(&q_empty[t], (q_phase >> t & 1) ^ 1u))) return;
+        q_phase ^= 1u << t;
+        mbar_arrive_expect_tx(&q_full[t], C::HALVES * tokens * p.group * 128);
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_3d(sq + t * C::TILE + h * 128 * 128, &tq, &q_full[t], 64 * h, it.head * p.group, it.s.q0 + it.token0 + t * tokens);
+      };
+      auto load = [&](const PromptItem& it, uint8_t* at, const CUtensorMap* map, uint64_t* full, int i) {
+        mbar_arrive_expect_tx(full, C::TILE);
+        for (int h = 0; h < C::HALVES; ++h)
+          tma_load_3d(at + ((base + i) % C::STAGES) * C::TILE + h * 128 * 128, map, full, 64 * h, it.head, it.s.k0 + i * kPromptKeys);
+      };
+      auto load_k = [&](const PromptItem& it, int i) {
+        const int stage = (base + i) % C::STAGES;
+        if (!(ok = wait(&k_empty[stage], (((base + i) / C::STAGES) & 1) ^ 1u))) return;
+        k_phase ^= 1u << stage;
+        load(it, sk, &tk, &k_full[stage], i);
+      };
+      auto publish = [&](const PromptItem& it) {
+        const int at = n & 1;
+        if (lane == 0) ok = wait(&item_empty[at], ((n >> 1) & 1) ^ 1u);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        __syncwarp();
+        if (!ok) return;
+        if (any_odd[at] != 0) {
+          for (int i = lane; i < 3 * D; i += 32) ((int*)odd[at])[i] = INT_MAX;
+          __syncwarp();
+          if (lane == 0) any_odd[at] = 0;
         }
-        int nk = steps > 0, nv = 0;
-        for (int i = 0; ok && i < steps; ++i) {
-          if (!(ok = wait(&v_empty[i % C::STAGES], ((i / C::STAGES) & 1) ^ 1u))) break;
-          load(sv, &tv, i < first_fixed ? &v_full[i % C::STAGES] : &v_raw[i % C::STAGES], i);
-          ++nv;
-          if (i + 1 < steps) {
-            load_k(i + 1);
-            nk += ok;
+        if (lane == 0) items[at] = it;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_full[at]);
+        ++n;
+      };
+      bool more = true;
+      int end = INT_MAX;                                      // no tile is there or behind it
+      while (ok && more) {
+        PromptItem it;
+        int pair;
+        const int index = x / p.Hk;
+        if (index < end && !prompt_tile(p, index, 2 * tokens, it.s, pair)) end = index;
+        if (index < end) {
+          it.head = x % p.Hk;
+          it.split = y;
+          it.token0 = pair * 2 * tokens;
+          it.tiles = it.token0 + tokens < it.s.nq ? 2 : 1;
+          const int keys = prompt_visible(p, it.s, min(it.token0 + 2 * tokens, it.s.nq) - 1);
+          it.steps = prompt_share(p, y, (keys + kPromptKeys - 1) / kPromptKeys, kPromptKeys, it.s);
+          it.first_fixed = min(prompt_visible(p, it.s, it.token0), it.s.nk) / kPromptKeys;
+          publish(it);
+          if (ok && it.steps > 0 && lane == 0) {
+            load_q(it, 0);
+            if (ok) load_k(it, 0);
+            if (ok && it.tiles == 2) load_q(it, 1);
+            for (int i = 0; ok && i < it.steps; ++i) {
+              const int stage = (base + i) % C::STAGES;
+              if (!(ok = wait(&v_empty[stage], (((base + i) / C::STAGES) & 1) ^ 1u))) break;
+              (i < it.first_fixed ? full_phase : raw_phase) ^= 1u << stage;
+              load(it, sv, &tv, i < it.first_fixed ? &v_full[stage] : &v_raw[stage], i);
+              if (i + 1 < it.steps) load_k(it, i + 1);
+            }
           }
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          base += max(it.steps, 0);
         }
-        // the copies land before the CTA leaves
-        for (int x = 0; x < tiles && steps > 0; ++x) wait(&q_full[x], 0);
-        for (int i = max(0, nk - C::STAGES); i < nk; ++i) wait(&k_full[i % C::STAGES], (i / C::STAGES) & 1);
-        for (int i = max(0, nv - C::STAGES); i < nv; ++i)
-          if (i < first_fixed) wait(&v_full[i % C::STAGES], (i / C::STAGES) & 1);
-          else wait(&v_raw[i % C::STAGES], fixed_phase(i));
+        // Asked for when the last two steps are to be done yet, not before: a CTA that is done earlier may take it.
+        if (ok) {
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&answered, 16);
+            ask_next_cta(&answer, &answered);
+            ok = wait(&answered, asked & 1);
+            if (ok) more = next_cta(&answer, x, y);
+            fence_proxy_async_smem();
+          }
+          ++asked;
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          more = __shfl_sync(0xffffffffu, more, 0);
+          x = __shfl_sync(0xffffffffu, x, 0);
+          y = __shfl_sync(0xffffffffu, y, 0);
+        }
+      }
+      if (ok) {
+        PromptItem none{};
+        none.steps = -1;
+        publish(none);
+      }
+      // the copies land before the CTA leaves
+      if (lane == 0) {
+        for (int i = 0; i < 2; ++i) wait(&q_full[i], (q_phase >> i & 1) ^ 1u);
+        for (int i = 0; i < C::STAGES; ++i) {
+          wait(&k_full[i], (k_phase >> i & 1) ^ 1u);
+          wait(&v_full[i], (full_phase >> i & 1) ^ 1u);
+          wait(&v_raw[i], (raw_phase >> i & 1) ^ 1u);
+        }
       }
     } else if (warp == 9) {
       // -------------------------------------------------------------- products
-      if (steps > 0 && elect_one_sync()) {
+      if (elect_one_sync()) {
         constexpr uint32_t iqk = umma_idesc(1u, 128, 128), ipv = umma_idesc(1u, 128, D) | (1u << 16);
         const uint64_t krow = umma_desc_k_sw128(0), vrow = umma_desc_mn_sw128(0, 128 * 128);
         auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
+        int base = 0, base_b = 0;                              // steps before, of A and of B
+        uint32_t q_phase = 0, ready_phase = 0, full_phase = 0;
         auto qk = [&](int x, int i) {
-          const uint64_t a = desc_at(krow, smem_u32(sq + x * C::TILE)), b = desc_at(krow, smem_u32(sk + (i % C::STAGES) * C::TILE));
+          const uint64_t a = desc_at(krow, smem_u32(sq + x * C::TILE)),
+                         b = desc_at(krow, smem_u32(sk + ((base + i) % C::STAGES) * C::TILE));
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t at = (k / 4) * (128 * 128 / 16) + (k % 4) * 2;
@@ -253,216 +347,257 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           }
           umma_commit(&s_full[x]);
         };
-        bool ok = wait(&k_full[0], 0);
-        for (int x = 0; ok && x < tiles; ++x)
-          if ((ok = wait(&q_full[x], 0))) { tc_fence_after_sync(); qk(x, 0); }
-        if (ok) umma_commit(&k_empty[0]);
-        for (int i = 0; ok && i < steps; ++i) {
-          const int stage = i % C::STAGES;
-          const uint32_t phase = (i / C::STAGES) & 1;
-          for (int x = 0; ok && x < tiles; ++x) {
-            if (x == 0) {
-              if (!(ok = i < first_fixed ? wait(&v_full[stage], phase) : wait(&v_ready[stage], fixed_phase(i)))) break;
-            }
-            const uint64_t b = desc_at(vrow, smem_u32(sv + stage * C::TILE));
-            for (int h = 0; ok && h < 2; ++h) {              // the first half of P's columns, then the other
-              if (!(ok = wait(h ? &p_full[x] : &p_half[x], i & 1))) break;
-              tc_fence_after_sync();
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+          if (!(ok = wait(&item_full[n & 1], (n >> 1) & 1))) break;
+          const int tiles = items[n & 1].tiles, steps = items[n & 1].steps, first_fixed = items[n & 1].first_fixed;
+          if (steps < 0) break;
+          for (int i = -1; ok && i < steps && steps > 0; ++i) {  // P V of step i, then Q K^T of the next
+            const int stage = (base + i) % C::STAGES, next = (base + i + 1) % C::STAGES;
+            for (int x = 0; ok && x < tiles; ++x) {
+              if (i >= 0) {
+                if (x == 0) {
+                  uint32_t& phase = i < first_fixed ? full_phase : ready_phase;
+                  if (!(ok = wait(i < first_fixed ? &v_full[stage] : &v_ready[stage], phase >> stage & 1))) break;
+                  phase ^= 1u << stage;
+                }
+                const uint64_t b = desc_at(vrow, smem_u32(sv + stage * C::TILE));
+                for (int h = 0; ok && h < 2; ++h) {            // the first half of P's columns, then the other
+                  if (!(ok = wait(h ? &p_full[x] : &p_half[x], ((x ? base_b : base) + i) & 1))) break;
+                  tc_fence_after_sync();
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 32 * h + 8 * k, b + (4 * h + k) * (16 * 128 / 16), ipv, i > 0 || h > 0 || k > 0);
-            }
-            if (!ok) break;
-            if (x + 1 == tiles) umma_commit(&v_empty[stage]);
-            if (i + 1 == steps) {
-              umma_commit(&o_full[x]);
-              continue;
-            }
-            if (x == 0) {
-              if (!(ok = wait(&k_full[(i + 1) % C::STAGES], ((i + 1) / C::STAGES) & 1))) break;
+                  for (int k = 0; k < 4; ++k)
+                    umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 32 * h + 8 * k, b + (4 * h + k) * (16 * 128 / 16), ipv,
+                                i > 0 || h > 0 || k > 0);
+                }
+                if (!ok) break;
+                if (x + 1 == tiles) umma_commit(&v_empty[stage]);
+                if (i + 1 == steps) {
+                  umma_commit(&o_full[x]);
+                  continue;
+                }
+              } else {
+                if (!(ok = wait(&q_full[x], q_phase >> x & 1))) break;
+                q_phase ^= 1u << x;
+              }
+              if (x == 0 && !(ok = wait(&k_full[next], ((base + i + 1) / C::STAGES) & 1))) break;
               tc_fence_after_sync();
+              qk(x, i + 1);
+              if (i + 2 == steps) umma_commit(&q_empty[x]);
+              if (x + 1 == tiles) umma_commit(&k_empty[next]);
             }
-            qk(x, i + 1);
-            if (x + 1 == tiles) umma_commit(&k_empty[(i + 1) % C::STAGES]);
           }
+          base += steps;
+          if (tiles == 2) base_b += steps;
+          mbar_arrive(&item_empty[n & 1]);
         }
         umma_commit(&drained);
         wait(&drained, 0);
       }
     } else {
       // -------------------------------------------------------------- values of tiles that some row does not see whole
-      for (int i = first_fixed; i < steps; ++i) {
-        const int stage = i % C::STAGES;
-        if (!mbar_wait_warp(&v_raw[stage], fixed_phase(i), p.status, kPromptKernelId, kPromptWaitNs)) break;
-        uint4* const at = (uint4*)(sv + stage * C::TILE);
+      int base = 0;
+      uint32_t raw_phase = 0;
+      bool ok = true;
+      for (int n = 0; ok; ++n) {
+        if (!(ok = mbar_wait_warp(&item_full[n & 1], (n >> 1) & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+        const int k_end = items[n & 1].s.nk, steps = items[n & 1].steps;
+        if (steps < 0) break;
+        for (int i = items[n & 1].first_fixed; i < steps; ++i) {
+          const int stage = (base + i) % C::STAGES;
+          if (!(ok = mbar_wait_warp(&v_raw[stage], raw_phase >> stage & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+          raw_phase ^= 1u << stage;
+          uint4* const at = (uint4*)(sv + stage * C::TILE);
 #pragma unroll 4
-        for (int c = (warp - 10) * 32 + lane; c < C::TILE / 16; c += 64) {
-          const int half = c / 1024, row = (c / 8) % 128;
-          const int key = i * kPromptKeys + row;
-          if (key >= s.nk) {
-            at[c] = make_uint4(0, 0, 0, 0);
-            continue;
-          }
-          uint4 v = at[c];
-          auto bad = [](uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; };   // an exponent of ones
-          if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
-            uint32_t w[4] = {v.x, v.y, v.z, v.w};
-            const int d = 64 * half + 8 * ((c & 7) ^ (row & 7));    // the swizzle's order of 16-byte pieces
-            for (int e = 0; e < 8; ++e) {
-              const float f = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-              if (fabsf(f) < INFINITY) continue;
-              atomicMin(&odd[odd_kind(f)][d + e], key);
-              w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+          for (int c = (warp - 10) * 32 + lane; c < C::TILE / 16; c += 64) {
+            const int half = c / 1024, row = (c / 8) % 128;
+            const int key = i * kPromptKeys + row;
+            if (key >= k_end) {
+              at[c] = make_uint4(0, 0, 0, 0);
+              continue;
             }
-            any_odd = 1;
-            at[c] = make_uint4(w[0], w[1], w[2], w[3]);
+            uint4 v = at[c];
+            auto bad = [](uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; };   // an exponent of ones
+            if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
+              uint32_t w[4] = {v.x, v.y, v.z, v.w};
+              const int d = 64 * half + 8 * ((c & 7) ^ (row & 7));    // the swizzle's order of 16-byte pieces
+              for (int e = 0; e < 8; ++e) {
+                const float f = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+                if (fabsf(f) < INFINITY) continue;
+                atomicMin(&odd[n & 1][odd_kind(f)][d + e], key);
+                w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
+              }
+              any_odd[n & 1] = 1;
+              at[c] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_ready[stage]);
         }
-        fence_proxy_async_smem();
+        base += steps;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_ready[stage]);
+        if (lane == 0) mbar_arrive(&item_empty[n & 1]);
       }
     }
   } else {
     // ---------------------------------------------------------------- softmax, one row to a thread
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int x = warp >> 2, row = threadIdx.x & 127;
-    const int token = token0 + x * tokens + row / p.group, hq = head * p.group + row % p.group;
-    const bool mine = row < tokens * p.group && token < s.nq;
-    const int visible = mine ? min(prompt_visible(p, s, token), s.nk) : 0;
-    const int all = __reduce_min_sync(0xffffffffu, mine ? visible : INT_MAX);   // keys that the warp's rows all see
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + 128 * x, to = tmem + lanes + 256 + 128 * x;
     // logits are turned positive multiples of S: a scale that is not positive goes into S itself
     float mult = p.scale * 1.44269504088896341f;
-    const float turn = mult > 0.f ? 1.f : mult < 0.f ? -1.f : 0.f;
-    mult = turn == 0.f ? 1.f : fabsf(mult);
-    float m = -INFINITY, l = 0.f;
-    bool ok = x < tiles;
-    for (int i = 0; ok && i < steps; ++i) {
-      if (!(ok = mbar_wait_warp(&s_full[x], i & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
-      tc_fence_after_sync();
-      uint32_t r[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
-      tmem_ld_wait();
-      if (turn != 1.f) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * turn);
-      }
-      const int k0 = i * kPromptKeys;
-      if (k0 + kPromptKeys > all) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (k0 + c >= visible) r[c] = __float_as_uint(-INFINITY);
-      }
-      // Weights are exp2(c S - m) for any m that lets them neither overflow nor vanish: bf16 and fp32 hold 2^64 as exactly as
-      // 1.  So m follows the maximum only when that is 2^64 past it (and in the first tile), and the first half of the weights
-      // is worked out before it is known whether it is.  The product begins with that half.  (A quarter of the exponentials
-      // by a polynomial, to spare the special-function unit: no difference, 16384 tokens run into the power limit.)
-      uint64_t sum[2];
-      uint32_t w[32];
-      auto half = [&](int h, float base) {
-        const uint64_t mult2 = pair_f32(mult, mult), base2 = pair_f32(base, base);
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          float a, b;
-          unpair_f32(fma2(pair_f32(__uint_as_float(r[64 * h + 2 * c]), __uint_as_float(r[64 * h + 2 * c + 1])), mult2, base2), a, b);
-          a = prompt_exp2(a);
-          b = prompt_exp2(b);
-          sum[c & 1] = add2(sum[c & 1], pair_f32(a, b));
-          w[c] = pack_bf16(a, b);
+    mult = mult == 0.f ? 1.f : fabsf(mult);
+    bool ok = true;
+    uint32_t s_phase = 0, o_phase = 0;
+    for (int n = 0; ok; ++n) {
+      if (!(ok = mbar_wait_warp(&item_full[n & 1], (n >> 1) & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+      const int steps = items[n & 1].steps;
+      if (steps < 0) break;
+      if (x < items[n & 1].tiles) {
+        int visible = 0;
+        bool mine;
+        {
+          const PromptSeq s = items[n & 1].s;
+          const int token = items[n & 1].token0 + x * tokens + row / p.group;
+          mine = row < tokens * p.group && token < s.nq;
+          if (mine) visible = min(prompt_visible(p, s, token), s.nk);
         }
-      };
-      auto store = [&](int h) {
-        tmem_st32(ts + 32 * h, w);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(h ? &p_full[x] : &p_half[x]);
-      };
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      bool again;
+        const int all = __reduce_min_sync(0xffffffffu, mine ? visible : INT_MAX);   // keys that the warp's rows all see
+        float m = -INFINITY, l = 0.f;
+        for (int i = 0; ok && i < steps; ++i) {
+          if (!(ok = mbar_wait_warp(&s_full[x], s_phase, p.status, kPromptKernelId, kPromptWaitNs))) break;
+          s_phase ^= 1u;
+          tc_fence_after_sync();
+          uint32_t r[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
+          tmem_ld_wait();
+          if (!(p.scale > 0.f)) {
+            const float turn = p.scale < 0.f ? -1.f : 0.f;
+
+#pragma unroll
+            for (int c = 0; c < 128; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * turn);
+          }
+          const int k0 = i * kPromptKeys;
+          if (k0 + kPromptKeys > all) {
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (k0 + c >= visible) r[c] = __float_as_uint(-INFINITY);
+          }
+          // Weights are exp2(c S - m) for any m that lets them neither overflow nor vanish: bf16 and fp32 hold 2^64 as exactly as
+          // 1.  So m follows the maximum only when that is 2^64 past it (and in the first tile), and the first half of the weights
+          // is worked out before it is known whether it is.  The product begins with that half.  (A quarter of the exponentials
+          // by a polynomial, to spare the special-function unit: no difference, 16384 tokens run into the power limit.)
+          uint64_t sum[2];
+          uint32_t w[32];
+          auto half = [&](int h, float base) {
+            const uint64_t mult2 = pair_f32(mult, mult), base2 = pair_f32(base, base);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              float a, b;
+              unpair_f32(fma2(pair_f32(__uint_as_float(r[64 * h + 2 * c]), __uint_as_float(r[64 * h + 2 * c + 1])), mult2, base2), a, b);
+              a = prompt_exp2(a);
+              b = prompt_exp2(b);
+              sum[c & 1] = add2(sum[c & 1], pair_f32(a, b));
+              w[c] = pack_bf16(a, b);
+            }
+          };
+          auto store = [&](int h) {
+            tmem_st32(ts + 32 * h, w);
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(h ? &p_full[x] : &p_half[x]);
+          };
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          bool again;
 #pragma unroll 1
-      do {
-        sum[0] = sum[1] = 0;
-        half(0, m == -INFINITY ? 0.f : -m);
+          do {
+            sum[0] = sum[1] = 0;
+            half(0, m == -INFINITY ? 0.f : -m);
 #pragma unroll
-        for (int c = 0; c < 128; c += 8)
+            for (int c = 0; c < 128; c += 8)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
-        const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
-        const bool grow = peak > m + 64.f;
-        again = __any_sync(0xffffffffu, grow);
-        if (again) {
-          const float now = grow ? peak : m;
-          const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
-          m = now;
-          l *= shrink;
-          if (i > 0) {
+              for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
+            const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
+            const bool grow = peak > m + 64.f;
+            again = __any_sync(0xffffffffu, grow);
+            if (again) {
+              const float now = grow ? peak : m;
+              const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
+              m = now;
+              l *= shrink;
+              if (i > 0) {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld32(to + c, o);
+                  tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(to + c, o);
-              tmem_ld_wait();
+                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+                  tmem_st32(to + c, o);
+                }
+              }
+            }
+          } while (again);
+          store(0);
+          half(1, m == -INFINITY ? 0.f : -m);
+          store(1);
+          float s0, s1;
+          unpair_f32(add2(sum[0], sum[1]), s0, s1);
+          l += s0 + s1;
+        }
+        if (ok && steps > 0) {
+          ok = mbar_wait_warp(&o_full[x], o_phase, p.status, kPromptKernelId, kPromptWaitNs);
+          o_phase ^= 1u;
+          tc_fence_after_sync();
+        }
+        const volatile PromptItem& it = items[n & 1];             // not kept over the steps: S takes the registers
+        const int token = it.token0 + x * tokens + row / p.group, hq = it.head * p.group + row % p.group;
+        // a row that sees keys has a sum, unless all its logits are -inf
+        if (l == 0.f && visible > 0 && steps > 0) l = NAN;
+        const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const bool put_back = any_odd[n & 1] != 0;
+        const long long at = (long long)(it.s.q0 + token) * p.o_token + (long long)hq * p.o_head;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          if (steps > 0) {
+            tmem_ld32(to + c, o);
+            tmem_ld_wait();
+          }
+          float v[32];
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-              tmem_st32(to + c, o);
+          for (int e = 0; e < 32; ++e) v[e] = steps > 0 && visible > 0 ? __uint_as_float(o[e]) * inv : 0.f;
+          if (put_back) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = put_back_odd<D>(odd[n & 1], c + e, visible, v[e]);
+          }
+          if (mine && p.splits > 1) {
+            float4* const dst = (float4*)(p.parts + (((long long)it.split * p.Nq + it.s.q0 + token) * p.Hq + hq) * D + c);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) dst[e / 4] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          } else if (mine) {
+            __nv_bfloat16* const dst = (__nv_bfloat16*)p.out + at + c;
+            if (p.o_vec) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                *(uint4*)(dst + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]), pack_bf16(v[e + 4], v[e + 5]),
+                                                pack_bf16(v[e + 6], v[e + 7]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) dst[e] = __float2bfloat16_rn(v[e]);
             }
           }
+          __syncwarp();
         }
-      } while (again);
-      store(0);
-      half(1, m == -INFINITY ? 0.f : -m);
-      store(1);
-      float s0, s1;
-      unpair_f32(add2(sum[0], sum[1]), s0, s1);
-      l += s0 + s1;
-    }
-    if (x < tiles) {
-      if (ok && steps > 0) {
-        ok = mbar_wait_warp(&o_full[x], 0, p.status, kPromptKernelId, kPromptWaitNs);
-        tc_fence_after_sync();
+        if (mine && p.splits > 1) p.stats[((long long)it.split * p.Nq + it.s.q0 + token) * p.Hq + hq] = make_float2(m, l);
+        else if (mine && p.lse != nullptr) p.lse[(long long)(it.s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
       }
-      // a row that sees keys has a sum, unless all its logits are -inf
-      if (l == 0.f && visible > 0 && steps > 0) l = NAN;
-      const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      const bool put_back = any_odd != 0;
-      const long long at = (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head;
-#pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        if (steps > 0) {
-          tmem_ld32(to + c, o);
-          tmem_ld_wait();
-        }
-        float v[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = steps > 0 && visible > 0 ? __uint_as_float(o[e]) * inv : 0.f;
-        if (put_back) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = put_back_odd<D>(odd, c + e, visible, v[e]);
-        }
-        if (mine && p.splits > 1) {
-          float4* const dst = (float4*)(p.parts + (((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq) * D + c);
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) dst[e / 4] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-        } else if (mine) {
-          __nv_bfloat16* const dst = (__nv_bfloat16*)p.out + at + c;
-          if (p.o_vec) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              *(uint4*)(dst + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]), pack_bf16(v[e + 4], v[e + 5]),
-                                              pack_bf16(v[e + 6], v[e + 7]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) dst[e] = __float2bfloat16_rn(v[e]);
-          }
-        }
-        __syncwarp();
-      }
-      if (mine && p.splits > 1) p.stats[((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq] = make_float2(m, l);
-      else if (mine && p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[n & 1]);
     }
   }
   __syncwarp();
