@@ -30,15 +30,15 @@
 
 namespace raiccl {
 
-constexpr int kFp32Threads = 256;   // the softmax's four warps; loads, products, two warps for the values
+constexpr int kFp32Threads = 384;   // two warpgroups of softmax; loads, products, two warps for the values
 
 template <int D>
 struct PromptFp32 {
   static constexpr int KT = D == 64 ? 128 : 64;               // keys of a step
   static constexpr int HALVES = D / 64;
   static constexpr int Q_PART = 128 * D * 2, KV_PART = KT * D * 2;
-  static constexpr int KSTAGES = D == 64 ? 2 : 1;             // of keys; values have one
-  static constexpr int SMEM = 1024 + 3 * (Q_PART + (KSTAGES + 1) * KV_PART);
+  static constexpr int SLOTS = D == 64 ? 10 : 7;              // of one part of a step's keys or values each
+  static constexpr int SMEM = 1024 + 3 * Q_PART + SLOTS * KV_PART;
   static constexpr uint32_t P_AT = 2 * KT, O_AT = D == 64 ? 448 : 256;   // columns of TMEM behind the two of S
 };
 
@@ -47,6 +47,14 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* desc, ui
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
       "l"(desc), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 
@@ -107,26 +115,27 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* const sq = smem;
-  uint8_t* const sk = smem + 3 * C::Q_PART;
-  uint8_t* const sv = sk + C::KSTAGES * 3 * C::KV_PART;
-  __shared__ uint64_t q_full, k_full[C::KSTAGES], k_empty[C::KSTAGES], v_raw, v_ready, v_empty, s_full[2], p_full, o_full, drained;
+  uint8_t* const ring = smem + 3 * C::Q_PART;
+  __shared__ uint64_t q_full, full[C::SLOTS], empty[C::SLOTS], v_ready[2], s_full[2], p_full, o_full, met[4], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int odd[3][D], any_odd;
+  __shared__ float told[2][2][128];                           // by turns, from each half of a row to the other
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Nothing of this needs what the kernels before wrote.  TMEM has to be taken before the next kernel may start: one that took
   // it first would keep it until this CTA is done.
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 1);
-    for (int i = 0; i < C::KSTAGES; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
-    mbar_init(&v_raw, 1); mbar_init(&v_ready, 2); mbar_init(&v_empty, 1);
+    for (int i = 0; i < C::SLOTS; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    mbar_init(&v_ready[0], 2); mbar_init(&v_ready[1], 2);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
-    mbar_init(&p_full, 4); mbar_init(&o_full, 1); mbar_init(&drained, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&met[i], 2);
+    mbar_init(&p_full, 8); mbar_init(&o_full, 1); mbar_init(&drained, 1);
     fence_mbarrier_init();
     any_odd = 0;
     tma_prefetch_desc(&tq); tma_prefetch_desc(&tk); tma_prefetch_desc(&tv);
   }
   for (int i = threadIdx.x; i < 3 * D; i += kFp32Threads) ((int*)odd)[i] = INT_MAX;
-  if (warp == 5) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+  if (warp == 9) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
   __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
@@ -134,7 +143,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   const uint32_t tmem = tmem_slot;
   griddep_wait();
   griddep_launch_dependents();
-  if (blockIdx.x + blockIdx.y == 0 && warp == 7) prompt_record(p);
+  if (blockIdx.x + blockIdx.y == 0 && warp == 11) prompt_record(p);
 
   const int tokens = 128 / p.group;
   const int head = blockIdx.x % p.Hk;
@@ -143,7 +152,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   const bool some = prompt_tile(p, blockIdx.x / p.Hk, tokens, s, tile);
   if (!some) {
     __syncthreads();
-    if (warp == 5) tmem_dealloc(tmem, 512);
+    if (warp == 9) tmem_dealloc(tmem, 512);
     return;
   }
   const int token0 = tile * tokens;
@@ -152,97 +161,105 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
 
   auto wait = [&](uint64_t* bar, uint32_t parity) { return serving_wait(bar, parity, p.status, kPromptKernelId, kPromptWaitNs); };
 
-  if (warp == 4) {
+  // Parts go through the ring in the order of their products: K(0), K(1), V(0), K(2), V(1), ..., of each the last part first.
+  auto k_at = [&](int i) { return i == 0 ? 0 : 6 * i - 3; };
+  auto v_at = [&](int i) { return 6 * i + (i + 1 < steps ? 6 : 3); };
+
+  if (warp == 8) {
     // ---------------------------------------------------------------- loads
     if (steps > 0 && elect_one_sync()) {
       mbar_arrive_expect_tx(&q_full, 3 * C::HALVES * tokens * p.group * 128);
       for (int part = 0; part < 3; ++part)
         for (int h = 0; h < C::HALVES; ++h)
           tma_load_4d(sq + part * C::Q_PART + h * 128 * 128, &tq, &q_full, 64 * h, head * p.group, s.q0 + token0, part);
-      auto load = [&](uint8_t* at, const CUtensorMap* map, uint64_t* full, int i) {
-        mbar_arrive_expect_tx(full, 3 * C::KV_PART);
-        for (int part = 0; part < 3; ++part)
-          for (int h = 0; h < C::HALVES; ++h)
-            tma_load_4d(at + part * C::KV_PART + h * KT * 128, map, full, 64 * h, head, s.k0 + i * KT, part);
-      };
-      int nk = 0, nv = 0;
+      int n = 0;
       bool ok = true;
-      auto load_k = [&] {
-        const int st = nk % C::KSTAGES;
-        if (!(ok = wait(&k_empty[st], ((nk / C::KSTAGES) & 1) ^ 1u))) return;
-        load(sk + st * 3 * C::KV_PART, &tk, &k_full[st], nk);
-        ++nk;
+      auto load = [&](const CUtensorMap* map, int i) {
+        for (int part = 2; ok && part >= 0; --part) {
+          const int slot = n % C::SLOTS;
+          if (!(ok = wait(&empty[slot], ((n / C::SLOTS) & 1) ^ 1u))) return;
+          mbar_arrive_expect_tx(&full[slot], C::KV_PART);
+          for (int h = 0; h < C::HALVES; ++h)
+            tma_load_4d(ring + slot * C::KV_PART + h * KT * 128, map, &full[slot], 64 * h, head, s.k0 + i * KT, part);
+          ++n;
+        }
       };
-      load_k();
+      load(&tk, 0);
       for (int i = 0; ok && i < steps; ++i) {
-        if (C::KSTAGES == 2 && nk < steps) load_k();
-        if (!ok || !(ok = wait(&v_empty, (i & 1) ^ 1u))) break;
-        load(sv, &tv, &v_raw, i);
-        ++nv;
-        if (C::KSTAGES == 1 && nk < steps) load_k();
+        if (i + 1 < steps) load(&tk, i + 1);
+        if (ok) load(&tv, i);
       }
       // the copies land before the CTA leaves
       wait(&q_full, 0);
-      for (int i = max(0, nk - C::KSTAGES); i < nk; ++i) wait(&k_full[i % C::KSTAGES], (i / C::KSTAGES) & 1);
-      if (nv > 0) wait(&v_raw, (nv - 1) & 1);
+      for (int i = max(0, n - C::SLOTS); i < n; ++i) wait(&full[i % C::SLOTS], (i / C::SLOTS) & 1);
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ---------------------------------------------------------------- products
     if (steps > 0 && elect_one_sync()) {
       constexpr uint32_t iqk = umma_idesc(1u, 128, KT), ipv = umma_idesc(1u, 128, D) | (1u << 16);
-      constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};   // parts, the small products first
       const uint64_t krow = umma_desc_k_sw128(0), vrow = umma_desc_mn_sw128(0, KT * 128);
+      bool ok = wait(&q_full, 0);
+      // The parts b of keys or values come in the order 2, 1, 0, and with them the parts a + b <= 2 of q or P: the largest
+      // product is the last, and a part's place is free after its own products.
       auto qk = [&](int i) {
-        const uint64_t a = desc_at(krow, smem_u32(sq)), b = desc_at(krow, smem_u32(sk + (i % C::KSTAGES) * 3 * C::KV_PART));
 #pragma unroll
-        for (int j = 0; j < 6; ++j)
+        for (int j = 0; j < 3; ++j) {
+          const int n = k_at(i) + j, slot = n % C::SLOTS;
+          if (!(ok = ok && wait(&full[slot], (n / C::SLOTS) & 1))) return;
+          tc_fence_after_sync();
+          const uint64_t a = desc_at(krow, smem_u32(sq)), b = desc_at(krow, smem_u32(ring + slot * C::KV_PART));
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_f16(tmem + KT * (i & 1), a + (A[j] * C::Q_PART + (k / 4) * 128 * 128) / 16 + (k % 4) * 2,
-                     b + (B[j] * C::KV_PART + (k / 4) * KT * 128) / 16 + (k % 4) * 2, iqk, j > 0 || k > 0);
+          for (int part = j; part >= 0; --part)
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_f16(tmem + KT * (i & 1), a + (part * C::Q_PART + (k / 4) * 128 * 128) / 16 + (k % 4) * 2,
+                       b + ((k / 4) * KT * 128) / 16 + (k % 4) * 2, iqk, j > 0 || k > 0);
+          umma_commit(&empty[slot]);
+        }
         umma_commit(&s_full[i & 1]);
-        umma_commit(&k_empty[i % C::KSTAGES]);
       };
-      bool ok = wait(&q_full, 0) && wait(&k_full[0], 0);
-      if (ok) {
-        tc_fence_after_sync();
-        qk(0);
-      }
+      qk(0);
       for (int i = 0; ok && i < steps; ++i) {
         // S of the step after this one goes where the one before was, which was read before its P came
-        if (i + 1 < steps) {
-          if (!(ok = wait(&k_full[(i + 1) % C::KSTAGES], ((i + 1) / C::KSTAGES) & 1))) break;
-          tc_fence_after_sync();
-          qk(i + 1);
-        }
-        if (!(ok = wait(&v_ready, i & 1) && wait(&p_full, i & 1))) break;
+        if (i + 1 < steps) qk(i + 1);
+        if (!(ok = ok && wait(&v_ready[i & 1], (i >> 1) & 1) && wait(&p_full, i & 1))) break;
         tc_fence_after_sync();
-        const uint64_t b = desc_at(vrow, smem_u32(sv));
 #pragma unroll
-        for (int j = 0; j < 6; ++j)
+        for (int j = 0; j < 3; ++j) {
+          const int slot = (v_at(i) + j) % C::SLOTS;
+          const uint64_t b = desc_at(vrow, smem_u32(ring + slot * C::KV_PART));
 #pragma unroll
-          for (int k = 0; k < KT / 16; ++k)
-            umma_f16_ts(tmem + C::O_AT, tmem + C::P_AT + A[j] * (KT / 2) + 8 * k, b + (B[j] * C::KV_PART + k * 16 * 128) / 16, ipv, j > 0 || k > 0);
-        umma_commit(&v_empty);
+          for (int part = j; part >= 0; --part)
+#pragma unroll
+            for (int k = 0; k < KT / 16; ++k)
+              umma_f16_ts(tmem + C::O_AT, tmem + C::P_AT + part * (KT / 2) + 8 * k, b + (k * 16 * 128) / 16, ipv, j > 0 || k > 0);
+          umma_commit(&empty[slot]);
+        }
         umma_commit(&o_full);
       }
       umma_commit(&drained);
       wait(&drained, 0);
     }
-  } else if (warp >= 6) {
+  } else if (warp >= 10) {
     // ---------------------------------------------------------------- values
     for (int i = 0; i < steps; ++i) {
-      if (!mbar_wait_warp(&v_raw, i & 1, p.status, kPromptKernelId, kPromptWaitNs)) break;
-      uint4* const at = (uint4*)sv;
+      uint4* at[3];                // the parts
+      bool ok = true;
+      for (int part = 2; ok && part >= 0; --part) {
+        const int n = v_at(i) + 2 - part, slot = n % C::SLOTS;
+        ok = mbar_wait_warp(&full[slot], (n / C::SLOTS) & 1, p.status, kPromptKernelId, kPromptWaitNs);
+        at[part] = (uint4*)(ring + slot * C::KV_PART);
+      }
+      if (!ok) break;
 #pragma unroll 4
-      for (int c = (warp - 6) * 32 + lane; c < C::KV_PART / 16; c += 64) {
+      for (int c = (warp - 10) * 32 + lane; c < C::KV_PART / 16; c += 64) {
         const int half = c / (KT * 8), row = (c / 8) % KT, key = i * KT + row;
         if (key >= s.nk) {           // behind the sequence's end
 #pragma unroll
-          for (int part = 0; part < 3; ++part) at[part * (C::KV_PART / 16) + c] = make_uint4(0, 0, 0, 0);
+          for (int part = 0; part < 3; ++part) at[part][c] = make_uint4(0, 0, 0, 0);
           continue;
         }
-        const uint4 v = at[c];       // the first part: what is not finite is there
+        const uint4 v = at[0][c];    // the first part: what is not finite is there
         auto bad = [](uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; };
         if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
           uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -254,34 +271,44 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
           }
           any_odd = 1;
-          at[c] = make_uint4(w[0], w[1], w[2], w[3]);
+          at[0][c] = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&v_ready);
+      if (lane == 0) mbar_arrive(&v_ready[i & 1]);
     }
   } else {
-    // ---------------------------------------------------------------- softmax, one row to a thread
-    const int row = threadIdx.x, token = token0 + row / p.group, hq = head * p.group + row % p.group;
+    // ---------------------------------------------------------------- softmax, half a row to a thread
+    constexpr int KH = KT / 2, DH = D / 2;                      // keys and dimensions of one half
+    const int half = warp >> 2, row = threadIdx.x & 127, token = token0 + row / p.group, hq = head * p.group + row % p.group;
     const bool mine = row < tokens * p.group && token < s.nq;
     const int visible = mine ? min(prompt_visible(p, s, token), s.nk) : 0;
     const int all = __reduce_min_sync(0xffffffffu, mine ? visible : INT_MAX);
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float mult = p.scale * 1.44269504088896341f;
     const float turn = mult > 0.f ? 1.f : mult < 0.f ? -1.f : 0.f;
     mult = turn == 0.f ? 1.f : fabsf(mult);
-    float m = -INFINITY, l = 0.f, o[D];
+    float m = -INFINITY, l = 0.f, o[DH];
 #pragma unroll
-    for (int d = 0; d < D; ++d) o[d] = 0.f;
+    for (int d = 0; d < DH; ++d) o[d] = 0.f;
+    // The other half's number of the same row; the place is written again two turns on, when both have met once more.
+    auto exchange = [&](int turn_of, float v, float& other) {
+      told[turn_of & 1][half][row] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&met[warp & 3]);
+      if (!mbar_wait_warp(&met[warp & 3], turn_of & 1, p.status, kPromptKernelId, kPromptWaitNs)) return false;
+      other = told[turn_of & 1][half ^ 1][row];
+      return true;
+    };
     // the sums of step i, once its products are done
     auto add = [&](int i) {
       if (!mbar_wait_warp(&o_full, i & 1, p.status, kPromptKernelId, kPromptWaitNs)) return false;
       tc_fence_after_sync();
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c = 0; c < DH; c += 32) {
         uint32_t r[32];
-        tmem_ld32(lanes + C::O_AT + c, r);
+        tmem_ld32(lanes + C::O_AT + half * DH + c, r);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[c + e] += __uint_as_float(r[e]);
@@ -293,26 +320,28 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     for (int i = 0; i < steps; ++i) {
       if (!(ok = mbar_wait_warp(&s_full[i & 1], (i >> 1) & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
       tc_fence_after_sync();
-      uint32_t r[KT];
+      uint32_t r[KH];
 #pragma unroll
-      for (int c = 0; c < KT; c += 32) tmem_ld32(lanes + KT * (i & 1) + c, r + c);
+      for (int c = 0; c < KH; c += 32) tmem_ld32(lanes + KT * (i & 1) + half * KH + c, r + c);
       tmem_ld_wait();
       if (turn != 1.f) {
 #pragma unroll
-        for (int c = 0; c < KT; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * turn);
+        for (int c = 0; c < KH; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * turn);
       }
-      const int k0 = i * KT;
-      if (k0 + KT > all) {
+      const int k0 = i * KT + half * KH;
+      if (k0 + KH > all) {
 #pragma unroll
-        for (int c = 0; c < KT; ++c)
+        for (int c = 0; c < KH; ++c)
           if (k0 + c >= visible) r[c] = __float_as_uint(-INFINITY);
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < KT; c += 8)
+      for (int c = 0; c < KH; c += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
-      const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
+      float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), other;
+      if (!(ok = exchange(i, peak, other))) break;
+      peak = fmaxf(peak, other) * mult;
       if (i > 0 && !(ok = add(i - 1))) break;    // before P is written where its operand was
       const bool grow = peak > m + 8.f;
       if (__any_sync(0xffffffffu, grow)) {
@@ -321,16 +350,16 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
         m = now;
         l *= shrink;
 #pragma unroll
-        for (int d = 0; d < D; ++d) o[d] *= shrink;
+        for (int d = 0; d < DH; ++d) o[d] *= shrink;
       }
       const float base = m == -INFINITY ? 0.f : -m;
       const uint64_t mult2 = pair_f32(mult, mult), base2 = pair_f32(base, base);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int h = 0; h < KT; h += 64) {
-        uint32_t w[3][32];
+      for (int h = 0; h < KH; h += 32) {
+        uint32_t w[3][16];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
+        for (int c = 0; c < 16; ++c) {
           float u, v;
           unpair_f32(fma2(pair_f32(__uint_as_float(r[h + 2 * c]), __uint_as_float(r[h + 2 * c + 1])), mult2, base2), u, v);
           uint64_t x = pair_f32(prompt_exp2(u), prompt_exp2(v));
@@ -344,7 +373,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
           }
         }
 #pragma unroll
-        for (int part = 0; part < 3; ++part) tmem_st32(lanes + C::P_AT + part * (KT / 2) + h / 2, w[part]);
+        for (int part = 0; part < 3; ++part) tmem_st16(lanes + C::P_AT + part * (KT / 2) + (half * KH + h) / 2, w[part]);
       }
       float s0, s1;
       unpair_f32(add2(sum[0], sum[1]), s0, s1);
@@ -355,35 +384,39 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       if (lane == 0) mbar_arrive(&p_full);
     }
     if (ok && steps > 0) ok = add(steps - 1);
+    float other = 0.f;
+    if (ok && exchange(max(steps, 0), l, other)) l += other;
     // a row that sees keys has a sum, unless all its logits are -inf
     if (l == 0.f && visible > 0 && steps > 0) l = NAN;
     const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
     const long long at = ((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq;   // of the parts
-    float* const dst = p.splits > 1 ? p.parts + at * D : (float*)p.out + (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head;
+    float* const dst = (p.splits > 1 ? p.parts + at * D : (float*)p.out + (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head) + half * DH;
     if (any_odd) {
 #pragma unroll
-      for (int d = 0; d < D; ++d) o[d] = put_back_odd<D>(odd, d, visible, o[d] * inv);
+      for (int d = 0; d < DH; ++d) o[d] = put_back_odd<D>(odd, half * DH + d, visible, o[d] * inv);
     } else {
 #pragma unroll
-      for (int d = 0; d < D; ++d) o[d] *= inv;
+      for (int d = 0; d < DH; ++d) o[d] *= inv;
     }
     if (mine) {
       if (p.o_vec || p.splits > 1) {
 #pragma unroll
-        for (int d = 0; d < D; d += 4) *(float4*)(dst + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+        for (int d = 0; d < DH; d += 4) *(float4*)(dst + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
       } else {
 #pragma unroll
-        for (int d = 0; d < D; ++d) dst[d] = o[d];
+        for (int d = 0; d < DH; ++d) dst[d] = o[d];
       }
-      if (p.splits > 1) p.stats[at] = make_float2(m, l);
-      else if (p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+      if (half == 0) {
+        if (p.splits > 1) p.stats[at] = make_float2(m, l);
+        else if (p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+      }
     }
   }
   __syncwarp();
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if (warp == 5) tmem_dealloc(tmem, 512);
+  if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace raiccl
