@@ -113,6 +113,47 @@ __device__ __forceinline__ int prompt_visible(const PromptParams& p, const Promp
 // the keys, so that is enough to put them back.  first[0]: NaN, [1]: +inf, [2]: -inf.
 __device__ __forceinline__ int odd_kind(float v) { return v != v ? 0 : v > 0.f ? 1 : 2; }
 
+// So 64 threads look through a tile of KT values (rows of 128 bytes in the 128-byte swizzle, 64 dimensions; the next 64
+// behind them), of which rows from `behind` on are of no key of this sequence's: those become zeros, in every part.  What is not
+// finite is in the first part.  16-byte pieces are loaded BATCH at a time, and put back one by one only where one of them has such
+// a number: with each stored before the next was loaded a tile of 16 KB took 4000 clocks, more than its products.
+template <int D, int KT, int BATCH, int PARTS>
+__device__ __forceinline__ void prompt_fix_values(uint8_t* const (&part)[PARTS], int thread, int key0, int behind, int (*first)[D], int* any_odd) {
+  constexpr int PIECES = KT * D / 8;
+  static_assert(PIECES % (64 * BATCH) == 0, "whole batches");
+  if (behind < KT) {
+    for (int c = thread; c < PIECES; c += 64)
+      if ((c / 8) % KT >= behind)
+#pragma unroll
+        for (int j = 0; j < PARTS; ++j) ((uint4*)part[j])[c] = make_uint4(0, 0, 0, 0);
+  }
+  auto bad = [](uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; };   // an exponent of ones
+  uint4* const at = (uint4*)part[0];
+#pragma unroll 1
+  for (int c0 = thread; c0 < PIECES; c0 += 64 * BATCH) {
+    uint32_t some = 0;
+    uint4 v[BATCH];
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) v[e] = at[c0 + 64 * e];
+#pragma unroll
+    for (int e = 0; e < BATCH; ++e) some |= bad(v[e].x) | bad(v[e].y) | bad(v[e].z) | bad(v[e].w);
+    if (some == 0) continue;
+#pragma unroll 1
+    for (int c = c0; c < c0 + 64 * BATCH; c += 64) {
+      const int row = (c / 8) % KT, d = 64 * (c / (8 * KT)) + 8 * ((c & 7) ^ (row & 7));
+      __nv_bfloat16* const x = (__nv_bfloat16*)(at + c);
+#pragma unroll 1
+      for (int e = 0; e < 8; ++e) {
+        const float f = __bfloat162float(x[e]);
+        if (fabsf(f) < INFINITY) continue;
+        atomicMin(&first[odd_kind(f)][d + e], key0 + row);
+        x[e] = __float2bfloat16_rn(0.f);
+      }
+    }
+    *any_odd = 1;
+  }
+}
+
 template <int D>
 __device__ __forceinline__ float put_back_odd(const int (*first)[D], int d, int visible, float v) {
   // v may hold some already, of tiles that all rows saw whole

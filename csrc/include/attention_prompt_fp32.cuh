@@ -243,37 +243,15 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   } else if (warp >= 10) {
     // ---------------------------------------------------------------- values
     for (int i = 0; i < steps; ++i) {
-      uint4* at[3];                // the parts
+      uint8_t* at[3];              // the parts
       bool ok = true;
       for (int part = 2; ok && part >= 0; --part) {
         const int n = v_at(i) + 2 - part, slot = n % C::SLOTS;
         ok = mbar_wait_warp(&full[slot], (n / C::SLOTS) & 1, p.status, kPromptKernelId, kPromptWaitNs);
-        at[part] = (uint4*)(ring + slot * C::KV_PART);
+        at[part] = ring + slot * C::KV_PART;
       }
       if (!ok) break;
-#pragma unroll 4
-      for (int c = (warp - 10) * 32 + lane; c < C::KV_PART / 16; c += 64) {
-        const int half = c / (KT * 8), row = (c / 8) % KT, key = i * KT + row;
-        if (key >= s.nk) {           // behind the sequence's end
-#pragma unroll
-          for (int part = 0; part < 3; ++part) at[part][c] = make_uint4(0, 0, 0, 0);
-          continue;
-        }
-        const uint4 v = at[0][c];    // the first part: what is not finite is there
-        auto bad = [](uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; };
-        if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          const int d = 64 * half + 8 * ((c & 7) ^ (row & 7));
-          for (int e = 0; e < 8; ++e) {
-            const float f = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-            if (fabsf(f) < INFINITY) continue;
-            atomicMin(&odd[odd_kind(f)][d + e], key);
-            w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-          }
-          any_odd = 1;
-          at[0][c] = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+      prompt_fix_values<D, KT, 8>(at, threadIdx.x - 320, i * KT, s.nk - i * KT, odd, &any_odd);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&v_ready[i & 1]);

@@ -407,30 +407,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           const int stage = (base + i) % C::STAGES;
           if (!(ok = mbar_wait_warp(&v_raw[stage], raw_phase >> stage & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
           raw_phase ^= 1u << stage;
-          uint4* const at = (uint4*)(sv + stage * C::TILE);
-#pragma unroll 4
-          for (int c = (warp - 10) * 32 + lane; c < C::TILE / 16; c += 64) {
-            const int half = c / 1024, row = (c / 8) % 128;
-            const int key = i * kPromptKeys + row;
-            if (key >= k_end) {
-              at[c] = make_uint4(0, 0, 0, 0);
-              continue;
-            }
-            uint4 v = at[c];
-            auto bad = [](uint32_t w) { return (((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; };   // an exponent of ones
-            if (bad(v.x) | bad(v.y) | bad(v.z) | bad(v.w)) {
-              uint32_t w[4] = {v.x, v.y, v.z, v.w};
-              const int d = 64 * half + 8 * ((c & 7) ^ (row & 7));    // the swizzle's order of 16-byte pieces
-              for (int e = 0; e < 8; ++e) {
-                const float f = __uint_as_float((e & 1) ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
-                if (fabsf(f) < INFINITY) continue;
-                atomicMin(&odd[n & 1][odd_kind(f)][d + e], key);
-                w[e / 2] &= (e & 1) ? 0x0000ffffu : 0xffff0000u;
-              }
-              any_odd[n & 1] = 1;
-              at[c] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
+          uint8_t* const at[1] = {sv + stage * C::TILE};
+          const int key0 = i * kPromptKeys;
+          prompt_fix_values<D, kPromptKeys, 4>(at, threadIdx.x - 320, key0, k_end - key0, odd[n & 1], &any_odd[n & 1]);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(&v_ready[stage]);
