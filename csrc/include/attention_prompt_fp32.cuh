@@ -8,18 +8,21 @@
 // prompt_split_kernel, as TMA reads them; those of the weights P by the threads
 // that work them out, into TMEM.
 //
-// One tile of 128 rows to a CTA; KT keys a step.  S has two buffers, so that Q K^T
-// of the next step runs while the softmax has this one; the softmax waits for P V
-// of the last step before it writes P.  The tensor core cuts what does not fit its
-// sums: the small products come first, and P V leaves it after every step and is
-// added up in registers (with one sum for all steps 2048 keys were 4e-6 off).
+// One tile of 128 rows to a CTA; KT keys a step, half a row of them to a thread
+// of the softmax.  S has two buffers, so that Q K^T of the next step runs while
+// the softmax has this one; the softmax waits for P V of the last step before it
+// writes P.  Keys and values go through one ring, by their parts.  The tensor core
+// cuts what does not fit its sums: the largest product comes last, and P V leaves
+// it after every step and is added up in registers (with one sum for all steps
+// 2048 keys were 4e-6 off).
 //
 // What bounds it.  Three sequences of 2049 tokens in all, 16 heads of 64, every key
-// seen: 74 us, 11 of them the splitting, 0.33e-6 off (the formula in 32 bits: 0.65e-6).
-// The six products would take 24: from S to P is 3800 clocks of 4 warps, and P V and
-// Q K^T of 1536 each wait for it every other time; tensor cores busy 34 %.  Two
-// warpgroups on alternate steps: 70 us, but 292 for 249 with heads of 128 (spills).
-// As two tf32 parts on mma.sync: 200 us.
+// seen: 53 us, 11 of them the splitting, 0.33e-6 off (the formula in 32 bits: 0.65e-6).
+// The six products would take 24.  A step takes about 3900 clocks, 3400 of them
+// products (P V, with heads of 64, 1850): weights from S to P are 1800 of 8 warps,
+// half of them behind the sums of the last step.  A row to a thread: 76 us; values
+// in one stage, loaded when the last ones were done: 72 us.  As two tf32 parts on
+// mma.sync: 200 us.
 //
 // Values go through two warps that look for numbers that are not finite
 // (attention_prompt.cuh): an infinity times a part of a weight that is negative
@@ -320,16 +323,27 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), other;
       if (!(ok = exchange(i, peak, other))) break;
       peak = fmaxf(peak, other) * mult;
-      if (i > 0 && !(ok = add(i - 1))) break;    // before P is written where its operand was
-      const bool grow = peak > m + 8.f;
-      if (__any_sync(0xffffffffu, grow)) {
+      const bool grow = peak > m + 8.f, follow = __any_sync(0xffffffffu, grow);
+      float shrink = 1.f;
+      if (follow) {
         const float now = grow ? peak : m;
-        const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
+        shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
         m = now;
         l *= shrink;
-#pragma unroll
-        for (int d = 0; d < DH; ++d) o[d] *= shrink;
       }
+      // P is written where the last step's was, so that one's products come first: ahead of them the first 32 weights, where
+      // a thread has 64 (three sequences of 2049 tokens in all, heads of 64: 56 -> 53 us); where it has 32, that is slower
+      // (2000 tokens, 32 heads of 128: 381 -> 386 us; causal, over 8 key heads, 184 -> 187).
+      constexpr bool AHEAD = KH > 32;
+      auto sums = [&] {
+        if (i > 0 && !add(i - 1)) return false;
+        if (follow) {
+#pragma unroll
+          for (int d = 0; d < DH; ++d) o[d] *= shrink;
+        }
+        return true;
+      };
+      if (!AHEAD && !(ok = sums())) break;
       const float base = m == -INFINITY ? 0.f : -m;
       const uint64_t mult2 = pair_f32(mult, mult), base2 = pair_f32(base, base);
       uint64_t sum[2] = {0, 0};
@@ -350,9 +364,11 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
             if (part < 2) x = add2(x, pair_f32(__uint_as_float((rounded << 16) ^ 0x80000000u), __uint_as_float((rounded & 0xffff0000u) ^ 0x80000000u)));
           }
         }
+        if (AHEAD && h == 0 && !(ok = sums())) break;
 #pragma unroll
         for (int part = 0; part < 3; ++part) tmem_st16(lanes + C::P_AT + part * (KT / 2) + (half * KH + h) / 2, w[part]);
       }
+      if (!ok) break;
       float s0, s1;
       unpair_f32(add2(sum[0], sum[1]), s0, s1);
       l += s0 + s1;
