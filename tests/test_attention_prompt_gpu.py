@@ -282,3 +282,26 @@ def test_captured(dtype):
         for side, q, k, v, cq, ck, graph, out in states:
             want, _, bound, *_ = _want(q, k, v, q_lens, k_lens, True)
             check_close(out[:sum(q_lens)], want, bound)
+
+
+@DTYPES
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("times", [4, 5], ids=["by_length", "in_order"])
+def test_tiles_one_after_another(times, dim, dtype):
+    """More tiles than SMs, of sequences long, short, empty and without keys: what one leaves behind does not reach the next."""
+    q_lens, k_lens = [300, 17, 0, 260, 130, 1, 520] * times, [300, 17, 40, 261, 0, 700, 520] * times
+    hk = 10
+    q, k, v = _make(q_lens, k_lens, hk, 1, dim, dtype, seed=33)
+    base, base_lse = _check(q, k, v, q_lens, k_lens)
+    v2 = v.clone()
+    rows, ends = [], _cu(k_lens).tolist()[1:]
+    for i, (end, row) in enumerate(zip(ends, _cu(q_lens).tolist()[1:])):
+        if i % 2 and k_lens[i] and q_lens[i]:       # the last key, which the last row alone sees
+            v2[end - 1, :, i % dim] = (NAN, INF, -INF)[i % 3]
+            rows.append((row - 1, i % dim, (NAN, INF, -INF)[i % 3]))
+    out, lse = _attend(q, k, v2, _cu(q_lens), _cu(k_lens), return_lse=True, check=True)
+    want = base.clone()
+    for row, d, x in rows:
+        want[row, :, d] = x
+    assert len(rows) > 2 * times and torch.equal(out.isnan(), want.isnan())
+    assert torch.equal(out.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0)) and torch.equal(lse, base_lse)
