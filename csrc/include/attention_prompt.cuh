@@ -42,7 +42,8 @@ __device__ __forceinline__ int prompt_tiles(const PromptParams& p, int b, int to
 // sequence the last tile, which sees the most keys, comes first.
 //
 // Up to 32 sequences, one to a lane, go by their number of keys, the longest first, so that no long tile begins when the
-// others are done.  More of them even that out by themselves and go in their order: every lane counts an equal number of
+// others are done (eight chunks of 512 tokens on average: 168 -> 161 us).  More of them even that out by themselves and go in their
+// order: every lane counts an equal number of
 // sequences, then the warp goes through those of the lane that has the tile.
 __device__ __forceinline__ bool prompt_tile(const PromptParams& p, int index, int tokens, PromptSeq& s, int& tile) {
   const int lane = threadIdx.x & 31;

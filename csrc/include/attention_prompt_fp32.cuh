@@ -384,7 +384,8 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     if (l == 0.f && visible > 0 && steps > 0) l = NAN;
     const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
     const long long at = ((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq;   // of the parts
-    float* const dst = (p.splits > 1 ? p.parts + at * D : (float*)p.out + (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head) + half * DH;
+    float* const dst = half * DH + (p.splits > 1 ? p.parts + at * D
+                                                 : (float*)p.out + (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head);
     if (any_odd) {
 #pragma unroll
       for (int d = 0; d < DH; ++d) o[d] = put_back_odd<D>(odd, half * DH + d, visible, o[d] * inv);
