@@ -108,7 +108,7 @@ struct PromptParams {
   int B, Hq, Hk, group, D;
   int bf16, causal, o_vec;
   float scale;
-  // by the plan: CTAs that share a tile's keys, [splits][Nq][Hq][D] their sums, [splits][Nq][Hq] maxima and sums of exponentials
+  // by the plan: CTAs that share a tile's keys, [splits][Nq][Hq][D] means over their keys, [splits][Nq][Hq] their maxima and sums of weights
   int splits;
   float* parts;
   float2* stats;

@@ -108,6 +108,21 @@ __device__ __forceinline__ int prompt_visible(const PromptParams& p, const Promp
   return n < 0 ? 0 : n;
 }
 
+// Weights are exp2(z - m).  Where m is set it is 15 above the row's maximum, and it is set again once a logit comes nearer to
+// it than 9 or the sum l of the weights passes 1/4 (by 8 at least).  So no weight is above 2^-9, a step's 128 add 1/4 at
+// most, l stays below 1/2, and sums of weights times finite values below the largest of those: they never overflow,
+// however large the values.  Weights near the largest are 2^-15 to 2^-9: products with values down to 2^-100 keep all
+// their bits.  (At logits of 2^27 the distance is lost in rounding, and values above 2^128 / keys may overflow.)
+//
+// With m at the maximum and followed at 2^64 times (bf16) or 2^8 times (fp32) that, values above 2^64 or 2^120 by the number of
+// keys became infinities.  A rise of 6 after a row's first step is rare all the same, and z - m is off by 2^-21 at most.
+constexpr float kPromptHead = 15.f, kPromptNear = 9.f, kPromptSum = 0.25f, kPromptLeast = 8.f;
+
+// log sum exp(z); l is mostly near 2^-15 of exponents at the maximum.
+__device__ __forceinline__ float prompt_lse(float m, float l) {
+  return ((m - kPromptHead) + log2f(l * 32768.f)) * 0.69314718055994531f;
+}
+
 // Values that are not finite must not reach rows that do not see them, but a
 // product adds 0 * NaN there.  They go into the products as zeros, and for each
 // kind and dimension the first key that has one is kept; a row sees a prefix of

@@ -122,7 +122,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
   __shared__ uint64_t q_full, full[C::SLOTS], empty[C::SLOTS], v_ready[2], s_full[2], p_full, o_full, met[4], drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int odd[3][D], any_odd;
-  __shared__ float told[2][2][128];                           // by turns, from each half of a row to the other
+  __shared__ float2 told[2][2][128];                          // by turns, from each half of a row to the other
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // Nothing of this needs what the kernels before wrote.  TMEM has to be taken before the next kernel may start: one that took
   // it first would keep it until this CTA is done.
@@ -273,8 +273,8 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     float m = -INFINITY, l = 0.f, o[DH];
 #pragma unroll
     for (int d = 0; d < DH; ++d) o[d] = 0.f;
-    // The other half's number of the same row; the place is written again two turns on, when both have met once more.
-    auto exchange = [&](int turn_of, float v, float& other) {
+    // The other half's numbers of the same row; the place is written again two turns on, when both have met once more.
+    auto exchange = [&](int turn_of, float2 v, float2& other) {
       told[turn_of & 1][half][row] = v;
       __syncwarp();
       if (lane == 0) mbar_arrive(&met[warp & 3]);
@@ -320,13 +320,14 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       for (int c = 0; c < KH; c += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
-      float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), other;
-      if (!(ok = exchange(i, peak, other))) break;
-      peak = fmaxf(peak, other) * mult;
-      const bool grow = peak > m + 8.f, follow = __any_sync(0xffffffffu, grow);
+      float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      float2 other;
+      if (!(ok = exchange(i, make_float2(peak, l), other))) break;
+      peak = fmaxf(peak, other.x) * mult;
+      const bool grow = peak > m - kPromptNear || l + other.y > kPromptSum, follow = __any_sync(0xffffffffu, grow);
       float shrink = 1.f;
       if (follow) {
-        const float now = grow ? peak : m;
+        const float now = grow ? fmaxf(peak + kPromptHead, m + kPromptLeast) : m;
         shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
         m = now;
         l *= shrink;
@@ -378,11 +379,11 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       if (lane == 0) mbar_arrive(&p_full);
     }
     if (ok && steps > 0) ok = add(steps - 1);
-    float other = 0.f;
-    if (ok && exchange(max(steps, 0), l, other)) l += other;
+    float2 other;
+    if (ok && exchange(max(steps, 0), make_float2(0.f, l), other)) l += other.y;
     // a row that sees keys has a sum, unless all its logits are -inf
     if (l == 0.f && visible > 0 && steps > 0) l = NAN;
-    const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     const long long at = ((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq;   // of the parts
     float* const dst = half * DH + (p.splits > 1 ? p.parts + at * D
                                                  : (float*)p.out + (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head);
@@ -403,7 +404,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       }
       if (half == 0) {
         if (p.splits > 1) p.stats[at] = make_float2(m, l);
-        else if (p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+        else if (p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = prompt_lse(m, l);
       }
     }
   }

@@ -7,7 +7,7 @@
 //
 //   S = Q K^T,  P = exp2(c S - m),  O = O + P V,  l = l + sum P
 //
-// with O multiplied by exp2 of the change where m has to follow the maximum.
+// with O and l multiplied by exp2 of the change where m has to follow the maximum.
 //
 // One warp loads (TMA), one issues the products (tcgen05.mma, 128 x 128 sums in
 // TMEM), and a warpgroup to each tile does the softmax, one row to a thread: no
@@ -446,10 +446,29 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         }
         const int all = __reduce_min_sync(0xffffffffu, mine ? visible : INT_MAX);   // keys that the warp's rows all see
         float m = -INFINITY, l = 0.f;
+        auto follow = [&](float now, bool sums) {
+          const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
+          m = now;
+          l *= shrink;
+          if (!sums) return;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(to + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
+            tmem_st32(to + c, o);
+          }
+        };
         for (int i = 0; ok && i < steps; ++i) {
           if (!(ok = mbar_wait_warp(&s_full[x], s_phase, p.status, kPromptKernelId, kPromptWaitNs))) break;
           s_phase ^= 1u;
           tc_fence_after_sync();
+          if (__any_sync(0xffffffffu, l > kPromptSum)) {
+            follow(l > kPromptSum ? m + kPromptLeast : m, true);
+            tmem_st_wait();
+          }
           uint32_t r[128];
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, r + 32 * c);
@@ -466,10 +485,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
             for (int c = 0; c < 128; ++c)
               if (k0 + c >= visible) r[c] = __float_as_uint(-INFINITY);
           }
-          // Weights are exp2(c S - m) for any m that lets them neither overflow nor vanish: bf16 and fp32 hold 2^64 as exactly as
-          // 1.  So m follows the maximum only when that is 2^64 past it (and in the first tile), and the first half of the weights
-          // is worked out before it is known whether it is.  The product begins with that half.  (A quarter of the exponentials
-          // by a polynomial, to spare the special-function unit: no difference, 16384 tokens run into the power limit.)
+          // The first half of the weights is worked out before it is known whether m has to follow the maximum (attention_prompt.cuh),
+          // which is rare, and the product begins with that half.  (A quarter of the exponentials by a polynomial, to spare the
+          // special-function unit: no difference, 16384 tokens run into the power limit.)
           uint64_t sum[2];
           uint32_t w[32];
           auto half = [&](int h, float base) {
@@ -502,25 +520,9 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
 #pragma unroll
               for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
             const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
-            const bool grow = peak > m + 64.f;
-            again = __any_sync(0xffffffffu, grow);
-            if (again) {
-              const float now = grow ? peak : m;
-              const float shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
-              m = now;
-              l *= shrink;
-              if (i > 0) {
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                  uint32_t o[32];
-                  tmem_ld32(to + c, o);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * shrink);
-                  tmem_st32(to + c, o);
-                }
-              }
-            }
+            const bool grow = peak > m - kPromptNear;
+            again = __any_sync(0xffffffffu, grow);   // once: it does not hold for peak + kPromptHead, however that is rounded
+            if (again) follow(grow ? peak + kPromptHead : m, i > 0);
           } while (again);
           store(0);
           half(1, m == -INFINITY ? 0.f : -m);
@@ -538,7 +540,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         const int token = it.token0 + x * tokens + row / p.group, hq = it.head * p.group + row % p.group;
         // a row that sees keys has a sum, unless all its logits are -inf
         if (l == 0.f && visible > 0 && steps > 0) l = NAN;
-        const float inv = p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         const bool put_back = any_odd[n & 1] != 0;
         const long long at = (long long)(it.s.q0 + token) * p.o_token + (long long)hq * p.o_head;
 #pragma unroll 1
@@ -551,6 +553,16 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = steps > 0 && visible > 0 ? __uint_as_float(o[e]) * inv : 0.f;
+          // weights that were rounded up may lift a mean of the largest numbers past them
+          constexpr float most = 3.3895313892515355e38f;
+          float size = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) size = max3(size, fabsf(v[e]), fabsf(v[e + 1]));
+          if (size > most) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (fabsf(__uint_as_float(o[e])) < INFINITY) v[e] = fminf(fmaxf(v[e], -most), most);
+          }
           if (put_back) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = put_back_odd<D>(odd[n & 1], c + e, visible, v[e]);
@@ -574,7 +586,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           __syncwarp();
         }
         if (mine && p.splits > 1) p.stats[((long long)it.split * p.Nq + it.s.q0 + token) * p.Hq + hq] = make_float2(m, l);
-        else if (mine && p.lse != nullptr) p.lse[(long long)(it.s.q0 + token) * p.Hq + hq] = (m + log2f(l)) * 0.69314718055994531f;
+        else if (mine && p.lse != nullptr) p.lse[(long long)(it.s.q0 + token) * p.Hq + hq] = prompt_lse(m, l);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[n & 1]);

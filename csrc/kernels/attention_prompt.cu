@@ -17,8 +17,8 @@
 
 namespace raiccl {
 
-// The results of tiles whose keys several CTAs shared, a warp to a row.  Rows before the first sequence and behind the last
-// stay as they are.
+// The results of tiles whose keys up to 32 CTAs shared, a warp to a row.  Parts are means of their own keys' values, so that what
+// is added up here stays below the largest of these too.  Rows before the first sequence and behind the last stay as they are.
 template <int D>
 __global__ void __launch_bounds__(256) prompt_join_kernel(PromptParams p) {
   griddep_wait();
@@ -28,13 +28,32 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptParams p) {
   if (row >= p.Nq * p.Hq) return;
   const long long token = row / p.Hq, hq = row - token * p.Hq;
   if (token < __ldg(p.cu_q) || token >= __ldg(p.cu_q + p.B)) return;
-  float top, l, v[D / 32];
   auto at = [&](int j) { return j * p.Nq * p.Hq + row; };
-  warp_join<D>(p.splits, [&](int j) { return p.stats[at(j)]; }, [&](int j) { return p.parts + at(j) * D; }, top, l, v);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float2 st = lane < p.splits ? p.stats[at(lane)] : make_float2(-INFINITY, 0.f);
+  float top = st.x;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) store_elem(p.out, token * p.o_token + hq * p.o_head + D / 32 * lane + i, v[i] * inv, p.bf16);
-  if (p.lse != nullptr && lane == 0) p.lse[row] = (top + log2f(l)) * 0.69314718055994531f;
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // no maximum: nothing there, or logits that are all NaN or -inf, whose sum is NaN
+  const float share = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : st.y * exp2_fast(st.x - top);
+  float l = share;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const float weight = l == 0.f ? 0.f : share / l;
+  float v[D / 32];
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) v[d] = 0.f;
+#pragma unroll 4
+  for (int j = 0; j < p.splits; ++j) {
+    float a[D / 32];
+    load_lanes<D>(p.parts + at(j) * D, a);
+    const float w = __shfl_sync(0xffffffffu, weight, j);
+    if (w == 0.f) continue;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) v[d] = fmaf(a[d], w, v[d]);
+  }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) store_elem(p.out, token * p.o_token + hq * p.o_head + D / 32 * lane + i, v[i], p.bf16);
+  if (p.lse != nullptr && lane == 0) p.lse[row] = prompt_lse(top, l);
 }
 
 // Rows of a tensor [n, heads, D] that TMA can read: on 16 bytes, and apart.
