@@ -45,12 +45,15 @@ __device__ __forceinline__ void warp_join(int n, Stat stat, Row row, float& top,
   for (int d = 0; d < D / 32; ++d) v[d] = 0.f;
   for (int j0 = 0; j0 < n; j0 += 32) {
     float f = 0.f, y = 0.f;
+    bool some = false;
     if (j0 + lane < n) {
       const float2 st = stat(j0 + lane);
+      some = st.x != -INFINITY || st.y != 0.f;
       // no maximum: nothing there, or logits that are all NaN or -inf, whose sum is NaN
       f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : exp2_fast(st.x - top);
       y = st.y;
     }
+    const uint32_t with = __ballot_sync(0xffffffffu, some);
     const int here = n - j0 < 32 ? n - j0 : 32;
 #pragma unroll 4
     for (int j = 0; j < here; ++j) {
@@ -58,7 +61,7 @@ __device__ __forceinline__ void warp_join(int n, Stat stat, Row row, float& top,
       load_lanes<D>(row(j0 + j), a);
       const float fj = __shfl_sync(0xffffffffu, f, j);
       l = fmaf(__shfl_sync(0xffffffffu, y, j), fj, l);
-      if (fj == 0.f) continue;             // (a part that is nothing holds anything)
+      if (!(with >> j & 1)) continue;      // a part that is nothing holds anything; one whose factor vanishes may hold a NaN
 #pragma unroll
       for (int d = 0; d < D / 32; ++d) v[d] = fmaf(a[d], fj, v[d]);
     }

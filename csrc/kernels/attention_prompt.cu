@@ -39,6 +39,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptParams p) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   const float weight = l == 0.f ? 0.f : share / l;
+  const uint32_t with = __ballot_sync(0xffffffffu, st.x != -INFINITY || st.y != 0.f);
   float v[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) v[d] = 0.f;
@@ -47,9 +48,10 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptParams p) {
     float a[D / 32];
     load_lanes<D>(p.parts + at(j) * D, a);
     const float w = __shfl_sync(0xffffffffu, weight, j);
-    if (w == 0.f) continue;
+    if (!(with >> j & 1)) continue;
+    // an infinity or NaN of a part whose weight vanishes is seen all the same
 #pragma unroll
-    for (int d = 0; d < D / 32; ++d) v[d] = fmaf(a[d], w, v[d]);
+    for (int d = 0; d < D / 32; ++d) v[d] = fabsf(a[d]) < INFINITY ? fmaf(a[d], w, v[d]) : v[d] + a[d];
   }
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) store_elem(p.out, token * p.o_token + hq * p.o_head + D / 32 * lane + i, v[i], p.bf16);

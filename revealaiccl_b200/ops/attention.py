@@ -79,7 +79,8 @@ def attention_prompt(
     less, so k and v may begin with earlier tokens of a chunked prompt.  A token
     that sees nothing gets zeros, and rows of ``out`` before the first and behind
     the last sequence are left as they were.  What a token does not see does not
-    enter its result, infinities and NaN included.  scale: default head_dim **
+    enter its result, infinities and NaN included; of what it does see, an
+    infinity whose weight is below 2^-110 may come out as NaN.  scale: default head_dim **
     -0.5.  At most 2^16 sequences.
 
     Sums, maxima and the result are kept in fp32 and rounded once, to q's type.

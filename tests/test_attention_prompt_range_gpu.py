@@ -132,3 +132,29 @@ def test_nan_and_infinities_behind_a_rise(dim, dtype):
     want = base.clone()
     want[250:, :, 3], want[260:, :, 7], want[270:, :, 8] = NAN, math.inf, -math.inf
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
+@DTYPES
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("below", [1.0, 80.0, 200.0])
+def test_nan_and_infinities_of_a_part_that_hardly_counts(below, dim, dtype):
+    """Keys that several CTAs share, most of them `below` under the last ones: what they see is not lost in the joining."""
+    logits = [0.0] * 2500 + [below] * 500
+    q, k, v = _steered([5], logits, 2, 3, dim, dtype, seed=50)
+    q[:, :, 0] = 1.0
+    assert _plan(q, k, v, 1)["splits"] > 1
+    base = _attend(q, k, v, _cu([5]), _cu([3000]), scale=1.0, check=True)
+    v2 = v.clone()
+    v2[10, 0, 3] = NAN
+    v2[2400, 1, 5] = NAN
+    v2[2998, 0, 9] = NAN                    # which rows 3 and 4 see
+    out = _attend(q, k, v2, _cu([5]), _cu([3000]), scale=1.0, check=True)
+    want = base.clone()
+    want[:, :3, 3], want[:, 3:, 5], want[3:, :3, 9] = NAN, NAN, NAN
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+    v2 = v.clone()
+    v2[10, 0, 3], v2[2400, 1, 5] = math.inf, -math.inf
+    out = _attend(q, k, v2, _cu([5]), _cu([3000]), scale=1.0, check=True)
+    assert not out[:, :3, 3].isfinite().any() and not out[:, 3:, 5].isfinite().any()
+    out[:, :3, 3], out[:, 3:, 5] = base[:, :3, 3], base[:, 3:, 5]
+    assert torch.equal(out, base)
