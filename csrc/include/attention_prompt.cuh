@@ -123,6 +123,12 @@ __device__ __forceinline__ float prompt_lse(float m, float l) {
   return ((m - kPromptHead) + log2f(l * 32768.f)) * 0.69314718055994531f;
 }
 
+// 1 / l.  A row without keys has l = 0, and zeros for a result.  One that sees keys whose logits are all -inf has l = -0: NaN,
+// but not yet where other CTAs have some of its keys, whose logits may be finite; -0 tells the join that there were keys.
+__device__ __forceinline__ float prompt_per_sum(const PromptParams& p, float l) {
+  return l != 0.f ? 1.f / l : __float_as_uint(l) != 0u && p.splits == 1 ? NAN : 0.f;
+}
+
 // Values that are not finite must not reach rows that do not see them, but a
 // product adds 0 * NaN there.  They go into the products as zeros, and for each
 // kind and dimension the first key that has one is kept; a row sees a prefix of

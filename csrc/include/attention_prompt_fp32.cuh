@@ -381,9 +381,8 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
     if (ok && steps > 0) ok = add(steps - 1);
     float2 other;
     if (ok && exchange(max(steps, 0), make_float2(0.f, l), other)) l += other.y;
-    // a row that sees keys has a sum, unless all its logits are -inf
-    if (l == 0.f && visible > 0 && steps > 0) l = NAN;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (l == 0.f && visible > 0 && steps > 0) l = -0.f;
+    const float inv = prompt_per_sum(p, l);
     const long long at = ((long long)blockIdx.y * p.Nq + s.q0 + token) * p.Hq + hq;   // of the parts
     float* const dst = half * DH + (p.splits > 1 ? p.parts + at * D
                                                  : (float*)p.out + (long long)(s.q0 + token) * p.o_token + (long long)hq * p.o_head);

@@ -538,9 +538,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
         }
         const volatile PromptItem& it = items[n & 1];             // not kept over the steps: S takes the registers
         const int token = it.token0 + x * tokens + row / p.group, hq = it.head * p.group + row % p.group;
-        // a row that sees keys has a sum, unless all its logits are -inf
-        if (l == 0.f && visible > 0 && steps > 0) l = NAN;
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (l == 0.f && visible > 0 && steps > 0) l = -0.f;
+        const float inv = prompt_per_sum(p, l);
         const bool put_back = any_odd[n & 1] != 0;
         const long long at = (long long)(it.s.q0 + token) * p.o_token + (long long)hq * p.o_head;
 #pragma unroll 1

@@ -33,13 +33,13 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptParams p) {
   float top = st.x;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // no maximum: nothing there, or logits that are all NaN or -inf, whose sum is NaN
+  // no maximum: no keys (0), logits that are all -inf (-0), or NaN
   const float share = st.x == -INFINITY ? (st.y == 0.f ? 0.f : NAN) : st.y * exp2_fast(st.x - top);
+  const uint32_t with = __ballot_sync(0xffffffffu, st.x != -INFINITY || __float_as_uint(st.y) != 0u);
   float l = share;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  const float weight = l == 0.f ? 0.f : share / l;
-  const uint32_t with = __ballot_sync(0xffffffffu, st.x != -INFINITY || st.y != 0.f);
+  const float weight = l != 0.f ? share / l : with != 0 ? NAN : 0.f;
   float v[D / 32];
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) v[d] = 0.f;

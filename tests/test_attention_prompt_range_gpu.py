@@ -5,8 +5,9 @@ import math
 import pytest
 import torch
 
+from attention_reference import attention64
 from serving_reference import check_close
-from test_attention_prompt_gpu import BF16, DEV, DTYPES, FP32, NAN, _attend, _check, _cu, _make, _plan, _want
+from test_attention_prompt_gpu import BF16, DEV, DTYPES, FP32, NAN, WEIGHT, _attend, _check, _cu, _make, _plan, _want
 
 pytestmark = pytest.mark.gpu
 MOST = {BF16: torch.finfo(BF16).max, FP32: 3e38}
@@ -158,3 +159,35 @@ def test_nan_and_infinities_of_a_part_that_hardly_counts(below, dim, dtype):
     assert not out[:, :3, 3].isfinite().any() and not out[:, 3:, 5].isfinite().any()
     out[:, :3, 3], out[:, 3:, 5] = base[:, :3, 3], base[:, 3:, 5]
     assert torch.equal(out, base)
+
+
+@DTYPES
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("q_len,k_len", [(5, 3000), (290, 900)], ids=["shared", "one_cta"])
+def test_keys_whose_logits_are_all_minus_infinity(q_len, k_len, causal, dim, dtype):
+    """Keys shut out by a number that makes their logit -inf (in fp32 by overflow): whole tiles and whole CTAs' shares of them."""
+    for shut in (slice(0, 2 * k_len // 3), slice(k_len // 3, k_len), slice(128, k_len - 1)):
+        q, k, v = _make([q_len], [k_len], 2, 3, dim, dtype, seed=52)
+        assert (_plan(q, k, v, 1)["splits"] > 1) == (q_len == 5)
+        q[:, :, 0], k[:, :, 0] = 10.0, 0.0
+        k[shut, :, 0] = -math.inf if dtype == BF16 else -3e38
+        out, lse = _attend(q, k, v, _cu([q_len]), _cu([k_len]), causal=causal, return_lse=True, check=True)
+        keep = torch.ones(k_len, dtype=torch.bool, device=DEV)
+        keep[shut] = False
+        see = torch.arange(q_len, device=DEV) + (k_len - q_len + 1) if causal else torch.full((q_len,), k_len, device=DEV)
+        want, wlse, bound, lbound, _ = attention64(q, k[keep], v[keep], keep.cumsum(0)[see - 1], None, WEIGHT[dtype])
+        check_close(out, want, bound)
+        check_close(lse, wlse, lbound)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_len,k_len", [(5, 3000), (290, 900)], ids=["shared", "one_cta"])
+def test_no_key_but_at_minus_infinity(q_len, k_len, dim):
+    q, k, v = _make([q_len], [k_len], 2, 3, dim, BF16, seed=54)
+    q[:, :, 0], k[:, 0, 0] = 1.0, -math.inf
+    out, lse = _attend(q, k, v, _cu([q_len]), _cu([k_len]), return_lse=True, check=True)
+    assert out[:, :3].isnan().all() and (lse[:, :3] == -math.inf).all()
+    want, wlse, bound, lbound, _ = _want(q[:, 3:], k[:, 1:], v[:, 1:], [q_len], [k_len], True)
+    check_close(out[:, 3:], want, bound)
+    check_close(lse[:, 3:], wlse, lbound)
