@@ -142,7 +142,9 @@ __device__ __forceinline__ int cached_tokens(const CachedParams& p, int n) {
 }
 __device__ __forceinline__ int cached_length(const CachedParams& p, int b) { return cached_tokens(p, __ldg(p.lengths + b)); }
 
-__device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) { return (cached_length(p, b) + kCachedTile - 1) / kCachedTile; }
+// Tiles of n tokens, which may be 2^31 - 16.
+__device__ __forceinline__ int tiles_of(int n) { return n / kCachedTile + (n % kCachedTile != 0); }
+__device__ __forceinline__ int cached_tiles(const CachedParams& p, int b) { return tiles_of(cached_length(p, b)); }
 
 // CTAs that take part (two tiles to one at least), the first tile of one, and the CTA of a tile.
 __device__ __forceinline__ int cached_ctas(long long tiles, int ctas) {
@@ -809,13 +811,13 @@ __global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p) {
   // kernel before lets it start only after its own wait, so this is worked out ahead of the wait for the parts (one
   // sequence of 1000 tokens 13.5 -> 11.0 us, 37 ragged ones 25.0 -> 22.8).  Read from L2, which the lengths' writer has
   // reached: no wait of this kernel's has dropped what this SM's L1 may hold of them.
-  const auto tiles_of = [&](int i) { return (cached_tokens(p, __ldcg(p.lengths + i)) + kCachedTile - 1) / kCachedTile; };
+  const auto tiles_at = [&](int i) { return tiles_of(cached_tokens(p, __ldcg(p.lengths + i))); };
   const int HC = p.c.heads * p.chunks, b = blockIdx.x / HC, hc = blockIdx.x - b * HC, h = blockIdx.y;
   int head0;
   const int heads = piece_heads(p, hc, head0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   long long all = 0, ahead = 0;
   for (int i = threadIdx.x; i < p.B; i += 256) {
-    const int n = tiles_of(i);
+    const int n = tiles_at(i);
     all += n;
     if (i < b) ahead += n;
   }
@@ -828,7 +830,7 @@ __global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p) {
   __syncthreads();
   all = ahead = 0;
   for (int w = 0; w < 8; ++w) { all += sum_of[0][w]; ahead += sum_of[1][w]; }
-  const int n = tiles_of(b);
+  const int n = tiles_at(b);
   int c0 = 0, c1 = 0;
   if (n > 0) {
     const long long tiles = all * HC, first = ahead * HC + (long long)hc * n;

@@ -36,3 +36,30 @@ def test_nan_of_a_part_that_hardly_counts(below, tokens, dim, dtype):
     want[:, :3, 16:32] = NAN
     got = out(v2)
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
+@pytest.mark.parametrize("page", [16, 32])
+def test_longest_row_of_the_table(page):
+    """2^31 tokens but a page's, of one page over and over; a length behind the row is cut to that and recorded."""
+    from revealaiccl_b200.ops.kv_cache import KVCache4, kv_cache_write
+    from revealaiccl_b200.ops.status import DeviceStatusError, check_serving
+    cache = KVCache4.empty(1, page, 1, 64)
+    v = torch.randint(-6, 7, (page, 1, 64), generator=_gen(3), device=DEV).float()
+    v[v.abs() == 5] = 0.0                          # what 4 bits have, at a scale of 1
+    v[:, :, ::16] = 6.0
+    kv_cache_write(cache, torch.zeros_like(v), v, torch.arange(page, device=DEV), check=True)
+    row = torch.zeros(1, 2 ** 31 // page - 1, dtype=torch.int32, device=DEV)
+    most = 2 ** 31 - page
+    for lengths in ([most, 5, 0, page], [5, 2 ** 31 - 1, 1, most]):
+        q = torch.randn(4, 3, 64, generator=_gen(4), device=DEV).to(BF16)
+        out, lse = _attend(q, cache, row.expand(4, -1), torch.tensor(lengths, dtype=torch.int32, device=DEV), return_lse=True)
+        if max(lengths) > most:
+            with pytest.raises(DeviceStatusError, match="bounds"):
+                check_serving(DEV)
+        check_serving(DEV)
+        for b, n in enumerate(lengths):
+            n = min(n, most)
+            want = torch.zeros(64, dtype=torch.float64, device=DEV) if n == 0 else v[:min(n, page), 0].double().mean(0)
+            # weights of 128 and small whole numbers add up exactly up to 2^24 times their unit, which a warp's share is below
+            assert ((out[b].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all()
+            assert (lse[b].double() - (torch.tensor(float(n), dtype=torch.float64).log().item() if n else -float("inf"))).abs().nan_to_num(0.0).max() < 1e-5
