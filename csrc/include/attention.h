@@ -15,6 +15,7 @@ namespace raiccl {
 
 constexpr int kCacheGroup = 16;      // numbers that share a scale
 constexpr int kCachePage = 16;       // smallest page
+constexpr int kCachedTile = 64;      // tokens of a sequence that attention_cached works on at once
 constexpr int kCachedKernelId = 640, kCacheWriteKernelId = 641, kCacheReadKernelId = 642, kPromptKernelId = 643;
 
 // The cache: pages of page_size tokens, [pages, heads, page_size, D / 2] codes

@@ -247,12 +247,21 @@ std::tuple<torch::Tensor, OptTensor> attention_cached(torch::Tensor q, torch::Te
                     ": the output is fp32, or bf16 where q is bf16");
   CachedParams p{};
   p.scale = check_scale(op, scale, D);
+  p.c = c;
+  p.group = (int)(Hq / c.heads);
+  p.bf16 = q.scalar_type() == torch::kBFloat16;
+  p.out_bf16 = dt == torch::kBFloat16;
+  // tiles that the table has room for, as the kernels count them: in 32 bits within a sequence, and a CTA's share
+  const int64_t tiles = ((block_table.size(1) << c.page_shift) + kCachedTile - 1) / kCachedTile * c.heads * plan_cached(p, 1).chunks;
+  TORCH_CHECK_VALUE(tiles < (1ll << 32), op, ": block_table has room for ", text(tiles), " tiles of 64 tokens of a sequence and a chunk of heads, "
+                    "2^32 or more");
+  TORCH_CHECK_VALUE(B * tiles < (1ll << 37), op, ": block_table has room for ", text(B * tiles), " tiles of 64 tokens of a sequence and a chunk of "
+                    "heads in all, 2^37 or more");
   torch::Tensor res = attention_out(op, out, dt, q, {&q, &k_codes, &k_scales, &v_codes, &v_scales, &block_table, &lengths});
   const c10::cuda::CUDAGuard guard(dev);
   OptTensor lse;
   if (return_lse) lse = fresh({B, Hq}, torch::kFloat32, dev);
   if (B == 0) return {res, lse};
-  p.c = c;
   p.q = q.data_ptr();
   p.q_seq = q.stride(0);
   p.q_head = q.stride(1);
@@ -266,9 +275,6 @@ std::tuple<torch::Tensor, OptTensor> attention_cached(torch::Tensor q, torch::Te
   p.lengths = lengths.data_ptr<int>();
   p.B = (int)B;
   p.Hq = (int)Hq;
-  p.group = (int)(Hq / c.heads);
-  p.bf16 = q.scalar_type() == torch::kBFloat16;
-  p.out_bf16 = dt == torch::kBFloat16;
   p.q_vec = rows16(q);
   p.o_vec = rows16(res);
   p.status = serving_status();

@@ -57,7 +57,6 @@
 
 namespace raiccl {
 
-constexpr int kCachedTile = 64;
 // Probabilities are exp2(z - m + 7) and m follows the maximum once that passes 15: f16 holds them (below 2^15), and small
 // ones keep their bits down to 2^-21 of the largest.
 constexpr float kCachedHead = 7.f, kCachedRoom = 15.f;

@@ -36,6 +36,11 @@ def attention_cached(
     behind a sequence's last page are not read.  lengths int32 [B]; an empty
     sequence gets zeros.  scale: default head_dim ** -0.5.
 
+    The query heads of a key head are worked on in equal chunks of up to 16, or 8
+    where q or the result is fp32, and each chunk reads the cache again.  A row of
+    the table has room for less than 2^31 tokens, and for less than 2^38 by key
+    heads and chunks; all rows for less than 2^43 by them.
+
     Sums, maxima and the result are kept in fp32 and rounded once, to out_dtype
     (default: q's type; fp32 queries give fp32).  For bf16 results the
     probabilities enter their product as f16 numbers; for fp32 results queries

@@ -1,0 +1,29 @@
+"""How wide a table attention_cached takes: beyond that its counts of tiles would not hold.  Refused before any GPU is needed."""
+
+import pytest
+import torch
+
+from revealaiccl_b200.ops import _native
+
+if not _native.has_kernels():  # pragma: no cover
+    pytest.skip("kernel library not built", allow_module_level=True)
+
+from revealaiccl_b200.ops.attention import attention_cached
+from revealaiccl_b200.ops.kv_cache import KVCache4
+
+BF16, FP32 = torch.bfloat16, torch.float32
+NO_GPU = "must be on a CUDA device"     # what the CPU's tensors meet behind all other checks
+
+
+@pytest.mark.parametrize("seqs,heads,group,dtype,out_dtype,words", [
+    (1, 127, 1, BF16, BF16, NO_GPU), (1, 129, 1, BF16, BF16, "2\\^32 or more"), (1, 256, 2, BF16, BF16, "2\\^32 or more"),
+    (1, 16, 128, BF16, BF16, NO_GPU), (1, 16, 128, BF16, FP32, "2\\^32 or more"), (1, 16, 128, FP32, FP32, "2\\^32 or more"),
+    (4096, 1, 1, BF16, BF16, NO_GPU), (4097, 1, 1, BF16, BF16, "2\\^37 or more"), (2049, 1, 17, BF16, BF16, "2\\^37 or more"),
+    (2049, 1, 16, BF16, BF16, NO_GPU), (0, 1, 1, BF16, BF16, NO_GPU),
+])
+def test_widest_tables(seqs, heads, group, dtype, out_dtype, words):
+    cache = KVCache4.empty(0, 65536, heads, 64, device="cpu")
+    table = torch.zeros(1, 32767, dtype=torch.int32).expand(seqs, -1)     # 2^31 - 65536 tokens to a sequence
+    q = torch.zeros(1, heads * group, 64, dtype=dtype).expand(seqs, -1, -1)
+    with pytest.raises(ValueError, match=words):
+        attention_cached(q, cache, table, torch.zeros(seqs, dtype=torch.int32), out_dtype=out_dtype)
