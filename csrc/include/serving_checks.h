@@ -9,8 +9,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <string>
 #include <utility>
+#include <vector>
 
 namespace raiccl {
 
@@ -52,6 +54,41 @@ inline std::pair<const char*, const char*> extent(const torch::Tensor& t) {
 inline bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
   const auto x = extent(a), y = extent(b);
   return x.first < y.second && y.first < x.second;
+}
+
+// A tensor's elements as bytes: dimensions by falling stride, the element itself last.
+struct Spread {
+  const char* at;
+  std::vector<std::pair<int64_t, int64_t>> dims;   // stride, size
+  int64_t element;
+  explicit Spread(const torch::Tensor& t) : at((const char*)t.data_ptr()), element(t.element_size()) {
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (t.size(d) > 1 && t.stride(d) != 0) dims.emplace_back(t.stride(d) * element, t.size(d));
+    std::sort(dims.rbegin(), dims.rend());
+  }
+  int64_t span(size_t from) const {                // bytes from the first to the last, of the dimensions from this one on
+    int64_t n = element;
+    for (size_t i = from; i < dims.size(); ++i) n += (dims[i].second - 1) * dims[i].first;
+    return n;
+  }
+};
+
+// Whether b, which begins d bytes behind a, may have a byte of a's; `i` dimensions of both are done with.  Where both go on
+// by the same stride and fit into it, a block of a's meets at most two of b's: those that begin less than a stride before or
+// behind it.  Otherwise what lies within the other's reach counts as shared.
+inline bool may_meet(const Spread& a, const Spread& b, size_t i, int64_t d) {
+  if (d >= a.span(i) || d + b.span(i) <= 0) return false;
+  if (i >= a.dims.size() || i >= b.dims.size() || a.dims[i].first != b.dims[i].first) return true;
+  const int64_t s = a.dims[i].first;
+  if (a.span(i + 1) > s || b.span(i + 1) > s) return true;
+  const int64_t r = (d % s + s) % s;
+  return may_meet(a, b, i + 1, r) || may_meet(a, b, i + 1, r - s);
+}
+
+inline bool may_share_memory(const torch::Tensor& a, const torch::Tensor& b) {
+  if (!overlap(a, b)) return false;
+  const Spread x(a), y(b);
+  return may_meet(x, y, 0, y.at - x.at);
 }
 
 // Behind a shape there may be no numbers to read: a sparse layout, a lazy zero or

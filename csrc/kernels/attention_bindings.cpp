@@ -121,7 +121,9 @@ void check_slots(const char* op, const torch::Tensor& slots, const torch::Device
 
 void check_apart(const char* op, const char* name, const torch::Tensor& out, std::initializer_list<const torch::Tensor*> inputs) {
   TORCH_CHECK_VALUE(apart(out), op, ": the elements of ", name, " share memory");
-  for (const torch::Tensor* t : inputs) TORCH_CHECK_VALUE(!overlap(out, *t), op, ": ", name, " shares memory with another tensor of the call");
+  for (const torch::Tensor* t : inputs)
+    TORCH_CHECK_VALUE(!may_share_memory(out, *t), op, ": ", name, " shares memory with another tensor of the call, or lies between its elements by "
+                      "other strides");
 }
 
 void kv_cache_write(torch::Tensor k_codes, torch::Tensor k_scales, torch::Tensor v_codes, torch::Tensor v_scales, double k_unit,

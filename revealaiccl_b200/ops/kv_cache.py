@@ -109,7 +109,8 @@ def kv_cache_read(
 
     dtype: bf16 (default) or fp32, or by ``k_out`` and ``v_out``, which may have
     any strides with contiguous rows but may not share memory with the cache or
-    each other.  Nothing is rounded: a code times its scale has at most 6 bits.
+    each other; they may lie between each other's rows by the same strides, as the
+    two halves of a joint buffer do.  Nothing is rounded: a code times its scale has at most 6 bits.
     slots: int32 or int64, the same one any number of times; zeros come back for
     a slot below zero, and for one behind the cache's end, which is recorded:
     ``check=True`` waits and raises.
