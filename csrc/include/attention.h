@@ -60,6 +60,12 @@ struct CacheReadParams {
 void launch_cache_write(const CacheWriteParams& p, cudaStream_t s);
 void launch_cache_read(const CacheReadParams& p, cudaStream_t s);
 
+// What a CTA of attention_cached and those behind it have parts of: query heads of a sequence, up to tile `last` of all `tiles`.
+struct CachedJoin {
+  int b, head0, heads;
+  long long last, tiles;
+};
+
 // out[b, h] = softmax(scale q[b, h] K^T) V over the first lengths[b] tokens of sequence b.
 struct CachedParams {
   CacheView c;
@@ -79,16 +85,18 @@ struct CachedParams {
   // by the plan
   int chunk, chunks;                 // query heads that are worked on together, such chunks of a group
   int ctas;                          // that share the work
+  int notes;                         // joins are told by p.joins, not found from the lengths
   float* parts;                      // [ctas][2][chunk][D] sums of sequences that several CTAs share
   float2* stats;                     // [ctas][2][chunk] their maxima and sums of exponentials
   float* spill;                      // [ctas][warps][8 or 16][D] sums that a warp puts aside
+  CachedJoin* joins;                 // [ctas] pieces that begin within a CTA's share and end behind it; no heads: none
   DeviceStatus* status;
 };
 
 struct CachedPlan {
   int chunk, chunks, ctas;
-  long long parts_bytes, stats_bytes, spill_bytes;
-  long long bytes() const { return parts_bytes + stats_bytes + spill_bytes; }
+  long long parts_bytes, stats_bytes, spill_bytes, joins_bytes;
+  long long bytes() const { return parts_bytes + stats_bytes + spill_bytes + joins_bytes; }
 };
 
 CachedPlan plan_cached(const CachedParams& p, int sms);

@@ -235,6 +235,7 @@ struct CachedPart {
 // the CTA's parts 0 (it began before the CTA's share) and 1 (it ends after it), 2 the output.
 struct CachedChain {
   int warp, side, end, b, head0, heads, where;
+  long long last;      // its last tile
 };
 
 template <int D, int NT, int PARTS>
@@ -251,6 +252,7 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   griddep_wait();
   griddep_launch_dependents();
+  if (p.notes && tid == 0) p.joins[blockIdx.x].heads = 0;   // none, unless a piece is found to go on behind this CTA's share
 
   // ------------------------------------------------------------ all tiles, and this CTA's and this warp's
   const int HC = p.c.heads * p.chunks, per = (p.B + C::THREADS - 1) / C::THREADS;
@@ -771,7 +773,9 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
       int head0;
       const int nheads = piece_heads(p, s.hc, head0);
       const bool early = s.first < c0, late = s.first + s.n > c1;
-      chain[(heads != 0) * side + (side ? __popc(tails & ((1u << lane) - 1)) : 0)] = {lane, side, end, s.b, head0, nheads, early ? 0 : late ? 1 : 2};
+      chain[(heads != 0) * side + (side ? __popc(tails & ((1u << lane) - 1)) : 0)] = {lane,  side,   end,
+                                                                                      s.b,   head0,  nheads,
+                                                                                      early ? 0 : late ? 1 : 2, s.first + s.n - 1};
     }
     if (lane == 0) { chains = __popc(tails) + (heads != 0); all_with = with; }
   }
@@ -794,58 +798,84 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
     } else {
       const long long at = ((long long)blockIdx.x * 2 + x.where) * p.chunk + h;
       store_lanes<D>(p.parts + at * D, v);
-      if (lane == 0) p.stats[at] = make_float2(top, l);
+      if (lane == 0) {
+        p.stats[at] = make_float2(top, l);
+        if (p.notes && x.where == 1 && h == 0) p.joins[blockIdx.x] = {x.b, x.head0, x.heads, x.last, tiles};
+      }
     }
   }
 }
 
-// Sequences that several CTAs share, one head to a CTA; a warp takes every
-// eighth part.  Empty sequences too, which no tile stands for.
+// Pieces that several CTAs share, one head to a CTA; a warp takes every eighth part.  Empty sequences too, which no tile stands for.
+//
+// With no more pieces than CTAs in the kernel before, a CTA to each piece finds out whose parts it has from the lengths.  They are
+// final once this kernel runs at all, since every CTA of the kernel before lets it start only after its own wait, so that is done
+// ahead of the wait for the parts (one sequence of 1000 tokens 13.5 -> 11.0 us, 37 ragged ones 25.0 -> 22.8).  Read from L2, which
+// the lengths' writer has reached: no wait of this kernel's has dropped what this SM's L1 may hold of them.
+//
+// With more pieces that would read the lengths by the square of the batch (65536 sequences of one token: 129 ms, now 1.3; 4096: 940
+// us, now 83).  A CTA of the kernel before has at most one piece that begins in its share and ends behind it, and leaves a note of
+// it (p.joins) for the CTA here; empty sequences are found by a lane each.  (32 sequences of 100 tokens, 256 pieces: 14.0 -> 11.5
+// us.  With notes, one sequence of 1000 tokens took 11.2 us instead of 10.8, by one more load behind the wait.)
 template <int D>
 __global__ void __launch_bounds__(256) cached_join_kernel(CachedParams p) {
   __shared__ long long sum_of[2][8];
   __shared__ float4 acc[8][D / 4];
   __shared__ float2 ml[8];
-  // Whose parts these are goes by the lengths.  They are final once this kernel runs at all, since every CTA of the
-  // kernel before lets it start only after its own wait, so this is worked out ahead of the wait for the parts (one
-  // sequence of 1000 tokens 13.5 -> 11.0 us, 37 ragged ones 25.0 -> 22.8).  Read from L2, which the lengths' writer has
-  // reached: no wait of this kernel's has dropped what this SM's L1 may hold of them.
+  const int h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const auto tiles_at = [&](int i) { return tiles_of(cached_tokens(p, __ldcg(p.lengths + i))); };
-  const int HC = p.c.heads * p.chunks, b = blockIdx.x / HC, hc = blockIdx.x - b * HC, h = blockIdx.y;
-  int head0;
-  const int heads = piece_heads(p, hc, head0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  long long all = 0, ahead = 0;
-  for (int i = threadIdx.x; i < p.B; i += 256) {
-    const int n = tiles_at(i);
-    all += n;
-    if (i < b) ahead += n;
-  }
+  int b = 0, head0 = 0, heads = 0, c0 = blockIdx.x, c1 = c0;
+  if (!p.notes) {
+    const int HC = p.c.heads * p.chunks;
+    b = blockIdx.x / HC;
+    const int hc = blockIdx.x - b * HC;
+    heads = piece_heads(p, hc, head0);
+    long long all = 0, ahead = 0;
+    for (int i = threadIdx.x; i < p.B; i += 256) {
+      const int n = tiles_at(i);
+      all += n;
+      if (i < b) ahead += n;
+    }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
-  }
-  if (lane == 0) { sum_of[0][warp] = all; sum_of[1][warp] = ahead; }
-  __syncthreads();
-  all = ahead = 0;
-  for (int w = 0; w < 8; ++w) { all += sum_of[0][w]; ahead += sum_of[1][w]; }
-  const int n = tiles_at(b);
-  int c0 = 0, c1 = 0;
-  if (n > 0) {
-    const long long tiles = all * HC, first = ahead * HC + (long long)hc * n;
-    const int ctas = cached_ctas(tiles, p.ctas);
-    c0 = cached_cta(tiles, ctas, first);
-    c1 = cached_cta(tiles, ctas, first + n - 1);
+    for (int o = 16; o > 0; o >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    }
+    if (lane == 0) { sum_of[0][warp] = all; sum_of[1][warp] = ahead; }
+    __syncthreads();
+    all = ahead = 0;
+    for (int w = 0; w < 8; ++w) { all += sum_of[0][w]; ahead += sum_of[1][w]; }
+    const int n = tiles_at(b);
+    c0 = c1 = 0;
+    if (n > 0) {
+      const long long tiles = all * HC, first = ahead * HC + (long long)hc * n;
+      const int ctas = cached_ctas(tiles, p.ctas);
+      c0 = cached_cta(tiles, ctas, first);
+      c1 = cached_cta(tiles, ctas, first + n - 1);
+    } else if (warp == 0 && h < heads) {   // (nothing before this kernel's predecessor is still at work on the result)
+      const float zeros[D / 32] = {};
+      cached_row(p, b, head0 + h, -INFINITY, 0.f, zeros);
+    }
+  } else {
+    for (int b0 = 32 * (warp * gridDim.x + blockIdx.x); b0 < p.B; b0 += 256 * gridDim.x) {
+      const bool none = b0 + lane < p.B && tiles_at(b0 + lane) == 0;
+      for (uint32_t empty = __ballot_sync(0xffffffffu, none); empty != 0; empty &= empty - 1)
+        for (int head = h; head < p.Hq; head += gridDim.y) {
+          const float zeros[D / 32] = {};
+          cached_row(p, b0 + __ffs(empty) - 1, head, -INFINITY, 0.f, zeros);
+        }
+    }
   }
   griddep_wait();
   griddep_launch_dependents();
-  if (h >= heads) return;
-  if (n == 0) {
-    if (threadIdx.x < D / 4) cached_store4(p, b, head0 + h, 4 * threadIdx.x, make_float4(0.f, 0.f, 0.f, 0.f));
-    if (p.lse != nullptr && threadIdx.x == 0) p.lse[(long long)b * p.Hq + head0 + h] = -INFINITY;
-    return;
+  if (p.notes) {
+    const CachedJoin join = p.joins[c0];
+    b = join.b;
+    head0 = join.head0;
+    heads = join.heads;
+    if (heads > 0) c1 = cached_cta(join.tiles, cached_ctas(join.tiles, p.ctas), join.last);
   }
-  if (c0 == c1) return;
+  if (h >= heads || c0 == c1) return;
   float m = -INFINITY, l = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   const bool mine = lane < D / 4;
@@ -891,6 +921,7 @@ CachedPlan plan_cached(const CachedParams& p, int sms) {
   plan.stats_bytes = ((long long)plan.ctas * 2 * plan.chunk * 8 + 255) / 256 * 256;
   const int warps = most == 8 ? kCachedWarps<1, 2> : plan.chunk <= 8 ? kCachedWarps<1, 1> : kCachedWarps<2, 1>;
   plan.spill_bytes = (long long)plan.ctas * warps * (plan.chunk > 8 ? 16 : 8) * p.c.D * 4;
+  plan.joins_bytes = plan.ctas * (long long)sizeof(CachedJoin);
   return plan;
 }
 
@@ -908,7 +939,7 @@ static void launch_cached_as(const CachedParams& p, cudaStream_t s) {
     configured.fetch_or(bit);
   }
   launch_with_pdl(kern, dim3(p.ctas), dim3(C::THREADS), C::SMEM, s, true, p);
-  launch_with_pdl(cached_join_kernel<D>, dim3(p.B * p.c.heads * p.chunks, p.chunk), dim3(256), 0, s, true, p);
+  launch_with_pdl(cached_join_kernel<D>, dim3(p.notes ? p.ctas : p.B * p.c.heads * p.chunks, p.chunk), dim3(256), 0, s, true, p);
 }
 
 void launch_cached(const CachedParams& params, const CachedPlan& plan, void* workspace, cudaStream_t s) {
@@ -916,9 +947,11 @@ void launch_cached(const CachedParams& params, const CachedPlan& plan, void* wor
   p.chunk = plan.chunk;
   p.chunks = plan.chunks;
   p.ctas = plan.ctas;
+  p.notes = (long long)p.B * p.c.heads * p.chunks > p.ctas;
   p.parts = (float*)workspace;
   p.stats = (float2*)((char*)workspace + plan.parts_bytes);
   p.spill = (float*)((char*)workspace + plan.parts_bytes + plan.stats_bytes);
+  p.joins = (CachedJoin*)((char*)workspace + plan.parts_bytes + plan.stats_bytes + plan.spill_bytes);
   const bool two = !(p.bf16 && p.out_bf16);
   if (p.c.D == 128) {
     if (two) launch_cached_as<128, 1, 2>(p, s);

@@ -63,3 +63,35 @@ def test_longest_row_of_the_table(page):
             # weights of 128 and small whole numbers add up exactly up to 2^24 times their unit, which a warp's share is below
             assert ((out[b].double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all()
             assert (lse[b].double() - (torch.tensor(float(n), dtype=torch.float64).log().item() if n else -float("inf"))).abs().nan_to_num(0.0).max() < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+def test_tens_of_thousands_of_sequences(dtype):
+    """Short ones, empty ones and some that several CTAs share; the time grows with their number, not with its square."""
+    from revealaiccl_b200.ops.kv_cache import KVCache4, kv_cache_write
+    n, heads, group, dim, page = 65536, 2, 3, 64, 16
+    cache = KVCache4.empty(400, page, heads, dim)
+    kv = torch.randn(2, 6400, heads, dim, generator=_gen(5), device=DEV)
+    kv_cache_write(cache, kv[0], kv[1], torch.arange(6400, device=DEV), check=True)
+    table = torch.arange(400, dtype=torch.int32, device=DEV).expand(n, -1)
+    lens = torch.randint(0, 70, (n,), generator=_gen(6), device=DEV).int()
+    lens[1000:3000] = 0
+    long = torch.tensor([0, 17, 2999, 40000, n - 1], device=DEV)
+    lens[long] = torch.tensor([6400, 6399, 3000, 6001, 5000], device=DEV).int()
+    q = torch.randn(1, heads * group, dim, generator=_gen(7), device=DEV).to(dtype)
+    out, lse = _attend(q.expand(n, -1, -1), cache, table, lens, return_lse=True, check=True)
+    kinds = torch.cat([torch.arange(70, device=DEV), lens[long]]).int()     # one sequence of each length
+    want, wlse = _attend(q.expand(len(kinds), -1, -1), cache, table[:len(kinds)], kinds, return_lse=True, check=True)
+    kind = lens.long().clamp_max(69)
+    kind[long] = torch.arange(70, 75, device=DEV)
+    # both are within 2^-8 (bf16), 2^-18 of the values' mean size (fp32) of the formula; equal where a warp has all of a sequence
+    bound = (2.0 ** -7 if dtype == BF16 else 2.0 ** -17) * 4
+    assert ((out.float() - want[kind].float()).abs() <= bound).all()
+    assert torch.equal(lse == -float("inf"), wlse[kind] == -float("inf")) and not out[lens == 0].any()
+    assert ((lse - wlse[kind]).nan_to_num(0.0).abs() <= 1e-5).all()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    _attend(q.expand(n, -1, -1), cache, table, lens)
+    end.record()
+    end.synchronize()
+    assert start.elapsed_time(end) < 10.0, "65536 sequences of 35 tokens: 0.4 ms of tiles"
