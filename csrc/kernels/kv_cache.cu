@@ -33,6 +33,7 @@ namespace raiccl {
 
 constexpr int kWriteThreads = 256;
 constexpr int kWriteTokens = 2048;         // of a CTA at most
+constexpr int kWriteAtOnce = 1 << 20;      // of a launch at most
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float d;
@@ -349,19 +350,28 @@ __global__ void __launch_bounds__(256) kv_cache_read_kernel(CacheReadParams p) {
   }
 }
 
-// Tokens of a CTA: up to four CTAs to an SM, which all fit.
+// Tokens of a CTA: up to four CTAs to an SM, which all fit.  A CTA looks through all later slots of its launch, so that grows with the
+// square of the tokens: launches have up to kWriteAtOnce, in the tokens' order, the later one's tokens over the earlier one's (2^23
+// tokens of one head of 64: 7.9 -> 2.5 ms, in slots all over the cache 68 -> 21).
 void launch_cache_write(const CacheWriteParams& params, cudaStream_t s) {
-  CacheWriteParams p = params;
   const long long wave = 4ll * serving_sm_count();
-  while ((p.N >> p.per_shift) > wave && (1 << p.per_shift) < kWriteTokens) ++p.per_shift;
-  const int per = 1 << p.per_shift;
-  const dim3 grid((unsigned)((p.N + per - 1) / per));
-  const size_t smem = 5 * per * sizeof(int);
-  p.per_k_unit = 1.f / p.c.k_unit;
-  p.per_v_unit = 1.f / p.c.v_unit;
-  auto run = [&](auto kern) { launch_with_pdl(kern, grid, dim3(kWriteThreads), smem, s, true, p); };
-  if (p.c.D == 128) p.bf16 ? run(kv_cache_write_kernel<__nv_bfloat16, 128>) : run(kv_cache_write_kernel<float, 128>);
-  else p.bf16 ? run(kv_cache_write_kernel<__nv_bfloat16, 64>) : run(kv_cache_write_kernel<float, 64>);
+  for (long long done = 0; done < params.N; done += kWriteAtOnce) {
+    CacheWriteParams p = params;
+    p.N = std::min<long long>(params.N - done, kWriteAtOnce);
+    const long long eb = p.bf16 ? 2 : 4;
+    p.k = (const char*)p.k + done * p.k_token * eb;
+    p.v = (const char*)p.v + done * p.v_token * eb;
+    p.slots = (const char*)p.slots + done * (p.slots64 ? 8 : 4);
+    while ((p.N >> p.per_shift) > wave && (1 << p.per_shift) < kWriteTokens) ++p.per_shift;
+    const int per = 1 << p.per_shift;
+    const dim3 grid((unsigned)((p.N + per - 1) / per));
+    const size_t smem = 5 * per * sizeof(int);
+    p.per_k_unit = 1.f / p.c.k_unit;
+    p.per_v_unit = 1.f / p.c.v_unit;
+    auto run = [&](auto kern) { launch_with_pdl(kern, grid, dim3(kWriteThreads), smem, s, true, p); };
+    if (p.c.D == 128) p.bf16 ? run(kv_cache_write_kernel<__nv_bfloat16, 128>) : run(kv_cache_write_kernel<float, 128>);
+    else p.bf16 ? run(kv_cache_write_kernel<__nv_bfloat16, 64>) : run(kv_cache_write_kernel<float, 64>);
+  }
 }
 
 void launch_cache_read(const CacheReadParams& p, cudaStream_t s) {

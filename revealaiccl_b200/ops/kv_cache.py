@@ -88,8 +88,8 @@ def kv_cache_write(cache: KVCache4, k: torch.Tensor, v: torch.Tensor, slots: tor
     tokens of a call name one slot, the last of them is kept.  A slot behind the
     cache's end is left out too, and recorded: ``check=True`` waits and raises.
 
-    Enqueues one launch on the current stream without synchronising and can be
-    captured in a CUDA graph.  There is no backward.
+    Enqueues one launch (for every 2^20 tokens) on the current stream without
+    synchronising and can be captured in a CUDA graph.  There is no backward.
     """
     kernels().kv_cache_write(*cache._parts(), k, v, slots)
     if check:
