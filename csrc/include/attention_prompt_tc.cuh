@@ -42,6 +42,8 @@ namespace raiccl {
 constexpr int kPromptThreads = 384;   // two warpgroups of softmax; loads, products, two warps for masked tiles' values
 constexpr int kPromptKeys = 128;
 constexpr unsigned long long kPromptWaitNs = 2000000000ull;
+// Warps that have nothing to do for a pair of tiles wait for all its steps: 1.5 to 2 us for 128 keys, and 20 at most.
+constexpr unsigned long long kPromptKeyNs = 160ull;
 
 template <int D>
 struct PromptTc {
@@ -399,14 +401,15 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
       // -------------------------------------------------------------- values of tiles that some row does not see whole
       int base = 0;
       uint32_t raw_phase = 0;
+      const unsigned long long limit = kPromptWaitNs + p.Nk * kPromptKeyNs;
       bool ok = true;
       for (int n = 0; ok; ++n) {
-        if (!(ok = mbar_wait_warp(&item_full[n & 1], (n >> 1) & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+        if (!(ok = mbar_wait_warp(&item_full[n & 1], (n >> 1) & 1, p.status, kPromptKernelId, limit))) break;
         const int k_end = items[n & 1].s.nk, steps = items[n & 1].steps;
         if (steps < 0) break;
         for (int i = items[n & 1].first_fixed; i < steps; ++i) {
           const int stage = (base + i) % C::STAGES;
-          if (!(ok = mbar_wait_warp(&v_raw[stage], raw_phase >> stage & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+          if (!(ok = mbar_wait_warp(&v_raw[stage], raw_phase >> stage & 1, p.status, kPromptKernelId, limit))) break;
           raw_phase ^= 1u << stage;
           uint8_t* const at[1] = {sv + stage * C::TILE};
           const int key0 = i * kPromptKeys;
@@ -432,7 +435,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
     bool ok = true;
     uint32_t s_phase = 0, o_phase = 0;
     for (int n = 0; ok; ++n) {
-      if (!(ok = mbar_wait_warp(&item_full[n & 1], (n >> 1) & 1, p.status, kPromptKernelId, kPromptWaitNs))) break;
+      if (!(ok = mbar_wait_warp(&item_full[n & 1], (n >> 1) & 1, p.status, kPromptKernelId, kPromptWaitNs + p.Nk * kPromptKeyNs))) break;
       const int steps = items[n & 1].steps;
       if (steps < 0) break;
       if (x < items[n & 1].tiles) {

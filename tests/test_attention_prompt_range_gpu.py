@@ -191,3 +191,21 @@ def test_no_key_but_at_minus_infinity(q_len, k_len, dim):
     want, wlse, bound, lbound, _ = _want(q[:, 3:], k[:, 1:], v[:, 1:], [q_len], [k_len], True)
     check_close(out[:, 3:], want, bound)
     check_close(lse[:, 3:], wlse, lbound)
+
+
+def test_more_keys_than_two_seconds_of_steps():
+    """One token behind 4 * 10^8 keys, all of one CTA's (80 tiles for all that the plan can tell): warps without work wait that long."""
+    n, dim = 400_000_000, 64
+    if torch.cuda.mem_get_info()[0] < 70e9:
+        pytest.skip("needs 51 GB of device memory")
+    x = torch.zeros(n + 1, 1, dim, dtype=BF16, device=DEV)
+    x[:128] = 1.0
+    x[-1, 0, 3] = math.inf                             # of the last key's value, which no key has
+    q = torch.ones(1, 1, dim, dtype=BF16, device=DEV)
+    cu_q, cu_k = _cu([1] + [0] * 79), _cu([n] + [0] * 79)
+    assert _plan(q, x[:-1], x[1:], 80)["splits"] == 1
+    out = _attend(q, x[:-1], x[1:], cu_q, cu_k, scale=0.5, check=True)
+    # the first 128 keys lie 32 nats above the others, which all together are 4e8 exp(-32) / 128 = 4e-8 of them; 127 of their values are 1
+    assert out[0, 0, 3] == math.inf
+    out[0, 0, 3] = out[0, 0, 4]
+    assert (out == 127 / 128).all()
