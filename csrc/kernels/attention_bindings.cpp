@@ -56,9 +56,11 @@ void check_index(const char* op, const char* name, const torch::Tensor& t, const
                     " must be a contiguous int32 tensor of shape ", text({n}));
 }
 
+constexpr double kLog2e = 1.44269504088896340736;
+
 float check_scale(const char* op, c10::optional<double> scale, int64_t D) {
   const double s = scale ? *scale : 1.0 / std::sqrt((double)D);
-  TORCH_CHECK_VALUE(std::isfinite((float)s), op, ": scale must be a finite number");
+  TORCH_CHECK_VALUE(std::isfinite((float)(s * kLog2e)), op, ": scale must be a finite number, and by log2(e) in fp32 too");
   return (float)s;
 }
 

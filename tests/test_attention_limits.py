@@ -1,4 +1,4 @@
-"""How wide a table attention_cached takes: beyond that its counts of tiles would not hold.  Refused before any GPU is needed."""
+"""Where numbers of a call would not hold in the kernels: tables too wide for their counts, scales too large.  Refused before any GPU is needed."""
 
 import pytest
 import torch
@@ -8,7 +8,7 @@ from revealaiccl_b200.ops import _native
 if not _native.has_kernels():  # pragma: no cover
     pytest.skip("kernel library not built", allow_module_level=True)
 
-from revealaiccl_b200.ops.attention import attention_cached
+from revealaiccl_b200.ops.attention import attention_cached, attention_prompt
 from revealaiccl_b200.ops.kv_cache import KVCache4
 
 BF16, FP32 = torch.bfloat16, torch.float32
@@ -27,3 +27,15 @@ def test_widest_tables(seqs, heads, group, dtype, out_dtype, words):
     q = torch.zeros(1, heads * group, 64, dtype=dtype).expand(seqs, -1, -1)
     with pytest.raises(ValueError, match=words):
         attention_cached(q, cache, table, torch.zeros(seqs, dtype=torch.int32), out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("scale,words", [(2.3e38, NO_GPU), (-2.3e38, NO_GPU), (2.4e38, "scale must be"), (-3.4e38, "scale must be"), (1e300, "scale must be"),
+                                         (float("nan"), "scale must be"), (float("inf"), "scale must be"), (0.0, NO_GPU)])
+def test_scales(scale, words):
+    """Exponentials are of base 2: a scale that overflows by log2(e) would turn logits of 0 into NaN."""
+    cache = KVCache4.empty(1, 16, 1, 64, device="cpu")
+    q, lens, table = torch.zeros(1, 1, 64, dtype=BF16), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match=words):
+        attention_cached(q, cache, table, lens, scale=scale)
+    with pytest.raises(ValueError, match=words):
+        attention_prompt(q, q, q, torch.zeros(2, dtype=torch.int32), scale=scale)
