@@ -81,7 +81,8 @@ struct CachedParams {
   int B, Hq, group;                  // group = Hq / heads
   int bf16, out_bf16;
   int q_vec, o_vec;                  // rows may be read and written 16 bytes at a time
-  float scale;
+  float mult;                        // logits to base 2 are q . codes * scales by mult 2^mult_exp: scale, log2(e) and the keys' unit
+  int mult_exp;
   // by the plan
   int chunk, chunks;                 // query heads that are worked on together, such chunks of a group
   int ctas;                          // that share the work

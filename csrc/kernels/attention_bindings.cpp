@@ -58,10 +58,10 @@ void check_index(const char* op, const char* name, const torch::Tensor& t, const
 
 constexpr double kLog2e = 1.44269504088896340736;
 
-float check_scale(const char* op, c10::optional<double> scale, int64_t D) {
+double check_scale(const char* op, c10::optional<double> scale, int64_t D) {
   const double s = scale ? *scale : 1.0 / std::sqrt((double)D);
   TORCH_CHECK_VALUE(std::isfinite((float)(s * kLog2e)), op, ": scale must be a finite number, and by log2(e) in fp32 too");
-  return (float)s;
+  return s;
 }
 
 float check_unit(const char* op, const char* name, double unit) {
@@ -250,7 +250,7 @@ std::tuple<torch::Tensor, OptTensor> attention_cached(torch::Tensor q, torch::Te
   TORCH_CHECK_VALUE(dt == torch::kFloat32 || (dt == torch::kBFloat16 && q.scalar_type() == torch::kBFloat16), op,
                     ": the output is fp32, or bf16 where q is bf16");
   CachedParams p{};
-  p.scale = check_scale(op, scale, D);
+  p.mult = (float)std::frexp(check_scale(op, scale, D) * kLog2e * c.k_unit, &p.mult_exp);
   p.c = c;
   p.group = (int)(Hq / c.heads);
   p.bf16 = q.scalar_type() == torch::kBFloat16;
@@ -347,7 +347,7 @@ std::tuple<torch::Tensor, OptTensor> attention_prompt(torch::Tensor q, torch::Te
   check_index(op, "cu_seqlens_q", cu_seqlens_q, dev, B + 1);
   check_index(op, "cu_seqlens_k", cu_seqlens_k, dev, B + 1);
   PromptParams p{};
-  p.scale = check_scale(op, scale, D);
+  p.scale = (float)check_scale(op, scale, D);
   torch::Tensor res = attention_out(op, out, q.scalar_type(), q, {&q, &k, &v, &cu_seqlens_q, &cu_seqlens_k});
   const c10::cuda::CUDAGuard guard(dev);
   OptTensor lse;

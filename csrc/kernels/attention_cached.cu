@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         if (e == 0 || e == 255) e = 127;
         if (e > 253) e = 253;
         const float down = __uint_as_float((254u - e) << 23);
-        const float up = __uint_as_float(e << 23) * p.c.k_unit * p.scale * 1.44269504088896341f;
+        const float up = scalbnf(p.mult, (int)e - 127 + p.mult_exp);   // one after the other, the factors may overflow
         mult[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t);
         mult[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
 #pragma unroll

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_attention_cached_gpu import BF16, DEV, FP32, NAN, _attend, _gen
+from test_attention_cached_gpu import BF16, DEV, FP32, NAN, _attend, _check, _filled, _gen, _q, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,15 @@ def test_tens_of_thousands_of_sequences(dtype):
     end.record()
     end.synchronize()
     assert start.elapsed_time(end) < 10.0, "65536 sequences of 35 tokens: 0.4 ms of tiles"
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size,unit", [(1e30, 2.0 ** 40), (1e38, 2.0 ** 63), (1e-30, 2.0 ** 63), (1e-10, 2.0 ** -64), (1e30, 2.0 ** -64)])
+def test_queries_and_units_that_meet_in_the_scale(size, unit, dtype):
+    """Logits of ordinary size from queries, a unit of the keys and a scale whose products are not, two by two."""
+    lengths = [500, 77]
+    cache = _filled(40, 16, 2, 128, k_unit=unit, v_unit=0.25)
+    table = _table(lengths, 16, cache.pages)
+    q = (_q(2, 6, 128, FP32).clamp(-3, 3) * size).to(dtype)
+    for sign in (1, -1):
+        _check(q, cache, table, lengths, scale=sign * 0.05 / size / unit)
