@@ -20,7 +20,7 @@ HEAD_DIMS = (64, 128)
 PAGE_SIZES = tuple(1 << i for i in range(4, 17))
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)   # equal to itself: tensors' comparisons have no one answer
 class KVCache4:
     """Pages of ``page_size`` tokens for every key head, 4.5 bits a number.
 

@@ -39,3 +39,8 @@ def test_scales(scale, words):
         attention_cached(q, cache, table, lens, scale=scale)
     with pytest.raises(ValueError, match=words):
         attention_prompt(q, q, q, torch.zeros(2, dtype=torch.int32), scale=scale)
+
+
+def test_caches_are_told_apart_and_found():
+    one, other = (KVCache4.empty(1, 16, 1, 64, device="cpu") for _ in range(2))
+    assert one == one and one != other and [other, one].index(one) == 1 and {one: 1, other: 2}[other] == 2
