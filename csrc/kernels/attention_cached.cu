@@ -445,9 +445,10 @@ __global__ void __launch_bounds__(Cached<D, NT, PARTS>::THREADS, 1) cached_kerne
         for (int i = 0; i < D / 4; ++i) top = fmaxf(top, fabsf(x[i]));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the power of two at or below the largest (1 for zeros and infinities), and its reciprocal
+        // the power of two at or below the largest (1 for infinities, the least normal number for what lies below it), and its reciprocal
         uint32_t e = __float_as_uint(top) >> 23;
-        if (e == 0 || e == 255) e = 127;
+        if (e == 0) e = 1;
+        if (e == 255) e = 127;
         if (e > 253) e = 253;
         const float down = __uint_as_float((254u - e) << 23);
         const float up = scalbnf(p.mult, (int)e - 127 + p.mult_exp);   // one after the other, the factors may overflow

@@ -107,3 +107,18 @@ def test_queries_and_units_that_meet_in_the_scale(size, unit, dtype):
     q = (_q(2, 6, 128, FP32).clamp(-3, 3) * size).to(dtype)
     for sign in (1, -1):
         _check(q, cache, table, lengths, scale=sign * 0.05 / size / unit)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("size", [3e-38, 1e-39, 1e-40])
+def test_queries_below_the_least_normal_number(size, dtype):
+    """They keep the bits that they have."""
+    lengths = [500, 77]
+    cache = _filled(40, 16, 2, 128)
+    table = _table(lengths, 16, cache.pages)
+    q = _q(2, 6, 128, FP32)
+    q[1, 2:4] = 0.0
+    q = (q * size).to(dtype)
+    assert q.any()                              # torch has not made zeros of them
+    for sign in (1, -1):
+        _check(q, cache, table, lengths, scale=sign * min(0.05 / size, 2e38))
