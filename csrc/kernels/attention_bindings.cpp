@@ -312,6 +312,8 @@ void prompt_tensors(PromptParams& p, const torch::Tensor& q, const torch::Tensor
 
 // How a call runs on a device of `sms` SMs: for tests.  Launches nothing; the tensors may lie on any device.
 py::dict attention_prompt_plan(torch::Tensor q, torch::Tensor k, torch::Tensor v, int64_t seqs, int64_t sms) {
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3 && k.size(1) >= 1 && q.size(1) >= k.size(1) && q.size(1) / k.size(1) <= 128,
+                    "attention_prompt_plan: tensors [tokens, heads, head_dim], 1 to 128 heads of q for each of k's");
   PromptParams p{};
   prompt_tensors(p, q, k, v);
   p.B = (int)seqs;

@@ -44,3 +44,15 @@ def test_scales(scale, words):
 def test_caches_are_told_apart_and_found():
     one, other = (KVCache4.empty(1, 16, 1, 64, device="cpu") for _ in range(2))
     assert one == one and one != other and [other, one].index(one) == 1 and {one: 1, other: 2}[other] == 2
+
+
+@pytest.mark.parametrize("q_heads,kv_heads", [(2, 0), (0, 1), (1, 2), (129, 1)])
+def test_plans_of_no_call(q_heads, kv_heads):
+    """A quotient of zero heads would end the process."""
+    q, k = torch.zeros(3, q_heads, 64, dtype=BF16), torch.zeros(3, kv_heads, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="heads"):
+        _native.kernels().attention_prompt_plan(q, k, k, 1, 148)
+    with pytest.raises(ValueError, match="heads"):
+        attention_prompt(q, k, k, torch.zeros(2, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        _native.kernels().attention_prompt_plan(q[0], k, k, 1, 148)
