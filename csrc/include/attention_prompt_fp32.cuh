@@ -17,7 +17,7 @@
 // 2048 keys were 4e-6 off).
 //
 // What bounds it.  Three sequences of 2049 tokens in all, 16 heads of 64, every key
-// seen: 53 us, 11 of them the splitting, 0.33e-6 off (the formula in 32 bits: 0.65e-6).
+// seen: 53 to 59 us, 11 of them the splitting, 0.45e-6 off (the formula in 32 bits: 0.68e-6).
 // The six products would take 24.  A step takes about 3900 clocks, 3400 of them
 // products (P V, with heads of 64, 1850): weights from S to P are 1800 of 8 warps,
 // half of them behind the sums of the last step.  A row to a thread: 76 us; values

@@ -19,8 +19,9 @@
 // TMEM: S (and P) of A and B, O of A and B, 128 columns each.
 //
 // What bounds it.  16384 tokens, causal, 32 heads of 128 over 8 key heads: 1.82 to
-// 2.02 ms, 1.09 to 1.21 PFLOP/s, where cuBLAS sustains 1.36 under the same power
-// limit (clocks near 1.45 GHz).  A step of both tiles takes 3000 clocks, 2048 of
+// 2.07 ms, 1.06 to 1.21 PFLOP/s, where cuBLAS sustains 1.36 under the same power
+// limit (clocks near 1.45 GHz); heads of 64, where exponentials are as many and
+// products half: 1.56 ms.  A step of both tiles takes 3000 clocks, 2048 of
 // them products: softmax 1750 (loads 90, the first half of the weights with the
 // maxima 1100, the other 600), then the rest of P V and Q K^T behind it.
 //
@@ -28,8 +29,8 @@
 // begun yet (cluster launch control), and loads that while the last two steps and
 // the results of the first are worked on: beginnings and ends, about 4 us of every
 // pair, are hidden, and the last ones spread over the SMs as they become free.
-// Eight chunks of 512 tokens on average, 3.7 pairs to an SM: 161 -> 150 us (142 to
-// 159 now, by the clock; the tensor cores are busy 55 % of it).
+// Eight chunks of 512 tokens on average, 3.7 pairs to an SM: 161 -> 150 us on one
+// box (142 to 164 over all of them; the tensor cores are busy 55 % of it).
 //
 // Two more warps look through the tiles of values that some row does not see
 // whole (attention_prompt.cuh), and clear what lies behind the sequence's end.

@@ -25,17 +25,20 @@
 // The sums S^T = K Q^T come out with tokens as rows; movmatrix turns two 8 x 8
 // blocks of exp(S) into the other operand of out^T = V^T P^T.
 //
-// What bounds it.  64 sequences of 16384 tokens, 8 key heads of 128: 219 us, 5.5
-// TB/s of the cache, where a copy reaches 6.4.  A tile of 32 tokens takes 520
+// What bounds it.  64 sequences of 16384 tokens, 8 key heads of 128: 219 to 253 us
+// by the box, 4.8 to 5.5 TB/s of the cache, where a copy reaches 6.4.  A tile of 32 tokens takes 520
 // instructions of a warp, 128 of them conversions and as many products by scales,
 // at half rate each: schedulers issue in 60 % of cycles, the ALUs are busy in 52 %.
 // More, smaller warps (128 registers) moved and spilled (790 instructions); one
 // warp that loads for all (bulk copies) could not keep up (408 us).  Few tokens
-// are a chain of latencies: lengths, table, tiles, join (1000 tokens: 11 us).
+// are a chain of latencies: lengths, table, tiles, join (1000 tokens: 11 us).  More
+// than 16 query heads to a key head (8 with two parts) go through the cache again
+// for each such chunk: 16 sequences of 16384 tokens, 128 heads over one, 106 us,
+// where one pass over the cache would be 6 at copy speed.
 //
 // Roundings.  Queries are scaled by a power of two and held in f16 (bf16 queries
 // exactly but for numbers 2^-14 below the row's largest, which lose bits below
-// 2^-25 of it), fp32 queries as two f16 parts (2^-22).  Probabilities go into
+// 2^-25 of it), fp32 queries as two f16 parts (2^-22 of a number's size).  Probabilities go into
 // the second product in f16 (2^-12 of each, unbiased, small against a bf16
 // result's own 2^-9), for fp32 results in two parts.  Maxima, sums and outputs
 // are fp32.  Tensor-core sums are cut rather than rounded, so for fp32 results

@@ -63,7 +63,17 @@ static bool tma_rows(const void* t, long long token, long long head, long long n
   return ((uintptr_t)t & 15) == 0 && (n <= 1 || (token > 0 && token % 8 == 0)) && (heads <= 1 || (head > 0 && head % 8 == 0));
 }
 
-// CTAs share a tile's keys where there are fewer tiles than SMs, at least 512 keys to one.
+// CTAs share a tile's keys where there are at least two SMs to a tile, at least 512 keys (of all sequences) to one.  32 heads of 128
+// over 8 key heads, bf16, us with one CTA to a tile and with two (or more, by the rule):
+//   tiles   1024 keys   2048 keys   8192 keys   32768 keys
+//     8     23.0 21.8   36.6 22.4   119  28.7   448  51.8
+//    40     23.5 26.3   37.5 30.4   121  58.8   455  172
+//    72     24.7 30.8   39.0 37.6   122  79.4   461  257
+//    80     26.4 43.1   41.6 57.2   128  140    490  480    (not shared)
+//   104     25.2 43.3   39.6 56.5   127  141    477  477    (not shared)
+//   144                 41.7 62.7   123  145    483  581    (not shared)
+// So the limit of two SMs is where it should be for two CTAs; 1024 keys are better not shared by 40 tiles and more.  Not taken: three
+// or four CTAs to each of 80 to 110 tiles of 8192 keys and more, in two rounds, 108 and 334 us for 80 of them.
 PromptPlan plan_prompt(const PromptParams& p, int sms) {
   PromptPlan plan{};
   const int tokens = (p.bf16 ? 2 : 1) * (128 / p.group);

@@ -14,7 +14,7 @@
 //
 // Both kernels only move memory: a scale's sixteen numbers to a thread, 32 bytes
 // of bf16 on one side and 9 on the other.  65536 tokens of 8 heads of 128 are read
-// in 61 us (5.6 TB/s, bound by memory), 16384 written in 29 (3 TB/s): half of that
+// in 61 us (5.6 TB/s, bound by memory), 16384 written in 27 to 29 (3 TB/s): half of that
 // is instructions (two thirds of cycles issue: 270 for sixteen numbers, 126 of them
 // the quantising), the rest the chain from the slots to the first store.
 #include <cuda_fp16.h>

@@ -44,7 +44,8 @@ def attention_cached(
     Sums, maxima and the result are kept in fp32 and rounded once, to out_dtype
     (default: q's type; fp32 queries give fp32).  For bf16 results the
     probabilities enter their product as f16 numbers; for fp32 results queries
-    and probabilities are two f16 numbers each, which is fp32's accuracy.
+    and probabilities are two f16 numbers each, 22 bits (for a number 2^-14 or
+    more below its row's largest, fewer).
     ``return_lse``: also log sum exp(scale * q K^T), fp32 [B, heads], -inf for
     empty sequences, to join results over parts of a context.
 
@@ -85,14 +86,15 @@ def attention_prompt(
     that sees nothing gets zeros, and rows of ``out`` before the first and behind
     the last sequence are left as they were.  What a token does not see does not
     enter its result, infinities and NaN included; of what it does see, an
-    infinity whose weight is below 2^-110 may come out as NaN.  scale: default head_dim **
-    -0.5.  At most 2^16 sequences.
+    infinity whose weight is below 2^-110 may come out as NaN.  scale: default
+    head_dim ** -0.5.  At most 2^16 sequences.
 
     Sums, maxima and the result are kept in fp32 and rounded once, to q's type.
-    With bf16 inputs the probabilities enter their product as bf16 numbers; fp32
-    inputs and their probabilities are three bf16 numbers each, which is fp32's
-    accuracy (an infinite logit may come out as NaN).  ``return_lse``: also log
-    sum exp(scale * q K^T), fp32 [tokens, heads], -inf where a token sees nothing,
+    With bf16 inputs the probabilities enter their product as bf16 numbers, up to
+    2^-8 off each; fp32 inputs and their probabilities are three bf16 numbers each,
+    24 bits (an infinite logit may come out as NaN).  Values below 2^-110 lose bits,
+    as do fp32 queries and keys.  ``return_lse``: also log sum exp(scale * q K^T),
+    fp32 [tokens, heads], -inf where a token sees nothing or logits of -inf alone,
     undefined outside of the sequences.
 
     Offsets that lie outside of the tensors or fall are cut and recorded:
