@@ -108,19 +108,24 @@ __device__ __forceinline__ int prompt_visible(const PromptParams& p, const Promp
   return n < 0 ? 0 : n;
 }
 
-// Weights are exp2(z - m).  Where m is set it is 15 above the row's maximum, and it is set again once a logit comes nearer to
+// Weights are exp2(z - m).  Where m is set it is HEAD above the row's maximum, and it is set again once a logit comes nearer to
 // it than 9 or the sum l of the weights passes 1/4 (by 8 at least).  So no weight is above 2^-9, a step's 128 add 1/4 at
 // most, l stays below 1/2, and sums of weights times finite values below the largest of those: they never overflow,
-// however large the values.  Weights near the largest are 2^-15 to 2^-9: products with values down to 2^-100 keep all
-// their bits.  (At logits of 2^27 the distance is lost in rounding, and values above 2^128 / keys may overflow.)
+// however large the values.  (At logits of 2^27 the distance is lost in rounding, and values above 2^128 / keys may overflow.)
+// With m at the maximum, and followed at 2^64 times (bf16) or 2^8 times (fp32) that, values above 2^64 or 2^120 by the number of
+// keys became infinities.
 //
-// With m at the maximum and followed at 2^64 times (bf16) or 2^8 times (fp32) that, values above 2^64 or 2^120 by the number of
-// keys became infinities.  A rise of 6 after a row's first step is rare all the same, and z - m is off by 2^-21 at most.
-constexpr float kPromptHead = 15.f, kPromptNear = 9.f, kPromptSum = 0.25f, kPromptLeast = 8.f;
+// What HEAD costs: weights near the largest are 2^-HEAD and up, whose products with values below 2^(HEAD - 130) or so lose
+// bits; and z - m is off by half a last place of HEAD.  What it gives: m is set again only where logits rise by HEAD - 9 after a
+// row's first step.  In fp32, where sums are in registers, that costs little: 15.  In bf16 it takes a third of a step from all
+// 128 rows of a tile, and for logits that spread by 3 nats or more a HEAD of 15 made prompts 25 % slower: 31 (22 powers of two, 15
+// nats); and 47 from then on, for rows that rise like that will again, and all rows of the warp at once.
+constexpr int kPromptHeadFp32 = 15, kPromptHeadTc = 31, kPromptHeadAgain = 47;
+constexpr float kPromptNear = 9.f, kPromptSum = 0.25f, kPromptLeast = 8.f;
 
-// log sum exp(z); l is mostly near 2^-15 of exponents at the maximum.
-__device__ __forceinline__ float prompt_lse(float m, float l) {
-  return ((m - kPromptHead) + log2f(l * 32768.f)) * 0.69314718055994531f;
+// log sum exp(z); l is mostly near 2^-head of exponents at the maximum.
+__device__ __forceinline__ float prompt_lse(float m, float l, int head) {
+  return ((m - head) + log2f(scalbnf(l, head))) * 0.69314718055994531f;
 }
 
 // 1 / l.  A row without keys has l = 0, and zeros for a result.  One that sees keys whose logits are all -inf has l = -0: NaN,

@@ -327,7 +327,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       const bool grow = peak > m - kPromptNear || l + other.y > kPromptSum, follow = __any_sync(0xffffffffu, grow);
       float shrink = 1.f;
       if (follow) {
-        const float now = grow ? fmaxf(peak + kPromptHead, m + kPromptLeast) : m;
+        const float now = grow ? fmaxf(peak + kPromptHeadFp32, m + kPromptLeast) : m;
         shrink = m == -INFINITY ? 0.f : prompt_exp2(m - now);
         m = now;
         l *= shrink;
@@ -403,7 +403,7 @@ prompt_fp32_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant
       }
       if (half == 0) {
         if (p.splits > 1) p.stats[at] = make_float2(m, l);
-        else if (p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = prompt_lse(m, l);
+        else if (p.lse != nullptr) p.lse[(long long)(s.q0 + token) * p.Hq + hq] = prompt_lse(m, l, kPromptHeadFp32);
       }
     }
   }

@@ -525,8 +525,8 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
               for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(r[c + 2 * e]), __uint_as_float(r[c + 2 * e + 1]));
             const float peak = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * mult;
             const bool grow = peak > m - kPromptNear;
-            again = __any_sync(0xffffffffu, grow);   // once: it does not hold for peak + kPromptHead, however that is rounded
-            if (again) follow(grow ? peak + kPromptHead : m, i > 0);
+            again = __any_sync(0xffffffffu, grow);   // once: it does not hold for peak + 31, however that is rounded
+            if (again) follow(fmaxf(m, peak + (i > 0 ? kPromptHeadAgain : kPromptHeadTc)), i > 0);
           } while (again);
           store(0);
           half(1, m == -INFINITY ? 0.f : -m);
@@ -589,7 +589,7 @@ prompt_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__
           __syncwarp();
         }
         if (mine && p.splits > 1) p.stats[((long long)it.split * p.Nq + it.s.q0 + token) * p.Hq + hq] = make_float2(m, l);
-        else if (mine && p.lse != nullptr) p.lse[(long long)(it.s.q0 + token) * p.Hq + hq] = prompt_lse(m, l);
+        else if (mine && p.lse != nullptr) p.lse[(long long)(it.s.q0 + token) * p.Hq + hq] = prompt_lse(m, l, kPromptHeadTc);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[n & 1]);

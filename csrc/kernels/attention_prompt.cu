@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(PromptParams p) {
   }
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) store_elem(p.out, token * p.o_token + hq * p.o_head + D / 32 * lane + i, v[i], p.bf16);
-  if (p.lse != nullptr && lane == 0) p.lse[row] = prompt_lse(top, l);
+  if (p.lse != nullptr && lane == 0) p.lse[row] = prompt_lse(top, l, p.bf16 ? kPromptHeadTc : kPromptHeadFp32);
 }
 
 // Rows of a tensor [n, heads, D] that TMA can read: on 16 bytes, and apart.

@@ -86,14 +86,15 @@ def attention_prompt(
     that sees nothing gets zeros, and rows of ``out`` before the first and behind
     the last sequence are left as they were.  What a token does not see does not
     enter its result, infinities and NaN included; of what it does see, an
-    infinity whose weight is below 2^-110 may come out as NaN.  scale: default
+    infinity whose weight is below 2^-75 may come out as NaN.  scale: default
     head_dim ** -0.5.  At most 2^16 sequences.
 
     Sums, maxima and the result are kept in fp32 and rounded once, to q's type.
     With bf16 inputs the probabilities enter their product as bf16 numbers, up to
     2^-8 off each; fp32 inputs and their probabilities are three bf16 numbers each,
-    24 bits (an infinite logit may come out as NaN).  Values below 2^-110 lose bits,
-    as do fp32 queries and keys.  ``return_lse``: also log sum exp(scale * q K^T),
+    24 bits (an infinite logit may come out as NaN).  Values below 2^-100 lose bits
+    (in bf16 below 2^-85 where logits rise by more than 15 after a token's first 128
+    keys), as do fp32 queries and keys below 2^-110.  ``return_lse``: also log sum exp(scale * q K^T),
     fp32 [tokens, heads], -inf where a token sees nothing or logits of -inf alone,
     undefined outside of the sequences.
 
